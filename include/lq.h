@@ -234,6 +234,65 @@ int lq_kv_attend_noalloc(const void* q, const uint32_t* kq, const void* ks, cons
                          const void* vs, const void* vb, const int32_t* start, int n, const float* sinks, float scale,
                          int B, int H, int KVH, int cap, int head_dim, int dtype, void* out, void* stream);
 
+/* ---- a paged key/value cache in 4 bits (no counterpart in the reference, whose cache is one 8-bit buffer a batch,
+ * locals/qkv.py) ----
+ * A pool of pages: words kq, vq uint32 (pages, KVH, page_size, head_dim / 8), scales and biases ks, kb, vs, vb (pages,
+ * KVH, page_size, head_dim / 64) in the activation dtype -- MLX affine 4-bit groups of 64, as lq_quantize writes them.
+ * head_dim 64, 128 or 256; page_size a multiple of 8, at most 65536; pages * page_size < 2^31. Slot = page * page_size +
+ * offset. What a kernel finds out of range in device memory (a position, a slot, a page id, a length beyond the block
+ * table) is recorded as LQ_DEV_BOUNDS in the device status and left out, never read or written. */
+
+/* A step's block tables and slot maps from the requests' lengths. cached, fresh (B): tokens held and new tokens
+ * (negative: 0). table (B, width): the first ceil(cached / page_size) entries of a row are its pages; the pages that the
+ * new tokens need beyond them are taken from free_pages[*head], free_pages[*head + 1], ... (nfree of them) in request
+ * order and entered. Written: lens (B) = cached + fresh; q_start (B + 1) the exclusive sums of fresh; for token t of the
+ * step (tokens of them; those past q_start[B] are padding: position 0, slot -1) its positions[t] and slots[t];
+ * head_out (1) the next free entry. head_out may not be head. A token that finds no page gets slot -1 (and
+ * LQ_DEV_BOUNDS). B <= 8192. */
+int lq_page_plan(const int32_t* cached, const int32_t* fresh, int B, int32_t* table, int width,
+                 const int32_t* free_pages, int nfree, const int32_t* head, int page_size, int tokens, int32_t* lens,
+                 int32_t* q_start, int32_t* positions, int32_t* slots, int32_t* head_out, void* stream);
+
+/* Rotary positions with several axes: the first rot dimensions of every head of q (N, H, head_dim) and k (N, KVH,
+ * head_dim) rotated, the others copied, to q_out and k_out (contiguous). Pair j of the rot / 2 pairs -- dimensions
+ * (j, j + rot / 2), or (2 j, 2 j + 1) when interleaved -- becomes (a c - b s, b c + a s), c and s from row
+ * positions[axes[j] * N + n] of cos and sin (max_pos, rot / 2) float32. positions (naxes, N); axes (rot / 2), NULL = all
+ * pairs on axis 0. q_row, k_row: elements from one token to the next (a token's heads are contiguous). Either of q and k
+ * may be absent (NULL, with H or KVH 0). 32-bit arithmetic, one rounding. A position outside the tables uses the nearest
+ * row (and LQ_DEV_BOUNDS). Any head_dim and even rot <= head_dim; interleaved rows must lie on 4-byte boundaries. An
+ * output may be its own input when that is contiguous. */
+int lq_rotary(const void* q, int64_t q_row, void* q_out, int H, const void* k, int64_t k_row, void* k_out, int KVH,
+              int N, int head_dim, int rot, const int32_t* positions, const float* cos, const float* sin, int max_pos,
+              const int32_t* axes, int naxes, int interleaved, int dtype, void* stream);
+
+/* A step's cache write in one launch: q rotated to q_out as lq_rotary does it (q NULL and H 0: none), k rotated in 32
+ * bits and, like v, quantized to 4 bits (lq_quantize's algorithm) into slots[n] of the pool; a negative slot stores
+ * nothing. positions NULL: no rotation. rot % 16 == 0; q_row, k_row, v_row and rows on 16-byte boundaries. Two tokens
+ * may not share a slot. */
+int lq_kv4_append(const void* q, int64_t q_row, void* q_out, int H, const void* k, int64_t k_row, const void* v,
+                  int64_t v_row, int KVH, int N, int head_dim, int rot, const int32_t* positions, const float* cos,
+                  const float* sin, int max_pos, const int32_t* axes, int naxes, int interleaved, const int32_t* slots,
+                  uint32_t* kq, void* ks, void* kb, uint32_t* vq, void* vs, void* vb, int pages, int page_size,
+                  int dtype, void* stream);
+
+/* The values that the cache holds at slots (N): k_out, v_out (N, KVH, head_dim) = scale * code + bias in dtype, zeros
+ * for a negative slot. */
+int lq_kv4_read(const uint32_t* kq, const void* ks, const void* kb, const uint32_t* vq, const void* vs, const void* vb,
+                int pages, int page_size, int KVH, int head_dim, const int32_t* slots, int N, void* k_out, void* v_out,
+                int dtype, void* stream);
+
+/* Attention over the pages: q and out (N, H, head_dim); request b's queries are rows q_start[b] .. q_start[b + 1] - 1
+ * (q_start NULL: row b, one each), at most max_q of them, the last of them at position lens[b] - 1; a query sees the
+ * keys up to its own position, the last `window` of them when window > 0. out = sum p v / (sum p + e^sink), p = e^(scale q . k), softmax statistics in 32 bits; sinks (H) float32 or NULL; 0 where a
+ * query sees nothing and for rows past q_start[B]. table (B, width) page ids, -1 where there is none. workspace:
+ * lq_kv4_attend_workspace(N, B, max_q, H, KVH, head_dim) bytes, 16-byte aligned (NULL when that is 0). */
+size_t lq_kv4_attend_workspace(int N, int B, int max_q, int H, int KVH, int head_dim);
+int lq_kv4_attend(const void* q, int N, const int32_t* q_start, int max_q, const uint32_t* kq, const void* ks,
+                  const void* kb, const uint32_t* vq, const void* vs, const void* vb, int pages, int page_size,
+                  const int32_t* table, int width, const int32_t* lens, int B, const float* sinks, float scale,
+                  int window, int H, int KVH, int head_dim, int dtype, void* workspace, size_t workspace_bytes,
+                  void* out, void* stream);
+
 /* The column-sharded prefill with its own all-gather: this rank's N output columns of y = x . dequant(w)^T (the
  * dense path of lq_qmm_dense) are written by the GEMM in place at columns [col_off, col_off + N) of dst[0], this GPU's
  * row-major (M, ldo) buffer, then copied by one kernel of plain 16-byte peer stores into the same columns of

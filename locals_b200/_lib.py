@@ -15,7 +15,7 @@ F16, BF16, F32 = 0, 1, 2
 FAM_AUTO, FAM_QMV, FAM_TC, FAM_TCV, FAM_QMVG, FAM_QMVQ = 0, 1, 2, 3, 4, 5
 
 # every function the header declares, with its argument types (checked by tests on CPU)
-_vp, _i, _u32p = ctypes.c_void_p, ctypes.c_int, ctypes.c_void_p
+_vp, _i, _i64, _u32p = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_void_p
 
 
 class Cfg(ctypes.Structure):
@@ -63,6 +63,14 @@ SIGNATURES = {
     "lq_ipc_close": ([_vp, ctypes.c_size_t], _i),
     "lq_kv_attend_noalloc": ([_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _vp, ctypes.c_float, _i, _i, _i, _i, _i, _i,
                               _vp, _vp], _i),
+    "lq_page_plan": ([_vp, _vp, _i, _vp, _i, _vp, _i, _vp, _i, _i, _vp, _vp, _vp, _vp, _vp, _vp], _i),
+    "lq_rotary": ([_vp, _i64, _vp, _i, _vp, _i64, _vp, _i, _i, _i, _i, _vp, _vp, _vp, _i, _vp, _i, _i, _i, _vp], _i),
+    "lq_kv4_append": ([_vp, _i64, _vp, _i, _vp, _i64, _vp, _i64, _i, _i, _i, _i, _vp, _vp, _vp, _i, _vp, _i, _i, _vp,
+                       _u32p, _vp, _vp, _u32p, _vp, _vp, _i, _i, _i, _vp], _i),
+    "lq_kv4_read": ([_u32p, _vp, _vp, _u32p, _vp, _vp, _i, _i, _i, _i, _vp, _i, _vp, _vp, _i, _vp], _i),
+    "lq_kv4_attend_workspace": ([_i, _i, _i, _i, _i, _i], ctypes.c_size_t),
+    "lq_kv4_attend": ([_vp, _i, _vp, _i, _u32p, _vp, _vp, _u32p, _vp, _vp, _i, _i, _vp, _i, _vp, _i, _vp,
+                       ctypes.c_float, _i, _i, _i, _i, _i, _vp, ctypes.c_size_t, _vp, _vp], _i),
     "lq_supported": ([_i, _i, _i, _i, _i, _i, _i], _i),
     "lq_list_configs": ([_i, _i, _i, _i, _i, _i, ctypes.POINTER(Cfg), _i], _i),
     "lq_device_status": ([_i], ctypes.c_uint),

@@ -5,8 +5,10 @@
 #include <string.h>
 
 #include "../../include/lq.h"
+#include "kv4.cuh"
 #include "lq_host.h"
 #include "qmv.h"
+#include "rotary.cuh"
 
 namespace lq {
 int quantize_run(const void* w, int w_dt, int N, int K, int bits, int group, uint32_t* wq, void* s, void* b,
@@ -91,6 +93,25 @@ int combine_norm_run(const void* ys, const float* wts, const int32_t* pos, const
                      const void* nw, void* y, void* n, int T, int K, int D, float eps, int dtype, cudaStream_t st);
 int scatter_rows_run(const void* src, const int32_t* idx, int R, int row_bytes, void* dst, int dst_rows,
                      cudaStream_t st);
+bool page_plan_shape_ok(int B, int width, int nfree, int page, int tokens);
+int page_plan_run(const int32_t* cached, const int32_t* fresh, int B, int32_t* table, int width,
+                  const int32_t* free_pages, int nfree, const int32_t* head, int page, int tokens, int32_t* lens,
+                  int32_t* q_start, int32_t* positions, int32_t* slots, int32_t* head_out, cudaStream_t st);
+bool rotary_shape_ok(int N, int H, int KVH, int D, int rot, int max_pos, int naxes);
+int rotary_run(const void* q, long long q_row, void* q_out, int H, const void* k, long long k_row, void* k_out,
+               int KVH, int N, int D, int rot, const int32_t* positions, const float* cos, const float* sin,
+               int max_pos, const int32_t* axes, int naxes, int interleaved, int dtype, cudaStream_t st);
+bool kv4_pool_ok(const Kv4Pool& p, int D);
+int kv4_append_run(const RotArgs& r, const Kv4Pool& pool, const void* q, long long q_row, void* q_out, int H,
+                   const void* k, long long k_row, const void* v, long long v_row, const int32_t* slots, int dtype,
+                   cudaStream_t st);
+int kv4_read_run(const Kv4Pool& pool, int D, const int32_t* slots, int N, void* k_out, void* v_out, int dtype,
+                 cudaStream_t st);
+bool kv4_attend_shape_ok(int N, int B, int max_q, int H, int KVH, int width, int window);
+size_t kv4_attend_workspace_bytes(int N, int B, int max_q, int H, int KVH, int D);
+int kv4_attend_run(const Kv4Pool& pool, const void* q, int N, const int32_t* q_start, int max_q, const int32_t* table,
+                   int width, const int32_t* lens, int B, const float* sinks, float scale, int window, int H, int D,
+                   int dtype, void* workspace, size_t workspace_bytes, void* out, cudaStream_t st);
 }  // namespace lq
 
 using namespace lq;
@@ -652,6 +673,114 @@ int lq_scatter_rows(const void* src, const int32_t* idx, int R, int N, void* dst
     int rc = check_device();
     if (rc) return rc;
     return finish(scatter_rows_run(src, idx, R, N * 2, dst, dst_rows, reinterpret_cast<cudaStream_t>(stream)));
+}
+
+int lq_page_plan(const int32_t* cached, const int32_t* fresh, int B, int32_t* table, int width,
+                 const int32_t* free_pages, int nfree, const int32_t* head, int page_size, int tokens, int32_t* lens,
+                 int32_t* q_start, int32_t* positions, int32_t* slots, int32_t* head_out, void* stream) {
+    if (!cached || !fresh || !table || !free_pages || !head || !lens || !q_start || !positions || !slots ||
+        !head_out || head_out == head)
+        return LQ_E_ARG;
+    if (!page_plan_shape_ok(B, width, nfree, page_size, tokens)) return LQ_E_SHAPE;
+    const void* all[] = {cached, fresh, table, free_pages, head, lens, q_start, positions, slots, head_out};
+    for (const void* p : all)
+        if (!aligned(p, 4)) return LQ_E_ALIGN;
+    int rc = check_device();
+    if (rc) return rc;
+    return finish(page_plan_run(cached, fresh, B, table, width, free_pages, nfree, head, page_size, tokens, lens,
+                                q_start, positions, slots, head_out, reinterpret_cast<cudaStream_t>(stream)));
+}
+
+int lq_rotary(const void* q, int64_t q_row, void* q_out, int H, const void* k, int64_t k_row, void* k_out, int KVH,
+              int N, int head_dim, int rot, const int32_t* positions, const float* cos, const float* sin, int max_pos,
+              const int32_t* axes, int naxes, int interleaved, int dtype, void* stream) {
+    if ((H > 0 && (!q || !q_out)) || (KVH > 0 && (!k || !k_out)) || !positions || !cos || !sin) return LQ_E_ARG;
+    if (!is16(dtype)) return LQ_E_UNSUPPORTED;
+    if (!rotary_shape_ok(N, H, KVH, head_dim, rot, max_pos, naxes)) return LQ_E_SHAPE;
+    if ((H > 0 && q_row < int64_t(H) * head_dim) || (KVH > 0 && k_row < int64_t(KVH) * head_dim)) return LQ_E_SHAPE;
+    if ((H > 0 && (!aligned(q, 2) || !aligned(q_out, 2))) || (KVH > 0 && (!aligned(k, 2) || !aligned(k_out, 2))) ||
+        !aligned(positions, 4) || !aligned(cos, 4) || !aligned(sin, 4) || (axes && !aligned(axes, 4)))
+        return LQ_E_ALIGN;
+    int rc = check_device();
+    if (rc) return rc;
+    return finish(rotary_run(q, q_row, q_out, H, k, k_row, k_out, KVH, N, head_dim, rot, positions, cos, sin, max_pos,
+                             axes, naxes, interleaved, dtype, reinterpret_cast<cudaStream_t>(stream)));
+}
+
+static bool kv4_aligned(const Kv4Pool& p) {
+    return aligned(p.kq, 16) && aligned(p.vq, 16) && aligned(p.ks, 16) && aligned(p.kb, 16) && aligned(p.vs, 16) &&
+           aligned(p.vb, 16);
+}
+
+int lq_kv4_append(const void* q, int64_t q_row, void* q_out, int H, const void* k, int64_t k_row, const void* v,
+                  int64_t v_row, int KVH, int N, int head_dim, int rot, const int32_t* positions, const float* cos,
+                  const float* sin, int max_pos, const int32_t* axes, int naxes, int interleaved, const int32_t* slots,
+                  uint32_t* kq, void* ks, void* kb, uint32_t* vq, void* vs, void* vb, int pages, int page_size,
+                  int dtype, void* stream) {
+    if ((H > 0 && (!q || !q_out)) || !k || !v || !slots || !kq || !ks || !kb || !vq || !vs || !vb) return LQ_E_ARG;
+    if (positions && (!cos || !sin)) return LQ_E_ARG;
+    if (!is16(dtype)) return LQ_E_UNSUPPORTED;
+    const Kv4Pool pool = {kq, static_cast<uint16_t*>(ks), static_cast<uint16_t*>(kb), vq, static_cast<uint16_t*>(vs),
+                          static_cast<uint16_t*>(vb), pages, KVH, page_size};
+    if (!kv4_pool_ok(pool, head_dim) || N < 0 || H < 0) return LQ_E_SHAPE;
+    if (positions && (!rotary_shape_ok(N, H, KVH, head_dim, rot, max_pos, naxes) || rot % 16)) return LQ_E_SHAPE;
+    if ((H > 0 && q_row < int64_t(H) * head_dim) || k_row < int64_t(KVH) * head_dim || v_row < int64_t(KVH) * head_dim)
+        return LQ_E_SHAPE;
+    if (!kv4_aligned(pool) || (H > 0 && (!aligned(q, 16) || !aligned(q_out, 16) || q_row % 8)) || !aligned(k, 16) ||
+        !aligned(v, 16) || k_row % 8 || v_row % 8 || !aligned(slots, 4) || !aligned(positions, 4) || !aligned(cos, 4) ||
+        !aligned(sin, 4) || !aligned(axes, 4))
+        return LQ_E_ALIGN;
+    int rc = check_device();
+    if (rc) return rc;
+    const RotArgs r = {positions, cos, sin, axes, N, head_dim, positions ? rot : 0, max_pos, naxes, interleaved};
+    return finish(kv4_append_run(r, pool, q, q_row, q_out, H, k, k_row, v, v_row, slots, dtype,
+                                 reinterpret_cast<cudaStream_t>(stream)));
+}
+
+// The pool of a call that only reads it.
+static Kv4Pool kv4_const_pool(const uint32_t* kq, const void* ks, const void* kb, const uint32_t* vq, const void* vs,
+                              const void* vb, int pages, int KVH, int page) {
+    auto h = [](const void* p) { return const_cast<uint16_t*>(static_cast<const uint16_t*>(p)); };
+    return {const_cast<uint32_t*>(kq), h(ks), h(kb), const_cast<uint32_t*>(vq), h(vs), h(vb), pages, KVH, page};
+}
+
+int lq_kv4_read(const uint32_t* kq, const void* ks, const void* kb, const uint32_t* vq, const void* vs, const void* vb,
+                int pages, int page_size, int KVH, int head_dim, const int32_t* slots, int N, void* k_out, void* v_out,
+                int dtype, void* stream) {
+    if (!kq || !ks || !kb || !vq || !vs || !vb || !slots || !k_out || !v_out) return LQ_E_ARG;
+    if (!is16(dtype)) return LQ_E_UNSUPPORTED;
+    const Kv4Pool pool = kv4_const_pool(kq, ks, kb, vq, vs, vb, pages, KVH, page_size);
+    if (!kv4_pool_ok(pool, head_dim) || N < 0) return LQ_E_SHAPE;
+    if (!kv4_aligned(pool) || !aligned(slots, 4) || !aligned(k_out, 16) || !aligned(v_out, 16)) return LQ_E_ALIGN;
+    int rc = check_device();
+    if (rc) return rc;
+    return finish(kv4_read_run(pool, head_dim, slots, N, k_out, v_out, dtype, reinterpret_cast<cudaStream_t>(stream)));
+}
+
+size_t lq_kv4_attend_workspace(int N, int B, int max_q, int H, int KVH, int head_dim) {
+    if (KVH < 1 || !kv4_attend_shape_ok(N, B, max_q, H, KVH, 1, 0)) return 0;
+    if (check_device() != LQ_OK) return 0;
+    return kv4_attend_workspace_bytes(N, B, max_q, H, KVH, head_dim);
+}
+
+int lq_kv4_attend(const void* q, int N, const int32_t* q_start, int max_q, const uint32_t* kq, const void* ks,
+                  const void* kb, const uint32_t* vq, const void* vs, const void* vb, int pages, int page_size,
+                  const int32_t* table, int width, const int32_t* lens, int B, const float* sinks, float scale,
+                  int window, int H, int KVH, int head_dim, int dtype, void* workspace, size_t workspace_bytes,
+                  void* out, void* stream) {
+    if (!q || !kq || !ks || !kb || !vq || !vs || !vb || !table || !lens || !out) return LQ_E_ARG;
+    if (!is16(dtype)) return LQ_E_UNSUPPORTED;
+    const Kv4Pool pool = kv4_const_pool(kq, ks, kb, vq, vs, vb, pages, KVH, page_size);
+    if (!kv4_pool_ok(pool, head_dim) || !kv4_attend_shape_ok(N, B, max_q, H, KVH, width, window) || !(scale == scale))
+        return LQ_E_SHAPE;
+    if (!q_start && (N != B || max_q != 1)) return LQ_E_SHAPE;
+    if (!kv4_aligned(pool) || !aligned(q, 16) || !aligned(out, 16) || !aligned(q_start, 4) || !aligned(table, 4) ||
+        !aligned(lens, 4) || !aligned(sinks, 4) || !aligned(workspace, 16))
+        return LQ_E_ALIGN;
+    int rc = check_device();
+    if (rc) return rc;
+    return finish(kv4_attend_run(pool, q, N, q_start, max_q, table, width, lens, B, sinks, scale, window, H, head_dim,
+                                 dtype, workspace, workspace_bytes, out, reinterpret_cast<cudaStream_t>(stream)));
 }
 
 int lq_supported(int family, int M, int N, int K, int bits, int group_size, int dtype) {

@@ -1,0 +1,165 @@
+// Rotary positions with several axes on queries and keys (the arithmetic is rotary.cuh's).
+//
+// A work item is one unit of a row (V pairs held as two vectors of V values a half apart, or V values of neighbouring
+// pairs, or V copied values) of R rows of one token: the token's cos and sin are read once for the R rows, and the R
+// rows' loads are issued together. Items are numbered unit fastest, so a warp's accesses run along rows. V is the
+// widest vector that the sizes, strides and addresses allow, 16 bytes where they allow it.
+// HBM-bound: 4 bytes a value, and the table rows (32-bit values, read from L2 after their first use).
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "lq_host.h"
+#include "rotary.cuh"
+
+namespace lq {
+
+constexpr int ROT_THREADS = 256;
+
+struct RotaryArgs {
+    RotArgs r;
+    const uint16_t* q;
+    uint16_t* qo;
+    const uint16_t* k;
+    uint16_t* ko;
+    long long q_row, k_row;  // values from one token's rows to the next's (inputs; outputs are contiguous)
+    int H, KVH, units, groups;
+    long long items;
+};
+
+template <typename T, int V, int R, bool PAIRS2>
+__global__ void __launch_bounds__(ROT_THREADS) rotary_kernel(const RotaryArgs a) {
+    grid_dep_wait();
+    const long long item = (long long)blockIdx.x * ROT_THREADS + threadIdx.x;
+    if (item >= a.items) return;
+    const int unit = int(item % a.units);
+    const long long rest = item / a.units;
+    const int g = int(rest % a.groups), n = int(rest / a.groups);
+    const int half = a.r.rot >> 1;
+    const int rows = a.H + a.KVH;
+    // where the unit's first vector starts in a row, and whether it is rotated
+    int at;
+    bool turned;
+    if (PAIRS2) {
+        at = unit * V;
+        turned = at < a.r.rot;
+    } else {
+        turned = unit * V < half;
+        at = turned ? unit * V : a.r.rot + (unit * V - half);
+    }
+    RotVec<T, V> lo[R], hi[R];
+    const uint16_t* src[R];
+    uint16_t* dst[R];
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+        const int row = g * R + i;
+        if (row >= rows) continue;
+        const bool isq = row < a.H;
+        src[i] = isq ? a.q + n * a.q_row + (long long)row * a.r.D
+                     : a.k + n * a.k_row + (long long)(row - a.H) * a.r.D;
+        dst[i] = isq ? a.qo + ((long long)n * a.H + row) * a.r.D
+                     : a.ko + ((long long)n * a.KVH + row - a.H) * a.r.D;
+        lo[i].load(src[i] + at);
+        if (!PAIRS2 && turned) hi[i].load(src[i] + at + half);
+    }
+    if (turned) {
+        constexpr int P = PAIRS2 ? V / 2 : V;
+        float c[P], s[P];
+        rot_cos_sin<P>(a.r, n, PAIRS2 ? at / 2 : at, c, s);
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+            if (g * R + i >= rows) continue;
+#pragma unroll
+            for (int j = 0; j < P; ++j) {
+                if (PAIRS2) {
+                    float x = lo[i].get(2 * j), y = lo[i].get(2 * j + 1);
+                    rot_pair(x, y, c[j], s[j]);
+                    lo[i].set(2 * j, x);
+                    lo[i].set(2 * j + 1, y);
+                } else {
+                    float x = lo[i].get(j), y = hi[i].get(j);
+                    rot_pair(x, y, c[j], s[j]);
+                    lo[i].set(j, x);
+                    hi[i].set(j, y);
+                }
+            }
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+        if (g * R + i >= rows) continue;
+        lo[i].store(dst[i] + at);
+        if (!PAIRS2 && turned) hi[i].store(dst[i] + at + half);
+    }
+}
+
+template <typename T, int V, int R, bool PAIRS2>
+static int rotary_launch(RotaryArgs a, cudaStream_t st) {
+    a.groups = (a.H + a.KVH + R - 1) / R;
+    a.items = (long long)a.r.N * a.groups * a.units;
+    const long long blocks = (a.items + ROT_THREADS - 1) / ROT_THREADS;
+    if (blocks > 0x7fffffffLL) return LQ_E_SHAPE;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(unsigned(blocks));
+    cfg.blockDim = dim3(ROT_THREADS);
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, rotary_kernel<T, V, R, PAIRS2>, a) == cudaSuccess ? LQ_OK : LQ_E_CUDA;
+}
+
+template <typename T, int V>
+static int rotary_v(RotaryArgs a, cudaStream_t st) {
+    // Four rows a thread once every SM has work for a few CTAs: one read of cos and sin then serves four rows.
+    const long long items1 = (long long)a.r.N * (a.H + a.KVH) * a.units;
+    const bool many = items1 >= 4LL * device_info().sm_count * 4 * ROT_THREADS;
+    if (a.r.interleaved) {
+        if constexpr (V >= 2)
+            return many ? rotary_launch<T, V, 4, true>(a, st) : rotary_launch<T, V, 1, true>(a, st);
+        else
+            return LQ_E_ALIGN;
+    }
+    return many ? rotary_launch<T, V, 4, false>(a, st) : rotary_launch<T, V, 1, false>(a, st);
+}
+
+bool rotary_shape_ok(int N, int H, int KVH, int D, int rot, int max_pos, int naxes) {
+    return N >= 0 && H >= 0 && KVH >= 0 && H + KVH >= 1 && D >= 2 && D <= 65536 && rot >= 2 && rot % 2 == 0 &&
+           rot <= D && max_pos >= 1 && naxes >= 1;
+}
+
+int rotary_run(const void* q, long long q_row, void* q_out, int H, const void* k, long long k_row, void* k_out,
+               int KVH, int N, int D, int rot, const int32_t* positions, const float* cos, const float* sin,
+               int max_pos, const int32_t* axes, int naxes, int interleaved, int dtype, cudaStream_t st) {
+    if (N == 0) return LQ_OK;
+    RotaryArgs a = {};
+    a.r = {positions, cos, sin, axes, N, D, rot, max_pos, naxes, interleaved};
+    a.q = static_cast<const uint16_t*>(q);
+    a.qo = static_cast<uint16_t*>(q_out);
+    a.k = static_cast<const uint16_t*>(k);
+    a.ko = static_cast<uint16_t*>(k_out);
+    a.q_row = q_row;
+    a.k_row = k_row;
+    a.H = H;
+    a.KVH = KVH;
+    // the widest vector that divides every offset: rows, pairs' halves, strides and addresses
+    const int half = rot / 2;
+    unsigned long long all = (unsigned long long)D | 8ull;
+    all |= interleaved ? (unsigned long long)rot : (unsigned long long)half;
+    if (H) all |= (unsigned long long)q_row | (reinterpret_cast<uintptr_t>(q) >> 1) | (reinterpret_cast<uintptr_t>(q_out) >> 1);
+    if (KVH) all |= (unsigned long long)k_row | (reinterpret_cast<uintptr_t>(k) >> 1) | (reinterpret_cast<uintptr_t>(k_out) >> 1);
+    const int V = int(all & (~all + 1));
+    a.units = (interleaved ? D : half + (D - rot)) / V;
+    const bool bf = dtype == LQ_BF16;
+    switch (V) {
+        case 8: return bf ? rotary_v<__nv_bfloat16, 8>(a, st) : rotary_v<__half, 8>(a, st);
+        case 4: return bf ? rotary_v<__nv_bfloat16, 4>(a, st) : rotary_v<__half, 4>(a, st);
+        case 2: return bf ? rotary_v<__nv_bfloat16, 2>(a, st) : rotary_v<__half, 2>(a, st);
+        default: return bf ? rotary_v<__nv_bfloat16, 1>(a, st) : rotary_v<__half, 1>(a, st);
+    }
+}
+
+}  // namespace lq
