@@ -4,8 +4,29 @@
 // (window 0: from 0) to its own: out = sum_j e^(s_j - m) v_j / (sum_j e^(s_j - m) + e^(sink - m)), s_j = scale q . k_j,
 // and 0 where nothing is seen.
 //
-// One CTA a (query, head); each of its warps takes every fourth key with a running maximum and sum of its own, a lane
-// holding D / 32 dimensions; the warps are joined in shared memory.
+// kv4_attend_kernel. The rows of a (request, kv head) are its queries times the G query heads of the kv head; a tile of
+// 8 NT rows is the n side of m16n8k16 fp16 MMAs whose m side is 16 keys (scores, S^T = K Q^T) or 16 dimensions (values,
+// O^T = V^T P^T), so that few rows fill the MMA and each key is unpacked once for all of them. The 4-bit codes enter the
+// MMA as fp16 subnormals, with no arithmetic at all: a word's bits & 0x000f000f are the pair (code 0, code 4) * 2^-24,
+// & 0x00f000f0 the pair (code 1, code 5) * 2^-20, and the same of word >> 8; every product and sum of them is exact in
+// the fp32 accumulator but for its roundings. What differs between the nibble's places is put right on the other side:
+// queries that meet 2^-20 codes are divided by 16 beforehand, output dimensions that they made are afterwards. The
+// groups' scales and biases never touch the codes:
+//   s_j = scale * sum_g ks_jg (q . codes)_g + kb_jg sum(q)_g,
+//   o_g = sum_j w_jg (codes_jg - z_jg) + p_j (vb_jg + z_jg vs_jg),   w_jg = p_j vs_jg,  z_jg = round(-vb_jg / vs_jg) in 0..15,
+// scores in fp32, and w rounded to fp16 once (2^-12 against the 2^-9 of a bf16 output), after a power of two that puts
+// the warp's largest value scale at 2^9 .. 2^14. codes - z (exact on subnormals, one packed subtraction a pair) takes out
+// of a group what its codes and its bias have in common, so that the rounding of w is one of the value itself, however
+// near to 0 it lies. Queries are put into fp16 with a power of two a row, exact for bf16 but for values 2^-27 below the
+// row's largest. A score tile's accumulator layout is transposed into the value MMA's operand by movmatrix.
+// A masked key's score is -inf and its w and p vb are set to 0, not multiplied, so that what it holds never matters.
+//
+// Each warp walks 32-key steps through a ring of its own, filled with cp.async STAGES - 1 steps ahead; the pages of the
+// next 8 steps are looked up by the 32 lanes at once (8 keys always lie in one page). Rows are permuted within a chunk
+// (P8) and 32-byte pieces swizzled (kv4_swz) so that every shared load is free of bank conflicts.
+// The keys of all (request, kv head, tile)s, in steps of 128, are dealt out evenly over one wave of CTAs, wherever the
+// boundaries fall; a CTA that holds only part of an item writes a part (m, l, O) to the workspace, at most two a CTA,
+// and kv4_join_kernel joins them. HBM-bound for few rows: D + D / 8 bytes a key and kv head (144 at D = 128).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -19,13 +40,11 @@
 
 namespace lq {
 
-constexpr int KV4_NW = 4;
+constexpr int KV4_NW = 4;                 // warps a CTA
+constexpr int KV4_KEYS = 32;              // keys a warp step
+constexpr int KV4_STEP = KV4_NW * KV4_KEYS;  // keys a CTA step
 constexpr float KV4_LOG2E = 1.4426950408889634f;
-
-// A sink's logit in base 2, finite at its upper end so that differences from it stay numbers.
-__device__ __forceinline__ float kv4_sink(const float* sinks, int head) {
-    return sinks ? fminf(sinks[head] * KV4_LOG2E, 3.4028234e38f) : -INFINITY;
-}
+constexpr uint32_t KV4_NONE = 0xffffffffu;  // no page
 
 struct Kv4AttArgs {
     Kv4Pool pool;
@@ -35,109 +54,747 @@ struct Kv4AttArgs {
     const int32_t* lens;
     const float* sinks;
     uint16_t* out;
+    float* part_ml;  // (CTA, 2, rows) x {m, l}, base 2
+    float* part_o;   // (CTA, 2, rows) x D
     float scale_log2;
-    int N, B, H, width, window;
+    int N, B, H, G, width, window, max_q;
 };
 
-template <typename T, int D>
-__global__ void __launch_bounds__(KV4_NW * 32) kv4_attend_kernel(const Kv4AttArgs a) {
-    constexpr int E = D / 32;  // dimensions a lane
-    __shared__ float sm[KV4_NW], sl[KV4_NW], so[KV4_NW][D];
-    grid_dep_wait();
-    const int n = blockIdx.x, h = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    uint16_t* out = a.out + ((size_t)n * a.H + h) * D;
-    int b = n, pos = 0, len = 0;
-    bool real = n < a.B;
+// A sink's logit in base 2, finite at its upper end so that differences from it stay numbers.
+__device__ __forceinline__ float kv4_sink(const float* sinks, int head) {
+    return sinks ? fminf(sinks[head] * KV4_LOG2E, 3.4028234e38f) : -INFINITY;
+}
+__device__ __forceinline__ float kv4_ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ uint32_t kv4_transpose(uint32_t x) {
+    uint32_t y;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+
+// A request's place in the step: its queries' first row, their number, its keys and the 128-key steps that they span.
+struct Kv4Req {
+    int first, fresh, len, s_lo, s_hi, tiles;
+    __device__ __forceinline__ int steps() const { return s_hi - s_lo; }
+};
+
+template <int R>
+__device__ __forceinline__ Kv4Req kv4_request(const Kv4AttArgs& a, int b) {
+    Kv4Req r;
+    r.first = b;
+    r.fresh = b < a.N ? 1 : 0;
     if (a.q_start) {
-        int lo = 0, hi = a.B;
-        while (hi - lo > 1) {
-            const int mid = (lo + hi) >> 1;
-            if (a.q_start[mid] <= n)
-                lo = mid;
-            else
-                hi = mid;
-        }
-        b = lo;
-        real = n < a.q_start[a.B];
+        r.first = max(a.q_start[b], 0);
+        r.fresh = max(min(a.q_start[b + 1], a.N) - r.first, 0);
+        if (r.fresh > a.max_q) r.fresh = a.max_q;
     }
-    if (real) {
-        len = a.lens[b];
-        if ((long long)len > (long long)a.width * a.pool.page) {
-            record_status(LQ_DEV_BOUNDS);
-            len = a.width * a.pool.page;
-        }
-        pos = a.q_start ? len - (a.q_start[b + 1] - n) : len - 1;
-    }
-    const int hi = real ? pos + 1 : 0, lo = a.window ? max(0, hi - a.window) : 0;
-    const int G = a.H / a.pool.KVH, kvh = h / G;
-    float q[E], o[E], m = -INFINITY, l = 0.0f;
+    r.len = a.lens[b];
+    const long long room = (long long)a.width * a.pool.page;
+    const int keys = int(min((long long)max(r.len, 0), room));
+    const int lo = a.window ? max(0, r.len - r.fresh + 1 - a.window) : 0;
+    r.s_lo = min(lo, keys) / KV4_STEP;
+    r.s_hi = max((keys + KV4_STEP - 1) / KV4_STEP, r.s_lo + 1);  // (a step at least: what sees nothing is written too)
+    r.tiles = (r.fresh * a.G + R - 1) / R;
+    return r;
+}
+
+// Steps of all of request b's items.
+template <int R>
+__device__ __forceinline__ int kv4_weight(const Kv4AttArgs& a, int b) {
+    const Kv4Req r = kv4_request<R>(a, b);
+    return r.tiles * r.steps() * a.pool.KVH;
+}
+
+// The CTA that the x-th of S steps falls to: CTA i of n has steps i S / n .. (i + 1) S / n - 1.
+__device__ __forceinline__ int kv4_owner(long long x, long long S, int n) { return int(((x + 1) * n - 1) / S); }
+
+// Sum over the CTA's 128 threads (every thread gets it).
+__device__ __forceinline__ int kv4_sum(int v, int* red) {
+    v = __reduce_add_sync(0xffffffffu, v);
+    __syncthreads();
+    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
+    __syncthreads();
+    return red[0] + red[1] + red[2] + red[3];
+}
+
+template <int D>
+struct Kv4Shape {
+    static constexpr int GR = D / 64;
+    static constexpr int RB = D / 2;                      // bytes of codes a key
+    static constexpr int KV_BYTES = KV4_KEYS * RB;        // a step's key (or value) codes
+    static constexpr int SC = 8 * GR;                     // bytes of scales and biases a key
+    static constexpr int STAGE = 2 * KV_BYTES + KV4_KEYS * SC;
+    static constexpr int STAGES = D == 64 ? 4 : D == 128 ? 3 : 2;
+    static constexpr int FL = 4 * GR;                     // floats a key made of its scales and biases
+    static constexpr int ZB = 2 * GR;                     // bytes of z a key
+    static constexpr int WARP = STAGES * STAGE + KV4_KEYS * (FL * 4 + ZB);
+    static constexpr int RING = KV4_NW * WARP;            // 39,168 / 59,904 / 82,944 bytes: 4, 3, 2 CTAs a SM
+};
+
+// Row x of a chunk's 8 keys in the MMA's order, and the 32-byte piece of group g in row r: with these, the 4 rows that
+// half a warp reads as keys, and the 4 that a warp reads as values, fall on different banks.
+__device__ __forceinline__ int kv4_p8(int x) { return (0x57463120u >> (4 * x)) & 7; }
+__device__ __forceinline__ int kv4_p8_inv(int r) { return (0x64753120u >> (4 * r)) & 7; }
+template <int D>
+__device__ __forceinline__ int kv4_swz(int r, int g) {
+    return D == 64 ? 0 : D == 128 ? (g ^ ((r >> 1) & 1)) : (g ^ (r & 3));
+}
+
+// a - b on pairs of fp16 subnormals: exact.
+__device__ __forceinline__ uint32_t kv4_sub(uint32_t a, uint32_t b) {
+    const __half2 d = __hsub2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
+    return *reinterpret_cast<const uint32_t*>(&d);
+}
+__device__ __forceinline__ uint32_t lds32(uint32_t addr) {
+    uint32_t v;
+    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(addr));
+    return v;
+}
+
+// N floats from shared memory: from a multiple of 16 bytes where N is above 3, of 8 else.
+template <int N>
+__device__ __forceinline__ void kv4_floats(uint32_t addr, float (&f)[N]) {
+    constexpr int Q = N / 4 * 4;
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-        q[e] = F16Traits<T>::to_f32(a.q[((size_t)n * a.H + h) * D + lane * E + e]) * a.scale_log2;
-        o[e] = 0.0f;
+    for (int i = 0; i < Q; i += 4)
+        asm volatile("ld.shared.v4.f32 {%0,%1,%2,%3}, [%4];"
+                     : "=f"(f[i]), "=f"(f[i + 1]), "=f"(f[i + 2]), "=f"(f[i + 3])
+                     : "r"(addr + 4 * i));
+    if constexpr (N % 4 >= 2) asm volatile("ld.shared.v2.f32 {%0,%1}, [%2];" : "=f"(f[Q]), "=f"(f[Q + 1]) : "r"(addr + 4 * Q));
+    if constexpr (N % 2 == 1) asm volatile("ld.shared.f32 %0, [%1];" : "=f"(f[N - 1]) : "r"(addr + 4 * (N - 1)));
+}
+
+// A row's softmax parts (m, l, O; base 2) with its sink: T(O / L), 0 where nothing was seen.
+template <typename T>
+__device__ __forceinline__ uint16_t kv4_finish(float m, float l, float o, float sink) {
+    const float M = fmaxf(m, sink);
+    if (M == -INFINITY) return F16Traits<T>::from_f32(l != l ? l : 0.0f);
+    const float f = kv4_ex2(m - M), L = l * f + kv4_ex2(sink - M);
+    return F16Traits<T>::from_f32(L == 0.0f ? 0.0f : o * f / L);
+}
+
+// CTAs a SM, by registers (8 rows: 128 / 168 / 255 a thread) and shared memory.
+constexpr int kv4_resident(int D, int NT) { return NT == 2 || D == 256 ? 2 : D == 128 ? 3 : 4; }
+
+template <typename T, int D, int NT>
+__global__ void __launch_bounds__(KV4_NW * 32, kv4_resident(D, NT)) kv4_attend_kernel(const Kv4AttArgs a) {
+    using S = Kv4Shape<D>;
+    constexpr int GR = S::GR, R = 8 * NT;
+    extern __shared__ __align__(128) uint8_t kv4_smem[];
+    __shared__ int red[KV4_NW];
+    grid_dep_wait();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gid = lane >> 2, c = lane & 3;
+    const int tid = threadIdx.x, KVH = a.pool.KVH, G = a.G;
+
+    // rows past the last query are 0
+    if (a.q_start) {
+        const long long from = (long long)max(min(a.q_start[a.B], a.N), 0) * a.H * D / 8, to = (long long)a.N * a.H * D / 8;
+        for (long long i = from + (long long)blockIdx.x * blockDim.x + tid; i < to; i += (long long)gridDim.x * blockDim.x)
+            reinterpret_cast<uint4*>(a.out)[i] = make_uint4(0, 0, 0, 0);
     }
-    for (int j = lo + warp; j < hi; j += KV4_NW) {
-        const int id = a.table[(size_t)b * a.width + j / a.pool.page];
-        if (unsigned(id) >= unsigned(a.pool.pages)) {
-            record_status(LQ_DEV_BOUNDS);
+
+    // ---- this CTA's share of the steps: requests are scanned 128 at a time ----
+    long long total = 0;
+    for (int b0 = 0; b0 < a.B; b0 += KV4_NW * 32) total += kv4_sum(b0 + tid < a.B ? kv4_weight<R>(a, b0 + tid) : 0, red);
+    const int n = int(min((long long)gridDim.x, total));  // (every CTA below n has a step, those above none)
+    if (int(blockIdx.x) >= n) return;
+    const long long x0 = (long long)blockIdx.x * total / n, x1 = ((long long)blockIdx.x + 1) * total / n;
+    int b = 0;
+    long long at = 0;  // steps before request b
+    for (int b0 = 0;; b0 += KV4_NW * 32) {
+        const int w = b0 + tid < a.B ? kv4_weight<R>(a, b0 + tid) : 0;
+        const int sum = kv4_sum(w, red);
+        if (at + sum <= x0) {
+            at += sum;
             continue;
         }
-        const size_t row = kv4_row(a.pool, id, kvh, j % a.pool.page);
-        const size_t g = row * (D / 64) + lane * E / 64;
-        const uint32_t kw = a.pool.kq[row * (D / 8) + lane * E / 8] >> (4 * (lane * E % 8));
-        const uint32_t vw = a.pool.vq[row * (D / 8) + lane * E / 8] >> (4 * (lane * E % 8));
-        const float ks = F16Traits<T>::to_f32(a.pool.ks[g]), kb = F16Traits<T>::to_f32(a.pool.kb[g]);
-        const float vs = F16Traits<T>::to_f32(a.pool.vs[g]), vb = F16Traits<T>::to_f32(a.pool.vb[g]);
-        float s = 0.0f;
+        // inclusive sums within the 128, then the first request whose steps reach past x0
+        int s = w;
 #pragma unroll
-        for (int e = 0; e < E; ++e) s = fmaf(q[e], fmaf(ks, float((kw >> (4 * e)) & 15u), kb), s);
-#pragma unroll
-        for (int d = 16; d; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
-        const float mn = fmaxf(m, s);
-        const float c = mn == -INFINITY ? 1.0f : exp2f(m - mn), p = mn == -INFINITY ? 0.0f : exp2f(s - mn);
-        l = l * c + p;
-        m = mn;
-#pragma unroll
-        for (int e = 0; e < E; ++e) o[e] = fmaf(p, fmaf(vs, float((vw >> (4 * e)) & 15u), vb), o[e] * c);
-    }
-    if (lane == 0) sm[warp] = m, sl[warp] = l;
-#pragma unroll
-    for (int e = 0; e < E; ++e) so[warp][lane * E + e] = o[e];
-    __syncthreads();
-    const float sink = kv4_sink(a.sinks, h);
-    float M = sink;
-#pragma unroll
-    for (int w = 0; w < KV4_NW; ++w) M = fmaxf(M, sm[w]);
-    for (int d = threadIdx.x; d < D; d += KV4_NW * 32) {
-        float L = sink == -INFINITY || !real ? 0.0f : exp2f(sink - M), O = 0.0f;
-#pragma unroll
-        for (int w = 0; w < KV4_NW; ++w) {
-            const float f = sm[w] == -INFINITY ? 0.0f : exp2f(sm[w] - M);
-            L += sl[w] * f;
-            O += so[w][d] * f;
+        for (int d = 1; d < 32; d <<= 1) {
+            const int u = __shfl_up_sync(0xffffffffu, s, d);
+            if (lane >= d) s += u;
         }
-        out[d] = F16Traits<T>::from_f32(L > 0.0f ? O / L : (L == L ? 0.0f : L));
+        __syncthreads();
+        if (lane == 31) red[warp] = s;
+        __syncthreads();
+        for (int k = 0; k < warp; ++k) s += red[k];
+        const bool past = at + s > x0;
+        const int before = kv4_sum(past ? 0 : 1, red);  // (sums ascend: these come first)
+        const int skipped = kv4_sum(past ? 0 : w, red);
+        b = b0 + before;
+        at += skipped;
+        break;
+    }
+
+    const uint32_t ring = smem_u32(kv4_smem) + warp * S::WARP;
+    const uint32_t made = ring + S::STAGES * S::STAGE;  // the step's floats: ks, kb, vs', vb' (GR each) a key
+    const uint32_t zeds = made + KV4_KEYS * S::FL * 4;  // and its z, 2 bytes each: (group, chunk, place in the MMA's order)
+    long long x = x0;
+    while (x < x1) {
+        Kv4Req rq = kv4_request<R>(a, b);
+        const int item = int((x - at) / max(rq.steps(), 1));
+        if (rq.tiles == 0 || item >= rq.tiles * KVH) {  // on to the next request
+            at += (long long)rq.tiles * rq.steps() * KVH;
+            ++b;
+            continue;
+        }
+        const int kvh = item / rq.tiles, row0 = (item - kvh * rq.tiles) * R;
+        const long long item_at = at + (long long)item * rq.steps();
+        const int st0 = int(x - item_at), st1 = int(min((long long)rq.steps(), x1 - item_at));
+        x = item_at + st1;
+        const int rows = min(R, rq.fresh * G - row0);
+        // what the tile's rows see: keys below hi_max, from lo_min on; all of them see [lo_max, hi_min)
+        const int base = rq.len - rq.fresh;  // position of query 0
+        const int room = int(min((long long)a.width * a.pool.page, 0x7fffffffLL));
+        if (rq.len > room) record_status(LQ_DEV_BOUNDS);
+        const int hi_min = min(base + row0 / G + 1, room), hi_max = min(base + (row0 + rows - 1) / G + 1, room);
+        const int lo_min = a.window ? max(base + row0 / G + 1 - a.window, 0) : 0;
+        const int lo_max = a.window ? max(base + (row0 + rows - 1) / G + 1 - a.window, 0) : 0;
+        const int k_lo = max((rq.s_lo + st0) * KV4_STEP, lo_min / KV4_KEYS * KV4_KEYS);
+        const int k_hi = min((rq.s_lo + st1) * KV4_STEP, hi_max);
+        // this warp's 32-key steps: first, first + 128, ...
+        const int first = ((k_lo + KV4_STEP - 1 - warp * KV4_KEYS) / KV4_STEP) * KV4_STEP + warp * KV4_KEYS;
+        const int steps = k_hi > first ? (k_hi - first + KV4_STEP - 1) / KV4_STEP : 0;
+
+        // lane l's page lookup: run l & 3 of 8 keys of step t0 + (l >> 2)
+        auto lookup = [&](int t0) -> uint32_t {
+            const int key = first + (t0 + (lane >> 2)) * KV4_STEP + (lane & 3) * 8;
+            if (t0 + (lane >> 2) >= steps || key >= hi_max) return KV4_NONE;
+            const int pg = key / a.pool.page;
+            const int id = a.table[(size_t)b * a.width + pg];
+            if (unsigned(id) >= unsigned(a.pool.pages)) {
+                record_status(LQ_DEV_BOUNDS);
+                return KV4_NONE;
+            }
+            return kv4_row(a.pool, id, kvh, key - pg * a.pool.page);
+        };
+        uint32_t runs = lookup(0), runs_next = lookup(8);
+        // bit 4 (t & 7) + r: run r of step t is within the range but has no page (of the steps computed, and issued)
+        auto missing = [&](int t0, uint32_t held) -> uint32_t {
+            const int key = first + (t0 + (lane >> 2)) * KV4_STEP + (lane & 3) * 8;
+            return __ballot_sync(0xffffffffu, held == KV4_NONE && t0 + (lane >> 2) < steps && key < hi_max);
+        };
+        uint32_t miss_now = missing(0, runs), miss_issued = miss_now;
+
+        // ---- queries: fp16 B fragments times a row's power of two, and the group sums of what the MMA sees ----
+        uint32_t qb[NT][GR][2][2][2];
+        float alpha[NT][2], qs[NT][GR][2];
+        int col_hi[NT][2], col_lo[NT][2];
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            const int row = row0 + 8 * t + gid;
+            const bool live = 8 * t + gid < rows;
+            const int qi = live ? row / G : 0, hd = kvh * G + (live ? row - qi * G : 0);
+            const uint4* src = reinterpret_cast<const uint4*>(a.q + ((size_t)(rq.first + qi) * a.H + hd) * D);
+            float mx = 0.0f;
+            uint4 raw[GR][2];
+#pragma unroll
+            for (int g = 0; g < GR; ++g)
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    raw[g][u] = live ? src[8 * g + 2 * c + u] : make_uint4(0, 0, 0, 0);
+                    const uint32_t* w = reinterpret_cast<const uint32_t*>(&raw[g][u]);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        mx = fmaxf(mx, fmaxf(fabsf(F16Traits<T>::to_f32(w[i] & 0xffffu)),
+                                             fabsf(F16Traits<T>::to_f32(w[i] >> 16))));
+                }
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+            // 2^E with the row's largest |q| at 2^13 .. 2^14
+            int E = mx > 0.0f ? 13 - (int((__float_as_uint(mx) >> 23) & 0xff) - 127) : 0;
+            E = min(max(E, -100), 100);
+            const float f = __uint_as_float(uint32_t(127 + E) << 23);
+            float sums[GR];
+#pragma unroll
+            for (int g = 0; g < GR; ++g) {
+                sums[g] = 0.0f;
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    const uint32_t* w = reinterpret_cast<const uint32_t*>(&raw[g][u]);
+                    float v[8];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        v[2 * i] = __half2float(__float2half_rn(F16Traits<T>::to_f32(w[i] & 0xffffu) * f));
+                        v[2 * i + 1] = __half2float(__float2half_rn(F16Traits<T>::to_f32(w[i] >> 16) * f));
+                    }
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) sums[g] += v[i];
+#pragma unroll
+                    for (int m = 0; m < 2; ++m) {
+                        qb[t][g][u][m][0] = cvt_f16x2(v[2 * m + 4], v[2 * m]);
+                        qb[t][g][u][m][1] = cvt_f16x2(v[2 * m + 5] * 0.0625f, v[2 * m + 1] * 0.0625f);
+                    }
+                }
+                sums[g] += __shfl_xor_sync(0xffffffffu, sums[g], 1);
+                sums[g] += __shfl_xor_sync(0xffffffffu, sums[g], 2);
+            }
+            const float back = a.scale_log2 * __uint_as_float(uint32_t(127 - E) << 23);
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {  // this lane's columns 2c + e of the score tile
+                const int from = (2 * c + e) * 4;
+                const float bk = __shfl_sync(0xffffffffu, back, from);
+                alpha[t][e] = bk * 16777216.0f;
+#pragma unroll
+                for (int g = 0; g < GR; ++g) qs[t][g][e] = bk * __shfl_sync(0xffffffffu, sums[g], from);
+                const int r = 8 * t + 2 * c + e, p = base + (row0 + min(r, rows - 1)) / G + 1;
+                col_hi[t][e] = min(p, room);
+                col_lo[t][e] = a.window ? max(p - a.window, 0) : 0;
+            }
+        }
+
+        // ---- the ring ----
+        auto issue = [&](int t, uint32_t lanes_runs) {
+            const uint32_t sb = ring + (t % S::STAGES) * S::STAGE;
+            constexpr int PIECES = S::RB / 16;  // 16-byte pieces a key
+            constexpr int J = KV4_KEYS * PIECES / 32;
+            const int sel = (t & 7) * 4;
+#pragma unroll
+            for (int j = 0; j < J; ++j) {
+                const int e = lane + 32 * j, r = e / PIECES, p = e % PIECES;
+                const uint32_t rb = __shfl_sync(0xffffffffu, lanes_runs, sel + r / 8);
+                const bool ok = rb != KV4_NONE;
+                const size_t row = ok ? rb + (r & 7) : 0;
+                const uint32_t off = r * S::RB + (kv4_swz<D>(r, p >> 1) << 5) + ((p & 1) << 4);
+                cp_async(sb + off, reinterpret_cast<const uint8_t*>(a.pool.kq) + row * S::RB + p * 16, 16, ok);
+                cp_async(sb + S::KV_BYTES + off, reinterpret_cast<const uint8_t*>(a.pool.vq) + row * S::RB + p * 16, 16, ok);
+            }
+            // scales and biases: a key's four arrays side by side (two keys' for one group: a pair of 2-byte values)
+            constexpr int PK = D == 64 ? 2 : 1, BY = D == 256 ? 8 : 4;
+            const int r = (lane % (KV4_KEYS / PK)) * PK;
+            const uint32_t rb = __shfl_sync(0xffffffffu, lanes_runs, sel + r / 8);
+            const bool ok = rb != KV4_NONE;
+            const size_t row = (ok ? rb + (r & 7) : 0) * GR;
+            const uint32_t dst = sb + 2 * S::KV_BYTES + r * S::SC;
+            if (D != 64 || lane < 16) {
+                cp_async(dst, a.pool.ks + row, BY, ok);
+                cp_async(dst + BY, a.pool.kb + row, BY, ok);
+                cp_async(dst + 2 * BY, a.pool.vs + row, BY, ok);
+                cp_async(dst + 3 * BY, a.pool.vb + row, BY, ok);
+            }
+        };
+        auto commit = [] { asm volatile("cp.async.commit_group;" ::: "memory"); };
+
+        float o[NT][4 * GR][4], hb[NT][GR][2], m[NT][2], l[NT][2];
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+#pragma unroll
+            for (int i = 0; i < 4 * GR; ++i)
+#pragma unroll
+                for (int u = 0; u < 4; ++u) o[t][i][u] = 0.0f;
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                m[t][e] = -INFINITY, l[t][e] = 0.0f;
+#pragma unroll
+                for (int g = 0; g < GR; ++g) hb[t][g][e] = 0.0f;
+            }
+        }
+        float vf = 1.0f;       // the value scales' power of two
+        uint32_t v_limit = 0;  // bits of the largest value scale that it fits (0: none met yet)
+
+#pragma unroll
+        for (int t = 0; t < S::STAGES - 1; ++t) {
+            if (t < steps) issue(t, runs);
+            commit();
+        }
+        for (int t = 0; t < steps; ++t) {
+            const int nx = t + S::STAGES - 1;
+            if (nx < steps) {
+                if ((nx & 7) == 0) {
+                    runs = runs_next;
+                    miss_issued = missing(nx, runs);
+                    runs_next = lookup(nx + 8);
+                }
+                issue(nx, runs);
+            }
+            if ((t & 7) == 0) miss_now = miss_issued;
+            commit();
+            asm volatile("cp.async.wait_group %0;" ::"n"(S::STAGES - 1) : "memory");
+            __syncwarp();
+            const uint32_t sb = ring + (t % S::STAGES) * S::STAGE;
+            const int key0 = first + t * KV4_STEP;
+            const bool inside = key0 >= lo_max && key0 + KV4_KEYS <= hi_min;
+
+
+            // one key a lane: its scales and biases in fp32, and the values' z; a key out of range has none
+            const uint32_t miss = (miss_now >> ((t & 7) * 4)) & 0xfu;  // runs of 8 keys whose page is missing
+            {
+                float w[4][GR];  // ks, kb, vs, vb
+                const uint32_t p = sb + 2 * S::KV_BYTES + (D == 64 ? lane & ~1 : lane) * S::SC;
+                if constexpr (D == 64) {
+                    const uint4 v = lds128(p);
+                    const int sh = (lane & 1) * 16;
+                    w[0][0] = F16Traits<T>::to_f32((v.x >> sh) & 0xffffu), w[1][0] = F16Traits<T>::to_f32((v.y >> sh) & 0xffffu);
+                    w[2][0] = F16Traits<T>::to_f32((v.z >> sh) & 0xffffu), w[3][0] = F16Traits<T>::to_f32((v.w >> sh) & 0xffffu);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < GR / 2; ++i) {
+                        const uint4 v = lds128(p + 16 * i);
+                        const uint32_t x[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {  // D = 128: one word an array; D = 256: two
+                            const int arr = D == 128 ? k : 2 * i + k / 2, g = D == 128 ? 0 : 2 * (k & 1);
+                            w[arr][g] = F16Traits<T>::to_f32(x[k] & 0xffffu);
+                            w[arr][g + 1] = F16Traits<T>::to_f32(x[k] >> 16);
+                        }
+                    }
+                }
+                const int key = key0 + lane;
+                if (key < lo_min || key >= hi_max || ((miss >> (lane >> 3)) & 1)) {
+#pragma unroll
+                    for (int g = 0; g < GR; ++g) w[2][g] = 0.0f, w[3][g] = 0.0f;
+                }
+                // the value scales' power of two: larger scales are met by a smaller one
+                float top = 0.0f;
+#pragma unroll
+                for (int g = 0; g < GR; ++g) top = fmaxf(top, fabsf(w[2][g]));
+                uint32_t bits = __reduce_max_sync(0xffffffffu, __float_as_uint(top));
+                if (bits > v_limit) {
+                    if (bits >= 0x7f800000u) {  // an infinite scale: go by the finite ones
+                        top = 0.0f;
+#pragma unroll
+                        for (int g = 0; g < GR; ++g)
+                            if (fabsf(w[2][g]) < INFINITY) top = fmaxf(top, fabsf(w[2][g]));
+                        bits = __reduce_max_sync(0xffffffffu, __float_as_uint(top));
+                    }
+                    if (bits > v_limit) {
+                        const int E = max(int(bits >> 23), 64);  // (at least 2^-63)
+                        const float nf = __uint_as_float(uint32_t(127 + 9 + 127 - E) << 23);  // to 2^9 .. 2^10
+                        const float ratio = nf / vf;
+#pragma unroll
+                        for (int tt = 0; tt < NT; ++tt) {
+#pragma unroll
+                            for (int i = 0; i < 4 * GR; ++i)
+#pragma unroll
+                                for (int u = 0; u < 4; ++u) o[tt][i][u] *= ratio;
+#pragma unroll
+                            for (int g = 0; g < GR; ++g) hb[tt][g][0] *= ratio, hb[tt][g][1] *= ratio;
+                        }
+                        vf = nf;
+                        v_limit = (uint32_t(E + 5) << 23) - 1;  // below 2^14 / vf
+                    }
+                }
+                float f[S::FL];
+#pragma unroll
+                for (int g = 0; g < GR; ++g) {
+                    const float z = fminf(fmaxf(rintf(__fdividef(-w[3][g], w[2][g])), 0.0f), 15.0f);
+                    f[g] = w[0][g];
+                    f[GR + g] = w[1][g];
+                    f[2 * GR + g] = w[2][g] * vf;
+                    f[3 * GR + g] = fmaf(z, w[2][g], w[3][g]) * vf;
+                    asm volatile("st.shared.u16 [%0], %1;" ::"r"(zeds + ((g * 2 + (lane >> 4)) * 16 + (lane & 8) + kv4_p8_inv(lane & 7)) * 2),
+                                 "h"(uint16_t(z))
+                                 : "memory");
+                }
+#pragma unroll
+                for (int i = 0; i < S::FL; i += 4)
+                    asm volatile("st.shared.v4.f32 [%0], {%1,%2,%3,%4};" ::"r"(made + (lane * S::FL + i) * 4), "f"(f[i]),
+                                 "f"(f[i + 1]), "f"(f[i + 2]), "f"(f[i + 3])
+                                 : "memory");
+                __syncwarp();
+            }
+
+            // scores of this lane's keys (chunk h, half u): key0 + 16 h + 8 u + p8(gid)
+            float sc[NT][2][2][2];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                float acc[NT][GR][4];
+#pragma unroll
+                for (int tt = 0; tt < NT; ++tt)
+#pragma unroll
+                    for (int g = 0; g < GR; ++g)
+#pragma unroll
+                        for (int u = 0; u < 4; ++u) acc[tt][g][u] = 0.0f;
+                const int r0 = 16 * h + kv4_p8(gid), r1 = r0 + 8;
+#pragma unroll
+                for (int g = 0; g < GR; ++g) {
+                    uint32_t xw[2], yw[2];
+                    asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];"
+                                 : "=r"(xw[0]), "=r"(xw[1])
+                                 : "r"(sb + r0 * S::RB + (kv4_swz<D>(r0, g) << 5) + 8 * c));
+                    asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];"
+                                 : "=r"(yw[0]), "=r"(yw[1])
+                                 : "r"(sb + r1 * S::RB + (kv4_swz<D>(r1, g) << 5) + 8 * c));
+#pragma unroll
+                    for (int u = 0; u < 2; ++u)
+#pragma unroll
+                        for (int mm = 0; mm < 2; ++mm) {
+                            const uint32_t xs = mm ? xw[u] >> 8 : xw[u], ys = mm ? yw[u] >> 8 : yw[u];
+#pragma unroll
+                            for (int tt = 0; tt < NT; ++tt)
+                                mma_16816<__half>(acc[tt][g], xs & 0x000f000fu, ys & 0x000f000fu, xs & 0x00f000f0u,
+                                                  ys & 0x00f000f0u, qb[tt][g][u][mm][0], qb[tt][g][u][mm][1]);
+                        }
+                }
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    float f[2 * GR];  // ks, kb
+                    kv4_floats<2 * GR>(made + (16 * h + 8 * u + kv4_p8(gid)) * S::FL * 4, f);
+#pragma unroll
+                    for (int tt = 0; tt < NT; ++tt)
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            float dot = f[0] * acc[tt][0][2 * u + e];
+#pragma unroll
+                            for (int g = 1; g < GR; ++g) dot = fmaf(f[g], acc[tt][g][2 * u + e], dot);
+                            float s = dot * alpha[tt][e];
+#pragma unroll
+                            for (int g = 0; g < GR; ++g) s = fmaf(f[GR + g], qs[tt][g][e], s);
+                            sc[tt][h][u][e] = s;
+                        }
+                }
+            }
+            if (!inside || miss) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) {
+                        const int key = key0 + 16 * h + 8 * u + kv4_p8(gid);
+                        const bool gone = (miss >> (2 * h + u)) & 1;
+#pragma unroll
+                        for (int tt = 0; tt < NT; ++tt)
+#pragma unroll
+                            for (int e = 0; e < 2; ++e)
+                                if (gone || key < col_lo[tt][e] || key >= col_hi[tt][e]) sc[tt][h][u][e] = -INFINITY;
+                    }
+            }
+
+            // running softmax a column (its 8 lanes agree on m)
+            uint32_t pb[NT][2][GR][2];
+#pragma unroll
+            for (int tt = 0; tt < NT; ++tt) {
+                float corr[2];
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    float mx = fmaxf(fmaxf(sc[tt][0][0][e], sc[tt][0][1][e]), fmaxf(sc[tt][1][0][e], sc[tt][1][1][e]));
+                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+                    const float mn = fmaxf(m[tt][e], mx), mz = mn == -INFINITY ? 0.0f : mn;
+                    corr[e] = kv4_ex2(m[tt][e] - mz);
+                    m[tt][e] = mn;
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
+#pragma unroll
+                        for (int u = 0; u < 2; ++u) sc[tt][h][u][e] = kv4_ex2(sc[tt][h][u][e] - mz);
+                    l[tt][e] = l[tt][e] * corr[e] + ((sc[tt][0][0][e] + sc[tt][0][1][e]) + (sc[tt][1][0][e] + sc[tt][1][1][e]));
+                }
+                if (__any_sync(0xffffffffu, corr[0] != 1.0f || corr[1] != 1.0f)) {
+#pragma unroll
+                    for (int i = 0; i < 4 * GR; ++i) {
+                        o[tt][i][0] *= corr[0];
+                        o[tt][i][1] *= corr[1];
+                        o[tt][i][2] *= corr[0];
+                        o[tt][i][3] *= corr[1];
+                    }
+#pragma unroll
+                    for (int g = 0; g < GR; ++g) hb[tt][g][0] *= corr[0], hb[tt][g][1] *= corr[1];
+                }
+            }
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    float f[2 * GR];  // vs', vb'
+                    kv4_floats<2 * GR>(made + ((16 * h + 8 * u + kv4_p8(gid)) * S::FL + 2 * GR) * 4, f);
+                    const int key = key0 + 16 * h + 8 * u + kv4_p8(gid);
+#pragma unroll
+                    for (int tt = 0; tt < NT; ++tt)
+#pragma unroll
+                        for (int g = 0; g < GR; ++g) {
+                            float w[2];
+#pragma unroll
+                            for (int e = 0; e < 2; ++e) {
+                                w[e] = sc[tt][h][u][e] * f[g];
+                                float y = sc[tt][h][u][e] * f[GR + g];
+                                if (!inside && (key < col_lo[tt][e] || key >= col_hi[tt][e])) w[e] = 0.0f, y = 0.0f;
+                                hb[tt][g][e] += y;
+                            }
+                            pb[tt][h][g][u] = kv4_transpose(cvt_f16x2(w[1], w[0]));
+                        }
+                }
+
+            // values: keys p8(2c), p8(2c + 1) (+ 8) of a chunk, dimensions 64 g + 8 gid + i
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int ra = 16 * h + kv4_p8(2 * c), rb = 16 * h + kv4_p8(2 * c + 1);
+#pragma unroll
+                for (int g = 0; g < GR; ++g) {
+                    const uint32_t pa = sb + S::KV_BYTES + ra * S::RB + (kv4_swz<D>(ra, g) << 5) + 4 * gid;
+                    const uint32_t pz = sb + S::KV_BYTES + rb * S::RB + (kv4_swz<D>(rb, g) << 5) + 4 * gid;
+                    const uint32_t wa = lds32(pa), wb = lds32(pz), wc = lds32(pa + 8 * S::RB), wd = lds32(pz + 8 * S::RB);
+                    uint32_t ab[2], cd[2];
+                    ab[0] = prmt(wa, wb, 0x5410u), ab[1] = prmt(wa, wb, 0x7632u);
+                    cd[0] = prmt(wc, wd, 0x5410u), cd[1] = prmt(wc, wd, 0x7632u);
+                    const uint32_t za = lds32(zeds + (g * 2 + h) * 32 + 4 * c), zc = lds32(zeds + (g * 2 + h) * 32 + 16 + 4 * c);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const uint32_t xs = i & 1 ? ab[i >> 1] >> 8 : ab[i >> 1], ys = i & 1 ? cd[i >> 1] >> 8 : cd[i >> 1];
+                        const uint32_t a0 = kv4_sub(xs & 0x000f000fu, za), a1 = kv4_sub(xs & 0x00f000f0u, za << 4);
+                        const uint32_t a2 = kv4_sub(ys & 0x000f000fu, zc), a3 = kv4_sub(ys & 0x00f000f0u, zc << 4);
+#pragma unroll
+                        for (int tt = 0; tt < NT; ++tt)
+                            mma_16816<__half>(o[tt][4 * g + i], a0, a1, a2, a3, pb[tt][h][g][0], pb[tt][h][g][1]);
+                    }
+                }
+            }
+            __syncwarp();
+        }
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
+        if (x >= x1) grid_dep_launch();
+
+        // ---- the four warps' states joined in shared memory (over the rings) ----
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+#pragma unroll
+                for (int d = 4; d < 32; d <<= 1) {
+                    l[t][e] += __shfl_xor_sync(0xffffffffu, l[t][e], d);
+#pragma unroll
+                    for (int g = 0; g < GR; ++g) hb[t][g][e] += __shfl_xor_sync(0xffffffffu, hb[t][g][e], d);
+                }
+        __syncthreads();  // every warp is done with its ring
+        float* cm = reinterpret_cast<float*>(kv4_smem);  // [warp][R] m, then l, then O [warp][R][D]
+        float *cl = cm + KV4_NW * R, *co = cl + KV4_NW * R;
+        const float inv = 1.0f / vf;
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const int col = warp * R + 8 * t + 2 * c + e;
+                if (gid == 0) cm[col] = m[t][e], cl[col] = l[t][e];
+                float* dst = co + col * D + 8 * gid;
+#pragma unroll
+                for (int g = 0; g < GR; ++g)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        *reinterpret_cast<float2*>(dst + 64 * g + 2 * i) =
+                            make_float2(fmaf(o[t][4 * g + i][e], 16777216.0f, hb[t][g][e]) * inv,
+                                        fmaf(o[t][4 * g + i][2 + e], 1048576.0f, hb[t][g][e]) * inv);
+            }
+        __syncthreads();
+        const bool whole = st0 == 0 && st1 == rq.steps();
+        const size_t part = ((size_t)blockIdx.x * 2 + (st0 == 0 ? 1 : 0)) * R;
+        for (int j = 0; j < rows; ++j) {
+            float M = -INFINITY;
+#pragma unroll
+            for (int w = 0; w < KV4_NW; ++w) M = fmaxf(M, cm[w * R + j]);
+            float f[KV4_NW], L = 0.0f;
+#pragma unroll
+            for (int w = 0; w < KV4_NW; ++w) {
+                f[w] = cm[w * R + j] == -INFINITY ? 0.0f : kv4_ex2(cm[w * R + j] - M);
+                L += cl[w * R + j] * f[w];
+            }
+            const int qi = (row0 + j) / G, head = kvh * G + (row0 + j) - qi * G;
+            for (int d = tid; d < D; d += KV4_NW * 32) {
+                float O = 0.0f;
+#pragma unroll
+                for (int w = 0; w < KV4_NW; ++w)
+                    if (f[w] != 0.0f) O += co[(w * R + j) * D + d] * f[w];
+                if (whole)
+                    a.out[((size_t)(rq.first + qi) * a.H + head) * D + d] = kv4_finish<T>(M, L, O, kv4_sink(a.sinks, head));
+                else
+                    a.part_o[(part + j) * D + d] = O;
+            }
+            if (!whole && tid == 0) a.part_ml[2 * (part + j)] = M, a.part_ml[2 * (part + j) + 1] = L;
+        }
+        __syncthreads();  // before the next item's ring
     }
 }
+
+// One CTA a (request, kv head, row of the request's tiles): the parts of an item that several CTAs share, joined.
+template <typename T, int D, int NT>
+__global__ void __launch_bounds__(128) kv4_join_kernel(const Kv4AttArgs a, int n) {
+    constexpr int R = 8 * NT;
+    __shared__ int red[KV4_NW];
+    grid_dep_wait();
+    const int b = blockIdx.z, kvh = blockIdx.y, row = blockIdx.x, tile = row / R;
+    long long total = 0, at = 0;
+    for (int b0 = 0; b0 < a.B; b0 += 128) {
+        const int i = b0 + threadIdx.x, w = i < a.B ? kv4_weight<R>(a, i) : 0;
+        total += kv4_sum(w, red);
+        at += kv4_sum(i < b ? w : 0, red);
+    }
+    n = int(min((long long)n, total));
+    const Kv4Req rq = kv4_request<R>(a, b);
+    if (row >= rq.fresh * a.G) return;
+    const long long item = at + ((long long)kvh * rq.tiles + tile) * rq.steps();
+    const int c0 = kv4_owner(item, total, n), c1 = kv4_owner(item + rq.steps() - 1, total, n);
+    if (c0 == c1) return;  // one CTA had it whole
+    const int j = row - tile * R;
+    auto part = [&](int cta) { return ((size_t)cta * 2 + (cta == c0 ? 1 : 0)) * R + j; };
+    float M = -INFINITY;
+    for (int cta = c0; cta <= c1; ++cta) M = fmaxf(M, a.part_ml[2 * part(cta)]);
+    const int qi = row / a.G, head = kvh * a.G + row - qi * a.G;
+    const float sink = kv4_sink(a.sinks, head);
+    for (int d = threadIdx.x; d < D; d += 128) {
+        float L = 0.0f, O = 0.0f;
+        for (int cta = c0; cta <= c1; ++cta) {
+            const size_t p = part(cta);
+            const float f = a.part_ml[2 * p] == -INFINITY ? 0.0f : kv4_ex2(a.part_ml[2 * p] - M);
+            L += a.part_ml[2 * p + 1] * f;
+            if (f != 0.0f) O += a.part_o[p * D + d] * f;
+        }
+        a.out[((size_t)(rq.first + qi) * a.H + head) * D + d] = kv4_finish<T>(M, L, O, sink);
+    }
+}
+
+// ---- host ----------------------------------------------------------------------------------------
 
 bool kv4_attend_shape_ok(int N, int B, int max_q, int H, int KVH, int width, int window) {
-    return N >= 0 && B >= 1 && max_q >= 1 && H >= 1 && H % KVH == 0 && H <= 65535 && width >= 1 && window >= 0;
+    return N >= 0 && B >= 1 && B <= 65535 && max_q >= 1 && H >= 1 && KVH >= 1 && KVH <= 65535 && H % KVH == 0 &&
+           (long long)max_q * (H / KVH) < (1 << 30) && width >= 1 && window >= 0;
 }
 
-size_t kv4_attend_workspace_bytes(int N, int B, int max_q, int H, int KVH, int D) { return 0; }
+// Row tiles: 8 rows where every request's fit, else 16 (a key's codes are then unpacked once for 16 rows).
+static int kv4_tile_rows(int max_q, int G) { return (long long)max_q * G <= 8 ? 8 : 16; }
 
-template <typename T, int D>
-static int kv4_attend_d(const Kv4AttArgs& a, cudaStream_t st) {
+// One wave of CTAs, as many as are resident (by shared memory and registers; see the launch bounds).
+static int kv4_ctas(int D, int R, int sms) { return sms * kv4_resident(D, R / 8); }
+
+size_t kv4_attend_workspace_bytes(int N, int B, int max_q, int H, int KVH, int D) {
+    const int R = kv4_tile_rows(max_q, H / KVH);
+    return size_t(kv4_ctas(D, R, device_info().sm_count)) * 2 * R * (2 + D) * sizeof(float);
+}
+
+template <typename K, typename... A>
+static int kv4_launch(K kern, dim3 grid, size_t smem, cudaStream_t st, A... args) {
+    if (smem > 48 * 1024 &&
+        cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem)) != cudaSuccess)
+        return LQ_E_CUDA;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(a.N, a.H);
+    cfg.gridDim = grid;
     cfg.blockDim = dim3(KV4_NW * 32);
+    cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, kv4_attend_kernel<T, D>, a) == cudaSuccess ? LQ_OK : LQ_E_CUDA;
+    return cudaLaunchKernelEx(&cfg, kern, args...) == cudaSuccess ? LQ_OK : LQ_E_CUDA;
+}
+
+template <typename T, int D, int NT>
+static int kv4_attend_n(const Kv4AttArgs& a, cudaStream_t st) {
+    constexpr int R = 8 * NT;
+    constexpr size_t merge = size_t(KV4_NW) * R * (2 + D) * sizeof(float);
+    constexpr size_t smem = merge > size_t(Kv4Shape<D>::RING) ? merge : size_t(Kv4Shape<D>::RING);
+    const int n = kv4_ctas(D, R, device_info().sm_count);
+    int rc = kv4_launch(kv4_attend_kernel<T, D, NT>, dim3(n), smem, st, a);
+    if (rc) return rc;
+    const int tiles = (a.max_q * a.G + R - 1) / R;
+    return kv4_launch(kv4_join_kernel<T, D, NT>, dim3(tiles * R, a.pool.KVH, a.B), 0, st, a, n);
+}
+
+template <typename T, int D>
+static int kv4_attend_d(const Kv4AttArgs& a, cudaStream_t st) {
+    return kv4_tile_rows(a.max_q, a.G) == 8 ? kv4_attend_n<T, D, 1>(a, st) : kv4_attend_n<T, D, 2>(a, st);
 }
 
 template <typename T>
@@ -149,6 +806,7 @@ int kv4_attend_run(const Kv4Pool& pool, const void* q, int N, const int32_t* q_s
                    int width, const int32_t* lens, int B, const float* sinks, float scale, int window, int H, int D,
                    int dtype, void* workspace, size_t workspace_bytes, void* out, cudaStream_t st) {
     if (N == 0) return LQ_OK;
+    if (!workspace || workspace_bytes < kv4_attend_workspace_bytes(N, B, max_q, H, pool.KVH, D)) return LQ_E_ARG;
     Kv4AttArgs a = {};
     a.pool = pool;
     a.q = static_cast<const uint16_t*>(q);
@@ -161,8 +819,13 @@ int kv4_attend_run(const Kv4Pool& pool, const void* q, int N, const int32_t* q_s
     a.N = N;
     a.B = B;
     a.H = H;
+    a.G = H / pool.KVH;
     a.width = width;
     a.window = window;
+    a.max_q = max_q;
+    const int R = kv4_tile_rows(max_q, a.G);
+    a.part_ml = static_cast<float*>(workspace);
+    a.part_o = a.part_ml + size_t(kv4_ctas(D, R, device_info().sm_count)) * 2 * R * 2;
     return dtype == LQ_BF16 ? kv4_attend_t<__nv_bfloat16>(a, D, st) : kv4_attend_t<__half>(a, D, st);
 }
 
