@@ -33,7 +33,7 @@
 #include <math.h>
 #include <stdint.h>
 
-#include "kv4.cuh"
+#include "kv4_attend.cuh"
 #include "lq_host.h"
 #include "lq_ptx.cuh"
 #include "lq_status.cuh"
@@ -43,55 +43,16 @@ namespace lq {
 constexpr int KV4_NW = 4;                 // warps a CTA
 constexpr int KV4_KEYS = 32;              // keys a warp step
 constexpr int KV4_STEP = KV4_NW * KV4_KEYS;  // keys a CTA step
-constexpr float KV4_LOG2E = 1.4426950408889634f;
-constexpr uint32_t KV4_NONE = 0xffffffffu;  // no page
-
-struct Kv4AttArgs {
-    Kv4Pool pool;
-    const uint16_t* q;
-    const int32_t* q_start;  // may be null: query b is request b's
-    const int32_t* table;
-    const int32_t* lens;
-    const float* sinks;
-    uint16_t* out;
-    float* part_ml;  // (CTA, 2, rows) x {m, l}, base 2
-    float* part_o;   // (CTA, 2, rows) x D
-    float scale_log2;
-    int N, B, H, G, width, window, max_q;
-};
-
-// A sink's logit in base 2, finite at its upper end so that differences from it stay numbers.
-__device__ __forceinline__ float kv4_sink(const float* sinks, int head) {
-    return sinks ? fminf(sinks[head] * KV4_LOG2E, 3.4028234e38f) : -INFINITY;
-}
-__device__ __forceinline__ float kv4_ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
 __device__ __forceinline__ uint32_t kv4_transpose(uint32_t x) {
     uint32_t y;
     asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
     return y;
 }
 
-// A request's place in the step: its queries' first row, their number, its keys and the 128-key steps that they span.
-struct Kv4Req {
-    int first, fresh, len, s_lo, s_hi, tiles;
-    __device__ __forceinline__ int steps() const { return s_hi - s_lo; }
-};
-
 template <int R>
 __device__ __forceinline__ Kv4Req kv4_request(const Kv4AttArgs& a, int b) {
-    Kv4Req r;
-    r.first = b;
-    r.fresh = b < a.N ? 1 : 0;
-    if (a.q_start) {
-        r.first = max(a.q_start[b], 0);
-        r.fresh = max(min(a.q_start[b + 1], a.N) - r.first, 0);
-        if (r.fresh > a.max_q) r.fresh = a.max_q;
-    }
-    r.len = a.lens[b];
+    Kv4Req r = kv4_new(a, b);
+    if (r.fresh * a.G > a.split_rows) r.fresh = 0;  // (kv4_prefill's)
     const long long room = (long long)a.width * a.pool.page;
     const int keys = int(min((long long)max(r.len, 0), room));
     const int lo = a.window ? max(0, r.len - r.fresh + 1 - a.window) : 0;
@@ -107,9 +68,6 @@ __device__ __forceinline__ int kv4_weight(const Kv4AttArgs& a, int b) {
     const Kv4Req r = kv4_request<R>(a, b);
     return r.tiles * r.steps() * a.pool.KVH;
 }
-
-// The CTA that the x-th of S steps falls to: CTA i of n has steps i S / n .. (i + 1) S / n - 1.
-__device__ __forceinline__ int kv4_owner(long long x, long long S, int n) { return int(((x + 1) * n - 1) / S); }
 
 // Sum over the CTA's 128 threads (every thread gets it).
 __device__ __forceinline__ int kv4_sum(int v, int* red) {
@@ -167,15 +125,6 @@ __device__ __forceinline__ void kv4_floats(uint32_t addr, float (&f)[N]) {
     if constexpr (N % 2 == 1) asm volatile("ld.shared.f32 %0, [%1];" : "=f"(f[N - 1]) : "r"(addr + 4 * (N - 1)));
 }
 
-// A row's softmax parts (m, l, O; base 2) with its sink: T(O / L), 0 where nothing was seen.
-template <typename T>
-__device__ __forceinline__ uint16_t kv4_finish(float m, float l, float o, float sink) {
-    const float M = fmaxf(m, sink);
-    if (M == -INFINITY) return F16Traits<T>::from_f32(l != l ? l : 0.0f);
-    const float f = kv4_ex2(m - M), L = l * f + kv4_ex2(sink - M);
-    return F16Traits<T>::from_f32(L == 0.0f ? 0.0f : o * f / L);
-}
-
 // CTAs a SM, by registers (8 rows: 128 / 168 / 255 a thread) and shared memory.
 constexpr int kv4_resident(int D, int NT) { return NT == 2 || D == 256 ? 2 : D == 128 ? 3 : 4; }
 
@@ -189,12 +138,7 @@ __global__ void __launch_bounds__(KV4_NW * 32, kv4_resident(D, NT)) kv4_attend_k
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gid = lane >> 2, c = lane & 3;
     const int tid = threadIdx.x, KVH = a.pool.KVH, G = a.G;
 
-    // rows past the last query are 0
-    if (a.q_start) {
-        const long long from = (long long)max(min(a.q_start[a.B], a.N), 0) * a.H * D / 8, to = (long long)a.N * a.H * D / 8;
-        for (long long i = from + (long long)blockIdx.x * blockDim.x + tid; i < to; i += (long long)gridDim.x * blockDim.x)
-            reinterpret_cast<uint4*>(a.out)[i] = make_uint4(0, 0, 0, 0);
-    }
+    kv4_zero_tail(a, D);
 
     // ---- this CTA's share of the steps: requests are scanned 128 at a time ----
     long long total = 0;
@@ -709,7 +653,7 @@ __global__ void __launch_bounds__(KV4_NW * 32, kv4_resident(D, NT)) kv4_attend_k
 
 // One CTA a (request, kv head, row of the request's tiles): the parts of an item that several CTAs share, joined.
 template <typename T, int D, int NT>
-__global__ void __launch_bounds__(128) kv4_join_kernel(const Kv4AttArgs a, int n) {
+__global__ void __launch_bounds__(128) kv4_join_kernel(const Kv4AttArgs a) {
     constexpr int R = 8 * NT;
     __shared__ int red[KV4_NW];
     grid_dep_wait();
@@ -720,28 +664,15 @@ __global__ void __launch_bounds__(128) kv4_join_kernel(const Kv4AttArgs a, int n
         total += kv4_sum(w, red);
         at += kv4_sum(i < b ? w : 0, red);
     }
-    n = int(min((long long)n, total));
+    const int n = int(min((long long)a.ctas, total));
     const Kv4Req rq = kv4_request<R>(a, b);
     if (row >= rq.fresh * a.G) return;
     const long long item = at + ((long long)kvh * rq.tiles + tile) * rq.steps();
     const int c0 = kv4_owner(item, total, n), c1 = kv4_owner(item + rq.steps() - 1, total, n);
     if (c0 == c1) return;  // one CTA had it whole
-    const int j = row - tile * R;
+    const int j = row - tile * R, qi = row / a.G, head = kvh * a.G + row - qi * a.G;
     auto part = [&](int cta) { return ((size_t)cta * 2 + (cta == c0 ? 1 : 0)) * R + j; };
-    float M = -INFINITY;
-    for (int cta = c0; cta <= c1; ++cta) M = fmaxf(M, a.part_ml[2 * part(cta)]);
-    const int qi = row / a.G, head = kvh * a.G + row - qi * a.G;
-    const float sink = kv4_sink(a.sinks, head);
-    for (int d = threadIdx.x; d < D; d += 128) {
-        float L = 0.0f, O = 0.0f;
-        for (int cta = c0; cta <= c1; ++cta) {
-            const size_t p = part(cta);
-            const float f = a.part_ml[2 * p] == -INFINITY ? 0.0f : kv4_ex2(a.part_ml[2 * p] - M);
-            L += a.part_ml[2 * p + 1] * f;
-            if (f != 0.0f) O += a.part_o[p * D + d] * f;
-        }
-        a.out[((size_t)(rq.first + qi) * a.H + head) * D + d] = kv4_finish<T>(M, L, O, sink);
-    }
+    kv4_join_row<T, D>(a, part, c0, c1, kv4_sink(a.sinks, head), a.out + ((size_t)(rq.first + qi) * a.H + head) * D);
 }
 
 // ---- host ----------------------------------------------------------------------------------------
@@ -751,55 +682,54 @@ bool kv4_attend_shape_ok(int N, int B, int max_q, int H, int KVH, int width, int
            (long long)max_q * (H / KVH) < (1 << 30) && width >= 1 && window >= 0;
 }
 
-// Row tiles: 8 rows where every request's fit, else 16 (a key's codes are then unpacked once for 16 rows).
-static int kv4_tile_rows(int max_q, int G) { return (long long)max_q * G <= 8 ? 8 : 16; }
-
-// One wave of CTAs, as many as are resident (by shared memory and registers; see the launch bounds).
-static int kv4_ctas(int D, int R, int sms) { return sms * kv4_resident(D, R / 8); }
-
-size_t kv4_attend_workspace_bytes(int N, int B, int max_q, int H, int KVH, int D) {
-    const int R = kv4_tile_rows(max_q, H / KVH);
-    return size_t(kv4_ctas(D, R, device_info().sm_count)) * 2 * R * (2 + D) * sizeof(float);
+// Rows of kv4_attend's tiles, and the rows up to which a request is its own (above: kv4_prefill). 16 rows where every
+// request fits them (a key is then unpacked once for all); else as many as one query has, 8 or 16, for the requests of
+// a mixed batch that only decode. 0: none.
+static void kv4_rows(int max_q, int G, int* R, int* split) {
+    const long long most = (long long)max_q * G;
+    *R = most <= 8 || (most > 16 && G <= 8) ? 8 : 16;
+    *split = most <= 16 ? int(most) : G <= 16 ? *R : 0;
 }
 
-template <typename K, typename... A>
-static int kv4_launch(K kern, dim3 grid, size_t smem, cudaStream_t st, A... args) {
-    if (smem > 48 * 1024 &&
-        cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem)) != cudaSuccess)
-        return LQ_E_CUDA;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = grid;
-    cfg.blockDim = dim3(KV4_NW * 32);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = st;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, kern, args...) == cudaSuccess ? LQ_OK : LQ_E_CUDA;
+// One wave of CTAs, as many as are resident.
+static int kv4_ctas(int D, int R, int sms) { return sms * kv4_resident(D, R / 8); }
+
+static size_t kv4_few_bytes(int D, int R, int sms) {
+    return (size_t(kv4_ctas(D, R, sms)) * 2 * R * (2 + D) * sizeof(float) + 255) / 256 * 256;
+}
+
+size_t kv4_prefill_workspace_bytes(int D, int sms);
+int kv4_prefill_run(const Kv4AttArgs& a, int D, int dtype, void* workspace, cudaStream_t st);
+
+size_t kv4_attend_workspace_bytes(int N, int B, int max_q, int H, int KVH, int D) {
+    int R, split;
+    kv4_rows(max_q, H / KVH, &R, &split);
+    const int sms = device_info().sm_count;
+    const bool many = (long long)max_q * (H / KVH) > split;
+    return (split ? kv4_few_bytes(D, R, sms) : 0) + (many ? kv4_prefill_workspace_bytes(D, sms) : 0);
 }
 
 template <typename T, int D, int NT>
-static int kv4_attend_n(const Kv4AttArgs& a, cudaStream_t st) {
+static int kv4_attend_n(Kv4AttArgs a, cudaStream_t st) {
     constexpr int R = 8 * NT;
     constexpr size_t merge = size_t(KV4_NW) * R * (2 + D) * sizeof(float);
     constexpr size_t smem = merge > size_t(Kv4Shape<D>::RING) ? merge : size_t(Kv4Shape<D>::RING);
-    const int n = kv4_ctas(D, R, device_info().sm_count);
-    int rc = kv4_launch(kv4_attend_kernel<T, D, NT>, dim3(n), smem, st, a);
+    a.ctas = kv4_ctas(D, R, device_info().sm_count);
+    int rc = kv4_launch(kv4_attend_kernel<T, D, NT>, dim3(a.ctas), dim3(KV4_NW * 32), smem, st, a);
     if (rc) return rc;
-    const int tiles = (a.max_q * a.G + R - 1) / R;
-    return kv4_launch(kv4_join_kernel<T, D, NT>, dim3(tiles * R, a.pool.KVH, a.B), 0, st, a, n);
+    return kv4_launch(kv4_join_kernel<T, D, NT>, dim3(a.split_rows, a.pool.KVH, a.B), dim3(128), 0, st, a);
 }
 
 template <typename T, int D>
-static int kv4_attend_d(const Kv4AttArgs& a, cudaStream_t st) {
-    return kv4_tile_rows(a.max_q, a.G) == 8 ? kv4_attend_n<T, D, 1>(a, st) : kv4_attend_n<T, D, 2>(a, st);
+static int kv4_attend_d(const Kv4AttArgs& a, int R, cudaStream_t st) {
+    return R == 8 ? kv4_attend_n<T, D, 1>(a, st) : kv4_attend_n<T, D, 2>(a, st);
 }
 
 template <typename T>
-static int kv4_attend_t(const Kv4AttArgs& a, int D, cudaStream_t st) {
-    return D == 64 ? kv4_attend_d<T, 64>(a, st) : D == 128 ? kv4_attend_d<T, 128>(a, st) : kv4_attend_d<T, 256>(a, st);
+static int kv4_attend_t(const Kv4AttArgs& a, int D, int R, cudaStream_t st) {
+    return D == 64    ? kv4_attend_d<T, 64>(a, R, st)
+           : D == 128 ? kv4_attend_d<T, 128>(a, R, st)
+                      : kv4_attend_d<T, 256>(a, R, st);
 }
 
 int kv4_attend_run(const Kv4Pool& pool, const void* q, int N, const int32_t* q_start, int max_q, const int32_t* table,
@@ -807,6 +737,7 @@ int kv4_attend_run(const Kv4Pool& pool, const void* q, int N, const int32_t* q_s
                    int dtype, void* workspace, size_t workspace_bytes, void* out, cudaStream_t st) {
     if (N == 0) return LQ_OK;
     if (!workspace || workspace_bytes < kv4_attend_workspace_bytes(N, B, max_q, H, pool.KVH, D)) return LQ_E_ARG;
+    const int sms = device_info().sm_count;
     Kv4AttArgs a = {};
     a.pool = pool;
     a.q = static_cast<const uint16_t*>(q);
@@ -823,10 +754,17 @@ int kv4_attend_run(const Kv4Pool& pool, const void* q, int N, const int32_t* q_s
     a.width = width;
     a.window = window;
     a.max_q = max_q;
-    const int R = kv4_tile_rows(max_q, a.G);
-    a.part_ml = static_cast<float*>(workspace);
-    a.part_o = a.part_ml + size_t(kv4_ctas(D, R, device_info().sm_count)) * 2 * R * 2;
-    return dtype == LQ_BF16 ? kv4_attend_t<__nv_bfloat16>(a, D, st) : kv4_attend_t<__half>(a, D, st);
+    int R;
+    kv4_rows(max_q, a.G, &R, &a.split_rows);
+    uint8_t* ws = static_cast<uint8_t*>(workspace);
+    if ((long long)max_q * a.G > a.split_rows) {
+        const int rc = kv4_prefill_run(a, D, dtype, ws, st);
+        if (rc || !a.split_rows) return rc;
+        ws += kv4_prefill_workspace_bytes(D, sms);
+    }
+    a.part_o = reinterpret_cast<float*>(ws);
+    a.part_ml = a.part_o + size_t(kv4_ctas(D, R, sms)) * 2 * R * D;
+    return dtype == LQ_BF16 ? kv4_attend_t<__nv_bfloat16>(a, D, R, st) : kv4_attend_t<__half>(a, D, R, st);
 }
 
 }  // namespace lq

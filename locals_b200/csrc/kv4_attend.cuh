@@ -1,0 +1,125 @@
+// What the two attention kernels over the paged 4-bit cache share (kv4_attend.cu: few rows a request; kv4_prefill.cu:
+// many): arguments, a request's place in the step, and the joining of parts.
+#pragma once
+
+#include <cuda_runtime.h>
+#include <math.h>
+#include <stdint.h>
+
+#include "kv4.cuh"
+#include "lq_host.h"
+#include "lq_ptx.cuh"
+#include "lq_status.cuh"
+
+namespace lq {
+
+constexpr float KV4_LOG2E = 1.4426950408889634f;
+constexpr uint32_t KV4_NONE = 0xffffffffu;  // no page
+
+struct Kv4AttArgs {
+    Kv4Pool pool;
+    const uint16_t* q;
+    const int32_t* q_start;  // may be null: query b is request b's
+    const int32_t* table;
+    const int32_t* lens;
+    const float* sinks;
+    uint16_t* out;
+    float* part_ml;    // (CTA, 2, rows) x {m, l}, base 2
+    float* part_o;     // (CTA, 2, rows) x D
+    int32_t* records;  // (CTA) x 8: the item that the start of a CTA's share divides
+    float scale_log2;
+    int N, B, H, G, width, window, max_q;
+    int ctas;        // CTAs that the steps are dealt out over (kv4_attend)
+    int split_rows;  // requests of more rows are kv4_prefill's
+};
+
+// A sink's logit in base 2, finite at its upper end so that differences from it stay numbers.
+__device__ __forceinline__ float kv4_sink(const float* sinks, int head) {
+    return sinks ? fminf(sinks[head] * KV4_LOG2E, 3.4028234e38f) : -INFINITY;
+}
+__device__ __forceinline__ float kv4_ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// A request's place in the step: its queries' first row, their number, its keys and the 128-key steps that they span.
+struct Kv4Req {
+    int first, fresh, len, s_lo, s_hi, tiles;
+    __device__ __forceinline__ int steps() const { return s_hi - s_lo; }
+};
+
+// first, fresh and len only.
+__device__ __forceinline__ Kv4Req kv4_new(const Kv4AttArgs& a, int b) {
+    Kv4Req r;
+    r.first = b;
+    r.fresh = b < a.N ? 1 : 0;
+    if (a.q_start) {
+        r.first = max(a.q_start[b], 0);
+        r.fresh = max(min(a.q_start[b + 1], a.N) - r.first, 0);
+        if (r.fresh > a.max_q) {
+            record_status(LQ_DEV_BOUNDS);
+            r.fresh = a.max_q;
+        }
+    }
+    r.len = a.lens[b];
+    return r;
+}
+
+// Rows past the last query are 0 (the CTAs share them).
+__device__ __forceinline__ void kv4_zero_tail(const Kv4AttArgs& a, int D) {
+    if (!a.q_start) return;
+    const long long row = (long long)a.H * D / 8;  // 16-byte pieces a token
+    const long long from = max(min(a.q_start[a.B], a.N), 0) * row, to = a.N * row;
+    for (long long i = from + (long long)blockIdx.x * blockDim.x + threadIdx.x; i < to; i += (long long)gridDim.x * blockDim.x)
+        reinterpret_cast<uint4*>(a.out)[i] = make_uint4(0, 0, 0, 0);
+}
+
+// The CTA that the x-th of S steps falls to: CTA i of n has steps i S / n .. (i + 1) S / n - 1.
+__device__ __forceinline__ int kv4_owner(long long x, long long S, int n) { return int(((x + 1) * n - 1) / S); }
+
+// A row's softmax parts (m, l, O; base 2) with its sink: T(O / L), 0 where nothing was seen.
+template <typename T>
+__device__ __forceinline__ uint16_t kv4_finish(float m, float l, float o, float sink) {
+    const float M = fmaxf(m, sink);
+    if (M == -INFINITY) return F16Traits<T>::from_f32(l != l ? l : 0.0f);
+    const float f = kv4_ex2(m - M), L = l * f + kv4_ex2(sink - M);
+    return F16Traits<T>::from_f32(L == 0.0f ? 0.0f : o * f / L);
+}
+
+// The parts of one row that CTAs c0 .. c1 hold (part(cta): their index), joined in that order by the CTA's 128 threads.
+template <typename T, int D, typename P>
+__device__ __forceinline__ void kv4_join_row(const Kv4AttArgs& a, P part, int c0, int c1, float sink, uint16_t* out) {
+    float M = -INFINITY;
+    for (int cta = c0; cta <= c1; ++cta) M = fmaxf(M, a.part_ml[2 * part(cta)]);
+    for (int d = threadIdx.x; d < D; d += 128) {
+        float L = 0.0f, O = 0.0f;
+        for (int cta = c0; cta <= c1; ++cta) {
+            const size_t p = part(cta);
+            const float f = a.part_ml[2 * p] == -INFINITY ? 0.0f : kv4_ex2(a.part_ml[2 * p] - M);
+            L += a.part_ml[2 * p + 1] * f;
+            if (f != 0.0f) O += a.part_o[p * D + d] * f;
+        }
+        out[d] = kv4_finish<T>(M, L, O, sink);
+    }
+}
+
+template <typename K, typename A>
+static int kv4_launch(K kern, dim3 grid, dim3 block, size_t smem, cudaStream_t st, const A& a) {
+    if (smem > 48 * 1024 &&
+        cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem)) != cudaSuccess)
+        return LQ_E_CUDA;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = block;
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kern, a) == cudaSuccess ? LQ_OK : LQ_E_CUDA;
+}
+
+}  // namespace lq

@@ -1,0 +1,756 @@
+// Attention over a paged 4-bit cache for requests with many rows (queries times query heads a kv head): the same
+// function as kv4_attend.cu, on the 5th-generation tensor cores.
+//
+// A CTA takes a tile of 256 rows of a (request, kv head) (128 at D = 256) and walks its keys in steps of 128 (64 at
+// D = 256). Per step
+//   * four warps unpack the codes of 128 keys and values to fp16 tiles in shared memory, one step ahead through
+//     registers: 16 bytes of codes a lane, (code | 1024) - 1024 and one fused multiply-add with the group's scale and
+//     bias, pairs (i, i + 4) of a word as they come out of one mask. The order of dimensions that this makes is met by
+//     the queries (stored in the same order) and undone when the output is written;
+//   * one thread issues S = Q K^T (both in shared memory, K-major) and O += P V (P in tensor memory, V in shared memory as
+//     it lies, dimensions contiguous: the transposed B operand) as tcgen05.mma with fp32 accumulators in tensor memory:
+//     for two query tiles in turn, S0 PV0 S1 PV1 ..., so that one tile's softmax runs beside the other's products;
+//   * each of 256 threads owns a row: it reads its scores, keeps the running maximum and sum in fp32, and writes its
+//     probabilities back over them as fp16. The row's output is only rescaled when its maximum has grown by 2^8.
+// Roundings: queries to fp16 after a power of two a row (exact for bf16 but for values 2^-26 below the row's largest),
+// keys, values and probabilities to fp16 (2^-12 each, against the 2^-9 of a bf16 output); values after a power of two
+// that follows their size, so that neither small nor large ones leave fp16's range.
+// A masked score is -inf, its probability 0; a value whose scale or bias is not finite is held as 0 and its key as NaN,
+// so that only rows that see it become NaN.
+// Work is dealt out as in kv4_attend.cu: the steps of all tiles (each as far as its last row sees) evenly over one CTA a
+// SM, parts joined by kv4_prefill_join_kernel. Tensor-bound: 4 D operations a row and key; the exponentials (one a row and
+// key, 16 a clock and SM) take as long as the products do at D = 128.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <math.h>
+#include <stdint.h>
+
+#include "kv4_attend.cuh"
+#include "lq_host.h"
+#include "lq_ptx.cuh"
+#include "lq_status.cuh"
+
+namespace lq {
+
+constexpr int PF_SOFT = 8;                       // softmax warps (a row a thread)
+constexpr int PF_UNPACK = 4;                     // unpacking warps
+constexpr int PF_MMA = PF_SOFT + PF_UNPACK;      // the issuing warp
+constexpr int PF_THREADS = (PF_MMA + 1) * 32;
+
+template <int D>
+struct PfShape {
+    static constexpr int GR = D / 64;
+    static constexpr int NQ = D == 256 ? 1 : 2;   // query tiles of 128 rows
+    static constexpr int R = 128 * NQ;
+    static constexpr int KT = D == 256 ? 64 : 128;  // keys a step
+    static constexpr int RB = D / 2;
+    static constexpr int QB = 128 * D * 2;        // bytes of a query tile
+    static constexpr int TB = KT * D * 2;         // bytes of a key (or value) tile
+    static constexpr int SLAB = KT * 128;         // bytes of 64 dimensions of a tile
+    static constexpr int SMEM = NQ * QB + 4 * TB; // + barriers
+    static constexpr int O_COL = 2 * KT;          // tensor memory: two score buffers, then the outputs
+    static_assert(2 * KT + NQ * D <= 512, "tensor memory columns");
+};
+
+// A tile's steps of keys: from the first that its first row sees to the last that its last row sees.
+template <int D>
+__device__ __forceinline__ void pf_steps(const Kv4AttArgs& a, int base, int fresh, int tile, int* lo, int* hi) {
+    using S = PfShape<D>;
+    const int room = int(min((long long)a.width * a.pool.page, 0x7fffffffLL));
+    const int q0 = tile * S::R / a.G, q1 = (min((tile + 1) * S::R, fresh * a.G) - 1) / a.G;
+    const int keys = max(min(base + q1 + 1, room), 0);
+    const int from = a.window ? min(max(base + q0 + 1 - a.window, 0), keys) : 0;
+    *lo = from / S::KT;
+    *hi = max((keys + S::KT - 1) / S::KT, *lo + 1);
+}
+
+template <int D>
+__device__ __forceinline__ int pf_tiles(const Kv4AttArgs& a, int b, int* first, int* fresh, int* base) {
+    const Kv4Req r = kv4_new(a, b);
+    *first = r.first;
+    *fresh = r.fresh;
+    *base = r.len - r.fresh;
+    return r.fresh * a.G > a.split_rows ? (r.fresh * a.G + PfShape<D>::R - 1) / PfShape<D>::R : 0;
+}
+
+// Steps of all of request b's tiles.
+template <int D>
+__device__ __forceinline__ long long pf_weight(const Kv4AttArgs& a, int b) {
+    int first, fresh, base;
+    const int tiles = pf_tiles<D>(a, b, &first, &fresh, &base);
+    long long w = 0;
+    for (int t = 0; t < tiles; ++t) {
+        int lo, hi;
+        pf_steps<D>(a, base, fresh, t, &lo, &hi);
+        w += hi - lo;
+    }
+    return w * a.pool.KVH;
+}
+
+// Sum over the CTA's threads.
+__device__ __forceinline__ long long pf_sum(long long v, long long* red) {
+#pragma unroll
+    for (int d = 16; d; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
+    __syncthreads();
+    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
+    __syncthreads();
+    long long s = 0;
+    for (int w = 0; w < int(blockDim.x >> 5); ++w) s += red[w];
+    return s;
+}
+
+// The CTA's walk over its steps: items (request, tile, kv head) in that order, each with its steps [st0, st1).
+template <int D>
+struct PfWalk {
+    long long x, x1, at;  // steps: next, end, those before request b
+    int b, tile, kvh, lo, hi, st0, st1, first, fresh, base, tiles;
+    long long item_at;
+
+    // The next item; false when the share is done. Every caller walks alike.
+    __device__ bool next(const Kv4AttArgs& a) {
+        if (x >= x1) return false;
+        for (;;) {
+            if (tile < tiles) {
+                const long long end = item_at + hi - lo;
+                if (x < end) break;
+                item_at = end;
+                if (++kvh == a.pool.KVH) {
+                    kvh = 0;
+                    if (++tile < tiles) pf_steps<D>(a, base, fresh, tile, &lo, &hi);
+                }
+            } else {
+                ++b;
+                tiles = pf_tiles<D>(a, b, &first, &fresh, &base);
+                tile = kvh = 0;
+                if (tiles) pf_steps<D>(a, base, fresh, 0, &lo, &hi);
+            }
+        }
+        st0 = int(x - item_at);
+        st1 = int(min((long long)(hi - lo), x1 - item_at));
+        x = item_at + st1;
+        return true;
+    }
+};
+
+__device__ __forceinline__ void pf_tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(
+            taddr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+        : "memory");
+}
+
+// Descriptor of a B operand whose N side is contiguous (128-byte swizzle): 8 keys of 64 dimensions are 1024 bytes, the
+// next 8 keys follow (stride offset), the next 64 dimensions lie a slab away (leading offset).
+__device__ __forceinline__ uint64_t pf_desc_v(uint32_t addr, uint32_t slab) {
+    return uint64_t((addr >> 4) & 0x3FFFu) | (uint64_t(slab >> 4) << 16) | (uint64_t(1024 >> 4) << 32) |
+           (uint64_t(1) << 46) | (uint64_t(2) << 61);
+}
+
+// (v - 1024) * s + b on fp16 pairs: v - 1024 exact, the rest rounded once.
+__device__ __forceinline__ uint32_t pf_affine(uint32_t v, uint32_t s2, uint32_t b2) {
+    const uint32_t magic = 0x64006400u;
+    const __half2 q = __hsub2(*reinterpret_cast<const __half2*>(&v), *reinterpret_cast<const __half2*>(&magic));
+    const __half2 r = __hfma2(q, *reinterpret_cast<const __half2*>(&s2), *reinterpret_cast<const __half2*>(&b2));
+    return *reinterpret_cast<const uint32_t*>(&r);
+}
+
+struct PfBars {
+    uint64_t q_full[2], k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], o_done[2], done;
+    uint32_t tmem;
+    int abort;          // a wait gave up: no one waits any more
+    int v_exp[4];       // power of two of the values of step i & 3
+    uint32_t miss[4];   // its runs of 8 keys without a page
+    float v_max[PF_UNPACK];
+};
+
+// A bounded wait that, once any has given up, none of the CTA's takes again.
+__device__ __forceinline__ void pf_wait(uint64_t* bar, uint32_t parity, volatile int* abort) {
+    if (*abort) return;
+    if (!mbar_wait(bar, parity)) *abort = 1;
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(PF_THREADS, 1) kv4_prefill_kernel(const Kv4AttArgs a) {
+    using S = PfShape<D>;
+    constexpr int GR = S::GR, KT = S::KT, NQ = S::NQ, R = S::R;
+    extern __shared__ __align__(1024) uint8_t pf_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(pf_raw) + 1023) & ~uintptr_t(1023));
+    PfBars& bar = *reinterpret_cast<PfBars*>(smem + S::SMEM);
+    __shared__ long long red[PF_MMA + 1];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+
+    grid_dep_wait();
+    if (a.split_rows == 0) kv4_zero_tail(a, D);  // (else kv4_attend does)
+    // ---- this CTA's share ----
+    long long total = 0;
+    for (int b0 = 0; b0 < a.B; b0 += PF_THREADS) total += pf_sum(b0 + tid < a.B ? pf_weight<D>(a, b0 + tid) : 0, red);
+    const int n = int(min((long long)gridDim.x, total));
+    int32_t* rec = a.records + blockIdx.x * 8;  // what the join kernel does for this CTA's first step
+    if (int(blockIdx.x) >= n) {
+        if (tid == 0) rec[0] = 0;
+        return;
+    }
+    PfWalk<D> walk;
+    walk.x = (long long)blockIdx.x * total / n;
+    walk.x1 = ((long long)blockIdx.x + 1) * total / n;
+    {
+        long long at = 0;
+        int b = 0;
+        for (int b0 = 0;; b0 += PF_THREADS) {
+            const long long w = b0 + tid < a.B ? pf_weight<D>(a, b0 + tid) : 0;
+            const long long sum = pf_sum(w, red);
+            if (at + sum <= walk.x) {
+                at += sum;
+                continue;
+            }
+            long long s = w;  // inclusive sums within the CTA
+#pragma unroll
+            for (int d = 1; d < 32; d <<= 1) {
+                const long long u = __shfl_up_sync(0xffffffffu, s, d);
+                if (lane >= d) s += u;
+            }
+            __syncthreads();
+            if (lane == 31) red[warp] = s;
+            __syncthreads();
+            for (int k = 0; k < warp; ++k) s += red[k];
+            const bool past = at + s > walk.x;
+            b = b0 + int(pf_sum(past ? 0 : 1, red));
+            at += pf_sum(past ? 0 : w, red);
+            break;
+        }
+        walk.b = b;
+        walk.at = at;
+        walk.tiles = pf_tiles<D>(a, b, &walk.first, &walk.fresh, &walk.base);
+        // the tile: the threads sum theirs, in rounds of PF_THREADS tiles
+        int t0 = 0;
+        for (;; t0 += PF_THREADS) {
+            int lo = 0, hi = 0;
+            if (t0 + tid < walk.tiles) pf_steps<D>(a, walk.base, walk.fresh, t0 + tid, &lo, &hi);
+            const long long w = (long long)(hi - lo) * a.pool.KVH;
+            const long long sum = pf_sum(w, red);
+            if (at + sum <= walk.x) {
+                at += sum;
+                continue;
+            }
+            long long s = w;
+#pragma unroll
+            for (int d = 1; d < 32; d <<= 1) {
+                const long long u = __shfl_up_sync(0xffffffffu, s, d);
+                if (lane >= d) s += u;
+            }
+            __syncthreads();
+            if (lane == 31) red[warp] = s;
+            __syncthreads();
+            for (int k = 0; k < warp; ++k) s += red[k];
+            const bool past = at + s > walk.x;
+            walk.tile = t0 + int(pf_sum(past ? 0 : 1, red));
+            at += pf_sum(past ? 0 : w, red);
+            break;
+        }
+        pf_steps<D>(a, walk.base, walk.fresh, walk.tile, &walk.lo, &walk.hi);
+        walk.kvh = int((walk.x - at) / (walk.hi - walk.lo));
+        walk.item_at = at + (long long)walk.kvh * (walk.hi - walk.lo);
+        if (tid == 0) {
+            const long long item = walk.item_at;
+            const int c0 = kv4_owner(item, total, n), c1 = kv4_owner(item + walk.hi - walk.lo - 1, total, n);
+            rec[0] = item < walk.x && c0 == int(blockIdx.x) - 1;  // the first boundary within its item
+            rec[1] = walk.first;
+            rec[2] = walk.tile * R;
+            rec[3] = min(R, walk.fresh * a.G - walk.tile * R);
+            rec[4] = walk.kvh;
+            rec[5] = c1;
+        }
+    }
+
+    if (tid == 0) {
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&bar.q_full[i], 4);
+            mbar_init(&bar.k_full[i], PF_UNPACK);
+            mbar_init(&bar.k_empty[i], 1);
+            mbar_init(&bar.v_full[i], PF_UNPACK);
+            mbar_init(&bar.v_empty[i], 1);
+            mbar_init(&bar.s_full[i], 1);
+            mbar_init(&bar.p_full[i], 4);
+            mbar_init(&bar.o_done[i], 1);
+        }
+        mbar_init(&bar.done, 1);
+        bar.abort = 0;
+        fence_barrier_init();
+    }
+    if (warp == PF_MMA) {
+        tmem_alloc(&bar.tmem, 512);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = bar.tmem;
+    volatile int* abort = &bar.abort;
+    const uint32_t sq = smem_u32(smem), sk = sq + NQ * S::QB, sv = sk + 2 * S::TB;
+    const int room = int(min((long long)a.width * a.pool.page, 0x7fffffffLL));
+
+    if (warp < PF_SOFT) {
+        // ------------------------------ softmax: a row a thread ------------------------------
+        const int w = warp >> 2, wr = (warp & 3) * 32 + lane;  // query tile, row in it
+        const uint32_t lanes = uint32_t((warp & 3) * 32) << 16;
+        int it = 0, used = 0;  // steps of the CTA, and of this query tile
+        while (walk.next(a)) {
+            const int row0 = walk.tile * R, rows = min(R, walk.fresh * a.G - row0);
+            const int steps = walk.st1 - walk.st0;
+            if (w * 128 >= rows || w >= NQ) {  // no rows here
+                it += steps;
+                continue;
+            }
+            const int row = w * 128 + wr;
+            const bool live = row < rows;
+            const int rr = row0 + (live ? row : rows - 1), qi = rr / a.G, head = walk.kvh * a.G + rr - qi * a.G;
+            const int row_hi = min(walk.base + qi + 1, room);
+            const int row_lo = a.window ? max(walk.base + qi + 1 - a.window, 0) : 0;
+            if (walk.base + walk.fresh > room) record_status(LQ_DEV_BOUNDS);
+            // the warp's rows all see [lo_all, hi_all)
+            const int hi_all = __reduce_min_sync(0xffffffffu, row_hi), lo_all = __reduce_max_sync(0xffffffffu, row_lo);
+
+            // the query row, a power of two larger, in the order of the unpacked codes
+            const size_t qo = ((size_t)(walk.first + qi) * a.H + head) * D;
+            float c;
+            {
+                const uint4* src = reinterpret_cast<const uint4*>(a.q + qo);
+                float mx = 0.0f;
+                if (live && a.scale_log2 != 0.0f) {
+#pragma unroll 4
+                    for (int i = 0; i < D / 8; ++i) {
+                        const uint4 v = src[i];
+                        const uint32_t x[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                        for (int k = 0; k < 4; ++k)
+                            mx = fmaxf(mx, fmaxf(fabsf(F16Traits<T>::to_f32(x[k] & 0xffffu)),
+                                                 fabsf(F16Traits<T>::to_f32(x[k] >> 16))));
+                    }
+                }
+                int E = mx > 0.0f ? 12 - (int((__float_as_uint(mx) >> 23) & 0xff) - 127) : 0;
+                E = min(max(E, -100), 100);
+                const float f = live && a.scale_log2 != 0.0f ? copysignf(__uint_as_float(uint32_t(127 + E) << 23), a.scale_log2) : 0.0f;
+                c = a.scale_log2 != 0.0f ? fabsf(a.scale_log2) * __uint_as_float(uint32_t(127 - E) << 23) : 1.0f;
+                const uint32_t dst = sq + w * S::QB + wr * 128;
+#pragma unroll 4
+                for (int i = 0; i < D / 8; ++i) {
+                    const uint4 v = live ? src[i] : make_uint4(0, 0, 0, 0);
+                    const uint32_t x[4] = {v.x, v.y, v.z, v.w};
+                    float q[8];
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        q[2 * k] = F16Traits<T>::to_f32(x[k] & 0xffffu) * f;
+                        q[2 * k + 1] = F16Traits<T>::to_f32(x[k] >> 16) * f;
+                    }
+                    asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(dst + (i >> 3) * 16384 + (((i & 7) ^ (wr & 7)) << 4)),
+                                 "r"(cvt_f16x2(q[4], q[0])), "r"(cvt_f16x2(q[5], q[1])), "r"(cvt_f16x2(q[6], q[2])),
+                                 "r"(cvt_f16x2(q[7], q[3]))
+                                 : "memory");
+                }
+            }
+            fence_proxy_async();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bar.q_full[w]);
+
+            float m = -INFINITY, l = 0.0f;
+            int ve = 0;
+            const uint32_t o_col = tmem + lanes + S::O_COL + w * D;
+            for (int t = 0; t < steps; ++t, ++it, ++used) {
+                const int buf = NQ == 2 ? w : used & 1;
+                const uint32_t par = NQ == 2 ? used & 1 : (used >> 1) & 1;
+                pf_wait(&bar.s_full[buf], par, abort);
+                tc_fence_after();
+                const int key0 = (walk.lo + walk.st0 + t) * KT;
+                const uint32_t miss = *reinterpret_cast<volatile uint32_t*>(&bar.miss[it & 3]);
+                const int ve_t = *reinterpret_cast<volatile int*>(&bar.v_exp[it & 3]);
+                const bool all = key0 >= lo_all && key0 + KT <= hi_all && miss == 0;
+                const uint32_t s_col = tmem + lanes + buf * KT;
+                float mx = -INFINITY;
+#pragma unroll
+                for (int ch = 0; ch < KT / 32; ++ch) {
+                    uint32_t r[32];
+                    tmem_ld_32x32b_x32(s_col + ch * 32, r);
+                    tmem_wait_ld();
+                    if (all) {
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) mx = fmaxf(mx, __uint_as_float(r[i]));
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) {
+                            const int key = key0 + ch * 32 + i;
+                            const bool in = key >= row_lo && key < row_hi && !((miss >> (ch * 4 + i / 8)) & 1);
+                            mx = fmaxf(mx, in ? __uint_as_float(r[i]) : -INFINITY);
+                        }
+                    }
+                }
+                const float mn = fmaxf(m, mx * c);
+                const bool grow = mn > m + 8.0f || (m == -INFINITY && mn > m) || ve_t != ve;
+                if (__any_sync(0xffffffffu, grow)) {
+                    const float corr = t == 0 ? 0.0f : (mn > m ? kv4_ex2(m - mn) : 1.0f) * exp2f(float(ve_t - ve));
+                    l *= mn > m ? kv4_ex2(m - mn) : 1.0f;
+                    m = mn;
+                    ve = ve_t;
+                    if (t > 0) {
+                        pf_wait(&bar.o_done[w], (used - 1) & 1, abort);  // the last product is in
+                        tc_fence_after();
+#pragma unroll 1
+                        for (int ch = 0; ch < D / 32; ++ch) {
+                            uint32_t r[32];
+                            tmem_ld_32x32b_x32(o_col + ch * 32, r);
+                            tmem_wait_ld();
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) r[i] = __float_as_uint(__uint_as_float(r[i]) * corr);
+                            tmem_st_32x32b_x32(o_col + ch * 32, r);
+                        }
+                    }
+                }
+                const float mz = m == -INFINITY ? 0.0f : m;
+                float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int ch = 0; ch < KT / 32; ++ch) {
+                    uint32_t r[32], p[16];
+                    tmem_ld_32x32b_x32(s_col + ch * 32, r);
+                    tmem_wait_ld();
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) {
+                        float s = __uint_as_float(r[i]);
+                        if (!all) {
+                            const int key = key0 + ch * 32 + i;
+                            const bool in = key >= row_lo && key < row_hi && !((miss >> (ch * 4 + i / 8)) & 1);
+                            s = in ? s : -INFINITY;
+                        }
+                        const float e = kv4_ex2(fmaf(s, c, -mz));
+                        sum[i & 3] += e;
+                        r[i] = __float_as_uint(e);
+                    }
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) p[i] = cvt_f16x2(__uint_as_float(r[2 * i + 1]), __uint_as_float(r[2 * i]));
+                    pf_tmem_st16(s_col + ch * 16, p);
+                }
+                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                tmem_wait_st();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&bar.p_full[buf]);
+            }
+            // ---- the row's output ----
+            pf_wait(&bar.o_done[w], (used - 1) & 1, abort);
+            tc_fence_after();
+            const bool whole = walk.st0 == 0 && walk.st1 == walk.hi - walk.lo;
+            const size_t part = ((size_t)blockIdx.x * 2 + (walk.st0 == 0 ? 1 : 0)) * R + row;
+            const float back = exp2f(float(-ve));
+            float f = back;
+            if (whole) {
+                const float sink = kv4_sink(a.sinks, head), M = fmaxf(m, sink);
+                const float L = M == -INFINITY ? l : l * kv4_ex2(m - M) + kv4_ex2(sink - M);
+                f = L == 0.0f ? 0.0f : back * (M == -INFINITY ? 1.0f : kv4_ex2(m - M)) / L;
+            } else if (live) {
+                a.part_ml[2 * part] = m;
+                a.part_ml[2 * part + 1] = l;
+            }
+#pragma unroll 1
+            for (int ch = 0; ch < D / 32; ++ch) {
+                uint32_t r[32];
+                tmem_ld_32x32b_x32(o_col + ch * 32, r);
+                tmem_wait_ld();
+                if (!live) continue;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    float v[8];  // back in order: place 2 j holds dimension j, place 2 j + 1 dimension j + 4
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        v[j] = __uint_as_float(r[8 * k + 2 * j]) * f;
+                        v[j + 4] = __uint_as_float(r[8 * k + 2 * j + 1]) * f;
+                    }
+                    if (whole) {
+                        uint4 o;
+                        o.x = F16Traits<T>::pack2(v[1], v[0]), o.y = F16Traits<T>::pack2(v[3], v[2]);
+                        o.z = F16Traits<T>::pack2(v[5], v[4]), o.w = F16Traits<T>::pack2(v[7], v[6]);
+                        *reinterpret_cast<uint4*>(a.out + qo + ch * 32 + k * 8) = o;
+                    } else {
+                        float4* dst = reinterpret_cast<float4*>(a.part_o + part * D + ch * 32 + k * 8);
+                        dst[0] = make_float4(v[0], v[1], v[2], v[3]);
+                        dst[1] = make_float4(v[4], v[5], v[6], v[7]);
+                    }
+                }
+            }
+            tc_fence_before();
+        }
+    } else if (warp < PF_MMA) {
+        // ------------------------------ codes to fp16 tiles ------------------------------
+        const int uw = warp - PF_SOFT, ut = uw * 32 + lane;
+        constexpr int NP = S::RB / 16, J = KT * NP / 128;  // 16-byte pieces a key, pieces a lane
+        constexpr int RUNS = KT / 8;
+        // this lane's piece j: key and piece (8 lanes are 8 keys: their stores fall on different banks)
+        auto key_of = [&](int j) {
+            const int blk = j * PF_UNPACK + uw;
+            return NP == 2 ? blk * 16 + (lane & 7) + ((lane >> 4) << 3) : NP == 4 ? blk * 8 + (lane & 7) : (blk >> 1) * 8 + (lane & 7);
+        };
+        auto piece_of = [&](int j) {
+            return NP == 2 ? (lane >> 3) & 1 : NP == 4 ? lane >> 3 : (lane >> 3) + 4 * ((j * PF_UNPACK + uw) & 1);
+        };
+        int it = 0;
+        PfWalk<D> w = walk;
+        bool more = w.next(a);
+        int step = 0;
+        uint4 kc[J], vc[J];
+        uint16_t sc[J][4];
+        uint32_t miss = 0;
+        int key_end = 0;
+        bool item_start = true;
+        // looks the pages of the step up and issues its loads
+        auto fetch = [&]() {
+            const int row0 = w.tile * R, rows = min(R, w.fresh * a.G - row0);
+            key_end = min(w.base + (row0 + rows - 1) / a.G + 1, room);
+            const int key0 = (w.lo + w.st0 + step) * KT;
+            uint32_t mine = KV4_NONE;
+            const int key = key0 + (lane % RUNS) * 8;
+            if (key < key_end) {
+                const int pg = key / a.pool.page, id = a.table[(size_t)w.b * a.width + pg];
+                if (unsigned(id) >= unsigned(a.pool.pages))
+                    record_status(LQ_DEV_BOUNDS);
+                else
+                    mine = kv4_row(a.pool, id, w.kvh, key - pg * a.pool.page);
+            }
+            miss = __ballot_sync(0xffffffffu, lane < RUNS && mine == KV4_NONE && key < key_end);
+#pragma unroll
+            for (int j = 0; j < J; ++j) {
+                const int k = key_of(j), p = piece_of(j);
+                const uint32_t run = __shfl_sync(0xffffffffu, mine, k / 8);
+                const bool ok = run != KV4_NONE && key0 + k < key_end;
+                const size_t row = ok ? run + (k & 7) : 0;
+                kc[j] = vc[j] = make_uint4(0, 0, 0, 0);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) sc[j][i] = 0;
+                if (ok) {
+                    kc[j] = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint8_t*>(a.pool.kq) + row * S::RB + p * 16);
+                    vc[j] = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint8_t*>(a.pool.vq) + row * S::RB + p * 16);
+                    const size_t g = row * GR + p / 2;
+                    sc[j][0] = a.pool.ks[g], sc[j][1] = a.pool.kb[g], sc[j][2] = a.pool.vs[g], sc[j][3] = a.pool.vb[g];
+                }
+            }
+        };
+        // 32 codes with one scale and bias -> 64 bytes of a tile row, 16 bytes at a time
+        auto unpack = [&](const uint4& codes, float s, float b, uint32_t tile, int key, int p) {
+            const uint32_t s1 = cvt_f16x2(s, s), s16 = cvt_f16x2(s * 0.0625f, s * 0.0625f), b2 = cvt_f16x2(b, b);
+            const uint32_t cw[4] = {codes.x, codes.y, codes.z, codes.w};
+            const uint32_t row = tile + (p >> 1) * S::SLAB + key * 128;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const uint32_t x = cw[i], y = cw[i] >> 8;
+                const uint32_t o0 = pf_affine(lop3_and_or(x, 0x000f000fu, 0x64006400u), s1, b2);
+                const uint32_t o1 = pf_affine(lop3_and_or(x, 0x00f000f0u, 0x64006400u), s16, b2);
+                const uint32_t o2 = pf_affine(lop3_and_or(y, 0x000f000fu, 0x64006400u), s1, b2);
+                const uint32_t o3 = pf_affine(lop3_and_or(y, 0x00f000f0u, 0x64006400u), s16, b2);
+                asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(row + ((((p & 1) * 4 + i) ^ (key & 7)) << 4)), "r"(o0),
+                             "r"(o1), "r"(o2), "r"(o3)
+                             : "memory");
+            }
+        };
+        float limit = 0.0f;
+        int ve = 0;
+        if (more) fetch();
+        while (more) {
+            const int st = it & 1;
+            const uint32_t par = ((it >> 1) & 1) ^ 1;
+            if (item_start) limit = 0.0f, ve = 0, item_start = false;
+            // the values' power of two: the largest |value| a group can hold at 2^10 .. 2^15
+            float top = 0.0f, ksf[J], kbf[J], vsf[J], vbf[J];
+#pragma unroll
+            for (int j = 0; j < J; ++j) {
+                ksf[j] = F16Traits<T>::to_f32(sc[j][0]), kbf[j] = F16Traits<T>::to_f32(sc[j][1]);
+                vsf[j] = F16Traits<T>::to_f32(sc[j][2]), vbf[j] = F16Traits<T>::to_f32(sc[j][3]);
+                const float most = fmaf(15.0f, fabsf(vsf[j]), fabsf(vbf[j]));
+                if (!(most < INFINITY)) {
+                    vsf[j] = vbf[j] = 0.0f;
+                    ksf[j] = kbf[j] = __int_as_float(0x7fffffff);
+                } else {
+                    top = fmaxf(top, most);
+                }
+            }
+            int over;
+            asm volatile(
+                "{\n\t.reg .pred p, q;\n\t"
+                "setp.gt.f32 p, %1, %2;\n\t"
+                "barrier.cta.red.or.pred q, 1, 128, p;\n\t"
+                "selp.s32 %0, 1, 0, q;\n\t}"
+                : "=r"(over)
+                : "f"(top), "f"(limit)
+                : "memory");
+            if (over) {
+                const float wm = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top)));
+                if (lane == 0) bar.v_max[uw] = wm;
+                named_barrier(1, 128);
+                float M = 0.0f;
+#pragma unroll
+                for (int i = 0; i < PF_UNPACK; ++i) M = fmaxf(M, reinterpret_cast<volatile float*>(bar.v_max)[i]);
+                ve = min(10 - (int(__float_as_uint(M) >> 23) - 127), 100);  // M below 2^128: at least -117
+                limit = exp2f(float(15 - ve));
+                named_barrier(1, 128);
+            }
+            const float vf = exp2f(float(ve));
+            if (ut == 0) {
+                bar.v_exp[it & 3] = ve;
+                bar.miss[it & 3] = miss;
+            }
+            pf_wait(&bar.k_empty[st], par, abort);
+#pragma unroll
+            for (int j = 0; j < J; ++j) unpack(kc[j], ksf[j], kbf[j], sk + st * S::TB, key_of(j), piece_of(j));
+            fence_proxy_async();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bar.k_full[st]);
+            pf_wait(&bar.v_empty[st], par, abort);
+#pragma unroll
+            for (int j = 0; j < J; ++j) unpack(vc[j], vsf[j] * vf, vbf[j] * vf, sv + st * S::TB, key_of(j), piece_of(j));
+            fence_proxy_async();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bar.v_full[st]);
+            ++it;
+            if (++step == w.st1 - w.st0) {
+                step = 0;
+                item_start = true;
+                more = w.next(a);
+            }
+            if (more) fetch();
+        }
+    } else {
+        // ------------------------------ MMA issuer ------------------------------
+        constexpr uint32_t id_s = umma_idesc_f16(0, 128, KT);
+        constexpr uint32_t id_o = umma_idesc_f16(0, 128, D) | (1u << 16);  // B's N side contiguous
+        int it = 0, used[2] = {0, 0}, items[2] = {0, 0};
+        auto scores = [&](int w, int buf, int st) {
+            if (lane == 0) {
+#pragma unroll
+                for (int k = 0; k < D / 16; ++k) {
+                    const uint32_t qa = sq + w * S::QB + (k >> 2) * 16384 + (k & 3) * 32;
+                    const uint32_t ka = sk + st * S::TB + (k >> 2) * S::SLAB + (k & 3) * 32;
+                    tc_mma_f16(tmem + buf * KT, umma_desc_sw128(qa), umma_desc_sw128(ka), id_s, k > 0);
+                }
+                tc_commit(&bar.s_full[buf]);
+            }
+            __syncwarp();
+        };
+        auto products = [&](int w, int buf, int st, bool first) {
+            if (lane == 0) {
+#pragma unroll
+                for (int k = 0; k < KT / 16; ++k)
+                    tc_mma_ts(tmem + S::O_COL + w * D, tmem + buf * KT + k * 8, pf_desc_v(sv + st * S::TB + k * 2048, S::SLAB),
+                              id_o, (first && k == 0) ? 0u : 1u);
+                tc_commit(&bar.o_done[w]);
+            }
+            __syncwarp();
+        };
+        auto commit = [&](uint64_t* b) {
+            if (lane == 0) tc_commit(b);
+            __syncwarp();
+        };
+        while (walk.next(a)) {
+            const int rows = min(R, walk.fresh * a.G - walk.tile * R), nq = rows > 128 ? 2 : 1;
+            const int steps = walk.st1 - walk.st0;
+            for (int w = 0; w < nq; ++w) pf_wait(&bar.q_full[w], items[w]++ & 1, abort);
+            if constexpr (NQ == 2) {
+                pf_wait(&bar.k_full[it & 1], (it >> 1) & 1, abort);
+                tc_fence_after();
+                for (int w = 0; w < nq; ++w) scores(w, w, it & 1);
+                commit(&bar.k_empty[it & 1]);
+                for (int t = 0; t < steps; ++t, ++it) {
+                    const int st = it & 1, nx = (it + 1) & 1;
+                    pf_wait(&bar.v_full[st], (it >> 1) & 1, abort);
+                    for (int w = 0; w < nq; ++w) {
+                        pf_wait(&bar.p_full[w], used[w]++ & 1, abort);
+                        tc_fence_after();
+                        products(w, w, st, t == 0);
+                        if (t + 1 < steps) {
+                            if (w == 0) {
+                                pf_wait(&bar.k_full[nx], ((it + 1) >> 1) & 1, abort);
+                                tc_fence_after();
+                            }
+                            scores(w, w, nx);
+                        }
+                    }
+                    commit(&bar.v_empty[st]);
+                    if (t + 1 < steps) commit(&bar.k_empty[nx]);
+                }
+            } else {
+                for (int t = 0; t <= steps; ++t) {
+                    if (t < steps) {
+                        const int i = it + t;
+                        pf_wait(&bar.k_full[i & 1], (i >> 1) & 1, abort);
+                        tc_fence_after();
+                        scores(0, (used[0] + t) & 1, i & 1);
+                        commit(&bar.k_empty[i & 1]);
+                    }
+                    if (t > 0) {
+                        const int i = it + t - 1, u = used[0] + t - 1;
+                        pf_wait(&bar.v_full[i & 1], (i >> 1) & 1, abort);
+                        pf_wait(&bar.p_full[u & 1], (u >> 1) & 1, abort);
+                        tc_fence_after();
+                        products(0, u & 1, i & 1, t == 1);
+                        commit(&bar.v_empty[i & 1]);
+                    }
+                }
+                it += steps;
+                used[0] += steps;
+            }
+        }
+        grid_dep_launch();
+        commit(&bar.done);  // nothing of this CTA's is in flight when its tensor memory goes (after an error too)
+        mbar_wait(&bar.done, 0);
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == PF_MMA) {
+        tc_fence_after();
+        tmem_dealloc(tmem, 512);
+    }
+}
+
+// One CTA a (share, 8 rows): the parts of the item that a share's start divides, joined with the rows' sinks.
+template <typename T, int D>
+__global__ void __launch_bounds__(128) kv4_prefill_join_kernel(const Kv4AttArgs a) {
+    constexpr int R = PfShape<D>::R;
+    grid_dep_wait();
+    const int i = blockIdx.x;
+    const int32_t* rec = a.records + i * 8;
+    if (!rec[0]) return;
+    const int first = rec[1], row0 = rec[2], rows = rec[3], kvh = rec[4], c0 = i - 1, c1 = rec[5];
+    for (int j = blockIdx.y * 8; j < min(rows, int(blockIdx.y) * 8 + 8); ++j) {
+        const int qi = (row0 + j) / a.G, head = kvh * a.G + row0 + j - qi * a.G;
+        auto part = [&](int cta) { return ((size_t)cta * 2 + (cta == c0 ? 1 : 0)) * R + j; };
+        kv4_join_row<T, D>(a, part, c0, c1, kv4_sink(a.sinks, head), a.out + ((size_t)(first + qi) * a.H + head) * D);
+    }
+}
+
+// ---- host ----------------------------------------------------------------------------------------
+
+size_t kv4_prefill_workspace_bytes(int D, int sms) {
+    const int R = D == 256 ? 128 : 256;
+    return size_t(sms) * 2 * R * (2 + D) * sizeof(float) + size_t(sms) * 8 * sizeof(int32_t);
+}
+
+template <typename T, int D>
+static int kv4_prefill_d(Kv4AttArgs a, void* workspace, cudaStream_t st) {
+    using S = PfShape<D>;
+    const int n = device_info().sm_count;
+    a.part_o = static_cast<float*>(workspace);
+    a.part_ml = a.part_o + size_t(n) * 2 * S::R * D;
+    a.records = reinterpret_cast<int32_t*>(a.part_ml + size_t(n) * 2 * S::R * 2);
+    int rc = kv4_launch(kv4_prefill_kernel<T, D>, dim3(n), dim3(PF_THREADS), S::SMEM + 1024 + sizeof(PfBars), st, a);
+    if (rc) return rc;
+    return kv4_launch(kv4_prefill_join_kernel<T, D>, dim3(n, S::R / 8), dim3(128), 0, st, a);
+}
+
+int kv4_prefill_run(const Kv4AttArgs& a, int D, int dtype, void* workspace, cudaStream_t st) {
+    if (dtype == LQ_BF16)
+        return D == 64    ? kv4_prefill_d<__nv_bfloat16, 64>(a, workspace, st)
+               : D == 128 ? kv4_prefill_d<__nv_bfloat16, 128>(a, workspace, st)
+                          : kv4_prefill_d<__nv_bfloat16, 256>(a, workspace, st);
+    return D == 64    ? kv4_prefill_d<__half, 64>(a, workspace, st)
+           : D == 128 ? kv4_prefill_d<__half, 128>(a, workspace, st)
+                      : kv4_prefill_d<__half, 256>(a, workspace, st);
+}
+
+}  // namespace lq
