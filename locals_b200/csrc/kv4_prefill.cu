@@ -3,7 +3,7 @@
 //
 // A CTA takes a tile of 256 rows of a (request, kv head) (128 at D = 256) and walks its keys in steps of 128 (64 at
 // D = 256). Per step
-//   * four warps unpack the codes of 128 keys and values to fp16 tiles in shared memory, one step ahead through
+//   * eight warps unpack the codes of 128 keys and values to fp16 tiles in shared memory, one step ahead through
 //     registers: 16 bytes of codes a lane, (code | 1024) - 1024 and one fused multiply-add with the group's scale and
 //     bias, pairs (i, i + 4) of a word as they come out of one mask. The order of dimensions that this makes is met by
 //     the queries (stored in the same order) and undone when the output is written;
@@ -26,6 +26,8 @@
 #include <math.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "kv4_attend.cuh"
 #include "lq_host.h"
 #include "lq_ptx.cuh"
@@ -34,7 +36,7 @@
 namespace lq {
 
 constexpr int PF_SOFT = 8;                       // softmax warps (a row a thread)
-constexpr int PF_UNPACK = 4;                     // unpacking warps
+constexpr int PF_UNPACK = 8;                     // unpacking warps
 constexpr int PF_MMA = PF_SOFT + PF_UNPACK;      // the issuing warp
 constexpr int PF_THREADS = (PF_MMA + 1) * 32;
 
@@ -133,13 +135,10 @@ struct PfWalk {
     }
 };
 
-__device__ __forceinline__ void pf_tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
-    asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(
-            taddr),
-        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
-        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
-        : "memory");
+__device__ __forceinline__ void pf_tmem_st8(uint32_t taddr, const uint32_t (&r)[8]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr), "r"(r[0]), "r"(r[1]),
+                 "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+                 : "memory");
 }
 
 // Descriptor of a B operand whose N side is contiguous (128-byte swizzle): 8 keys of 64 dimensions are 1024 bytes, the
@@ -368,23 +367,28 @@ __global__ void __launch_bounds__(PF_THREADS, 1) kv4_prefill_kernel(const Kv4Att
                 const int ve_t = *reinterpret_cast<volatile int*>(&bar.v_exp[it & 3]);
                 const bool all = key0 >= lo_all && key0 + KT <= hi_all && miss == 0;
                 const uint32_t s_col = tmem + lanes + buf * KT;
+                // whether this row sees place i of the step
+                auto in = [&](int i) {
+                    const int key = key0 + i;
+                    return key >= row_lo && key < row_hi && !((miss >> (i / 8)) & 1);
+                };
                 float mx = -INFINITY;
 #pragma unroll
-                for (int ch = 0; ch < KT / 32; ++ch) {
-                    uint32_t r[32];
-                    tmem_ld_32x32b_x32(s_col + ch * 32, r);
+                for (int ch = 0; ch < KT / 64; ++ch) {
+                    uint32_t r[2][32];
+                    tmem_ld_32x32b_x32(s_col + ch * 64, r[0]);
+                    tmem_ld_32x32b_x32(s_col + ch * 64 + 32, r[1]);
                     tmem_wait_ld();
+                    float part[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
                     if (all) {
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) mx = fmaxf(mx, __uint_as_float(r[i]));
+                        for (int i = 0; i < 64; ++i) part[i & 3] = fmaxf(part[i & 3], __uint_as_float(r[i >> 5][i & 31]));
                     } else {
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) {
-                            const int key = key0 + ch * 32 + i;
-                            const bool in = key >= row_lo && key < row_hi && !((miss >> (ch * 4 + i / 8)) & 1);
-                            mx = fmaxf(mx, in ? __uint_as_float(r[i]) : -INFINITY);
-                        }
+                        for (int i = 0; i < 64; ++i)
+                            part[i & 3] = fmaxf(part[i & 3], in(ch * 64 + i) ? __uint_as_float(r[i >> 5][i & 31]) : -INFINITY);
                     }
+                    mx = fmaxf(mx, fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3])));
                 }
                 const float mn = fmaxf(m, mx * c);
                 const bool grow = mn > m + 8.0f || (m == -INFINITY && mn > m) || ve_t != ve;
@@ -409,27 +413,34 @@ __global__ void __launch_bounds__(PF_THREADS, 1) kv4_prefill_kernel(const Kv4Att
                 }
                 const float mz = m == -INFINITY ? 0.0f : m;
                 float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                auto exps = [&](auto masked) {
+                    uint32_t r[2][16];
+                    tmem_ld_32x32b_x16(s_col, r[0]);
 #pragma unroll
-                for (int ch = 0; ch < KT / 32; ++ch) {
-                    uint32_t r[32], p[16];
-                    tmem_ld_32x32b_x32(s_col + ch * 32, r);
-                    tmem_wait_ld();
+                    for (int ch = 0; ch < KT / 16; ++ch) {  // the next 16 scores are read while these are worked on
+                        uint32_t(&x)[16] = r[ch & 1];
+                        tmem_wait_ld();
+                        if (ch + 1 < KT / 16) tmem_ld_32x32b_x16(s_col + ch * 16 + 16, r[(ch + 1) & 1]);
+                        uint32_t p[8];
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) {
-                        float s = __uint_as_float(r[i]);
-                        if (!all) {
-                            const int key = key0 + ch * 32 + i;
-                            const bool in = key >= row_lo && key < row_hi && !((miss >> (ch * 4 + i / 8)) & 1);
-                            s = in ? s : -INFINITY;
+                        for (int i = 0; i < 16; i += 2) {
+                            float s0 = __uint_as_float(x[i]), s1 = __uint_as_float(x[i + 1]);
+                            if constexpr (decltype(masked)::value) {
+                                s0 = in(ch * 16 + i) ? s0 : -INFINITY;
+                                s1 = in(ch * 16 + i + 1) ? s1 : -INFINITY;
+                            }
+                            const float e0 = kv4_ex2(fmaf(s0, c, -mz)), e1 = kv4_ex2(fmaf(s1, c, -mz));
+                            sum[i & 2] += e0;
+                            sum[(i & 2) + 1] += e1;
+                            p[i / 2] = cvt_f16x2(e1, e0);
                         }
-                        const float e = kv4_ex2(fmaf(s, c, -mz));
-                        sum[i & 3] += e;
-                        r[i] = __float_as_uint(e);
+                        pf_tmem_st8(s_col + ch * 8, p);
                     }
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) p[i] = cvt_f16x2(__uint_as_float(r[2 * i + 1]), __uint_as_float(r[2 * i]));
-                    pf_tmem_st16(s_col + ch * 16, p);
-                }
+                };
+                if (all)
+                    exps(std::false_type());
+                else
+                    exps(std::true_type());
                 l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
                 tmem_wait_st();
                 tc_fence_before();
@@ -481,8 +492,8 @@ __global__ void __launch_bounds__(PF_THREADS, 1) kv4_prefill_kernel(const Kv4Att
         }
     } else if (warp < PF_MMA) {
         // ------------------------------ codes to fp16 tiles ------------------------------
-        const int uw = warp - PF_SOFT, ut = uw * 32 + lane;
-        constexpr int NP = S::RB / 16, J = KT * NP / 128;  // 16-byte pieces a key, pieces a lane
+        const int uw = warp - PF_SOFT;
+        constexpr int NP = S::RB / 16, J = KT * NP / (PF_UNPACK * 32);  // 16-byte pieces a key, pieces a lane
         constexpr int RUNS = KT / 8;
         // this lane's piece j: key and piece (8 lanes are 8 keys: their stores fall on different banks)
         auto key_of = [&](int j) {
@@ -492,44 +503,56 @@ __global__ void __launch_bounds__(PF_THREADS, 1) kv4_prefill_kernel(const Kv4Att
         auto piece_of = [&](int j) {
             return NP == 2 ? (lane >> 3) & 1 : NP == 4 ? lane >> 3 : (lane >> 3) + 4 * ((j * PF_UNPACK + uw) & 1);
         };
-        int it = 0;
+        // A step's codes, scales and biases in registers, and what is to be known of it.
+        struct Held {
+            uint4 k[J], v[J];
+            uint32_t ks[J], vs[J];  // scale low, bias high
+            uint32_t miss;
+            bool item_start;
+        };
         PfWalk<D> w = walk;
         bool more = w.next(a);
         int step = 0;
-        uint4 kc[J], vc[J];
-        uint16_t sc[J][4];
-        uint32_t miss = 0;
-        int key_end = 0;
-        bool item_start = true;
-        // looks the pages of the step up and issues its loads
-        auto fetch = [&]() {
+        // the runs of the walk's step (lane l: run l), KV4_NONE without a page or beyond the tile's keys; moves on
+        struct Runs {
+            uint32_t row, miss;
+            int left;  // keys from the step's first to the tile's end
+            bool item_start;
+        };
+        auto lookup = [&]() -> Runs {
             const int row0 = w.tile * R, rows = min(R, w.fresh * a.G - row0);
-            key_end = min(w.base + (row0 + rows - 1) / a.G + 1, room);
-            const int key0 = (w.lo + w.st0 + step) * KT;
-            uint32_t mine = KV4_NONE;
-            const int key = key0 + (lane % RUNS) * 8;
+            const int key_end = min(w.base + (row0 + rows - 1) / a.G + 1, room);
+            const int key0 = (w.lo + w.st0 + step) * KT, key = key0 + (lane % RUNS) * 8;
+            Runs r = {KV4_NONE, 0, key_end - key0, step == 0};
             if (key < key_end) {
                 const int pg = key / a.pool.page, id = a.table[(size_t)w.b * a.width + pg];
                 if (unsigned(id) >= unsigned(a.pool.pages))
                     record_status(LQ_DEV_BOUNDS);
                 else
-                    mine = kv4_row(a.pool, id, w.kvh, key - pg * a.pool.page);
+                    r.row = kv4_row(a.pool, id, w.kvh, key - pg * a.pool.page);
             }
-            miss = __ballot_sync(0xffffffffu, lane < RUNS && mine == KV4_NONE && key < key_end);
+            r.miss = __ballot_sync(0xffffffffu, lane < RUNS && r.row == KV4_NONE && key < key_end);
+            if (++step == w.st1 - w.st0) {
+                step = 0;
+                more = w.next(a);
+            }
+            return r;
+        };
+        auto fetch = [&](const Runs& r, Held& h) {
+            h.miss = r.miss;
+            h.item_start = r.item_start;
 #pragma unroll
             for (int j = 0; j < J; ++j) {
                 const int k = key_of(j), p = piece_of(j);
-                const uint32_t run = __shfl_sync(0xffffffffu, mine, k / 8);
-                const bool ok = run != KV4_NONE && key0 + k < key_end;
-                const size_t row = ok ? run + (k & 7) : 0;
-                kc[j] = vc[j] = make_uint4(0, 0, 0, 0);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) sc[j][i] = 0;
-                if (ok) {
-                    kc[j] = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint8_t*>(a.pool.kq) + row * S::RB + p * 16);
-                    vc[j] = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint8_t*>(a.pool.vq) + row * S::RB + p * 16);
-                    const size_t g = row * GR + p / 2;
-                    sc[j][0] = a.pool.ks[g], sc[j][1] = a.pool.kb[g], sc[j][2] = a.pool.vs[g], sc[j][3] = a.pool.vb[g];
+                const uint32_t run = __shfl_sync(0xffffffffu, r.row, k / 8);
+                h.k[j] = h.v[j] = make_uint4(0, 0, 0, 0);
+                h.ks[j] = h.vs[j] = 0;
+                if (run != KV4_NONE && k < r.left) {
+                    const size_t row = run + (k & 7), g = row * GR + p / 2;
+                    h.k[j] = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint8_t*>(a.pool.kq) + row * S::RB + p * 16);
+                    h.v[j] = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint8_t*>(a.pool.vq) + row * S::RB + p * 16);
+                    h.ks[j] = a.pool.ks[g] | uint32_t(a.pool.kb[g]) << 16;
+                    h.vs[j] = a.pool.vs[g] | uint32_t(a.pool.vb[g]) << 16;
                 }
             }
         };
@@ -552,21 +575,21 @@ __global__ void __launch_bounds__(PF_THREADS, 1) kv4_prefill_kernel(const Kv4Att
         };
         float limit = 0.0f;
         int ve = 0;
-        if (more) fetch();
-        while (more) {
+        // one step from its registers to the tiles
+        auto step_out = [&](const Held& h, int it) {
             const int st = it & 1;
             const uint32_t par = ((it >> 1) & 1) ^ 1;
-            if (item_start) limit = 0.0f, ve = 0, item_start = false;
+            if (h.item_start) limit = 0.0f, ve = 0;
             // the values' power of two: the largest |value| a group can hold at 2^10 .. 2^15
-            float top = 0.0f, ksf[J], kbf[J], vsf[J], vbf[J];
+            float top = 0.0f, ks[J], kb[J], vs[J], vb[J];
 #pragma unroll
             for (int j = 0; j < J; ++j) {
-                ksf[j] = F16Traits<T>::to_f32(sc[j][0]), kbf[j] = F16Traits<T>::to_f32(sc[j][1]);
-                vsf[j] = F16Traits<T>::to_f32(sc[j][2]), vbf[j] = F16Traits<T>::to_f32(sc[j][3]);
-                const float most = fmaf(15.0f, fabsf(vsf[j]), fabsf(vbf[j]));
+                ks[j] = F16Traits<T>::to_f32(h.ks[j] & 0xffffu), kb[j] = F16Traits<T>::to_f32(h.ks[j] >> 16);
+                vs[j] = F16Traits<T>::to_f32(h.vs[j] & 0xffffu), vb[j] = F16Traits<T>::to_f32(h.vs[j] >> 16);
+                const float most = fmaf(15.0f, fabsf(vs[j]), fabsf(vb[j]));
                 if (!(most < INFINITY)) {
-                    vsf[j] = vbf[j] = 0.0f;
-                    ksf[j] = kbf[j] = __int_as_float(0x7fffffff);
+                    vs[j] = vb[j] = 0.0f;
+                    ks[j] = kb[j] = __int_as_float(0x7fffffff);
                 } else {
                     top = fmaxf(top, most);
                 }
@@ -575,46 +598,60 @@ __global__ void __launch_bounds__(PF_THREADS, 1) kv4_prefill_kernel(const Kv4Att
             asm volatile(
                 "{\n\t.reg .pred p, q;\n\t"
                 "setp.gt.f32 p, %1, %2;\n\t"
-                "barrier.cta.red.or.pred q, 1, 128, p;\n\t"
+                "barrier.cta.red.or.pred q, 1, %3, p;\n\t"
                 "selp.s32 %0, 1, 0, q;\n\t}"
                 : "=r"(over)
-                : "f"(top), "f"(limit)
+                : "f"(top), "f"(limit), "n"(PF_UNPACK * 32)
                 : "memory");
             if (over) {
                 const float wm = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top)));
                 if (lane == 0) bar.v_max[uw] = wm;
-                named_barrier(1, 128);
+                named_barrier(1, PF_UNPACK * 32);
                 float M = 0.0f;
 #pragma unroll
                 for (int i = 0; i < PF_UNPACK; ++i) M = fmaxf(M, reinterpret_cast<volatile float*>(bar.v_max)[i]);
                 ve = min(10 - (int(__float_as_uint(M) >> 23) - 127), 100);  // M below 2^128: at least -117
                 limit = exp2f(float(15 - ve));
-                named_barrier(1, 128);
+                named_barrier(1, PF_UNPACK * 32);
             }
             const float vf = exp2f(float(ve));
-            if (ut == 0) {
+            if (uw == 0 && lane == 0) {
                 bar.v_exp[it & 3] = ve;
-                bar.miss[it & 3] = miss;
+                bar.miss[it & 3] = h.miss;
             }
             pf_wait(&bar.k_empty[st], par, abort);
 #pragma unroll
-            for (int j = 0; j < J; ++j) unpack(kc[j], ksf[j], kbf[j], sk + st * S::TB, key_of(j), piece_of(j));
+            for (int j = 0; j < J; ++j) unpack(h.k[j], ks[j], kb[j], sk + st * S::TB, key_of(j), piece_of(j));
             fence_proxy_async();
             __syncwarp();
             if (lane == 0) mbar_arrive(&bar.k_full[st]);
             pf_wait(&bar.v_empty[st], par, abort);
 #pragma unroll
-            for (int j = 0; j < J; ++j) unpack(vc[j], vsf[j] * vf, vbf[j] * vf, sv + st * S::TB, key_of(j), piece_of(j));
+            for (int j = 0; j < J; ++j) unpack(h.v[j], vs[j] * vf, vb[j] * vf, sv + st * S::TB, key_of(j), piece_of(j));
             fence_proxy_async();
             __syncwarp();
             if (lane == 0) mbar_arrive(&bar.v_full[st]);
-            ++it;
-            if (++step == w.st1 - w.st0) {
-                step = 0;
-                item_start = true;
-                more = w.next(a);
+        };
+        // pages two steps ahead, codes one step ahead
+        Held h0, h1;
+        Runs ahead;
+        int held = 0, known = 0;  // steps in registers, looked up
+        if (more) ahead = lookup(), known = 1;
+        if (known) {
+            fetch(ahead, h0);
+            held = 1, known = 0;
+            if (more) ahead = lookup(), known = 1;
+        }
+        for (int it = 0; held; ++it) {
+            Held& now = h0;
+            held = 0;
+            if (known) {
+                fetch(ahead, h1);
+                held = 1, known = 0;
+                if (more) ahead = lookup(), known = 1;
             }
-            if (more) fetch();
+            step_out(now, it);
+            h0 = h1;
         }
     } else {
         // ------------------------------ MMA issuer ------------------------------
