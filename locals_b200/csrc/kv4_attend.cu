@@ -715,9 +715,10 @@ static int kv4_attend_n(Kv4AttArgs a, cudaStream_t st) {
     constexpr size_t merge = size_t(KV4_NW) * R * (2 + D) * sizeof(float);
     constexpr size_t smem = merge > size_t(Kv4Shape<D>::RING) ? merge : size_t(Kv4Shape<D>::RING);
     a.ctas = kv4_ctas(D, R, device_info().sm_count);
-    int rc = kv4_launch(kv4_attend_kernel<T, D, NT>, dim3(a.ctas), dim3(KV4_NW * 32), smem, st, a);
+    static std::atomic<uint32_t> set{0}, none{0};
+    int rc = kv4_launch(kv4_attend_kernel<T, D, NT>, set, dim3(a.ctas), dim3(KV4_NW * 32), smem, st, a);
     if (rc) return rc;
-    return kv4_launch(kv4_join_kernel<T, D, NT>, dim3(a.split_rows, a.pool.KVH, a.B), dim3(128), 0, st, a);
+    return kv4_launch(kv4_join_kernel<T, D, NT>, none, dim3(a.split_rows, a.pool.KVH, a.B), dim3(128), 0, st, a);
 }
 
 template <typename T, int D>

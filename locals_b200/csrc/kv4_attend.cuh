@@ -6,6 +6,8 @@
 #include <math.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #include "kv4.cuh"
 #include "lq_host.h"
 #include "lq_ptx.cuh"
@@ -104,11 +106,18 @@ __device__ __forceinline__ void kv4_join_row(const Kv4AttArgs& a, P part, int c0
     }
 }
 
+// The shared-memory limit is an attribute of the function on a device: set at the kernel's first launch on each (`set`
+// has a bit a device), not at every launch, where it costs about as much as a small launch itself.
 template <typename K, typename A>
-static int kv4_launch(K kern, dim3 grid, dim3 block, size_t smem, cudaStream_t st, const A& a) {
-    if (smem > 48 * 1024 &&
-        cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem)) != cudaSuccess)
-        return LQ_E_CUDA;
+static int kv4_launch(K kern, std::atomic<uint32_t>& set, dim3 grid, dim3 block, size_t smem, cudaStream_t st, const A& a) {
+    if (smem > 48 * 1024) {
+        const uint32_t bit = 1u << (device_info().device & 31);
+        if (!(set.load(std::memory_order_relaxed) & bit)) {
+            if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem)) != cudaSuccess)
+                return LQ_E_CUDA;
+            set.fetch_or(bit, std::memory_order_relaxed);
+        }
+    }
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = grid;
     cfg.blockDim = block;

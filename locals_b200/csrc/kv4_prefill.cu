@@ -775,9 +775,10 @@ static int kv4_prefill_d(Kv4AttArgs a, void* workspace, cudaStream_t st) {
     a.part_o = static_cast<float*>(workspace);
     a.part_ml = a.part_o + size_t(n) * 2 * S::R * D;
     a.records = reinterpret_cast<int32_t*>(a.part_ml + size_t(n) * 2 * S::R * 2);
-    int rc = kv4_launch(kv4_prefill_kernel<T, D>, dim3(n), dim3(PF_THREADS), S::SMEM + 1024 + sizeof(PfBars), st, a);
+    static std::atomic<uint32_t> set{0}, none{0};
+    int rc = kv4_launch(kv4_prefill_kernel<T, D>, set, dim3(n), dim3(PF_THREADS), S::SMEM + 1024 + sizeof(PfBars), st, a);
     if (rc) return rc;
-    return kv4_launch(kv4_prefill_join_kernel<T, D>, dim3(n, S::R / 8), dim3(128), 0, st, a);
+    return kv4_launch(kv4_prefill_join_kernel<T, D>, none, dim3(n, S::R / 8), dim3(128), 0, st, a);
 }
 
 int kv4_prefill_run(const Kv4AttArgs& a, int D, int dtype, void* workspace, cudaStream_t st) {

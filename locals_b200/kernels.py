@@ -48,7 +48,9 @@ def dtype_code(dt: torch.dtype) -> int:
 
 
 def _stream() -> int:
-    return torch.cuda.current_stream().cuda_stream
+    """The current device's current stream (torch.cuda.current_stream().cuda_stream without its Stream object: 0.2 us
+    against 3.2)."""
+    return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
 
 
 def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:

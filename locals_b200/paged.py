@@ -16,6 +16,7 @@ out, and set LQ_DEV_BOUNDS in the device status (``kernels.device_status``).
 
 from __future__ import annotations
 
+import functools
 from typing import NamedTuple, Optional, Sequence, Tuple
 
 import torch
@@ -59,29 +60,39 @@ def pool(pages: int, KVH: int, page_size: int, head_dim: int, dtype: torch.dtype
 
 def _ints(*ts: torch.Tensor) -> None:
     for t in ts:
-        if t.dtype != torch.int32 or not t.is_cuda or not t.is_contiguous():
-            raise ValueError("lengths, tables, page lists and slots are contiguous int32 CUDA tensors")
+        if t.dtype != torch.int32 or not t.is_contiguous() or not t.is_cuda or \
+                t.get_device() != torch._C._cuda_getDevice():
+            raise ValueError("lengths, tables, page lists and slots are contiguous int32 tensors of the current GPU")
 
 
-def _pool(keys: Sequence[torch.Tensor], values: Sequence[torch.Tensor], dtype: torch.dtype, device):
-    """(pages, KVH, page_size, head_dim) of a checked pool, and its six addresses."""
+def _pool(keys: Sequence[torch.Tensor], values: Sequence[torch.Tensor], dtype: torch.dtype):
+    """(pages, KVH, page_size, head_dim) of a checked pool on the current device, and its six addresses."""
     kq, ks, kb = keys
     vq, vs, vb = values
-    if kq.dim() != 4 or kq.dtype != torch.int32 or vq.dtype != torch.int32:
+    shape, small = kq.shape, ks.shape
+    if len(shape) != 4 or kq.dtype != torch.int32 or vq.dtype != torch.int32:
         raise ValueError("words: int32 (pages, KVH, page_size, head_dim / 8) expected")
-    pages, KVH, page, words = kq.shape
-    small = (pages, KVH, page, words * 8 // GROUP)
-    if vq.shape != kq.shape or any(t.shape != small for t in (ks, kb, vs, vb)):
-        raise ValueError(f"keys and values are not 4-bit triples of one pool: words {tuple(kq.shape)}, scales "
-                         f"{tuple(ks.shape)}")
-    for t in (ks, kb, vs, vb):
-        if t.dtype != dtype:
-            raise TypeError("scales and biases must have the queries' dtype")
-    for t in (kq, ks, kb, vq, vs, vb):
-        if t.device != device or not t.is_contiguous():
-            raise ValueError("the cache must be contiguous CUDA tensors on the queries' device")
-    return (pages, KVH, page, words * 8), (kq.data_ptr(), ks.data_ptr(), kb.data_ptr(), vq.data_ptr(), vs.data_ptr(),
-                                           vb.data_ptr())
+    pages, KVH, page, words = shape
+    if vq.shape != shape or small != (pages, KVH, page, words * 8 // GROUP) or kb.shape != small or \
+            vs.shape != small or vb.shape != small:
+        raise ValueError(f"keys and values are not 4-bit triples of one pool: words {tuple(shape)}, scales "
+                         f"{tuple(small)}")
+    if not (ks.dtype == kb.dtype == vs.dtype == vb.dtype == dtype):
+        raise TypeError("scales and biases must have the queries' dtype")
+    d = torch._C._cuda_getDevice()
+    if not (kq.get_device() == ks.get_device() == kb.get_device() == vq.get_device() == vs.get_device()
+            == vb.get_device() == d):
+        raise ValueError("the cache must be on the queries' device, the current one")
+    if not (kq.is_contiguous() and ks.is_contiguous() and kb.is_contiguous() and vq.is_contiguous()
+            and vs.is_contiguous() and vb.is_contiguous()):
+        raise ValueError("the cache must be contiguous")
+    return pages, KVH, page, words * 8, (kq.data_ptr(), ks.data_ptr(), kb.data_ptr(), vq.data_ptr(), vs.data_ptr(),
+                                         vb.data_ptr())
+
+
+@functools.lru_cache(maxsize=1024)
+def _attend_workspace(device: int, N: int, B: int, max_q: int, H: int, KVH: int, D: int) -> int:
+    return int(lib().lq_kv4_attend_workspace(N, B, max_q, H, KVH, D))
 
 
 def plan(cached: torch.Tensor, new: torch.Tensor, block_table: torch.Tensor, free: torch.Tensor, head: torch.Tensor,
@@ -96,17 +107,15 @@ def plan(cached: torch.Tensor, new: torch.Tensor, block_table: torch.Tensor, fre
     B = cached.shape[0]
     if cached.shape != new.shape or cached.dim() != 1 or block_table.dim() != 2 or block_table.shape[0] != B:
         raise ValueError("plan: cached (B,), new (B,), block_table (B, width)")
-    dev = cached.device
     n, B1 = int(tokens), B + 1
     if n < 0:
         raise ValueError("plan: tokens must not be negative")
-    buf = torch.empty(B + B1 + 2 * n + 1, dtype=torch.int32, device=dev)
-    lens, q_start, positions, slots, head_out = buf.split((B, B1, n, n, 1))
+    buf = cached.new_empty(B + B1 + 2 * n + 1)
     p = buf.data_ptr()
     call("lq_page_plan", cached.data_ptr(), new.data_ptr(), B, block_table.data_ptr(), block_table.shape[1],
          free.data_ptr(), free.shape[0], head.data_ptr(), int(page_size), n, p, p + 4 * B, p + 4 * (B + B1),
          p + 4 * (B + B1 + n), p + 4 * (B + B1 + 2 * n), _stream())
-    return Plan(lens, q_start, positions, slots, head_out)
+    return Plan(*buf.split_with_sizes((B, B1, n, n, 1)))
 
 
 def append(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor,
@@ -119,26 +128,25 @@ def append(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor, slots: t
     k, k_row = rotary._rows(k, "k")
     v, v_row = rotary._rows(v, "v")
     N, KVH, D = k.shape
-    dev = k.device
-    (pages, pool_kvh, page, pool_d), ptrs = _pool(keys, values, k.dtype, dev)
-    if v.shape != k.shape or v.dtype != k.dtype or v.device != dev or (KVH, D) != (pool_kvh, pool_d):
+    pages, pool_kvh, page, pool_d, ptrs = _pool(keys, values, k.dtype)
+    if v.shape != k.shape or v.dtype != k.dtype or (KVH, D) != (pool_kvh, pool_d):
         raise ValueError(f"append: k {tuple(k.shape)}, v {tuple(v.shape)} do not fit a cache of {pool_kvh} heads of "
                          f"{pool_d}")
     _ints(slots)
-    if tuple(slots.shape) != (N,) or slots.device != dev:
+    if slots.shape != (N,):
         raise ValueError(f"append: slots ({N},) expected")
     H, q_row, qo = 0, 0, None
     if q is not None:
         q, q_row = rotary._rows(q, "q")
         H = q.shape[1]
-        if q.shape[0] != N or q.shape[2] != D or q.dtype != k.dtype or q.device != dev:
-            raise ValueError("append: q and k must have the same tokens, head_dim, dtype and device")
-        qo = torch.empty((N, H, D), dtype=q.dtype, device=dev)
+        if q.shape[0] != N or q.shape[2] != D or q.dtype != k.dtype:
+            raise ValueError("append: q and k must have the same tokens, head_dim and dtype")
+        qo = rotary._like(q)
     rot, naxes, max_pos = 0, 1, 1
     if positions is not None:
         if cos is None or sin is None:
             raise ValueError("append: positions without cos and sin tables")
-        rot, naxes = rotary._angles(positions, cos, sin, axes, N, D, dev)
+        rot, naxes = rotary._angles(positions, cos, sin, axes, N, D)
         max_pos = cos.shape[0]
     if N:
         call("lq_kv4_append", None if q is None else q.data_ptr(), q_row, None if q is None else qo.data_ptr(), H,
@@ -154,12 +162,12 @@ def read(keys: Sequence[torch.Tensor], values: Sequence[torch.Tensor],
     """The keys and values that the cache holds at ``slots`` (N,), (N, KVH, D) each in the scales' dtype (zeros for a
     negative slot): what ``kernels.dequantize`` makes of those rows."""
     _ints(slots)
-    dtype, dev = keys[1].dtype, keys[0].device
-    (pages, KVH, page, D), ptrs = _pool(keys, values, dtype, dev)
-    if slots.dim() != 1 or slots.device != dev:
-        raise ValueError("read: slots (N,) on the cache's device expected")
+    dtype = keys[1].dtype
+    pages, KVH, page, D, ptrs = _pool(keys, values, dtype)
+    if slots.dim() != 1:
+        raise ValueError("read: slots (N,) expected")
     N = slots.shape[0]
-    ko = torch.empty((N, KVH, D), dtype=dtype, device=dev)
+    ko = keys[1].new_empty((N, KVH, D))
     vo = torch.empty_like(ko)
     if N:
         call("lq_kv4_read", *ptrs, pages, page, KVH, D, slots.data_ptr(), N, ko.data_ptr(), vo.data_ptr(),
@@ -177,37 +185,35 @@ def attend(q: torch.Tensor, keys: Sequence[torch.Tensor], values: Sequence[torch
     Returns (N, H, D) in q's dtype: 0 where a query sees nothing, and in rows past ``q_start[-1]``."""
     q, q_row = rotary._rows(q, "q")
     N, H, D = q.shape
-    if N > 1 and q_row != H * D:
+    if q_row != H * D:
         q = q.contiguous()
-    dev = q.device
-    (pages, KVH, page, pool_d), ptrs = _pool(keys, values, q.dtype, dev)
+    pages, KVH, page, pool_d, ptrs = _pool(keys, values, q.dtype)
     _ints(block_table, lens)
-    B = lens.shape[0]
+    B, table = lens.shape[0], block_table.shape
     if D != pool_d or H % KVH:
         raise ValueError(f"attend: {H} heads of {D} against a cache of {KVH} heads of {pool_d}")
-    if lens.dim() != 1 or block_table.dim() != 2 or block_table.shape[0] != B:
+    if lens.dim() != 1 or len(table) != 2 or table[0] != B:
         raise ValueError("attend: lens (B,), block_table (B, width)")
-    if block_table.device != dev or lens.device != dev:
-        raise ValueError("attend: block_table and lens must be on the queries' device")
+    max_q = int(max_q)
     if q_start is None:
         if N != B or max_q != 1:
             raise ValueError("attend: without q_start there is one query a request")
     else:
         _ints(q_start)
-        if tuple(q_start.shape) != (B + 1,) or q_start.device != dev:
+        if q_start.shape != (B + 1,):
             raise ValueError(f"attend: q_start ({B + 1},) expected")
-    if sinks is not None and (sinks.dtype != torch.float32 or tuple(sinks.shape) != (H,) or sinks.device != dev
-                              or not sinks.is_contiguous()):
-        sinks = sinks.to(device=dev, dtype=torch.float32).contiguous()
-        if tuple(sinks.shape) != (H,):
+    if sinks is not None:
+        if sinks.dtype != torch.float32 or sinks.get_device() != q.get_device() or not sinks.is_contiguous():
+            sinks = sinks.to(device=q.device, dtype=torch.float32).contiguous()
+        if sinks.shape != (H,):
             raise ValueError(f"attend: sinks ({H},) expected")
-    out = torch.empty((N, H, D), dtype=q.dtype, device=dev)
+    out = torch.empty_like(q)
     if N == 0:
         return out
-    nbytes = int(lib().lq_kv4_attend_workspace(N, B, int(max_q), H, KVH, D))
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
-    call("lq_kv4_attend", q.data_ptr(), N, None if q_start is None else q_start.data_ptr(), int(max_q), *ptrs, pages,
-         page, block_table.data_ptr(), block_table.shape[1], lens.data_ptr(), B,
-         None if sinks is None else sinks.data_ptr(), float(scale), int(window), H, KVH, D, dtype_code(q.dtype),
-         None if ws is None else ws.data_ptr(), nbytes, out.data_ptr(), _stream())
+    nbytes = _attend_workspace(q.get_device(), N, B, max_q, H, KVH, D)
+    ws = q.new_empty(nbytes // 2) if nbytes else None
+    call("lq_kv4_attend", q.data_ptr(), N, None if q_start is None else q_start.data_ptr(), max_q, *ptrs, pages, page,
+         block_table.data_ptr(), table[1], lens.data_ptr(), B, None if sinks is None else sinks.data_ptr(), float(scale),
+         int(window), H, KVH, D, dtype_code(q.dtype), None if ws is None else ws.data_ptr(), nbytes, out.data_ptr(),
+         _stream())
     return out

@@ -32,29 +32,37 @@ def _rows(x: torch.Tensor, name: str) -> Tuple[torch.Tensor, int]:
     one token to the next."""
     if x.dim() != 3:
         raise ValueError(f"{name}: (tokens, heads, head_dim) expected, got {tuple(x.shape)}")
-    if not x.is_cuda:
-        raise ValueError("locals_b200 kernels take CUDA tensors")
+    if not x.is_cuda or x.get_device() != torch._C._cuda_getDevice():
+        raise ValueError("locals_b200 kernels take CUDA tensors of the current device")
     N, H, D = x.shape
+    if x.is_contiguous():
+        return x, H * D
     sn, sh, sd = x.stride()
     if (sd != 1 and D > 1) or (sh != D and H > 1) or (N > 1 and sn < H * D):
-        x = x.contiguous()
-        sn = H * D
+        return x.contiguous(), H * D
     return x, (sn if N > 1 else H * D)
 
 
-def _angles(positions, cos, sin, axes, N: int, D: int, device) -> Tuple[int, int]:
+def _like(x: torch.Tensor) -> torch.Tensor:
+    """A contiguous tensor of x's shape, dtype and device."""
+    return torch.empty_like(x) if x.is_contiguous() else torch.empty_like(x, memory_format=torch.contiguous_format)
+
+
+def _angles(positions, cos, sin, axes, N: int, D: int) -> Tuple[int, int]:
     """(rot, number of axes) of checked angle arguments."""
-    if positions.dtype != torch.int32 or positions.dim() not in (1, 2) or positions.shape[-1] != N:
+    ps, cs = positions.shape, cos.shape
+    if positions.dtype != torch.int32 or len(ps) not in (1, 2) or ps[-1] != N:
         raise ValueError(f"positions: int32 ({N},) or (axes, {N}) expected")
-    if cos.dtype != torch.float32 or sin.dtype != torch.float32 or cos.dim() != 2 or cos.shape != sin.shape:
+    if cos.dtype != torch.float32 or sin.dtype != torch.float32 or len(cs) != 2 or cs != sin.shape:
         raise ValueError("cos and sin: float32 (positions, rot / 2) tables expected")
-    rot, naxes = 2 * cos.shape[1], 1 if positions.dim() == 1 else positions.shape[0]
-    if rot < 2 or rot > D or cos.shape[0] < 1 or naxes < 1:
+    rot, naxes = 2 * cs[1], 1 if len(ps) == 1 else ps[0]
+    if rot < 2 or rot > D or cs[0] < 1 or naxes < 1:
         raise ValueError(f"{rot} rotated dimensions do not fit head_dim {D}")
     if axes is not None and (axes.dtype != torch.int32 or tuple(axes.shape) != (rot // 2,)):
         raise ValueError(f"axes: int32 ({rot // 2},) expected")
+    d = torch._C._cuda_getDevice()
     for t in (positions, cos, sin, axes):
-        if t is not None and (t.device != device or not t.is_contiguous()):
+        if t is not None and (t.get_device() != d or not t.is_contiguous()):
             raise ValueError("positions, cos, sin and axes must be contiguous tensors on the queries' device")
     return rot, naxes
 
@@ -71,11 +79,11 @@ def rotate(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, 
     if k is not None:
         k, k_row = _rows(k, "k")
         KVH = k.shape[1]
-        if k.shape[0] != N or k.shape[2] != D or k.dtype != q.dtype or k.device != q.device:
-            raise ValueError("q and k must have the same tokens, head_dim, dtype and device")
-    rot, naxes = _angles(positions, cos, sin, axes, N, D, q.device)
-    qo = torch.empty((N, H, D), dtype=q.dtype, device=q.device)
-    ko = None if k is None else torch.empty((N, KVH, D), dtype=q.dtype, device=q.device)
+        if k.shape[0] != N or k.shape[2] != D or k.dtype != q.dtype:
+            raise ValueError("q and k must have the same tokens, head_dim and dtype")
+    rot, naxes = _angles(positions, cos, sin, axes, N, D)
+    qo = _like(q)
+    ko = None if k is None else _like(k)
     if N:
         call("lq_rotary", q.data_ptr(), q_row, qo.data_ptr(), H, None if k is None else k.data_ptr(), k_row,
              None if k is None else ko.data_ptr(), KVH, N, D, rot, positions.data_ptr(), cos.data_ptr(), sin.data_ptr(),
