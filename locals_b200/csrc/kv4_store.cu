@@ -6,7 +6,7 @@
 // three shuffles each, scale and bias as there from exact 32-bit operations, codes from the 32-bit scale and bias, both
 // then rounded to the activation dtype. A lane's 8 codes are one word. A token whose slot is negative is padding and
 // stores nothing; a slot outside the pool is recorded and stores nothing.
-// CTAs [0, q_blocks) rotate queries, the others write the cache. HBM-bound: q 4 bytes a value, k and v 2 bytes read and
+// CTAs [0, q_blocks) rotate queries (rot_rows), the others write the cache, a lane 8 values of a row. HBM-bound: q 4 bytes a value, k and v 2 bytes read and
 // 0.5625 written.
 //
 // read: the values that the cache holds at given slots (zeros for a negative slot), T(scale * code + bias).
@@ -32,12 +32,15 @@ struct StoreArgs {
     const uint16_t* v;
     const int32_t* slots;
     long long q_row, k_row, v_row;
-    int H, q_blocks;
+    int H;
+    unsigned q_blocks, q_items, units, q_groups;  // query part: units a row, groups of rows a token
+    unsigned kv_items, kv_groups;                 // cache part: (token, group of kv heads)
 };
 
 // cos and sin for the 8 dimensions d0 .. d0 + 7 of token n (rotated: d0 < rot): c, s of each dimension's pair.
+template <bool PAIRS2>
 __device__ __forceinline__ void st_cos_sin(const RotArgs& r, int n, int d0, float (&c)[8], float (&s)[8]) {
-    if (r.interleaved) {
+    if (PAIRS2) {
         float c4[4], s4[4];
         rot_cos_sin<4>(r, n, d0 >> 1, c4, s4);
 #pragma unroll
@@ -48,18 +51,15 @@ __device__ __forceinline__ void st_cos_sin(const RotArgs& r, int n, int d0, floa
     }
 }
 
-// x (8 dimensions from d0 of a row whose lanes are this warp's 8-dimension pieces) rotated in 32 bits. Every lane of
-// the warp takes part; `live` lanes hold a row.
-template <typename T>
-__device__ __forceinline__ void st_rotate(const RotArgs& r, const RotVec<T, 8>& w, int n, int d0, bool live,
-                                          float (&x)[8]) {
+// x: the 8 dimensions from d0 of a row whose lanes are this warp's 8-dimension pieces, rotated in 32 bits where `turned`.
+// Every lane of the warp takes part.
+template <typename T, bool PAIRS2>
+__device__ __forceinline__ void st_rotate(const RotArgs& r, const RotVec<T, 8>& w, int d0, bool turned, const float (&c)[8],
+                                          const float (&s)[8], float (&x)[8]) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) x[i] = w.get(i);
-    if (!r.positions) return;
-    float c[8], s[8];
-    const bool turned = live && d0 < r.rot;
-    if (turned) st_cos_sin(r, n, d0, c, s);
-    if (r.interleaved) {
+    if (r.rot == 0) return;
+    if (PAIRS2) {
         if (turned) {
 #pragma unroll
             for (int i = 0; i < 8; i += 2) rot_pair(x[i], x[i + 1], c[i], s[i]);
@@ -120,58 +120,61 @@ __device__ __forceinline__ uint32_t st_quantize(const float (&x)[8], float* scal
     return word;
 }
 
-template <typename T, int D>
+// RQ query rows a thread, RK kv heads a thread (one read of cos and sin for all of them).
+template <typename T, int D, int RQ, int RK, bool PAIRS2>
 __global__ void __launch_bounds__(ST_THREADS) kv4_append_kernel(const StoreArgs a) {
     constexpr int L = D / 8;  // lanes a row
     grid_dep_wait();
-    const int sub = threadIdx.x % L, d0 = sub * 8;
-    if (int(blockIdx.x) < a.q_blocks) {
-        const long long row = (long long)blockIdx.x * (ST_THREADS / L) + threadIdx.x / L;
-        const bool live = row < (long long)a.r.N * a.H;
-        const int n = live ? int(row / a.H) : 0, h = live ? int(row % a.H) : 0;
-        RotVec<T, 8> w = {};
-        if (live) w.load(a.q + n * a.q_row + (long long)h * D + d0);
-        float x[8];
-        st_rotate<T>(a.r, w, n, d0, live, x);
-        if (live) {
+    if (blockIdx.x < a.q_blocks) {
+        const unsigned item = blockIdx.x * ST_THREADS + threadIdx.x;
+        if (item >= a.q_items) return;
+        const unsigned rest = item / a.units, n = rest / a.q_groups;
+        const int unit = int(item - rest * a.units), row = int(rest - n * a.q_groups) * RQ;
+        rot_rows<T, 8, RQ, PAIRS2>(a.r, a.q + (long long)n * a.q_row + row * D, a.qo + ((long long)n * a.H + row) * D,
+                                   a.H - row, int(n), unit);
+        return;
+    }
+    const int KVH = a.pool.KVH, sub = threadIdx.x % L, d0 = sub * 8;
+    const unsigned item = (blockIdx.x - a.q_blocks) * (ST_THREADS / L) + threadIdx.x / L;
+    const bool live = item < a.kv_items;
+    const unsigned n = live ? item / a.kv_groups : 0;
+    const int h0 = live ? int(item - n * a.kv_groups) * RK : 0;
+    RotVec<T, 8> wk[RK], wv[RK];
+    const int slot = live ? a.slots[n] : -1;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) w.set(i, x[i]);
-            w.store(a.qo + row * D + d0);
+    for (int i = 0; i < RK; ++i) {
+        wk[i] = wv[i] = RotVec<T, 8>{};
+        if (live && h0 + i < KVH) {
+            wk[i].load(a.k + (long long)n * a.k_row + (h0 + i) * D + d0);
+            wv[i].load(a.v + (long long)n * a.v_row + (h0 + i) * D + d0);
         }
-        return;
     }
-    const int KVH = a.pool.KVH;
-    const long long row = (long long)(blockIdx.x - a.q_blocks) * (ST_THREADS / L) + threadIdx.x / L;
-    const bool live = row < (long long)a.r.N * KVH;
-    const int n = live ? int(row / KVH) : 0, h = live ? int(row % KVH) : 0;
-    RotVec<T, 8> wk = {}, wv = {};
-    int slot = -1;
-    if (live) {
-        slot = a.slots[n];
-        wk.load(a.k + n * a.k_row + (long long)h * D + d0);
-        wv.load(a.v + n * a.v_row + (long long)h * D + d0);
-    }
-    float x[8], ks, kb, vs, vb;
-    st_rotate<T>(a.r, wk, n, d0, live, x);
-    const uint32_t kw = st_quantize(x, &ks, &kb);
+    const bool turned = live && d0 < a.r.rot;
+    float c[8], s[8];
+    if (turned) st_cos_sin<PAIRS2>(a.r, int(n), d0, c, s);
+    const int id = slot < 0 ? -1 : slot / a.pool.page;
+    if (id >= a.pool.pages) record_status(LQ_DEV_BOUNDS);
+    const bool kept = id >= 0 && id < a.pool.pages;
+    const size_t at = kept ? kv4_row(a.pool, id, h0, slot - id * a.pool.page) : 0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = wv.get(i);
-    const uint32_t vw = st_quantize(x, &vs, &vb);
-    if (slot < 0) return;
-    const int id = slot / a.pool.page;
-    if (id >= a.pool.pages) {
-        record_status(LQ_DEV_BOUNDS);
-        return;
-    }
-    const size_t at = kv4_row(a.pool, id, h, slot - id * a.pool.page);
-    a.pool.kq[at * L + sub] = kw;
-    a.pool.vq[at * L + sub] = vw;
-    if (sub % 8 == 0) {
-        const size_t g = at * (D / 64) + sub / 8;
-        a.pool.ks[g] = F16Traits<T>::from_f32(ks);
-        a.pool.kb[g] = F16Traits<T>::from_f32(kb);
-        a.pool.vs[g] = F16Traits<T>::from_f32(vs);
-        a.pool.vb[g] = F16Traits<T>::from_f32(vb);
+    for (int i = 0; i < RK; ++i) {
+        float x[8], ks, kb, vs, vb;
+        st_rotate<T, PAIRS2>(a.r, wk[i], d0, turned, c, s, x);
+        const uint32_t kw = st_quantize(x, &ks, &kb);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = wv[i].get(e);
+        const uint32_t vw = st_quantize(x, &vs, &vb);
+        if (!kept || h0 + i >= KVH) continue;
+        const size_t row = at + size_t(i) * a.pool.page;
+        a.pool.kq[row * L + sub] = kw;
+        a.pool.vq[row * L + sub] = vw;
+        if (sub % 8 == 0) {
+            const size_t g = row * (D / 64) + sub / 8;
+            a.pool.ks[g] = F16Traits<T>::from_f32(ks);
+            a.pool.kb[g] = F16Traits<T>::from_f32(kb);
+            a.pool.vs[g] = F16Traits<T>::from_f32(vs);
+            a.pool.vb[g] = F16Traits<T>::from_f32(vb);
+        }
     }
 }
 
@@ -180,7 +183,7 @@ struct ReadArgs {
     const int32_t* slots;
     uint16_t* ko;
     uint16_t* vo;
-    int N;
+    unsigned items;  // (token, kv head)
 };
 
 template <typename T, int D>
@@ -188,9 +191,11 @@ __global__ void __launch_bounds__(ST_THREADS) kv4_read_kernel(const ReadArgs a) 
     constexpr int L = D / 8;
     grid_dep_wait();
     const int sub = threadIdx.x % L, KVH = a.pool.KVH;
-    const long long row = (long long)blockIdx.x * (ST_THREADS / L) + threadIdx.x / L;
-    if (row >= (long long)a.N * KVH) return;
-    const int n = int(row / KVH), h = int(row % KVH);
+    const unsigned item = blockIdx.x * (ST_THREADS / L) + threadIdx.x / L;
+    if (item >= a.items) return;
+    const unsigned n = item / unsigned(KVH);
+    const int h = int(item - n * KVH);
+    const size_t row = item;
     const int slot = a.slots[n];
     RotVec<T, 8> k = {}, v = {};
     const int id = slot < 0 ? -1 : slot / a.pool.page;
@@ -228,14 +233,27 @@ static int st_launch(K kern, long long blocks, cudaStream_t st, const A& a) {
     return cudaLaunchKernelEx(&cfg, kern, a) == cudaSuccess ? LQ_OK : LQ_E_CUDA;
 }
 
+template <typename T, int D, int RQ, int RK, bool PAIRS2>
+static int append_r(StoreArgs& a, cudaStream_t st) {
+    const int per = ST_THREADS / (D / 8);  // rows a CTA
+    a.q_groups = unsigned(a.H + RQ - 1) / RQ;
+    a.kv_groups = unsigned(a.pool.KVH + RK - 1) / RK;
+    a.units = unsigned(PAIRS2 ? D : D - a.r.rot / 2) / 8;
+    const unsigned long long qi = (unsigned long long)a.r.N * a.q_groups * a.units;
+    const unsigned long long ki = (unsigned long long)a.r.N * a.kv_groups;
+    if (qi >= 0xffffff00ull || ki * (D / 8) >= 0xffffff00ull) return LQ_E_SHAPE;
+    a.q_items = unsigned(qi);
+    a.kv_items = unsigned(ki);
+    a.q_blocks = unsigned((qi + ST_THREADS - 1) / ST_THREADS);
+    return st_launch(kv4_append_kernel<T, D, RQ, RK, PAIRS2>, (long long)a.q_blocks + (ki + per - 1) / per, st, a);
+}
+
 template <typename T, int D>
 static int append_d(StoreArgs& a, cudaStream_t st) {
-    const int per = ST_THREADS / (D / 8);  // rows a CTA
-    const long long qb = ((long long)a.r.N * a.H + per - 1) / per;
-    const long long kvb = ((long long)a.r.N * a.pool.KVH + per - 1) / per;
-    if (qb + kvb > 0x7fffffffLL) return LQ_E_SHAPE;
-    a.q_blocks = int(qb);
-    return st_launch(kv4_append_kernel<T, D>, qb + kvb, st, a);
+    // Several rows a thread (one read of cos and sin for all) once one row a thread would be several waves of CTAs.
+    const bool many = (long long)a.r.N * (a.H + 2 * a.pool.KVH) * (D / 8) >= 4LL * device_info().sm_count * 8 * ST_THREADS;
+    if (a.r.interleaved) return many ? append_r<T, D, 4, 2, true>(a, st) : append_r<T, D, 1, 1, true>(a, st);
+    return many ? append_r<T, D, 4, 2, false>(a, st) : append_r<T, D, 1, 1, false>(a, st);
 }
 
 template <typename T>
@@ -271,7 +289,7 @@ int kv4_append_run(const RotArgs& r, const Kv4Pool& pool, const void* q, long lo
 template <typename T>
 static int read_t(const ReadArgs& a, int D, cudaStream_t st) {
     const int per = ST_THREADS / (D / 8);
-    const long long blocks = ((long long)a.N * a.pool.KVH + per - 1) / per;
+    const long long blocks = ((long long)a.items + per - 1) / per;
     return D == 64    ? st_launch(kv4_read_kernel<T, 64>, blocks, st, a)
            : D == 128 ? st_launch(kv4_read_kernel<T, 128>, blocks, st, a)
                       : st_launch(kv4_read_kernel<T, 256>, blocks, st, a);
@@ -280,7 +298,8 @@ static int read_t(const ReadArgs& a, int D, cudaStream_t st) {
 int kv4_read_run(const Kv4Pool& pool, int D, const int32_t* slots, int N, void* k_out, void* v_out, int dtype,
                  cudaStream_t st) {
     if (N == 0) return LQ_OK;
-    const ReadArgs a = {pool, slots, static_cast<uint16_t*>(k_out), static_cast<uint16_t*>(v_out), N};
+    if ((unsigned long long)N * pool.KVH * (D / 8) >= 0xffffff00ull) return LQ_E_SHAPE;
+    const ReadArgs a = {pool, slots, static_cast<uint16_t*>(k_out), static_cast<uint16_t*>(v_out), unsigned(N) * pool.KVH};
     return dtype == LQ_BF16 ? read_t<__nv_bfloat16>(a, D, st) : read_t<__half>(a, D, st);
 }
 

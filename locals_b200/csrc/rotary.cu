@@ -1,10 +1,9 @@
 // Rotary positions with several axes on queries and keys (the arithmetic is rotary.cuh's).
 //
-// A work item is one unit of a row (V pairs held as two vectors of V values a half apart, or V values of neighbouring
-// pairs, or V copied values) of R rows of one token: the token's cos and sin are read once for the R rows, and the R
-// rows' loads are issued together. Items are numbered unit fastest, so a warp's accesses run along rows. V is the
-// widest vector that the sizes, strides and addresses allow, 16 bytes where they allow it.
-// HBM-bound: 4 bytes a value, and the table rows (32-bit values, read from L2 after their first use).
+// A work item is one unit (rot_rows) of R rows of one token, all of them queries or all keys. Items are numbered unit
+// fastest, so a warp's accesses run along rows. The vectors are the widest that the sizes, strides and addresses allow,
+// 16 bytes where they allow it. HBM-bound: 4 bytes a value, and the table rows (32-bit values, from L2 after their first
+// use, and from L1 for R rows at a time).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -24,84 +23,33 @@ struct RotaryArgs {
     const uint16_t* k;
     uint16_t* ko;
     long long q_row, k_row;  // values from one token's rows to the next's (inputs; outputs are contiguous)
-    int H, KVH, units, groups;
-    long long items;
+    int H, KVH;
+    unsigned units, q_groups, groups, items;  // units a row, groups of R rows of q and of q and k a token
 };
 
 template <typename T, int V, int R, bool PAIRS2>
 __global__ void __launch_bounds__(ROT_THREADS) rotary_kernel(const RotaryArgs a) {
     grid_dep_wait();
-    const long long item = (long long)blockIdx.x * ROT_THREADS + threadIdx.x;
+    const unsigned item = blockIdx.x * ROT_THREADS + threadIdx.x;
     if (item >= a.items) return;
-    const int unit = int(item % a.units);
-    const long long rest = item / a.units;
-    const int g = int(rest % a.groups), n = int(rest / a.groups);
-    const int half = a.r.rot >> 1;
-    const int rows = a.H + a.KVH;
-    // where the unit's first vector starts in a row, and whether it is rotated
-    int at;
-    bool turned;
-    if (PAIRS2) {
-        at = unit * V;
-        turned = at < a.r.rot;
-    } else {
-        turned = unit * V < half;
-        at = turned ? unit * V : a.r.rot + (unit * V - half);
-    }
-    RotVec<T, V> lo[R], hi[R];
-    const uint16_t* src[R];
-    uint16_t* dst[R];
-#pragma unroll
-    for (int i = 0; i < R; ++i) {
-        const int row = g * R + i;
-        if (row >= rows) continue;
-        const bool isq = row < a.H;
-        src[i] = isq ? a.q + n * a.q_row + (long long)row * a.r.D
-                     : a.k + n * a.k_row + (long long)(row - a.H) * a.r.D;
-        dst[i] = isq ? a.qo + ((long long)n * a.H + row) * a.r.D
-                     : a.ko + ((long long)n * a.KVH + row - a.H) * a.r.D;
-        lo[i].load(src[i] + at);
-        if (!PAIRS2 && turned) hi[i].load(src[i] + at + half);
-    }
-    if (turned) {
-        constexpr int P = PAIRS2 ? V / 2 : V;
-        float c[P], s[P];
-        rot_cos_sin<P>(a.r, n, PAIRS2 ? at / 2 : at, c, s);
-#pragma unroll
-        for (int i = 0; i < R; ++i) {
-            if (g * R + i >= rows) continue;
-#pragma unroll
-            for (int j = 0; j < P; ++j) {
-                if (PAIRS2) {
-                    float x = lo[i].get(2 * j), y = lo[i].get(2 * j + 1);
-                    rot_pair(x, y, c[j], s[j]);
-                    lo[i].set(2 * j, x);
-                    lo[i].set(2 * j + 1, y);
-                } else {
-                    float x = lo[i].get(j), y = hi[i].get(j);
-                    rot_pair(x, y, c[j], s[j]);
-                    lo[i].set(j, x);
-                    hi[i].set(j, y);
-                }
-            }
-        }
-    }
-#pragma unroll
-    for (int i = 0; i < R; ++i) {
-        if (g * R + i >= rows) continue;
-        lo[i].store(dst[i] + at);
-        if (!PAIRS2 && turned) hi[i].store(dst[i] + at + half);
-    }
+    const unsigned rest = item / a.units, n = rest / a.groups;
+    const int unit = int(item - rest * a.units), g = int(rest - n * a.groups);
+    const bool isq = unsigned(g) < a.q_groups;
+    const int row = (isq ? g : g - int(a.q_groups)) * R, D = a.r.D;
+    const uint16_t* src = isq ? a.q + (long long)n * a.q_row : a.k + (long long)n * a.k_row;
+    uint16_t* dst = isq ? a.qo + (long long)n * a.H * D : a.ko + (long long)n * a.KVH * D;
+    rot_rows<T, V, R, PAIRS2>(a.r, src + row * D, dst + row * D, (isq ? a.H : a.KVH) - row, int(n), unit);
 }
 
 template <typename T, int V, int R, bool PAIRS2>
 static int rotary_launch(RotaryArgs a, cudaStream_t st) {
-    a.groups = (a.H + a.KVH + R - 1) / R;
-    a.items = (long long)a.r.N * a.groups * a.units;
-    const long long blocks = (a.items + ROT_THREADS - 1) / ROT_THREADS;
-    if (blocks > 0x7fffffffLL) return LQ_E_SHAPE;
+    a.q_groups = unsigned(a.H + R - 1) / R;
+    a.groups = a.q_groups + unsigned(a.KVH + R - 1) / R;
+    const unsigned long long items = (unsigned long long)a.r.N * a.groups * a.units;
+    if (items >= 0xffffff00ull) return LQ_E_SHAPE;
+    a.items = unsigned(items);
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(unsigned(blocks));
+    cfg.gridDim = dim3(unsigned((items + ROT_THREADS - 1) / ROT_THREADS));
     cfg.blockDim = dim3(ROT_THREADS);
     cfg.stream = st;
     cudaLaunchAttribute attr[1];
@@ -152,7 +100,7 @@ int rotary_run(const void* q, long long q_row, void* q_out, int H, const void* k
     if (H) all |= (unsigned long long)q_row | (reinterpret_cast<uintptr_t>(q) >> 1) | (reinterpret_cast<uintptr_t>(q_out) >> 1);
     if (KVH) all |= (unsigned long long)k_row | (reinterpret_cast<uintptr_t>(k) >> 1) | (reinterpret_cast<uintptr_t>(k_out) >> 1);
     const int V = int(all & (~all + 1));
-    a.units = (interleaved ? D : half + (D - rot)) / V;
+    a.units = unsigned((interleaved ? D : half + (D - rot)) / V);
     const bool bf = dtype == LQ_BF16;
     switch (V) {
         case 8: return bf ? rotary_v<__nv_bfloat16, 8>(a, st) : rotary_v<__half, 8>(a, st);

@@ -108,4 +108,54 @@ struct RotVec {
     __device__ __forceinline__ void set(int i, float v) { h[i] = F16Traits<T>::from_f32(v); }
 };
 
+// Unit u of up to R rows of token n (src, dst: the first row; rows lie D values apart): V values and, where pairs are
+// halves, the V of their partners half a rotation further; or, past the rotated dimensions, V values copied. The
+// token's cos and sin are read once, the rows' loads are issued together.
+template <typename T, int V, int R, bool PAIRS2>
+__device__ __forceinline__ void rot_rows(const RotArgs& r, const uint16_t* src, uint16_t* dst, int rows, int n, int u) {
+    const int half = r.rot >> 1;
+    int at;
+    bool turned;
+    if (PAIRS2) {
+        at = u * V;
+        turned = at < r.rot;
+    } else {
+        turned = u * V < half;
+        at = turned ? u * V : r.rot + (u * V - half);
+    }
+    src += at;
+    dst += at;
+    RotVec<T, V> lo[R], hi[R];
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+        if (i >= rows) continue;
+        lo[i].load(src + i * r.D);
+        if (!PAIRS2 && turned) hi[i].load(src + i * r.D + half);
+    }
+    if (turned) {
+        constexpr int P = PAIRS2 ? V / 2 : V;
+        float c[P], s[P];
+        rot_cos_sin<P>(r, n, PAIRS2 ? at / 2 : at, c, s);
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+            if (i >= rows) continue;
+#pragma unroll
+            for (int j = 0; j < P; ++j) {
+                const int ja = PAIRS2 ? 2 * j : j, jb = PAIRS2 ? 2 * j + 1 : j;
+                RotVec<T, V>& other = PAIRS2 ? lo[i] : hi[i];
+                float x = lo[i].get(ja), y = other.get(jb);
+                rot_pair(x, y, c[j], s[j]);
+                lo[i].set(ja, x);
+                other.set(jb, y);
+            }
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+        if (i >= rows) continue;
+        lo[i].store(dst + i * r.D);
+        if (!PAIRS2 && turned) hi[i].store(dst + i * r.D + half);
+    }
+}
+
 }  // namespace lq
