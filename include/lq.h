@@ -259,7 +259,7 @@ int lq_page_plan(const int32_t* cached, const int32_t* fresh, int B, int32_t* ta
  * positions[axes[j] * N + n] of cos and sin (max_pos, rot / 2) float32. positions (naxes, N); axes (rot / 2), NULL = all
  * pairs on axis 0. q_row, k_row: elements from one token to the next (a token's heads are contiguous). Either of q and k
  * may be absent (NULL, with H or KVH 0). 32-bit arithmetic, one rounding. A position outside the tables uses the nearest
- * row (and LQ_DEV_BOUNDS). Any head_dim and even rot <= head_dim; interleaved rows must lie on 4-byte boundaries. An
+ * row (and LQ_DEV_BOUNDS). Any head_dim up to 1024 and even rot <= head_dim; interleaved rows must lie on 4-byte boundaries. An
  * output may be its own input when that is contiguous. */
 int lq_rotary(const void* q, int64_t q_row, void* q_out, int H, const void* k, int64_t k_row, void* k_out, int KVH,
               int N, int head_dim, int rot, const int32_t* positions, const float* cos, const float* sin, int max_pos,

@@ -2,12 +2,12 @@
 //
 // append: a step's queries and keys rotated (rotary.cuh), keys and values quantized to 4 bits and stored in their slots,
 // in one launch. The rotated keys are quantized from their 32-bit values, never rounded in between. Quantization is the
-// MLX affine algorithm of quant.cu, a group of 64 in the registers of 8 lanes (8 values each): minimum and maximum by
-// three shuffles each, scale and bias as there from exact 32-bit operations, codes from the 32-bit scale and bias, both
-// then rounded to the activation dtype. A lane's 8 codes are one word. A token whose slot is negative is padding and
-// stores nothing; a slot outside the pool is recorded and stores nothing.
-// CTAs [0, q_blocks) rotate queries (rot_rows), the others write the cache, a lane 8 values of a row. HBM-bound: q 4 bytes a value, k and v 2 bytes read and
-// 0.5625 written.
+// MLX affine algorithm of quant.cu, a group of 64 in the registers of 8 lanes (8 values each), the groups of two
+// heads' keys and values together; scale and bias as there from exact 32-bit operations, codes from the 32-bit scale and
+// bias, both then rounded to the activation dtype. A lane's 8 codes are one word. A token whose slot is negative is
+// padding and stores nothing; a slot outside the pool is recorded and stores nothing. Some CTAs rotate queries (rot_rows),
+// the others write the cache, a lane 8 values of a row. HBM-bound: q 4 bytes a value, k and v 2 bytes read and 0.5625
+// written; the quantization's instructions come close to the same time.
 //
 // read: the values that the cache holds at given slots (zeros for a negative slot), T(scale * code + bias).
 #include <cuda_bf16.h>
@@ -35,29 +35,15 @@ struct StoreArgs {
     int H;
     unsigned q_blocks, q_items, units, q_groups;  // query part: units a row, groups of rows a token
     unsigned kv_items, kv_groups;                 // cache part: (token, group of kv heads)
+    int staged;                                   // floats of cos (and of sin) in shared memory
 };
-
-// cos and sin for the 8 dimensions d0 .. d0 + 7 of token n (rotated: d0 < rot): c, s of each dimension's pair.
-template <bool PAIRS2>
-__device__ __forceinline__ void st_cos_sin(const RotArgs& r, int n, int d0, float (&c)[8], float (&s)[8]) {
-    if (PAIRS2) {
-        float c4[4], s4[4];
-        rot_cos_sin<4>(r, n, d0 >> 1, c4, s4);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) c[i] = c4[i >> 1], s[i] = s4[i >> 1];
-    } else {
-        const int half = r.rot >> 1;
-        rot_cos_sin<8>(r, n, d0 < half ? d0 : d0 - half, c, s);
-    }
-}
 
 // x: the 8 dimensions from d0 of a row whose lanes are this warp's 8-dimension pieces, rotated in 32 bits where `turned`.
 // Every lane of the warp takes part.
 template <typename T, bool PAIRS2>
 __device__ __forceinline__ void st_rotate(const RotArgs& r, const RotVec<T, 8>& w, int d0, bool turned, const float (&c)[8],
                                           const float (&s)[8], float (&x)[8]) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = w.get(i);
+    w.get(x);
     if (r.rot == 0) return;
     if (PAIRS2) {
         if (turned) {
@@ -70,35 +56,20 @@ __device__ __forceinline__ void st_rotate(const RotArgs& r, const RotVec<T, 8>& 
     const int half = r.rot >> 1, lane = threadIdx.x & 31;
     const bool first = d0 < half;
     const int from = turned ? (first ? lane + (half >> 3) : lane - (half >> 3)) : lane;
+    RotVec<T, 8> other;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) other.w[i] = __shfl_sync(0xffffffffu, w.w[i], from);
     float y[8];
-    const uint32_t* p = reinterpret_cast<const uint32_t*>(w.h);
+    other.get(y);
+    if (turned) {  // a c - b s in the first half, b c + a s in the second
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const uint32_t u = __shfl_sync(0xffffffffu, p[i], from);
-        y[2 * i] = F16Traits<T>::to_f32(u & 0xffffu);
-        y[2 * i + 1] = F16Traits<T>::to_f32(u >> 16);
-    }
-    if (turned) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            if (first)
-                rot_pair(x[i], y[i], c[i], s[i]);
-            else
-                rot_pair(y[i], x[i], c[i], s[i]);
-        }
+        for (int i = 0; i < 8; ++i)
+            x[i] = __fadd_rn(__fmul_rn(x[i], c[i]), __fmul_rn(y[i], first ? -s[i] : s[i]));
     }
 }
 
-// 8 values of a group of 64 held by 8 neighbouring lanes -> the lane's word of codes, and the group's scale and bias.
-__device__ __forceinline__ uint32_t st_quantize(const float (&x)[8], float* scale_out, float* bias_out) {
-    float lo = x[0], hi = x[0];
-#pragma unroll
-    for (int i = 1; i < 8; ++i) lo = fminf(lo, x[i]), hi = fmaxf(hi, x[i]);
-#pragma unroll
-    for (int d = 1; d < 8; d <<= 1) {
-        lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, d));
-        hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, d));
-    }
+// The scale and bias of a group from its least and largest value, and the scale's reciprocal.
+__device__ __forceinline__ void st_scale(float lo, float hi, float* scale_out, float* bias_out, float* inv) {
     const bool neg = fabsf(lo) > fabsf(hi);
     float scale = fmaxf(__fdiv_rn(hi - lo, 15.0f), 1e-7f);
     scale = neg ? scale : -scale;
@@ -109,33 +80,106 @@ __device__ __forceinline__ uint32_t st_quantize(const float (&x)[8], float* scal
         scale = __fdiv_rn(edge, q0);
         bias = edge;
     }
-    uint32_t word = 0;
+    *scale_out = scale;
+    *bias_out = bias;
+    *inv = __frcp_rn(scale);
+}
+
+// 8 values -> their word of codes round((x - bias) / scale), the division in 32 bits. A product with the reciprocal is
+// within 2^-18 of the quotient, so its rounding is the quotient's wherever it lies further than that from a half; only
+// there (a few in ten thousand) is the division itself done.
+__device__ __forceinline__ uint32_t st_codes(const float (&x)[8], float scale, float bias, float inv) {
+    const float magic = 12582912.0f;  // 1.5 * 2^23: adding it rounds to a whole number
+    uint32_t word = 0, near = 0;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-        const float q = fminf(fmaxf(rintf(__fdiv_rn(x[i] - bias, scale)), 0.0f), 15.0f);
-        word |= uint32_t(q) << (4 * i);
+        const float t = fminf(fmaxf((x[i] - bias) * inv, 0.0f), 15.0f), u = t + magic;
+        if (fabsf(t - (u - magic)) > 0.5f - 1.52587890625e-5f) near |= 1u << i;
+        word |= (__float_as_uint(u) & 15u) << (4 * i);
+    }
+    while (near) {
+        const int i = __ffs(near) - 1;
+        near &= near - 1;
+        float v = x[0];  // x[i] without an indexed register
+#pragma unroll
+        for (int k = 1; k < 8; ++k) v = k == i ? x[k] : v;
+        const float q = fminf(fmaxf(rintf(__fdiv_rn(v - bias, scale)), 0.0f), 15.0f);
+        word = (word & ~(15u << (4 * i))) | (uint32_t(q) << (4 * i));
+    }
+    return word;
+}
+
+// Q (2 or 4) groups of 64, 8 values of each in each of 8 neighbouring lanes -> the lane's words of codes. The groups'
+// extremes are reduced together, each step of the butterfly leaving a lane half of them, so that lane l ends with one
+// group, own(l), whose scale and bias it alone works out (and returns) and the others take from it.
+template <int Q>
+__device__ __forceinline__ int st_own(int lane) {
+    return Q == 4 ? 2 * (lane & 1) + ((lane >> 1) & 1) : lane & 1;
+}
+template <int Q>
+__device__ __forceinline__ void st_quantize(const float (&x)[Q][8], uint32_t (&words)[Q], float* scale_out, float* bias_out) {
+    const int lane = threadIdx.x & 31;
+    float lo[Q], hi[Q];
+#pragma unroll
+    for (int q = 0; q < Q; ++q) {
+        lo[q] = hi[q] = x[q][0];
+#pragma unroll
+        for (int i = 1; i < 8; ++i) lo[q] = fminf(lo[q], x[q][i]), hi[q] = fmaxf(hi[q], x[q][i]);
+    }
+#pragma unroll
+    for (int n = Q / 2, d = 1; n >= 1; n /= 2, d *= 2) {  // keep the upper or the lower n of 2 n groups
+        const bool up = lane & d;
+#pragma unroll
+        for (int i = 0; i < n; ++i) {
+            const float gl = __shfl_xor_sync(0xffffffffu, up ? lo[i] : lo[n + i], d);
+            const float gh = __shfl_xor_sync(0xffffffffu, up ? hi[i] : hi[n + i], d);
+            lo[i] = fminf(up ? lo[n + i] : lo[i], gl);
+            hi[i] = fmaxf(up ? hi[n + i] : hi[i], gh);
+        }
+    }
+#pragma unroll
+    for (int d = Q; d < 8; d <<= 1) {
+        lo[0] = fminf(lo[0], __shfl_xor_sync(0xffffffffu, lo[0], d));
+        hi[0] = fmaxf(hi[0], __shfl_xor_sync(0xffffffffu, hi[0], d));
+    }
+    float scale, bias, inv;
+    st_scale(lo[0], hi[0], &scale, &bias, &inv);
+#pragma unroll
+    for (int q = 0; q < Q; ++q) {
+        const int from = (lane & ~7) | (Q == 4 ? (q >> 1) | ((q & 1) << 1) : q);
+        words[q] = st_codes(x[q], __shfl_sync(0xffffffffu, scale, from), __shfl_sync(0xffffffffu, bias, from),
+                            __shfl_sync(0xffffffffu, inv, from));
     }
     *scale_out = scale;
     *bias_out = bias;
-    return word;
 }
 
 // RQ query rows a thread, RK kv heads a thread (one read of cos and sin for all of them).
 template <typename T, int D, int RQ, int RK, bool PAIRS2>
 __global__ void __launch_bounds__(ST_THREADS) kv4_append_kernel(const StoreArgs a) {
     constexpr int L = D / 8;  // lanes a row
+    extern __shared__ __align__(16) float st_smem[];
     grid_dep_wait();
-    if (blockIdx.x < a.q_blocks) {
-        const unsigned item = blockIdx.x * ST_THREADS + threadIdx.x;
+    const int half = a.r.rot >> 1;
+    float* sn = st_smem + a.staged;
+    // query and cache CTAs in turn, as long as there are both: the ones wait for memory, the others compute
+    const unsigned kv_blocks = gridDim.x - a.q_blocks, both = 2 * min(a.q_blocks, kv_blocks), b = blockIdx.x;
+    const bool is_q = b < both ? b & 1 : a.q_blocks > kv_blocks;
+    const unsigned blk = b < both ? b / 2 : b - both / 2;
+    if (is_q) {
+        const unsigned first = blk * ST_THREADS, item = first + threadIdx.x, per = a.units * a.q_groups;
+        const int n0 = int(first / per);
+        if (half) rot_stage(a.r, n0, int((min(first + ST_THREADS, a.q_items) - 1) / per) - n0 + 1, st_smem, sn);
         if (item >= a.q_items) return;
-        const unsigned rest = item / a.units, n = rest / a.q_groups;
-        const int unit = int(item - rest * a.units), row = int(rest - n * a.q_groups) * RQ;
+        const unsigned n = item / per, rest = item - n * per;
+        const int g = int(rest / a.units), unit = int(rest - unsigned(g) * a.units), row = g * RQ;
+        const int at = (int(n) - n0) * half;
         rot_rows<T, 8, RQ, PAIRS2>(a.r, a.q + (long long)n * a.q_row + row * D, a.qo + ((long long)n * a.H + row) * D,
-                                   a.H - row, int(n), unit);
+                                   a.H - row, unit, st_smem + at, sn + at);
         return;
     }
     const int KVH = a.pool.KVH, sub = threadIdx.x % L, d0 = sub * 8;
-    const unsigned item = (blockIdx.x - a.q_blocks) * (ST_THREADS / L) + threadIdx.x / L;
+    const unsigned first = blk * (ST_THREADS / L), item = first + threadIdx.x / L;
     const bool live = item < a.kv_items;
     const unsigned n = live ? item / a.kv_groups : 0;
     const int h0 = live ? int(item - n * a.kv_groups) * RK : 0;
@@ -149,32 +193,50 @@ __global__ void __launch_bounds__(ST_THREADS) kv4_append_kernel(const StoreArgs 
             wv[i].load(a.v + (long long)n * a.v_row + (h0 + i) * D + d0);
         }
     }
+    if (half) {
+        const int n0 = int(first / a.kv_groups);
+        rot_stage(a.r, n0, int((min(first + ST_THREADS / L, a.kv_items) - 1) / a.kv_groups) - n0 + 1, st_smem, sn);
+    }
     const bool turned = live && d0 < a.r.rot;
-    float c[8], s[8];
-    if (turned) st_cos_sin<PAIRS2>(a.r, int(n), d0, c, s);
+    float c[8], s[8];  // of the dimensions' pairs
+    if (turned) {
+        const int at = (int(n) - int(first / a.kv_groups)) * half;
+        if constexpr (PAIRS2) {
+            float c4[4], s4[4];
+            rot_staged(st_smem + at + d0 / 2, c4);
+            rot_staged(sn + at + d0 / 2, s4);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) c[i] = c4[i >> 1], s[i] = s4[i >> 1];
+        } else {
+            rot_staged(st_smem + at + (d0 < half ? d0 : d0 - half), c);
+            rot_staged(sn + at + (d0 < half ? d0 : d0 - half), s);
+        }
+    }
     const int id = slot < 0 ? -1 : slot / a.pool.page;
     if (id >= a.pool.pages) record_status(LQ_DEV_BOUNDS);
     const bool kept = id >= 0 && id < a.pool.pages;
     const size_t at = kept ? kv4_row(a.pool, id, h0, slot - id * a.pool.page) : 0;
+    float x[2 * RK][8], scale, bias;  // group 2 i: keys of head i, 2 i + 1: its values
+    uint32_t words[2 * RK];
 #pragma unroll
     for (int i = 0; i < RK; ++i) {
-        float x[8], ks, kb, vs, vb;
-        st_rotate<T, PAIRS2>(a.r, wk[i], d0, turned, c, s, x);
-        const uint32_t kw = st_quantize(x, &ks, &kb);
+        st_rotate<T, PAIRS2>(a.r, wk[i], d0, turned, c, s, x[2 * i]);
+        wv[i].get(x[2 * i + 1]);
+    }
+    st_quantize<2 * RK>(x, words, &scale, &bias);
+    if (!kept) return;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = wv[i].get(e);
-        const uint32_t vw = st_quantize(x, &vs, &vb);
-        if (!kept || h0 + i >= KVH) continue;
+    for (int i = 0; i < RK; ++i) {
+        if (h0 + i >= KVH) continue;
         const size_t row = at + size_t(i) * a.pool.page;
-        a.pool.kq[row * L + sub] = kw;
-        a.pool.vq[row * L + sub] = vw;
-        if (sub % 8 == 0) {
-            const size_t g = row * (D / 64) + sub / 8;
-            a.pool.ks[g] = F16Traits<T>::from_f32(ks);
-            a.pool.kb[g] = F16Traits<T>::from_f32(kb);
-            a.pool.vs[g] = F16Traits<T>::from_f32(vs);
-            a.pool.vb[g] = F16Traits<T>::from_f32(vb);
-        }
+        a.pool.kq[row * L + sub] = words[2 * i];
+        a.pool.vq[row * L + sub] = words[2 * i + 1];
+    }
+    const int own = st_own<2 * RK>(threadIdx.x & 31), mine = sub & 7;
+    if (mine < 2 * RK && h0 + own / 2 < KVH) {
+        const size_t g = (at + size_t(own / 2) * a.pool.page) * (D / 64) + sub / 8;
+        (own & 1 ? a.pool.vs : a.pool.ks)[g] = F16Traits<T>::from_f32(scale);
+        (own & 1 ? a.pool.vb : a.pool.kb)[g] = F16Traits<T>::from_f32(bias);
     }
 }
 
@@ -185,6 +247,11 @@ struct ReadArgs {
     uint16_t* vo;
     unsigned items;  // (token, kv head)
 };
+
+// Code i of a word: as the last bits of 2^23 + code, which a subtraction takes (a conversion runs at a quarter of its rate).
+__device__ __forceinline__ float st_code(uint32_t w, int i) {
+    return __uint_as_float(0x4b000000u | ((w >> (4 * i)) & 15u)) - 8388608.0f;
+}
 
 template <typename T, int D>
 __global__ void __launch_bounds__(ST_THREADS) kv4_read_kernel(const ReadArgs a) {
@@ -206,11 +273,14 @@ __global__ void __launch_bounds__(ST_THREADS) kv4_read_kernel(const ReadArgs a) 
         const uint32_t kw = a.pool.kq[at * L + sub], vw = a.pool.vq[at * L + sub];
         const float ks = F16Traits<T>::to_f32(a.pool.ks[g]), kb = F16Traits<T>::to_f32(a.pool.kb[g]);
         const float vs = F16Traits<T>::to_f32(a.pool.vs[g]), vb = F16Traits<T>::to_f32(a.pool.vb[g]);
+        float x[8], y[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            k.set(i, fmaf(ks, float((kw >> (4 * i)) & 15u), kb));
-            v.set(i, fmaf(vs, float((vw >> (4 * i)) & 15u), vb));
+            x[i] = fmaf(ks, st_code(kw, i), kb);
+            y[i] = fmaf(vs, st_code(vw, i), vb);
         }
+        k.set(x);
+        v.set(y);
     }
     k.store(a.ko + row * D + sub * 8);
     v.store(a.vo + row * D + sub * 8);
@@ -219,11 +289,12 @@ __global__ void __launch_bounds__(ST_THREADS) kv4_read_kernel(const ReadArgs a) 
 // ---- host ----------------------------------------------------------------------------------------
 
 template <typename K, typename A>
-static int st_launch(K kern, long long blocks, cudaStream_t st, const A& a) {
+static int st_launch(K kern, long long blocks, cudaStream_t st, const A& a, size_t smem = 0) {
     if (blocks > 0x7fffffffLL) return LQ_E_SHAPE;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(unsigned(blocks));
     cfg.blockDim = dim3(ST_THREADS);
+    cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -245,7 +316,12 @@ static int append_r(StoreArgs& a, cudaStream_t st) {
     a.q_items = unsigned(qi);
     a.kv_items = unsigned(ki);
     a.q_blocks = unsigned((qi + ST_THREADS - 1) / ST_THREADS);
-    return st_launch(kv4_append_kernel<T, D, RQ, RK, PAIRS2>, (long long)a.q_blocks + (ki + per - 1) / per, st, a);
+    // tokens that a CTA's items can lie in, of either part
+    const int qp = int(a.units * a.q_groups), kp = int(a.kv_groups);
+    const int qt = qp ? (ST_THREADS + qp - 2) / qp + 1 : 0, kt = (per + kp - 2) / kp + 1;
+    a.staged = (qt > kt ? qt : kt) * (a.r.rot / 2);
+    return st_launch(kv4_append_kernel<T, D, RQ, RK, PAIRS2>, (long long)a.q_blocks + (ki + per - 1) / per, st, a,
+                     size_t(a.staged) * 2 * sizeof(float));
 }
 
 template <typename T, int D>

@@ -25,20 +25,27 @@ struct RotaryArgs {
     long long q_row, k_row;  // values from one token's rows to the next's (inputs; outputs are contiguous)
     int H, KVH;
     unsigned units, q_groups, groups, items;  // units a row, groups of R rows of q and of q and k a token
+    int staged;                               // floats of cos (and of sin) in shared memory
 };
 
 template <typename T, int V, int R, bool PAIRS2>
 __global__ void __launch_bounds__(ROT_THREADS) rotary_kernel(const RotaryArgs a) {
+    extern __shared__ __align__(16) float rot_smem[];
     grid_dep_wait();
-    const unsigned item = blockIdx.x * ROT_THREADS + threadIdx.x;
+    const unsigned first = blockIdx.x * ROT_THREADS, item = first + threadIdx.x;
+    const unsigned per = a.units * a.groups;  // items a token
+    const int n0 = int(first / per), count = int(min(first + ROT_THREADS, a.items) - 1) / int(per) - n0 + 1;
+    const int half = a.r.rot >> 1;
+    float* sn = rot_smem + a.staged;
+    rot_stage(a.r, n0, count, rot_smem, sn);
     if (item >= a.items) return;
-    const unsigned rest = item / a.units, n = rest / a.groups;
-    const int unit = int(item - rest * a.units), g = int(rest - n * a.groups);
+    const unsigned n = item / per, rest = item - n * per;
+    const int g = int(rest / a.units), unit = int(rest - unsigned(g) * a.units);
     const bool isq = unsigned(g) < a.q_groups;
-    const int row = (isq ? g : g - int(a.q_groups)) * R, D = a.r.D;
+    const int row = (isq ? g : g - int(a.q_groups)) * R, D = a.r.D, at = (int(n) - n0) * half;
     const uint16_t* src = isq ? a.q + (long long)n * a.q_row : a.k + (long long)n * a.k_row;
     uint16_t* dst = isq ? a.qo + (long long)n * a.H * D : a.ko + (long long)n * a.KVH * D;
-    rot_rows<T, V, R, PAIRS2>(a.r, src + row * D, dst + row * D, (isq ? a.H : a.KVH) - row, int(n), unit);
+    rot_rows<T, V, R, PAIRS2>(a.r, src + row * D, dst + row * D, (isq ? a.H : a.KVH) - row, unit, rot_smem + at, sn + at);
 }
 
 template <typename T, int V, int R, bool PAIRS2>
@@ -46,11 +53,15 @@ static int rotary_launch(RotaryArgs a, cudaStream_t st) {
     a.q_groups = unsigned(a.H + R - 1) / R;
     a.groups = a.q_groups + unsigned(a.KVH + R - 1) / R;
     const unsigned long long items = (unsigned long long)a.r.N * a.groups * a.units;
-    if (items >= 0xffffff00ull) return LQ_E_SHAPE;
+    if (items >= 0x7fffff00ull) return LQ_E_SHAPE;
     a.items = unsigned(items);
+    const int per = int(a.units * a.groups);  // a CTA's items lie in at most this many tokens
+    a.staged = ((ROT_THREADS + per - 2) / per + 1) * (a.r.rot / 2);
+    a.staged = (a.staged + 3) / 4 * 4;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(unsigned((items + ROT_THREADS - 1) / ROT_THREADS));
     cfg.blockDim = dim3(ROT_THREADS);
+    cfg.dynamicSmemBytes = size_t(a.staged) * 2 * sizeof(float);
     cfg.stream = st;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -75,7 +86,7 @@ static int rotary_v(RotaryArgs a, cudaStream_t st) {
 }
 
 bool rotary_shape_ok(int N, int H, int KVH, int D, int rot, int max_pos, int naxes) {
-    return N >= 0 && H >= 0 && KVH >= 0 && H + KVH >= 1 && D >= 2 && D <= 65536 && rot >= 2 && rot % 2 == 0 &&
+    return N >= 0 && H >= 0 && KVH >= 0 && H + KVH >= 1 && D >= 2 && D <= 1024 && rot >= 2 && rot % 2 == 0 &&
            rot <= D && max_pos >= 1 && naxes >= 1;
 }
 

@@ -9,6 +9,8 @@
 
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "lq_ptx.cuh"
 #include "lq_status.cuh"
 
@@ -22,55 +24,41 @@ struct RotArgs {
     int N, D, rot, max_pos, naxes, interleaved;
 };
 
-// The table row of token n on axis `axis`. An axis or position outside the tables is recorded and moved to the nearest.
-__device__ __forceinline__ const float* rot_row(const RotArgs& r, const float* table, int n, int axis) {
-    if (unsigned(axis) >= unsigned(r.naxes)) {
-        record_status(LQ_DEV_BOUNDS);
-        axis = 0;
+// A CTA's tokens n0 .. n0 + count - 1: cos and sin of each pair into shared memory (count x rot / 2 floats each), one
+// table read a thread and pair whatever the axes' order, for all the rows that the CTA then rotates. An axis or position
+// outside the tables is recorded and moved to the nearest.
+__device__ __forceinline__ void rot_stage(const RotArgs& r, int n0, int count, float* c, float* s) {
+    const int half = r.rot >> 1;
+    for (int i = threadIdx.x; i < count * half; i += blockDim.x) {
+        const int t = i / half, j = i - t * half;
+        int axis = r.axes ? r.axes[j] : 0;
+        if (unsigned(axis) >= unsigned(r.naxes)) {
+            record_status(LQ_DEV_BOUNDS);
+            axis = 0;
+        }
+        int p = r.positions[size_t(axis) * r.N + n0 + t];
+        if (unsigned(p) >= unsigned(r.max_pos)) {
+            record_status(LQ_DEV_BOUNDS);
+            p = p < 0 ? 0 : r.max_pos - 1;
+        }
+        c[i] = r.cos[size_t(p) * half + j];
+        s[i] = r.sin[size_t(p) * half + j];
     }
-    int p = r.positions[size_t(axis) * r.N + n];
-    if (unsigned(p) >= unsigned(r.max_pos)) {
-        record_status(LQ_DEV_BOUNDS);
-        p = p < 0 ? 0 : r.max_pos - 1;
-    }
-    return table + size_t(p) * (r.rot >> 1);
+    __syncthreads();
 }
 
-// cos and sin of pairs j0 .. j0 + P - 1 of token n.
+// P (2, 4, 8: from a multiple of 4 P bytes, or 1) staged values.
 template <int P>
-__device__ __forceinline__ void rot_cos_sin(const RotArgs& r, int n, int j0, float (&c)[P], float (&s)[P]) {
-    const bool wide = P % 4 == 0 && ((r.rot >> 1) & 3) == 0 && (j0 & 3) == 0 &&
-                      ((reinterpret_cast<uintptr_t>(r.cos) | reinterpret_cast<uintptr_t>(r.sin)) & 15) == 0;
-    bool one = true;  // every pair on the same axis
-    int axis = 0;
-    if (r.axes) {
-        axis = r.axes[j0];
+__device__ __forceinline__ void rot_staged(const float* from, float (&x)[P]) {
+    if constexpr (P % 4 == 0) {
 #pragma unroll
-        for (int i = 1; i < P; ++i) one = one && r.axes[j0 + i] == axis;
-    }
-    if (one) {
-        const float *rc = rot_row(r, r.cos, n, axis) + j0, *rs = r.sin + (rc - r.cos);
-        if (wide) {
-            if constexpr (P % 4 == 0) {
-#pragma unroll
-                for (int i = 0; i < P; i += 4) {
-                    const float4 u = *reinterpret_cast<const float4*>(rc + i);
-                    const float4 v = *reinterpret_cast<const float4*>(rs + i);
-                    c[i] = u.x, c[i + 1] = u.y, c[i + 2] = u.z, c[i + 3] = u.w;
-                    s[i] = v.x, s[i + 1] = v.y, s[i + 2] = v.z, s[i + 3] = v.w;
-                }
-            }
-        } else {
-#pragma unroll
-            for (int i = 0; i < P; ++i) c[i] = rc[i], s[i] = rs[i];
+        for (int i = 0; i < P; i += 4) {
+            const float4 v = *reinterpret_cast<const float4*>(from + i);
+            x[i] = v.x, x[i + 1] = v.y, x[i + 2] = v.z, x[i + 3] = v.w;
         }
     } else {
 #pragma unroll
-        for (int i = 0; i < P; ++i) {
-            const float* rc = rot_row(r, r.cos, n, r.axes[j0 + i]) + j0 + i;
-            c[i] = *rc;
-            s[i] = r.sin[rc - r.cos];
-        }
+        for (int i = 0; i < P; ++i) x[i] = from[i];
     }
 }
 
@@ -80,39 +68,58 @@ __device__ __forceinline__ void rot_pair(float& a, float& b, float c, float s) {
     a = x;
 }
 
-// V values of T (V = 1, 2, 4, 8) as one load or store.
+// V values of T (V = 1, 2, 4, 8) as one load or store, converted in pairs.
 template <typename T, int V>
 struct RotVec {
-    alignas(2 * V) uint16_t h[V];
+    uint32_t w[(V + 1) / 2];
     __device__ __forceinline__ void load(const uint16_t* p) {
-        if constexpr (V == 8)
-            *reinterpret_cast<uint4*>(h) = *reinterpret_cast<const uint4*>(p);
-        else if constexpr (V == 4)
-            *reinterpret_cast<uint2*>(h) = *reinterpret_cast<const uint2*>(p);
-        else if constexpr (V == 2)
-            *reinterpret_cast<uint32_t*>(h) = *reinterpret_cast<const uint32_t*>(p);
-        else
-            h[0] = *p;
+        if constexpr (V == 8) {
+            const uint4 v = *reinterpret_cast<const uint4*>(p);
+            w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
+        } else if constexpr (V == 4) {
+            const uint2 v = *reinterpret_cast<const uint2*>(p);
+            w[0] = v.x, w[1] = v.y;
+        } else if constexpr (V == 2) {
+            w[0] = *reinterpret_cast<const uint32_t*>(p);
+        } else {
+            w[0] = *p;
+        }
     }
     __device__ __forceinline__ void store(uint16_t* p) const {
         if constexpr (V == 8)
-            *reinterpret_cast<uint4*>(p) = *reinterpret_cast<const uint4*>(h);
+            *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
         else if constexpr (V == 4)
-            *reinterpret_cast<uint2*>(p) = *reinterpret_cast<const uint2*>(h);
+            *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
         else if constexpr (V == 2)
-            *reinterpret_cast<uint32_t*>(p) = *reinterpret_cast<const uint32_t*>(h);
+            *reinterpret_cast<uint32_t*>(p) = w[0];
         else
-            *p = h[0];
+            *p = uint16_t(w[0]);
     }
-    __device__ __forceinline__ float get(int i) const { return F16Traits<T>::to_f32(h[i]); }
-    __device__ __forceinline__ void set(int i, float v) { h[i] = F16Traits<T>::from_f32(v); }
+    __device__ __forceinline__ void get(float (&x)[V]) const {
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            if constexpr (std::is_same<T, __nv_bfloat16>::value)  // bf16: the upper half of a float
+                x[i] = __uint_as_float(i & 1 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16);
+            else
+                x[i] = F16Traits<T>::to_f32(i & 1 ? w[i / 2] >> 16 : w[i / 2] & 0xffffu);
+        }
+    }
+    __device__ __forceinline__ void set(const float (&x)[V]) {
+        if constexpr (V == 1) {
+            w[0] = F16Traits<T>::from_f32(x[0]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < V; i += 2) w[i / 2] = F16Traits<T>::pack2(x[i + 1], x[i]);
+        }
+    }
 };
 
-// Unit u of up to R rows of token n (src, dst: the first row; rows lie D values apart): V values and, where pairs are
-// halves, the V of their partners half a rotation further; or, past the rotated dimensions, V values copied. The
-// token's cos and sin are read once, the rows' loads are issued together.
+// Unit u of up to R rows of a token (src, dst: the first row; rows lie D values apart): V values and, where pairs are
+// halves, the V of their partners half a rotation further; or, past the rotated dimensions, V values copied. The rows'
+// loads are issued together; cs, sn: the token's staged cos and sin, read once for the rows.
 template <typename T, int V, int R, bool PAIRS2>
-__device__ __forceinline__ void rot_rows(const RotArgs& r, const uint16_t* src, uint16_t* dst, int rows, int n, int u) {
+__device__ __forceinline__ void rot_rows(const RotArgs& r, const uint16_t* src, uint16_t* dst, int rows, int u,
+                                         const float* cs, const float* sn) {
     const int half = r.rot >> 1;
     int at;
     bool turned;
@@ -135,19 +142,24 @@ __device__ __forceinline__ void rot_rows(const RotArgs& r, const uint16_t* src, 
     if (turned) {
         constexpr int P = PAIRS2 ? V / 2 : V;
         float c[P], s[P];
-        rot_cos_sin<P>(r, n, PAIRS2 ? at / 2 : at, c, s);
+        rot_staged(cs + (PAIRS2 ? at / 2 : at), c);
+        rot_staged(sn + (PAIRS2 ? at / 2 : at), s);
 #pragma unroll
         for (int i = 0; i < R; ++i) {
             if (i >= rows) continue;
+            float x[V];
+            lo[i].get(x);
+            if constexpr (PAIRS2) {
 #pragma unroll
-            for (int j = 0; j < P; ++j) {
-                const int ja = PAIRS2 ? 2 * j : j, jb = PAIRS2 ? 2 * j + 1 : j;
-                RotVec<T, V>& other = PAIRS2 ? lo[i] : hi[i];
-                float x = lo[i].get(ja), y = other.get(jb);
-                rot_pair(x, y, c[j], s[j]);
-                lo[i].set(ja, x);
-                other.set(jb, y);
+                for (int j = 0; j < P; ++j) rot_pair(x[2 * j], x[2 * j + 1], c[j], s[j]);
+            } else {
+                float y[V];
+                hi[i].get(y);
+#pragma unroll
+                for (int j = 0; j < P; ++j) rot_pair(x[j], y[j], c[j], s[j]);
+                hi[i].set(y);
             }
+            lo[i].set(x);
         }
     }
 #pragma unroll
