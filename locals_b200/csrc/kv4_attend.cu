@@ -49,7 +49,9 @@ __device__ __forceinline__ uint32_t kv4_transpose(uint32_t x) {
     return y;
 }
 
-template <int R>
+// What an item costs beside its steps (pages and queries fetched, the ring filled, the warps joined), in steps.
+constexpr int KV4_ITEM = 2;
+
 __device__ __forceinline__ Kv4Req kv4_request(const Kv4AttArgs& a, int b) {
     Kv4Req r = kv4_new(a, b);
     if (r.fresh * a.G > a.split_rows) r.fresh = 0;  // (kv4_prefill's)
@@ -58,24 +60,35 @@ __device__ __forceinline__ Kv4Req kv4_request(const Kv4AttArgs& a, int b) {
     const int lo = a.window ? max(0, r.len - r.fresh + 1 - a.window) : 0;
     r.s_lo = min(lo, keys) / KV4_STEP;
     r.s_hi = max((keys + KV4_STEP - 1) / KV4_STEP, r.s_lo + 1);  // (a step at least: what sees nothing is written too)
-    r.tiles = (r.fresh * a.G + R - 1) / R;
     return r;
 }
 
 // Steps of all of request b's items.
-template <int R>
 __device__ __forceinline__ int kv4_weight(const Kv4AttArgs& a, int b) {
-    const Kv4Req r = kv4_request<R>(a, b);
-    return r.tiles * r.steps() * a.pool.KVH;
+    if (b >= a.B) return 0;
+    const Kv4Req r = kv4_request(a, b);
+    return r.fresh ? (r.steps() + KV4_ITEM) * a.pool.KVH : 0;
 }
 
-// Sum over the CTA's 128 threads (every thread gets it).
-__device__ __forceinline__ int kv4_sum(int v, int* red) {
-    v = __reduce_add_sync(0xffffffffu, v);
+// Inclusive sum over the CTA's 128 threads, and their total.
+__device__ __forceinline__ int kv4_scan(int v, int* red, int* total) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+        const int u = __shfl_up_sync(0xffffffffu, v, d);
+        if (lane >= d) v += u;
+    }
+    __syncthreads();  // (red may still be read from before)
+    if (lane == 31) red[warp] = v;
     __syncthreads();
-    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
-    __syncthreads();
-    return red[0] + red[1] + red[2] + red[3];
+    int sum = 0;
+#pragma unroll
+    for (int k = 0; k < KV4_NW; ++k) {
+        if (k == warp) v += sum;
+        sum += red[k];
+    }
+    *total = sum;
+    return v;
 }
 
 template <int D>
@@ -133,7 +146,7 @@ __global__ void __launch_bounds__(KV4_NW * 32, kv4_resident(D, NT)) kv4_attend_k
     using S = Kv4Shape<D>;
     constexpr int GR = S::GR, R = 8 * NT;
     extern __shared__ __align__(128) uint8_t kv4_smem[];
-    __shared__ int red[KV4_NW];
+    __shared__ int red[KV4_NW], found[2];
     grid_dep_wait();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gid = lane >> 2, c = lane & 3;
     const int tid = threadIdx.x, KVH = a.pool.KVH, G = a.G;
@@ -141,187 +154,205 @@ __global__ void __launch_bounds__(KV4_NW * 32, kv4_resident(D, NT)) kv4_attend_k
     kv4_zero_tail(a, D);
 
     // ---- this CTA's share of the steps: requests are scanned 128 at a time ----
-    long long total = 0;
-    for (int b0 = 0; b0 < a.B; b0 += KV4_NW * 32) total += kv4_sum(b0 + tid < a.B ? kv4_weight<R>(a, b0 + tid) : 0, red);
+    const int w0 = kv4_weight(a, tid);
+    int sum0;
+    const int s0 = kv4_scan(w0, red, &sum0);
+    long long total = sum0;
+    for (int b0 = KV4_NW * 32; b0 < a.B; b0 += KV4_NW * 32) {
+        int sum;
+        kv4_scan(kv4_weight(a, b0 + tid), red, &sum);
+        total += sum;
+    }
     const int n = int(min((long long)gridDim.x, total));  // (every CTA below n has a step, those above none)
+    int32_t* rec = a.records + blockIdx.x * 8;  // what the join kernel does for this CTA's first step
+    if (tid == 0) rec[0] = 0;
     if (int(blockIdx.x) >= n) return;
     const long long x0 = (long long)blockIdx.x * total / n, x1 = ((long long)blockIdx.x + 1) * total / n;
     int b = 0;
     long long at = 0;  // steps before request b
     for (int b0 = 0;; b0 += KV4_NW * 32) {
-        const int w = b0 + tid < a.B ? kv4_weight<R>(a, b0 + tid) : 0;
-        const int sum = kv4_sum(w, red);
+        int sum = sum0, s = s0, w = w0;
+        if (b0) {
+            w = kv4_weight(a, b0 + tid);
+            s = kv4_scan(w, red, &sum);
+        }
         if (at + sum <= x0) {
             at += sum;
             continue;
         }
-        // inclusive sums within the 128, then the first request whose steps reach past x0
-        int s = w;
-#pragma unroll
-        for (int d = 1; d < 32; d <<= 1) {
-            const int u = __shfl_up_sync(0xffffffffu, s, d);
-            if (lane >= d) s += u;
-        }
+        if (at + s > x0 && at + s - w <= x0) found[0] = b0 + tid, found[1] = s - w;  // one thread's
         __syncthreads();
-        if (lane == 31) red[warp] = s;
-        __syncthreads();
-        for (int k = 0; k < warp; ++k) s += red[k];
-        const bool past = at + s > x0;
-        const int before = kv4_sum(past ? 0 : 1, red);  // (sums ascend: these come first)
-        const int skipped = kv4_sum(past ? 0 : w, red);
-        b = b0 + before;
-        at += skipped;
+        b = found[0];
+        at += found[1];
         break;
     }
 
     const uint32_t ring = smem_u32(kv4_smem) + warp * S::WARP;
-    const uint32_t made = ring + S::STAGES * S::STAGE;  // the step's floats: ks, kb, vs', vb' (GR each) a key
+    const uint32_t made = ring + S::STAGES * S::STAGE;  // the step's floats: ks', kb, vs', vb' (GR each) a key
     const uint32_t zeds = made + KV4_KEYS * S::FL * 4;  // and its z, 2 bytes each: (group, chunk, place in the MMA's order)
+    // places in a stage that this lane reads: keys p8(gid) (+ 8) of a chunk and its floats, values p8(2c), p8(2c + 1) (+ 8)
+    uint32_t k_at[GR], va_at[GR], vb_at[GR];
+#pragma unroll
+    for (int g = 0; g < GR; ++g) {
+        k_at[g] = kv4_p8(gid) * S::RB + (kv4_swz<D>(kv4_p8(gid), g) << 5) + 8 * c;
+        va_at[g] = S::KV_BYTES + kv4_p8(2 * c) * S::RB + (kv4_swz<D>(kv4_p8(2 * c), g) << 5) + 4 * gid;
+        vb_at[g] = S::KV_BYTES + kv4_p8(2 * c + 1) * S::RB + (kv4_swz<D>(kv4_p8(2 * c + 1), g) << 5) + 4 * gid;
+    }
+    const uint32_t f_at = made + kv4_p8(gid) * S::FL * 4;
+    // this lane's place of z: key lane
+    const uint32_t z_at = zeds + (lane >> 4) * 32 + (kv4_p8_inv(lane & 7) >> 1) * 8 + ((lane >> 3) & 1) * 4 + (kv4_p8_inv(lane & 7) & 1) * 2;
+
     long long x = x0;
     while (x < x1) {
-        Kv4Req rq = kv4_request<R>(a, b);
-        const int item = int((x - at) / max(rq.steps(), 1));
-        if (rq.tiles == 0 || item >= rq.tiles * KVH) {  // on to the next request
-            at += (long long)rq.tiles * rq.steps() * KVH;
+        const Kv4Req rq = kv4_request(a, b);
+        const int units = rq.steps() + KV4_ITEM;
+        const int kvh = int((x - at) / units);
+        if (!rq.fresh || kvh >= KVH) {  // on to the next request
+            if (rq.fresh) at += (long long)units * KVH;
             ++b;
             continue;
         }
-        const int kvh = item / rq.tiles, row0 = (item - kvh * rq.tiles) * R;
-        const long long item_at = at + (long long)item * rq.steps();
-        const int st0 = int(x - item_at), st1 = int(min((long long)rq.steps(), x1 - item_at));
-        x = item_at + st1;
-        const int rows = min(R, rq.fresh * G - row0);
-        // what the tile's rows see: keys below hi_max, from lo_min on; all of them see [lo_max, hi_min)
+        const long long item_at = at + (long long)kvh * units;
+        const int u1 = int(min((long long)units, x1 - item_at));
+        const int st0 = max(int(x - item_at) - KV4_ITEM, 0), st1 = max(u1 - KV4_ITEM, 0);
+        x = item_at + u1;
+        if (st0 == st1) continue;
+        if (st0 > 0 && tid == 0) {  // (only a CTA's first item can begin before it)
+            const long long key0 = item_at + KV4_ITEM;
+            rec[1] = rq.first;
+            rec[2] = rq.fresh * G;
+            rec[3] = kvh;
+            rec[4] = kv4_owner(key0 + rq.steps() - 1, total, n);
+            rec[0] = kv4_owner(key0, total, n) == int(blockIdx.x) - 1;  // the first boundary within its item
+        }
+        const int rows = rq.fresh * G;
+        // what the rows see: keys below hi_max, from lo_min on; all of them see [lo_max, hi_min)
         const int base = rq.len - rq.fresh;  // position of query 0
         const int room = int(min((long long)a.width * a.pool.page, 0x7fffffffLL));
         if (rq.len > room) record_status(LQ_DEV_BOUNDS);
-        const int hi_min = min(base + row0 / G + 1, room), hi_max = min(base + (row0 + rows - 1) / G + 1, room);
-        const int lo_min = a.window ? max(base + row0 / G + 1 - a.window, 0) : 0;
-        const int lo_max = a.window ? max(base + (row0 + rows - 1) / G + 1 - a.window, 0) : 0;
+        const int hi_min = min(base + 1, room), hi_max = min(rq.len, room);
+        const int lo_min = a.window ? max(base + 1 - a.window, 0) : 0, lo_max = a.window ? max(rq.len - a.window, 0) : 0;
         const int k_lo = max((rq.s_lo + st0) * KV4_STEP, lo_min / KV4_KEYS * KV4_KEYS);
         const int k_hi = min((rq.s_lo + st1) * KV4_STEP, hi_max);
         // this warp's 32-key steps: first, first + 128, ...
         const int first = ((k_lo + KV4_STEP - 1 - warp * KV4_KEYS) / KV4_STEP) * KV4_STEP + warp * KV4_KEYS;
         const int steps = k_hi > first ? (k_hi - first + KV4_STEP - 1) / KV4_STEP : 0;
 
-        // lane l's page lookup: run l & 3 of 8 keys of step t0 + (l >> 2)
-        auto lookup = [&](int t0) -> uint32_t {
+        // lane l's page lookup: run l & 3 (of 8 keys) of step t0 + (l >> 2); row 0 where there is none. miss: bit l, the
+        // run is within the range but has no page
+        auto lookup = [&](int t0, uint32_t* miss) -> uint32_t {
             const int key = first + (t0 + (lane >> 2)) * KV4_STEP + (lane & 3) * 8;
-            if (t0 + (lane >> 2) >= steps || key >= hi_max) return KV4_NONE;
-            const int pg = key / a.pool.page;
-            const int id = a.table[(size_t)b * a.width + pg];
-            if (unsigned(id) >= unsigned(a.pool.pages)) {
-                record_status(LQ_DEV_BOUNDS);
-                return KV4_NONE;
+            uint32_t row = 0;
+            bool gone = false;
+            if (t0 + (lane >> 2) < steps && key < hi_max) {
+                const int pg = key / a.pool.page, id = a.table[(size_t)b * a.width + pg];
+                gone = unsigned(id) >= unsigned(a.pool.pages);
+                if (gone)
+                    record_status(LQ_DEV_BOUNDS);
+                else
+                    row = kv4_row(a.pool, id, kvh, key - pg * a.pool.page);
             }
-            return kv4_row(a.pool, id, kvh, key - pg * a.pool.page);
+            *miss = __ballot_sync(0xffffffffu, gone);
+            return row;
         };
-        uint32_t runs = lookup(0), runs_next = lookup(8);
-        // bit 4 (t & 7) + r: run r of step t is within the range but has no page (of the steps computed, and issued)
-        auto missing = [&](int t0, uint32_t held) -> uint32_t {
-            const int key = first + (t0 + (lane >> 2)) * KV4_STEP + (lane & 3) * 8;
-            return __ballot_sync(0xffffffffu, held == KV4_NONE && t0 + (lane >> 2) < steps && key < hi_max);
-        };
-        uint32_t miss_now = missing(0, runs), miss_issued = miss_now;
+        uint32_t miss_now, miss_next, miss_issued;  // of the steps computed, looked up, and issued
+        uint32_t runs = lookup(0, &miss_now), runs_next = lookup(8, &miss_next);
+        miss_issued = miss_now;
 
-        // ---- queries: fp16 B fragments times a row's power of two, and the group sums of what the MMA sees ----
-        uint32_t qb[NT][GR][2][2][2];
-        float alpha[NT][2], qs[NT][GR][2];
-        int col_hi[NT][2], col_lo[NT][2];
-#pragma unroll
-        for (int t = 0; t < NT; ++t) {
-            const int row = row0 + 8 * t + gid;
-            const bool live = 8 * t + gid < rows;
-            const int qi = live ? row / G : 0, hd = kvh * G + (live ? row - qi * G : 0);
-            const uint4* src = reinterpret_cast<const uint4*>(a.q + ((size_t)(rq.first + qi) * a.H + hd) * D);
-            float mx = 0.0f;
-            uint4 raw[GR][2];
-#pragma unroll
-            for (int g = 0; g < GR; ++g)
-#pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                    raw[g][u] = live ? src[8 * g + 2 * c + u] : make_uint4(0, 0, 0, 0);
-                    const uint32_t* w = reinterpret_cast<const uint32_t*>(&raw[g][u]);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        mx = fmaxf(mx, fmaxf(fabsf(F16Traits<T>::to_f32(w[i] & 0xffffu)),
-                                             fabsf(F16Traits<T>::to_f32(w[i] >> 16))));
-                }
-            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-            // 2^E with the row's largest |q| at 2^13 .. 2^14
-            int E = mx > 0.0f ? 13 - (int((__float_as_uint(mx) >> 23) & 0xff) - 127) : 0;
-            E = min(max(E, -100), 100);
-            const float f = __uint_as_float(uint32_t(127 + E) << 23);
-            float sums[GR];
-#pragma unroll
-            for (int g = 0; g < GR; ++g) {
-                sums[g] = 0.0f;
-#pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                    const uint32_t* w = reinterpret_cast<const uint32_t*>(&raw[g][u]);
-                    float v[8];
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        v[2 * i] = __half2float(__float2half_rn(F16Traits<T>::to_f32(w[i] & 0xffffu) * f));
-                        v[2 * i + 1] = __half2float(__float2half_rn(F16Traits<T>::to_f32(w[i] >> 16) * f));
-                    }
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) sums[g] += v[i];
-#pragma unroll
-                    for (int m = 0; m < 2; ++m) {
-                        qb[t][g][u][m][0] = cvt_f16x2(v[2 * m + 4], v[2 * m]);
-                        qb[t][g][u][m][1] = cvt_f16x2(v[2 * m + 5] * 0.0625f, v[2 * m + 1] * 0.0625f);
-                    }
-                }
-                sums[g] += __shfl_xor_sync(0xffffffffu, sums[g], 1);
-                sums[g] += __shfl_xor_sync(0xffffffffu, sums[g], 2);
-            }
-            const float back = a.scale_log2 * __uint_as_float(uint32_t(127 - E) << 23);
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {  // this lane's columns 2c + e of the score tile
-                const int from = (2 * c + e) * 4;
-                const float bk = __shfl_sync(0xffffffffu, back, from);
-                alpha[t][e] = bk * 16777216.0f;
-#pragma unroll
-                for (int g = 0; g < GR; ++g) qs[t][g][e] = bk * __shfl_sync(0xffffffffu, sums[g], from);
-                const int r = 8 * t + 2 * c + e, p = base + (row0 + min(r, rows - 1)) / G + 1;
-                col_hi[t][e] = min(p, room);
-                col_lo[t][e] = a.window ? max(p - a.window, 0) : 0;
-            }
-        }
-
-        // ---- the ring ----
-        auto issue = [&](int t, uint32_t lanes_runs) {
-            const uint32_t sb = ring + (t % S::STAGES) * S::STAGE;
+        // ---- the ring: a step's codes, scales and biases into its stage (a run without a page reads row 0, unused) ----
+        auto issue = [&](int t, uint32_t sb) {
             constexpr int PIECES = S::RB / 16;  // 16-byte pieces a key
             constexpr int J = KV4_KEYS * PIECES / 32;
             const int sel = (t & 7) * 4;
 #pragma unroll
             for (int j = 0; j < J; ++j) {
                 const int e = lane + 32 * j, r = e / PIECES, p = e % PIECES;
-                const uint32_t rb = __shfl_sync(0xffffffffu, lanes_runs, sel + r / 8);
-                const bool ok = rb != KV4_NONE;
-                const size_t row = ok ? rb + (r & 7) : 0;
+                const size_t from = size_t(__shfl_sync(0xffffffffu, runs, sel + r / 8)) * S::RB + (r & 7) * S::RB + p * 16;
                 const uint32_t off = r * S::RB + (kv4_swz<D>(r, p >> 1) << 5) + ((p & 1) << 4);
-                cp_async(sb + off, reinterpret_cast<const uint8_t*>(a.pool.kq) + row * S::RB + p * 16, 16, ok);
-                cp_async(sb + S::KV_BYTES + off, reinterpret_cast<const uint8_t*>(a.pool.vq) + row * S::RB + p * 16, 16, ok);
+                cp_async(sb + off, reinterpret_cast<const uint8_t*>(a.pool.kq) + from, 16, true);
+                cp_async(sb + S::KV_BYTES + off, reinterpret_cast<const uint8_t*>(a.pool.vq) + from, 16, true);
             }
             // scales and biases: a key's four arrays side by side (two keys' for one group: a pair of 2-byte values)
             constexpr int PK = D == 64 ? 2 : 1, BY = D == 256 ? 8 : 4;
             const int r = (lane % (KV4_KEYS / PK)) * PK;
-            const uint32_t rb = __shfl_sync(0xffffffffu, lanes_runs, sel + r / 8);
-            const bool ok = rb != KV4_NONE;
-            const size_t row = (ok ? rb + (r & 7) : 0) * GR;
+            const size_t row = size_t(__shfl_sync(0xffffffffu, runs, sel + r / 8) + (r & 7)) * GR;
             const uint32_t dst = sb + 2 * S::KV_BYTES + r * S::SC;
             if (D != 64 || lane < 16) {
-                cp_async(dst, a.pool.ks + row, BY, ok);
-                cp_async(dst + BY, a.pool.kb + row, BY, ok);
-                cp_async(dst + 2 * BY, a.pool.vs + row, BY, ok);
-                cp_async(dst + 3 * BY, a.pool.vb + row, BY, ok);
+                cp_async(dst, a.pool.ks + row, BY, true);
+                cp_async(dst + BY, a.pool.kb + row, BY, true);
+                cp_async(dst + 2 * BY, a.pool.vs + row, BY, true);
+                cp_async(dst + 3 * BY, a.pool.vb + row, BY, true);
             }
         };
         auto commit = [] { asm volatile("cp.async.commit_group;" ::: "memory"); };
+#pragma unroll
+        for (int t = 0; t < S::STAGES - 1; ++t) {
+            if (t < steps) issue(t, ring + t * S::STAGE);
+            commit();
+        }
+
+        // ---- queries: fp16 B fragments times one power of two, and the group sums of what the MMA sees ----
+        uint32_t qb[NT][GR][2][2][2];
+        float qs[NT][GR][2], alpha;
+        {
+            uint4 raw[NT][GR][2];
+            float mx = 0.0f;
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+                const int row = 8 * t + gid, qi = row / G;
+                const uint4* src = reinterpret_cast<const uint4*>(a.q + ((size_t)(rq.first + qi) * a.H + kvh * G + row - qi * G) * D);
+#pragma unroll
+                for (int g = 0; g < GR; ++g)
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) raw[t][g][u] = row < rows ? src[8 * g + 2 * c + u] : make_uint4(0, 0, 0, 0);
+            }
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+                for (int g = 0; g < GR; ++g)
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) {
+                        const uint32_t* w = reinterpret_cast<const uint32_t*>(&raw[t][g][u]);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            mx = fmaxf(mx, fmaxf(fabsf(F16Traits<T>::to_f32(w[i] & 0xffffu)),
+                                                 fabsf(F16Traits<T>::to_f32(w[i] >> 16))));
+                    }
+            // 2^E with the largest |q| at 2^13 .. 2^14
+            const uint32_t mb = __reduce_max_sync(0xffffffffu, __float_as_uint(mx));
+            const int E = min(max(mb ? 13 - (int(mb >> 23) - 127) : 0, -100), 100);
+            const float f = __uint_as_float(uint32_t(127 + E) << 23);
+            const float back = a.scale_log2 * __uint_as_float(uint32_t(127 - E) << 23);
+            alpha = back * 16777216.0f;
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+                for (int g = 0; g < GR; ++g) {
+                    float sum = 0.0f;
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) {
+                        const uint32_t* w = reinterpret_cast<const uint32_t*>(&raw[t][g][u]);
+                        float v[8];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            v[2 * i] = __half2float(__float2half_rn(F16Traits<T>::to_f32(w[i] & 0xffffu) * f));
+                            v[2 * i + 1] = __half2float(__float2half_rn(F16Traits<T>::to_f32(w[i] >> 16) * f));
+                        }
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) sum += v[i];
+#pragma unroll
+                        for (int m = 0; m < 2; ++m) {
+                            qb[t][g][u][m][0] = cvt_f16x2(v[2 * m + 4], v[2 * m]);
+                            qb[t][g][u][m][1] = cvt_f16x2(v[2 * m + 5] * 0.0625f, v[2 * m + 1] * 0.0625f);
+                        }
+                    }
+                    sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+                    sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+#pragma unroll
+                    for (int e = 0; e < 2; ++e)  // this lane's columns 2c + e of the score tile
+                        qs[t][g][e] = back * __shfl_sync(0xffffffffu, sum, (2 * c + e) * 4);
+                }
+        }
 
         float o[NT][4 * GR][4], hb[NT][GR][2], m[NT][2], l[NT][2];
 #pragma unroll
@@ -339,32 +370,38 @@ __global__ void __launch_bounds__(KV4_NW * 32, kv4_resident(D, NT)) kv4_attend_k
         }
         float vf = 1.0f;       // the value scales' power of two
         uint32_t v_limit = 0;  // bits of the largest value scale that it fits (0: none met yet)
-
+        // o and hb by f0 (even columns) and f1
+        auto rescale = [&](int t, float f0, float f1) {
 #pragma unroll
-        for (int t = 0; t < S::STAGES - 1; ++t) {
-            if (t < steps) issue(t, runs);
-            commit();
-        }
+            for (int i = 0; i < 4 * GR; ++i) {
+                o[t][i][0] *= f0;
+                o[t][i][1] *= f1;
+                o[t][i][2] *= f0;
+                o[t][i][3] *= f1;
+            }
+#pragma unroll
+            for (int g = 0; g < GR; ++g) hb[t][g][0] *= f0, hb[t][g][1] *= f1;
+        };
+
+        uint32_t sb = ring, sb_issue = ring + (S::STAGES - 1) * S::STAGE;
         for (int t = 0; t < steps; ++t) {
             const int nx = t + S::STAGES - 1;
             if (nx < steps) {
                 if ((nx & 7) == 0) {
                     runs = runs_next;
-                    miss_issued = missing(nx, runs);
-                    runs_next = lookup(nx + 8);
+                    miss_issued = miss_next;
+                    runs_next = lookup(nx + 8, &miss_next);
                 }
-                issue(nx, runs);
+                issue(nx, sb_issue);
             }
-            if ((t & 7) == 0) miss_now = miss_issued;
             commit();
+            if ((t & 7) == 0) miss_now = miss_issued;
             asm volatile("cp.async.wait_group %0;" ::"n"(S::STAGES - 1) : "memory");
             __syncwarp();
-            const uint32_t sb = ring + (t % S::STAGES) * S::STAGE;
             const int key0 = first + t * KV4_STEP;
-            const bool inside = key0 >= lo_max && key0 + KV4_KEYS <= hi_min;
 
-
-            // one key a lane: its scales and biases in fp32, and the values' z; a key out of range has none
+            // one key a lane: its scales and biases in fp32, and the values' z. A key out of range has none; one whose
+            // values are not finite has none either and a NaN for its key, which only the rows that see it meet.
             const uint32_t miss = (miss_now >> ((t & 7) * 4)) & 0xfu;  // runs of 8 keys whose page is missing
             {
                 float w[4][GR];  // ks, kb, vs, vb
@@ -378,61 +415,48 @@ __global__ void __launch_bounds__(KV4_NW * 32, kv4_resident(D, NT)) kv4_attend_k
 #pragma unroll
                     for (int i = 0; i < GR / 2; ++i) {
                         const uint4 v = lds128(p + 16 * i);
-                        const uint32_t x[4] = {v.x, v.y, v.z, v.w};
+                        const uint32_t x4[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
                         for (int k = 0; k < 4; ++k) {  // D = 128: one word an array; D = 256: two
                             const int arr = D == 128 ? k : 2 * i + k / 2, g = D == 128 ? 0 : 2 * (k & 1);
-                            w[arr][g] = F16Traits<T>::to_f32(x[k] & 0xffffu);
-                            w[arr][g + 1] = F16Traits<T>::to_f32(x[k] >> 16);
+                            w[arr][g] = F16Traits<T>::to_f32(x4[k] & 0xffffu);
+                            w[arr][g + 1] = F16Traits<T>::to_f32(x4[k] >> 16);
                         }
                     }
+                }
+                float top = 0.0f, most = 0.0f;
+#pragma unroll
+                for (int g = 0; g < GR; ++g) {
+                    top = fmaxf(top, fabsf(w[2][g]));
+                    most += fabsf(w[2][g]) + fabsf(w[3][g]);
                 }
                 const int key = key0 + lane;
-                if (key < lo_min || key >= hi_max || ((miss >> (lane >> 3)) & 1)) {
+                const bool dead = key < lo_min || key >= hi_max || ((miss >> (lane >> 3)) & 1);
+                if (dead || !(most < INFINITY)) {
+                    top = 0.0f;
 #pragma unroll
-                    for (int g = 0; g < GR; ++g) w[2][g] = 0.0f, w[3][g] = 0.0f;
+                    for (int g = 0; g < GR; ++g) w[0][g] = __int_as_float(0x7fffffff), w[2][g] = 0.0f, w[3][g] = 0.0f;
                 }
                 // the value scales' power of two: larger scales are met by a smaller one
-                float top = 0.0f;
-#pragma unroll
-                for (int g = 0; g < GR; ++g) top = fmaxf(top, fabsf(w[2][g]));
-                uint32_t bits = __reduce_max_sync(0xffffffffu, __float_as_uint(top));
+                const uint32_t bits = __reduce_max_sync(0xffffffffu, __float_as_uint(top));
                 if (bits > v_limit) {
-                    if (bits >= 0x7f800000u) {  // an infinite scale: go by the finite ones
-                        top = 0.0f;
+                    const int E = max(int(bits >> 23), 64);  // (at least 2^-63)
+                    const float nf = __uint_as_float(uint32_t(127 + 5 + 127 - E) << 23);  // to 2^5 .. 2^6
 #pragma unroll
-                        for (int g = 0; g < GR; ++g)
-                            if (fabsf(w[2][g]) < INFINITY) top = fmaxf(top, fabsf(w[2][g]));
-                        bits = __reduce_max_sync(0xffffffffu, __float_as_uint(top));
-                    }
-                    if (bits > v_limit) {
-                        const int E = max(int(bits >> 23), 64);  // (at least 2^-63)
-                        const float nf = __uint_as_float(uint32_t(127 + 9 + 127 - E) << 23);  // to 2^9 .. 2^10
-                        const float ratio = nf / vf;
-#pragma unroll
-                        for (int tt = 0; tt < NT; ++tt) {
-#pragma unroll
-                            for (int i = 0; i < 4 * GR; ++i)
-#pragma unroll
-                                for (int u = 0; u < 4; ++u) o[tt][i][u] *= ratio;
-#pragma unroll
-                            for (int g = 0; g < GR; ++g) hb[tt][g][0] *= ratio, hb[tt][g][1] *= ratio;
-                        }
-                        vf = nf;
-                        v_limit = (uint32_t(E + 5) << 23) - 1;  // below 2^14 / vf
-                    }
+                    for (int tt = 0; tt < NT; ++tt) rescale(tt, nf / vf, nf / vf);
+                    vf = nf;
+                    v_limit = (uint32_t(E + 5) << 23) - 1;  // below 2^10 / vf
                 }
                 float f[S::FL];
 #pragma unroll
                 for (int g = 0; g < GR; ++g) {
-                    const float z = fminf(fmaxf(rintf(__fdividef(-w[3][g], w[2][g])), 0.0f), 15.0f);
-                    f[g] = w[0][g];
+                    // round(-vb / vs) in 0 .. 15, its bits the last of 1.5 * 2^23 + z
+                    const float u = fminf(fmaxf(__fdividef(-w[3][g], w[2][g]), 0.0f), 15.0f) + 12582912.0f;
+                    f[g] = w[0][g] * alpha;
                     f[GR + g] = w[1][g];
                     f[2 * GR + g] = w[2][g] * vf;
-                    f[3 * GR + g] = fmaf(z, w[2][g], w[3][g]) * vf;
-                    asm volatile("st.shared.u16 [%0], %1;" ::"r"(zeds + ((g * 2 + (lane >> 4)) * 16 + (lane & 8) + kv4_p8_inv(lane & 7)) * 2),
-                                 "h"(uint16_t(z))
-                                 : "memory");
+                    f[3 * GR + g] = fmaf(u - 12582912.0f, w[2][g], w[3][g]) * vf;
+                    asm volatile("st.shared.u16 [%0], %1;" ::"r"(z_at + g * 64), "h"(uint16_t(__float_as_uint(u) & 15u)) : "memory");
                 }
 #pragma unroll
                 for (int i = 0; i < S::FL; i += 4)
@@ -453,128 +477,123 @@ __global__ void __launch_bounds__(KV4_NW * 32, kv4_resident(D, NT)) kv4_attend_k
                     for (int g = 0; g < GR; ++g)
 #pragma unroll
                         for (int u = 0; u < 4; ++u) acc[tt][g][u] = 0.0f;
-                const int r0 = 16 * h + kv4_p8(gid), r1 = r0 + 8;
 #pragma unroll
                 for (int g = 0; g < GR; ++g) {
+                    const uint32_t p = sb + k_at[g] + h * 16 * S::RB;
                     uint32_t xw[2], yw[2];
-                    asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];"
-                                 : "=r"(xw[0]), "=r"(xw[1])
-                                 : "r"(sb + r0 * S::RB + (kv4_swz<D>(r0, g) << 5) + 8 * c));
-                    asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];"
-                                 : "=r"(yw[0]), "=r"(yw[1])
-                                 : "r"(sb + r1 * S::RB + (kv4_swz<D>(r1, g) << 5) + 8 * c));
+                    asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(xw[0]), "=r"(xw[1]) : "r"(p));
+                    asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(yw[0]), "=r"(yw[1]) : "r"(p + 8 * S::RB));
 #pragma unroll
                     for (int u = 0; u < 2; ++u)
 #pragma unroll
                         for (int mm = 0; mm < 2; ++mm) {
                             const uint32_t xs = mm ? xw[u] >> 8 : xw[u], ys = mm ? yw[u] >> 8 : yw[u];
+                            const uint32_t a0 = xs & 0x000f000fu, a1 = ys & 0x000f000fu, a2 = xs & 0x00f000f0u, a3 = ys & 0x00f000f0u;
 #pragma unroll
                             for (int tt = 0; tt < NT; ++tt)
-                                mma_16816<__half>(acc[tt][g], xs & 0x000f000fu, ys & 0x000f000fu, xs & 0x00f000f0u,
-                                                  ys & 0x00f000f0u, qb[tt][g][u][mm][0], qb[tt][g][u][mm][1]);
+                                mma_16816<__half>(acc[tt][g], a0, a1, a2, a3, qb[tt][g][u][mm][0], qb[tt][g][u][mm][1]);
                         }
                 }
 #pragma unroll
                 for (int u = 0; u < 2; ++u) {
-                    float f[2 * GR];  // ks, kb
-                    kv4_floats<2 * GR>(made + (16 * h + 8 * u + kv4_p8(gid)) * S::FL * 4, f);
+                    float f[2 * GR];  // ks', kb
+                    kv4_floats<2 * GR>(f_at + (16 * h + 8 * u) * S::FL * 4, f);
 #pragma unroll
                     for (int tt = 0; tt < NT; ++tt)
 #pragma unroll
                         for (int e = 0; e < 2; ++e) {
-                            float dot = f[0] * acc[tt][0][2 * u + e];
+                            float s = f[GR] * qs[tt][0][e];
 #pragma unroll
-                            for (int g = 1; g < GR; ++g) dot = fmaf(f[g], acc[tt][g][2 * u + e], dot);
-                            float s = dot * alpha[tt][e];
+                            for (int g = 1; g < GR; ++g) s = fmaf(f[GR + g], qs[tt][g][e], s);
 #pragma unroll
-                            for (int g = 0; g < GR; ++g) s = fmaf(f[GR + g], qs[tt][g][e], s);
+                            for (int g = 0; g < GR; ++g) s = fmaf(f[g], acc[tt][g][2 * u + e], s);
                             sc[tt][h][u][e] = s;
                         }
                 }
             }
-            if (!inside || miss) {
+            if (key0 < lo_max || key0 + KV4_KEYS > hi_min || miss) {  // some row does not see some key
 #pragma unroll
-                for (int h = 0; h < 2; ++h)
+                for (int tt = 0; tt < NT; ++tt)
 #pragma unroll
-                    for (int u = 0; u < 2; ++u) {
-                        const int key = key0 + 16 * h + 8 * u + kv4_p8(gid);
-                        const bool gone = (miss >> (2 * h + u)) & 1;
+                    for (int e = 0; e < 2; ++e) {
+                        const int end = base + min(8 * tt + 2 * c + e, rows - 1) / G + 1;
+                        const int hi = min(end, room), lo = a.window ? max(end - a.window, 0) : 0;
 #pragma unroll
-                        for (int tt = 0; tt < NT; ++tt)
+                        for (int h = 0; h < 2; ++h)
 #pragma unroll
-                            for (int e = 0; e < 2; ++e)
-                                if (gone || key < col_lo[tt][e] || key >= col_hi[tt][e]) sc[tt][h][u][e] = -INFINITY;
+                            for (int u = 0; u < 2; ++u) {
+                                const int key = key0 + 16 * h + 8 * u + kv4_p8(gid);
+                                if (key < lo || key >= hi || ((miss >> (2 * h + u)) & 1)) sc[tt][h][u][e] = -INFINITY;
+                            }
                     }
             }
 
-            // running softmax a column (its 8 lanes agree on m)
+            // softmax: the reference m of a column (its 8 lanes agree on it) follows the maximum when that has grown by 2^4
+            bool grown = false;
+#pragma unroll
+            for (int tt = 0; tt < NT; ++tt)
+#pragma unroll
+                for (int e = 0; e < 2; ++e)
+                    grown = grown || fmaxf(fmaxf(sc[tt][0][0][e], sc[tt][0][1][e]), fmaxf(sc[tt][1][0][e], sc[tt][1][1][e])) >
+                                         m[tt][e] + 4.0f;
+            if (__any_sync(0xffffffffu, grown)) {
+#pragma unroll
+                for (int tt = 0; tt < NT; ++tt) {
+                    float corr[2];
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        float mx = fmaxf(fmaxf(sc[tt][0][0][e], sc[tt][0][1][e]), fmaxf(sc[tt][1][0][e], sc[tt][1][1][e]));
+                        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+                        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+                        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+                        mx = fmaxf(mx, m[tt][e]);
+                        corr[e] = mx == -INFINITY ? 1.0f : kv4_ex2(m[tt][e] - mx);
+                        m[tt][e] = mx;
+                        l[tt][e] *= corr[e];
+                    }
+                    rescale(tt, corr[0], corr[1]);
+                }
+            }
             uint32_t pb[NT][2][GR][2];
 #pragma unroll
-            for (int tt = 0; tt < NT; ++tt) {
-                float corr[2];
+            for (int tt = 0; tt < NT; ++tt)
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
-                    float mx = fmaxf(fmaxf(sc[tt][0][0][e], sc[tt][0][1][e]), fmaxf(sc[tt][1][0][e], sc[tt][1][1][e]));
-                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
-                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
-                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-                    const float mn = fmaxf(m[tt][e], mx), mz = mn == -INFINITY ? 0.0f : mn;
-                    corr[e] = kv4_ex2(m[tt][e] - mz);
-                    m[tt][e] = mn;
+                    const float mz = m[tt][e] == -INFINITY ? 0.0f : m[tt][e];
 #pragma unroll
                     for (int h = 0; h < 2; ++h)
 #pragma unroll
                         for (int u = 0; u < 2; ++u) sc[tt][h][u][e] = kv4_ex2(sc[tt][h][u][e] - mz);
-                    l[tt][e] = l[tt][e] * corr[e] + ((sc[tt][0][0][e] + sc[tt][0][1][e]) + (sc[tt][1][0][e] + sc[tt][1][1][e]));
+                    l[tt][e] += (sc[tt][0][0][e] + sc[tt][0][1][e]) + (sc[tt][1][0][e] + sc[tt][1][1][e]);
                 }
-                if (__any_sync(0xffffffffu, corr[0] != 1.0f || corr[1] != 1.0f)) {
-#pragma unroll
-                    for (int i = 0; i < 4 * GR; ++i) {
-                        o[tt][i][0] *= corr[0];
-                        o[tt][i][1] *= corr[1];
-                        o[tt][i][2] *= corr[0];
-                        o[tt][i][3] *= corr[1];
-                    }
-#pragma unroll
-                    for (int g = 0; g < GR; ++g) hb[tt][g][0] *= corr[0], hb[tt][g][1] *= corr[1];
-                }
-            }
 #pragma unroll
             for (int h = 0; h < 2; ++h)
 #pragma unroll
                 for (int u = 0; u < 2; ++u) {
                     float f[2 * GR];  // vs', vb'
-                    kv4_floats<2 * GR>(made + ((16 * h + 8 * u + kv4_p8(gid)) * S::FL + 2 * GR) * 4, f);
-                    const int key = key0 + 16 * h + 8 * u + kv4_p8(gid);
+                    kv4_floats<2 * GR>(f_at + ((16 * h + 8 * u) * S::FL + 2 * GR) * 4, f);
 #pragma unroll
                     for (int tt = 0; tt < NT; ++tt)
 #pragma unroll
                         for (int g = 0; g < GR; ++g) {
-                            float w[2];
-#pragma unroll
-                            for (int e = 0; e < 2; ++e) {
-                                w[e] = sc[tt][h][u][e] * f[g];
-                                float y = sc[tt][h][u][e] * f[GR + g];
-                                if (!inside && (key < col_lo[tt][e] || key >= col_hi[tt][e])) w[e] = 0.0f, y = 0.0f;
-                                hb[tt][g][e] += y;
-                            }
-                            pb[tt][h][g][u] = kv4_transpose(cvt_f16x2(w[1], w[0]));
+                            hb[tt][g][0] = fmaf(sc[tt][h][u][0], f[GR + g], hb[tt][g][0]);
+                            hb[tt][g][1] = fmaf(sc[tt][h][u][1], f[GR + g], hb[tt][g][1]);
+                            pb[tt][h][g][u] = kv4_transpose(cvt_f16x2(sc[tt][h][u][1] * f[g], sc[tt][h][u][0] * f[g]));
                         }
                 }
 
             // values: keys p8(2c), p8(2c + 1) (+ 8) of a chunk, dimensions 64 g + 8 gid + i
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                const int ra = 16 * h + kv4_p8(2 * c), rb = 16 * h + kv4_p8(2 * c + 1);
 #pragma unroll
                 for (int g = 0; g < GR; ++g) {
-                    const uint32_t pa = sb + S::KV_BYTES + ra * S::RB + (kv4_swz<D>(ra, g) << 5) + 4 * gid;
-                    const uint32_t pz = sb + S::KV_BYTES + rb * S::RB + (kv4_swz<D>(rb, g) << 5) + 4 * gid;
+                    const uint32_t pa = sb + va_at[g] + h * 16 * S::RB, pz = sb + vb_at[g] + h * 16 * S::RB;
                     const uint32_t wa = lds32(pa), wb = lds32(pz), wc = lds32(pa + 8 * S::RB), wd = lds32(pz + 8 * S::RB);
+                    uint32_t za, zc;
+                    asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(za), "=r"(zc) : "r"(zeds + (g * 2 + h) * 32 + 8 * c));
                     uint32_t ab[2], cd[2];
                     ab[0] = prmt(wa, wb, 0x5410u), ab[1] = prmt(wa, wb, 0x7632u);
                     cd[0] = prmt(wc, wd, 0x5410u), cd[1] = prmt(wc, wd, 0x7632u);
-                    const uint32_t za = lds32(zeds + (g * 2 + h) * 32 + 4 * c), zc = lds32(zeds + (g * 2 + h) * 32 + 16 + 4 * c);
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         const uint32_t xs = i & 1 ? ab[i >> 1] >> 8 : ab[i >> 1], ys = i & 1 ? cd[i >> 1] >> 8 : cd[i >> 1];
@@ -587,6 +606,8 @@ __global__ void __launch_bounds__(KV4_NW * 32, kv4_resident(D, NT)) kv4_attend_k
                 }
             }
             __syncwarp();
+            sb = sb == ring + (S::STAGES - 1) * S::STAGE ? ring : sb + S::STAGE;
+            sb_issue = sb_issue == ring + (S::STAGES - 1) * S::STAGE ? ring : sb_issue + S::STAGE;
         }
         asm volatile("cp.async.wait_group 0;" ::: "memory");
         if (x >= x1) grid_dep_launch();
@@ -634,7 +655,7 @@ __global__ void __launch_bounds__(KV4_NW * 32, kv4_resident(D, NT)) kv4_attend_k
                 f[w] = cm[w * R + j] == -INFINITY ? 0.0f : kv4_ex2(cm[w * R + j] - M);
                 L += cl[w * R + j] * f[w];
             }
-            const int qi = (row0 + j) / G, head = kvh * G + (row0 + j) - qi * G;
+            const int qi = j / G, head = kvh * G + j - qi * G;
             for (int d = tid; d < D; d += KV4_NW * 32) {
                 float O = 0.0f;
 #pragma unroll
@@ -651,28 +672,19 @@ __global__ void __launch_bounds__(KV4_NW * 32, kv4_resident(D, NT)) kv4_attend_k
     }
 }
 
-// One CTA a (request, kv head, row of the request's tiles): the parts of an item that several CTAs share, joined.
+// One CTA a (share, row): the parts of the item that a share's start divides, joined with the row's sink.
 template <typename T, int D, int NT>
 __global__ void __launch_bounds__(128) kv4_join_kernel(const Kv4AttArgs a) {
     constexpr int R = 8 * NT;
-    __shared__ int red[KV4_NW];
+    __shared__ float4 sum[4][D / 4];
+    __shared__ float4 sml[4];
     grid_dep_wait();
-    const int b = blockIdx.z, kvh = blockIdx.y, row = blockIdx.x, tile = row / R;
-    long long total = 0, at = 0;
-    for (int b0 = 0; b0 < a.B; b0 += 128) {
-        const int i = b0 + threadIdx.x, w = i < a.B ? kv4_weight<R>(a, i) : 0;
-        total += kv4_sum(w, red);
-        at += kv4_sum(i < b ? w : 0, red);
-    }
-    const int n = int(min((long long)a.ctas, total));
-    const Kv4Req rq = kv4_request<R>(a, b);
-    if (row >= rq.fresh * a.G) return;
-    const long long item = at + ((long long)kvh * rq.tiles + tile) * rq.steps();
-    const int c0 = kv4_owner(item, total, n), c1 = kv4_owner(item + rq.steps() - 1, total, n);
-    if (c0 == c1) return;  // one CTA had it whole
-    const int j = row - tile * R, qi = row / a.G, head = kvh * a.G + row - qi * a.G;
-    auto part = [&](int cta) { return ((size_t)cta * 2 + (cta == c0 ? 1 : 0)) * R + j; };
-    kv4_join_row<T, D>(a, part, c0, c1, kv4_sink(a.sinks, head), a.out + ((size_t)(rq.first + qi) * a.H + head) * D);
+    const int i = blockIdx.x, j = blockIdx.y, warp = threadIdx.x >> 5;
+    const int32_t* rec = a.records + i * 8;
+    if (!rec[0] || j >= rec[2]) return;
+    const int qi = j / a.G, head = rec[3] * a.G + j - qi * a.G;
+    kv4_join_row<T, D, 4>(a, R, j, i - 1, rec[4], warp, kv4_sink(a.sinks, head), a.out + ((size_t)(rec[1] + qi) * a.H + head) * D,
+                          sum, sml);
 }
 
 // ---- host ----------------------------------------------------------------------------------------
@@ -695,7 +707,7 @@ static void kv4_rows(int max_q, int G, int* R, int* split) {
 static int kv4_ctas(int D, int R, int sms) { return sms * kv4_resident(D, R / 8); }
 
 static size_t kv4_few_bytes(int D, int R, int sms) {
-    return (size_t(kv4_ctas(D, R, sms)) * 2 * R * (2 + D) * sizeof(float) + 255) / 256 * 256;
+    return size_t(kv4_ctas(D, R, sms)) * (2 * R * (2 + D) * sizeof(float) + 8 * sizeof(int32_t));
 }
 
 size_t kv4_prefill_workspace_bytes(int D, int sms);
@@ -714,11 +726,11 @@ static int kv4_attend_n(Kv4AttArgs a, cudaStream_t st) {
     constexpr int R = 8 * NT;
     constexpr size_t merge = size_t(KV4_NW) * R * (2 + D) * sizeof(float);
     constexpr size_t smem = merge > size_t(Kv4Shape<D>::RING) ? merge : size_t(Kv4Shape<D>::RING);
-    a.ctas = kv4_ctas(D, R, device_info().sm_count);
+    const int n = kv4_ctas(D, R, device_info().sm_count);
     static std::atomic<uint32_t> set{0}, none{0};
-    int rc = kv4_launch(kv4_attend_kernel<T, D, NT>, set, dim3(a.ctas), dim3(KV4_NW * 32), smem, st, a);
+    int rc = kv4_launch(kv4_attend_kernel<T, D, NT>, set, dim3(n), dim3(KV4_NW * 32), smem, st, a);
     if (rc) return rc;
-    return kv4_launch(kv4_join_kernel<T, D, NT>, none, dim3(a.split_rows, a.pool.KVH, a.B), dim3(128), 0, st, a);
+    return kv4_launch(kv4_join_kernel<T, D, NT>, none, dim3(n, a.split_rows), dim3(128), 0, st, a);
 }
 
 template <typename T, int D>
@@ -765,6 +777,7 @@ int kv4_attend_run(const Kv4Pool& pool, const void* q, int N, const int32_t* q_s
     }
     a.part_o = reinterpret_cast<float*>(ws);
     a.part_ml = a.part_o + size_t(kv4_ctas(D, R, sms)) * 2 * R * D;
+    a.records = reinterpret_cast<int32_t*>(a.part_ml + size_t(kv4_ctas(D, R, sms)) * 2 * R * 2);
     return dtype == LQ_BF16 ? kv4_attend_t<__nv_bfloat16>(a, D, R, st) : kv4_attend_t<__half>(a, D, R, st);
 }
 

@@ -31,7 +31,6 @@ struct Kv4AttArgs {
     int32_t* records;  // (CTA) x 8: the item that the start of a CTA's share divides
     float scale_log2;
     int N, B, H, G, width, window, max_q;
-    int ctas;        // CTAs that the steps are dealt out over (kv4_attend)
     int split_rows;  // requests of more rows are kv4_prefill's
 };
 
@@ -47,7 +46,7 @@ __device__ __forceinline__ float kv4_ex2(float x) {
 
 // A request's place in the step: its queries' first row, their number, its keys and the 128-key steps that they span.
 struct Kv4Req {
-    int first, fresh, len, s_lo, s_hi, tiles;
+    int first, fresh, len, s_lo, s_hi;
     __device__ __forceinline__ int steps() const { return s_hi - s_lo; }
 };
 
@@ -89,20 +88,80 @@ __device__ __forceinline__ uint16_t kv4_finish(float m, float l, float o, float 
     return F16Traits<T>::from_f32(L == 0.0f ? 0.0f : o * f / L);
 }
 
-// The parts of one row that CTAs c0 .. c1 hold (part(cta): their index), joined in that order by the CTA's 128 threads.
-template <typename T, int D, typename P>
-__device__ __forceinline__ void kv4_join_row(const Kv4AttArgs& a, P part, int c0, int c1, float sink, uint16_t* out) {
+// The parts of row j that CTAs c0 .. c1 hold (R rows a part; c0's is its second, the others' their first), joined by W
+// warps (this one: `warp`): each sums every W-th part, four at a time, a lane 4 dimensions, and the first adds them up in
+// order. sum, sml: W x D / 4 and W of shared memory (W = 1: unused).
+template <typename T, int D, int W>
+__device__ __forceinline__ void kv4_join_row(const Kv4AttArgs& a, int R, int j, int c0, int c1, int warp, float sink, uint16_t* out,
+                                             float4 (*sum)[D / 4], float4* sml) {
+    constexpr int V = (D + 127) / 128;  // float4s a lane (D = 64: half the lanes)
+    const int lane = threadIdx.x & 31;
+    const bool in = lane * 4 < D;
+    auto part = [&](int cta) { return ((size_t)cta * 2 + (cta == c0 ? 1 : 0)) * R + j; };
     float M = -INFINITY;
-    for (int cta = c0; cta <= c1; ++cta) M = fmaxf(M, a.part_ml[2 * part(cta)]);
-    for (int d = threadIdx.x; d < D; d += 128) {
-        float L = 0.0f, O = 0.0f;
-        for (int cta = c0; cta <= c1; ++cta) {
-            const size_t p = part(cta);
-            const float f = a.part_ml[2 * p] == -INFINITY ? 0.0f : kv4_ex2(a.part_ml[2 * p] - M);
-            L += a.part_ml[2 * p + 1] * f;
-            if (f != 0.0f) O += a.part_o[p * D + d] * f;
+    for (int p = c0 + lane; p <= c1; p += 32) M = fmaxf(M, a.part_ml[2 * part(p)]);
+#pragma unroll
+    for (int d = 16; d; d >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, d));
+    float4 O[V];
+    float L = 0.0f;
+#pragma unroll
+    for (int v = 0; v < V; ++v) O[v] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (int p0 = c0 + warp; p0 <= c1; p0 += 4 * W) {
+        float2 ml[4];
+        float4 o[4][V];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const int p = p0 + k * W;
+            ml[k] = make_float2(-INFINITY, 0.0f);
+#pragma unroll
+            for (int v = 0; v < V; ++v) o[k][v] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            if (p <= c1) {
+                const size_t at = part(p);
+                ml[k] = *reinterpret_cast<const float2*>(a.part_ml + 2 * at);
+                if (in) {
+#pragma unroll
+                    for (int v = 0; v < V; ++v) o[k][v] = *reinterpret_cast<const float4*>(a.part_o + at * D + v * 128 + lane * 4);
+                }
+            }
         }
-        out[d] = kv4_finish<T>(M, L, O, sink);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const float f = ml[k].x == -INFINITY ? 0.0f : kv4_ex2(ml[k].x - M);
+            L += ml[k].y == 0.0f ? 0.0f : ml[k].y * (ml[k].x == -INFINITY ? 1.0f : f);  // (l without an m is a NaN's)
+            if (f == 0.0f) continue;
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                O[v].x = fmaf(o[k][v].x, f, O[v].x), O[v].y = fmaf(o[k][v].y, f, O[v].y);
+                O[v].z = fmaf(o[k][v].z, f, O[v].z), O[v].w = fmaf(o[k][v].w, f, O[v].w);
+            }
+        }
+    }
+    if constexpr (W > 1) {
+        if (in) {
+#pragma unroll
+            for (int v = 0; v < V; ++v) sum[warp][v * 32 + lane] = O[v];
+        }
+        if (lane == 0) sml[warp].x = L;
+        __syncthreads();
+        if (warp) return;
+#pragma unroll
+        for (int w = 1; w < W; ++w) {
+            L += sml[w].x;
+            if (in) {
+#pragma unroll
+                for (int v = 0; v < V; ++v) {
+                    const float4 x = sum[w][v * 32 + lane];
+                    O[v].x += x.x, O[v].y += x.y, O[v].z += x.z, O[v].w += x.w;
+                }
+            }
+        }
+    }
+    if (!in) return;
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+        const uint32_t lo = kv4_finish<T>(M, L, O[v].x, sink) | uint32_t(kv4_finish<T>(M, L, O[v].y, sink)) << 16;
+        const uint32_t hi = kv4_finish<T>(M, L, O[v].z, sink) | uint32_t(kv4_finish<T>(M, L, O[v].w, sink)) << 16;
+        *reinterpret_cast<uint2*>(out + v * 128 + lane * 4) = make_uint2(lo, hi);
     }
 }
 

@@ -745,20 +745,16 @@ __global__ void __launch_bounds__(PF_THREADS, 1) kv4_prefill_kernel(const Kv4Att
     }
 }
 
-// One CTA a (share, 8 rows): the parts of the item that a share's start divides, joined with the rows' sinks.
+// One warp a (share, row): the parts of the item that a share's start divides, joined with the row's sink.
 template <typename T, int D>
 __global__ void __launch_bounds__(128) kv4_prefill_join_kernel(const Kv4AttArgs a) {
-    constexpr int R = PfShape<D>::R;
     grid_dep_wait();
-    const int i = blockIdx.x;
+    const int i = blockIdx.x, j = blockIdx.y * 4 + (threadIdx.x >> 5);
     const int32_t* rec = a.records + i * 8;
-    if (!rec[0]) return;
-    const int first = rec[1], row0 = rec[2], rows = rec[3], kvh = rec[4], c0 = i - 1, c1 = rec[5];
-    for (int j = blockIdx.y * 8; j < min(rows, int(blockIdx.y) * 8 + 8); ++j) {
-        const int qi = (row0 + j) / a.G, head = kvh * a.G + row0 + j - qi * a.G;
-        auto part = [&](int cta) { return ((size_t)cta * 2 + (cta == c0 ? 1 : 0)) * R + j; };
-        kv4_join_row<T, D>(a, part, c0, c1, kv4_sink(a.sinks, head), a.out + ((size_t)(first + qi) * a.H + head) * D);
-    }
+    if (!rec[0] || j >= rec[3]) return;
+    const int row = rec[2] + j, qi = row / a.G, head = rec[4] * a.G + row - qi * a.G;
+    kv4_join_row<T, D, 1>(a, PfShape<D>::R, j, i - 1, rec[5], 0, kv4_sink(a.sinks, head),
+                          a.out + ((size_t)(rec[1] + qi) * a.H + head) * D, nullptr, nullptr);
 }
 
 // ---- host ----------------------------------------------------------------------------------------
@@ -778,7 +774,7 @@ static int kv4_prefill_d(Kv4AttArgs a, void* workspace, cudaStream_t st) {
     static std::atomic<uint32_t> set{0}, none{0};
     int rc = kv4_launch(kv4_prefill_kernel<T, D>, set, dim3(n), dim3(PF_THREADS), S::SMEM + 1024 + sizeof(PfBars), st, a);
     if (rc) return rc;
-    return kv4_launch(kv4_prefill_join_kernel<T, D>, none, dim3(n, S::R / 8), dim3(128), 0, st, a);
+    return kv4_launch(kv4_prefill_join_kernel<T, D>, none, dim3(n, S::R / 4), dim3(128), 0, st, a);
 }
 
 int kv4_prefill_run(const Kv4AttArgs& a, int D, int dtype, void* workspace, cudaStream_t st) {
