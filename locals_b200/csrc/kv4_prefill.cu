@@ -653,36 +653,28 @@ __global__ void __launch_bounds__(PF_THREADS, 1) kv4_prefill_kernel(const Kv4Att
             step_out(now, it);
             h0 = h1;
         }
-    } else {
-        // ------------------------------ MMA issuer ------------------------------
+    } else if (lane == 0) {
+        // ------------------------------ MMA issuer: one thread ------------------------------
         constexpr uint32_t id_s = umma_idesc_f16(0, 128, KT);
         constexpr uint32_t id_o = umma_idesc_f16(0, 128, D) | (1u << 16);  // B's N side contiguous
         int it = 0, used[2] = {0, 0}, items[2] = {0, 0};
+        // (descriptors: a start address in 16-byte units in the low bits, the rest the same for every k)
+        const uint64_t d_q = umma_desc_sw128(sq), d_k = umma_desc_sw128(sk), d_v = pf_desc_v(sv, S::SLAB);
         auto scores = [&](int w, int buf, int st) {
-            if (lane == 0) {
+            const uint64_t q = d_q + uint32_t(w * S::QB / 16), k = d_k + uint32_t(st * S::TB / 16);
 #pragma unroll
-                for (int k = 0; k < D / 16; ++k) {
-                    const uint32_t qa = sq + w * S::QB + (k >> 2) * 16384 + (k & 3) * 32;
-                    const uint32_t ka = sk + st * S::TB + (k >> 2) * S::SLAB + (k & 3) * 32;
-                    tc_mma_f16(tmem + buf * KT, umma_desc_sw128(qa), umma_desc_sw128(ka), id_s, k > 0);
-                }
-                tc_commit(&bar.s_full[buf]);
-            }
-            __syncwarp();
+            for (int i = 0; i < D / 16; ++i)
+                tc_mma_f16(tmem + buf * KT, q + uint32_t(((i >> 2) * 16384 + (i & 3) * 32) / 16),
+                           k + uint32_t(((i >> 2) * S::SLAB + (i & 3) * 32) / 16), id_s, i > 0);
+            tc_commit(&bar.s_full[buf]);
         };
         auto products = [&](int w, int buf, int st, bool first) {
-            if (lane == 0) {
+            const uint64_t v = d_v + uint32_t(st * S::TB / 16);
+            const uint32_t o = tmem + S::O_COL + w * D, p = tmem + buf * KT;
+            tc_mma_ts(o, p, v, id_o, first ? 0u : 1u);
 #pragma unroll
-                for (int k = 0; k < KT / 16; ++k)
-                    tc_mma_ts(tmem + S::O_COL + w * D, tmem + buf * KT + k * 8, pf_desc_v(sv + st * S::TB + k * 2048, S::SLAB),
-                              id_o, (first && k == 0) ? 0u : 1u);
-                tc_commit(&bar.o_done[w]);
-            }
-            __syncwarp();
-        };
-        auto commit = [&](uint64_t* b) {
-            if (lane == 0) tc_commit(b);
-            __syncwarp();
+            for (int i = 1; i < KT / 16; ++i) tc_mma_ts(o, p + i * 8, v + uint32_t(i * 2048 / 16), id_o, 1u);
+            tc_commit(&bar.o_done[w]);
         };
         while (walk.next(a)) {
             const int rows = min(R, walk.fresh * a.G - walk.tile * R), nq = rows > 128 ? 2 : 1;
@@ -692,7 +684,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1) kv4_prefill_kernel(const Kv4Att
                 pf_wait(&bar.k_full[it & 1], (it >> 1) & 1, abort);
                 tc_fence_after();
                 for (int w = 0; w < nq; ++w) scores(w, w, it & 1);
-                commit(&bar.k_empty[it & 1]);
+                tc_commit(&bar.k_empty[it & 1]);
                 for (int t = 0; t < steps; ++t, ++it) {
                     const int st = it & 1, nx = (it + 1) & 1;
                     pf_wait(&bar.v_full[st], (it >> 1) & 1, abort);
@@ -708,8 +700,8 @@ __global__ void __launch_bounds__(PF_THREADS, 1) kv4_prefill_kernel(const Kv4Att
                             scores(w, w, nx);
                         }
                     }
-                    commit(&bar.v_empty[st]);
-                    if (t + 1 < steps) commit(&bar.k_empty[nx]);
+                    tc_commit(&bar.v_empty[st]);
+                    if (t + 1 < steps) tc_commit(&bar.k_empty[nx]);
                 }
             } else {
                 for (int t = 0; t <= steps; ++t) {
@@ -718,7 +710,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1) kv4_prefill_kernel(const Kv4Att
                         pf_wait(&bar.k_full[i & 1], (i >> 1) & 1, abort);
                         tc_fence_after();
                         scores(0, (used[0] + t) & 1, i & 1);
-                        commit(&bar.k_empty[i & 1]);
+                        tc_commit(&bar.k_empty[i & 1]);
                     }
                     if (t > 0) {
                         const int i = it + t - 1, u = used[0] + t - 1;
@@ -726,7 +718,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1) kv4_prefill_kernel(const Kv4Att
                         pf_wait(&bar.p_full[u & 1], (u >> 1) & 1, abort);
                         tc_fence_after();
                         products(0, u & 1, i & 1, t == 1);
-                        commit(&bar.v_empty[i & 1]);
+                        tc_commit(&bar.v_empty[i & 1]);
                     }
                 }
                 it += steps;
@@ -734,12 +726,13 @@ __global__ void __launch_bounds__(PF_THREADS, 1) kv4_prefill_kernel(const Kv4Att
             }
         }
         grid_dep_launch();
-        commit(&bar.done);  // nothing of this CTA's is in flight when its tensor memory goes (after an error too)
+        tc_commit(&bar.done);  // nothing of this CTA's is in flight when its tensor memory goes (after an error too)
         mbar_wait(&bar.done, 0);
     }
     tc_fence_before();
     __syncthreads();
     if (warp == PF_MMA) {
+        __syncwarp();
         tc_fence_after();
         tmem_dealloc(tmem, 512);
     }
