@@ -285,8 +285,10 @@ int lq_kv4_read(const uint32_t* kq, const void* ks, const void* kb, const uint32
  * (q_start NULL: row b, one each), at most max_q of them, the last of them at position lens[b] - 1; a query sees the
  * keys up to its own position, the last `window` of them when window > 0. out = sum p v / (sum p + e^sink), p = e^(scale q . k), softmax statistics in 32 bits; sinks (H) float32 or NULL; 0 where a
  * query sees nothing and for rows past q_start[B]. table (B, width) page ids, -1 where there is none. workspace:
- * lq_kv4_attend_workspace(N, B, max_q, H, KVH, head_dim) bytes, 16-byte aligned (NULL when that is 0). */
-size_t lq_kv4_attend_workspace(int N, int B, int max_q, int H, int KVH, int head_dim);
+ * lq_kv4_attend_workspace(B, max_q, H, KVH, head_dim, width, page_size) bytes, 128-byte aligned (NULL when that is 0):
+ * the parts of split softmaxes, and, where max_q is large and width * page_size * B keys fit 1 GiB that way, the keys and
+ * values of requests with many rows as fp16 tiles. */
+size_t lq_kv4_attend_workspace(int B, int max_q, int H, int KVH, int head_dim, int width, int page_size);
 int lq_kv4_attend(const void* q, int N, const int32_t* q_start, int max_q, const uint32_t* kq, const void* ks,
                   const void* kb, const uint32_t* vq, const void* vs, const void* vb, int pages, int page_size,
                   const int32_t* table, int width, const int32_t* lens, int B, const float* sinks, float scale,

@@ -108,7 +108,7 @@ int kv4_append_run(const RotArgs& r, const Kv4Pool& pool, const void* q, long lo
 int kv4_read_run(const Kv4Pool& pool, int D, const int32_t* slots, int N, void* k_out, void* v_out, int dtype,
                  cudaStream_t st);
 bool kv4_attend_shape_ok(int N, int B, int max_q, int H, int KVH, int width, int window);
-size_t kv4_attend_workspace_bytes(int N, int B, int max_q, int H, int KVH, int D);
+size_t kv4_attend_workspace_bytes(int B, int max_q, int H, int KVH, int D, long long room);
 int kv4_attend_run(const Kv4Pool& pool, const void* q, int N, const int32_t* q_start, int max_q, const int32_t* table,
                    int width, const int32_t* lens, int B, const float* sinks, float scale, int window, int H, int D,
                    int dtype, void* workspace, size_t workspace_bytes, void* out, cudaStream_t st);
@@ -757,10 +757,10 @@ int lq_kv4_read(const uint32_t* kq, const void* ks, const void* kb, const uint32
     return finish(kv4_read_run(pool, head_dim, slots, N, k_out, v_out, dtype, reinterpret_cast<cudaStream_t>(stream)));
 }
 
-size_t lq_kv4_attend_workspace(int N, int B, int max_q, int H, int KVH, int head_dim) {
-    if (KVH < 1 || !kv4_attend_shape_ok(N, B, max_q, H, KVH, 1, 0)) return 0;
+size_t lq_kv4_attend_workspace(int B, int max_q, int H, int KVH, int head_dim, int width, int page_size) {
+    if (KVH < 1 || page_size < 1 || !kv4_attend_shape_ok(0, B, max_q, H, KVH, width, 0)) return 0;
     if (check_device() != LQ_OK) return 0;
-    return kv4_attend_workspace_bytes(N, B, max_q, H, KVH, head_dim);
+    return kv4_attend_workspace_bytes(B, max_q, H, KVH, head_dim, (long long)width * page_size);
 }
 
 int lq_kv4_attend(const void* q, int N, const int32_t* q_start, int max_q, const uint32_t* kq, const void* ks,
@@ -775,7 +775,7 @@ int lq_kv4_attend(const void* q, int N, const int32_t* q_start, int max_q, const
         return LQ_E_SHAPE;
     if (!q_start && (N != B || max_q != 1)) return LQ_E_SHAPE;
     if (!kv4_aligned(pool) || !aligned(q, 16) || !aligned(out, 16) || !aligned(q_start, 4) || !aligned(table, 4) ||
-        !aligned(lens, 4) || !aligned(sinks, 4) || !aligned(workspace, 16))
+        !aligned(lens, 4) || !aligned(sinks, 4) || !aligned(workspace, 128))
         return LQ_E_ALIGN;
     int rc = check_device();
     if (rc) return rc;

@@ -710,15 +710,15 @@ static size_t kv4_few_bytes(int D, int R, int sms) {
     return size_t(kv4_ctas(D, R, sms)) * (2 * R * (2 + D) * sizeof(float) + 8 * sizeof(int32_t));
 }
 
-size_t kv4_prefill_workspace_bytes(int D, int sms);
+size_t kv4_prefill_workspace_bytes(int D, int sms, int B, int KVH, int G, int max_q, long long room);
 int kv4_prefill_run(const Kv4AttArgs& a, int D, int dtype, void* workspace, cudaStream_t st);
 
-size_t kv4_attend_workspace_bytes(int N, int B, int max_q, int H, int KVH, int D) {
+size_t kv4_attend_workspace_bytes(int B, int max_q, int H, int KVH, int D, long long room) {
     int R, split;
     kv4_rows(max_q, H / KVH, &R, &split);
     const int sms = device_info().sm_count;
     const bool many = (long long)max_q * (H / KVH) > split;
-    return (split ? kv4_few_bytes(D, R, sms) : 0) + (many ? kv4_prefill_workspace_bytes(D, sms) : 0);
+    return (split ? kv4_few_bytes(D, R, sms) : 0) + (many ? kv4_prefill_workspace_bytes(D, sms, B, KVH, H / KVH, max_q, room) : 0);
 }
 
 template <typename T, int D, int NT>
@@ -749,7 +749,7 @@ int kv4_attend_run(const Kv4Pool& pool, const void* q, int N, const int32_t* q_s
                    int width, const int32_t* lens, int B, const float* sinks, float scale, int window, int H, int D,
                    int dtype, void* workspace, size_t workspace_bytes, void* out, cudaStream_t st) {
     if (N == 0) return LQ_OK;
-    if (!workspace || workspace_bytes < kv4_attend_workspace_bytes(N, B, max_q, H, pool.KVH, D)) return LQ_E_ARG;
+    if (!workspace || workspace_bytes < kv4_attend_workspace_bytes(B, max_q, H, pool.KVH, D, (long long)width * pool.page)) return LQ_E_ARG;
     const int sms = device_info().sm_count;
     Kv4AttArgs a = {};
     a.pool = pool;
@@ -773,7 +773,7 @@ int kv4_attend_run(const Kv4Pool& pool, const void* q, int N, const int32_t* q_s
     if ((long long)max_q * a.G > a.split_rows) {
         const int rc = kv4_prefill_run(a, D, dtype, ws, st);
         if (rc || !a.split_rows) return rc;
-        ws += kv4_prefill_workspace_bytes(D, sms);
+        ws += kv4_prefill_workspace_bytes(D, sms, B, pool.KVH, a.G, max_q, (long long)width * pool.page);
     }
     a.part_o = reinterpret_cast<float*>(ws);
     a.part_ml = a.part_o + size_t(kv4_ctas(D, R, sms)) * 2 * R * D;

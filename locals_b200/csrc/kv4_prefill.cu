@@ -27,6 +27,7 @@
 #include <stdint.h>
 
 #include <type_traits>
+#include <utility>
 
 #include "kv4_attend.cuh"
 #include "lq_host.h"
@@ -37,8 +38,11 @@ namespace lq {
 
 constexpr int PF_SOFT = 8;                       // softmax warps (a row a thread)
 constexpr int PF_UNPACK = 8;                     // unpacking warps
-constexpr int PF_MMA = PF_SOFT + PF_UNPACK;      // the issuing warp
-constexpr int PF_THREADS = (PF_MMA + 1) * 32;
+constexpr int PF_FIRST = 4;                      // the first warpgroup: an issuing warp, one for pages or copies, two idle
+// Threads a CTA: without unpacking warps 168 registers each, with them 96 each at launch, then shared out.
+constexpr int pf_threads(bool dense) { return (PF_FIRST + PF_SOFT + (dense ? 0 : PF_UNPACK)) * 32; }
+constexpr int PF_REGS_SOFT = 120, PF_REGS_UNPACK = 88, PF_REGS_MMA = 64;
+static_assert(PF_SOFT * PF_REGS_SOFT + PF_UNPACK * PF_REGS_UNPACK + PF_FIRST * PF_REGS_MMA <= pf_threads(false) / 32 * 96, "registers");
 
 template <int D>
 struct PfShape {
@@ -63,7 +67,7 @@ __device__ __forceinline__ void pf_steps(const Kv4AttArgs& a, int base, int fres
     const int q0 = tile * S::R / a.G, q1 = (min((tile + 1) * S::R, fresh * a.G) - 1) / a.G;
     const int keys = max(min(base + q1 + 1, room), 0);
     const int from = a.window ? min(max(base + q0 + 1 - a.window, 0), keys) : 0;
-    *lo = from / S::KT;
+    *lo = min(from, max(keys - 1, 0)) / S::KT;
     *hi = max((keys + S::KT - 1) / S::KT, *lo + 1);
 }
 
@@ -102,35 +106,32 @@ __device__ __forceinline__ long long pf_sum(long long v, long long* red) {
     return s;
 }
 
-// The CTA's walk over its steps: items (request, tile, kv head) in that order, each with its steps [st0, st1).
+// The CTA's walk over its share: items (request, tile, kv head) in that order, each with its steps [st0, st1).
 template <int D>
 struct PfWalk {
-    long long x, x1, at;  // steps: next, end, those before request b
+    int left, skip;  // steps of the share left; steps of the next item that come before the share
+    bool begun;
     int b, tile, kvh, lo, hi, st0, st1, first, fresh, base, tiles;
-    long long item_at;
 
     // The next item; false when the share is done. Every caller walks alike.
     __device__ bool next(const Kv4AttArgs& a) {
-        if (x >= x1) return false;
-        for (;;) {
-            if (tile < tiles) {
-                const long long end = item_at + hi - lo;
-                if (x < end) break;
-                item_at = end;
-                if (++kvh == a.pool.KVH) {
-                    kvh = 0;
-                    if (++tile < tiles) pf_steps<D>(a, base, fresh, tile, &lo, &hi);
-                }
-            } else {
-                ++b;
-                tiles = pf_tiles<D>(a, b, &first, &fresh, &base);
-                tile = kvh = 0;
-                if (tiles) pf_steps<D>(a, base, fresh, 0, &lo, &hi);
+        if (left == 0) return false;
+        if (begun && ++kvh == a.pool.KVH) {
+            kvh = 0;
+            if (++tile >= tiles) {
+                do {
+                    ++b;
+                    tiles = pf_tiles<D>(a, b, &first, &fresh, &base);
+                } while (!tiles);
+                tile = 0;
             }
+            pf_steps<D>(a, base, fresh, tile, &lo, &hi);
         }
-        st0 = int(x - item_at);
-        st1 = int(min((long long)(hi - lo), x1 - item_at));
-        x = item_at + st1;
+        begun = true;
+        st0 = skip;
+        st1 = min(hi - lo, skip + left);
+        left -= st1 - st0;
+        skip = 0;
         return true;
     }
 };
@@ -139,6 +140,74 @@ __device__ __forceinline__ void pf_tmem_st8(uint32_t taddr, const uint32_t (&r)[
     asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr), "r"(r[0]), "r"(r[1]),
                  "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
                  : "memory");
+}
+
+__device__ __forceinline__ void pf_tmem_st32(uint32_t taddr, const uint32_t* r) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,"
+        "%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
+        "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
+        "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+        : "memory");
+}
+
+// tc_mma_f16 and tc_mma_ts with the operands' places as constant offsets from a tile's, put together inside: kept as values,
+// the descriptors of all products would take more registers than the issuing thread has, and each reload delays a product.
+template <int A_OFF, int B_OFF, int ACC>
+__device__ __forceinline__ void pf_mma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t hi, uint32_t idesc) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t.reg .b32 x, y;\n\t.reg .b64 da, db;\n\t"
+        "add.u32 x, %1, %5;\n\tadd.u32 y, %2, %6;\n\t"
+        "mov.b64 da, {x, %3};\n\tmov.b64 db, {y, %3};\n\t"
+        "setp.ne.b32 p, %7, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %4, p;\n\t}" ::"r"(d),
+        "r"(a), "r"(b), "r"(hi), "r"(idesc), "n"(A_OFF), "n"(B_OFF), "n"(ACC)
+        : "memory");
+}
+template <int A_OFF, int B_OFF>
+__device__ __forceinline__ void pf_mma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t hi, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t.reg .b32 x, y;\n\t.reg .b64 db;\n\t"
+        "add.u32 x, %1, %5;\n\tadd.u32 y, %2, %6;\n\t"
+        "mov.b64 db, {y, %3};\n\t"
+        "setp.ne.b32 p, %7, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [x], db, %4, p;\n\t}" ::"r"(d),
+        "r"(a), "r"(b), "r"(hi), "r"(idesc), "n"(A_OFF), "n"(B_OFF), "r"(accumulate)
+        : "memory");
+}
+// S (128 rows x KT keys) = Q K^T over the D dimensions, 16 at a time.
+template <int D, int SLAB, int... I>
+__device__ __forceinline__ void pf_scores(uint32_t d, uint32_t q, uint32_t k, uint32_t hi, uint32_t idesc,
+                                          std::integer_sequence<int, I...>) {
+    (pf_mma_ss<((I >> 2) * 16384 + (I & 3) * 32) / 16, ((I >> 2) * SLAB + (I & 3) * 32) / 16, (I > 0)>(d, q, k, hi, idesc), ...);
+}
+// O (128 rows x D) (+)= P V over the step's keys, 16 at a time.
+template <int... I>
+__device__ __forceinline__ void pf_products(uint32_t d, uint32_t p, uint32_t v, uint32_t hi, uint32_t idesc, uint32_t first,
+                                            std::integer_sequence<int, I...>) {
+    (pf_mma_ts<I * 8, I * 2048 / 16>(d, p, v, hi, idesc, I > 0 ? 1u : first), ...);
+}
+
+// Two 32-bit floats at a time.
+__device__ __forceinline__ uint64_t pf_pair(float lo, float hi) {
+    uint64_t d;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(lo), "f"(hi));
+    return d;
+}
+__device__ __forceinline__ void pf_unpair(uint64_t v, float* lo, float* hi) {
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(*lo), "=f"(*hi) : "l"(v));
+}
+__device__ __forceinline__ uint64_t pf_fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+__device__ __forceinline__ uint64_t pf_add2(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
 }
 
 // Descriptor of a B operand whose N side is contiguous (128-byte swizzle): 8 keys of 64 dimensions are 1024 bytes, the
@@ -157,12 +226,17 @@ __device__ __forceinline__ uint32_t pf_affine(uint32_t v, uint32_t s2, uint32_t 
 }
 
 struct PfBars {
-    uint64_t q_full[2], k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], o_done[2], done;
-    uint32_t tmem;
+    uint64_t q_full[2], k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], o_done[2], r_full[4], r_empty[4], done;
     int abort;          // a wait gave up: no one waits any more
     int v_exp[4];       // power of two of the values of step i & 3
     uint32_t miss[4];   // its runs of 8 keys without a page
+    // what the page warp tells the unpacking warps of step i & 3: the pool row of each run of 8 keys (none: KV4_NONE), the
+    // keys from its first to the tile's end (0: no more steps), whether an item starts, and the runs without a page
+    uint32_t run[4][16];
+    int left[4], start[4];
+    uint32_t gone[4];
     float v_max[PF_UNPACK];
+    int rows, steps;    // the item's (0: no more), from the first softmax warp to the issuing thread
 };
 
 // A bounded wait that, once any has given up, none of the CTA's takes again.
@@ -171,14 +245,140 @@ __device__ __forceinline__ void pf_wait(uint64_t* bar, uint32_t parity, volatile
     if (!mbar_wait(bar, parity)) *abort = 1;
 }
 
+// Which keys and which 16 bytes of codes piece j of a lane of warp uw (of W) is: 8 lanes are 8 keys, so that their stores
+// fall on different banks.
+template <int D, int W>
+struct PfPieces {
+    static constexpr int NP = D / 32, J = PfShape<D>::KT * NP / (W * 32);  // pieces a key, a lane
+    __device__ static __forceinline__ int key(int j, int uw, int lane) {
+        const int blk = j * W + uw;
+        return NP == 2 ? blk * 16 + (lane & 7) + ((lane >> 4) << 3) : NP == 4 ? blk * 8 + (lane & 7) : (blk >> 1) * 8 + (lane & 7);
+    }
+    __device__ static __forceinline__ int piece(int j, int uw, int lane) {
+        return NP == 2 ? (lane >> 3) & 1 : NP == 4 ? lane >> 3 : (lane >> 3) + 4 * ((j * W + uw) & 1);
+    }
+};
+
+// 32 codes with one scale and bias -> 64 bytes of a tile row (128-byte swizzle), 16 bytes at a time.
+template <int D>
+__device__ __forceinline__ void pf_unpack(const uint4& codes, float s, float b, uint32_t tile, int key, int p) {
+    const uint32_t s1 = cvt_f16x2(s, s), s16 = cvt_f16x2(s * 0.0625f, s * 0.0625f), b2 = cvt_f16x2(b, b);
+    const uint32_t cw[4] = {codes.x, codes.y, codes.z, codes.w};
+    const uint32_t row = tile + (p >> 1) * PfShape<D>::SLAB + key * 128;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const uint32_t x = cw[i], y = cw[i] >> 8;
+        const uint32_t o0 = pf_affine(lop3_and_or(x, 0x000f000fu, 0x64006400u), s1, b2);
+        const uint32_t o1 = pf_affine(lop3_and_or(x, 0x00f000f0u, 0x64006400u), s16, b2);
+        const uint32_t o2 = pf_affine(lop3_and_or(y, 0x000f000fu, 0x64006400u), s1, b2);
+        const uint32_t o3 = pf_affine(lop3_and_or(y, 0x00f000f0u, 0x64006400u), s16, b2);
+        asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(row + ((((p & 1) * 4 + i) ^ (key & 7)) << 4)), "r"(o0), "r"(o1),
+                     "r"(o2), "r"(o3)
+                     : "memory");
+    }
+}
+
+// A piece's scales and biases in fp32. A value scale or bias that is not finite makes the values 0 and the key NaN, which
+// only the rows that see it meet. Returns the largest |value| that the group can hold.
+template <typename T>
+__device__ __forceinline__ float pf_scales(uint16_t ks16, uint16_t kb16, uint16_t vs16, uint16_t vb16, float* ks, float* kb,
+                                           float* vs, float* vb) {
+    *ks = F16Traits<T>::to_f32(ks16), *kb = F16Traits<T>::to_f32(kb16);
+    *vs = F16Traits<T>::to_f32(vs16), *vb = F16Traits<T>::to_f32(vb16);
+    const float most = fmaf(15.0f, fabsf(*vs), fabsf(*vb));
+    if (most < INFINITY) return most;
+    *vs = *vb = 0.0f;
+    *ks = *kb = __int_as_float(0x7fffffff);
+    return 0.0f;
+}
+// The power of two that puts M at 2^10 .. 2^11 (M below 2^128: at least -117).
+__device__ __forceinline__ int pf_exponent(float M) { return min(10 - (int(__float_as_uint(M) >> 23) - 127), 100); }
+
+// ---- the dense form's first pass: the keys and values of requests with many tiles, unpacked once ----
+// One CTA a (step of KT keys, kv head, request): the step's two tiles as they are to lie in shared memory, copied out whole,
+// and its values' power of two (0 wherever they lie within fp16's comfort) and missing pages.
+constexpr int PD_WARPS = 8;
 template <typename T, int D>
-__global__ void __launch_bounds__(PF_THREADS, 1) kv4_prefill_kernel(const Kv4AttArgs a) {
+__global__ void __launch_bounds__(PD_WARPS * 32) kv4_dense_kernel(const Kv4AttArgs a) {
     using S = PfShape<D>;
-    constexpr int GR = S::GR, KT = S::KT, NQ = S::NQ, R = S::R;
+    using P = PfPieces<D, PD_WARPS>;
     extern __shared__ __align__(1024) uint8_t pf_raw[];
-    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(pf_raw) + 1023) & ~uintptr_t(1023));
-    PfBars& bar = *reinterpret_cast<PfBars*>(smem + S::SMEM);
-    __shared__ long long red[PF_MMA + 1];
+    __shared__ float part[PD_WARPS];
+    grid_dep_wait();
+    const int s = blockIdx.x, kvh = blockIdx.y, b = blockIdx.z;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    int first, fresh, base, lo, hi;
+    if (!pf_tiles<D>(a, b, &first, &fresh, &base)) return;
+    pf_steps<D>(a, base, fresh, 0, &lo, &hi);
+    const int room = int(min((long long)a.width * a.pool.page, 0x7fffffffLL)), keys = max(min(base + fresh, room), 0);
+    if (s < lo || s >= max((keys + S::KT - 1) / S::KT, 1)) return;
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(pf_raw) + 127) & ~uintptr_t(127));
+    const uint32_t tile = smem_u32(smem);
+    constexpr int RUNS = S::KT / 8;
+    const int key0 = s * S::KT, run_key = key0 + (lane % RUNS) * 8;
+    uint32_t mine = KV4_NONE;
+    bool gone = false;
+    if (run_key < keys) {
+        const int pg = run_key / a.pool.page, id = a.table[(size_t)b * a.width + pg];
+        gone = unsigned(id) >= unsigned(a.pool.pages);
+        if (gone)
+            record_status(LQ_DEV_BOUNDS);
+        else
+            mine = kv4_row(a.pool, id, kvh, run_key - pg * a.pool.page);
+    }
+    const uint32_t miss = __ballot_sync(0xffffffffu, lane < RUNS && gone);
+    uint4 kc[P::J], vc[P::J];
+    float ks[P::J], kb[P::J], vs[P::J], vb[P::J], top = 0.0f;
+    uint16_t sc[P::J][4];
+#pragma unroll
+    for (int j = 0; j < P::J; ++j) {
+        const int k = P::key(j, warp, lane), p = P::piece(j, warp, lane);
+        const uint32_t run = __shfl_sync(0xffffffffu, mine, k / 8);
+        kc[j] = vc[j] = make_uint4(0, 0, 0, 0);
+        sc[j][0] = sc[j][1] = sc[j][2] = sc[j][3] = 0;
+        if (run != KV4_NONE && key0 + k < keys) {
+            const size_t row = run + (k & 7), g = row * S::GR + p / 2;
+            kc[j] = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint8_t*>(a.pool.kq) + row * S::RB + p * 16);
+            vc[j] = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint8_t*>(a.pool.vq) + row * S::RB + p * 16);
+            sc[j][0] = a.pool.ks[g], sc[j][1] = a.pool.kb[g], sc[j][2] = a.pool.vs[g], sc[j][3] = a.pool.vb[g];
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < P::J; ++j)
+        top = fmaxf(top, pf_scales<T>(sc[j][0], sc[j][1], sc[j][2], sc[j][3], &ks[j], &kb[j], &vs[j], &vb[j]));
+    top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top)));
+    if (lane == 0) part[warp] = top;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < PD_WARPS; ++i) top = fmaxf(top, part[i]);
+    const int ve = top == 0.0f || (top >= 0.015625f && top < 16384.0f) ? 0 : pf_exponent(top);
+    const float vf = exp2f(float(ve));
+#pragma unroll
+    for (int j = 0; j < P::J; ++j) {
+        const int k = P::key(j, warp, lane), p = P::piece(j, warp, lane);
+        pf_unpack<D>(kc[j], ks[j], kb[j], tile, k, p);
+        pf_unpack<D>(vc[j], vs[j] * vf, vb[j] * vf, tile + S::TB, k, p);
+    }
+    fence_proxy_async();
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        const size_t at = ((size_t)b * a.pool.KVH + kvh) * a.dense_steps + s;
+        a.dense_meta[at] = make_int2(ve, int(miss));
+        asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(a.dense + at * (2 * S::TB)), "r"(tile),
+                     "r"(2 * S::TB)
+                     : "memory");
+        asm volatile("cp.async.bulk.commit_group;\n\tcp.async.bulk.wait_group 0;" ::: "memory");
+    }
+}
+
+// DENSE: the tiles come unpacked, by bulk copies, from what kv4_dense_kernel left.
+template <typename T, int D, bool DENSE>
+__global__ void __launch_bounds__(pf_threads(DENSE), 1) kv4_prefill_kernel(const Kv4AttArgs a) {
+    using S = PfShape<D>;
+    constexpr int GR = S::GR, KT = S::KT, NQ = S::NQ, R = S::R, PF_THREADS = pf_threads(DENSE);
+    extern __shared__ __align__(1024) uint8_t pf_raw[];
+    __shared__ long long red[PF_THREADS / 32];
+    __shared__ uint8_t* volatile pf_base;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
     grid_dep_wait();
@@ -192,16 +392,15 @@ __global__ void __launch_bounds__(PF_THREADS, 1) kv4_prefill_kernel(const Kv4Att
         if (tid == 0) rec[0] = 0;
         return;
     }
+    const long long x0 = (long long)blockIdx.x * total / n, x1 = ((long long)blockIdx.x + 1) * total / n;
     PfWalk<D> walk;
-    walk.x = (long long)blockIdx.x * total / n;
-    walk.x1 = ((long long)blockIdx.x + 1) * total / n;
     {
         long long at = 0;
         int b = 0;
         for (int b0 = 0;; b0 += PF_THREADS) {
             const long long w = b0 + tid < a.B ? pf_weight<D>(a, b0 + tid) : 0;
             const long long sum = pf_sum(w, red);
-            if (at + sum <= walk.x) {
+            if (at + sum <= x0) {
                 at += sum;
                 continue;
             }
@@ -215,13 +414,12 @@ __global__ void __launch_bounds__(PF_THREADS, 1) kv4_prefill_kernel(const Kv4Att
             if (lane == 31) red[warp] = s;
             __syncthreads();
             for (int k = 0; k < warp; ++k) s += red[k];
-            const bool past = at + s > walk.x;
+            const bool past = at + s > x0;
             b = b0 + int(pf_sum(past ? 0 : 1, red));
             at += pf_sum(past ? 0 : w, red);
             break;
         }
         walk.b = b;
-        walk.at = at;
         walk.tiles = pf_tiles<D>(a, b, &walk.first, &walk.fresh, &walk.base);
         // the tile: the threads sum theirs, in rounds of PF_THREADS tiles
         int t0 = 0;
@@ -230,7 +428,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1) kv4_prefill_kernel(const Kv4Att
             if (t0 + tid < walk.tiles) pf_steps<D>(a, walk.base, walk.fresh, t0 + tid, &lo, &hi);
             const long long w = (long long)(hi - lo) * a.pool.KVH;
             const long long sum = pf_sum(w, red);
-            if (at + sum <= walk.x) {
+            if (at + sum <= x0) {
                 at += sum;
                 continue;
             }
@@ -244,18 +442,21 @@ __global__ void __launch_bounds__(PF_THREADS, 1) kv4_prefill_kernel(const Kv4Att
             if (lane == 31) red[warp] = s;
             __syncthreads();
             for (int k = 0; k < warp; ++k) s += red[k];
-            const bool past = at + s > walk.x;
+            const bool past = at + s > x0;
             walk.tile = t0 + int(pf_sum(past ? 0 : 1, red));
             at += pf_sum(past ? 0 : w, red);
             break;
         }
         pf_steps<D>(a, walk.base, walk.fresh, walk.tile, &walk.lo, &walk.hi);
-        walk.kvh = int((walk.x - at) / (walk.hi - walk.lo));
-        walk.item_at = at + (long long)walk.kvh * (walk.hi - walk.lo);
+        const int steps = walk.hi - walk.lo;
+        walk.kvh = int((x0 - at) / steps);
+        const long long item = at + (long long)walk.kvh * steps;
+        walk.skip = int(x0 - item);
+        walk.left = int(x1 - x0);
+        walk.begun = false;
         if (tid == 0) {
-            const long long item = walk.item_at;
-            const int c0 = kv4_owner(item, total, n), c1 = kv4_owner(item + walk.hi - walk.lo - 1, total, n);
-            rec[0] = item < walk.x && c0 == int(blockIdx.x) - 1;  // the first boundary within its item
+            const int c0 = kv4_owner(item, total, n), c1 = kv4_owner(item + steps - 1, total, n);
+            rec[0] = item < x0 && c0 == int(blockIdx.x) - 1;  // the first boundary within its item
             rec[1] = walk.first;
             rec[2] = walk.tile * R;
             rec[3] = min(R, walk.fresh * a.G - walk.tile * R);
@@ -265,35 +466,58 @@ __global__ void __launch_bounds__(PF_THREADS, 1) kv4_prefill_kernel(const Kv4Att
     }
 
     if (tid == 0) {
+        uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(pf_raw) + 1023) & ~uintptr_t(1023));
+        PfBars& bar = *reinterpret_cast<PfBars*>(smem + S::SMEM);
+        pf_base = smem;
         for (int i = 0; i < 2; ++i) {
             mbar_init(&bar.q_full[i], 4);
-            mbar_init(&bar.k_full[i], PF_UNPACK);
+            mbar_init(&bar.k_full[i], DENSE ? 1 : PF_UNPACK);
             mbar_init(&bar.k_empty[i], 1);
-            mbar_init(&bar.v_full[i], PF_UNPACK);
+            mbar_init(&bar.v_full[i], DENSE ? 1 : PF_UNPACK);
             mbar_init(&bar.v_empty[i], 1);
             mbar_init(&bar.s_full[i], 1);
             mbar_init(&bar.p_full[i], 4);
             mbar_init(&bar.o_done[i], 1);
         }
+        for (int i = 0; i < 4; ++i) {
+            mbar_init(&bar.r_full[i], 1);
+            mbar_init(&bar.r_empty[i], PF_UNPACK);
+        }
         mbar_init(&bar.done, 1);
         bar.abort = 0;
         fence_barrier_init();
     }
-    if (warp == PF_MMA) {
-        tmem_alloc(&bar.tmem, 512);
+    __shared__ uint32_t tmem_base;
+    if (warp == 0) {
+        tmem_alloc(&tmem_base, 512);
         tmem_relinquish();
     }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = bar.tmem;
-    volatile int* abort = &bar.abort;
-    const uint32_t sq = smem_u32(smem), sk = sq + NQ * S::QB, sv = sk + 2 * S::TB;
+    // Each role reads the bases for itself from here on: values shared by all roles would be kept on the stack by all,
+    // those with registers to spare too, and the issuing thread's reloads would delay its products.
+    struct Places {
+        PfBars& bar;
+        volatile int* abort;
+        uint32_t tmem, sq, sk, sv;
+    };
+    auto places = [&]() -> Places {
+        uint8_t* smem = pf_base;
+        PfBars& bar = *reinterpret_cast<PfBars*>(smem + S::SMEM);
+        const uint32_t sq = smem_u32(smem), sk = sq + NQ * S::QB;
+        return {bar, &bar.abort, *reinterpret_cast<volatile uint32_t*>(&tmem_base), sq, sk, sk + 2 * S::TB};
+    };
     const int room = int(min((long long)a.width * a.pool.page, 0x7fffffffLL));
 
-    if (warp < PF_SOFT) {
+    if (warp >= PF_FIRST && warp < PF_FIRST + PF_SOFT) {
         // ------------------------------ softmax: a row a thread ------------------------------
-        const int w = warp >> 2, wr = (warp & 3) * 32 + lane;  // query tile, row in it
+        if constexpr (!DENSE) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(PF_REGS_SOFT));
+        const Places at = places();
+        PfBars& bar = at.bar;
+        volatile int* const abort = at.abort;
+        const uint32_t tmem = at.tmem, sq = at.sq;
+        const int w = (warp - PF_FIRST) >> 2, wr = (warp & 3) * 32 + lane;  // query tile, row in it
         const uint32_t lanes = uint32_t((warp & 3) * 32) << 16;
         int it = 0, used = 0;  // steps of the CTA, and of this query tile
         while (walk.next(a)) {
@@ -350,6 +574,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1) kv4_prefill_kernel(const Kv4Att
                                  : "memory");
                 }
             }
+            if (warp == PF_FIRST && lane == 0) bar.rows = rows, bar.steps = steps;
             fence_proxy_async();
             __syncwarp();
             if (lane == 0) mbar_arrive(&bar.q_full[w]);
@@ -367,6 +592,45 @@ __global__ void __launch_bounds__(PF_THREADS, 1) kv4_prefill_kernel(const Kv4Att
                 const int ve_t = *reinterpret_cast<volatile int*>(&bar.v_exp[it & 3]);
                 const bool all = key0 >= lo_all && key0 + KT <= hi_all && miss == 0;
                 const uint32_t s_col = tmem + lanes + buf * KT;
+                // The common case, one pass: every row of the warp sees the whole step, and the reference from the steps
+                // before serves it (found out at the end: the probabilities stay in registers until then, the scores in place).
+                if (all && ve_t == ve && __all_sync(0xffffffffu, m != -INFINITY)) {
+                    const uint64_t c2 = pf_pair(c, c), m2 = pf_pair(-m, -m);
+                    uint32_t r[2][16], p[KT / 2];
+                    uint64_t sums[2] = {0, 0};
+                    float mx[2] = {-INFINITY, -INFINITY};
+                    tmem_ld_32x32b_x16(s_col, r[0]);
+#pragma unroll
+                    for (int ch = 0; ch < KT / 16; ++ch) {  // the next 16 scores are read while these are worked on
+                        uint32_t(&x)[16] = r[ch & 1];
+                        tmem_wait_ld();
+                        if (ch + 1 < KT / 16) tmem_ld_32x32b_x16(s_col + ch * 16 + 16, r[(ch + 1) & 1]);
+#pragma unroll
+                        for (int i = 0; i < 16; i += 2) {
+                            const float s0 = __uint_as_float(x[i]), s1 = __uint_as_float(x[i + 1]);
+                            mx[(i >> 1) & 1] = fmaxf(fmaxf(mx[(i >> 1) & 1], s0), s1);
+                            float e0, e1;
+                            pf_unpair(pf_fma2(pf_pair(s0, s1), c2, m2), &e0, &e1);
+                            e0 = kv4_ex2(e0);
+                            e1 = kv4_ex2(e1);
+                            sums[(i >> 1) & 1] = pf_add2(sums[(i >> 1) & 1], pf_pair(e0, e1));
+                            p[ch * 8 + i / 2] = cvt_f16x2(e1, e0);
+                        }
+                    }
+                    if (!__any_sync(0xffffffffu, fmaxf(mx[0], mx[1]) * c > m + 8.0f)) {
+#pragma unroll
+                        for (int ch = 0; ch < KT / 64; ++ch) pf_tmem_st32(s_col + ch * 32, &p[ch * 32]);
+                        float a0, a1, b0, b1;
+                        pf_unpair(sums[0], &a0, &a1);
+                        pf_unpair(sums[1], &b0, &b1);
+                        l += (a0 + a1) + (b0 + b1);
+                        tmem_wait_st();
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(&bar.p_full[buf]);
+                        continue;
+                    }
+                }
                 // whether this row sees place i of the step
                 auto in = [&](int i) {
                     const int key = key0 + i;
@@ -490,88 +754,49 @@ __global__ void __launch_bounds__(PF_THREADS, 1) kv4_prefill_kernel(const Kv4Att
             }
             tc_fence_before();
         }
-    } else if (warp < PF_MMA) {
+        if (w == 0) {  // no more items
+            if (warp == PF_FIRST && lane == 0) bar.rows = 0;
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bar.q_full[0]);
+        }
+    } else if (warp >= PF_FIRST) {
+        if constexpr (!DENSE) {
         // ------------------------------ codes to fp16 tiles ------------------------------
-        const int uw = warp - PF_SOFT;
-        constexpr int NP = S::RB / 16, J = KT * NP / (PF_UNPACK * 32);  // 16-byte pieces a key, pieces a lane
-        constexpr int RUNS = KT / 8;
-        // this lane's piece j: key and piece (8 lanes are 8 keys: their stores fall on different banks)
-        auto key_of = [&](int j) {
-            const int blk = j * PF_UNPACK + uw;
-            return NP == 2 ? blk * 16 + (lane & 7) + ((lane >> 4) << 3) : NP == 4 ? blk * 8 + (lane & 7) : (blk >> 1) * 8 + (lane & 7);
-        };
-        auto piece_of = [&](int j) {
-            return NP == 2 ? (lane >> 3) & 1 : NP == 4 ? lane >> 3 : (lane >> 3) + 4 * ((j * PF_UNPACK + uw) & 1);
-        };
-        // A step's codes, scales and biases in registers, and what is to be known of it.
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(PF_REGS_UNPACK));
+        const Places at = places();
+        PfBars& bar = at.bar;
+        volatile int* const abort = at.abort;
+        const uint32_t sk = at.sk, sv = at.sv;
+        const int uw = warp - PF_FIRST - PF_SOFT;
+        using P = PfPieces<D, PF_UNPACK>;
+        constexpr int J = P::J;
+        // A step's codes, scales and biases in registers.
         struct Held {
             uint4 k[J], v[J];
-            uint32_t ks[J], vs[J];  // scale low, bias high
-            uint32_t miss;
-            bool item_start;
+            uint16_t ks[J], kb[J], vs[J], vb[J];
         };
-        PfWalk<D> w = walk;
-        bool more = w.next(a);
-        int step = 0;
-        // the runs of the walk's step (lane l: run l), KV4_NONE without a page or beyond the tile's keys; moves on
-        struct Runs {
-            uint32_t row, miss;
-            int left;  // keys from the step's first to the tile's end
-            bool item_start;
-        };
-        auto lookup = [&]() -> Runs {
-            const int row0 = w.tile * R, rows = min(R, w.fresh * a.G - row0);
-            const int key_end = min(w.base + (row0 + rows - 1) / a.G + 1, room);
-            const int key0 = (w.lo + w.st0 + step) * KT, key = key0 + (lane % RUNS) * 8;
-            Runs r = {KV4_NONE, 0, key_end - key0, step == 0};
-            if (key < key_end) {
-                const int pg = key / a.pool.page, id = a.table[(size_t)w.b * a.width + pg];
-                if (unsigned(id) >= unsigned(a.pool.pages))
-                    record_status(LQ_DEV_BOUNDS);
-                else
-                    r.row = kv4_row(a.pool, id, w.kvh, key - pg * a.pool.page);
-            }
-            r.miss = __ballot_sync(0xffffffffu, lane < RUNS && r.row == KV4_NONE && key < key_end);
-            if (++step == w.st1 - w.st0) {
-                step = 0;
-                more = w.next(a);
-            }
-            return r;
-        };
-        auto fetch = [&](const Runs& r, Held& h) {
-            h.miss = r.miss;
-            h.item_start = r.item_start;
+        int asked = 0;
+        // issues the next step's loads; false when there is none
+        auto fetch = [&](Held& h) -> bool {
+            const int slot = asked & 3;
+            pf_wait(&bar.r_full[slot], (asked >> 2) & 1, abort);
+            const int left = *reinterpret_cast<volatile int*>(&bar.left[slot]);
+            if (left == 0 || *abort) return false;
+            ++asked;
 #pragma unroll
             for (int j = 0; j < J; ++j) {
-                const int k = key_of(j), p = piece_of(j);
-                const uint32_t run = __shfl_sync(0xffffffffu, r.row, k / 8);
+                const int k = P::key(j, uw, lane), p = P::piece(j, uw, lane);
+                const uint32_t run = *reinterpret_cast<volatile uint32_t*>(&bar.run[slot][k / 8]);
                 h.k[j] = h.v[j] = make_uint4(0, 0, 0, 0);
-                h.ks[j] = h.vs[j] = 0;
-                if (run != KV4_NONE && k < r.left) {
+                h.ks[j] = h.kb[j] = h.vs[j] = h.vb[j] = 0;
+                if (run != KV4_NONE && k < left) {
                     const size_t row = run + (k & 7), g = row * GR + p / 2;
                     h.k[j] = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint8_t*>(a.pool.kq) + row * S::RB + p * 16);
                     h.v[j] = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint8_t*>(a.pool.vq) + row * S::RB + p * 16);
-                    h.ks[j] = a.pool.ks[g] | uint32_t(a.pool.kb[g]) << 16;
-                    h.vs[j] = a.pool.vs[g] | uint32_t(a.pool.vb[g]) << 16;
+                    h.ks[j] = a.pool.ks[g], h.kb[j] = a.pool.kb[g], h.vs[j] = a.pool.vs[g], h.vb[j] = a.pool.vb[g];
                 }
             }
-        };
-        // 32 codes with one scale and bias -> 64 bytes of a tile row, 16 bytes at a time
-        auto unpack = [&](const uint4& codes, float s, float b, uint32_t tile, int key, int p) {
-            const uint32_t s1 = cvt_f16x2(s, s), s16 = cvt_f16x2(s * 0.0625f, s * 0.0625f), b2 = cvt_f16x2(b, b);
-            const uint32_t cw[4] = {codes.x, codes.y, codes.z, codes.w};
-            const uint32_t row = tile + (p >> 1) * S::SLAB + key * 128;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const uint32_t x = cw[i], y = cw[i] >> 8;
-                const uint32_t o0 = pf_affine(lop3_and_or(x, 0x000f000fu, 0x64006400u), s1, b2);
-                const uint32_t o1 = pf_affine(lop3_and_or(x, 0x00f000f0u, 0x64006400u), s16, b2);
-                const uint32_t o2 = pf_affine(lop3_and_or(y, 0x000f000fu, 0x64006400u), s1, b2);
-                const uint32_t o3 = pf_affine(lop3_and_or(y, 0x00f000f0u, 0x64006400u), s16, b2);
-                asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(row + ((((p & 1) * 4 + i) ^ (key & 7)) << 4)), "r"(o0),
-                             "r"(o1), "r"(o2), "r"(o3)
-                             : "memory");
-            }
+            return true;
         };
         float limit = 0.0f;
         int ve = 0;
@@ -579,20 +804,12 @@ __global__ void __launch_bounds__(PF_THREADS, 1) kv4_prefill_kernel(const Kv4Att
         auto step_out = [&](const Held& h, int it) {
             const int st = it & 1;
             const uint32_t par = ((it >> 1) & 1) ^ 1;
-            if (h.item_start) limit = 0.0f, ve = 0;
+            if (*reinterpret_cast<volatile int*>(&bar.start[it & 3])) limit = 0.0f, ve = 0;
             // the values' power of two: the largest |value| a group can hold at 2^10 .. 2^15
             float top = 0.0f, ks[J], kb[J], vs[J], vb[J];
 #pragma unroll
             for (int j = 0; j < J; ++j) {
-                ks[j] = F16Traits<T>::to_f32(h.ks[j] & 0xffffu), kb[j] = F16Traits<T>::to_f32(h.ks[j] >> 16);
-                vs[j] = F16Traits<T>::to_f32(h.vs[j] & 0xffffu), vb[j] = F16Traits<T>::to_f32(h.vs[j] >> 16);
-                const float most = fmaf(15.0f, fabsf(vs[j]), fabsf(vb[j]));
-                if (!(most < INFINITY)) {
-                    vs[j] = vb[j] = 0.0f;
-                    ks[j] = kb[j] = __int_as_float(0x7fffffff);
-                } else {
-                    top = fmaxf(top, most);
-                }
+                top = fmaxf(top, pf_scales<T>(h.ks[j], h.kb[j], h.vs[j], h.vb[j], &ks[j], &kb[j], &vs[j], &vb[j]));
             }
             int over;
             asm volatile(
@@ -610,76 +827,151 @@ __global__ void __launch_bounds__(PF_THREADS, 1) kv4_prefill_kernel(const Kv4Att
                 float M = 0.0f;
 #pragma unroll
                 for (int i = 0; i < PF_UNPACK; ++i) M = fmaxf(M, reinterpret_cast<volatile float*>(bar.v_max)[i]);
-                ve = min(10 - (int(__float_as_uint(M) >> 23) - 127), 100);  // M below 2^128: at least -117
+                ve = pf_exponent(M);
                 limit = exp2f(float(15 - ve));
                 named_barrier(1, PF_UNPACK * 32);
             }
             const float vf = exp2f(float(ve));
             if (uw == 0 && lane == 0) {
                 bar.v_exp[it & 3] = ve;
-                bar.miss[it & 3] = h.miss;
+                bar.miss[it & 3] = bar.gone[it & 3];
             }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bar.r_empty[it & 3]);
             pf_wait(&bar.k_empty[st], par, abort);
 #pragma unroll
-            for (int j = 0; j < J; ++j) unpack(h.k[j], ks[j], kb[j], sk + st * S::TB, key_of(j), piece_of(j));
+            for (int j = 0; j < J; ++j) pf_unpack<D>(h.k[j], ks[j], kb[j], sk + st * S::TB, P::key(j, uw, lane), P::piece(j, uw, lane));
             fence_proxy_async();
             __syncwarp();
             if (lane == 0) mbar_arrive(&bar.k_full[st]);
             pf_wait(&bar.v_empty[st], par, abort);
 #pragma unroll
-            for (int j = 0; j < J; ++j) unpack(h.v[j], vs[j] * vf, vb[j] * vf, sv + st * S::TB, key_of(j), piece_of(j));
+            for (int j = 0; j < J; ++j) pf_unpack<D>(h.v[j], vs[j] * vf, vb[j] * vf, sv + st * S::TB, P::key(j, uw, lane), P::piece(j, uw, lane));
             fence_proxy_async();
             __syncwarp();
             if (lane == 0) mbar_arrive(&bar.v_full[st]);
         };
-        // pages two steps ahead, codes one step ahead
+        // two steps a turn, so that what is in flight stays in its registers
         Held h0, h1;
-        Runs ahead;
-        int held = 0, known = 0;  // steps in registers, looked up
-        if (more) ahead = lookup(), known = 1;
-        if (known) {
-            fetch(ahead, h0);
-            held = 1, known = 0;
-            if (more) ahead = lookup(), known = 1;
+        bool held = fetch(h0);
+        for (int it = 0; held; it += 2) {
+            const bool second = fetch(h1);
+            step_out(h0, it);
+            if (!second) break;
+            held = fetch(h0);
+            step_out(h1, it + 1);
         }
-        for (int it = 0; held; ++it) {
-            Held& now = h0;
-            held = 0;
-            if (known) {
-                fetch(ahead, h1);
-                held = 1, known = 0;
-                if (more) ahead = lookup(), known = 1;
+        }
+    } else {
+        if constexpr (!DENSE) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(PF_REGS_MMA));
+    }
+    if (DENSE && warp == 1) {
+        // ------------------------------ copies of the unpacked tiles: one thread ------------------------------
+        if (lane == 0) {
+            const Places at = places();
+            PfBars& bar = at.bar;
+            volatile int* const abort = at.abort;
+            const uint32_t sk = at.sk, sv = at.sv;
+            auto copy = [&](uint64_t* full, uint32_t dst, const uint8_t* src) {
+                mbar_arrive_expect_tx(full, S::TB);
+                asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
+                             "l"(src), "r"(S::TB), "r"(smem_u32(full))
+                             : "memory");
+            };
+            int it = 0;
+            while (walk.next(a) && !*abort) {
+                const size_t tile0 = ((size_t)walk.b * a.pool.KVH + walk.kvh) * a.dense_steps + walk.lo;
+                for (int t = walk.st0; t < walk.st1; ++t, ++it) {
+                    const int st = it & 1;
+                    const uint32_t par = ((it >> 1) & 1) ^ 1;
+                    const int2 meta = a.dense_meta[tile0 + t];
+                    const uint8_t* src = a.dense + (tile0 + t) * (2 * S::TB);
+                    pf_wait(&bar.k_empty[st], par, abort);
+                    if (*abort) break;
+                    bar.v_exp[it & 3] = meta.x;
+                    bar.miss[it & 3] = uint32_t(meta.y);
+                    copy(&bar.k_full[st], sk + st * S::TB, src);
+                    pf_wait(&bar.v_empty[st], par, abort);
+                    if (*abort) break;
+                    copy(&bar.v_full[st], sv + st * S::TB, src + S::TB);
+                }
             }
-            step_out(now, it);
-            h0 = h1;
+            // (what was copied has been waited for by the issuing thread, or, after an error, is waited for here)
+            for (int i = max(it - 2, 0); i < it && *abort; ++i) {
+                mbar_wait(&bar.k_full[i & 1], (i >> 1) & 1);
+                mbar_wait(&bar.v_full[i & 1], (i >> 1) & 1);
+            }
         }
-    } else if (lane == 0) {
+        __syncwarp();
+    } else if (!DENSE && warp == 1) {
+        // ------------------------------ pages: a step's table entries, up to four steps ahead ------------------------------
+        const Places at = places();
+        PfBars& bar = at.bar;
+        volatile int* const abort = at.abort;
+        constexpr int RUNS = KT / 8;
+        int it = 0;
+        while (walk.next(a) && !*abort) {
+            const int row0 = walk.tile * R, rows = min(R, walk.fresh * a.G - row0);
+            const int key_end = min(walk.base + (row0 + rows - 1) / a.G + 1, room);
+            for (int t = walk.st0; t < walk.st1; ++t, ++it) {
+                const int slot = it & 3, key0 = (walk.lo + t) * KT, key = key0 + (lane % RUNS) * 8;
+                uint32_t row = KV4_NONE;
+                bool gone = false;
+                if (key < key_end) {
+                    const int pg = key / a.pool.page, id = a.table[(size_t)walk.b * a.width + pg];
+                    gone = unsigned(id) >= unsigned(a.pool.pages);
+                    if (gone)
+                        record_status(LQ_DEV_BOUNDS);
+                    else
+                        row = kv4_row(a.pool, id, walk.kvh, key - pg * a.pool.page);
+                }
+                const uint32_t all_gone = __ballot_sync(0xffffffffu, lane < RUNS && gone);
+                pf_wait(&bar.r_empty[slot], ((it >> 2) & 1) ^ 1, abort);
+                if (lane < RUNS) bar.run[slot][lane] = row;
+                if (lane == 0) {
+                    bar.left[slot] = max(key_end - key0, 1);  // (a step that sees no key has no runs either)
+                    bar.start[slot] = t == walk.st0;
+                    bar.gone[slot] = all_gone;
+                }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&bar.r_full[slot]);
+            }
+        }
+        pf_wait(&bar.r_empty[it & 3], ((it >> 2) & 1) ^ 1, abort);
+        if (lane == 0) {
+            bar.left[it & 3] = 0;  // no more
+            mbar_arrive(&bar.r_full[it & 3]);
+        }
+        __syncwarp();
+    } else if (tid == 0) {
         // ------------------------------ MMA issuer: one thread ------------------------------
+        const Places at = places();
+        PfBars& bar = at.bar;
+        volatile int* const abort = at.abort;
+        const uint32_t tmem = at.tmem, sq = at.sq, sk = at.sk, sv = at.sv;
         constexpr uint32_t id_s = umma_idesc_f16(0, 128, KT);
         constexpr uint32_t id_o = umma_idesc_f16(0, 128, D) | (1u << 16);  // B's N side contiguous
         int it = 0, used[2] = {0, 0}, items[2] = {0, 0};
-        // (descriptors: a start address in 16-byte units in the low bits, the rest the same for every k)
-        const uint64_t d_q = umma_desc_sw128(sq), d_k = umma_desc_sw128(sk), d_v = pf_desc_v(sv, S::SLAB);
+        // (descriptors: a start address in 16-byte units in the low word, the rest the same for all)
+        const uint32_t d_q = uint32_t(umma_desc_sw128(sq)), d_k = uint32_t(umma_desc_sw128(sk));
+        const uint32_t d_v = uint32_t(pf_desc_v(sv, S::SLAB));
+        const uint32_t hi = uint32_t(umma_desc_sw128(0) >> 32);  // (both kinds')
         auto scores = [&](int w, int buf, int st) {
-            const uint64_t q = d_q + uint32_t(w * S::QB / 16), k = d_k + uint32_t(st * S::TB / 16);
-#pragma unroll
-            for (int i = 0; i < D / 16; ++i)
-                tc_mma_f16(tmem + buf * KT, q + uint32_t(((i >> 2) * 16384 + (i & 3) * 32) / 16),
-                           k + uint32_t(((i >> 2) * S::SLAB + (i & 3) * 32) / 16), id_s, i > 0);
+            pf_scores<D, S::SLAB>(tmem + buf * KT, d_q + w * (S::QB / 16), d_k + st * (S::TB / 16), hi, id_s,
+                                  std::make_integer_sequence<int, D / 16>());
             tc_commit(&bar.s_full[buf]);
         };
         auto products = [&](int w, int buf, int st, bool first) {
-            const uint64_t v = d_v + uint32_t(st * S::TB / 16);
-            const uint32_t o = tmem + S::O_COL + w * D, p = tmem + buf * KT;
-            tc_mma_ts(o, p, v, id_o, first ? 0u : 1u);
-#pragma unroll
-            for (int i = 1; i < KT / 16; ++i) tc_mma_ts(o, p + i * 8, v + uint32_t(i * 2048 / 16), id_o, 1u);
+            pf_products(tmem + S::O_COL + w * D, tmem + buf * KT, d_v + st * (S::TB / 16), hi, id_o, first ? 0u : 1u,
+                        std::make_integer_sequence<int, KT / 16>());
             tc_commit(&bar.o_done[w]);
         };
-        while (walk.next(a)) {
-            const int rows = min(R, walk.fresh * a.G - walk.tile * R), nq = rows > 128 ? 2 : 1;
-            const int steps = walk.st1 - walk.st0;
-            for (int w = 0; w < nq; ++w) pf_wait(&bar.q_full[w], items[w]++ & 1, abort);
+        for (;;) {
+            pf_wait(&bar.q_full[0], items[0]++ & 1, abort);
+            const int rows = *reinterpret_cast<volatile int*>(&bar.rows), steps = *reinterpret_cast<volatile int*>(&bar.steps);
+            if (rows == 0 || *abort) break;
+            const int nq = rows > 128 ? 2 : 1;
+            if (nq == 2) pf_wait(&bar.q_full[1], items[1]++ & 1, abort);
             if constexpr (NQ == 2) {
                 pf_wait(&bar.k_full[it & 1], (it >> 1) & 1, abort);
                 tc_fence_after();
@@ -731,10 +1023,10 @@ __global__ void __launch_bounds__(PF_THREADS, 1) kv4_prefill_kernel(const Kv4Att
     }
     tc_fence_before();
     __syncthreads();
-    if (warp == PF_MMA) {
+    if (warp == 0) {
         __syncwarp();
         tc_fence_after();
-        tmem_dealloc(tmem, 512);
+        tmem_dealloc(*reinterpret_cast<volatile uint32_t*>(&tmem_base), 512);
     }
 }
 
@@ -752,20 +1044,48 @@ __global__ void __launch_bounds__(128) kv4_prefill_join_kernel(const Kv4AttArgs 
 
 // ---- host ----------------------------------------------------------------------------------------
 
-size_t kv4_prefill_workspace_bytes(int D, int sms) {
+// Unpack first where a request can have more than two tiles of rows, so that its keys would be unpacked again for each (a
+// tile's steps cost about twice as long with the unpacking beside them), and all keys that the table can name fit 1 GiB as
+// fp16 tiles.
+static bool pf_dense(int D, int B, int KVH, int G, int max_q, long long room, size_t* bytes, int* steps) {
+    const int R = D == 256 ? 128 : 256, KT = D == 256 ? 64 : 128;
+    const long long n = (room + KT - 1) / KT, tiles = n * B * KVH;
+    *steps = int(n);
+    *bytes = size_t(tiles) * (size_t(4) * KT * D + sizeof(int2));
+    return (long long)max_q * G > 2 * R && tiles <= (1LL << 30) / (4LL * KT * D) && B <= 65535 && KVH <= 65535;
+}
+
+static size_t pf_parts_bytes(int D, int sms) {
     const int R = D == 256 ? 128 : 256;
-    return size_t(sms) * 2 * R * (2 + D) * sizeof(float) + size_t(sms) * 8 * sizeof(int32_t);
+    return (size_t(sms) * 2 * R * (2 + D) * sizeof(float) + size_t(sms) * 8 * sizeof(int32_t) + 127) / 128 * 128;
+}
+
+size_t kv4_prefill_workspace_bytes(int D, int sms, int B, int KVH, int G, int max_q, long long room) {
+    size_t bytes;
+    int steps;
+    return pf_parts_bytes(D, sms) + (pf_dense(D, B, KVH, G, max_q, room, &bytes, &steps) ? (bytes + 127) / 128 * 128 : 0);
 }
 
 template <typename T, int D>
 static int kv4_prefill_d(Kv4AttArgs a, void* workspace, cudaStream_t st) {
     using S = PfShape<D>;
+    static std::atomic<uint32_t> set{0}, set_dense{0}, set_first{0}, none{0};
     const int n = device_info().sm_count;
     a.part_o = static_cast<float*>(workspace);
     a.part_ml = a.part_o + size_t(n) * 2 * S::R * D;
     a.records = reinterpret_cast<int32_t*>(a.part_ml + size_t(n) * 2 * S::R * 2);
-    static std::atomic<uint32_t> set{0}, none{0};
-    int rc = kv4_launch(kv4_prefill_kernel<T, D>, set, dim3(n), dim3(PF_THREADS), S::SMEM + 1024 + sizeof(PfBars), st, a);
+    size_t bytes;
+    const size_t smem = S::SMEM + 1024 + sizeof(PfBars);
+    int rc;
+    if (pf_dense(D, a.B, a.pool.KVH, a.G, a.max_q, (long long)a.width * a.pool.page, &bytes, &a.dense_steps)) {
+        a.dense = static_cast<uint8_t*>(workspace) + pf_parts_bytes(D, n);
+        a.dense_meta = reinterpret_cast<int2*>(a.dense + size_t(a.dense_steps) * a.B * a.pool.KVH * 2 * S::TB);
+        rc = kv4_launch(kv4_dense_kernel<T, D>, set_first, dim3(a.dense_steps, a.pool.KVH, a.B), dim3(PD_WARPS * 32),
+                        2 * S::TB + 128, st, a);
+        if (!rc) rc = kv4_launch(kv4_prefill_kernel<T, D, true>, set_dense, dim3(n), dim3(pf_threads(true)), smem, st, a);
+    } else {
+        rc = kv4_launch(kv4_prefill_kernel<T, D, false>, set, dim3(n), dim3(pf_threads(false)), smem, st, a);
+    }
     if (rc) return rc;
     return kv4_launch(kv4_prefill_join_kernel<T, D>, none, dim3(n, S::R / 4), dim3(128), 0, st, a);
 }

@@ -91,8 +91,8 @@ def _pool(keys: Sequence[torch.Tensor], values: Sequence[torch.Tensor], dtype: t
 
 
 @functools.lru_cache(maxsize=1024)
-def _attend_workspace(device: int, N: int, B: int, max_q: int, H: int, KVH: int, D: int) -> int:
-    return int(lib().lq_kv4_attend_workspace(N, B, max_q, H, KVH, D))
+def _attend_workspace(device: int, B: int, max_q: int, H: int, KVH: int, D: int, width: int, page: int) -> int:
+    return int(lib().lq_kv4_attend_workspace(B, max_q, H, KVH, D, width, page))
 
 
 def plan(cached: torch.Tensor, new: torch.Tensor, block_table: torch.Tensor, free: torch.Tensor, head: torch.Tensor,
@@ -210,7 +210,7 @@ def attend(q: torch.Tensor, keys: Sequence[torch.Tensor], values: Sequence[torch
     out = torch.empty_like(q)
     if N == 0:
         return out
-    nbytes = _attend_workspace(q.get_device(), N, B, max_q, H, KVH, D)
+    nbytes = _attend_workspace(q.get_device(), B, max_q, H, KVH, D, table[1], page)
     ws = q.new_empty(nbytes // 2) if nbytes else None
     call("lq_kv4_attend", q.data_ptr(), N, None if q_start is None else q_start.data_ptr(), max_q, *ptrs, pages, page,
          block_table.data_ptr(), table[1], lens.data_ptr(), B, None if sinks is None else sinks.data_ptr(), float(scale),
