@@ -59,6 +59,9 @@ struct PfShape {
     static_assert(2 * KT + NQ * D <= 512, "tensor memory columns");
 };
 
+// What an item costs beside its steps (queries fetched, the pipeline filled, outputs written), in steps.
+constexpr int PF_ITEM = 10;
+
 // A tile's steps of keys: from the first that its first row sees to the last that its last row sees.
 template <int D>
 __device__ __forceinline__ void pf_steps(const Kv4AttArgs& a, int base, int fresh, int tile, int* lo, int* hi) {
@@ -89,7 +92,7 @@ __device__ __forceinline__ long long pf_weight(const Kv4AttArgs& a, int b) {
     for (int t = 0; t < tiles; ++t) {
         int lo, hi;
         pf_steps<D>(a, base, fresh, t, &lo, &hi);
-        w += hi - lo;
+        w += hi - lo + PF_ITEM;
     }
     return w * a.pool.KVH;
 }
@@ -106,33 +109,37 @@ __device__ __forceinline__ long long pf_sum(long long v, long long* red) {
     return s;
 }
 
-// The CTA's walk over its share: items (request, tile, kv head) in that order, each with its steps [st0, st1).
+// The CTA's walk over its share: items (request, tile, kv head) in that order, each with its steps [st0, st1). A share is
+// counted in units: PF_ITEM of each item, then its steps.
 template <int D>
 struct PfWalk {
-    int left, skip;  // steps of the share left; steps of the next item that come before the share
+    int left, skip;  // units of the share left; units of the next item that come before the share
     bool begun;
     int b, tile, kvh, lo, hi, st0, st1, first, fresh, base, tiles;
 
-    // The next item; false when the share is done. Every caller walks alike.
+    // The next item with a step in the share; false when the share is done. Every caller walks alike.
     __device__ bool next(const Kv4AttArgs& a) {
-        if (left == 0) return false;
-        if (begun && ++kvh == a.pool.KVH) {
-            kvh = 0;
-            if (++tile >= tiles) {
-                do {
-                    ++b;
-                    tiles = pf_tiles<D>(a, b, &first, &fresh, &base);
-                } while (!tiles);
-                tile = 0;
+        while (left) {
+            if (begun && ++kvh == a.pool.KVH) {
+                kvh = 0;
+                if (++tile >= tiles) {
+                    do {
+                        ++b;
+                        tiles = pf_tiles<D>(a, b, &first, &fresh, &base);
+                    } while (!tiles);
+                    tile = 0;
+                }
+                pf_steps<D>(a, base, fresh, tile, &lo, &hi);
             }
-            pf_steps<D>(a, base, fresh, tile, &lo, &hi);
+            begun = true;
+            const int end = min(hi - lo + PF_ITEM, skip + left);
+            st0 = max(skip - PF_ITEM, 0);
+            st1 = max(end - PF_ITEM, 0);
+            left -= end - skip;
+            skip = 0;
+            if (st0 < st1) return true;
         }
-        begun = true;
-        st0 = skip;
-        st1 = min(hi - lo, skip + left);
-        left -= st1 - st0;
-        skip = 0;
-        return true;
+        return false;
     }
 };
 
@@ -142,6 +149,8 @@ __device__ __forceinline__ void pf_tmem_st8(uint32_t taddr, const uint32_t (&r)[
                  : "memory");
 }
 
+__device__ __forceinline__ void pf_tmem_ld(uint32_t taddr, uint32_t (&r)[16]) { tmem_ld_32x32b_x16(taddr, r); }
+__device__ __forceinline__ void pf_tmem_ld(uint32_t taddr, uint32_t (&r)[32]) { tmem_ld_32x32b_x32(taddr, r); }
 __device__ __forceinline__ void pf_tmem_st32(uint32_t taddr, const uint32_t* r) {
     asm volatile(
         "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,"
@@ -426,7 +435,7 @@ __global__ void __launch_bounds__(pf_threads(DENSE), 1) kv4_prefill_kernel(const
         for (;; t0 += PF_THREADS) {
             int lo = 0, hi = 0;
             if (t0 + tid < walk.tiles) pf_steps<D>(a, walk.base, walk.fresh, t0 + tid, &lo, &hi);
-            const long long w = (long long)(hi - lo) * a.pool.KVH;
+            const long long w = t0 + tid < walk.tiles ? (long long)(hi - lo + PF_ITEM) * a.pool.KVH : 0;
             const long long sum = pf_sum(w, red);
             if (at + sum <= x0) {
                 at += sum;
@@ -448,15 +457,15 @@ __global__ void __launch_bounds__(pf_threads(DENSE), 1) kv4_prefill_kernel(const
             break;
         }
         pf_steps<D>(a, walk.base, walk.fresh, walk.tile, &walk.lo, &walk.hi);
-        const int steps = walk.hi - walk.lo;
-        walk.kvh = int((x0 - at) / steps);
-        const long long item = at + (long long)walk.kvh * steps;
+        const int units = walk.hi - walk.lo + PF_ITEM;
+        walk.kvh = int((x0 - at) / units);
+        const long long item = at + (long long)walk.kvh * units;
         walk.skip = int(x0 - item);
         walk.left = int(x1 - x0);
         walk.begun = false;
         if (tid == 0) {
-            const int c0 = kv4_owner(item, total, n), c1 = kv4_owner(item + steps - 1, total, n);
-            rec[0] = item < x0 && c0 == int(blockIdx.x) - 1;  // the first boundary within its item
+            const int c0 = kv4_owner(item + PF_ITEM, total, n), c1 = kv4_owner(item + units - 1, total, n);
+            rec[0] = walk.skip > PF_ITEM && c0 == int(blockIdx.x) - 1;  // the first boundary within its item's steps
             rec[1] = walk.first;
             rec[2] = walk.tile * R;
             rec[3] = min(R, walk.fresh * a.G - walk.tile * R);
@@ -541,12 +550,17 @@ __global__ void __launch_bounds__(pf_threads(DENSE), 1) kv4_prefill_kernel(const
             float c;
             {
                 const uint4* src = reinterpret_cast<const uint4*>(a.q + qo);
+                constexpr int NV = D == 256 ? 16 : D / 8;  // 16-byte pieces held at a time
+                const bool some = live && a.scale_log2 != 0.0f;
+                uint4 raw[NV];
                 float mx = 0.0f;
-                if (live && a.scale_log2 != 0.0f) {
-#pragma unroll 4
-                    for (int i = 0; i < D / 8; ++i) {
-                        const uint4 v = src[i];
-                        const uint32_t x[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                for (int h = 0; h < D / 8; h += NV) {
+#pragma unroll
+                    for (int i = 0; i < NV; ++i) raw[i] = some ? src[h + i] : make_uint4(0, 0, 0, 0);
+#pragma unroll
+                    for (int i = 0; i < NV; ++i) {
+                        const uint32_t x[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
 #pragma unroll
                         for (int k = 0; k < 4; ++k)
                             mx = fmaxf(mx, fmaxf(fabsf(F16Traits<T>::to_f32(x[k] & 0xffffu)),
@@ -555,23 +569,29 @@ __global__ void __launch_bounds__(pf_threads(DENSE), 1) kv4_prefill_kernel(const
                 }
                 int E = mx > 0.0f ? 12 - (int((__float_as_uint(mx) >> 23) & 0xff) - 127) : 0;
                 E = min(max(E, -100), 100);
-                const float f = live && a.scale_log2 != 0.0f ? copysignf(__uint_as_float(uint32_t(127 + E) << 23), a.scale_log2) : 0.0f;
+                const float f = some ? copysignf(__uint_as_float(uint32_t(127 + E) << 23), a.scale_log2) : 0.0f;
                 c = a.scale_log2 != 0.0f ? fabsf(a.scale_log2) * __uint_as_float(uint32_t(127 - E) << 23) : 1.0f;
                 const uint32_t dst = sq + w * S::QB + wr * 128;
-#pragma unroll 4
-                for (int i = 0; i < D / 8; ++i) {
-                    const uint4 v = live ? src[i] : make_uint4(0, 0, 0, 0);
-                    const uint32_t x[4] = {v.x, v.y, v.z, v.w};
-                    float q[8];
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        q[2 * k] = F16Traits<T>::to_f32(x[k] & 0xffffu) * f;
-                        q[2 * k + 1] = F16Traits<T>::to_f32(x[k] >> 16) * f;
+                for (int h = 0; h < D / 8; h += NV) {
+                    if (D / 8 > NV) {
+#pragma unroll
+                        for (int i = 0; i < NV; ++i) raw[i] = some ? src[h + i] : make_uint4(0, 0, 0, 0);
                     }
-                    asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(dst + (i >> 3) * 16384 + (((i & 7) ^ (wr & 7)) << 4)),
-                                 "r"(cvt_f16x2(q[4], q[0])), "r"(cvt_f16x2(q[5], q[1])), "r"(cvt_f16x2(q[6], q[2])),
-                                 "r"(cvt_f16x2(q[7], q[3]))
-                                 : "memory");
+#pragma unroll
+                    for (int i = 0; i < NV; ++i) {
+                        const uint32_t x[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+                        float q[8];
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            q[2 * k] = F16Traits<T>::to_f32(x[k] & 0xffffu) * f;
+                            q[2 * k + 1] = F16Traits<T>::to_f32(x[k] >> 16) * f;
+                        }
+                        asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(dst + ((h + i) >> 3) * 16384 + (((i & 7) ^ (wr & 7)) << 4)),
+                                     "r"(cvt_f16x2(q[4], q[0])), "r"(cvt_f16x2(q[5], q[1])), "r"(cvt_f16x2(q[6], q[2])),
+                                     "r"(cvt_f16x2(q[7], q[3]))
+                                     : "memory");
+                    }
                 }
             }
             if (warp == PF_FIRST && lane == 0) bar.rows = rows, bar.steps = steps;
@@ -596,25 +616,27 @@ __global__ void __launch_bounds__(pf_threads(DENSE), 1) kv4_prefill_kernel(const
                 // before serves it (found out at the end: the probabilities stay in registers until then, the scores in place).
                 if (all && ve_t == ve && __all_sync(0xffffffffu, m != -INFINITY)) {
                     const uint64_t c2 = pf_pair(c, c), m2 = pf_pair(-m, -m);
-                    uint32_t r[2][16], p[KT / 2];
+                    constexpr int CH = 16;  // scores at a time (32: 1082 against 1040 us for a 4096-token prompt piece)
+                    uint32_t r[2][CH], p[KT / 2];
                     uint64_t sums[2] = {0, 0};
                     float mx[2] = {-INFINITY, -INFINITY};
-                    tmem_ld_32x32b_x16(s_col, r[0]);
+                    pf_tmem_ld(s_col, r[0]);
 #pragma unroll
-                    for (int ch = 0; ch < KT / 16; ++ch) {  // the next 16 scores are read while these are worked on
-                        uint32_t(&x)[16] = r[ch & 1];
+                    for (int ch = 0; ch < KT / CH; ++ch) {  // the next scores are read while these are worked on
+                        uint32_t(&x)[CH] = r[ch & 1];
                         tmem_wait_ld();
-                        if (ch + 1 < KT / 16) tmem_ld_32x32b_x16(s_col + ch * 16 + 16, r[(ch + 1) & 1]);
+                        if (ch + 1 < KT / CH) pf_tmem_ld(s_col + (ch + 1) * CH, r[(ch + 1) & 1]);
 #pragma unroll
-                        for (int i = 0; i < 16; i += 2) {
+                        for (int i = 0; i < CH; i += 2) {
                             const float s0 = __uint_as_float(x[i]), s1 = __uint_as_float(x[i + 1]);
                             mx[(i >> 1) & 1] = fmaxf(fmaxf(mx[(i >> 1) & 1], s0), s1);
                             float e0, e1;
-                            pf_unpair(pf_fma2(pf_pair(s0, s1), c2, m2), &e0, &e1);
+                            const uint64_t x2 = pf_fma2(pf_pair(s0, s1), c2, m2);
+                            pf_unpair(x2, &e0, &e1);
                             e0 = kv4_ex2(e0);
                             e1 = kv4_ex2(e1);
                             sums[(i >> 1) & 1] = pf_add2(sums[(i >> 1) & 1], pf_pair(e0, e1));
-                            p[ch * 8 + i / 2] = cvt_f16x2(e1, e0);
+                            p[(ch * CH + i) / 2] = cvt_f16x2(e1, e0);
                         }
                     }
                     if (!__any_sync(0xffffffffu, fmaxf(mx[0], mx[1]) * c > m + 8.0f)) {
