@@ -111,6 +111,22 @@ def lib():
     return _lib
 
 
+_ext = None
+
+
+def ext():
+    """The loaded _paged_ext.so (built beside liblq.so, which it is linked to): the host side of paged.py and rotary.py."""
+    global _ext
+    if _ext is None:
+        lib()
+        try:
+            from . import _paged_ext
+        except ImportError as e:
+            raise RuntimeError(f"_paged_ext.so is missing or does not load ({e}): run `python -m locals_b200.build`") from e
+        _ext = _paged_ext
+    return _ext
+
+
 def call(name: str, *args) -> None:
     rc = getattr(lib(), name)(*args)
     if rc != LQ_OK:

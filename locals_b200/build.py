@@ -4,6 +4,9 @@
     python -m locals_b200.build --force    # recompile every translation unit
     python -m locals_b200.build -v         # with ptxas register / spill / shared-memory reports
 
+and _paged_ext.so beside it (csrc/paged_ext.cpp with the host compiler against the installed torch: the Python side of
+paged.py and rotary.py, linked to liblq.so).
+
 Each csrc/*.cu file is its own translation unit (compiled in parallel into csrc/../_build/*.o, then linked with the
 static CUDA runtime). The library is rebuilt whenever the hash of its sources, headers and flags differs from the
 one recorded beside it (liblq.so.srchash) -- never on file times alone, so a library left over from other sources
@@ -24,6 +27,9 @@ CSRC = os.path.join(HERE, "csrc")
 OBJ = os.path.join(HERE, "_build")
 LIB = os.path.join(HERE, "liblq.so")
 HASH = LIB + ".srchash"
+EXT = os.path.join(HERE, "_paged_ext.so")
+EXT_SRC = os.path.join(CSRC, "paged_ext.cpp")
+EXT_HASH = EXT + ".srchash"
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 HEADER = os.path.join(HERE, "..", "include", "lq.h")
 
@@ -100,7 +106,47 @@ def _compile(unit, verbose):
     return obj, r.stderr
 
 
+def _ext_hash() -> str:
+    import torch
+
+    return _digest([EXT_SRC, HEADER], torch.__version__)
+
+
+def build_ext(force: bool = False) -> str:
+    """_paged_ext.so, rebuilt when its source, include/lq.h or the torch version changes."""
+    want = _ext_hash()
+    if not force and os.path.exists(EXT) and os.path.exists(EXT_HASH):
+        with open(EXT_HASH) as f:
+            if f.read().strip() == want:
+                return EXT
+    import sysconfig
+
+    import torch
+    from torch.utils import cpp_extension
+
+    cuda = os.path.dirname(os.path.dirname(os.path.realpath(NVCC)))
+    includes = [*cpp_extension.include_paths(), sysconfig.get_paths()["include"], os.path.join(cuda, "include")]
+    libs = os.path.join(os.path.dirname(torch.__file__), "lib")
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *[f"-I{p}" for p in includes], EXT_SRC,
+           "-o", EXT + ".tmp", f"-L{libs}", "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_cuda",
+           f"-L{HERE}", "-l:liblq.so", "-Wl,-rpath,$ORIGIN"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"{cmd[0]} failed on {os.path.basename(EXT_SRC)}:\n{r.stdout}\n{r.stderr}")
+    os.replace(EXT + ".tmp", EXT)
+    with open(EXT_HASH, "w") as f:
+        f.write(want)
+    return EXT
+
+
 def build(force: bool = False, verbose: bool = False) -> str:
+    lib = _build_lib(force, verbose)
+    build_ext(force)
+    return lib
+
+
+def _build_lib(force: bool, verbose: bool) -> str:
     if not force and not verbose and up_to_date():
         return LIB
     os.makedirs(OBJ, exist_ok=True)

@@ -50,7 +50,7 @@ __device__ __forceinline__ uint32_t kv4_transpose(uint32_t x) {
 }
 
 // What an item costs beside its steps (pages and queries fetched, the ring filled, the warps joined), in steps.
-constexpr int KV4_ITEM = 2;
+constexpr int KV4_ITEM = 5;
 
 __device__ __forceinline__ Kv4Req kv4_request(const Kv4AttArgs& a, int b) {
     Kv4Req r = kv4_new(a, b);
