@@ -43,6 +43,11 @@ namespace lq {
 constexpr int KV4_NW = 4;                 // warps a CTA
 constexpr int KV4_KEYS = 32;              // keys a warp step
 constexpr int KV4_STEP = KV4_NW * KV4_KEYS;  // keys a CTA step
+__device__ __forceinline__ uint32_t kv4_cluster_size() {
+    uint32_t n;
+    asm("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(n));
+    return n;
+}
 __device__ __forceinline__ uint32_t kv4_transpose(uint32_t x) {
     uint32_t y;
     asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
@@ -141,7 +146,9 @@ __device__ __forceinline__ void kv4_floats(uint32_t addr, float (&f)[N]) {
 // CTAs a SM, by registers (8 rows: 128 / 168 / 255 a thread) and shared memory.
 constexpr int kv4_resident(int D, int NT) { return NT == 2 || D == 256 ? 2 : D == 128 ? 3 : 4; }
 
-template <typename T, int D, int NT>
+// CL: one cluster of CTAs an item, each with a run of its steps, joined through distributed shared memory instead of the
+// workspace and a second launch.
+template <typename T, int D, int NT, bool CL>
 __global__ void __launch_bounds__(KV4_NW * 32, kv4_resident(D, NT)) kv4_attend_kernel(const Kv4AttArgs a) {
     using S = Kv4Shape<D>;
     constexpr int GR = S::GR, R = 8 * NT;
@@ -153,38 +160,40 @@ __global__ void __launch_bounds__(KV4_NW * 32, kv4_resident(D, NT)) kv4_attend_k
 
     kv4_zero_tail(a, D);
 
-    // ---- this CTA's share of the steps: requests are scanned 128 at a time ----
-    const int w0 = kv4_weight(a, tid);
-    int sum0;
-    const int s0 = kv4_scan(w0, red, &sum0);
-    long long total = sum0;
-    for (int b0 = KV4_NW * 32; b0 < a.B; b0 += KV4_NW * 32) {
-        int sum;
-        kv4_scan(kv4_weight(a, b0 + tid), red, &sum);
-        total += sum;
-    }
-    const int n = int(min((long long)gridDim.x, total));  // (every CTA below n has a step, those above none)
-    int32_t* rec = a.records + blockIdx.x * 8;  // what the join kernel does for this CTA's first step
-    if (tid == 0) rec[0] = 0;
-    if (int(blockIdx.x) >= n) return;
-    const long long x0 = (long long)blockIdx.x * total / n, x1 = ((long long)blockIdx.x + 1) * total / n;
-    int b = 0;
-    long long at = 0;  // steps before request b
-    for (int b0 = 0;; b0 += KV4_NW * 32) {
-        int sum = sum0, s = s0, w = w0;
-        if (b0) {
-            w = kv4_weight(a, b0 + tid);
-            s = kv4_scan(w, red, &sum);
+    int b = 0, n = 0;
+    long long at = 0, total = 0, x0 = 0, x1 = 1;  // steps before request b; of all; this CTA's
+    int32_t* rec = a.records + blockIdx.x * 8;    // what the join kernel does for this CTA's first step
+    if constexpr (!CL) {
+        // ---- this CTA's share of the steps: requests are scanned 128 at a time ----
+        const int w0 = kv4_weight(a, tid);
+        int sum0;
+        const int s0 = kv4_scan(w0, red, &sum0);
+        total = sum0;
+        for (int b0 = KV4_NW * 32; b0 < a.B; b0 += KV4_NW * 32) {
+            int sum;
+            kv4_scan(kv4_weight(a, b0 + tid), red, &sum);
+            total += sum;
         }
-        if (at + sum <= x0) {
-            at += sum;
-            continue;
+        n = int(min((long long)gridDim.x, total));  // (every CTA below n has a step, those above none)
+        if (tid == 0) rec[0] = 0;
+        if (int(blockIdx.x) >= n) return;
+        x0 = (long long)blockIdx.x * total / n, x1 = ((long long)blockIdx.x + 1) * total / n;
+        for (int b0 = 0;; b0 += KV4_NW * 32) {
+            int sum = sum0, s = s0, w = w0;
+            if (b0) {
+                w = kv4_weight(a, b0 + tid);
+                s = kv4_scan(w, red, &sum);
+            }
+            if (at + sum <= x0) {
+                at += sum;
+                continue;
+            }
+            if (at + s > x0 && at + s - w <= x0) found[0] = b0 + tid, found[1] = s - w;  // one thread's
+            __syncthreads();
+            b = found[0];
+            at += found[1];
+            break;
         }
-        if (at + s > x0 && at + s - w <= x0) found[0] = b0 + tid, found[1] = s - w;  // one thread's
-        __syncthreads();
-        b = found[0];
-        at += found[1];
-        break;
     }
 
     const uint32_t ring = smem_u32(kv4_smem) + warp * S::WARP;
@@ -204,26 +213,36 @@ __global__ void __launch_bounds__(KV4_NW * 32, kv4_resident(D, NT)) kv4_attend_k
 
     long long x = x0;
     while (x < x1) {
+        int kvh, st0, st1;
+        if constexpr (CL) b = int(blockIdx.x / kv4_cluster_size()) / KVH;
         const Kv4Req rq = kv4_request(a, b);
-        const int units = rq.steps() + KV4_ITEM;
-        const int kvh = int((x - at) / units);
-        if (!rq.fresh || kvh >= KVH) {  // on to the next request
-            if (rq.fresh) at += (long long)units * KVH;
-            ++b;
-            continue;
-        }
-        const long long item_at = at + (long long)kvh * units;
-        const int u1 = int(min((long long)units, x1 - item_at));
-        const int st0 = max(int(x - item_at) - KV4_ITEM, 0), st1 = max(u1 - KV4_ITEM, 0);
-        x = item_at + u1;
-        if (st0 == st1) continue;
-        if (st0 > 0 && tid == 0) {  // (only a CTA's first item can begin before it)
-            const long long key0 = item_at + KV4_ITEM;
-            rec[1] = rq.first;
-            rec[2] = rq.fresh * G;
-            rec[3] = kvh;
-            rec[4] = kv4_owner(key0 + rq.steps() - 1, total, n);
-            rec[0] = kv4_owner(key0, total, n) == int(blockIdx.x) - 1;  // the first boundary within its item
+        if constexpr (CL) {
+            kvh = int(blockIdx.x / kv4_cluster_size()) - b * KVH;
+            st0 = rq.steps() * int(cluster_ctarank()) / int(kv4_cluster_size());
+            st1 = rq.steps() * int(cluster_ctarank() + 1) / int(kv4_cluster_size());
+            x = x1;
+            if (!rq.fresh) return;  // (the whole cluster)
+        } else {
+            const int units = rq.steps() + KV4_ITEM;
+            kvh = int((x - at) / units);
+            if (!rq.fresh || kvh >= KVH) {  // on to the next request
+                if (rq.fresh) at += (long long)units * KVH;
+                ++b;
+                continue;
+            }
+            const long long item_at = at + (long long)kvh * units;
+            const int u1 = int(min((long long)units, x1 - item_at));
+            st0 = max(int(x - item_at) - KV4_ITEM, 0), st1 = max(u1 - KV4_ITEM, 0);
+            x = item_at + u1;
+            if (st0 == st1) continue;
+            if (st0 > 0 && tid == 0) {  // (only a CTA's first item can begin before it)
+                const long long key0 = item_at + KV4_ITEM;
+                rec[1] = rq.first;
+                rec[2] = rq.fresh * G;
+                rec[3] = kvh;
+                rec[4] = kv4_owner(key0 + rq.steps() - 1, total, n);
+                rec[0] = kv4_owner(key0, total, n) == int(blockIdx.x) - 1;  // the first boundary within its item
+            }
         }
         const int rows = rq.fresh * G;
         // what the rows see: keys below hi_max, from lo_min on; all of them see [lo_max, hi_min)
@@ -610,7 +629,7 @@ __global__ void __launch_bounds__(KV4_NW * 32, kv4_resident(D, NT)) kv4_attend_k
             sb_issue = sb_issue == ring + (S::STAGES - 1) * S::STAGE ? ring : sb_issue + S::STAGE;
         }
         asm volatile("cp.async.wait_group 0;" ::: "memory");
-        if (x >= x1) grid_dep_launch();
+        if (CL || x >= x1) grid_dep_launch();
 
         // ---- the four warps' states joined in shared memory (over the rings) ----
 #pragma unroll
@@ -643,7 +662,8 @@ __global__ void __launch_bounds__(KV4_NW * 32, kv4_resident(D, NT)) kv4_attend_k
                                         fmaf(o[t][4 * g + i][2 + e], 1048576.0f, hb[t][g][e]) * inv);
             }
         __syncthreads();
-        const bool whole = st0 == 0 && st1 == rq.steps();
+        const bool whole = !CL && st0 == 0 && st1 == rq.steps();
+        float* mine = co + KV4_NW * R * D;  // (CL) this CTA's [R] m, [R] l, [R][D] O
         const size_t part = ((size_t)blockIdx.x * 2 + (st0 == 0 ? 1 : 0)) * R;
         for (int j = 0; j < rows; ++j) {
             float M = -INFINITY;
@@ -663,10 +683,37 @@ __global__ void __launch_bounds__(KV4_NW * 32, kv4_resident(D, NT)) kv4_attend_k
                     if (f[w] != 0.0f) O += co[(w * R + j) * D + d] * f[w];
                 if (whole)
                     a.out[((size_t)(rq.first + qi) * a.H + head) * D + d] = kv4_finish<T>(M, L, O, kv4_sink(a.sinks, head));
+                else if (CL)
+                    mine[2 * R + j * D + d] = O;
                 else
                     a.part_o[(part + j) * D + d] = O;
             }
-            if (!whole && tid == 0) a.part_ml[2 * (part + j)] = M, a.part_ml[2 * (part + j) + 1] = L;
+            if (CL && tid == 0) mine[j] = M, mine[R + j] = L;
+            if (!CL && !whole && tid == 0) a.part_ml[2 * (part + j)] = M, a.part_ml[2 * (part + j) + 1] = L;
+        }
+        if constexpr (CL) {
+            cluster_sync();
+            const int C = int(kv4_cluster_size());
+            const uint32_t base32 = smem_u32(mine);
+            for (int j = int(cluster_ctarank()); j < rows; j += C) {
+                float M = -INFINITY;
+                for (int k = 0; k < C; ++k) M = fmaxf(M, ld_dsmem_f(map_peer(base32 + j * 4, k)));
+                const int qi = j / G, head = kvh * G + j - qi * G;
+                const float sink = kv4_sink(a.sinks, head);
+                for (int d = tid; d < D; d += KV4_NW * 32) {
+                    float L = 0.0f, O = 0.0f;
+                    for (int k = 0; k < C; ++k) {
+                        const uint32_t peer = map_peer(base32, k);
+                        const float m = ld_dsmem_f(peer + j * 4), l = ld_dsmem_f(peer + (R + j) * 4);
+                        const float o = ld_dsmem_f(peer + (2 * R + j * D + d) * 4);
+                        const float f = m == -INFINITY ? 0.0f : kv4_ex2(m - M);
+                        L += l * f;  // (a NaN's l has no m: NaN * 0)
+                        if (f != 0.0f) O += o * f;
+                    }
+                    a.out[((size_t)(rq.first + qi) * a.H + head) * D + d] = kv4_finish<T>(M, L, O, sink);
+                }
+            }
+            cluster_sync();  // no CTA leaves while another reads it
         }
         __syncthreads();  // before the next item's ring
     }
@@ -721,14 +768,28 @@ size_t kv4_attend_workspace_bytes(int B, int max_q, int H, int KVH, int D, long 
     return (split ? kv4_few_bytes(D, R, sms) : 0) + (many ? kv4_prefill_workspace_bytes(D, sms, B, KVH, H / KVH, max_q, room) : 0);
 }
 
+// CTAs a cluster where the clustered form is used, 0 where it is not: as many (up to 8) as leave every item's cluster
+// resident at once, if no request can have more than 8 steps a CTA. That spares the second launch and the scan of the
+// lengths; beyond, the even split is worth more (items differ, and steps go to every SM).
+static int kv4_cluster(const Kv4AttArgs& a, int D, int R, int sms) {
+    const long long items = (long long)a.B * a.pool.KVH, room = (long long)a.width * a.pool.page;
+    const long long seen = a.window ? (room < (long long)a.window + a.max_q + KV4_STEP ? room : (long long)a.window + a.max_q + KV4_STEP) : room;
+    const long long steps = (seen + KV4_STEP - 1) / KV4_STEP;
+    int C = 8;
+    while (C > 1 && (items * C > kv4_ctas(D, R, sms) || C / 2 >= steps)) C /= 2;
+    return items * C <= kv4_ctas(D, R, sms) && steps <= 8 * C ? C : 0;
+}
+
 template <typename T, int D, int NT>
 static int kv4_attend_n(Kv4AttArgs a, cudaStream_t st) {
     constexpr int R = 8 * NT;
-    constexpr size_t merge = size_t(KV4_NW) * R * (2 + D) * sizeof(float);
+    constexpr size_t merge = size_t(KV4_NW + 1) * R * (2 + D) * sizeof(float);
     constexpr size_t smem = merge > size_t(Kv4Shape<D>::RING) ? merge : size_t(Kv4Shape<D>::RING);
-    const int n = kv4_ctas(D, R, device_info().sm_count);
-    static std::atomic<uint32_t> set{0}, none{0};
-    int rc = kv4_launch(kv4_attend_kernel<T, D, NT>, set, dim3(n), dim3(KV4_NW * 32), smem, st, a);
+    static std::atomic<uint32_t> set{0}, set_cl{0}, none{0};
+    const int sms = device_info().sm_count, C = kv4_cluster(a, D, R, sms), n = kv4_ctas(D, R, sms);
+    if (C)
+        return kv4_launch(kv4_attend_kernel<T, D, NT, true>, set_cl, dim3(a.B * a.pool.KVH * C), dim3(KV4_NW * 32), smem, st, a, C);
+    int rc = kv4_launch(kv4_attend_kernel<T, D, NT, false>, set, dim3(n), dim3(KV4_NW * 32), smem, st, a);
     if (rc) return rc;
     return kv4_launch(kv4_join_kernel<T, D, NT>, none, dim3(n, a.split_rows), dim3(128), 0, st, a);
 }

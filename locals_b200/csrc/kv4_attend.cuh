@@ -171,7 +171,8 @@ __device__ __forceinline__ void kv4_join_row(const Kv4AttArgs& a, int R, int j, 
 // The shared-memory limit is an attribute of the function on a device: set at the kernel's first launch on each (`set`
 // has a bit a device), not at every launch, where it costs about as much as a small launch itself.
 template <typename K, typename A>
-static int kv4_launch(K kern, std::atomic<uint32_t>& set, dim3 grid, dim3 block, size_t smem, cudaStream_t st, const A& a) {
+static int kv4_launch(K kern, std::atomic<uint32_t>& set, dim3 grid, dim3 block, size_t smem, cudaStream_t st, const A& a,
+                      int cluster = 1) {
     if (smem > 48 * 1024) {
         const uint32_t bit = 1u << (device_info().device & 31);
         if (!(set.load(std::memory_order_relaxed) & bit)) {
@@ -185,11 +186,14 @@ static int kv4_launch(K kern, std::atomic<uint32_t>& set, dim3 grid, dim3 block,
     cfg.blockDim = block;
     cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
-    cudaLaunchAttribute attr[1];
+    cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = cluster;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = 1;
+    cfg.numAttrs = cluster > 1 ? 2 : 1;
     return cudaLaunchKernelEx(&cfg, kern, a) == cudaSuccess ? LQ_OK : LQ_E_CUDA;
 }
 
