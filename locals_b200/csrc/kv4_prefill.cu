@@ -60,7 +60,7 @@ struct PfShape {
 };
 
 // What an item costs beside its steps (queries fetched, the pipeline filled, outputs written), in steps.
-constexpr int PF_ITEM = 10;
+constexpr int PF_ITEM = 7;
 
 // A tile's steps of keys: from the first that its first row sees to the last that its last row sees.
 template <int D>
@@ -149,8 +149,6 @@ __device__ __forceinline__ void pf_tmem_st8(uint32_t taddr, const uint32_t (&r)[
                  : "memory");
 }
 
-__device__ __forceinline__ void pf_tmem_ld(uint32_t taddr, uint32_t (&r)[16]) { tmem_ld_32x32b_x16(taddr, r); }
-__device__ __forceinline__ void pf_tmem_ld(uint32_t taddr, uint32_t (&r)[32]) { tmem_ld_32x32b_x32(taddr, r); }
 __device__ __forceinline__ void pf_tmem_st32(uint32_t taddr, const uint32_t* r) {
     asm volatile(
         "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,"
@@ -612,52 +610,64 @@ __global__ void __launch_bounds__(pf_threads(DENSE), 1) kv4_prefill_kernel(const
                 const int ve_t = *reinterpret_cast<volatile int*>(&bar.v_exp[it & 3]);
                 const bool all = key0 >= lo_all && key0 + KT <= hi_all && miss == 0;
                 const uint32_t s_col = tmem + lanes + buf * KT;
-                // The common case, one pass: every row of the warp sees the whole step, and the reference from the steps
-                // before serves it (found out at the end: the probabilities stay in registers until then, the scores in place).
-                if (all && ve_t == ve && __all_sync(0xffffffffu, m != -INFINITY)) {
+                // what this row sees of the step, a bit a key
+                uint32_t vis[KT / 32];
+#pragma unroll
+                for (int i = 0; i < KT / 32; ++i) {
+                    const int from = min(max(row_lo - key0 - 32 * i, 0), 32), to = min(max(row_hi - key0 - 32 * i, 0), 32);
+                    vis[i] = all ? 0xffffffffu : uint32_t((1ull << to) - 1) & ~uint32_t((1ull << from) - 1);
+                    if (miss) {
+#pragma unroll
+                        for (int k = 0; k < 4; ++k)
+                            if ((miss >> (4 * i + k)) & 1) vis[i] &= ~(0xffu << (8 * k));
+                    }
+                }
+                auto seen = [&](uint32_t score, int i) {
+                    return (vis[i >> 5] >> (i & 31)) & 1 ? __uint_as_float(score) : -INFINITY;
+                };
+                // The common case, one pass: the reference from the steps before serves the step (found out at its end: the
+                // probabilities stay in registers until then, the scores in place).
+                auto once = [&](auto masked) -> bool {
                     const uint64_t c2 = pf_pair(c, c), m2 = pf_pair(-m, -m);
                     constexpr int CH = 16;  // scores at a time (32: 1082 against 1040 us for a 4096-token prompt piece)
                     uint32_t r[2][CH], p[KT / 2];
                     uint64_t sums[2] = {0, 0};
                     float mx[2] = {-INFINITY, -INFINITY};
-                    pf_tmem_ld(s_col, r[0]);
+                    tmem_ld_32x32b_x16(s_col, r[0]);
 #pragma unroll
                     for (int ch = 0; ch < KT / CH; ++ch) {  // the next scores are read while these are worked on
                         uint32_t(&x)[CH] = r[ch & 1];
                         tmem_wait_ld();
-                        if (ch + 1 < KT / CH) pf_tmem_ld(s_col + (ch + 1) * CH, r[(ch + 1) & 1]);
+                        if (ch + 1 < KT / CH) tmem_ld_32x32b_x16(s_col + (ch + 1) * CH, r[(ch + 1) & 1]);
 #pragma unroll
                         for (int i = 0; i < CH; i += 2) {
-                            const float s0 = __uint_as_float(x[i]), s1 = __uint_as_float(x[i + 1]);
+                            float s0 = __uint_as_float(x[i]), s1 = __uint_as_float(x[i + 1]);
+                            if constexpr (decltype(masked)::value) s0 = seen(x[i], ch * CH + i), s1 = seen(x[i + 1], ch * CH + i + 1);
                             mx[(i >> 1) & 1] = fmaxf(fmaxf(mx[(i >> 1) & 1], s0), s1);
                             float e0, e1;
-                            const uint64_t x2 = pf_fma2(pf_pair(s0, s1), c2, m2);
-                            pf_unpair(x2, &e0, &e1);
+                            pf_unpair(pf_fma2(pf_pair(s0, s1), c2, m2), &e0, &e1);
                             e0 = kv4_ex2(e0);
                             e1 = kv4_ex2(e1);
                             sums[(i >> 1) & 1] = pf_add2(sums[(i >> 1) & 1], pf_pair(e0, e1));
                             p[(ch * CH + i) / 2] = cvt_f16x2(e1, e0);
                         }
                     }
-                    if (!__any_sync(0xffffffffu, fmaxf(mx[0], mx[1]) * c > m + 8.0f)) {
+                    if (__any_sync(0xffffffffu, fmaxf(mx[0], mx[1]) * c > m + 8.0f)) return false;
 #pragma unroll
-                        for (int ch = 0; ch < KT / 64; ++ch) pf_tmem_st32(s_col + ch * 32, &p[ch * 32]);
-                        float a0, a1, b0, b1;
-                        pf_unpair(sums[0], &a0, &a1);
-                        pf_unpair(sums[1], &b0, &b1);
-                        l += (a0 + a1) + (b0 + b1);
-                        tmem_wait_st();
-                        tc_fence_before();
-                        __syncwarp();
-                        if (lane == 0) mbar_arrive(&bar.p_full[buf]);
-                        continue;
-                    }
-                }
-                // whether this row sees place i of the step
-                auto in = [&](int i) {
-                    const int key = key0 + i;
-                    return key >= row_lo && key < row_hi && !((miss >> (i / 8)) & 1);
+                    for (int ch = 0; ch < KT / 64; ++ch) pf_tmem_st32(s_col + ch * 32, &p[ch * 32]);
+                    float a0, a1, b0, b1;
+                    pf_unpair(sums[0], &a0, &a1);
+                    pf_unpair(sums[1], &b0, &b1);
+                    l += (a0 + a1) + (b0 + b1);
+                    tmem_wait_st();
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&bar.p_full[buf]);
+                    return true;
                 };
+                if (ve_t == ve && __all_sync(0xffffffffu, m != -INFINITY)) {
+                    if (all ? once(std::false_type()) : once(std::true_type())) continue;
+                }
                 float mx = -INFINITY;
 #pragma unroll
                 for (int ch = 0; ch < KT / 64; ++ch) {
@@ -665,16 +675,12 @@ __global__ void __launch_bounds__(pf_threads(DENSE), 1) kv4_prefill_kernel(const
                     tmem_ld_32x32b_x32(s_col + ch * 64, r[0]);
                     tmem_ld_32x32b_x32(s_col + ch * 64 + 32, r[1]);
                     tmem_wait_ld();
-                    float part[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-                    if (all) {
+                    float part[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-                        for (int i = 0; i < 64; ++i) part[i & 3] = fmaxf(part[i & 3], __uint_as_float(r[i >> 5][i & 31]));
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < 64; ++i)
-                            part[i & 3] = fmaxf(part[i & 3], in(ch * 64 + i) ? __uint_as_float(r[i >> 5][i & 31]) : -INFINITY);
-                    }
-                    mx = fmaxf(mx, fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3])));
+                    for (int i = 0; i < 64; i += 2)
+                        part[(i >> 1) & 1] = fmaxf(fmaxf(part[(i >> 1) & 1], seen(r[i >> 5][i & 31], ch * 64 + i)),
+                                                   seen(r[i >> 5][(i & 31) + 1], ch * 64 + i + 1));
+                    mx = fmaxf(mx, fmaxf(part[0], part[1]));
                 }
                 const float mn = fmaxf(m, mx * c);
                 const bool grow = mn > m + 8.0f || (m == -INFINITY && mn > m) || ve_t != ve;
@@ -699,34 +705,24 @@ __global__ void __launch_bounds__(pf_threads(DENSE), 1) kv4_prefill_kernel(const
                 }
                 const float mz = m == -INFINITY ? 0.0f : m;
                 float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                auto exps = [&](auto masked) {
-                    uint32_t r[2][16];
-                    tmem_ld_32x32b_x16(s_col, r[0]);
+                uint32_t r[2][16];
+                tmem_ld_32x32b_x16(s_col, r[0]);
 #pragma unroll
-                    for (int ch = 0; ch < KT / 16; ++ch) {  // the next 16 scores are read while these are worked on
-                        uint32_t(&x)[16] = r[ch & 1];
-                        tmem_wait_ld();
-                        if (ch + 1 < KT / 16) tmem_ld_32x32b_x16(s_col + ch * 16 + 16, r[(ch + 1) & 1]);
-                        uint32_t p[8];
+                for (int ch = 0; ch < KT / 16; ++ch) {
+                    uint32_t(&x)[16] = r[ch & 1];
+                    tmem_wait_ld();
+                    if (ch + 1 < KT / 16) tmem_ld_32x32b_x16(s_col + ch * 16 + 16, r[(ch + 1) & 1]);
+                    uint32_t p[8];
 #pragma unroll
-                        for (int i = 0; i < 16; i += 2) {
-                            float s0 = __uint_as_float(x[i]), s1 = __uint_as_float(x[i + 1]);
-                            if constexpr (decltype(masked)::value) {
-                                s0 = in(ch * 16 + i) ? s0 : -INFINITY;
-                                s1 = in(ch * 16 + i + 1) ? s1 : -INFINITY;
-                            }
-                            const float e0 = kv4_ex2(fmaf(s0, c, -mz)), e1 = kv4_ex2(fmaf(s1, c, -mz));
-                            sum[i & 2] += e0;
-                            sum[(i & 2) + 1] += e1;
-                            p[i / 2] = cvt_f16x2(e1, e0);
-                        }
-                        pf_tmem_st8(s_col + ch * 8, p);
+                    for (int i = 0; i < 16; i += 2) {
+                        const float e0 = kv4_ex2(fmaf(seen(x[i], ch * 16 + i), c, -mz));
+                        const float e1 = kv4_ex2(fmaf(seen(x[i + 1], ch * 16 + i + 1), c, -mz));
+                        sum[i & 2] += e0;
+                        sum[(i & 2) + 1] += e1;
+                        p[i / 2] = cvt_f16x2(e1, e0);
                     }
-                };
-                if (all)
-                    exps(std::false_type());
-                else
-                    exps(std::true_type());
+                    pf_tmem_st8(s_col + ch * 8, p);
+                }
                 l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
                 tmem_wait_st();
                 tc_fence_before();
