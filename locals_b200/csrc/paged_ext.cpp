@@ -76,6 +76,13 @@ int64_t rows(Tensor& x, int dev) {
     return N > 1 ? x.stride(0) : H * D;
 }
 
+// x where its rows lie on `bytes`-byte boundaries, else a copy that does.
+void on_boundary(Tensor& x, int64_t& row, int bytes) {
+    if (reinterpret_cast<uintptr_t>(x.data_ptr()) % bytes == 0 && row * 2 % bytes == 0) return;
+    x = x.clone(at::MemoryFormat::Contiguous);
+    row = x.size(1) * x.size(2);
+}
+
 Tensor like(const Tensor& x) { return at::empty(x.sizes(), x.options(), at::MemoryFormat::Contiguous); }
 
 struct Angles {
@@ -156,10 +163,12 @@ std::vector<Tensor> plan(const Tensor& cached, const Tensor& fresh, const Tensor
 std::tuple<Tensor, MaybeTensor> rotate(Tensor q, MaybeTensor k, const Tensor& positions, const Tensor& cos, const Tensor& sin,
                                        const MaybeTensor& axes, bool interleaved) {
     const int dev = current(q);
-    const int64_t q_row = rows(q, dev), N = q.size(0), H = q.size(1), D = q.size(2);
-    int64_t k_row = 0, KVH = 0;
+    int64_t q_row = rows(q, dev), k_row = 0, KVH = 0;
+    const int64_t N = q.size(0), H = q.size(1), D = q.size(2);
+    if (interleaved) on_boundary(q, q_row, 4);
     if (k) {
         k_row = rows(*k, dev);
+        if (interleaved) on_boundary(*k, k_row, 4);
         KVH = k->size(1);
         need(k->size(0) == N && k->size(2) == D && k->scalar_type() == q.scalar_type(),
              "q and k must have the same tokens, head_dim and dtype");
@@ -179,7 +188,10 @@ MaybeTensor append(MaybeTensor q, Tensor k, Tensor v, const Tensor& slots, const
                    const MaybeTensor& positions, const MaybeTensor& cos, const MaybeTensor& sin, const MaybeTensor& axes,
                    bool interleaved) {
     const int dev = current(k);
-    const int64_t k_row = rows(k, dev), v_row = rows(v, dev), N = k.size(0), KVH = k.size(1), D = k.size(2);
+    int64_t k_row = rows(k, dev), v_row = rows(v, dev);
+    on_boundary(k, k_row, 16);
+    on_boundary(v, v_row, 16);
+    const int64_t N = k.size(0), KVH = k.size(1), D = k.size(2);
     const Pool p = pool(keys, values, k.scalar_type(), dev);
     need(v.sizes() == k.sizes() && v.scalar_type() == k.scalar_type() && KVH == p.KVH && D == p.D,
          "append: k and v do not fit the cache's heads and head_dim");
@@ -189,6 +201,7 @@ MaybeTensor append(MaybeTensor q, Tensor k, Tensor v, const Tensor& slots, const
     MaybeTensor qo;
     if (q) {
         q_row = rows(*q, dev);
+        on_boundary(*q, q_row, 16);
         H = q->size(1);
         need(q->size(0) == N && q->size(2) == D && q->scalar_type() == k.scalar_type(),
              "append: q and k must have the same tokens, head_dim and dtype");
@@ -226,8 +239,10 @@ std::tuple<Tensor, Tensor> read_slots(const Triple& keys, const Triple& values, 
 Tensor attend(Tensor q, const Triple& keys, const Triple& values, const Tensor& table, const Tensor& lens, double scale,
               const MaybeTensor& q_start, int64_t max_q, MaybeTensor sinks, int64_t window) {
     const int dev = current(q);
-    const int64_t q_row = rows(q, dev), N = q.size(0), H = q.size(1), D = q.size(2);
-    if (q_row != H * D) q = q.contiguous();
+    int64_t q_row = rows(q, dev);
+    const int64_t N = q.size(0), H = q.size(1), D = q.size(2);
+    if (q_row != H * D) q = q.contiguous(), q_row = H * D;
+    on_boundary(q, q_row, 16);
     const Pool p = pool(keys, values, q.scalar_type(), dev);
     ints(table, dev);
     ints(lens, dev);

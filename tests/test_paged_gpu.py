@@ -501,3 +501,46 @@ def test_step_of_a_batch(cuda):
         cached, head = p.lens, p.head
     assert cached.tolist() == [52, 4, 22] and head.item() == 4 + 1 + 2
     assert _status() == 0
+
+
+def test_queries_keys_and_values_on_any_boundary(cuda):
+    """Slices whose rows start 2 bytes past a boundary, or lie an odd number of values apart, give what copies give."""
+    import torch
+    from locals_b200 import paged, rotary
+
+    g = _gen(cuda, 31)
+    N, H, KVH, D, page = 5, 4, 2, 64, 8
+    cos, sin = rotary.tables(64, D, device=cuda)
+    pos = torch.arange(N, dtype=torch.int32, device=cuda)
+    slots = _i32([0, 9, 3, 12, 5], cuda)
+    for width, off in (((H + 2 * KVH) * D + 1, 1), ((H + 2 * KVH) * D + 8, 3)):
+        qkv = torch.randn((N, width), generator=g, device=cuda).to(torch.bfloat16)
+        q, k, v = (qkv[:, off + a * D:off + (a + h) * D].view(N, h, D) for a, h in ((0, H), (H, KVH), (H + KVH, KVH)))
+        for inter in (False, True):
+            caches = [paged.pool(3, KVH, page, D, torch.bfloat16, cuda) for _ in range(2)]
+            a = paged.append(q, k, v, slots, *caches[0], pos, cos, sin, interleaved=inter)
+            b = paged.append(q.contiguous(), k.contiguous(), v.contiguous(), slots, *caches[1], pos, cos, sin,
+                             interleaved=inter)
+            assert torch.equal(a, b)
+            for x, y in zip((*caches[0][0], *caches[0][1]), (*caches[1][0], *caches[1][1])):
+                assert torch.equal(x, y)
+            for x, y in zip(rotary.rotate(q, k, pos, cos, sin, interleaved=inter),
+                            rotary.rotate(q.contiguous(), k.contiguous(), pos, cos, sin, interleaved=inter)):
+                assert torch.equal(x, y)
+        table = _i32([[0, 1], [1, 0], [2, 1], [0, 2], [1, 2]], cuda)
+        lens = _i32([9, 3, 16, 1, 8], cuda)
+        keys, values = caches[0]
+        assert torch.equal(paged.attend(q, keys, values, table, lens, 0.1),
+                           paged.attend(q.contiguous(), keys, values, table, lens, 0.1))
+
+
+def test_attend_on_the_other_side_of_each_rule(cuda):
+    """Lengths, batches and rows at which another form takes over: clusters of 8 to 1 CTAs, the even split, tiles unpacked
+    in place and unpacked first."""
+    _attend(cuda, [1], [900], 4, 1, 128, 16, "bfloat16", seed=40)              # one cluster of 8
+    _attend(cuda, [1] * 70, [130 + 7 * i for i in range(70)], 8, 2, 64, 16, "float16", seed=41)   # clusters of fewer
+    _attend(cuda, [1] * 130, [3 * i + 1 for i in range(130)], 4, 4, 64, 8, "bfloat16", seed=42)   # more items than CTAs
+    _attend(cuda, [2, 2], [9000, 12], 16, 2, 128, 32, "bfloat16", seed=43)     # 16 rows, the even split
+    _attend(cuda, [64, 3], [200, 3000], 8, 1, 128, 16, "float16", seed=44)     # two tiles of rows: unpacked in place
+    _attend(cuda, [65, 3], [200, 3000], 8, 1, 128, 16, "float16", seed=45)     # a third: unpacked first
+    _attend(cuda, [300, 1, 40], [700, 600, 41], 3, 1, 256, 24, "bfloat16", 0, True, seed=46)
