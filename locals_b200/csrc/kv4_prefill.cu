@@ -83,13 +83,13 @@ __device__ __forceinline__ int pf_tiles(const Kv4AttArgs& a, int b, int* first, 
     return r.fresh * a.G > a.split_rows ? (r.fresh * a.G + PfShape<D>::R - 1) / PfShape<D>::R : 0;
 }
 
-// Steps of all of request b's tiles.
+// Units of every `step`-th of request b's tiles, from tile `from` on.
 template <int D>
-__device__ __forceinline__ long long pf_weight(const Kv4AttArgs& a, int b) {
+__device__ __forceinline__ long long pf_weight(const Kv4AttArgs& a, int b, int from, int step) {
     int first, fresh, base;
     const int tiles = pf_tiles<D>(a, b, &first, &fresh, &base);
     long long w = 0;
-    for (int t = 0; t < tiles; ++t) {
+    for (int t = from; t < tiles; t += step) {
         int lo, hi;
         pf_steps<D>(a, base, fresh, t, &lo, &hi);
         w += hi - lo + PF_ITEM;
@@ -97,16 +97,24 @@ __device__ __forceinline__ long long pf_weight(const Kv4AttArgs& a, int b) {
     return w * a.pool.KVH;
 }
 
-// Sum over the CTA's threads.
-__device__ __forceinline__ long long pf_sum(long long v, long long* red) {
+// Inclusive sum over the CTA's threads, and their total.
+__device__ __forceinline__ long long pf_scan(long long v, long long* red, long long* total) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
 #pragma unroll
-    for (int d = 16; d; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
+    for (int d = 1; d < 32; d <<= 1) {
+        const long long u = __shfl_up_sync(0xffffffffu, v, d);
+        if (lane >= d) v += u;
+    }
+    __syncthreads();  // (red may still be read from before)
+    if (lane == 31) red[warp] = v;
     __syncthreads();
-    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
-    __syncthreads();
-    long long s = 0;
-    for (int w = 0; w < int(blockDim.x >> 5); ++w) s += red[w];
-    return s;
+    long long sum = 0;
+    for (int k = 0; k < int(blockDim.x >> 5); ++k) {
+        if (k == warp) v += sum;
+        sum += red[k];
+    }
+    *total = sum;
+    return v;
 }
 
 // The CTA's walk over its share: items (request, tile, kv head) in that order, each with its steps [st0, st1). A share is
@@ -388,90 +396,6 @@ __global__ void __launch_bounds__(pf_threads(DENSE), 1) kv4_prefill_kernel(const
     __shared__ uint8_t* volatile pf_base;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
-    grid_dep_wait();
-    if (a.split_rows == 0) kv4_zero_tail(a, D);  // (else kv4_attend does)
-    // ---- this CTA's share ----
-    long long total = 0;
-    for (int b0 = 0; b0 < a.B; b0 += PF_THREADS) total += pf_sum(b0 + tid < a.B ? pf_weight<D>(a, b0 + tid) : 0, red);
-    const int n = int(min((long long)gridDim.x, total));
-    int32_t* rec = a.records + blockIdx.x * 8;  // what the join kernel does for this CTA's first step
-    if (int(blockIdx.x) >= n) {
-        if (tid == 0) rec[0] = 0;
-        return;
-    }
-    const long long x0 = (long long)blockIdx.x * total / n, x1 = ((long long)blockIdx.x + 1) * total / n;
-    PfWalk<D> walk;
-    {
-        long long at = 0;
-        int b = 0;
-        for (int b0 = 0;; b0 += PF_THREADS) {
-            const long long w = b0 + tid < a.B ? pf_weight<D>(a, b0 + tid) : 0;
-            const long long sum = pf_sum(w, red);
-            if (at + sum <= x0) {
-                at += sum;
-                continue;
-            }
-            long long s = w;  // inclusive sums within the CTA
-#pragma unroll
-            for (int d = 1; d < 32; d <<= 1) {
-                const long long u = __shfl_up_sync(0xffffffffu, s, d);
-                if (lane >= d) s += u;
-            }
-            __syncthreads();
-            if (lane == 31) red[warp] = s;
-            __syncthreads();
-            for (int k = 0; k < warp; ++k) s += red[k];
-            const bool past = at + s > x0;
-            b = b0 + int(pf_sum(past ? 0 : 1, red));
-            at += pf_sum(past ? 0 : w, red);
-            break;
-        }
-        walk.b = b;
-        walk.tiles = pf_tiles<D>(a, b, &walk.first, &walk.fresh, &walk.base);
-        // the tile: the threads sum theirs, in rounds of PF_THREADS tiles
-        int t0 = 0;
-        for (;; t0 += PF_THREADS) {
-            int lo = 0, hi = 0;
-            if (t0 + tid < walk.tiles) pf_steps<D>(a, walk.base, walk.fresh, t0 + tid, &lo, &hi);
-            const long long w = t0 + tid < walk.tiles ? (long long)(hi - lo + PF_ITEM) * a.pool.KVH : 0;
-            const long long sum = pf_sum(w, red);
-            if (at + sum <= x0) {
-                at += sum;
-                continue;
-            }
-            long long s = w;
-#pragma unroll
-            for (int d = 1; d < 32; d <<= 1) {
-                const long long u = __shfl_up_sync(0xffffffffu, s, d);
-                if (lane >= d) s += u;
-            }
-            __syncthreads();
-            if (lane == 31) red[warp] = s;
-            __syncthreads();
-            for (int k = 0; k < warp; ++k) s += red[k];
-            const bool past = at + s > x0;
-            walk.tile = t0 + int(pf_sum(past ? 0 : 1, red));
-            at += pf_sum(past ? 0 : w, red);
-            break;
-        }
-        pf_steps<D>(a, walk.base, walk.fresh, walk.tile, &walk.lo, &walk.hi);
-        const int units = walk.hi - walk.lo + PF_ITEM;
-        walk.kvh = int((x0 - at) / units);
-        const long long item = at + (long long)walk.kvh * units;
-        walk.skip = int(x0 - item);
-        walk.left = int(x1 - x0);
-        walk.begun = false;
-        if (tid == 0) {
-            const int c0 = kv4_owner(item + PF_ITEM, total, n), c1 = kv4_owner(item + units - 1, total, n);
-            rec[0] = walk.skip > PF_ITEM && c0 == int(blockIdx.x) - 1;  // the first boundary within its item's steps
-            rec[1] = walk.first;
-            rec[2] = walk.tile * R;
-            rec[3] = min(R, walk.fresh * a.G - walk.tile * R);
-            rec[4] = walk.kvh;
-            rec[5] = c1;
-        }
-    }
-
     if (tid == 0) {
         uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(pf_raw) + 1023) & ~uintptr_t(1023));
         PfBars& bar = *reinterpret_cast<PfBars*>(smem + S::SMEM);
@@ -494,6 +418,83 @@ __global__ void __launch_bounds__(pf_threads(DENSE), 1) kv4_prefill_kernel(const
         bar.abort = 0;
         fence_barrier_init();
     }
+    grid_dep_wait();
+    if (a.split_rows == 0) kv4_zero_tail(a, D);  // (else kv4_attend does)
+    // ---- this CTA's share ----
+    // up to 32 threads a request sum its tiles' units; then requests, and the tiles of the one found, are scanned together
+    int each = 32;
+    while (each > 1 && a.B * each > PF_THREADS) each >>= 1;
+    const int round = PF_THREADS / each;
+    auto weight = [&](int b0) -> long long {  // (in the first of a request's threads)
+        const int b = b0 + tid / each, from = tid & (each - 1);
+        long long w = b < a.B ? pf_weight<D>(a, b, from, each) : 0;
+        for (int d = 1; d < each; d <<= 1) w += __shfl_xor_sync(0xffffffffu, w, d);
+        return from ? 0 : w;
+    };
+    __shared__ long long found_at;
+    __shared__ int found;
+    long long sum0, total;
+    const long long w0 = weight(0), s0 = pf_scan(w0, red, &sum0);
+    total = sum0;
+    for (int b0 = round; b0 < a.B; b0 += round) {
+        long long sum;
+        pf_scan(weight(b0), red, &sum);
+        total += sum;
+    }
+    const int n = int(min((long long)gridDim.x, total));
+    int32_t* rec = a.records + blockIdx.x * 8;  // what the join kernel does for this CTA's first step
+    if (int(blockIdx.x) >= n) {
+        if (tid == 0) rec[0] = 0;
+        return;
+    }
+    const long long x0 = (long long)blockIdx.x * total / n, x1 = ((long long)blockIdx.x + 1) * total / n;
+    PfWalk<D> walk;
+    long long item;
+    {
+        long long at = 0;
+        for (int b0 = 0;; b0 += round) {
+            long long w = w0, s = s0, sum = sum0;
+            if (b0) {
+                w = weight(b0);
+                s = pf_scan(w, red, &sum);
+            }
+            if (at + sum <= x0) {
+                at += sum;
+                continue;
+            }
+            if (at + s > x0 && at + s - w <= x0) found = b0 + tid / each, found_at = at + s - w;  // one thread's
+            __syncthreads();
+            walk.b = found;
+            at = found_at;
+            break;
+        }
+        walk.tiles = pf_tiles<D>(a, walk.b, &walk.first, &walk.fresh, &walk.base);
+        walk.tile = 0;
+        for (int t0 = 0; walk.tiles > 1; t0 += PF_THREADS) {
+            int lo = 0, hi = 0;
+            if (t0 + tid < walk.tiles) pf_steps<D>(a, walk.base, walk.fresh, t0 + tid, &lo, &hi);
+            const long long w = t0 + tid < walk.tiles ? (long long)(hi - lo + PF_ITEM) * a.pool.KVH : 0;
+            long long sum;
+            const long long s = pf_scan(w, red, &sum);
+            if (at + sum <= x0) {
+                at += sum;
+                continue;
+            }
+            if (at + s > x0 && at + s - w <= x0) found = t0 + tid, found_at = at + s - w;
+            __syncthreads();
+            walk.tile = found;
+            at = found_at;
+            break;
+        }
+        pf_steps<D>(a, walk.base, walk.fresh, walk.tile, &walk.lo, &walk.hi);
+        const int units = walk.hi - walk.lo + PF_ITEM;
+        walk.kvh = int((x0 - at) / units);
+        item = at + (long long)walk.kvh * units;
+        walk.skip = int(x0 - item);
+        walk.left = int(x1 - x0);
+        walk.begun = false;
+    }
+
     __shared__ uint32_t tmem_base;
     if (warp == 0) {
         tmem_alloc(&tmem_base, 512);
@@ -502,6 +503,15 @@ __global__ void __launch_bounds__(pf_threads(DENSE), 1) kv4_prefill_kernel(const
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
+    if (tid == 64) {  // (an idle warp's)
+        const int c0 = kv4_owner(item + PF_ITEM, total, n), c1 = kv4_owner(item + walk.hi - walk.lo + PF_ITEM - 1, total, n);
+        rec[0] = walk.skip > PF_ITEM && c0 == int(blockIdx.x) - 1;  // the first boundary within its item's steps
+        rec[1] = walk.first;
+        rec[2] = walk.tile * R;
+        rec[3] = min(R, walk.fresh * a.G - walk.tile * R);
+        rec[4] = walk.kvh;
+        rec[5] = c1;
+    }
     // Each role reads the bases for itself from here on: values shared by all roles would be kept on the stack by all,
     // those with registers to spare too, and the issuing thread's reloads would delay its products.
     struct Places {
@@ -610,21 +620,19 @@ __global__ void __launch_bounds__(pf_threads(DENSE), 1) kv4_prefill_kernel(const
                 const int ve_t = *reinterpret_cast<volatile int*>(&bar.v_exp[it & 3]);
                 const bool all = key0 >= lo_all && key0 + KT <= hi_all && miss == 0;
                 const uint32_t s_col = tmem + lanes + buf * KT;
-                // what this row sees of the step, a bit a key
-                uint32_t vis[KT / 32];
-#pragma unroll
-                for (int i = 0; i < KT / 32; ++i) {
+                // what this row sees of 32 of the step's keys, a bit a key
+                auto sees = [&](int i) -> uint32_t {
                     const int from = min(max(row_lo - key0 - 32 * i, 0), 32), to = min(max(row_hi - key0 - 32 * i, 0), 32);
-                    vis[i] = all ? 0xffffffffu : uint32_t((1ull << to) - 1) & ~uint32_t((1ull << from) - 1);
-                    if (miss) {
+                    uint32_t v = uint32_t((1ull << to) - 1) & ~uint32_t((1ull << from) - 1);
+                    const uint32_t gone = (miss >> (4 * i)) & 15;
+                    if (gone) {
 #pragma unroll
                         for (int k = 0; k < 4; ++k)
-                            if ((miss >> (4 * i + k)) & 1) vis[i] &= ~(0xffu << (8 * k));
+                            if ((gone >> k) & 1) v &= ~(0xffu << (8 * k));
                     }
-                }
-                auto seen = [&](uint32_t score, int i) {
-                    return (vis[i >> 5] >> (i & 31)) & 1 ? __uint_as_float(score) : -INFINITY;
+                    return v;
                 };
+                auto seen = [](uint32_t score, uint32_t v, int i) { return (v >> i) & 1 ? __uint_as_float(score) : -INFINITY; };
                 // The common case, one pass: the reference from the steps before serves the step (found out at its end: the
                 // probabilities stay in registers until then, the scores in place).
                 auto once = [&](auto masked) -> bool {
@@ -633,16 +641,18 @@ __global__ void __launch_bounds__(pf_threads(DENSE), 1) kv4_prefill_kernel(const
                     uint32_t r[2][CH], p[KT / 2];
                     uint64_t sums[2] = {0, 0};
                     float mx[2] = {-INFINITY, -INFINITY};
+                    uint32_t v = 0;
                     tmem_ld_32x32b_x16(s_col, r[0]);
 #pragma unroll
                     for (int ch = 0; ch < KT / CH; ++ch) {  // the next scores are read while these are worked on
                         uint32_t(&x)[CH] = r[ch & 1];
                         tmem_wait_ld();
                         if (ch + 1 < KT / CH) tmem_ld_32x32b_x16(s_col + (ch + 1) * CH, r[(ch + 1) & 1]);
+                        if constexpr (decltype(masked)::value) v = ch & 1 ? v >> 16 : sees(ch / 2);
 #pragma unroll
                         for (int i = 0; i < CH; i += 2) {
                             float s0 = __uint_as_float(x[i]), s1 = __uint_as_float(x[i + 1]);
-                            if constexpr (decltype(masked)::value) s0 = seen(x[i], ch * CH + i), s1 = seen(x[i + 1], ch * CH + i + 1);
+                            if constexpr (decltype(masked)::value) s0 = seen(x[i], v, i), s1 = seen(x[i + 1], v, i + 1);
                             mx[(i >> 1) & 1] = fmaxf(fmaxf(mx[(i >> 1) & 1], s0), s1);
                             float e0, e1;
                             pf_unpair(pf_fma2(pf_pair(s0, s1), c2, m2), &e0, &e1);
@@ -668,18 +678,17 @@ __global__ void __launch_bounds__(pf_threads(DENSE), 1) kv4_prefill_kernel(const
                 if (ve_t == ve && __all_sync(0xffffffffu, m != -INFINITY)) {
                     if (all ? once(std::false_type()) : once(std::true_type())) continue;
                 }
+                // A new reference (an item's first step, mostly): two passes, in loops, since their code is not often in reach.
                 float mx = -INFINITY;
-#pragma unroll
-                for (int ch = 0; ch < KT / 64; ++ch) {
-                    uint32_t r[2][32];
-                    tmem_ld_32x32b_x32(s_col + ch * 64, r[0]);
-                    tmem_ld_32x32b_x32(s_col + ch * 64 + 32, r[1]);
+#pragma unroll 1
+                for (int ch = 0; ch < KT / 32; ++ch) {
+                    uint32_t r[32];
+                    tmem_ld_32x32b_x32(s_col + ch * 32, r);
+                    const uint32_t v = sees(ch);
                     tmem_wait_ld();
                     float part[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-                    for (int i = 0; i < 64; i += 2)
-                        part[(i >> 1) & 1] = fmaxf(fmaxf(part[(i >> 1) & 1], seen(r[i >> 5][i & 31], ch * 64 + i)),
-                                                   seen(r[i >> 5][(i & 31) + 1], ch * 64 + i + 1));
+                    for (int i = 0; i < 32; i += 2) part[(i >> 1) & 1] = fmaxf(fmaxf(part[(i >> 1) & 1], seen(r[i], v, i)), seen(r[i + 1], v, i + 1));
                     mx = fmaxf(mx, fmaxf(part[0], part[1]));
                 }
                 const float mn = fmaxf(m, mx * c);
@@ -705,18 +714,16 @@ __global__ void __launch_bounds__(pf_threads(DENSE), 1) kv4_prefill_kernel(const
                 }
                 const float mz = m == -INFINITY ? 0.0f : m;
                 float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                uint32_t r[2][16];
-                tmem_ld_32x32b_x16(s_col, r[0]);
-#pragma unroll
+#pragma unroll 1
                 for (int ch = 0; ch < KT / 16; ++ch) {
-                    uint32_t(&x)[16] = r[ch & 1];
+                    uint32_t x[16], p[8];
+                    tmem_ld_32x32b_x16(s_col + ch * 16, x);
+                    const uint32_t v = sees(ch >> 1) >> (16 * (ch & 1));
                     tmem_wait_ld();
-                    if (ch + 1 < KT / 16) tmem_ld_32x32b_x16(s_col + ch * 16 + 16, r[(ch + 1) & 1]);
-                    uint32_t p[8];
 #pragma unroll
                     for (int i = 0; i < 16; i += 2) {
-                        const float e0 = kv4_ex2(fmaf(seen(x[i], ch * 16 + i), c, -mz));
-                        const float e1 = kv4_ex2(fmaf(seen(x[i + 1], ch * 16 + i + 1), c, -mz));
+                        const float e0 = kv4_ex2(fmaf(seen(x[i], v, i), c, -mz));
+                        const float e1 = kv4_ex2(fmaf(seen(x[i + 1], v, i + 1), c, -mz));
                         sum[i & 2] += e0;
                         sum[(i & 2) + 1] += e1;
                         p[i / 2] = cvt_f16x2(e1, e0);
