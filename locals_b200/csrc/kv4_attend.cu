@@ -33,6 +33,8 @@
 #include <math.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "kv4_attend.cuh"
 #include "lq_host.h"
 #include "lq_ptx.cuh"
@@ -665,53 +667,97 @@ __global__ void __launch_bounds__(KV4_NW * 32, kv4_resident(D, NT)) kv4_attend_k
         const bool whole = !CL && st0 == 0 && st1 == rq.steps();
         float* mine = co + KV4_NW * R * D;  // (CL) this CTA's [R] m, [R] l, [R][D] O
         const size_t part = ((size_t)blockIdx.x * 2 + (st0 == 0 ? 1 : 0)) * R;
-        for (int j = 0; j < rows; ++j) {
-            float M = -INFINITY;
+        // a warp a row, a lane V neighbouring dimensions at a time
+        constexpr int V = D >= 128 ? 4 : 2, VU = D / (32 * V);
+        using Vec = std::conditional_t<V == 4, float4, float2>;
+        auto put = [&](int j, float M, float L, const float (&O)[VU][V], float sink) {
+            const int qi = j / G, head = kvh * G + j - qi * G;
+            uint16_t* dst = a.out + ((size_t)(rq.first + qi) * a.H + head) * D + lane * V;
+#pragma unroll
+            for (int u = 0; u < VU; ++u) {
+                uint32_t h[V / 2];
+#pragma unroll
+                for (int i = 0; i < V; i += 2)
+                    h[i / 2] = kv4_finish<T>(M, L, O[u][i], sink) | uint32_t(kv4_finish<T>(M, L, O[u][i + 1], sink)) << 16;
+                if constexpr (V == 4) *reinterpret_cast<uint2*>(dst + u * 32 * V) = make_uint2(h[0], h[1]);
+                else *reinterpret_cast<uint32_t*>(dst + u * 32 * V) = h[0];
+            }
+        };
+        for (int j = warp; j < rows; j += KV4_NW) {
+            alignas(16) float O[VU][V];
+            float M = -INFINITY, L = 0.0f;
+            const float sink = kv4_sink(a.sinks, kvh * G + j % G);
+#pragma unroll
+            for (int u = 0; u < VU; ++u)
+#pragma unroll
+                for (int i = 0; i < V; ++i) O[u][i] = 0.0f;
 #pragma unroll
             for (int w = 0; w < KV4_NW; ++w) M = fmaxf(M, cm[w * R + j]);
-            float f[KV4_NW], L = 0.0f;
 #pragma unroll
             for (int w = 0; w < KV4_NW; ++w) {
-                f[w] = cm[w * R + j] == -INFINITY ? 0.0f : kv4_ex2(cm[w * R + j] - M);
-                L += cl[w * R + j] * f[w];
-            }
-            const int qi = j / G, head = kvh * G + j - qi * G;
-            for (int d = tid; d < D; d += KV4_NW * 32) {
-                float O = 0.0f;
+                const float f = cm[w * R + j] == -INFINITY ? 0.0f : kv4_ex2(cm[w * R + j] - M);
+                L += cl[w * R + j] * f;  // (a NaN's l has no m: NaN * 0)
 #pragma unroll
-                for (int w = 0; w < KV4_NW; ++w)
-                    if (f[w] != 0.0f) O += co[(w * R + j) * D + d] * f[w];
-                if (whole)
-                    a.out[((size_t)(rq.first + qi) * a.H + head) * D + d] = kv4_finish<T>(M, L, O, kv4_sink(a.sinks, head));
-                else if (CL)
-                    mine[2 * R + j * D + d] = O;
-                else
-                    a.part_o[(part + j) * D + d] = O;
+                for (int u = 0; u < VU; ++u) {
+                    alignas(16) float x[V];
+                    *reinterpret_cast<Vec*>(x) = *reinterpret_cast<const Vec*>(co + (w * R + j) * D + (u * 32 + lane) * V);
+#pragma unroll
+                    for (int i = 0; i < V; ++i) O[u][i] += f != 0.0f ? x[i] * f : 0.0f;
+                }
             }
-            if (CL && tid == 0) mine[j] = M, mine[R + j] = L;
-            if (!CL && !whole && tid == 0) a.part_ml[2 * (part + j)] = M, a.part_ml[2 * (part + j) + 1] = L;
+            if (whole) {
+                put(j, M, L, O, sink);
+                continue;
+            }
+            float* dst = (CL ? mine + 2 * R + j * D : a.part_o + (part + j) * D) + lane * V;
+#pragma unroll
+            for (int u = 0; u < VU; ++u) *reinterpret_cast<Vec*>(dst + u * 32 * V) = *reinterpret_cast<const Vec*>(O[u]);
+            if (CL && lane == 0) mine[j] = M, mine[R + j] = L;
+            if (!CL && lane == 0) a.part_ml[2 * (part + j)] = M, a.part_ml[2 * (part + j) + 1] = L;
         }
         if constexpr (CL) {
             cluster_sync();
             const int C = int(kv4_cluster_size());
             const uint32_t base32 = smem_u32(mine);
-            for (int j = int(cluster_ctarank()); j < rows; j += C) {
-                float M = -INFINITY;
-                for (int k = 0; k < C; ++k) M = fmaxf(M, ld_dsmem_f(map_peer(base32 + j * 4, k)));
-                const int qi = j / G, head = kvh * G + j - qi * G;
-                const float sink = kv4_sink(a.sinks, head);
-                for (int d = tid; d < D; d += KV4_NW * 32) {
-                    float L = 0.0f, O = 0.0f;
-                    for (int k = 0; k < C; ++k) {
-                        const uint32_t peer = map_peer(base32, k);
-                        const float m = ld_dsmem_f(peer + j * 4), l = ld_dsmem_f(peer + (R + j) * 4);
-                        const float o = ld_dsmem_f(peer + (2 * R + j * D + d) * 4);
-                        const float f = m == -INFINITY ? 0.0f : kv4_ex2(m - M);
-                        L += l * f;  // (a NaN's l has no m: NaN * 0)
-                        if (f != 0.0f) O += o * f;
+            for (int j = int(cluster_ctarank()) + C * warp; j < rows; j += C * KV4_NW) {
+                const float sink = kv4_sink(a.sinks, kvh * G + j % G);
+                const uint32_t own = map_peer(base32 + j * 4, min(lane, C - 1));  // lane k: CTA k's m and l
+                const float m = lane < C ? ld_dsmem_f(own) : -INFINITY, l = lane < C ? ld_dsmem_f(own + R * 4) : 0.0f;
+                alignas(16) float x[8][VU * V], O[VU][V];
+                float M = m;
+#pragma unroll
+                for (int k = 0; k < 8; ++k)
+#pragma unroll
+                    for (int i = 0; i < VU * V; i += V) {
+                        const uint32_t at = map_peer(base32, min(k, C - 1)) + (2 * R + j * D + i * 32 + lane * V) * 4;
+                        if constexpr (V == 4) {
+                            *reinterpret_cast<float4*>(&x[k][i]) = k < C ? ld_dsmem_f4(at) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                        } else {
+#pragma unroll
+                            for (int e = 0; e < V; ++e) x[k][i + e] = k < C ? ld_dsmem_f(at + 4 * e) : 0.0f;
+                        }
                     }
-                    a.out[((size_t)(rq.first + qi) * a.H + head) * D + d] = kv4_finish<T>(M, L, O, sink);
+#pragma unroll
+                for (int d = 1; d < 8; d <<= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, d));
+                M = __shfl_sync(0xffffffffu, M, 0);
+                const float f = m == -INFINITY ? 0.0f : kv4_ex2(m - M);
+                float L = l * f;  // (a NaN's l has no m: NaN * 0)
+#pragma unroll
+                for (int d = 1; d < 8; d <<= 1) L += __shfl_xor_sync(0xffffffffu, L, d);
+                L = __shfl_sync(0xffffffffu, L, 0);
+#pragma unroll
+                for (int u = 0; u < VU; ++u)
+#pragma unroll
+                    for (int i = 0; i < V; ++i) O[u][i] = 0.0f;
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    const float fk = __shfl_sync(0xffffffffu, f, k);
+#pragma unroll
+                    for (int u = 0; u < VU; ++u)
+#pragma unroll
+                        for (int i = 0; i < V; ++i) O[u][i] += fk != 0.0f ? x[k][u * V + i] * fk : 0.0f;
                 }
+                put(j, M, L, O, sink);
             }
             cluster_sync();  // no CTA leaves while another reads it
         }

@@ -60,7 +60,7 @@ struct PfShape {
 };
 
 // What an item costs beside its steps (queries fetched, the pipeline filled, outputs written), in steps.
-constexpr int PF_ITEM = 7;
+constexpr int PF_ITEM = 5;
 
 // A tile's steps of keys: from the first that its first row sees to the last that its last row sees.
 template <int D>
