@@ -6,6 +6,7 @@ Public surface (names follow the reference):
   fuse.concat_quantized / FusedQKV / FusedMLP                                  (locals/fuse.py)
   moe.router_logits / route_topk / group / switch_glu / MoELayer               (locals/moe.py, moe_kernel.py)
   tune.choose / lookup                                                         (locals/kernels.py tuner)
+  paged.plan / pool / append / read / attend, rotary.tables / rotate           (a paged 4-bit key/value cache)
   shard.ColumnShardedLinear / ExpertParallelMoE                                (multi-GPU, NCCL)
 """
 

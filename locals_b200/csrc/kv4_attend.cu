@@ -4,29 +4,43 @@
 // (window 0: from 0) to its own: out = sum_j e^(s_j - m) v_j / (sum_j e^(s_j - m) + e^(sink - m)), s_j = scale q . k_j,
 // and 0 where nothing is seen.
 //
-// kv4_attend_kernel. The rows of a (request, kv head) are its queries times the G query heads of the kv head; a tile of
-// 8 NT rows is the n side of m16n8k16 fp16 MMAs whose m side is 16 keys (scores, S^T = K Q^T) or 16 dimensions (values,
+// kv4_attend_kernel. The rows of a (request, kv head) are its queries times the G query heads of the kv head; up to 8 NT
+// of them are the n side of m16n8k16 fp16 MMAs whose m side is 16 keys (scores, S^T = K Q^T) or 16 dimensions (values,
 // O^T = V^T P^T), so that few rows fill the MMA and each key is unpacked once for all of them. The 4-bit codes enter the
 // MMA as fp16 subnormals, with no arithmetic at all: a word's bits & 0x000f000f are the pair (code 0, code 4) * 2^-24,
-// & 0x00f000f0 the pair (code 1, code 5) * 2^-20, and the same of word >> 8; every product and sum of them is exact in
-// the fp32 accumulator but for its roundings. What differs between the nibble's places is put right on the other side:
-// queries that meet 2^-20 codes are divided by 16 beforehand, output dimensions that they made are afterwards. The
-// groups' scales and biases never touch the codes:
+// & 0x00f000f0 the pair (code 1, code 5) * 2^-20, and the same of word >> 8; every product of them is exact in the fp32
+// accumulator. What differs between the nibble's places is put right on the other side: queries that meet 2^-20 codes are
+// divided by 16 beforehand, output dimensions that they made are afterwards. The groups' scales and biases never touch the
+// key codes:
 //   s_j = scale * sum_g ks_jg (q . codes)_g + kb_jg sum(q)_g,
-//   o_g = sum_j w_jg (codes_jg - z_jg) + p_j (vb_jg + z_jg vs_jg),   w_jg = p_j vs_jg,  z_jg = round(-vb_jg / vs_jg) in 0..15,
-// scores in fp32, and w rounded to fp16 once (2^-12 against the 2^-9 of a bf16 output), after a power of two that puts
-// the warp's largest value scale at 2^9 .. 2^14. codes - z (exact on subnormals, one packed subtraction a pair) takes out
-// of a group what its codes and its bias have in common, so that the rounding of w is one of the value itself, however
-// near to 0 it lies. Queries are put into fp16 with a power of two a row, exact for bf16 but for values 2^-27 below the
-// row's largest. A score tile's accumulator layout is transposed into the value MMA's operand by movmatrix.
-// A masked key's score is -inf and its w and p vb are set to 0, not multiplied, so that what it holds never matters.
+//   o_g = sum_j w_jg (codes_jg - z_jg) + p_j (vb_jg + z_jg vs_jg),   w_jg = p_j vs_jg,  z_jg = round(-vb_jg / vs_jg) in 0..15.
+// Scores, softmax statistics and outputs are fp32. Two roundings to fewer bits:
+//   queries to fp16 after one power of two an item that puts the largest at 2^13 .. 2^14: exact for fp16 and bf16 but for
+//     values 2^-27 below the item's largest;
+//   w to fp16 (2^-11 against the 2^-8 of a bf16 output; an fp16 output's error grows from 2.0e-4 to 2.2e-4 by it), after a
+//     power of two that puts the warp's largest value scale at 2^5 .. 2^10. codes - z (exact on subnormals, one packed subtraction a pair) takes out of a group
+//     what its codes and its bias have in common, so that this is a rounding of the value itself, however near to 0 it lies.
+// A score tile's accumulator layout is transposed into the value MMA's operand by movmatrix. The running maximum of a row is
+// only followed when it has grown by 2^4, so that most steps rescale nothing.
+// A key's scales and biases become floats once a step, one key a lane, and go to its reads through shared memory. A masked
+// key's score is -inf; a key without a page has none; a key whose values are not finite has zero values and a NaN key, so
+// that what a place holds reaches only the rows that see it.
 //
 // Each warp walks 32-key steps through a ring of its own, filled with cp.async STAGES - 1 steps ahead; the pages of the
 // next 8 steps are looked up by the 32 lanes at once (8 keys always lie in one page). Rows are permuted within a chunk
 // (P8) and 32-byte pieces swizzled (kv4_swz) so that every shared load is free of bank conflicts.
-// The keys of all (request, kv head, tile)s, in steps of 128, are dealt out evenly over one wave of CTAs, wherever the
-// boundaries fall; a CTA that holds only part of an item writes a part (m, l, O) to the workspace, at most two a CTA,
-// and kv4_join_kernel joins them. HBM-bound for few rows: D + D / 8 bytes a key and kv head (144 at D = 128).
+// The keys of all (request, kv head)s, in steps of 128, are dealt out evenly over one wave of CTAs, wherever the boundaries
+// fall; a CTA that holds only part of an item writes a part (m, l, O) to the workspace, at most two a CTA, and
+// kv4_join_kernel joins each divided item. Where every item can have a cluster of CTAs and few steps (kv4_cluster), the
+// cluster's CTAs share the item and join through distributed shared memory: one launch.
+//
+// What bounds it. The bytes are (D + D / 8) a key and kv head (144 at D = 128); the instructions are about 730 a warp and 32
+// keys (unpacking 200, z 64, MMAs 48, the rest loads, scales and softmax), and they are what the time goes to: 2.3 a clock
+// and SM, the ALU pipe 48% busy, tensor pipe 22%. Measured, GPU time of a call: 4 requests of 131,072 keys, 32 heads on 4,
+// D = 128, fp16: 81.7 us = 3.70 TB/s (56% of the copy rate); 64 requests of up to 8,191 keys, 32 heads on 4, bf16: 53.5 us =
+// 2.88 TB/s; one request of 1,001 keys: 8.4 us (launch, one pass of dependent loads, two cluster barriers).
+// Tried and slower: 4 CTAs a SM at 128 registers (89.6 against 83.3 us, it spills), 5 (126); a ring of 2 stages is as fast
+// as 3 at D = 128.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -56,7 +70,8 @@ __device__ __forceinline__ uint32_t kv4_transpose(uint32_t x) {
     return y;
 }
 
-// What an item costs beside its steps (pages and queries fetched, the ring filled, the warps joined), in steps.
+// What an item costs beside its steps (pages and queries fetched, the ring filled, the warps joined), in steps. 64 requests
+// of up to 8,191 keys: 1: 69 us, 2: 63, 4 to 7: 56.
 constexpr int KV4_ITEM = 5;
 
 __device__ __forceinline__ Kv4Req kv4_request(const Kv4AttArgs& a, int b) {
@@ -789,7 +804,8 @@ bool kv4_attend_shape_ok(int N, int B, int max_q, int H, int KVH, int width, int
 
 // Rows of kv4_attend's tiles, and the rows up to which a request is its own (above: kv4_prefill). 16 rows where every
 // request fits them (a key is then unpacked once for all); else as many as one query has, 8 or 16, for the requests of
-// a mixed batch that only decode. 0: none.
+// a mixed batch that only decode. 0: none. 16 requests of 8,192 keys, 4 kv heads, D = 128: 8 rows 31 us, 16 rows
+// 39; 24 and 32 rows 111 and 117 in kv4_prefill.
 static void kv4_rows(int max_q, int G, int* R, int* split) {
     const long long most = (long long)max_q * G;
     *R = most <= 8 || (most > 16 && G <= 8) ? 8 : 16;
@@ -816,7 +832,8 @@ size_t kv4_attend_workspace_bytes(int B, int max_q, int H, int KVH, int D, long 
 
 // CTAs a cluster where the clustered form is used, 0 where it is not: as many (up to 8) as leave every item's cluster
 // resident at once, if no request can have more than 8 steps a CTA. That spares the second launch and the scan of the
-// lengths; beyond, the even split is worth more (items differ, and steps go to every SM).
+// lengths: one request of 1,001 keys takes 8.5 us, 12.5 with the even split. Beyond, the split is worth more (items differ,
+// and steps go to every SM): 4 requests of 131,072 keys leave a cluster form 128 of 444 CTAs.
 static int kv4_cluster(const Kv4AttArgs& a, int D, int R, int sms) {
     const long long items = (long long)a.B * a.pool.KVH, room = (long long)a.width * a.pool.page;
     const long long seen = a.window ? (room < (long long)a.window + a.max_q + KV4_STEP ? room : (long long)a.window + a.max_q + KV4_STEP) : room;

