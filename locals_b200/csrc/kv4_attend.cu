@@ -4,8 +4,8 @@
 // (window 0: from 0) to its own: out = sum_j e^(s_j - m) v_j / (sum_j e^(s_j - m) + e^(sink - m)), s_j = scale q . k_j,
 // and 0 where nothing is seen.
 //
-// kv4_attend_kernel. The rows of a (request, kv head) are its queries times the G query heads of the kv head; up to 8 NT
-// of them are the n side of m16n8k16 fp16 MMAs whose m side is 16 keys (scores, S^T = K Q^T) or 16 dimensions (values,
+// kv4_attend_kernel. The rows of a (request, kv head) are its queries times the G query heads of the kv head; a tile of 8 NT
+// of them is the n side of m16n8k16 fp16 MMAs whose m side is 16 keys (scores, S^T = K Q^T) or 16 dimensions (values,
 // O^T = V^T P^T), so that few rows fill the MMA and each key is unpacked once for all of them. The 4-bit codes enter the
 // MMA as fp16 subnormals, with no arithmetic at all: a word's bits & 0x000f000f are the pair (code 0, code 4) * 2^-24,
 // & 0x00f000f0 the pair (code 1, code 5) * 2^-20, and the same of word >> 8; every product of them is exact in the fp32
@@ -29,7 +29,7 @@
 // Each warp walks 32-key steps through a ring of its own, filled with cp.async STAGES - 1 steps ahead; the pages of the
 // next 8 steps are looked up by the 32 lanes at once (8 keys always lie in one page). Rows are permuted within a chunk
 // (P8) and 32-byte pieces swizzled (kv4_swz) so that every shared load is free of bank conflicts.
-// The keys of all (request, kv head)s, in steps of 128, are dealt out evenly over one wave of CTAs, wherever the boundaries
+// The keys of all (request, kv head, tile)s, in steps of 128, are dealt out evenly over one wave of CTAs, wherever the boundaries
 // fall; a CTA that holds only part of an item writes a part (m, l, O) to the workspace, at most two a CTA, and
 // kv4_join_kernel joins each divided item. Where every item can have a cluster of CTAs and few steps (kv4_cluster), the
 // cluster's CTAs share the item and join through distributed shared memory: one launch.
@@ -85,11 +85,18 @@ __device__ __forceinline__ Kv4Req kv4_request(const Kv4AttArgs& a, int b) {
     return r;
 }
 
-// Steps of all of request b's items.
+// Items of a request: its kv heads' tiles of R rows, a kv head's side by side (they read the same keys).
+template <int R>
+__device__ __forceinline__ int kv4_items(const Kv4AttArgs& a, const Kv4Req& r) {
+    return (r.fresh * a.G + R - 1) / R * a.pool.KVH;
+}
+
+// Units of all of request b's items.
+template <int R>
 __device__ __forceinline__ int kv4_weight(const Kv4AttArgs& a, int b) {
     if (b >= a.B) return 0;
     const Kv4Req r = kv4_request(a, b);
-    return r.fresh ? (r.steps() + KV4_ITEM) * a.pool.KVH : 0;
+    return r.fresh ? (r.steps() + KV4_ITEM) * kv4_items<R>(a, r) : 0;
 }
 
 // Inclusive sum over the CTA's 128 threads, and their total.
@@ -182,13 +189,13 @@ __global__ void __launch_bounds__(KV4_NW * 32, kv4_resident(D, NT)) kv4_attend_k
     int32_t* rec = a.records + blockIdx.x * 8;    // what the join kernel does for this CTA's first step
     if constexpr (!CL) {
         // ---- this CTA's share of the steps: requests are scanned 128 at a time ----
-        const int w0 = kv4_weight(a, tid);
+        const int w0 = kv4_weight<R>(a, tid);
         int sum0;
         const int s0 = kv4_scan(w0, red, &sum0);
         total = sum0;
         for (int b0 = KV4_NW * 32; b0 < a.B; b0 += KV4_NW * 32) {
             int sum;
-            kv4_scan(kv4_weight(a, b0 + tid), red, &sum);
+            kv4_scan(kv4_weight<R>(a, b0 + tid), red, &sum);
             total += sum;
         }
         n = int(min((long long)gridDim.x, total));  // (every CTA below n has a step, those above none)
@@ -198,7 +205,7 @@ __global__ void __launch_bounds__(KV4_NW * 32, kv4_resident(D, NT)) kv4_attend_k
         for (int b0 = 0;; b0 += KV4_NW * 32) {
             int sum = sum0, s = s0, w = w0;
             if (b0) {
-                w = kv4_weight(a, b0 + tid);
+                w = kv4_weight<R>(a, b0 + tid);
                 s = kv4_scan(w, red, &sum);
             }
             if (at + sum <= x0) {
@@ -230,24 +237,29 @@ __global__ void __launch_bounds__(KV4_NW * 32, kv4_resident(D, NT)) kv4_attend_k
 
     long long x = x0;
     while (x < x1) {
-        int kvh, st0, st1;
-        if constexpr (CL) b = int(blockIdx.x / kv4_cluster_size()) / KVH;
-        const Kv4Req rq = kv4_request(a, b);
+        int item, st0, st1;  // the request's item: kv head, tile
         if constexpr (CL) {
-            kvh = int(blockIdx.x / kv4_cluster_size()) - b * KVH;
+            const int per = KVH * ((a.split_rows + R - 1) / R);
+            item = int(blockIdx.x / kv4_cluster_size());
+            b = item / per;
+            item -= b * per;
+        }
+        const Kv4Req rq = kv4_request(a, b);
+        const int items = kv4_items<R>(a, rq), tiles = items / KVH;
+        if constexpr (CL) {
             st0 = rq.steps() * int(cluster_ctarank()) / int(kv4_cluster_size());
             st1 = rq.steps() * int(cluster_ctarank() + 1) / int(kv4_cluster_size());
             x = x1;
-            if (!rq.fresh) return;  // (the whole cluster)
+            if (item >= items) return;  // (the whole cluster)
         } else {
             const int units = rq.steps() + KV4_ITEM;
-            kvh = int((x - at) / units);
-            if (!rq.fresh || kvh >= KVH) {  // on to the next request
-                if (rq.fresh) at += (long long)units * KVH;
+            item = int((x - at) / units);
+            if (!rq.fresh || item >= items) {  // on to the next request
+                if (rq.fresh) at += (long long)units * items;
                 ++b;
                 continue;
             }
-            const long long item_at = at + (long long)kvh * units;
+            const long long item_at = at + (long long)item * units;
             const int u1 = int(min((long long)units, x1 - item_at));
             st0 = max(int(x - item_at) - KV4_ITEM, 0), st1 = max(u1 - KV4_ITEM, 0);
             x = item_at + u1;
@@ -255,19 +267,21 @@ __global__ void __launch_bounds__(KV4_NW * 32, kv4_resident(D, NT)) kv4_attend_k
             if (st0 > 0 && tid == 0) {  // (only a CTA's first item can begin before it)
                 const long long key0 = item_at + KV4_ITEM;
                 rec[1] = rq.first;
-                rec[2] = rq.fresh * G;
-                rec[3] = kvh;
+                rec[2] = min(rq.fresh * G - item % tiles * R, R);
+                rec[3] = item / tiles;
+                rec[5] = item % tiles * R;
                 rec[4] = kv4_owner(key0 + rq.steps() - 1, total, n);
                 rec[0] = kv4_owner(key0, total, n) == int(blockIdx.x) - 1;  // the first boundary within its item
             }
         }
-        const int rows = rq.fresh * G;
+        const int kvh = item / tiles, row0 = (item - kvh * tiles) * R, rows = min(rq.fresh * G - row0, R);
         // what the rows see: keys below hi_max, from lo_min on; all of them see [lo_max, hi_min)
         const int base = rq.len - rq.fresh;  // position of query 0
+        const int p0 = base + row0 / G, p1 = base + (row0 + rows - 1) / G;  // of the first and the last row
         const int room = int(min((long long)a.width * a.pool.page, 0x7fffffffLL));
         if (rq.len > room) record_status(LQ_DEV_BOUNDS);
-        const int hi_min = min(base + 1, room), hi_max = min(rq.len, room);
-        const int lo_min = a.window ? max(base + 1 - a.window, 0) : 0, lo_max = a.window ? max(rq.len - a.window, 0) : 0;
+        const int hi_min = min(p0 + 1, room), hi_max = min(p1 + 1, room);
+        const int lo_min = a.window ? max(p0 + 1 - a.window, 0) : 0, lo_max = a.window ? max(p1 + 1 - a.window, 0) : 0;
         const int k_lo = max((rq.s_lo + st0) * KV4_STEP, lo_min / KV4_KEYS * KV4_KEYS);
         const int k_hi = min((rq.s_lo + st1) * KV4_STEP, hi_max);
         // this warp's 32-key steps: first, first + 128, ...
@@ -335,8 +349,8 @@ __global__ void __launch_bounds__(KV4_NW * 32, kv4_resident(D, NT)) kv4_attend_k
             float mx = 0.0f;
 #pragma unroll
             for (int t = 0; t < NT; ++t) {
-                const int row = 8 * t + gid, qi = row / G;
-                const uint4* src = reinterpret_cast<const uint4*>(a.q + ((size_t)(rq.first + qi) * a.H + kvh * G + row - qi * G) * D);
+                const int row = 8 * t + gid, qi = (row0 + row) / G;
+                const uint4* src = reinterpret_cast<const uint4*>(a.q + ((size_t)(rq.first + qi) * a.H + kvh * G + row0 + row - qi * G) * D);
 #pragma unroll
                 for (int g = 0; g < GR; ++g)
 #pragma unroll
@@ -552,7 +566,7 @@ __global__ void __launch_bounds__(KV4_NW * 32, kv4_resident(D, NT)) kv4_attend_k
                 for (int tt = 0; tt < NT; ++tt)
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
-                        const int end = base + min(8 * tt + 2 * c + e, rows - 1) / G + 1;
+                        const int end = base + (row0 + min(8 * tt + 2 * c + e, rows - 1)) / G + 1;
                         const int hi = min(end, room), lo = a.window ? max(end - a.window, 0) : 0;
 #pragma unroll
                         for (int h = 0; h < 2; ++h)
@@ -686,7 +700,7 @@ __global__ void __launch_bounds__(KV4_NW * 32, kv4_resident(D, NT)) kv4_attend_k
         constexpr int V = D >= 128 ? 4 : 2, VU = D / (32 * V);
         using Vec = std::conditional_t<V == 4, float4, float2>;
         auto put = [&](int j, float M, float L, const float (&O)[VU][V], float sink) {
-            const int qi = j / G, head = kvh * G + j - qi * G;
+            const int qi = (row0 + j) / G, head = kvh * G + row0 + j - qi * G;
             uint16_t* dst = a.out + ((size_t)(rq.first + qi) * a.H + head) * D + lane * V;
 #pragma unroll
             for (int u = 0; u < VU; ++u) {
@@ -701,7 +715,7 @@ __global__ void __launch_bounds__(KV4_NW * 32, kv4_resident(D, NT)) kv4_attend_k
         for (int j = warp; j < rows; j += KV4_NW) {
             alignas(16) float O[VU][V];
             float M = -INFINITY, L = 0.0f;
-            const float sink = kv4_sink(a.sinks, kvh * G + j % G);
+            const float sink = kv4_sink(a.sinks, kvh * G + (row0 + j) % G);
 #pragma unroll
             for (int u = 0; u < VU; ++u)
 #pragma unroll
@@ -735,7 +749,7 @@ __global__ void __launch_bounds__(KV4_NW * 32, kv4_resident(D, NT)) kv4_attend_k
             const int C = int(kv4_cluster_size());
             const uint32_t base32 = smem_u32(mine);
             for (int j = int(cluster_ctarank()) + C * warp; j < rows; j += C * KV4_NW) {
-                const float sink = kv4_sink(a.sinks, kvh * G + j % G);
+                const float sink = kv4_sink(a.sinks, kvh * G + (row0 + j) % G);
                 const uint32_t own = map_peer(base32 + j * 4, min(lane, C - 1));  // lane k: CTA k's m and l
                 const float m = lane < C ? ld_dsmem_f(own) : -INFINITY, l = lane < C ? ld_dsmem_f(own + R * 4) : 0.0f;
                 alignas(16) float x[8][VU * V], O[VU][V];
@@ -790,7 +804,7 @@ __global__ void __launch_bounds__(128) kv4_join_kernel(const Kv4AttArgs a) {
     const int i = blockIdx.x, j = blockIdx.y, warp = threadIdx.x >> 5;
     const int32_t* rec = a.records + i * 8;
     if (!rec[0] || j >= rec[2]) return;
-    const int qi = j / a.G, head = rec[3] * a.G + j - qi * a.G;
+    const int row = rec[5] + j, qi = row / a.G, head = rec[3] * a.G + row - qi * a.G;
     kv4_join_row<T, D, 4>(a, R, j, i - 1, rec[4], warp, kv4_sink(a.sinks, head), a.out + ((size_t)(rec[1] + qi) * a.H + head) * D,
                           sum, sml);
 }
@@ -802,14 +816,16 @@ bool kv4_attend_shape_ok(int N, int B, int max_q, int H, int KVH, int width, int
            (long long)max_q * (H / KVH) < (1 << 30) && width >= 1 && window >= 0;
 }
 
-// Rows of kv4_attend's tiles, and the rows up to which a request is its own (above: kv4_prefill). 16 rows where every
-// request fits them (a key is then unpacked once for all); else as many as one query has, 8 or 16, for the requests of
-// a mixed batch that only decode. 0: none. 16 requests of 8,192 keys, 4 kv heads, D = 128: 8 rows 31 us, 16 rows
-// 39; 24 and 32 rows 111 and 117 in kv4_prefill.
-static void kv4_rows(int max_q, int G, int* R, int* split) {
-    const long long most = (long long)max_q * G;
-    *R = most <= 8 || (most > 16 && G <= 8) ? 8 : 16;
-    *split = most <= 16 ? int(most) : G <= 16 ? *R : 0;
+// Rows of kv4_attend's tiles, and the rows up to which a request is its own (above: kv4_prefill). 8 rows, or tiles of 16
+// up to 64 rows (32 at D = 256, where 16 rows' registers spill) if every request fits them; else as many as one query has, 8
+// or 16, for the requests of a mixed batch that only decode. 0: none. Each tile unpacks the keys again, but kv4_prefill
+// unpacks slower. 16 requests of 8,192 keys, 4 kv heads, here and there: D = 128, 24 rows 66 and 111 us, 48 rows 91 and 118,
+// 64 rows 116 and 123; D = 64, 64 rows 77 and 92; D = 256 (2 kv heads), 32 rows 99 and 100, 40 rows 132 and 99. 4 requests of
+// 700 keys, D = 128, 48 rows: 12.6 and 28.6 us.
+static void kv4_rows(int max_q, int G, int D, int* R, int* split) {
+    const long long most = (long long)max_q * G, own = D == 256 ? 32 : 64;
+    *R = most <= 8 || (most > own && G <= 8) ? 8 : 16;
+    *split = most <= own ? int(most) : G <= 16 ? *R : 0;
 }
 
 // One wave of CTAs, as many as are resident.
@@ -824,7 +840,7 @@ int kv4_prefill_run(const Kv4AttArgs& a, int D, int dtype, void* workspace, cuda
 
 size_t kv4_attend_workspace_bytes(int B, int max_q, int H, int KVH, int D, long long room) {
     int R, split;
-    kv4_rows(max_q, H / KVH, &R, &split);
+    kv4_rows(max_q, H / KVH, D, &R, &split);
     const int sms = device_info().sm_count;
     const bool many = (long long)max_q * (H / KVH) > split;
     return (split ? kv4_few_bytes(D, R, sms) : 0) + (many ? kv4_prefill_workspace_bytes(D, sms, B, KVH, H / KVH, max_q, room) : 0);
@@ -835,7 +851,7 @@ size_t kv4_attend_workspace_bytes(int B, int max_q, int H, int KVH, int D, long 
 // lengths: one request of 1,001 keys takes 8.5 us, 12.5 with the even split. Beyond, the split is worth more (items differ,
 // and steps go to every SM): 4 requests of 131,072 keys leave a cluster form 128 of 444 CTAs.
 static int kv4_cluster(const Kv4AttArgs& a, int D, int R, int sms) {
-    const long long items = (long long)a.B * a.pool.KVH, room = (long long)a.width * a.pool.page;
+    const long long items = (long long)a.B * a.pool.KVH * ((a.split_rows + R - 1) / R), room = (long long)a.width * a.pool.page;
     const long long seen = a.window ? (room < (long long)a.window + a.max_q + KV4_STEP ? room : (long long)a.window + a.max_q + KV4_STEP) : room;
     const long long steps = (seen + KV4_STEP - 1) / KV4_STEP;
     int C = 8;
@@ -851,10 +867,10 @@ static int kv4_attend_n(Kv4AttArgs a, cudaStream_t st) {
     static std::atomic<uint32_t> set{0}, set_cl{0}, none{0};
     const int sms = device_info().sm_count, C = kv4_cluster(a, D, R, sms), n = kv4_ctas(D, R, sms);
     if (C)
-        return kv4_launch(kv4_attend_kernel<T, D, NT, true>, set_cl, dim3(a.B * a.pool.KVH * C), dim3(KV4_NW * 32), smem, st, a, C);
+        return kv4_launch(kv4_attend_kernel<T, D, NT, true>, set_cl, dim3(a.B * a.pool.KVH * ((a.split_rows + R - 1) / R) * C), dim3(KV4_NW * 32), smem, st, a, C);
     int rc = kv4_launch(kv4_attend_kernel<T, D, NT, false>, set, dim3(n), dim3(KV4_NW * 32), smem, st, a);
     if (rc) return rc;
-    return kv4_launch(kv4_join_kernel<T, D, NT>, none, dim3(n, a.split_rows), dim3(128), 0, st, a);
+    return kv4_launch(kv4_join_kernel<T, D, NT>, none, dim3(n, R), dim3(128), 0, st, a);
 }
 
 template <typename T, int D>
@@ -892,7 +908,7 @@ int kv4_attend_run(const Kv4Pool& pool, const void* q, int N, const int32_t* q_s
     a.window = window;
     a.max_q = max_q;
     int R;
-    kv4_rows(max_q, a.G, &R, &a.split_rows);
+    kv4_rows(max_q, a.G, D, &R, &a.split_rows);
     uint8_t* ws = static_cast<uint8_t*>(workspace);
     if ((long long)max_q * a.G > a.split_rows) {
         const int rc = kv4_prefill_run(a, D, dtype, ws, st);

@@ -20,9 +20,9 @@
 //     128 keys at D = 128 take 1.45 us of products alone, 1.29 of unpacking alone, 2.5 together.
 // Roundings to fp16: queries after a power of two a row (exact for bf16 but for values 2^-26 below the row's largest); keys,
 // values and probabilities, 2^-11 each against the 2^-8 of a bf16 output (an fp16 output's error against 64 bits grows by
-// them from 2.1e-4 to 3.2e-4 .. 4.0e-4 of its size: the tensor cores take the operands in no finer type but at half the rate); values after a power of two that follows
-// their size, so that neither small nor large ones leave fp16's range. Keys beyond 65,504 are beyond what this form holds
-// and come out as infinities.
+// them from 2.1e-4 to 3.2e-4 .. 4.0e-4 of its size: the tensor cores take the operands in no finer type but at half the
+// rate); values after a power of two that follows their size, so that neither small nor large ones leave fp16's range. Keys
+// beyond 65,504 are beyond what this form holds and come out as infinities.
 // A masked score is -inf, its probability 0; a value whose scale or bias is not finite is held as 0 and its key as NaN,
 // so that only rows that see it become NaN.
 // Work is dealt out as in kv4_attend.cu: the steps of all tiles (each as far as its last row sees) evenly over one CTA a

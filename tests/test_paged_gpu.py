@@ -544,3 +544,25 @@ def test_attend_on_the_other_side_of_each_rule(cuda):
     _attend(cuda, [64, 3], [200, 3000], 8, 1, 128, 16, "float16", seed=44)     # two tiles of rows: unpacked in place
     _attend(cuda, [65, 3], [200, 3000], 8, 1, 128, 16, "float16", seed=45)     # a third: unpacked first
     _attend(cuda, [300, 1, 40], [700, 600, 41], 3, 1, 256, 24, "bfloat16", 0, True, seed=46)
+
+
+@pytest.mark.parametrize("new,lens,H,KVH,D,page,dtype,window,sinks", [
+    ([3, 2, 1, 3], [5, 700, 1, 131], 8, 1, 128, 16, "bfloat16", 0, True),       # 24 rows: two tiles, cut within a query's heads
+    ([7] * 40, [7 + 61 * i for i in range(40)], 9, 3, 64, 8, "float16", 0, False),  # 21 rows of 3 heads
+    ([2, 1], [40, 9000], 64, 4, 128, 32, "bfloat16", 100, False),               # 32 rows, a window, clusters
+    ([5, 0, 4], [2000, 30, 6000], 12, 2, 64, 16, "float16", 777, True),         # 30 rows; a request without queries
+    ([1] * 3, [300, 17, 5000], 32, 1, 128, 16, "float16", 0, True),             # one query of 32 heads
+    ([3, 3], [2500, 3], 8, 1, 256, 16, "bfloat16", 0, False),                   # 24 rows at 256 dimensions
+])
+def test_attend_two_tiles_of_rows(cuda, new, lens, H, KVH, D, page, dtype, window, sinks):
+    _attend(cuda, new, lens, H, KVH, D, page, dtype, window, sinks, seed=50)
+
+
+@pytest.mark.parametrize("new,lens,H,KVH,D,page,dtype,window,sinks", [
+    ([8, 5], [1000, 64], 16, 2, 128, 16, "bfloat16", 0, False),      # 64 rows: four tiles
+    ([9, 5], [1000, 64], 16, 2, 128, 16, "bfloat16", 0, False),      # 72: unpacked to tiles in place
+    ([16] * 9, [16 + 400 * i for i in range(9)], 4, 1, 64, 8, "float16", 300, True),
+    ([5, 1], [3000, 2], 8, 1, 256, 32, "float16", 0, True),          # 40 rows at 256 dimensions, in place
+])
+def test_attend_on_both_sides_of_the_row_limit(cuda, new, lens, H, KVH, D, page, dtype, window, sinks):
+    _attend(cuda, new, lens, H, KVH, D, page, dtype, window, sinks, seed=60)
