@@ -816,20 +816,25 @@ bool kv4_attend_shape_ok(int N, int B, int max_q, int H, int KVH, int width, int
            (long long)max_q * (H / KVH) < (1 << 30) && width >= 1 && window >= 0;
 }
 
-// Rows of kv4_attend's tiles, and the rows up to which a request is its own (above: kv4_prefill). 8 rows, or tiles of 16
-// up to 64 rows (32 at D = 256, where 16 rows' registers spill) if every request fits them; else as many as one query has, 8
-// or 16, for the requests of a mixed batch that only decode. 0: none. Each tile unpacks the keys again, but kv4_prefill
-// unpacks slower. 16 requests of 8,192 keys, 4 kv heads, here and there: D = 128, 24 rows 66 and 111 us, 48 rows 91 and 118,
-// 64 rows 116 and 123; D = 64, 64 rows 77 and 92; D = 256 (2 kv heads), 32 rows 99 and 100, 40 rows 132 and 99. 4 requests of
-// 700 keys, D = 128, 48 rows: 12.6 and 28.6 us.
-static void kv4_rows(int max_q, int G, int D, int* R, int* split) {
-    const long long most = (long long)max_q * G, own = D == 256 ? 32 : 64;
-    *R = most <= 8 || (most > own && G <= 8) ? 8 : 16;
-    *split = most <= own ? int(most) : G <= 16 ? *R : 0;
-}
-
 // One wave of CTAs, as many as are resident.
 static int kv4_ctas(int D, int R, int sms) { return sms * kv4_resident(D, R / 8); }
+
+// Rows of kv4_attend's tiles, and the rows up to which a request is its own (above: kv4_prefill). 8 rows, or tiles of 16, if
+// every request has at most 64 rows (32 at D = 256, where 16 rows' registers spill), or if all tiles' steps, by the keys that
+// the table can name, are no more than 8 a CTA (4 at D = 256); else as many as one query has, 8 or 16, for the requests of a
+// mixed batch that only decode. 0: none.
+// Each tile unpacks the keys again, but kv4_prefill unpacks slower. 16 requests of 8,192 keys, 4 kv heads, here and there:
+// D = 128, 24 rows 66 and 111 us, 48 rows 91 and 118, 64 rows 116 and 123; D = 64, 64 rows 77 and 92; D = 256 (2 kv heads),
+// 32 rows 99 and 100, 40 rows 132 and 99. And its items cost more to begin and end. One request, 4 kv heads, D = 128: 128 rows
+// on 500 keys 12.5 and 26.6 us, 1,024 rows on 128 keys 12.8 and 33.7; at the limit, 1,024 rows on 2,000 keys, 42.9 and 43.2;
+// D = 256 (2 kv heads): 512 rows on 500 keys 22.8 and 36.7.
+static void kv4_rows(int max_q, int G, int D, int B, int KVH, long long room, int* R, int* split) {
+    const long long most = (long long)max_q * G, own = D == 256 ? 32 : 64;
+    const double steps = double((most + 15) / 16) * B * KVH * double((room + KV4_STEP - 1) / KV4_STEP);
+    const bool few = most <= own || steps <= (D == 256 ? 4.0 : 8.0) * kv4_ctas(D, 16, device_info().sm_count);
+    *R = most <= 8 || (!few && G <= 8) ? 8 : 16;
+    *split = few ? int(most) : G <= 16 ? *R : 0;
+}
 
 static size_t kv4_few_bytes(int D, int R, int sms) {
     return size_t(kv4_ctas(D, R, sms)) * (2 * R * (2 + D) * sizeof(float) + 8 * sizeof(int32_t));
@@ -840,7 +845,7 @@ int kv4_prefill_run(const Kv4AttArgs& a, int D, int dtype, void* workspace, cuda
 
 size_t kv4_attend_workspace_bytes(int B, int max_q, int H, int KVH, int D, long long room) {
     int R, split;
-    kv4_rows(max_q, H / KVH, D, &R, &split);
+    kv4_rows(max_q, H / KVH, D, B, KVH, room, &R, &split);
     const int sms = device_info().sm_count;
     const bool many = (long long)max_q * (H / KVH) > split;
     return (split ? kv4_few_bytes(D, R, sms) : 0) + (many ? kv4_prefill_workspace_bytes(D, sms, B, KVH, H / KVH, max_q, room) : 0);
@@ -908,7 +913,7 @@ int kv4_attend_run(const Kv4Pool& pool, const void* q, int N, const int32_t* q_s
     a.window = window;
     a.max_q = max_q;
     int R;
-    kv4_rows(max_q, a.G, D, &R, &a.split_rows);
+    kv4_rows(max_q, a.G, D, B, pool.KVH, (long long)width * pool.page, &R, &a.split_rows);
     uint8_t* ws = static_cast<uint8_t*>(workspace);
     if ((long long)max_q * a.G > a.split_rows) {
         const int rc = kv4_prefill_run(a, D, dtype, ws, st);

@@ -305,12 +305,14 @@ def _cache(cuda, lens, KVH, D, page, dtype, seed, extra=3):
     return out[0], out[1], table
 
 
-def _attend(cuda, new, lens, H, KVH, D, page, dtype, window=0, sinks=False, seed=0, scale=None, pad=0, max_q=None):
+def _attend(cuda, new, lens, H, KVH, D, page, dtype, window=0, sinks=False, seed=0, scale=None, pad=0, max_q=None, columns=0):
     import torch
     from locals_b200 import paged
 
     g = _gen(cuda, seed + 77)
     keys, values, table = _cache(cuda, lens, KVH, D, page, dtype, seed)
+    if columns:  # room for more than the requests have
+        table = torch.cat([table, torch.full((len(lens), columns), -1, dtype=torch.int32, device=cuda)], 1)
     start = [0]
     for n in new:
         start.append(start[-1] + n)
@@ -566,3 +568,19 @@ def test_attend_two_tiles_of_rows(cuda, new, lens, H, KVH, D, page, dtype, windo
 ])
 def test_attend_on_both_sides_of_the_row_limit(cuda, new, lens, H, KVH, D, page, dtype, window, sinks):
     _attend(cuda, new, lens, H, KVH, D, page, dtype, window, sinks, seed=60)
+
+
+@pytest.mark.parametrize("new,lens,H,KVH,D,page,dtype,window,sinks", [
+    ([33], [33], 16, 4, 128, 16, "bfloat16", 0, False),                  # one tile of rows
+    ([130, 1, 64], [190, 500, 64], 8, 2, 128, 16, "bfloat16", 0, True),  # three tiles; prompts and decoding in one batch
+    ([257], [300], 5, 1, 64, 24, "float16", 0, False),                   # six tiles
+    ([60, 33], [1000, 35], 12, 2, 64, 8, "float16", 77, True),           # two tiles, windows
+    ([129], [640], 4, 2, 256, 16, "bfloat16", 50, False),
+    ([30, 0, 9], [30, 9, 2000], 8, 1, 256, 32, "float16", 0, True),      # a request without queries
+    ([200, 1, 1], [1500, 1, 2000], 16, 2, 128, 64, "float16", 0, True),
+])
+@pytest.mark.parametrize("room", [130_000, 2_400_000])
+def test_attend_in_a_wide_table(cuda, new, lens, H, KVH, D, page, dtype, window, sinks, room):
+    """Tables with room for long contexts: requests of many rows are taken in tiles of 128 and 256 rows, their keys unpacked
+    first, or, where all that the table can name would not fit the workspace as fp16, tile by tile."""
+    _attend(cuda, new, lens, H, KVH, D, page, dtype, window, sinks, seed=70, columns=room // page)
