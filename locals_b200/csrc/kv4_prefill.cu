@@ -31,7 +31,7 @@
 // which take as long as the products do at D = 128. Measured, GPU time of a call, bf16: 4,096 new tokens on 28,672 cached,
 // 16 heads on 2, D = 128: 1,016 to 1,020 us = 1,012 TFLOP/s (62% of the measured peak; 1,081 before the one pass); a mixed
 // batch of 8 (1 to 1,024 new on up to 2,048 cached, 32 heads on 8): 177 us = 543 TFLOP/s, the items' ends and short tiles;
-// 16 requests of 5 drafted tokens on up to 4,003 keys, 16 heads on 2, D = 256: 41.3 us, latency: 4 us to find the share, 6
+// 16 requests of 5 drafted tokens on up to 4,003 keys, 16 heads on 2, D = 256: 42.2 us, latency: 4 us to find the share, 6
 // to fetch the queries, 2 to 8 steps, 2 to write, and the joins.
 // Tried and slower: half the exponentials as polynomials (1,128 against 1,081 us); 4 unpacking warps of 128 registers (1,778);
 // 48 registers for the issuing warp (1,904); query rows fetched by neighbouring lanes (no faster, and 1,061 against 1,029).
@@ -659,6 +659,12 @@ __global__ void __launch_bounds__(pf_threads(DENSE), 1) kv4_prefill_kernel(const
                     return v;
                 };
                 auto seen = [](uint32_t score, uint32_t v, int i) { return (v >> i) & 1 ? __uint_as_float(score) : -INFINITY; };
+                // One query tile: a step's scores are issued before the last step's product, so that without this a warp could
+                // be done with an item while two products are to come, and the barrier's parity would take the one before both
+                // for the last. Before this step's probabilities are given out, the next product cannot be mistaken.
+                auto settled = [&]() {
+                    if (NQ == 1 && used > 0) pf_wait(&bar.o_done[w], (used - 1) & 1, abort);
+                };
                 // The common case, one pass: the reference from the steps before serves the step (found out at its end: the
                 // probabilities stay in registers until then, the scores in place).
                 auto once = [&](auto masked) -> bool {
@@ -700,6 +706,7 @@ __global__ void __launch_bounds__(pf_threads(DENSE), 1) kv4_prefill_kernel(const
                     tmem_wait_st();
                     tc_fence_before();
                     __syncwarp();
+                    settled();
                     if (lane == 0) mbar_arrive(&bar.p_full[buf]);
                     return true;
                 };
@@ -763,6 +770,7 @@ __global__ void __launch_bounds__(pf_threads(DENSE), 1) kv4_prefill_kernel(const
                 tmem_wait_st();
                 tc_fence_before();
                 __syncwarp();
+                settled();
                 if (lane == 0) mbar_arrive(&bar.p_full[buf]);
             }
             // ---- the row's output ----

@@ -584,3 +584,19 @@ def test_attend_in_a_wide_table(cuda, new, lens, H, KVH, D, page, dtype, window,
     """Tables with room for long contexts: requests of many rows are taken in tiles of 128 and 256 rows, their keys unpacked
     first, or, where all that the table can name would not fit the workspace as fp16, tile by tile."""
     _attend(cuda, new, lens, H, KVH, D, page, dtype, window, sinks, seed=70, columns=room // page)
+
+
+@pytest.mark.parametrize("most", [51, 101])
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
+def test_attend_prompts_at_256_dimensions(cuda, dtype, most):
+    """Many items of few steps a CTA: every warp has to have its row's last product before it writes the row."""
+    import torch
+
+    new = [most, 1, most - 20, 1, most, 30, 1, most // 2, 1, most - 1, 1]
+    lens = [144, 623, 2692, 592, 565, 909, 659, 119, 1495, 803, 1523]
+    for seed in (80, 81):
+        got, (q, keys, values, table, qs, scale, sk) = _attend(cuda, new, lens, 5, 1, 256, 16, dtype, seed=seed, columns=4000)
+        from locals_b200 import paged
+        for _ in range(5):
+            again = paged.attend(q, keys, values, table, _i32(lens, cuda), scale, q_start=qs, max_q=max(new))
+            assert torch.equal(got, again)
