@@ -243,8 +243,8 @@ int lq_kv_attend_noalloc(const void* q, const uint32_t* kq, const void* ks, cons
  * table) is recorded as LQ_DEV_BOUNDS in the device status and left out, never read or written. */
 
 /* A step's block tables and slot maps from the requests' lengths. cached, fresh (B): tokens held and new tokens
- * (negative: 0). table (B, width): the first ceil(cached / page_size) entries of a row are its pages; the pages that the
- * new tokens need beyond them are taken from free_pages[*head], free_pages[*head + 1], ... (nfree of them) in request
+ * (negative: 0; tokens beyond 2^31 - 65,537 a request are left out, with LQ_DEV_BOUNDS). table (B, width): the first
+ * ceil(cached / page_size) entries of a row are its pages; the pages that the new tokens need beyond them are taken from free_pages[*head], free_pages[*head + 1], ... (nfree of them) in request
  * order and entered. Written: lens (B) = cached + fresh; q_start (B + 1) the exclusive sums of fresh; for token t of the
  * step (tokens of them; those past q_start[B] are padding: position 0, slot -1) its positions[t] and slots[t];
  * head_out (1) the next free entry. head_out may not be head. A token that finds no page gets slot -1 (and

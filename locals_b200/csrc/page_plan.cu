@@ -9,9 +9,10 @@
 // One launch. Every CTA scans all the lengths for itself (B values, at most 8192: one load a thread and two warp scans
 // a 512 requests) and then takes its share of the tokens and of the new pages, each finding its request by a binary
 // search of the sums in shared memory; no CTA waits for another. A token whose page is new reads its id from the free
-// list, never from the table entry that another CTA may still be writing. What bounds it is latency: the launch, one
-// dependent load of the lengths, the scan, the search and one dependent page load. Measured, GPU time of a call: 64
-// requests of one token each 4.4 us, 200 of up to 512 each 6.4 us.
+// list, never from the table entry that another CTA may still be writing. Lengths are brought into range where they are
+// read (plan_length), and the sums stop at 2^31 - 1, so that no column or position wraps around, whatever the lengths
+// hold. What bounds it is latency: the launch, one dependent load of the lengths, the scan, the search and one dependent
+// page load. Measured, GPU time of a call: 64 requests of one token each 4.4 us, 200 of up to 512 each 6.4 us.
 #include <cuda_runtime.h>
 #include <stdint.h>
 
@@ -37,6 +38,18 @@ struct PlanArgs {
     int32_t* head_out;
     int B, width, nfree, page, tokens;
 };
+
+constexpr int PLAN_FAR = 0x7fffffff - 65536;  // a request's tokens at most: a page more is still below 2^31
+
+// Request b's cached tokens and new ones (negative: none); those beyond PLAN_FAR in all are left out.
+__device__ __forceinline__ void plan_length(const PlanArgs& a, int b, int* cached, int* fresh) {
+    const int c = a.cached[b], t = a.fresh[b];
+    *cached = min(max(c, 0), PLAN_FAR);
+    *fresh = min(max(t, 0), PLAN_FAR - *cached);
+    if (c > *cached || t > *fresh) record_status(LQ_DEV_BOUNDS);
+}
+// a + b of numbers from 0 on, at most 2^31 - 1.
+__device__ __forceinline__ int plan_add(int a, int b) { return int(min(unsigned(a) + unsigned(b), 0x7fffffffu)); }
 
 // The last i in [0, n) with a[i] <= x (a ascending, a[0] <= x).
 __device__ __forceinline__ int plan_find(const int32_t* a, int n, int x) {
@@ -64,8 +77,8 @@ __global__ void __launch_bounds__(PLAN_THREADS) page_plan_kernel(const PlanArgs 
         const int b = b0 + threadIdx.x;
         int t = 0, p = 0;
         if (b < a.B) {
-            const int c = max(a.cached[b], 0);
-            t = max(a.fresh[b], 0);
+            int c;
+            plan_length(a, b, &c, &t);
             p = (c + t + a.page - 1) / a.page - (c + a.page - 1) / a.page;
             if (blockIdx.x == 0) a.lens[b] = c + t;
         }
@@ -73,45 +86,49 @@ __global__ void __launch_bounds__(PLAN_THREADS) page_plan_kernel(const PlanArgs 
 #pragma unroll
         for (int d = 1; d < 32; d <<= 1) {
             const int ut = __shfl_up_sync(0xffffffffu, st, d), up = __shfl_up_sync(0xffffffffu, sp, d);
-            if (lane >= d) st += ut, sp += up;
+            if (lane >= d) st = plan_add(st, ut), sp = plan_add(sp, up);
         }
         if (lane == 31) wt[warp] = st, wp[warp] = sp;
         __syncthreads();
         int at = base_t, ap = base_p;
         for (int w = 0; w < PLAN_THREADS / 32; ++w) {
-            if (w < warp) at += wt[w], ap += wp[w];
-            base_t += wt[w];
-            base_p += wp[w];
+            if (w < warp) at = plan_add(at, wt[w]), ap = plan_add(ap, wp[w]);
+            base_t = plan_add(base_t, wt[w]);
+            base_p = plan_add(base_p, wp[w]);
         }
+        st = __shfl_up_sync(0xffffffffu, st, 1), sp = __shfl_up_sync(0xffffffffu, sp, 1);  // exclusive
+        if (lane == 0) st = sp = 0;
         if (b < a.B) {
-            tok[b] = at + st - t;
-            pag[b] = ap + sp - p;
-            if (blockIdx.x == 0) a.q_start[b] = at + st - t;
+            tok[b] = plan_add(at, st);
+            pag[b] = plan_add(ap, sp);
+            if (blockIdx.x == 0) a.q_start[b] = tok[b];
         }
         __syncthreads();  // the sums are in place, and wt / wp free for the next round
     }
     grid_dep_launch();
     if (blockIdx.x == 0 && threadIdx.x == 0) {
         a.q_start[a.B] = base_t;
-        *a.head_out = head + base_p;
+        *a.head_out = head < 0 ? head : plan_add(head, base_p);
         if (base_t > a.tokens || head < 0 || (long long)head + base_p > a.nfree) record_status(LQ_DEV_BOUNDS);
     }
-    const int step = gridDim.x * PLAN_THREADS, first = blockIdx.x * PLAN_THREADS + threadIdx.x;
-    for (int j = first; j < base_p; j += step) {  // the new pages
-        const int b = plan_find(pag, a.B, j);
-        const int col = (max(a.cached[b], 0) + a.page - 1) / a.page + j - pag[b];
+    const unsigned step = gridDim.x * PLAN_THREADS, first = blockIdx.x * PLAN_THREADS + threadIdx.x;
+    for (unsigned j = first; j < unsigned(base_p); j += step) {  // the new pages
+        const int b = plan_find(pag, a.B, int(j));
+        const int col = (min(max(a.cached[b], 0), PLAN_FAR) + a.page - 1) / a.page + int(j) - pag[b];
         const long long f = (long long)head + j;
-        if (col >= a.width)
+        if (col >= a.width) {  // on to the next request's
             record_status(LQ_DEV_BOUNDS);
-        else
+            j += ((b + 1 < a.B ? pag[b + 1] : base_p) - 1 - j) / step * step;
+        } else {
             a.table[size_t(b) * a.width + col] = f >= 0 && f < a.nfree ? a.free_pages[f] : -1;
+        }
     }
-    for (int i = first; i < a.tokens; i += step) {  // the new tokens (past the last one: position 0, no slot)
+    for (unsigned i = first; i < unsigned(a.tokens); i += step) {  // the new tokens (past the last one: position 0, no slot)
         int pos = 0, slot = -1;
-        if (i < base_t) {
-            const int b = plan_find(tok, a.B, i);
-            const int c = max(a.cached[b], 0);
-            pos = c + i - tok[b];
+        if (i < unsigned(base_t)) {
+            const int b = plan_find(tok, a.B, int(i));
+            const int c = min(max(a.cached[b], 0), PLAN_FAR);
+            pos = c + (int(i) - tok[b]);
             const int col = pos / a.page, have = (c + a.page - 1) / a.page;
             int id = -1;
             if (col < a.width) {

@@ -1,0 +1,52 @@
+"""Edges of the paged 4-bit cache's operators on the GPU: lengths and page ids that no server sends, queries, keys and values
+of very different sizes, pages freed behind a window, batches that break their bounds -- each in every form of the attention
+that a call can take (tests/paged_reference.py holds the plain statements in 64 bits)."""
+
+import pytest
+
+from tests.test_paged_gpu import BOUNDS, _i32, _status
+
+pytestmark = pytest.mark.gpu
+
+
+# ---- plan ----------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("cached,new", [
+    ([2 ** 31 - 1, 9], [1, 3]),                    # the page count of the first would wrap around
+    ([2 ** 31 - 1, 9], [2 ** 31 - 1, 3]),
+    ([2 ** 30, 9], [2 ** 31 - 1, 3]),
+    ([0, 9], [2 ** 31 - 1, 3]),
+    ([2 ** 31 - 65537, 2 ** 31 - 65537, 9], [5, 2 ** 31 - 1, 3]),
+    ([-2 ** 31, 5, 9], [-2 ** 31, 2 ** 31 - 1, 2 ** 31 - 1]),
+])
+@pytest.mark.parametrize("page", [8, 65536])
+def test_plan_lengths_beyond_31_bits(cuda, cached, new, page):
+    """Nothing is written outside the requests' table rows, positions never wrap around, and sums stop at 2^31 - 1."""
+    import torch
+    from locals_b200 import paged
+
+    B, width, tokens, most = len(cached), 4, 9, 2 ** 31 - 1
+    whole = torch.full((B + 64, width), -7, dtype=torch.int32, device=cuda)
+    table = whole[32:32 + B]
+    free = torch.arange(100, 200, dtype=torch.int32, device=cuda)
+    p = paged.plan(_i32(cached, cuda), _i32(new, cuda), table, free, _i32([1], cuda), page, tokens)
+    assert _status() == BOUNDS
+    assert bool((whole[:32] == -7).all()) and bool((whole[32 + B:] == -7).all())
+    far, lens, start, pages = most - 65536, [], [0], 0
+    for c, n in zip(cached, new):
+        c = min(max(c, 0), far)
+        n = min(max(n, 0), far - c)
+        lens.append(c + n)
+        start.append(min(start[-1] + n, most))
+        pages = min(pages + -(-(c + n) // page) - -(-c // page), most)
+    assert p.lens.tolist() == lens and p.q_start.tolist() == start and p.head.item() == min(1 + pages, most)
+    for t, (pos, slot) in enumerate(zip(p.positions.tolist(), p.slots.tolist())):
+        if t >= start[-1]:
+            assert (pos, slot) == (0, -1)
+            continue
+        b = max(i for i in range(B) if start[i] <= t)
+        assert pos == min(max(cached[b], 0), far) + t - start[b]
+        if slot >= 0:
+            col = pos // page
+            assert col < width and slot % page == pos % page
+            assert slot // page == table[b, col].item()
