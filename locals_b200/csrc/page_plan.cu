@@ -139,8 +139,9 @@ __global__ void __launch_bounds__(PLAN_THREADS) page_plan_kernel(const PlanArgs 
                     if (f >= 0 && f < a.nfree) id = a.free_pages[f];
                 }
             }
-            if (id >= 0)
-                slot = id * a.page + (pos - col * a.page);
+            const int off = pos - col * a.page;
+            if (id >= 0 && id <= (0x7fffffff - off) / a.page)  // (an id whose slots are beyond 31 bits is none)
+                slot = id * a.page + off;
             else
                 record_status(LQ_DEV_BOUNDS);
         }

@@ -50,3 +50,19 @@ def test_plan_lengths_beyond_31_bits(cuda, cached, new, page):
             col = pos // page
             assert col < width and slot % page == pos % page
             assert slot // page == table[b, col].item()
+
+
+def test_plan_page_ids_beyond_any_pool(cuda):
+    """An id whose slots are beyond 31 bits gets none of them: not a slot that its product wraps around to."""
+    import torch
+    from locals_b200 import paged
+
+    table = _i32([[2 ** 26 + 3, 5], [2 ** 31 - 1, -1]], cuda)
+    free = _i32([2 ** 27 + 1, 2 ** 27 - 1], cuda)
+    p = paged.plan(_i32([62, 0], cuda), _i32([4, 0], cuda), table, free, _i32([0], cuda), 64, 4)
+    # request 0: places 62 and 63 of an id beyond, then the second column is its own new page free[0], beyond too
+    assert p.positions.tolist() == [62, 63, 64, 65] and p.slots.tolist() == [-1, -1, -1, -1]
+    assert _status() == BOUNDS
+    last = 2 ** 31 // 16 - 1  # the last id whose slots fit
+    p = paged.plan(_i32([0], cuda), _i32([16], cuda), _i32([[-1]], cuda), _i32([last], cuda), _i32([0], cuda), 16, 16)
+    assert p.slots.tolist() == list(range(2 ** 31 - 16, 2 ** 31)) and _status() == 0
