@@ -16,6 +16,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #include "lq_host.h"
 #include "lq_ptx.cuh"
 #include "lq_status.cuh"
@@ -160,10 +162,17 @@ int page_plan_run(const int32_t* cached, const int32_t* fresh, int B, int32_t* t
                   int32_t* q_start, int32_t* positions, int32_t* slots, int32_t* head_out, cudaStream_t st) {
     const PlanArgs a = {cached, fresh, table, free_pages, head, lens, q_start, positions, slots, head_out,
                         B, width, nfree, page, tokens};
+    // Shared memory beyond the default limit, the static arrays among it: allowed once a device, up to the largest batch, so
+    // that a call depends on none before or beside it.
     const size_t smem = size_t(2 * B + 2) * sizeof(int32_t);
-    if (smem > 48 * 1024 && cudaFuncSetAttribute(page_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                                 int(smem)) != cudaSuccess)
-        return LQ_E_CUDA;
+    static std::atomic<uint32_t> set{0};
+    const uint32_t bit = 1u << (device_info().device & 31);
+    if (smem > 32 * 1024 && !(set.load(std::memory_order_relaxed) & bit)) {
+        if (cudaFuncSetAttribute(page_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                 int((2 * PLAN_MAX_B + 2) * sizeof(int32_t))) != cudaSuccess)
+            return LQ_E_CUDA;
+        set.fetch_or(bit, std::memory_order_relaxed);
+    }
     // one CTA a 512 tokens, at most one a SM (each further CTA scans the lengths again)
     const int ctas = max(1, min((tokens + PLAN_THREADS - 1) / PLAN_THREADS, device_info().sm_count));
     cudaLaunchConfig_t cfg = {};

@@ -66,3 +66,17 @@ def test_plan_page_ids_beyond_any_pool(cuda):
     last = 2 ** 31 // 16 - 1  # the last id whose slots fit
     p = paged.plan(_i32([0], cuda), _i32([16], cuda), _i32([[-1]], cuda), _i32([last], cuda), _i32([0], cuda), 16, 16)
     assert p.slots.tolist() == list(range(2 ** 31 - 16, 2 ** 31)) and _status() == 0
+
+
+@pytest.mark.parametrize("B", [6127, 6128, 6143, 6144])
+def test_plan_of_any_batch_in_a_new_process(B):
+    """A process's first plan, at the sizes around the default limit of shared memory."""
+    import subprocess
+    import sys
+
+    code = ("import torch\nfrom locals_b200 import paged\n"
+            f"B = {B}\ni = lambda *s, v=0: torch.full(s, v, dtype=torch.int32, device='cuda')\n"
+            "p = paged.plan(i(B), i(B, v=1), i(B, 1, v=-1), torch.arange(B, dtype=torch.int32, device='cuda'), i(1), 16, B)\n"
+            "assert p.slots.tolist() == [16 * b for b in range(B)]\n")
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True)
+    assert r.returncode == 0, r.stderr[-500:]
