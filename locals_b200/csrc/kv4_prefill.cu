@@ -276,11 +276,14 @@ struct PfBars {
     uint32_t run[4][16];
     int left[4], start[4];
     uint32_t gone[4];
-    float v_max[PF_UNPACK];
+    float v_max[2][PF_UNPACK];  // of step i & 1: each unpacking warp's largest |value|, negative from one that has no step
     int rows, steps;    // the item's (0: no more), from the first softmax warp to the issuing thread
 };
 
-// A bounded wait that, once any has given up, none of the CTA's takes again.
+// A bounded wait that, once any has given up, none of the CTA's takes again. After that every role still comes to its end by
+// itself: what it computes is void, but no warp waits at a barrier that another has passed by. Warps that meet at a barrier
+// (the unpacking ones, and the lanes of the page warp) leave their loops only together, on a word that all of them read
+// after they met; the others meet no one before the end. Copies and products in flight are waited for before the CTA ends.
 __device__ __forceinline__ void pf_wait(uint64_t* bar, uint32_t parity, volatile int* abort) {
     if (*abort) return;
     if (!mbar_wait(bar, parity)) *abort = 1;
@@ -838,12 +841,12 @@ __global__ void __launch_bounds__(pf_threads(DENSE), 1) kv4_prefill_kernel(const
             uint16_t ks[J], kb[J], vs[J], vb[J];
         };
         int asked = 0;
-        // issues the next step's loads; false when there is none
+        // issues the next step's loads; false (for the whole warp) when there is none
         auto fetch = [&](Held& h) -> bool {
             const int slot = asked & 3;
             pf_wait(&bar.r_full[slot], (asked >> 2) & 1, abort);
             const int left = *reinterpret_cast<volatile int*>(&bar.left[slot]);
-            if (left == 0 || *abort) return false;
+            if (__any_sync(0xffffffffu, left == 0 || *abort)) return false;
             ++asked;
 #pragma unroll
             for (int j = 0; j < J; ++j) {
@@ -862,36 +865,34 @@ __global__ void __launch_bounds__(pf_threads(DENSE), 1) kv4_prefill_kernel(const
         };
         float limit = 0.0f;
         int ve = 0;
-        // one step from its registers to the tiles
-        auto step_out = [&](const Held& h, int it) {
+        // one step from its registers to the tiles; false, in all warps at the same step, once one of them has none (at the
+        // end, or after an error, which they need not see at the same step)
+        auto step_out = [&](const Held& h, int it, bool have) -> bool {
             const int st = it & 1;
             const uint32_t par = ((it >> 1) & 1) ^ 1;
+            float top = 0.0f, ks[J], kb[J], vs[J], vb[J];
+            if (have) {
+#pragma unroll
+                for (int j = 0; j < J; ++j)
+                    top = fmaxf(top, pf_scales<T>(h.ks[j], h.kb[j], h.vs[j], h.vb[j], &ks[j], &kb[j], &vs[j], &vb[j]));
+            }
+            top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top)));
+            if (lane == 0) bar.v_max[st][uw] = have ? top : -1.0f;
+            named_barrier(1, PF_UNPACK * 32);  // (a slot is written again after the next step's barrier, which its readers pass later)
+            float M = 0.0f;
+            bool over = false;
+#pragma unroll
+            for (int i = 0; i < PF_UNPACK; ++i) {
+                const float x = reinterpret_cast<volatile float*>(bar.v_max[st])[i];
+                M = fmaxf(M, x);
+                over = over || x < 0.0f;
+            }
+            if (over) return false;
             if (*reinterpret_cast<volatile int*>(&bar.start[it & 3])) limit = 0.0f, ve = 0;
             // the values' power of two: the largest |value| a group can hold at 2^10 .. 2^15
-            float top = 0.0f, ks[J], kb[J], vs[J], vb[J];
-#pragma unroll
-            for (int j = 0; j < J; ++j) {
-                top = fmaxf(top, pf_scales<T>(h.ks[j], h.kb[j], h.vs[j], h.vb[j], &ks[j], &kb[j], &vs[j], &vb[j]));
-            }
-            int over;
-            asm volatile(
-                "{\n\t.reg .pred p, q;\n\t"
-                "setp.gt.f32 p, %1, %2;\n\t"
-                "barrier.cta.red.or.pred q, 1, %3, p;\n\t"
-                "selp.s32 %0, 1, 0, q;\n\t}"
-                : "=r"(over)
-                : "f"(top), "f"(limit), "n"(PF_UNPACK * 32)
-                : "memory");
-            if (over) {
-                const float wm = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top)));
-                if (lane == 0) bar.v_max[uw] = wm;
-                named_barrier(1, PF_UNPACK * 32);
-                float M = 0.0f;
-#pragma unroll
-                for (int i = 0; i < PF_UNPACK; ++i) M = fmaxf(M, reinterpret_cast<volatile float*>(bar.v_max)[i]);
+            if (M > limit) {
                 ve = pf_exponent(M);
                 limit = exp2f(float(15 - ve));
-                named_barrier(1, PF_UNPACK * 32);
             }
             const float vf = exp2f(float(ve));
             if (uw == 0 && lane == 0) {
@@ -912,16 +913,16 @@ __global__ void __launch_bounds__(pf_threads(DENSE), 1) kv4_prefill_kernel(const
             fence_proxy_async();
             __syncwarp();
             if (lane == 0) mbar_arrive(&bar.v_full[st]);
+            return true;
         };
         // two steps a turn, so that what is in flight stays in its registers
         Held h0, h1;
-        bool held = fetch(h0);
-        for (int it = 0; held; it += 2) {
-            const bool second = fetch(h1);
-            step_out(h0, it);
-            if (!second) break;
-            held = fetch(h0);
-            step_out(h1, it + 1);
+        bool first = fetch(h0);
+        for (int it = 0;; it += 2) {
+            const bool second = first && fetch(h1);
+            if (!step_out(h0, it, first)) break;
+            first = second && fetch(h0);
+            if (!step_out(h1, it + 1, second)) break;
         }
         }
     } else {
@@ -940,7 +941,7 @@ __global__ void __launch_bounds__(pf_threads(DENSE), 1) kv4_prefill_kernel(const
                              "l"(src), "r"(S::TB), "r"(smem_u32(full))
                              : "memory");
             };
-            int it = 0;
+            int it = 0, keys = 0, values = 0;  // steps, copies
             while (walk.next(a) && !*abort) {
                 const size_t tile0 = ((size_t)walk.b * a.pool.KVH + walk.kvh) * a.dense_steps + walk.lo;
                 for (int t = walk.st0; t < walk.st1; ++t, ++it) {
@@ -953,16 +954,17 @@ __global__ void __launch_bounds__(pf_threads(DENSE), 1) kv4_prefill_kernel(const
                     bar.v_exp[it & 3] = meta.x;
                     bar.miss[it & 3] = uint32_t(meta.y);
                     copy(&bar.k_full[st], sk + st * S::TB, src);
+                    ++keys;
                     pf_wait(&bar.v_empty[st], par, abort);
                     if (*abort) break;
                     copy(&bar.v_full[st], sv + st * S::TB, src + S::TB);
+                    ++values;
                 }
             }
-            // (what was copied has been waited for by the issuing thread, or, after an error, is waited for here)
-            for (int i = max(it - 2, 0); i < it && *abort; ++i) {
-                mbar_wait(&bar.k_full[i & 1], (i >> 1) & 1);
-                mbar_wait(&bar.v_full[i & 1], (i >> 1) & 1);
-            }
+            // The last copies into each buffer have landed before the CTA ends: the issuing thread waits for them too, but may
+            // have left after an error that this thread never saw. (Those before them were waited for with k_empty and v_empty.)
+            for (int i = max(keys - 2, 0); i < keys; ++i) mbar_wait(&bar.k_full[i & 1], (i >> 1) & 1);
+            for (int i = max(values - 2, 0); i < values; ++i) mbar_wait(&bar.v_full[i & 1], (i >> 1) & 1);
         }
         __syncwarp();
     } else if (!DENSE && warp == 1) {
@@ -972,7 +974,8 @@ __global__ void __launch_bounds__(pf_threads(DENSE), 1) kv4_prefill_kernel(const
         volatile int* const abort = at.abort;
         constexpr int RUNS = KT / 8;
         int it = 0;
-        while (walk.next(a) && !*abort) {
+        while (walk.next(a)) {
+            if (__any_sync(0xffffffffu, *abort)) break;  // (all lanes: they meet at each step's ballot)
             const int row0 = walk.tile * R, rows = min(R, walk.fresh * a.G - row0);
             const int key_end = min(walk.base + (row0 + rows - 1) / a.G + 1, room);
             for (int t = walk.st0; t < walk.st1; ++t, ++it) {
