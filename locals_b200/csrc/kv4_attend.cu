@@ -182,7 +182,7 @@ __global__ void __launch_bounds__(KV4_NW * 32, kv4_resident(D, NT)) kv4_attend_k
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gid = lane >> 2, c = lane & 3;
     const int tid = threadIdx.x, KVH = a.pool.KVH, G = a.G;
 
-    kv4_zero_tail(a, D);
+    kv4_zero_rest(a, D);
 
     int b = 0, n = 0;
     long long at = 0, total = 0, x0 = 0, x1 = 1;  // steps before request b; of all; this CTA's

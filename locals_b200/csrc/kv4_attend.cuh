@@ -53,30 +53,50 @@ struct Kv4Req {
     __device__ __forceinline__ int steps() const { return s_hi - s_lo; }
 };
 
-// first, fresh and len only.
+// Rows that request b names, within the queries.
+__device__ __forceinline__ void kv4_rows_of(const Kv4AttArgs& a, int b, int* from, int* to) {
+    *from = min(max(a.q_start[b], 0), a.N);
+    *to = max(min(a.q_start[b + 1], a.N), *from);
+}
+
+// first, fresh and len only. Of more than max_q queries (or of ones beyond the query rows) the first are kept, where they
+// stand: len then ends with the last that is kept.
 __device__ __forceinline__ Kv4Req kv4_new(const Kv4AttArgs& a, int b) {
     Kv4Req r;
     r.first = b;
     r.fresh = b < a.N ? 1 : 0;
+    r.len = max(a.lens[b], 0);
     if (a.q_start) {
-        r.first = max(a.q_start[b], 0);
-        r.fresh = max(min(a.q_start[b + 1], a.N) - r.first, 0);
-        if (r.fresh > a.max_q) {
+        int to;
+        kv4_rows_of(a, b, &r.first, &to);
+        r.fresh = min(to - r.first, a.max_q);
+        const int named = max(max(a.q_start[b + 1], 0) - r.first, 0);
+        if (named > r.fresh) {
             record_status(LQ_DEV_BOUNDS);
-            r.fresh = a.max_q;
+            r.len -= named - r.fresh;
         }
     }
-    r.len = a.lens[b];
     return r;
 }
 
-// Rows past the last query are 0 (the CTAs share them).
-__device__ __forceinline__ void kv4_zero_tail(const Kv4AttArgs& a, int D) {
+// Rows that no request's queries are: before the first, past the last, and beyond a request's max_q. They are 0 (the CTAs
+// share them).
+__device__ __forceinline__ void kv4_zero_rest(const Kv4AttArgs& a, int D) {
     if (!a.q_start) return;
     const long long row = (long long)a.H * D / 8;  // 16-byte pieces a token
-    const long long from = max(min(a.q_start[a.B], a.N), 0) * row, to = a.N * row;
-    for (long long i = from + (long long)blockIdx.x * blockDim.x + threadIdx.x; i < to; i += (long long)gridDim.x * blockDim.x)
-        reinterpret_cast<uint4*>(a.out)[i] = make_uint4(0, 0, 0, 0);
+    const long long tid = (long long)blockIdx.x * blockDim.x + threadIdx.x, threads = (long long)gridDim.x * blockDim.x;
+    auto zero = [&](int from, int to, long long first, long long step) {
+        for (long long i = from * row + first; i < to * row; i += step) reinterpret_cast<uint4*>(a.out)[i] = make_uint4(0, 0, 0, 0);
+    };
+    zero(0, min(max(a.q_start[0], 0), a.N), tid, threads);
+    zero(max(min(a.q_start[a.B], a.N), 0), a.N, tid, threads);
+    const int lane = threadIdx.x & 31;
+    for (long long b0 = tid & ~31LL; b0 < a.B; b0 += threads) {  // a warp 32 requests
+        int from = 0, to = 0;
+        if (b0 + lane < a.B) kv4_rows_of(a, int(b0) + lane, &from, &to);
+        for (uint32_t more = __ballot_sync(0xffffffffu, to - from > a.max_q); more; more &= more - 1)
+            zero(__shfl_sync(0xffffffffu, from, __ffs(more) - 1) + a.max_q, __shfl_sync(0xffffffffu, to, __ffs(more) - 1), lane, 32);
+    }
 }
 
 // The CTA that the x-th of S steps falls to: CTA i of n has steps i S / n .. (i + 1) S / n - 1.

@@ -448,7 +448,7 @@ __global__ void __launch_bounds__(pf_threads(DENSE), 1) kv4_prefill_kernel(const
         fence_barrier_init();
     }
     grid_dep_wait();
-    if (a.split_rows == 0) kv4_zero_tail(a, D);  // (else kv4_attend does)
+    if (a.split_rows == 0) kv4_zero_rest(a, D);  // (else kv4_attend does)
     // ---- this CTA's share ----
     // up to 32 threads a request sum its tiles' units; then requests, and the tiles of the one found, are scanned together
     int each = 32;

@@ -87,8 +87,8 @@ def attend(q: torch.Tensor, keys: Sequence[torch.Tensor], values: Sequence[torch
            lens: torch.Tensor, scale: float, q_start: Optional[torch.Tensor] = None, max_q: int = 1,
            sinks: Optional[torch.Tensor] = None, window: int = 0) -> torch.Tensor:
     """Attention of a step's queries over the pages: ``q`` (N, H, D), request b's queries being rows ``q_start[b]`` to
-    ``q_start[b + 1]`` - 1 (None: row b, one each), at most ``max_q`` of them; they are the last of its ``lens[b]`` tokens,
-    whose keys and values are already in the cache, in the pages of ``block_table[b]``. A query sees the keys up to its
+    ``q_start[b + 1]`` - 1 (None: row b, one each), at most ``max_q`` of them (of more, the first ``max_q`` are answered, and
+    LQ_DEV_BOUNDS is set); they are the last of its ``lens[b]`` tokens, whose keys and values are already in the cache, in the pages of ``block_table[b]``. A query sees the keys up to its
     own position, the last ``window`` of them when that is not 0. ``sinks`` (H,) float32 logits join the softmax's sum.
-    Returns (N, H, D) in q's dtype: 0 where a query sees nothing, and in rows past ``q_start[-1]``."""
+    Returns (N, H, D) in q's dtype: 0 where a query sees nothing, and in rows that are no answered query's."""
     return ext().attend(q, keys, values, block_table, lens, scale, q_start, max_q, sinks, window)

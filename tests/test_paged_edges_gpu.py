@@ -4,7 +4,8 @@ that a call can take (tests/paged_reference.py holds the plain statements in 64 
 
 import pytest
 
-from tests.test_paged_gpu import BOUNDS, _i32, _status
+from tests import paged_reference as R
+from tests.test_paged_gpu import BOUNDS, _cache, _gen, _i32, _status
 
 pytestmark = pytest.mark.gpu
 
@@ -80,3 +81,28 @@ def test_plan_of_any_batch_in_a_new_process(B):
             "assert p.slots.tolist() == [16 * b for b in range(B)]\n")
     r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True)
     assert r.returncode == 0, r.stderr[-500:]
+
+
+# ---- attend: bounds of a batch -----------------------------------------------------------------------
+
+@pytest.mark.parametrize("columns", [0, 9000])
+def test_attend_more_queries_than_max_q(cuda, columns):
+    """The first max_q of a request's queries stand where they stand; its others, rows before q_start[0] and rows past
+    q_start[-1] are 0."""
+    import torch
+    from locals_b200 import paged
+
+    g = _gen(cuda, 5)
+    lens, H, KVH, D = [300, 90, 41], 8, 2, 128
+    keys, values, table = _cache(cuda, lens, KVH, D, 16, "bfloat16", 5)
+    table = torch.cat([table, torch.full((3, columns), -1, dtype=torch.int32, device=cuda)], 1)
+    start, most = [3, 53, 54, 94], 40  # 50, 1 and 40 queries
+    q = torch.randn((100, H, D), generator=g, device=cuda).to(torch.bfloat16)
+    torch.full((4, 100, H, D), float("nan"), device=cuda)  # (what the output's memory may hold)
+    got = paged.attend(q, keys, values, table, _i32(lens, cuda), 0.1, q_start=_i32(start, cuda), max_q=most)
+    assert _status() == BOUNDS
+    ref, bound = R.attended(q, keys, values, table, _i32(lens, cuda), 0.1, _i32(start, cuda), None, 0)
+    ref[3 + most:53], bound[3 + most:53] = 0, 0
+    assert bool(((got.double() - ref).abs() <= bound).all())
+    for rows in (got[:3], got[3 + most:53], got[94:]):
+        assert torch.count_nonzero(rows).item() == 0
