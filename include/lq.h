@@ -285,7 +285,8 @@ int lq_kv4_read(const uint32_t* kq, const void* ks, const void* kb, const uint32
  * (q_start NULL: row b, one each), the last of them at position lens[b] - 1; of more than max_q the first max_q are
  * answered (and LQ_DEV_BOUNDS). A query sees the keys up to its own position, the last `window` of them when window > 0.
  * out = sum p v / (sum p + e^sink), p = e^(scale q . k), softmax statistics in 32 bits; sinks (H) float32 or NULL; 0 where a
- * query sees nothing and in rows that are no answered query's. table (B, width) page ids, -1 where there is none. workspace:
+ * query sees nothing and in rows that are no answered query's. table (B, width) page ids, -1 where there is none (pages wholly
+ * behind the window of all of a request's queries may be gone). workspace:
  * lq_kv4_attend_workspace(B, max_q, H, KVH, head_dim, width, page_size) bytes, 128-byte aligned (NULL when that is 0):
  * the parts of split softmaxes, and, where max_q is large and width * page_size * B keys fit 1 GiB that way, the keys and
  * values of requests with many rows as fp16 tiles. */

@@ -288,13 +288,13 @@ __global__ void __launch_bounds__(KV4_NW * 32, kv4_resident(D, NT)) kv4_attend_k
         const int first = ((k_lo + KV4_STEP - 1 - warp * KV4_KEYS) / KV4_STEP) * KV4_STEP + warp * KV4_KEYS;
         const int steps = k_hi > first ? (k_hi - first + KV4_STEP - 1) / KV4_STEP : 0;
 
-        // lane l's page lookup: run l & 3 (of 8 keys) of step t0 + (l >> 2); row 0 where there is none. miss: bit l, the
-        // run is within the range but has no page
+        // lane l's page lookup: run l & 3 (of 8 keys) of step t0 + (l >> 2); row 0 where there is none. miss: bit l, some row
+        // sees the run but it has no page (what lies behind a window may have been freed)
         auto lookup = [&](int t0, uint32_t* miss) -> uint32_t {
             const int key = first + (t0 + (lane >> 2)) * KV4_STEP + (lane & 3) * 8;
             uint32_t row = 0;
             bool gone = false;
-            if (t0 + (lane >> 2) < steps && key < hi_max) {
+            if (t0 + (lane >> 2) < steps && key < hi_max && key + 8 > lo_min) {
                 const int pg = key / a.pool.page, id = a.table[(size_t)b * a.width + pg];
                 gone = unsigned(id) >= unsigned(a.pool.pages);
                 if (gone)

@@ -359,10 +359,11 @@ __global__ void __launch_bounds__(PD_WARPS * 32) kv4_dense_kernel(const Kv4AttAr
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(pf_raw) + 127) & ~uintptr_t(127));
     const uint32_t tile = smem_u32(smem);
     constexpr int RUNS = S::KT / 8;
+    const int seen_from = a.window ? max(base + 1 - a.window, 0) : 0;  // (the first query's)
     const int key0 = s * S::KT, run_key = key0 + (lane % RUNS) * 8;
     uint32_t mine = KV4_NONE;
     bool gone = false;
-    if (run_key < keys) {
+    if (run_key < keys && run_key + 8 > seen_from) {  // (what lies behind a window may have been freed)
         const int pg = run_key / a.pool.page, id = a.table[(size_t)b * a.width + pg];
         gone = unsigned(id) >= unsigned(a.pool.pages);
         if (gone)
@@ -978,11 +979,12 @@ __global__ void __launch_bounds__(pf_threads(DENSE), 1) kv4_prefill_kernel(const
             if (__any_sync(0xffffffffu, *abort)) break;  // (all lanes: they meet at each step's ballot)
             const int row0 = walk.tile * R, rows = min(R, walk.fresh * a.G - row0);
             const int key_end = min(walk.base + (row0 + rows - 1) / a.G + 1, room);
+            const int seen_from = a.window ? max(walk.base + row0 / a.G + 1 - a.window, 0) : 0;
             for (int t = walk.st0; t < walk.st1; ++t, ++it) {
                 const int slot = it & 3, key0 = (walk.lo + t) * KT, key = key0 + (lane % RUNS) * 8;
                 uint32_t row = KV4_NONE;
                 bool gone = false;
-                if (key < key_end) {
+                if (key < key_end && key + 8 > seen_from) {  // (what lies behind a window may have been freed)
                     const int pg = key / a.pool.page, id = a.table[(size_t)walk.b * a.width + pg];
                     gone = unsigned(id) >= unsigned(a.pool.pages);
                     if (gone)

@@ -5,7 +5,7 @@ that a call can take (tests/paged_reference.py holds the plain statements in 64 
 import pytest
 
 from tests import paged_reference as R
-from tests.test_paged_gpu import BOUNDS, _cache, _gen, _i32, _status
+from tests.test_paged_gpu import BOUNDS, _attend, _cache, _gen, _i32, _status
 
 pytestmark = pytest.mark.gpu
 
@@ -106,3 +106,22 @@ def test_attend_more_queries_than_max_q(cuda, columns):
     assert bool(((got.double() - ref).abs() <= bound).all())
     for rows in (got[:3], got[3 + most:53], got[94:]):
         assert torch.count_nonzero(rows).item() == 0
+
+
+@pytest.mark.parametrize("new,columns,H,D", [(1, 0, 8, 128), (3, 0, 8, 64), (40, 9000, 8, 128), (140, 9000, 8, 128),
+                                             (60, 9000, 4, 256), (140, 9000, 4, 256)])
+def test_attend_pages_freed_behind_a_window(cuda, new, columns, H, D):
+    """Table entries wholly behind the window may be -1, or anything: no key there is missed."""
+    import torch
+    from locals_b200 import paged
+
+    n, page, window = 1000, 16, 333
+    got, (q, keys, values, table, qs, scale, _) = _attend(cuda, [new], [n], H, 2, D, page, "bfloat16", window, seed=9,
+                                                          columns=columns, max_q=new)
+    freed = table.clone()
+    behind = max(0, n - new + 1 - window) // page
+    assert behind > 20
+    freed[0, :behind] = -1
+    again = paged.attend(q, keys, values, freed, _i32([n], cuda), scale, q_start=qs, max_q=new, window=window)
+    assert _status() == 0
+    assert torch.equal(again, got)
