@@ -15,8 +15,8 @@
 //   s_j = scale * sum_g ks_jg (q . codes)_g + kb_jg sum(q)_g,
 //   o_g = sum_j w_jg (codes_jg - z_jg) + p_j (vb_jg + z_jg vs_jg),   w_jg = p_j vs_jg,  z_jg = round(-vb_jg / vs_jg) in 0..15.
 // Scores, softmax statistics and outputs are fp32. Two roundings to fewer bits:
-//   queries to fp16 after one power of two an item that puts the largest at 2^13 .. 2^14: exact for fp16 and bf16 but for
-//     values 2^-27 below the item's largest;
+//   queries to fp16 after a power of two a row that puts its largest at 2^13 .. 2^14: exact for fp16 and bf16 but for
+//     values 2^-27 below the row's largest. A row by itself: the tile holds other heads and other tokens of the request;
 //   w to fp16 (2^-11 against the 2^-8 of a bf16 output; an fp16 output's error grows from 2.0e-4 to 2.2e-4 by it), after a
 //     power of two that puts the warp's largest value scale at 2^5 .. 2^10. codes - z (exact on subnormals, one packed subtraction a pair) takes out of a group
 //     what its codes and its bias have in common, so that this is a rounding of the value itself, however near to 0 it lies.
@@ -341,12 +341,12 @@ __global__ void __launch_bounds__(KV4_NW * 32, kv4_resident(D, NT)) kv4_attend_k
             commit();
         }
 
-        // ---- queries: fp16 B fragments times one power of two, and the group sums of what the MMA sees ----
+        // ---- queries: fp16 B fragments times a row's power of two, and the group sums of what the MMA sees ----
+        // (2^24 of the codes: 2^12 with the scales, 2^12 with the row's factor alpha, so that neither leaves its range)
         uint32_t qb[NT][GR][2][2][2];
-        float qs[NT][GR][2], alpha;
+        float qs[NT][GR][2], alpha[NT][2];
         {
             uint4 raw[NT][GR][2];
-            float mx = 0.0f;
 #pragma unroll
             for (int t = 0; t < NT; ++t) {
                 const int row = 8 * t + gid, qi = (row0 + row) / G;
@@ -357,7 +357,8 @@ __global__ void __launch_bounds__(KV4_NW * 32, kv4_resident(D, NT)) kv4_attend_k
                     for (int u = 0; u < 2; ++u) raw[t][g][u] = row < rows ? src[8 * g + 2 * c + u] : make_uint4(0, 0, 0, 0);
             }
 #pragma unroll
-            for (int t = 0; t < NT; ++t)
+            for (int t = 0; t < NT; ++t) {
+                float mx = 0.0f;  // of row gid: its four lanes'
 #pragma unroll
                 for (int g = 0; g < GR; ++g)
 #pragma unroll
@@ -368,14 +369,14 @@ __global__ void __launch_bounds__(KV4_NW * 32, kv4_resident(D, NT)) kv4_attend_k
                             mx = fmaxf(mx, fmaxf(fabsf(F16Traits<T>::to_f32(w[i] & 0xffffu)),
                                                  fabsf(F16Traits<T>::to_f32(w[i] >> 16))));
                     }
-            // 2^E with the largest |q| at 2^13 .. 2^14
-            const uint32_t mb = __reduce_max_sync(0xffffffffu, __float_as_uint(mx));
-            const int E = min(max(mb ? 13 - (int(mb >> 23) - 127) : 0, -100), 100);
-            const float f = __uint_as_float(uint32_t(127 + E) << 23);
-            const float back = a.scale_log2 * __uint_as_float(uint32_t(127 - E) << 23);
-            alpha = back * 16777216.0f;
+                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+                // 2^E with the largest |q| at 2^13 .. 2^14
+                const int E = mx > 0.0f ? min(13 - (int(__float_as_uint(mx) >> 23) - 127), 126) : 0;
+                const float f = __uint_as_float(uint32_t(127 + E) << 23);
+                const float back = a.scale_log2 * __uint_as_float(uint32_t(127 + 12 - E) << 23);
 #pragma unroll
-            for (int t = 0; t < NT; ++t)
+                for (int e = 0; e < 2; ++e) alpha[t][e] = __shfl_sync(0xffffffffu, back, (2 * c + e) * 4);
 #pragma unroll
                 for (int g = 0; g < GR; ++g) {
                     float sum = 0.0f;
@@ -400,8 +401,9 @@ __global__ void __launch_bounds__(KV4_NW * 32, kv4_resident(D, NT)) kv4_attend_k
                     sum += __shfl_xor_sync(0xffffffffu, sum, 2);
 #pragma unroll
                     for (int e = 0; e < 2; ++e)  // this lane's columns 2c + e of the score tile
-                        qs[t][g][e] = back * __shfl_sync(0xffffffffu, sum, (2 * c + e) * 4);
+                        qs[t][g][e] = 0x1p-12f * __shfl_sync(0xffffffffu, sum, (2 * c + e) * 4);
                 }
+            }
         }
 
         float o[NT][4 * GR][4], hb[NT][GR][2], m[NT][2], l[NT][2];
@@ -502,7 +504,7 @@ __global__ void __launch_bounds__(KV4_NW * 32, kv4_resident(D, NT)) kv4_attend_k
                 for (int g = 0; g < GR; ++g) {
                     // round(-vb / vs) in 0 .. 15, its bits the last of 1.5 * 2^23 + z
                     const float u = fminf(fmaxf(__fdividef(-w[3][g], w[2][g]), 0.0f), 15.0f) + 12582912.0f;
-                    f[g] = w[0][g] * alpha;
+                    f[g] = w[0][g] * 4096.0f;
                     f[GR + g] = w[1][g];
                     f[2 * GR + g] = w[2][g] * vf;
                     f[3 * GR + g] = fmaf(u - 12582912.0f, w[2][g], w[3][g]) * vf;
@@ -557,7 +559,7 @@ __global__ void __launch_bounds__(KV4_NW * 32, kv4_resident(D, NT)) kv4_attend_k
                             for (int g = 1; g < GR; ++g) s = fmaf(f[GR + g], qs[tt][g][e], s);
 #pragma unroll
                             for (int g = 0; g < GR; ++g) s = fmaf(f[g], acc[tt][g][2 * u + e], s);
-                            sc[tt][h][u][e] = s;
+                            sc[tt][h][u][e] = s * alpha[tt][e];
                         }
                 }
             }

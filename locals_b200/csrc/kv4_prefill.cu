@@ -606,7 +606,7 @@ __global__ void __launch_bounds__(pf_threads(DENSE), 1) kv4_prefill_kernel(const
                     }
                 }
                 int E = mx > 0.0f ? 12 - (int((__float_as_uint(mx) >> 23) & 0xff) - 127) : 0;
-                E = min(max(E, -100), 100);
+                E = min(E, 126);  // (from -116, an infinity's)
                 const float f = some ? copysignf(__uint_as_float(uint32_t(127 + E) << 23), a.scale_log2) : 0.0f;
                 c = a.scale_log2 != 0.0f ? fabsf(a.scale_log2) * __uint_as_float(uint32_t(127 - E) << 23) : 1.0f;
                 const uint32_t dst = sq + w * S::QB + wr * 128;

@@ -2,6 +2,8 @@
 of very different sizes, pages freed behind a window, batches that break their bounds -- each in every form of the attention
 that a call can take (tests/paged_reference.py holds the plain statements in 64 bits)."""
 
+import math
+
 import pytest
 
 from tests import paged_reference as R
@@ -125,3 +127,71 @@ def test_attend_pages_freed_behind_a_window(cuda, new, columns, H, D):
     again = paged.attend(q, keys, values, freed, _i32([n], cuda), scale, q_start=qs, max_q=new, window=window)
     assert _status() == 0
     assert torch.equal(again, got)
+
+
+# ---- attend: sizes -----------------------------------------------------------------------------------
+
+FORMS = [  # new, query heads, kv heads, head_dim, columns of 16 keys
+    (5, 8, 2, 128, 0),        # few rows, a cluster an item
+    (5, 8, 2, 128, 9000),     # few rows, the even split
+    (5, 8, 2, 64, 9000),
+    (5, 8, 2, 256, 9000),
+    (40, 8, 2, 128, 9000),    # many rows, unpacked in place
+    (140, 8, 2, 64, 9000),    # many rows, unpacked first
+    (140, 8, 2, 128, 9000),
+    (40, 8, 2, 256, 9000),
+    (140, 8, 2, 256, 9000),
+]
+
+
+def _case(cuda, new, H, KVH, D, columns, seed, n=300, dtype="bfloat16"):
+    import torch
+
+    g = _gen(cuda, seed)
+    keys, values, table = _cache(cuda, [n], KVH, D, 16, dtype, seed)
+    table = torch.cat([table, torch.full((1, columns), -1, dtype=torch.int32, device=cuda)], 1)
+    q = (1.5 * torch.randn((new, H, D), generator=g, device=cuda)).to(getattr(torch, dtype))
+    return q, keys, values, table, _i32([n], cuda), _i32([0, new], cuda)
+
+
+def _held(q, keys, values, table, lens, scale, qs, sinks=None, window=0):
+    """The attention, checked against the 64-bit statement where that is a number."""
+    import torch
+    from locals_b200 import paged
+
+    got = paged.attend(q, keys, values, table, lens, scale, q_start=qs, max_q=q.shape[0], sinks=sinks, window=window)
+    ref, bound = R.attended(q, keys, values, table, lens, scale, qs, sinks, window)
+    off = (got.double() - ref).abs() - bound
+    assert bool((off <= 0).all()), f"beyond the bound by {off.max().item()}, {(got.double() - ref).abs().max().item()} in all"
+    return got
+
+
+@pytest.mark.parametrize("new,H,KVH,D,columns", FORMS)
+def test_attend_a_query_of_any_size_moves_no_other_row(cuda, new, H, KVH, D, columns):
+    import torch
+    from locals_b200 import paged
+
+    q, keys, values, table, lens, qs = _case(cuda, new, H, KVH, D, columns, 21)
+    got = _held(q, keys, values, table, lens, D ** -0.5, qs)
+    for bad in (math.inf, -math.inf, math.nan, 2.0 ** 100, -2.0 ** 40):
+        poisoned = q.clone()
+        poisoned[new - 1, 2, 7] = bad  # the last token's third head
+        again = paged.attend(poisoned, keys, values, table, lens, D ** -0.5, q_start=qs, max_q=new)
+        same = torch.ones_like(q, dtype=torch.bool)
+        same[new - 1, 2] = False
+        assert torch.equal(again[same], got[same]), bad
+        if not math.isfinite(bad):
+            assert not bool(torch.isfinite(again[new - 1, 2].float()).all())
+
+
+@pytest.mark.parametrize("new,H,KVH,D,columns", FORMS)
+def test_attend_queries_of_very_different_sizes(cuda, new, H, KVH, D, columns):
+    """Rows 2^-30 to 2^30 times the usual: each is held to its own size (a large one's largest score takes all)."""
+    import torch
+
+    q, keys, values, table, lens, qs = _case(cuda, new, H, KVH, D, columns, 22)
+    size = 2.0 ** torch.linspace(-30, 0, new * H, device=q.device).round().view(new, H, 1)
+    _held((q.float() * size).to(q.dtype), keys, values, table, lens, D ** -0.5, qs)
+    # both inverse sizes at once: the scores are ordinary ones again
+    for e in (20, -20, 110, -110):
+        _held((q.float() * 2.0 ** e).to(q.dtype), keys, values, table, lens, D ** -0.5 * 2.0 ** -e, qs)
