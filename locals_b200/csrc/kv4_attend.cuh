@@ -37,9 +37,10 @@ struct Kv4AttArgs {
     int split_rows;  // requests of more rows are kv4_prefill's
 };
 
-// A sink's logit in base 2, finite at its upper end so that differences from it stay numbers.
+// A sink's logit in base 2, finite at its upper end so that differences from it stay numbers. (A NaN stays one.)
 __device__ __forceinline__ float kv4_sink(const float* sinks, int head) {
-    return sinks ? fminf(sinks[head] * KV4_LOG2E, 3.4028234e38f) : -INFINITY;
+    const float s = sinks ? sinks[head] * KV4_LOG2E : -INFINITY;
+    return s > 3.4028234e38f ? 3.4028234e38f : s;
 }
 __device__ __forceinline__ float kv4_ex2(float x) {
     float y;

@@ -195,3 +195,21 @@ def test_attend_queries_of_very_different_sizes(cuda, new, H, KVH, D, columns):
     # both inverse sizes at once: the scores are ordinary ones again
     for e in (20, -20, 110, -110):
         _held((q.float() * 2.0 ** e).to(q.dtype), keys, values, table, lens, D ** -0.5 * 2.0 ** -e, qs)
+
+
+@pytest.mark.parametrize("new,H,KVH,D,columns", FORMS)
+def test_attend_a_sink_that_is_not_a_number(cuda, new, H, KVH, D, columns):
+    """It makes its own head NaN and no other; a query that sees nothing stays 0."""
+    import torch
+    from locals_b200 import paged
+
+    q, keys, values, table, lens, qs = _case(cuda, new, H, KVH, D, columns, 27)
+    sinks = torch.linspace(-1, 1, H, device=q.device)
+    got = _held(q, keys, values, table, lens, D ** -0.5, qs, sinks)
+    sinks[3] = math.nan
+    again = paged.attend(q, keys, values, table, lens, D ** -0.5, q_start=qs, max_q=new, sinks=sinks)
+    assert bool(torch.isnan(again[:, 3]).all())
+    others = [h for h in range(H) if h != 3]
+    assert torch.equal(again[:, others], got[:, others])
+    none = paged.attend(q, keys, values, table, _i32([0], q.device), D ** -0.5, q_start=qs, max_q=new, sinks=sinks)
+    assert torch.count_nonzero(none).item() == 0
