@@ -291,6 +291,15 @@ int lq_kv4_read(const uint32_t* kq, const void* ks, const void* kb, const uint32
  * the parts of split softmaxes, and, where max_q is large and width * page_size * B keys fit 1 GiB that way, the keys and
  * values of requests with many rows as fp16 tiles. */
 size_t lq_kv4_attend_workspace(int B, int max_q, int H, int KVH, int head_dim, int width, int page_size);
+
+/* The forms that a call of these sizes runs, ORed (0: refused). Few rows (mma.sync): a cluster of CTAs an item, or all keys
+ * split evenly over the CTAs. Many rows (tcgen05): codes unpacked tile by tile, or once, first. A batch with both kinds of
+ * requests runs one of each. */
+#define LQ_KV4_CLUSTERS 1
+#define LQ_KV4_SPLIT 2
+#define LQ_KV4_TILES 4
+#define LQ_KV4_DENSE 8
+int lq_kv4_attend_forms(int B, int max_q, int H, int KVH, int head_dim, int width, int page_size, int window);
 int lq_kv4_attend(const void* q, int N, const int32_t* q_start, int max_q, const uint32_t* kq, const void* ks,
                   const void* kb, const uint32_t* vq, const void* vs, const void* vb, int pages, int page_size,
                   const int32_t* table, int width, const int32_t* lens, int B, const float* sinks, float scale,

@@ -69,6 +69,7 @@ SIGNATURES = {
                        _u32p, _vp, _vp, _u32p, _vp, _vp, _i, _i, _i, _vp], _i),
     "lq_kv4_read": ([_u32p, _vp, _vp, _u32p, _vp, _vp, _i, _i, _i, _i, _vp, _i, _vp, _vp, _i, _vp], _i),
     "lq_kv4_attend_workspace": ([_i, _i, _i, _i, _i, _i, _i], ctypes.c_size_t),
+    "lq_kv4_attend_forms": ([_i, _i, _i, _i, _i, _i, _i, _i], _i),
     "lq_kv4_attend": ([_vp, _i, _vp, _i, _u32p, _vp, _vp, _u32p, _vp, _vp, _i, _i, _vp, _i, _vp, _i, _vp,
                        ctypes.c_float, _i, _i, _i, _i, _i, _vp, ctypes.c_size_t, _vp, _vp], _i),
     "lq_supported": ([_i, _i, _i, _i, _i, _i, _i], _i),

@@ -109,6 +109,7 @@ int kv4_read_run(const Kv4Pool& pool, int D, const int32_t* slots, int N, void* 
                  cudaStream_t st);
 bool kv4_attend_shape_ok(int N, int B, int max_q, int H, int KVH, int width, int window);
 size_t kv4_attend_workspace_bytes(int B, int max_q, int H, int KVH, int D, long long room);
+int kv4_attend_forms(int B, int max_q, int H, int KVH, int D, int width, int page, int window);
 int kv4_attend_run(const Kv4Pool& pool, const void* q, int N, const int32_t* q_start, int max_q, const int32_t* table,
                    int width, const int32_t* lens, int B, const float* sinks, float scale, int window, int H, int D,
                    int dtype, void* workspace, size_t workspace_bytes, void* out, cudaStream_t st);
@@ -761,6 +762,13 @@ size_t lq_kv4_attend_workspace(int B, int max_q, int H, int KVH, int head_dim, i
     if (KVH < 1 || page_size < 1 || !kv4_attend_shape_ok(0, B, max_q, H, KVH, width, 0)) return 0;
     if (check_device() != LQ_OK) return 0;
     return kv4_attend_workspace_bytes(B, max_q, H, KVH, head_dim, (long long)width * page_size);
+}
+
+int lq_kv4_attend_forms(int B, int max_q, int H, int KVH, int head_dim, int width, int page_size, int window) {
+    const Kv4Pool one = {nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, 1, KVH, page_size};
+    if (!kv4_pool_ok(one, head_dim) || !kv4_attend_shape_ok(0, B, max_q, H, KVH, width, window)) return 0;
+    if (check_device() != LQ_OK) return 0;
+    return kv4_attend_forms(B, max_q, H, KVH, head_dim, width, page_size, window);
 }
 
 int lq_kv4_attend(const void* q, int N, const int32_t* q_start, int max_q, const uint32_t* kq, const void* ks,

@@ -843,6 +843,7 @@ static size_t kv4_few_bytes(int D, int R, int sms) {
 }
 
 size_t kv4_prefill_workspace_bytes(int D, int sms, int B, int KVH, int G, int max_q, long long room);
+bool kv4_prefill_dense(int D, int B, int KVH, int G, int max_q, long long room);
 int kv4_prefill_run(const Kv4AttArgs& a, int D, int dtype, void* workspace, cudaStream_t st);
 
 size_t kv4_attend_workspace_bytes(int B, int max_q, int H, int KVH, int D, long long room) {
@@ -857,13 +858,23 @@ size_t kv4_attend_workspace_bytes(int B, int max_q, int H, int KVH, int D, long 
 // resident at once, if no request can have more than 8 steps a CTA. That spares the second launch and the scan of the
 // lengths: one request of 1,001 keys takes 8.5 us, 12.5 with the even split. Beyond, the split is worth more (items differ,
 // and steps go to every SM): 4 requests of 131,072 keys leave a cluster form 128 of 444 CTAs.
-static int kv4_cluster(const Kv4AttArgs& a, int D, int R, int sms) {
-    const long long items = (long long)a.B * a.pool.KVH * ((a.split_rows + R - 1) / R), room = (long long)a.width * a.pool.page;
-    const long long seen = a.window ? (room < (long long)a.window + a.max_q + KV4_STEP ? room : (long long)a.window + a.max_q + KV4_STEP) : room;
+static int kv4_cluster(int B, int KVH, int split_rows, int max_q, int window, long long room, int D, int R, int sms) {
+    const long long items = (long long)B * KVH * ((split_rows + R - 1) / R);
+    const long long seen = window ? (room < (long long)window + max_q + KV4_STEP ? room : (long long)window + max_q + KV4_STEP) : room;
     const long long steps = (seen + KV4_STEP - 1) / KV4_STEP;
     int C = 8;
     while (C > 1 && (items * C > kv4_ctas(D, R, sms) || C / 2 >= steps)) C /= 2;
     return items * C <= kv4_ctas(D, R, sms) && steps <= 8 * C ? C : 0;
+}
+
+int kv4_attend_forms(int B, int max_q, int H, int KVH, int D, int width, int page, int window) {
+    const int G = H / KVH;
+    const long long room = (long long)width * page;
+    int R, split, forms = 0;
+    kv4_rows(max_q, G, D, B, KVH, room, &R, &split);
+    if (split) forms |= kv4_cluster(B, KVH, split, max_q, window, room, D, R, device_info().sm_count) ? LQ_KV4_CLUSTERS : LQ_KV4_SPLIT;
+    if ((long long)max_q * G > split) forms |= kv4_prefill_dense(D, B, KVH, G, max_q, room) ? LQ_KV4_DENSE : LQ_KV4_TILES;
+    return forms;
 }
 
 template <typename T, int D, int NT>
@@ -872,7 +883,8 @@ static int kv4_attend_n(Kv4AttArgs a, cudaStream_t st) {
     constexpr size_t merge = size_t(KV4_NW + 1) * R * (2 + D) * sizeof(float);
     constexpr size_t smem = merge > size_t(Kv4Shape<D>::RING) ? merge : size_t(Kv4Shape<D>::RING);
     static std::atomic<uint32_t> set{0}, set_cl{0}, none{0};
-    const int sms = device_info().sm_count, C = kv4_cluster(a, D, R, sms), n = kv4_ctas(D, R, sms);
+    const int sms = device_info().sm_count, n = kv4_ctas(D, R, sms);
+    const int C = kv4_cluster(a.B, a.pool.KVH, a.split_rows, a.max_q, a.window, (long long)a.width * a.pool.page, D, R, sms);
     if (C)
         return kv4_launch(kv4_attend_kernel<T, D, NT, true>, set_cl, dim3(a.B * a.pool.KVH * ((a.split_rows + R - 1) / R) * C), dim3(KV4_NW * 32), smem, st, a, C);
     int rc = kv4_launch(kv4_attend_kernel<T, D, NT, false>, set, dim3(n), dim3(KV4_NW * 32), smem, st, a);

@@ -1123,6 +1123,12 @@ static bool pf_dense(int D, int B, int KVH, int G, int max_q, long long room, si
     return (long long)max_q * G > 2 * R && tiles <= (1LL << 30) / (4LL * KT * D) && B <= 65535 && KVH <= 65535;
 }
 
+bool kv4_prefill_dense(int D, int B, int KVH, int G, int max_q, long long room) {
+    size_t bytes;
+    int steps;
+    return pf_dense(D, B, KVH, G, max_q, room, &bytes, &steps);
+}
+
 static size_t pf_parts_bytes(int D, int sms) {
     const int R = D == 256 ? 128 : 256;
     return (size_t(sms) * 2 * R * (2 + D) * sizeof(float) + size_t(sms) * 8 * sizeof(int32_t) + 127) / 128 * 128;
