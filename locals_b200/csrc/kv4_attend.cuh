@@ -30,7 +30,7 @@ struct Kv4AttArgs {
     float* part_o;     // (CTA, 2, rows) x D
     int32_t* records;  // (CTA) x 8: the item that the start of a CTA's share divides
     uint8_t* dense;    // (request, kv head, dense_steps) x {keys, values} of a step as fp16 tiles (kv4_prefill's dense form)
-    int2* dense_meta;  // their values' power of two, and the runs of 8 keys without a page
+    int2* dense_meta;  // their keys' and values' powers of two, and the runs of 8 keys without a page
     int dense_steps;
     float scale_log2;
     int N, B, H, G, width, window, max_q;

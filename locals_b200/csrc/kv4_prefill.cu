@@ -4,7 +4,7 @@
 // A CTA takes a tile of 256 rows of a (request, kv head) (128 at D = 256) and walks its keys in steps of 128 (64 at
 // D = 256). Per step
 //   * the codes of its keys and values become fp16 tiles in shared memory, (code | 1024) - 1024 and one fused multiply-add
-//     with the group's scale and bias, pairs (i, i + 4) of a word as they come out of one mask. The order of dimensions that
+//     with the group's scale and bias (times a power of two), pairs (i, i + 4) of a word as they come out of one mask. The order of dimensions that
 //     this makes is met by the queries (stored in the same order) and undone when the output is written;
 //   * one thread issues S = Q K^T (both in shared memory, K-major) and O += P V (P in tensor memory, V in shared memory as
 //     it lies, dimensions contiguous: the transposed B operand) as tcgen05.mma with fp32 accumulators in tensor memory:
@@ -21,8 +21,10 @@
 // Roundings to fp16: queries after a power of two a row (exact for bf16 but for values 2^-26 below the row's largest); keys,
 // values and probabilities, 2^-11 each against the 2^-8 of a bf16 output (an fp16 output's error against 64 bits grows by
 // them from 2.1e-4 to 3.2e-4 .. 4.0e-4 of its size: the tensor cores take the operands in no finer type but at half the
-// rate); values after a power of two that follows their size, so that neither small nor large ones leave fp16's range. Keys
-// beyond 65,504 are beyond what this form holds and come out as infinities.
+// rate). Keys after a power of two a step that puts the largest that its groups can hold at 2^13 .. 2^14, taken back with the
+// scores' factor: a group's scale and a sixteenth of it stay normal numbers down to 2^-19 of that, where the group's share of
+// a score is as small. Values after a power of two that follows their size, so that neither small nor large ones leave
+// fp16's range.
 // A masked score is -inf, its probability 0; a value whose scale or bias is not finite is held as 0 and its key as NaN,
 // so that only rows that see it become NaN.
 // Work is dealt out as in kv4_attend.cu: the steps of all tiles (each as far as its last row sees) evenly over one CTA a
@@ -269,14 +271,15 @@ __device__ __forceinline__ uint32_t pf_affine(uint32_t v, uint32_t s2, uint32_t 
 struct PfBars {
     uint64_t q_full[2], k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], o_done[2], r_full[4], r_empty[4], done;
     int abort;          // a wait gave up: no one waits any more
-    int v_exp[4];       // power of two of the values of step i & 3
+    int exps[4];        // powers of two of the keys and values of step i & 3 (pf_exps)
     uint32_t miss[4];   // its runs of 8 keys without a page
     // what the page warp tells the unpacking warps of step i & 3: the pool row of each run of 8 keys (none: KV4_NONE), the
     // keys from its first to the tile's end (0: no more steps), whether an item starts, and the runs without a page
     uint32_t run[4][16];
     int left[4], start[4];
     uint32_t gone[4];
-    float v_max[2][PF_UNPACK];  // of step i & 1: each unpacking warp's largest |value|, negative from one that has no step
+    float k_max[2][PF_UNPACK], v_max[2][PF_UNPACK];  // of step i & 1: what each unpacking warp's groups can hold at most
+                                                     // (values: negative from a warp that has no step)
     int rows, steps;    // the item's (0: no more), from the first softmax warp to the issuing thread
 };
 
@@ -323,31 +326,40 @@ __device__ __forceinline__ void pf_unpack(const uint4& codes, float s, float b, 
 }
 
 // A piece's scales and biases in fp32. A value scale or bias that is not finite makes the values 0 and the key NaN, which
-// only the rows that see it meet. Returns the largest |value| that the group can hold.
+// only the rows that see it meet; so does an infinite key. Adds the largest |key| and |value| that the groups can hold.
 template <typename T>
-__device__ __forceinline__ float pf_scales(uint16_t ks16, uint16_t kb16, uint16_t vs16, uint16_t vb16, float* ks, float* kb,
-                                           float* vs, float* vb) {
+__device__ __forceinline__ void pf_scales(uint16_t ks16, uint16_t kb16, uint16_t vs16, uint16_t vb16, float* ks, float* kb,
+                                          float* vs, float* vb, float* k_top, float* v_top) {
     *ks = F16Traits<T>::to_f32(ks16), *kb = F16Traits<T>::to_f32(kb16);
     *vs = F16Traits<T>::to_f32(vs16), *vb = F16Traits<T>::to_f32(vb16);
-    const float most = fmaf(15.0f, fabsf(*vs), fabsf(*vb));
-    if (most < INFINITY) return most;
-    *vs = *vb = 0.0f;
-    *ks = *kb = __int_as_float(0x7fffffff);
-    return 0.0f;
+    const float k_most = fmaf(15.0f, fabsf(*ks), fabsf(*kb)), v_most = fmaf(15.0f, fabsf(*vs), fabsf(*vb));
+    if (!(v_most < INFINITY)) {
+        *vs = *vb = 0.0f;
+        *ks = *kb = __int_as_float(0x7fffffff);
+        return;
+    }
+    *v_top = fmaxf(*v_top, v_most);
+    if (k_most < INFINITY) *k_top = fmaxf(*k_top, k_most);
 }
+// 2^e, e in -126 .. 127.
+__device__ __forceinline__ float pf_pow2(int e) { return __uint_as_float(uint32_t(127 + e) << 23); }
+// The power of two that puts M at 2^13 .. 2^14 (at least -114; 0 for 0).
+__device__ __forceinline__ int pf_fit(float M) { return M > 0.0f ? min(13 - (int(__float_as_uint(M) >> 23) - 127), 120) : 0; }
+// The powers of two of a step's keys and values in one word.
+__device__ __forceinline__ int pf_exps(int ke, int ve) { return int(uint32_t(ke) << 16 | (uint32_t(ve) & 0xffffu)); }
 // The power of two that puts M at 2^10 .. 2^11 (M below 2^128: at least -117).
 __device__ __forceinline__ int pf_exponent(float M) { return min(10 - (int(__float_as_uint(M) >> 23) - 127), 100); }
 
 // ---- the dense form's first pass: the keys and values of requests with many tiles, unpacked once ----
 // One CTA a (step of KT keys, kv head, request): the step's two tiles as they are to lie in shared memory, copied out whole,
-// and its values' power of two (0 wherever they lie within fp16's comfort) and missing pages.
+// and its keys' and values' powers of two (the values' 0 wherever they lie within fp16's comfort) and missing pages.
 constexpr int PD_WARPS = 8;
 template <typename T, int D>
 __global__ void __launch_bounds__(PD_WARPS * 32) kv4_dense_kernel(const Kv4AttArgs a) {
     using S = PfShape<D>;
     using P = PfPieces<D, PD_WARPS>;
     extern __shared__ __align__(1024) uint8_t pf_raw[];
-    __shared__ float part[PD_WARPS];
+    __shared__ float part[PD_WARPS], k_part[PD_WARPS];
     grid_dep_wait();
     const int s = blockIdx.x, kvh = blockIdx.y, b = blockIdx.z;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -373,7 +385,7 @@ __global__ void __launch_bounds__(PD_WARPS * 32) kv4_dense_kernel(const Kv4AttAr
     }
     const uint32_t miss = __ballot_sync(0xffffffffu, lane < RUNS && gone);
     uint4 kc[P::J], vc[P::J];
-    float ks[P::J], kb[P::J], vs[P::J], vb[P::J], top = 0.0f;
+    float ks[P::J], kb[P::J], vs[P::J], vb[P::J], k_top = 0.0f, top = 0.0f;
     uint16_t sc[P::J][4];
 #pragma unroll
     for (int j = 0; j < P::J; ++j) {
@@ -390,25 +402,28 @@ __global__ void __launch_bounds__(PD_WARPS * 32) kv4_dense_kernel(const Kv4AttAr
     }
 #pragma unroll
     for (int j = 0; j < P::J; ++j)
-        top = fmaxf(top, pf_scales<T>(sc[j][0], sc[j][1], sc[j][2], sc[j][3], &ks[j], &kb[j], &vs[j], &vb[j]));
+        pf_scales<T>(sc[j][0], sc[j][1], sc[j][2], sc[j][3], &ks[j], &kb[j], &vs[j], &vb[j], &k_top, &top);
     top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top)));
-    if (lane == 0) part[warp] = top;
+    k_top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(k_top)));
+    if (lane == 0) part[warp] = top, k_part[warp] = k_top;
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < PD_WARPS; ++i) top = fmaxf(top, part[i]);
+    for (int i = 0; i < PD_WARPS; ++i) top = fmaxf(top, part[i]), k_top = fmaxf(k_top, k_part[i]);
+    const int ke = pf_fit(k_top);
+    const float kf = pf_pow2(ke);
     const int ve = top == 0.0f || (top >= 0.015625f && top < 16384.0f) ? 0 : pf_exponent(top);
     const float vf = exp2f(float(ve));
 #pragma unroll
     for (int j = 0; j < P::J; ++j) {
         const int k = P::key(j, warp, lane), p = P::piece(j, warp, lane);
-        pf_unpack<D>(kc[j], ks[j], kb[j], tile, k, p);
+        pf_unpack<D>(kc[j], ks[j] * kf, kb[j] * kf, tile, k, p);
         pf_unpack<D>(vc[j], vs[j] * vf, vb[j] * vf, tile + S::TB, k, p);
     }
     fence_proxy_async();
     __syncthreads();
     if (threadIdx.x == 0) {
         const size_t at = ((size_t)b * a.pool.KVH + kvh) * a.dense_steps + s;
-        a.dense_meta[at] = make_int2(ve, int(miss));
+        a.dense_meta[at] = make_int2(pf_exps(ke, ve), int(miss));
         asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(a.dense + at * (2 * S::TB)), "r"(tile),
                      "r"(2 * S::TB)
                      : "memory");
@@ -647,7 +662,9 @@ __global__ void __launch_bounds__(pf_threads(DENSE), 1) kv4_prefill_kernel(const
                 tc_fence_after();
                 const int key0 = (walk.lo + walk.st0 + t) * KT;
                 const uint32_t miss = *reinterpret_cast<volatile uint32_t*>(&bar.miss[it & 3]);
-                const int ve_t = *reinterpret_cast<volatile int*>(&bar.v_exp[it & 3]);
+                const int exps = *reinterpret_cast<volatile int*>(&bar.exps[it & 3]), ve_t = int16_t(exps);
+                // the scores' factor (a positive number, so that a masked score stays -inf)
+                const float ct = fminf(fmaxf(c * pf_pow2(-(exps >> 16)), 1.17549435e-38f), 3.4028234e38f);
                 const bool all = key0 >= lo_all && key0 + KT <= hi_all && miss == 0;
                 const uint32_t s_col = tmem + lanes + buf * KT;
                 // what this row sees of 32 of the step's keys, a bit a key
@@ -672,7 +689,7 @@ __global__ void __launch_bounds__(pf_threads(DENSE), 1) kv4_prefill_kernel(const
                 // The common case, one pass: the reference from the steps before serves the step (found out at its end: the
                 // probabilities stay in registers until then, the scores in place).
                 auto once = [&](auto masked) -> bool {
-                    const uint64_t c2 = pf_pair(c, c), m2 = pf_pair(-m, -m);
+                    const uint64_t c2 = pf_pair(ct, ct), m2 = pf_pair(-m, -m);
                     constexpr int CH = 16;  // scores at a time (32: 1082 against 1040 us for a 4096-token prompt piece)
                     uint32_t r[2][CH], p[KT / 2];
                     uint64_t sums[2] = {0, 0};
@@ -700,7 +717,7 @@ __global__ void __launch_bounds__(pf_threads(DENSE), 1) kv4_prefill_kernel(const
                             p[(ch * CH + i) / 2] = h;
                         }
                     }
-                    if (__any_sync(0xffffffffu, fmaxf(mx[0], mx[1]) * c > m + 8.0f)) return false;
+                    if (__any_sync(0xffffffffu, fmaxf(mx[0], mx[1]) * ct > m + 8.0f)) return false;
 #pragma unroll
                     for (int ch = 0; ch < KT / 64; ++ch) pf_tmem_st32(s_col + ch * 32, &p[ch * 32]);
                     float a0, a1, b0, b1;
@@ -730,7 +747,7 @@ __global__ void __launch_bounds__(pf_threads(DENSE), 1) kv4_prefill_kernel(const
                     for (int i = 0; i < 32; i += 2) part[(i >> 1) & 1] = fmaxf(fmaxf(part[(i >> 1) & 1], seen(r[i], v, i)), seen(r[i + 1], v, i + 1));
                     mx = fmaxf(mx, fmaxf(part[0], part[1]));
                 }
-                const float mn = fmaxf(m, mx * c);
+                const float mn = fmaxf(m, mx * ct);
                 const bool grow = mn > m + 8.0f || (m == -INFINITY && mn > m) || ve_t != ve;
                 if (__any_sync(0xffffffffu, grow)) {
                     const float corr = t == 0 ? 0.0f : (mn > m ? kv4_ex2(m - mn) : 1.0f) * exp2f(float(ve_t - ve));
@@ -761,8 +778,8 @@ __global__ void __launch_bounds__(pf_threads(DENSE), 1) kv4_prefill_kernel(const
                     tmem_wait_ld();
 #pragma unroll
                     for (int i = 0; i < 16; i += 2) {
-                        float e0 = kv4_ex2(fmaf(seen(x[i], v, i), c, -mz));
-                        float e1 = kv4_ex2(fmaf(seen(x[i + 1], v, i + 1), c, -mz));
+                        float e0 = kv4_ex2(fmaf(seen(x[i], v, i), ct, -mz));
+                        float e1 = kv4_ex2(fmaf(seen(x[i + 1], v, i + 1), ct, -mz));
                         p[i / 2] = cvt_f16x2(e1, e0);
                         pf_summand<T>(p[i / 2], &e0, &e1);
                         sum[i & 2] += e0;
@@ -871,14 +888,15 @@ __global__ void __launch_bounds__(pf_threads(DENSE), 1) kv4_prefill_kernel(const
         auto step_out = [&](const Held& h, int it, bool have) -> bool {
             const int st = it & 1;
             const uint32_t par = ((it >> 1) & 1) ^ 1;
-            float top = 0.0f, ks[J], kb[J], vs[J], vb[J];
+            float k_top = 0.0f, top = 0.0f, ks[J], kb[J], vs[J], vb[J];
             if (have) {
 #pragma unroll
                 for (int j = 0; j < J; ++j)
-                    top = fmaxf(top, pf_scales<T>(h.ks[j], h.kb[j], h.vs[j], h.vb[j], &ks[j], &kb[j], &vs[j], &vb[j]));
+                    pf_scales<T>(h.ks[j], h.kb[j], h.vs[j], h.vb[j], &ks[j], &kb[j], &vs[j], &vb[j], &k_top, &top);
             }
             top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top)));
-            if (lane == 0) bar.v_max[st][uw] = have ? top : -1.0f;
+            k_top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(k_top)));
+            if (lane == 0) bar.v_max[st][uw] = have ? top : -1.0f, bar.k_max[st][uw] = k_top;
             named_barrier(1, PF_UNPACK * 32);  // (a slot is written again after the next step's barrier, which its readers pass later)
             float M = 0.0f;
             bool over = false;
@@ -886,9 +904,12 @@ __global__ void __launch_bounds__(pf_threads(DENSE), 1) kv4_prefill_kernel(const
             for (int i = 0; i < PF_UNPACK; ++i) {
                 const float x = reinterpret_cast<volatile float*>(bar.v_max[st])[i];
                 M = fmaxf(M, x);
+                k_top = fmaxf(k_top, reinterpret_cast<volatile float*>(bar.k_max[st])[i]);
                 over = over || x < 0.0f;
             }
             if (over) return false;
+            const int ke = pf_fit(k_top);
+            const float kf = pf_pow2(ke);
             if (*reinterpret_cast<volatile int*>(&bar.start[it & 3])) limit = 0.0f, ve = 0;
             // the values' power of two: the largest |value| a group can hold at 2^10 .. 2^15
             if (M > limit) {
@@ -897,14 +918,14 @@ __global__ void __launch_bounds__(pf_threads(DENSE), 1) kv4_prefill_kernel(const
             }
             const float vf = exp2f(float(ve));
             if (uw == 0 && lane == 0) {
-                bar.v_exp[it & 3] = ve;
+                bar.exps[it & 3] = pf_exps(ke, ve);
                 bar.miss[it & 3] = bar.gone[it & 3];
             }
             __syncwarp();
             if (lane == 0) mbar_arrive(&bar.r_empty[it & 3]);
             pf_wait(&bar.k_empty[st], par, abort);
 #pragma unroll
-            for (int j = 0; j < J; ++j) pf_unpack<D>(h.k[j], ks[j], kb[j], sk + st * S::TB, P::key(j, uw, lane), P::piece(j, uw, lane));
+            for (int j = 0; j < J; ++j) pf_unpack<D>(h.k[j], ks[j] * kf, kb[j] * kf, sk + st * S::TB, P::key(j, uw, lane), P::piece(j, uw, lane));
             fence_proxy_async();
             __syncwarp();
             if (lane == 0) mbar_arrive(&bar.k_full[st]);
@@ -952,7 +973,7 @@ __global__ void __launch_bounds__(pf_threads(DENSE), 1) kv4_prefill_kernel(const
                     const uint8_t* src = a.dense + (tile0 + t) * (2 * S::TB);
                     pf_wait(&bar.k_empty[st], par, abort);
                     if (*abort) break;
-                    bar.v_exp[it & 3] = meta.x;
+                    bar.exps[it & 3] = meta.x;
                     bar.miss[it & 3] = uint32_t(meta.y);
                     copy(&bar.k_full[st], sk + st * S::TB, src);
                     ++keys;

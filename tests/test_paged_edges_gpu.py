@@ -213,3 +213,21 @@ def test_attend_a_sink_that_is_not_a_number(cuda, new, H, KVH, D, columns):
     assert torch.equal(again[:, others], got[:, others])
     none = paged.attend(q, keys, values, table, _i32([0], q.device), D ** -0.5, q_start=qs, max_q=new, sinks=sinks)
     assert torch.count_nonzero(none).item() == 0
+
+
+@pytest.mark.parametrize("new,H,KVH,D,columns", FORMS)
+def test_attend_keys_of_any_size(cuda, new, H, KVH, D, columns):
+    """Keys of 2^-60 to 2^20 of the usual size met by queries of the inverse size; and one group of 64 dimensions of the keys
+    2^-16 of the others, its queries 2^16 of theirs: all scores as they were."""
+    import torch
+
+    q, keys, values, table, lens, qs = _case(cuda, new, H, KVH, D, columns, 23)
+    for e in (-8, -12, -16, -60, 14, 20):
+        small = (keys[0], keys[1] * 2.0 ** e, keys[2] * 2.0 ** e)
+        _held(q * 2.0 ** -e, small, values, table, lens, D ** -0.5, qs)
+    if D > 64:
+        s, b, x = keys[1].clone(), keys[2].clone(), q.clone()
+        s[..., 1] *= 2.0 ** -16
+        b[..., 1] *= 2.0 ** -16
+        x[..., 64:128] *= 2.0 ** 16
+        _held(x, (keys[0], s, b), values, table, lens, D ** -0.5, qs)
