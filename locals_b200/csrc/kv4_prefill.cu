@@ -23,8 +23,10 @@
 // them from 2.1e-4 to 3.2e-4 .. 4.0e-4 of its size: the tensor cores take the operands in no finer type but at half the
 // rate). Keys after a power of two a step that puts the largest that its groups can hold at 2^13 .. 2^14, taken back with the
 // scores' factor: a group's scale and a sixteenth of it stay normal numbers down to 2^-19 of that, where the group's share of
-// a score is as small. Values after a power of two that follows their size, so that neither small nor large ones leave
-// fp16's range.
+// a score is as small. Values after a power of two a step in the same way; a row's outputs have one of their own, and its
+// probabilities are multiplied by the difference while that is small, its outputs (as its maximum's growth does) where it
+// is not: so a step's values cost another step's no bits, and a row only those of the keys that it sees. Within a step,
+// values are held to 2^-35 of the largest.
 // A masked score is -inf, its probability 0; a value whose scale or bias is not finite is held as 0 and its key as NaN,
 // so that only rows that see it become NaN.
 // Work is dealt out as in kv4_attend.cu: the steps of all tiles (each as far as its last row sees) evenly over one CTA a
@@ -274,9 +276,9 @@ struct PfBars {
     int exps[4];        // powers of two of the keys and values of step i & 3 (pf_exps)
     uint32_t miss[4];   // its runs of 8 keys without a page
     // what the page warp tells the unpacking warps of step i & 3: the pool row of each run of 8 keys (none: KV4_NONE), the
-    // keys from its first to the tile's end (0: no more steps), whether an item starts, and the runs without a page
+    // keys from its first to the tile's end (0: no more steps), and the runs without a page
     uint32_t run[4][16];
-    int left[4], start[4];
+    int left[4];
     uint32_t gone[4];
     float k_max[2][PF_UNPACK], v_max[2][PF_UNPACK];  // of step i & 1: what each unpacking warp's groups can hold at most
                                                      // (values: negative from a warp that has no step)
@@ -347,12 +349,15 @@ __device__ __forceinline__ float pf_pow2(int e) { return __uint_as_float(uint32_
 __device__ __forceinline__ int pf_fit(float M) { return M > 0.0f ? min(13 - (int(__float_as_uint(M) >> 23) - 127), 120) : 0; }
 // The powers of two of a step's keys and values in one word.
 __device__ __forceinline__ int pf_exps(int ke, int ve) { return int(uint32_t(ke) << 16 | (uint32_t(ve) & 0xffffu)); }
-// The power of two that puts M at 2^10 .. 2^11 (M below 2^128: at least -117).
-__device__ __forceinline__ int pf_exponent(float M) { return min(10 - (int(__float_as_uint(M) >> 23) - 127), 100); }
+// The values' of a step that holds none but zeros: any.
+constexpr int PF_ANY = 127;
+// How far a row's outputs may lie from a step's values before they are multiplied: probabilities, at most 2^8, times 2^6 are
+// within fp16; times 2^-4, those below 2^-10 begin to lose bits, of values that are 2^-4 as large.
+constexpr int PF_UP = 6, PF_DOWN = -4;
 
 // ---- the dense form's first pass: the keys and values of requests with many tiles, unpacked once ----
 // One CTA a (step of KT keys, kv head, request): the step's two tiles as they are to lie in shared memory, copied out whole,
-// and its keys' and values' powers of two (the values' 0 wherever they lie within fp16's comfort) and missing pages.
+// and its keys' and values' powers of two and missing pages.
 constexpr int PD_WARPS = 8;
 template <typename T, int D>
 __global__ void __launch_bounds__(PD_WARPS * 32) kv4_dense_kernel(const Kv4AttArgs a) {
@@ -411,8 +416,8 @@ __global__ void __launch_bounds__(PD_WARPS * 32) kv4_dense_kernel(const Kv4AttAr
     for (int i = 0; i < PD_WARPS; ++i) top = fmaxf(top, part[i]), k_top = fmaxf(k_top, k_part[i]);
     const int ke = pf_fit(k_top);
     const float kf = pf_pow2(ke);
-    const int ve = top == 0.0f || (top >= 0.015625f && top < 16384.0f) ? 0 : pf_exponent(top);
-    const float vf = exp2f(float(ve));
+    const int ve = pf_fit(top);
+    const float vf = pf_pow2(ve);
 #pragma unroll
     for (int j = 0; j < P::J; ++j) {
         const int k = P::key(j, warp, lane), p = P::piece(j, warp, lane);
@@ -423,7 +428,7 @@ __global__ void __launch_bounds__(PD_WARPS * 32) kv4_dense_kernel(const Kv4AttAr
     __syncthreads();
     if (threadIdx.x == 0) {
         const size_t at = ((size_t)b * a.pool.KVH + kvh) * a.dense_steps + s;
-        a.dense_meta[at] = make_int2(pf_exps(ke, ve), int(miss));
+        a.dense_meta[at] = make_int2(pf_exps(ke, top > 0.0f ? ve : PF_ANY), int(miss));
         asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(a.dense + at * (2 * S::TB)), "r"(tile),
                      "r"(2 * S::TB)
                      : "memory");
@@ -653,7 +658,7 @@ __global__ void __launch_bounds__(pf_threads(DENSE), 1) kv4_prefill_kernel(const
             if (lane == 0) mbar_arrive(&bar.q_full[w]);
 
             float m = -INFINITY, l = 0.0f;
-            int ve = 0;
+            int ve = 0, ve_low = 1000;  // the row's outputs' power of two; the least of the steps' that it was fitted to
             const uint32_t o_col = tmem + lanes + S::O_COL + w * D;
             for (int t = 0; t < steps; ++t, ++it, ++used) {
                 const int buf = NQ == 2 ? w : used & 1;
@@ -662,9 +667,15 @@ __global__ void __launch_bounds__(pf_threads(DENSE), 1) kv4_prefill_kernel(const
                 tc_fence_after();
                 const int key0 = (walk.lo + walk.st0 + t) * KT;
                 const uint32_t miss = *reinterpret_cast<volatile uint32_t*>(&bar.miss[it & 3]);
-                const int exps = *reinterpret_cast<volatile int*>(&bar.exps[it & 3]), ve_t = int16_t(exps);
-                // the scores' factor (a positive number, so that a masked score stays -inf)
-                const float ct = fminf(fmaxf(c * pf_pow2(-(exps >> 16)), 1.17549435e-38f), 3.4028234e38f);
+                // The scores' factor (a positive number, so that a masked score stays -inf), and how far the row's outputs lie from
+                // the step's values: its probabilities are multiplied by 2^that. (Read where they are used: the one pass needs the
+                // registers.)
+                auto exps = [&]() { return *reinterpret_cast<volatile int*>(&bar.exps[it & 3]); };
+                auto factor = [&]() { return fminf(fmaxf(c * pf_pow2(-(exps() >> 16)), 1.17549435e-38f), 3.4028234e38f); };
+                auto apart = [&]() -> int {
+                    const int ve_t = int16_t(exps());
+                    return ve_t == PF_ANY ? 0 : ve - ve_t;
+                };
                 const bool all = key0 >= lo_all && key0 + KT <= hi_all && miss == 0;
                 const uint32_t s_col = tmem + lanes + buf * KT;
                 // what this row sees of 32 of the step's keys, a bit a key
@@ -689,7 +700,8 @@ __global__ void __launch_bounds__(pf_threads(DENSE), 1) kv4_prefill_kernel(const
                 // The common case, one pass: the reference from the steps before serves the step (found out at its end: the
                 // probabilities stay in registers until then, the scores in place).
                 auto once = [&](auto masked) -> bool {
-                    const uint64_t c2 = pf_pair(ct, ct), m2 = pf_pair(-m, -m);
+                    const float ct = factor(), md = float(apart()) - m;
+                    const uint64_t c2 = pf_pair(ct, ct), m2 = pf_pair(md, md);
                     constexpr int CH = 16;  // scores at a time (32: 1082 against 1040 us for a 4096-token prompt piece)
                     uint32_t r[2][CH], p[KT / 2];
                     uint64_t sums[2] = {0, 0};
@@ -723,7 +735,7 @@ __global__ void __launch_bounds__(pf_threads(DENSE), 1) kv4_prefill_kernel(const
                     float a0, a1, b0, b1;
                     pf_unpair(sums[0], &a0, &a1);
                     pf_unpair(sums[1], &b0, &b1);
-                    l += (a0 + a1) + (b0 + b1);
+                    l = fmaf((a0 + a1) + (b0 + b1), pf_pow2(-apart()), l);
                     tmem_wait_st();
                     tc_fence_before();
                     __syncwarp();
@@ -731,10 +743,12 @@ __global__ void __launch_bounds__(pf_threads(DENSE), 1) kv4_prefill_kernel(const
                     if (lane == 0) mbar_arrive(&bar.p_full[buf]);
                     return true;
                 };
-                if (ve_t == ve && __all_sync(0xffffffffu, m != -INFINITY)) {
+                if (__all_sync(0xffffffffu, m != -INFINITY && unsigned(apart() - PF_DOWN) <= unsigned(PF_UP - PF_DOWN))) {
                     if (all ? once(std::false_type()) : once(std::true_type())) continue;
                 }
                 // A new reference (an item's first step, mostly): two passes, in loops, since their code is not often in reach.
+                const float ct = factor();
+                int d = apart();
                 float mx = -INFINITY;
 #pragma unroll 1
                 for (int ch = 0; ch < KT / 32; ++ch) {
@@ -748,12 +762,19 @@ __global__ void __launch_bounds__(pf_threads(DENSE), 1) kv4_prefill_kernel(const
                     mx = fmaxf(mx, fmaxf(part[0], part[1]));
                 }
                 const float mn = fmaxf(m, mx * ct);
-                const bool grow = mn > m + 8.0f || (m == -INFINITY && mn > m) || ve_t != ve;
+                const bool some = mx != -INFINITY;
+                const bool grow = mn > m + 8.0f || (m == -INFINITY && mn > m) || (some && (d < PF_DOWN || d > PF_UP));
                 if (__any_sync(0xffffffffu, grow)) {
-                    const float corr = t == 0 ? 0.0f : (mn > m ? kv4_ex2(m - mn) : 1.0f) * exp2f(float(ve_t - ve));
-                    l *= mn > m ? kv4_ex2(m - mn) : 1.0f;
+                    // The outputs' new power of two: the step's, but no more than 2^64 above the least of the steps' before, whose
+                    // sums (below 2^43) then stay within 32 bits' range.
+                    int to = ve;
+                    if (some) ve_low = min(ve_low, ve - d), to = min(ve - d, ve_low + 64);
+                    const float decay = mn > m ? kv4_ex2(m - mn) : 1.0f;
+                    const float corr = t == 0 || m == -INFINITY ? 0.0f : decay * pf_pow2(max(to - ve, -126));
+                    l *= decay;
                     m = mn;
-                    ve = ve_t;
+                    d += to - ve;
+                    ve = to;
                     if (t > 0) {
                         pf_wait(&bar.o_done[w], (used - 1) & 1, abort);  // the last product is in
                         tc_fence_after();
@@ -768,7 +789,10 @@ __global__ void __launch_bounds__(pf_threads(DENSE), 1) kv4_prefill_kernel(const
                         }
                     }
                 }
-                const float mz = m == -INFINITY ? 0.0f : m;
+                // (d is below PF_DOWN only after so large values that this step's are nothing beside them: their probabilities are 0
+                // in fp16, and still in the row's sum; and beyond PF_UP only in rows that see nothing of the step)
+                const int dd = min(max(d, -60), 60);
+                const float mz = (m == -INFINITY ? 0.0f : m) - float(dd);
                 float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll 1
                 for (int ch = 0; ch < KT / 16; ++ch) {
@@ -787,7 +811,7 @@ __global__ void __launch_bounds__(pf_threads(DENSE), 1) kv4_prefill_kernel(const
                     }
                     pf_tmem_st8(s_col + ch * 8, p);
                 }
-                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                l = fmaf((sum[0] + sum[1]) + (sum[2] + sum[3]), pf_pow2(-dd), l);
                 tmem_wait_st();
                 tc_fence_before();
                 __syncwarp();
@@ -799,7 +823,7 @@ __global__ void __launch_bounds__(pf_threads(DENSE), 1) kv4_prefill_kernel(const
             tc_fence_after();
             const bool whole = walk.st0 == 0 && walk.st1 == walk.hi - walk.lo;
             const size_t part = ((size_t)blockIdx.x * 2 + (walk.st0 == 0 ? 1 : 0)) * R + row;
-            const float back = exp2f(float(-ve));
+            const float back = pf_pow2(-ve);
             float f = back;
             if (whole) {
                 const float sink = kv4_sink(a.sinks, head), M = fmaxf(m, sink);
@@ -881,8 +905,6 @@ __global__ void __launch_bounds__(pf_threads(DENSE), 1) kv4_prefill_kernel(const
             }
             return true;
         };
-        float limit = 0.0f;
-        int ve = 0;
         // one step from its registers to the tiles; false, in all warps at the same step, once one of them has none (at the
         // end, or after an error, which they need not see at the same step)
         auto step_out = [&](const Held& h, int it, bool have) -> bool {
@@ -910,15 +932,10 @@ __global__ void __launch_bounds__(pf_threads(DENSE), 1) kv4_prefill_kernel(const
             if (over) return false;
             const int ke = pf_fit(k_top);
             const float kf = pf_pow2(ke);
-            if (*reinterpret_cast<volatile int*>(&bar.start[it & 3])) limit = 0.0f, ve = 0;
-            // the values' power of two: the largest |value| a group can hold at 2^10 .. 2^15
-            if (M > limit) {
-                ve = pf_exponent(M);
-                limit = exp2f(float(15 - ve));
-            }
-            const float vf = exp2f(float(ve));
+            const int ve = pf_fit(M);
+            const float vf = pf_pow2(ve);
             if (uw == 0 && lane == 0) {
-                bar.exps[it & 3] = pf_exps(ke, ve);
+                bar.exps[it & 3] = pf_exps(ke, M > 0.0f ? ve : PF_ANY);
                 bar.miss[it & 3] = bar.gone[it & 3];
             }
             __syncwarp();
@@ -1018,7 +1035,6 @@ __global__ void __launch_bounds__(pf_threads(DENSE), 1) kv4_prefill_kernel(const
                 if (lane < RUNS) bar.run[slot][lane] = row;
                 if (lane == 0) {
                     bar.left[slot] = max(key_end - key0, 1);  // (a step that sees no key has no runs either)
-                    bar.start[slot] = t == walk.st0;
                     bar.gone[slot] = all_gone;
                 }
                 __syncwarp();

@@ -231,3 +231,34 @@ def test_attend_keys_of_any_size(cuda, new, H, KVH, D, columns):
         b[..., 1] *= 2.0 ** -16
         x[..., 64:128] *= 2.0 ** 16
         _held(x, (keys[0], s, b), values, table, lens, D ** -0.5, qs)
+
+
+@pytest.mark.parametrize("new,H,KVH,D,columns", FORMS)
+def test_attend_value_groups_of_any_size(cuda, new, H, KVH, D, columns):
+    """A group of 64 dimensions of the values 2^-6 to 2^-14 of the others: its outputs are held to their own size."""
+    import torch
+
+    if D == 64:
+        pytest.skip("one group a head")
+    q, keys, values, table, lens, qs = _case(cuda, new, H, KVH, D, columns, 24)
+    for e, all_e in ((-6, -5), (-10, 0), (-14, 0), (-14, 8)):
+        s, b = values[1] * 2.0 ** all_e, values[2] * 2.0 ** all_e
+        s[..., 1] *= 2.0 ** e
+        b[..., 1] *= 2.0 ** e
+        _held(q, keys, (values[0], s, b), table, lens, D ** -0.5, qs)
+
+
+@pytest.mark.parametrize("new,H,KVH,D,columns", FORMS)
+def test_attend_values_that_grow_and_shrink_along_the_keys(cuda, new, H, KVH, D, columns):
+    """Keys in runs of 64 whose values are 2^-40 to 2^100 of the usual size, in every order: finite, and within the bound."""
+    import torch
+
+    q, keys, values, table, lens, qs = _case(cuda, new, H, KVH, D, columns, 25, n=640)
+    for sizes in ([0, 2, -3, 6, 9, -8, 1, 0, -2, 5], [100, 0, -40, 3, 0, 100, -40, 0, 8, 20], [-40, 0, 100, 0, -40, 0, 0, 0, 0, 0],
+                  [0, -40, -40, 0, 0, 0, -20, 0, 0, 10], [100, 100, -40, -40, 0, 0, -40, -40, 0, 0]):
+        s, b = values[1].clone(), values[2].clone()
+        for r, e in enumerate(sizes):
+            ids = table[0, 4 * r:4 * r + 4].long()
+            s[ids] *= 2.0 ** e
+            b[ids] *= 2.0 ** e
+        _held(q, keys, (values[0], s, b), table, lens, D ** -0.5, qs)
