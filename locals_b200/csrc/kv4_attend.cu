@@ -18,7 +18,8 @@
 //   queries to fp16 after a power of two a row that puts its largest at 2^13 .. 2^14: exact for fp16 and bf16 but for
 //     values 2^-27 below the row's largest. A row by itself: the tile holds other heads and other tokens of the request;
 //   w to fp16 (2^-11 against the 2^-8 of a bf16 output; an fp16 output's error grows from 2.0e-4 to 2.2e-4 by it), after a
-//     power of two that puts the warp's largest value scale at 2^5 .. 2^10. codes - z (exact on subnormals, one packed subtraction a pair) takes out of a group
+//     power of two a row that puts the largest value scale that the row has seen at 2^5 .. 2^10 (vf for the warp, a row's
+//     difference from it, xl, in its probabilities). codes - z (exact on subnormals, one packed subtraction a pair) takes out of a group
 //     what its codes and its bias have in common, so that this is a rounding of the value itself, however near to 0 it lies.
 // A score tile's accumulator layout is transposed into the value MMA's operand by movmatrix. The running maximum of a row is
 // only followed when it has grown by 2^4, so that most steps rescale nothing.
@@ -420,8 +421,12 @@ __global__ void __launch_bounds__(KV4_NW * 32, kv4_resident(D, NT)) kv4_attend_k
                 for (int g = 0; g < GR; ++g) hb[t][g][e] = 0.0f;
             }
         }
-        float vf = 1.0f;       // the value scales' power of two
-        uint32_t v_limit = 0;  // bits of the largest value scale that it fits (0: none met yet)
+        float vf = 1.0f;       // the value scales' power of two: 2^(132 - e0), for a largest scale whose exponent bits are e0
+        int e0 = 0;
+        float xl[NT][2];       // and a column's beyond it: p and l are 2^xl times as large (negative: it has seen none yet)
+        uint32_t v_limit = 0;  // bits of the least value scale that some column's power does not fit
+#pragma unroll
+        for (int t = 0; t < NT; ++t) xl[t][0] = xl[t][1] = -1.0f;
         // o and hb by f0 (even columns) and f1
         auto rescale = [&](int t, float f0, float f1) {
 #pragma unroll
@@ -433,6 +438,66 @@ __global__ void __launch_bounds__(KV4_NW * 32, kv4_resident(D, NT)) kv4_attend_k
             }
 #pragma unroll
             for (int g = 0; g < GR; ++g) hb[t][g][0] *= f0, hb[t][g][1] *= f1;
+        };
+
+        // Column 8 t + 2 c + e's keys: [lo, hi).
+        auto column = [&](int t, int e, int* lo, int* hi) {
+            const int end = base + (row0 + min(8 * t + 2 * c + e, rows - 1)) / G + 1;
+            *hi = min(end, room), *lo = a.window ? max(end - a.window, 0) : 0;
+        };
+        auto partly = [&](int key0, uint32_t miss) { return key0 < lo_max || key0 + KV4_KEYS > hi_min || miss; };
+        // Fits the columns' powers of two to the scales that they see in a step (bits: the largest; top: this lane's key's):
+        // one that grows leaves its limit at once, to 2^5 .. 2^6, the others stay as they are.
+        auto fit = [&](uint32_t bits, float top, int key0) {
+            int ce[NT][2], seen[NT][2], most = 0;  // exponent bits: that a column is fitted to (0: none yet), of what it sees
+#pragma unroll
+            for (int t = 0; t < NT; ++t) seen[t][0] = seen[t][1] = int(bits >> 23);
+            if (p0 != p1 && partly(key0, 0)) {  // (what no row sees is 0 in top)
+                int lo[NT][2], hi[NT][2];
+#pragma unroll
+                for (int t = 0; t < NT; ++t)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) column(t, e, &lo[t][e], &hi[t][e]), seen[t][e] = -1;
+#pragma unroll 4
+                for (int k = 0; k < KV4_KEYS; ++k) {
+                    const int x = int(__shfl_sync(0xffffffffu, __float_as_uint(top), k) >> 23);
+#pragma unroll
+                    for (int t = 0; t < NT; ++t)
+#pragma unroll
+                        for (int e = 0; e < 2; ++e)
+                            if (key0 + k >= lo[t][e] && key0 + k < hi[t][e]) seen[t][e] = max(seen[t][e], x);
+                }
+            }
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    ce[t][e] = xl[t][e] < 0.0f ? 0 : e0 - int(xl[t][e]);
+                    if (seen[t][e] >= (ce[t][e] ? ce[t][e] + 5 : 0)) ce[t][e] = max(seen[t][e], 64);  // (at least 2^-63)
+                    most = max(most, ce[t][e]);
+                }
+            const int e1 = int(__reduce_max_sync(0xffffffffu, unsigned(most)));
+            int least = 255;
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+                float f[2] = {1.0f, 1.0f};
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    if (ce[t][e]) ce[t][e] = max(ce[t][e], e1 - 100);
+                    least = min(least, ce[t][e]);
+                    if (xl[t][e] >= 0.0f) {
+                        const int was = e0 - int(xl[t][e]), grows = (e1 - ce[t][e]) - int(xl[t][e]);
+                        f[e] = __uint_as_float(uint32_t(max(127 + was - ce[t][e], 1)) << 23);
+                        l[t][e] *= __uint_as_float(uint32_t(127 + grows) << 23);
+                    }
+                    if (ce[t][e]) xl[t][e] = float(e1 - ce[t][e]);
+                }
+                rescale(t, f[0], f[1]);
+            }
+            e0 = e1;
+            if (e1) vf = __uint_as_float(uint32_t(127 + 132 - e1) << 23);
+            least = int(__reduce_min_sync(0xffffffffu, unsigned(least)));
+            v_limit = least ? uint32_t(least + 5) << 23 : 0;
         };
 
         uint32_t sb = ring, sb_issue = ring + (S::STAGES - 1) * S::STAGE;
@@ -489,16 +554,9 @@ __global__ void __launch_bounds__(KV4_NW * 32, kv4_resident(D, NT)) kv4_attend_k
 #pragma unroll
                     for (int g = 0; g < GR; ++g) w[0][g] = __int_as_float(0x7fffffff), w[2][g] = 0.0f, w[3][g] = 0.0f;
                 }
-                // the value scales' power of two: larger scales are met by a smaller one
+                // the value scales' powers of two: larger scales are met by a smaller one
                 const uint32_t bits = __reduce_max_sync(0xffffffffu, __float_as_uint(top));
-                if (bits > v_limit) {
-                    const int E = max(int(bits >> 23), 64);  // (at least 2^-63)
-                    const float nf = __uint_as_float(uint32_t(127 + 5 + 127 - E) << 23);  // to 2^5 .. 2^6
-#pragma unroll
-                    for (int tt = 0; tt < NT; ++tt) rescale(tt, nf / vf, nf / vf);
-                    vf = nf;
-                    v_limit = (uint32_t(E + 5) << 23) - 1;  // below 2^10 / vf
-                }
+                if (bits >= v_limit) fit(bits, top, key0);
                 float f[S::FL];
 #pragma unroll
                 for (int g = 0; g < GR; ++g) {
@@ -563,13 +621,13 @@ __global__ void __launch_bounds__(KV4_NW * 32, kv4_resident(D, NT)) kv4_attend_k
                         }
                 }
             }
-            if (key0 < lo_max || key0 + KV4_KEYS > hi_min || miss) {  // some row does not see some key
+            if (partly(key0, miss)) {  // some row does not see some key
 #pragma unroll
                 for (int tt = 0; tt < NT; ++tt)
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
-                        const int end = base + (row0 + min(8 * tt + 2 * c + e, rows - 1)) / G + 1;
-                        const int hi = min(end, room), lo = a.window ? max(end - a.window, 0) : 0;
+                        int lo, hi;
+                        column(tt, e, &lo, &hi);
 #pragma unroll
                         for (int h = 0; h < 2; ++h)
 #pragma unroll
@@ -611,7 +669,7 @@ __global__ void __launch_bounds__(KV4_NW * 32, kv4_resident(D, NT)) kv4_attend_k
             for (int tt = 0; tt < NT; ++tt)
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
-                    const float mz = m[tt][e] == -INFINITY ? 0.0f : m[tt][e];
+                    const float mz = (m[tt][e] == -INFINITY ? 0.0f : m[tt][e]) - xl[tt][e];
 #pragma unroll
                     for (int h = 0; h < 2; ++h)
 #pragma unroll
@@ -678,13 +736,13 @@ __global__ void __launch_bounds__(KV4_NW * 32, kv4_resident(D, NT)) kv4_attend_k
         __syncthreads();  // every warp is done with its ring
         float* cm = reinterpret_cast<float*>(kv4_smem);  // [warp][R] m, then l, then O [warp][R][D]
         float *cl = cm + KV4_NW * R, *co = cl + KV4_NW * R;
-        const float inv = 1.0f / vf;
 #pragma unroll
         for (int t = 0; t < NT; ++t)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
+                const float up = __uint_as_float(uint32_t(127 - int(fmaxf(xl[t][e], 0.0f))) << 23), inv = up / vf;
                 const int col = warp * R + 8 * t + 2 * c + e;
-                if (gid == 0) cm[col] = m[t][e], cl[col] = l[t][e];
+                if (gid == 0) cm[col] = m[t][e], cl[col] = l[t][e] * up;
                 float* dst = co + col * D + 8 * gid;
 #pragma unroll
                 for (int g = 0; g < GR; ++g)

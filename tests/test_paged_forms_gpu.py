@@ -162,3 +162,48 @@ def test_values_of_any_size(cuda, form, new, H, KVH, D, columns):
         got = paged.attend(q, keys, vals, table, lens, scale, q_start=qs, max_q=new)
         ref, bound = R.attended(q, keys, vals, table, lens, scale, qs, None, 0)
         assert bool(((got.double() - ref).abs() <= bound - 2.0 ** -24 + 2.0 ** -24 * min(size, 1.0)).all()), size
+
+
+def _sizes(q, keys, values, table, n, scale, window):
+    """sum p |v| / sum p of each output, in 64 bits."""
+    import torch
+
+    new, H, D = q.shape
+    k, v = R.unpacked(keys), R.unpacked(values)
+    KVH, page = k.shape[1], k.shape[2]
+    ids = table[0, :-(-n // page)].long()
+    kb, vb = (x[ids].transpose(0, 1).flatten(1, 2)[:, :n] for x in (k, v))
+    s = scale * torch.einsum("ihgd,hjd->hgij", q.double().view(new, KVH, H // KVH, D), kb)
+    at, j = (n - new + torch.arange(new, device=q.device))[:, None], torch.arange(n, device=q.device)[None]
+    seen = (j <= at) & (j > at - window) if window else j <= at
+    p = s.masked_fill(~seen, -math.inf).softmax(-1)
+    return torch.einsum("hgij,hjd->ihgd", p, vb.abs()).reshape(new, H, D)
+
+
+def _out_of_sight(cuda, form, new, H, KVH, D, columns, e):
+    """Values 2^e of the usual size reach only the rows that see them: the first 64 keys, behind the windows of all queries but
+    the first two, and the last token's but one. The others' outputs are those beside ordinary values there, but for the roundings
+    of 16-bit operands (2 * 2^-11 of sum p |v|) and outputs, of each."""
+    import torch
+    from locals_b200 import paged
+
+    n = 6000 if form in (CLUSTERS, SPLIT) else 640  # (several steps a CTA)
+    for window, places, rows in ((n - 64 - new + 2, range(64), slice(2, None)), (0, range(n - 2, n - 1), slice(0, -2))):
+        plain, (q, keys, values, table, qs, scale, _) = _one(cuda, form, new, n, H, KVH, D, columns, seed=31, window=window)
+        s, b = values[1].clone(), values[2].clone()
+        for j in places:
+            at = int(table[0, j // 16]), slice(None), j % 16
+            s[at] *= 2.0 ** e
+            b[at] *= 2.0 ** e
+        got = paged.attend(q, keys, (values[0], s, b), table, _i32([n], cuda), scale, q_start=qs, max_q=new, window=window)
+        size = _sizes(q, keys, values, table, n, scale, window)
+        bound = 2 * (R.U[q.dtype] * size.clamp(max=plain.double().abs()) + size * (2.0 ** -10 + 2.0 ** -14)) + 2.0 ** -24
+        off = ((got.double() - plain.double()).abs() - bound)[rows]
+        assert bool((off <= 0).all()), (window, off.max().item())
+    assert _status() == 0
+
+
+@pytest.mark.parametrize("e", [10, 20, 60, 100])
+@pytest.mark.parametrize("form,new,H,KVH,D,columns", [x for x in EACH if x[0] in (CLUSTERS, SPLIT)])
+def test_large_values_out_of_sight(cuda, form, new, H, KVH, D, columns, e):
+    _out_of_sight(cuda, form, new, H, KVH, D, columns, e)
