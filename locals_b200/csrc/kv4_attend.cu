@@ -149,11 +149,6 @@ __device__ __forceinline__ uint32_t kv4_sub(uint32_t a, uint32_t b) {
     const __half2 d = __hsub2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
     return *reinterpret_cast<const uint32_t*>(&d);
 }
-__device__ __forceinline__ uint32_t lds32(uint32_t addr) {
-    uint32_t v;
-    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(addr));
-    return v;
-}
 
 // N floats from shared memory: from a multiple of 16 bytes where N is above 3, of 8 else.
 template <int N>

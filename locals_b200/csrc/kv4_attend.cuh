@@ -30,6 +30,7 @@ struct Kv4AttArgs {
     float* part_o;     // (CTA, 2, rows) x D
     int32_t* records;  // (CTA) x 8: the item that the start of a CTA's share divides
     uint8_t* dense;    // (request, kv head, dense_steps) x {keys, values} of a step as fp16 tiles (kv4_prefill's dense form)
+    int8_t* dense_keys;  // powers of two of the keys' values, where those of a step differ widely
     int2* dense_meta;  // their keys' and values' powers of two, and the runs of 8 keys without a page
     int dense_steps;
     float scale_log2;
@@ -46,6 +47,12 @@ __device__ __forceinline__ float kv4_ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
+}
+
+__device__ __forceinline__ uint32_t lds32(uint32_t addr) {
+    uint32_t v;
+    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(addr));
+    return v;
 }
 
 // A request's place in the step: its queries' first row, their number, its keys and the 128-key steps that they span.

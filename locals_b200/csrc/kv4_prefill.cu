@@ -25,8 +25,9 @@
 // scores' factor: a group's scale and a sixteenth of it stay normal numbers down to 2^-19 of that, where the group's share of
 // a score is as small. Values after a power of two a step in the same way; a row's outputs have one of their own, and its
 // probabilities are multiplied by the difference while that is small, its outputs (as its maximum's growth does) where it
-// is not: so a step's values cost another step's no bits, and a row only those of the keys that it sees. Within a step,
-// values are held to 2^-35 of the largest.
+// is not: so a step's values cost another step's no bits, and a row only those of the keys that it sees. A step with keys
+// whose values are 2^-16 of the largest or less has one a key (PF_WILD; key_exp), which each row's probabilities take in, in
+// the two-pass step: the large ones may be out of a row's sight. Within a key, values are held to 2^-35 of its largest.
 // A masked score is -inf, its probability 0; a value whose scale or bias is not finite is held as 0 and its key as NaN,
 // so that only rows that see it become NaN.
 // Work is dealt out as in kv4_attend.cu: the steps of all tiles (each as far as its last row sees) evenly over one CTA a
@@ -275,13 +276,15 @@ struct PfBars {
     int abort;          // a wait gave up: no one waits any more
     int exps[4];        // powers of two of the keys and values of step i & 3 (pf_exps)
     uint32_t miss[4];   // its runs of 8 keys without a page
+    alignas(16) int8_t key_exp[4][128];  // powers of two of its keys' values, where they differ widely (PF_WILD)
+    int key_top[128];   // bits of the largest |value| that a key's groups can hold, while those are found
     // what the page warp tells the unpacking warps of step i & 3: the pool row of each run of 8 keys (none: KV4_NONE), the
     // keys from its first to the tile's end (0: no more steps), and the runs without a page
     uint32_t run[4][16];
     int left[4];
     uint32_t gone[4];
     float k_max[2][PF_UNPACK], v_max[2][PF_UNPACK];  // of step i & 1: what each unpacking warp's groups can hold at most
-                                                     // (values: negative from a warp that has no step)
+    float v_min[2][PF_UNPACK];                       // (values: negative from a warp that has no step), and the least of that
     int rows, steps;    // the item's (0: no more), from the first softmax warp to the issuing thread
 };
 
@@ -328,10 +331,11 @@ __device__ __forceinline__ void pf_unpack(const uint4& codes, float s, float b, 
 }
 
 // A piece's scales and biases in fp32. A value scale or bias that is not finite makes the values 0 and the key NaN, which
-// only the rows that see it meet; so does an infinite key. Adds the largest |key| and |value| that the groups can hold.
+// only the rows that see it meet; so does an infinite key. Adds the largest |key| and |value| that the groups can hold, and
+// the least that is not 0 of the values'.
 template <typename T>
 __device__ __forceinline__ void pf_scales(uint16_t ks16, uint16_t kb16, uint16_t vs16, uint16_t vb16, float* ks, float* kb,
-                                          float* vs, float* vb, float* k_top, float* v_top) {
+                                          float* vs, float* vb, float* k_top, float* v_top, float* v_low) {
     *ks = F16Traits<T>::to_f32(ks16), *kb = F16Traits<T>::to_f32(kb16);
     *vs = F16Traits<T>::to_f32(vs16), *vb = F16Traits<T>::to_f32(vb16);
     const float k_most = fmaf(15.0f, fabsf(*ks), fabsf(*kb)), v_most = fmaf(15.0f, fabsf(*vs), fabsf(*vb));
@@ -341,6 +345,7 @@ __device__ __forceinline__ void pf_scales(uint16_t ks16, uint16_t kb16, uint16_t
         return;
     }
     *v_top = fmaxf(*v_top, v_most);
+    if (v_most > 0.0f) *v_low = fminf(*v_low, v_most);
     if (k_most < INFINITY) *k_top = fmaxf(*k_top, k_most);
 }
 // 2^e, e in -126 .. 127.
@@ -349,11 +354,15 @@ __device__ __forceinline__ float pf_pow2(int e) { return __uint_as_float(uint32_
 __device__ __forceinline__ int pf_fit(float M) { return M > 0.0f ? min(13 - (int(__float_as_uint(M) >> 23) - 127), 120) : 0; }
 // The powers of two of a step's keys and values in one word.
 __device__ __forceinline__ int pf_exps(int ke, int ve) { return int(uint32_t(ke) << 16 | (uint32_t(ve) & 0xffffu)); }
-// The values' of a step that holds none but zeros: any.
-constexpr int PF_ANY = 127;
+// The values' of a step (or key) that holds none but zeros: any; and of a step whose keys have one each.
+constexpr int PF_ANY = 127, PF_WILD = 126;
+__device__ __forceinline__ bool pf_wild(float least, float most) { return least < most * 0x1p-16f; }
+__device__ __forceinline__ int8_t pf_key_exp(int top) { return int8_t(top ? pf_fit(__int_as_float(top)) : PF_ANY); }
+// A key's values' power of two from its largest (a finite |value| group): bits of an int are in a float's order.
+__device__ __forceinline__ void pf_key_max(int* top, float vs, float vb) { atomicMax(top, __float_as_int(fmaf(15.0f, fabsf(vs), fabsf(vb)))); }
 // How far a row's outputs may lie from a step's values before they are multiplied: probabilities, at most 2^8, times 2^6 are
 // within fp16; times 2^-4, those below 2^-10 begin to lose bits, of values that are 2^-4 as large.
-constexpr int PF_UP = 6, PF_DOWN = -4;
+constexpr int PF_UP = 6, PF_DOWN = -4;  // (ve is at most 120)
 
 // ---- the dense form's first pass: the keys and values of requests with many tiles, unpacked once ----
 // One CTA a (step of KT keys, kv head, request): the step's two tiles as they are to lie in shared memory, copied out whole,
@@ -364,7 +373,8 @@ __global__ void __launch_bounds__(PD_WARPS * 32) kv4_dense_kernel(const Kv4AttAr
     using S = PfShape<D>;
     using P = PfPieces<D, PD_WARPS>;
     extern __shared__ __align__(1024) uint8_t pf_raw[];
-    __shared__ float part[PD_WARPS], k_part[PD_WARPS];
+    __shared__ float part[PD_WARPS], k_part[PD_WARPS], low_part[PD_WARPS];
+    __shared__ int key_top[S::KT];
     grid_dep_wait();
     const int s = blockIdx.x, kvh = blockIdx.y, b = blockIdx.z;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -390,7 +400,7 @@ __global__ void __launch_bounds__(PD_WARPS * 32) kv4_dense_kernel(const Kv4AttAr
     }
     const uint32_t miss = __ballot_sync(0xffffffffu, lane < RUNS && gone);
     uint4 kc[P::J], vc[P::J];
-    float ks[P::J], kb[P::J], vs[P::J], vb[P::J], k_top = 0.0f, top = 0.0f;
+    float ks[P::J], kb[P::J], vs[P::J], vb[P::J], k_top = 0.0f, top = 0.0f, low = INFINITY;
     uint16_t sc[P::J][4];
 #pragma unroll
     for (int j = 0; j < P::J; ++j) {
@@ -407,13 +417,26 @@ __global__ void __launch_bounds__(PD_WARPS * 32) kv4_dense_kernel(const Kv4AttAr
     }
 #pragma unroll
     for (int j = 0; j < P::J; ++j)
-        pf_scales<T>(sc[j][0], sc[j][1], sc[j][2], sc[j][3], &ks[j], &kb[j], &vs[j], &vb[j], &k_top, &top);
+        pf_scales<T>(sc[j][0], sc[j][1], sc[j][2], sc[j][3], &ks[j], &kb[j], &vs[j], &vb[j], &k_top, &top, &low);
     top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top)));
     k_top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(k_top)));
-    if (lane == 0) part[warp] = top, k_part[warp] = k_top;
+    low = __uint_as_float(__reduce_min_sync(0xffffffffu, __float_as_uint(low)));
+    if (lane == 0) part[warp] = top, k_part[warp] = k_top, low_part[warp] = low;
+    if (threadIdx.x < S::KT) key_top[threadIdx.x] = 0;
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < PD_WARPS; ++i) top = fmaxf(top, part[i]), k_top = fmaxf(k_top, k_part[i]);
+    for (int i = 0; i < PD_WARPS; ++i) {
+        top = fmaxf(top, part[i]), k_top = fmaxf(k_top, k_part[i]);
+        low = fminf(low, low_part[i]);
+    }
+    const size_t at = ((size_t)b * a.pool.KVH + kvh) * a.dense_steps + s;
+    const bool wild = pf_wild(low, top);
+    if (wild) {
+#pragma unroll
+        for (int j = 0; j < P::J; ++j) pf_key_max(&key_top[P::key(j, warp, lane)], vs[j], vb[j]);
+        __syncthreads();
+        if (threadIdx.x < S::KT) a.dense_keys[at * S::KT + threadIdx.x] = pf_key_exp(key_top[threadIdx.x]);
+    }
     const int ke = pf_fit(k_top);
     const float kf = pf_pow2(ke);
     const int ve = pf_fit(top);
@@ -421,19 +444,133 @@ __global__ void __launch_bounds__(PD_WARPS * 32) kv4_dense_kernel(const Kv4AttAr
 #pragma unroll
     for (int j = 0; j < P::J; ++j) {
         const int k = P::key(j, warp, lane), p = P::piece(j, warp, lane);
+        const float f = wild ? pf_pow2(pf_fit(__int_as_float(key_top[k]))) : vf;
         pf_unpack<D>(kc[j], ks[j] * kf, kb[j] * kf, tile, k, p);
-        pf_unpack<D>(vc[j], vs[j] * vf, vb[j] * vf, tile + S::TB, k, p);
+        pf_unpack<D>(vc[j], vs[j] * f, vb[j] * f, tile + S::TB, k, p);
     }
     fence_proxy_async();
     __syncthreads();
     if (threadIdx.x == 0) {
-        const size_t at = ((size_t)b * a.pool.KVH + kvh) * a.dense_steps + s;
-        a.dense_meta[at] = make_int2(pf_exps(ke, top > 0.0f ? ve : PF_ANY), int(miss));
+        a.dense_meta[at] = make_int2(pf_exps(ke, wild ? PF_WILD : top > 0.0f ? ve : PF_ANY), int(miss));
         asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(a.dense + at * (2 * S::TB)), "r"(tile),
                      "r"(2 * S::TB)
                      : "memory");
         asm volatile("cp.async.bulk.commit_group;\n\tcp.async.bulk.wait_group 0;" ::: "memory");
     }
+}
+
+// What a row sees of keys 32 i .. 32 i + 31 of a step, a bit a key: [lo, hi) of the step's keys but for its missing runs.
+__device__ __forceinline__ uint32_t pf_sees(int lo, int hi, uint32_t miss, int i) {
+    const int from = min(max(lo - 32 * i, 0), 32), to = min(max(hi - 32 * i, 0), 32);
+    uint32_t v = uint32_t((1ull << to) - 1) & ~uint32_t((1ull << from) - 1);
+    const uint32_t gone = (miss >> (4 * i)) & 15;
+    if (gone) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            if ((gone >> k) & 1) v &= ~(0xffu << (8 * k));
+    }
+    return v;
+}
+__device__ __forceinline__ float pf_seen(uint32_t score, uint32_t v, int i) { return (v >> i) & 1 ? __uint_as_float(score) : -INFINITY; }
+// The scores' factor (a positive number, so that a masked score stays -inf).
+__device__ __forceinline__ float pf_factor(float c, int exps) {
+    return fminf(fmaxf(c * pf_pow2(-(exps >> 16)), 1.17549435e-38f), 3.4028234e38f);
+}
+
+// A row's running maximum (base 2) and sum, its outputs' power of two, and the least of the steps' that this was fitted to.
+struct PfRow {
+    float m, l;
+    int ve, ve_low;
+};
+
+// A new maximum mn, and, of a step that gives one (sized), a new power of two of the outputs: the step's, but no more than 2^64
+// above the least of the steps' before, whose sums (below 2^43) then stay within 32 bits' range. Returns what the outputs are
+// multiplied by.
+__device__ __forceinline__ float pf_refit(PfRow& row, float mn, int ve_t, bool sized) {
+    int to = row.ve;
+    if (sized) row.ve_low = min(row.ve_low, ve_t), to = min(ve_t, row.ve_low + 64);
+    const float decay = mn > row.m ? kv4_ex2(row.m - mn) : 1.0f;
+    const float corr = row.m == -INFINITY ? 0.0f : decay * pf_pow2(max(to - row.ve, -126));
+    row.l *= decay;
+    row.m = mn;
+    row.ve = to;
+    return corr;
+}
+
+// A row's step whose keys' values have a power of two each (PF_WILD), in two passes over its scores (s_col), which its
+// probabilities replace; before: products into its outputs (o_col) so far, 0 for none. Out of line, since it is rare.
+template <typename T, int D>
+__device__ __noinline__ PfRow pf_wild_step(PfRow row, PfBars* bars, int it, int w, int before, uint32_t s_col, uint32_t o_col,
+                                            int lo, int hi, float c) {
+    constexpr int KT = PfShape<D>::KT;
+    const int exps = *reinterpret_cast<volatile int*>(&bars->exps[it & 3]);
+    const uint32_t miss = *reinterpret_cast<volatile uint32_t*>(&bars->miss[it & 3]), key_exp = smem_u32(bars->key_exp[it & 3]);
+    const float ct = pf_factor(c, exps);
+    int ve_t = PF_ANY;  // the largest values' that the row sees
+#pragma unroll 1
+    for (int k = 0; k < KT; k += 4) {
+        const uint32_t v = pf_sees(lo, hi, miss, k / 32) >> (k & 31), x = lds32(key_exp + k);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if ((v >> i) & 1) ve_t = min(ve_t, int(int8_t(x >> (8 * i))));
+    }
+    const bool sized = ve_t != PF_ANY;
+    if (!sized) ve_t = row.ve;
+    float mx = -INFINITY;
+#pragma unroll 1
+    for (int ch = 0; ch < KT / 32; ++ch) {
+        uint32_t r[32];
+        tmem_ld_32x32b_x32(s_col + ch * 32, r);
+        const uint32_t v = pf_sees(lo, hi, miss, ch);
+        tmem_wait_ld();
+        float part[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+        for (int i = 0; i < 32; i += 2) part[(i >> 1) & 1] = fmaxf(fmaxf(part[(i >> 1) & 1], pf_seen(r[i], v, i)), pf_seen(r[i + 1], v, i + 1));
+        mx = fmaxf(mx, fmaxf(part[0], part[1]));
+    }
+    const float mn = fmaxf(row.m, mx * ct);
+    const bool some = mx != -INFINITY;
+    const int d = row.ve - ve_t;
+    const bool grow = mn > row.m + 8.0f || (row.m == -INFINITY && mn > row.m) || (some && (d < PF_DOWN || d > PF_UP));
+    if (__any_sync(0xffffffffu, grow)) {
+        const float corr = pf_refit(row, mn, ve_t, some && sized);
+        if (before) {
+            pf_wait(&bars->o_done[w], (before - 1) & 1, &bars->abort);  // the last product is in
+            tc_fence_after();
+#pragma unroll 1
+            for (int ch = 0; ch < D / 32; ++ch) {
+                uint32_t r[32];
+                tmem_ld_32x32b_x32(o_col + ch * 32, r);
+                tmem_wait_ld();
+#pragma unroll
+                for (int i = 0; i < 32; ++i) r[i] = __float_as_uint(__uint_as_float(r[i]) * corr);
+                tmem_st_32x32b_x32(o_col + ch * 32, r);
+            }
+        }
+    }
+    const float mz = row.m == -INFINITY ? 0.0f : row.m;
+    float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 1
+    for (int ch = 0; ch < KT / 16; ++ch) {
+        uint32_t x[16], p[8];
+        tmem_ld_32x32b_x16(s_col + ch * 16, x);
+        const uint32_t v = pf_sees(lo, hi, miss, ch >> 1) >> (16 * (ch & 1));
+        tmem_wait_ld();
+#pragma unroll
+        for (int i = 0; i < 16; i += 2) {
+            const float e0 = kv4_ex2(fmaf(pf_seen(x[i], v, i), ct, -mz));
+            const float e1 = kv4_ex2(fmaf(pf_seen(x[i + 1], v, i + 1), ct, -mz));
+            // (the large ones' probabilities are at most 2^8 times 2^PF_UP, the small ones' may become 0 beside them)
+            const uint32_t k = lds32(key_exp + ch * 16 + (i & ~3)) >> (8 * (i & 2));
+            p[i / 2] = cvt_f16x2(e1 * pf_pow2(min(max(row.ve - int(int8_t(k >> 8)), -126), 100)),
+                                 e0 * pf_pow2(min(max(row.ve - int(int8_t(k)), -126), 100)));
+            sum[i & 2] += e0;
+            sum[(i & 2) + 1] += e1;
+        }
+        pf_tmem_st8(s_col + ch * 8, p);
+    }
+    row.l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+    return row;
 }
 
 // DENSE: the tiles come unpacked, by bulk copies, from what kv4_dense_kernel left.
@@ -446,8 +583,12 @@ __global__ void __launch_bounds__(pf_threads(DENSE), 1) kv4_prefill_kernel(const
     __shared__ uint8_t* volatile pf_base;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
+    if (smem_u32(pf_raw) & 1023) {  // (the declaration's alignment; there is no room to make up for it)
+        if (tid == 0) record_status(LQ_DEV_BOUNDS);
+        return;
+    }
     if (tid == 0) {
-        uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(pf_raw) + 1023) & ~uintptr_t(1023));
+        uint8_t* smem = pf_raw;
         PfBars& bar = *reinterpret_cast<PfBars*>(smem + S::SMEM);
         pf_base = smem;
         for (int i = 0; i < 2; ++i) {
@@ -657,8 +798,7 @@ __global__ void __launch_bounds__(pf_threads(DENSE), 1) kv4_prefill_kernel(const
             __syncwarp();
             if (lane == 0) mbar_arrive(&bar.q_full[w]);
 
-            float m = -INFINITY, l = 0.0f;
-            int ve = 0, ve_low = 1000;  // the row's outputs' power of two; the least of the steps' that it was fitted to
+            PfRow row_at = {-INFINITY, 0.0f, 0, 1000};
             const uint32_t o_col = tmem + lanes + S::O_COL + w * D;
             for (int t = 0; t < steps; ++t, ++it, ++used) {
                 const int buf = NQ == 2 ? w : used & 1;
@@ -667,30 +807,12 @@ __global__ void __launch_bounds__(pf_threads(DENSE), 1) kv4_prefill_kernel(const
                 tc_fence_after();
                 const int key0 = (walk.lo + walk.st0 + t) * KT;
                 const uint32_t miss = *reinterpret_cast<volatile uint32_t*>(&bar.miss[it & 3]);
-                // The scores' factor (a positive number, so that a masked score stays -inf), and how far the row's outputs lie from
-                // the step's values: its probabilities are multiplied by 2^that. (Read where they are used: the one pass needs the
-                // registers.)
+                // How far the row's outputs lie from the step's values: its probabilities are multiplied by 2^that. (Below PF_DOWN
+                // for PF_ANY and PF_WILD. Read where it is used: the one pass needs the registers.)
                 auto exps = [&]() { return *reinterpret_cast<volatile int*>(&bar.exps[it & 3]); };
-                auto factor = [&]() { return fminf(fmaxf(c * pf_pow2(-(exps() >> 16)), 1.17549435e-38f), 3.4028234e38f); };
-                auto apart = [&]() -> int {
-                    const int ve_t = int16_t(exps());
-                    return ve_t == PF_ANY ? 0 : ve - ve_t;
-                };
+                auto apart = [&]() { return row_at.ve - int(int16_t(exps())); };
                 const bool all = key0 >= lo_all && key0 + KT <= hi_all && miss == 0;
                 const uint32_t s_col = tmem + lanes + buf * KT;
-                // what this row sees of 32 of the step's keys, a bit a key
-                auto sees = [&](int i) -> uint32_t {
-                    const int from = min(max(row_lo - key0 - 32 * i, 0), 32), to = min(max(row_hi - key0 - 32 * i, 0), 32);
-                    uint32_t v = uint32_t((1ull << to) - 1) & ~uint32_t((1ull << from) - 1);
-                    const uint32_t gone = (miss >> (4 * i)) & 15;
-                    if (gone) {
-#pragma unroll
-                        for (int k = 0; k < 4; ++k)
-                            if ((gone >> k) & 1) v &= ~(0xffu << (8 * k));
-                    }
-                    return v;
-                };
-                auto seen = [](uint32_t score, uint32_t v, int i) { return (v >> i) & 1 ? __uint_as_float(score) : -INFINITY; };
                 // One query tile: a step's scores are issued before the last step's product, so that without this a warp could
                 // be done with an item while two products are to come, and the barrier's parity would take the one before both
                 // for the last. Before this step's probabilities are given out, the next product cannot be mistaken.
@@ -700,7 +822,7 @@ __global__ void __launch_bounds__(pf_threads(DENSE), 1) kv4_prefill_kernel(const
                 // The common case, one pass: the reference from the steps before serves the step (found out at its end: the
                 // probabilities stay in registers until then, the scores in place).
                 auto once = [&](auto masked) -> bool {
-                    const float ct = factor(), md = float(apart()) - m;
+                    const float ct = pf_factor(c, exps()), md = float(apart()) - row_at.m;
                     const uint64_t c2 = pf_pair(ct, ct), m2 = pf_pair(md, md);
                     constexpr int CH = 16;  // scores at a time (32: 1082 against 1040 us for a 4096-token prompt piece)
                     uint32_t r[2][CH], p[KT / 2];
@@ -713,11 +835,11 @@ __global__ void __launch_bounds__(pf_threads(DENSE), 1) kv4_prefill_kernel(const
                         uint32_t(&x)[CH] = r[ch & 1];
                         tmem_wait_ld();
                         if (ch + 1 < KT / CH) tmem_ld_32x32b_x16(s_col + (ch + 1) * CH, r[(ch + 1) & 1]);
-                        if constexpr (decltype(masked)::value) v = ch & 1 ? v >> 16 : sees(ch / 2);
+                        if constexpr (decltype(masked)::value) v = ch & 1 ? v >> 16 : pf_sees(row_lo - key0, row_hi - key0, miss, ch / 2);
 #pragma unroll
                         for (int i = 0; i < CH; i += 2) {
                             float s0 = __uint_as_float(x[i]), s1 = __uint_as_float(x[i + 1]);
-                            if constexpr (decltype(masked)::value) s0 = seen(x[i], v, i), s1 = seen(x[i + 1], v, i + 1);
+                            if constexpr (decltype(masked)::value) s0 = pf_seen(x[i], v, i), s1 = pf_seen(x[i + 1], v, i + 1);
                             mx[(i >> 1) & 1] = fmaxf(fmaxf(mx[(i >> 1) & 1], s0), s1);
                             float e0, e1;
                             pf_unpair(pf_fma2(pf_pair(s0, s1), c2, m2), &e0, &e1);
@@ -729,13 +851,13 @@ __global__ void __launch_bounds__(pf_threads(DENSE), 1) kv4_prefill_kernel(const
                             p[(ch * CH + i) / 2] = h;
                         }
                     }
-                    if (__any_sync(0xffffffffu, fmaxf(mx[0], mx[1]) * ct > m + 8.0f)) return false;
+                    if (__any_sync(0xffffffffu, fmaxf(mx[0], mx[1]) * ct > row_at.m + 8.0f)) return false;
 #pragma unroll
                     for (int ch = 0; ch < KT / 64; ++ch) pf_tmem_st32(s_col + ch * 32, &p[ch * 32]);
                     float a0, a1, b0, b1;
                     pf_unpair(sums[0], &a0, &a1);
                     pf_unpair(sums[1], &b0, &b1);
-                    l = fmaf((a0 + a1) + (b0 + b1), pf_pow2(-apart()), l);
+                    row_at.l = fmaf((a0 + a1) + (b0 + b1), pf_pow2(-apart()), row_at.l);
                     tmem_wait_st();
                     tc_fence_before();
                     __syncwarp();
@@ -743,75 +865,74 @@ __global__ void __launch_bounds__(pf_threads(DENSE), 1) kv4_prefill_kernel(const
                     if (lane == 0) mbar_arrive(&bar.p_full[buf]);
                     return true;
                 };
-                if (__all_sync(0xffffffffu, m != -INFINITY && unsigned(apart() - PF_DOWN) <= unsigned(PF_UP - PF_DOWN))) {
+                if (__all_sync(0xffffffffu, row_at.m != -INFINITY && unsigned(apart() - PF_DOWN) <= unsigned(PF_UP - PF_DOWN))) {
                     if (all ? once(std::false_type()) : once(std::true_type())) continue;
                 }
                 // A new reference (an item's first step, mostly): two passes, in loops, since their code is not often in reach.
-                const float ct = factor();
-                int d = apart();
-                float mx = -INFINITY;
+                int ve_t = int16_t(exps());
+                if (ve_t == PF_WILD) {
+                    row_at = pf_wild_step<T, D>(row_at, &bar, it, w, t > 0 ? used : 0, s_col, o_col, row_lo - key0, row_hi - key0, c);
+                } else {
+                    const float ct = pf_factor(c, exps());
+                    const bool sized = ve_t != PF_ANY;
+                    if (!sized) ve_t = row_at.ve;
+                    float mx = -INFINITY;
 #pragma unroll 1
-                for (int ch = 0; ch < KT / 32; ++ch) {
-                    uint32_t r[32];
-                    tmem_ld_32x32b_x32(s_col + ch * 32, r);
-                    const uint32_t v = sees(ch);
-                    tmem_wait_ld();
-                    float part[2] = {-INFINITY, -INFINITY};
+                    for (int ch = 0; ch < KT / 32; ++ch) {
+                        uint32_t r[32];
+                        tmem_ld_32x32b_x32(s_col + ch * 32, r);
+                        const uint32_t v = pf_sees(row_lo - key0, row_hi - key0, miss, ch);
+                        tmem_wait_ld();
+                        float part[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-                    for (int i = 0; i < 32; i += 2) part[(i >> 1) & 1] = fmaxf(fmaxf(part[(i >> 1) & 1], seen(r[i], v, i)), seen(r[i + 1], v, i + 1));
-                    mx = fmaxf(mx, fmaxf(part[0], part[1]));
-                }
-                const float mn = fmaxf(m, mx * ct);
-                const bool some = mx != -INFINITY;
-                const bool grow = mn > m + 8.0f || (m == -INFINITY && mn > m) || (some && (d < PF_DOWN || d > PF_UP));
-                if (__any_sync(0xffffffffu, grow)) {
-                    // The outputs' new power of two: the step's, but no more than 2^64 above the least of the steps' before, whose
-                    // sums (below 2^43) then stay within 32 bits' range.
-                    int to = ve;
-                    if (some) ve_low = min(ve_low, ve - d), to = min(ve - d, ve_low + 64);
-                    const float decay = mn > m ? kv4_ex2(m - mn) : 1.0f;
-                    const float corr = t == 0 || m == -INFINITY ? 0.0f : decay * pf_pow2(max(to - ve, -126));
-                    l *= decay;
-                    m = mn;
-                    d += to - ve;
-                    ve = to;
-                    if (t > 0) {
-                        pf_wait(&bar.o_done[w], (used - 1) & 1, abort);  // the last product is in
-                        tc_fence_after();
+                        for (int i = 0; i < 32; i += 2)
+                            part[(i >> 1) & 1] = fmaxf(fmaxf(part[(i >> 1) & 1], pf_seen(r[i], v, i)), pf_seen(r[i + 1], v, i + 1));
+                        mx = fmaxf(mx, fmaxf(part[0], part[1]));
+                    }
+                    const float mn = fmaxf(row_at.m, mx * ct);
+                    const bool some = mx != -INFINITY;
+                    const int d = row_at.ve - ve_t;
+                    const bool grow = mn > row_at.m + 8.0f || (row_at.m == -INFINITY && mn > row_at.m) || (some && (d < PF_DOWN || d > PF_UP));
+                    if (__any_sync(0xffffffffu, grow)) {
+                        const float corr = pf_refit(row_at, mn, ve_t, some && sized);
+                        if (t > 0) {
+                            pf_wait(&bar.o_done[w], (used - 1) & 1, abort);  // the last product is in
+                            tc_fence_after();
 #pragma unroll 1
-                        for (int ch = 0; ch < D / 32; ++ch) {
-                            uint32_t r[32];
-                            tmem_ld_32x32b_x32(o_col + ch * 32, r);
-                            tmem_wait_ld();
+                            for (int ch = 0; ch < D / 32; ++ch) {
+                                uint32_t r[32];
+                                tmem_ld_32x32b_x32(o_col + ch * 32, r);
+                                tmem_wait_ld();
 #pragma unroll
-                            for (int i = 0; i < 32; ++i) r[i] = __float_as_uint(__uint_as_float(r[i]) * corr);
-                            tmem_st_32x32b_x32(o_col + ch * 32, r);
+                                for (int i = 0; i < 32; ++i) r[i] = __float_as_uint(__uint_as_float(r[i]) * corr);
+                                tmem_st_32x32b_x32(o_col + ch * 32, r);
+                            }
                         }
                     }
-                }
-                // (d is below PF_DOWN only after so large values that this step's are nothing beside them: their probabilities are 0
-                // in fp16, and still in the row's sum; and beyond PF_UP only in rows that see nothing of the step)
-                const int dd = min(max(d, -60), 60);
-                const float mz = (m == -INFINITY ? 0.0f : m) - float(dd);
-                float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                    // (below PF_DOWN only after so large values that this step's are nothing beside them: their probabilities are 0
+                    // in fp16, and still in the row's sum; and beyond PF_UP only in rows that see nothing of the step)
+                    const int dd = min(max(row_at.ve - ve_t, -60), 60);
+                    const float mz = (row_at.m == -INFINITY ? 0.0f : row_at.m) - float(dd);
+                    float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll 1
-                for (int ch = 0; ch < KT / 16; ++ch) {
-                    uint32_t x[16], p[8];
-                    tmem_ld_32x32b_x16(s_col + ch * 16, x);
-                    const uint32_t v = sees(ch >> 1) >> (16 * (ch & 1));
-                    tmem_wait_ld();
+                    for (int ch = 0; ch < KT / 16; ++ch) {
+                        uint32_t x[16], p[8];
+                        tmem_ld_32x32b_x16(s_col + ch * 16, x);
+                        const uint32_t v = pf_sees(row_lo - key0, row_hi - key0, miss, ch >> 1) >> (16 * (ch & 1));
+                        tmem_wait_ld();
 #pragma unroll
-                    for (int i = 0; i < 16; i += 2) {
-                        float e0 = kv4_ex2(fmaf(seen(x[i], v, i), ct, -mz));
-                        float e1 = kv4_ex2(fmaf(seen(x[i + 1], v, i + 1), ct, -mz));
-                        p[i / 2] = cvt_f16x2(e1, e0);
-                        pf_summand<T>(p[i / 2], &e0, &e1);
-                        sum[i & 2] += e0;
-                        sum[(i & 2) + 1] += e1;
+                        for (int i = 0; i < 16; i += 2) {
+                            float e0 = kv4_ex2(fmaf(pf_seen(x[i], v, i), ct, -mz));
+                            float e1 = kv4_ex2(fmaf(pf_seen(x[i + 1], v, i + 1), ct, -mz));
+                            p[i / 2] = cvt_f16x2(e1, e0);
+                            pf_summand<T>(p[i / 2], &e0, &e1);
+                            sum[i & 2] += e0;
+                            sum[(i & 2) + 1] += e1;
+                        }
+                        pf_tmem_st8(s_col + ch * 8, p);
                     }
-                    pf_tmem_st8(s_col + ch * 8, p);
+                    row_at.l = fmaf((sum[0] + sum[1]) + (sum[2] + sum[3]), pf_pow2(-dd), row_at.l);
                 }
-                l = fmaf((sum[0] + sum[1]) + (sum[2] + sum[3]), pf_pow2(-dd), l);
                 tmem_wait_st();
                 tc_fence_before();
                 __syncwarp();
@@ -823,7 +944,7 @@ __global__ void __launch_bounds__(pf_threads(DENSE), 1) kv4_prefill_kernel(const
             tc_fence_after();
             const bool whole = walk.st0 == 0 && walk.st1 == walk.hi - walk.lo;
             const size_t part = ((size_t)blockIdx.x * 2 + (walk.st0 == 0 ? 1 : 0)) * R + row;
-            const float back = pf_pow2(-ve);
+            const float m = row_at.m, l = row_at.l, back = pf_pow2(-row_at.ve);
             float f = back;
             if (whole) {
                 const float sink = kv4_sink(a.sinks, head), M = fmaxf(m, sink);
@@ -910,15 +1031,16 @@ __global__ void __launch_bounds__(pf_threads(DENSE), 1) kv4_prefill_kernel(const
         auto step_out = [&](const Held& h, int it, bool have) -> bool {
             const int st = it & 1;
             const uint32_t par = ((it >> 1) & 1) ^ 1;
-            float k_top = 0.0f, top = 0.0f, ks[J], kb[J], vs[J], vb[J];
+            float k_top = 0.0f, top = 0.0f, low = INFINITY, ks[J], kb[J], vs[J], vb[J];
             if (have) {
 #pragma unroll
                 for (int j = 0; j < J; ++j)
-                    pf_scales<T>(h.ks[j], h.kb[j], h.vs[j], h.vb[j], &ks[j], &kb[j], &vs[j], &vb[j], &k_top, &top);
+                    pf_scales<T>(h.ks[j], h.kb[j], h.vs[j], h.vb[j], &ks[j], &kb[j], &vs[j], &vb[j], &k_top, &top, &low);
             }
             top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top)));
             k_top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(k_top)));
-            if (lane == 0) bar.v_max[st][uw] = have ? top : -1.0f, bar.k_max[st][uw] = k_top;
+            low = __uint_as_float(__reduce_min_sync(0xffffffffu, __float_as_uint(low)));
+            if (lane == 0) bar.v_max[st][uw] = have ? top : -1.0f, bar.k_max[st][uw] = k_top, bar.v_min[st][uw] = low;
             named_barrier(1, PF_UNPACK * 32);  // (a slot is written again after the next step's barrier, which its readers pass later)
             float M = 0.0f;
             bool over = false;
@@ -927,6 +1049,7 @@ __global__ void __launch_bounds__(pf_threads(DENSE), 1) kv4_prefill_kernel(const
                 const float x = reinterpret_cast<volatile float*>(bar.v_max[st])[i];
                 M = fmaxf(M, x);
                 k_top = fmaxf(k_top, reinterpret_cast<volatile float*>(bar.k_max[st])[i]);
+                low = fminf(low, reinterpret_cast<volatile float*>(bar.v_min[st])[i]);
                 over = over || x < 0.0f;
             }
             if (over) return false;
@@ -934,8 +1057,18 @@ __global__ void __launch_bounds__(pf_threads(DENSE), 1) kv4_prefill_kernel(const
             const float kf = pf_pow2(ke);
             const int ve = pf_fit(M);
             const float vf = pf_pow2(ve);
+            const bool wild = pf_wild(low, M);  // (the same in all warps)
+            if (wild) {
+                const int me = uw * 32 + lane;
+                if (me < KT) bar.key_top[me] = 0;
+                named_barrier(1, PF_UNPACK * 32);
+#pragma unroll
+                for (int j = 0; j < J; ++j) pf_key_max(&bar.key_top[P::key(j, uw, lane)], vs[j], vb[j]);
+                named_barrier(1, PF_UNPACK * 32);
+                if (me < KT) bar.key_exp[it & 3][me] = pf_key_exp(bar.key_top[me]);
+            }
             if (uw == 0 && lane == 0) {
-                bar.exps[it & 3] = pf_exps(ke, M > 0.0f ? ve : PF_ANY);
+                bar.exps[it & 3] = pf_exps(ke, wild ? PF_WILD : M > 0.0f ? ve : PF_ANY);
                 bar.miss[it & 3] = bar.gone[it & 3];
             }
             __syncwarp();
@@ -948,7 +1081,10 @@ __global__ void __launch_bounds__(pf_threads(DENSE), 1) kv4_prefill_kernel(const
             if (lane == 0) mbar_arrive(&bar.k_full[st]);
             pf_wait(&bar.v_empty[st], par, abort);
 #pragma unroll
-            for (int j = 0; j < J; ++j) pf_unpack<D>(h.v[j], vs[j] * vf, vb[j] * vf, sv + st * S::TB, P::key(j, uw, lane), P::piece(j, uw, lane));
+            for (int j = 0; j < J; ++j) {
+                const float f = wild ? pf_pow2(pf_fit(__int_as_float(bar.key_top[P::key(j, uw, lane)]))) : vf;
+                pf_unpack<D>(h.v[j], vs[j] * f, vb[j] * f, sv + st * S::TB, P::key(j, uw, lane), P::piece(j, uw, lane));
+            }
             fence_proxy_async();
             __syncwarp();
             if (lane == 0) mbar_arrive(&bar.v_full[st]);
@@ -974,10 +1110,9 @@ __global__ void __launch_bounds__(pf_threads(DENSE), 1) kv4_prefill_kernel(const
             PfBars& bar = at.bar;
             volatile int* const abort = at.abort;
             const uint32_t sk = at.sk, sv = at.sv;
-            auto copy = [&](uint64_t* full, uint32_t dst, const uint8_t* src) {
-                mbar_arrive_expect_tx(full, S::TB);
+            auto copy = [&](uint64_t* full, uint32_t dst, const void* src, uint32_t bytes) {
                 asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
-                             "l"(src), "r"(S::TB), "r"(smem_u32(full))
+                             "l"(src), "r"(bytes), "r"(smem_u32(full))
                              : "memory");
             };
             int it = 0, keys = 0, values = 0;  // steps, copies
@@ -992,11 +1127,15 @@ __global__ void __launch_bounds__(pf_threads(DENSE), 1) kv4_prefill_kernel(const
                     if (*abort) break;
                     bar.exps[it & 3] = meta.x;
                     bar.miss[it & 3] = uint32_t(meta.y);
-                    copy(&bar.k_full[st], sk + st * S::TB, src);
+                    const bool wild = int16_t(meta.x) == PF_WILD;
+                    mbar_arrive_expect_tx(&bar.k_full[st], wild ? S::TB + KT : S::TB);
+                    copy(&bar.k_full[st], sk + st * S::TB, src, S::TB);
+                    if (wild) copy(&bar.k_full[st], smem_u32(bar.key_exp[it & 3]), a.dense_keys + (tile0 + t) * KT, KT);
                     ++keys;
                     pf_wait(&bar.v_empty[st], par, abort);
                     if (*abort) break;
-                    copy(&bar.v_full[st], sv + st * S::TB, src + S::TB);
+                    mbar_arrive_expect_tx(&bar.v_full[st], S::TB);
+                    copy(&bar.v_full[st], sv + st * S::TB, src + S::TB, S::TB);
                     ++values;
                 }
             }
@@ -1156,7 +1295,7 @@ static bool pf_dense(int D, int B, int KVH, int G, int max_q, long long room, si
     const int R = D == 256 ? 128 : 256, KT = D == 256 ? 64 : 128;
     const long long n = (room + KT - 1) / KT, tiles = n * B * KVH;
     *steps = int(n);
-    *bytes = size_t(tiles) * (size_t(4) * KT * D + sizeof(int2));
+    *bytes = size_t(tiles) * (size_t(4) * KT * D + KT + sizeof(int2));
     return (long long)max_q * G > 2 * R && tiles <= (1LL << 30) / (4LL * KT * D) && B <= 65535 && KVH <= 65535;
 }
 
@@ -1186,11 +1325,16 @@ static int kv4_prefill_d(Kv4AttArgs a, void* workspace, cudaStream_t st) {
     a.part_ml = a.part_o + size_t(n) * 2 * S::R * D;
     a.records = reinterpret_cast<int32_t*>(a.part_ml + size_t(n) * 2 * S::R * 2);
     size_t bytes;
-    const size_t smem = S::SMEM + 1024 + sizeof(PfBars);
+    const size_t smem = S::SMEM + sizeof(PfBars);
+    // One CTA a SM, but within 196 KB with the static arrays and what the system keeps: beyond, the rest of the SM's 256 KB
+    // that is left to the L1 falls from 60 KB to 28, less than the stacks (a 4096-token prompt piece 1137 -> 1290 us).
+    static_assert(S::SMEM + sizeof(PfBars) + 2 * 1024 <= 196 * 1024, "shared memory");
     int rc;
     if (pf_dense(D, a.B, a.pool.KVH, a.G, a.max_q, (long long)a.width * a.pool.page, &bytes, &a.dense_steps)) {
         a.dense = static_cast<uint8_t*>(workspace) + pf_parts_bytes(D, n);
-        a.dense_meta = reinterpret_cast<int2*>(a.dense + size_t(a.dense_steps) * a.B * a.pool.KVH * 2 * S::TB);
+        const size_t tiles = size_t(a.dense_steps) * a.B * a.pool.KVH;
+        a.dense_keys = reinterpret_cast<int8_t*>(a.dense + tiles * 2 * S::TB);
+        a.dense_meta = reinterpret_cast<int2*>(a.dense_keys + tiles * S::KT);
         rc = kv4_launch(kv4_dense_kernel<T, D>, set_first, dim3(a.dense_steps, a.pool.KVH, a.B), dim3(PD_WARPS * 32),
                         2 * S::TB + 128, st, a);
         if (!rc) rc = kv4_launch(kv4_prefill_kernel<T, D, true>, set_dense, dim3(n), dim3(pf_threads(true)), smem, st, a);

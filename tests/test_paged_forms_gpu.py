@@ -207,3 +207,9 @@ def _out_of_sight(cuda, form, new, H, KVH, D, columns, e):
 @pytest.mark.parametrize("form,new,H,KVH,D,columns", [x for x in EACH if x[0] in (CLUSTERS, SPLIT)])
 def test_large_values_out_of_sight(cuda, form, new, H, KVH, D, columns, e):
     _out_of_sight(cuda, form, new, H, KVH, D, columns, e)
+
+
+@pytest.mark.parametrize("e", [10, 20, 60, 100])
+@pytest.mark.parametrize("form,new,H,KVH,D,columns", [x for x in EACH if x[0] in (TILES, DENSE)])
+def test_large_values_out_of_sight_of_many_rows(cuda, form, new, H, KVH, D, columns, e):
+    _out_of_sight(cuda, form, new, H, KVH, D, columns, e)
