@@ -106,19 +106,8 @@ def _compile(unit, verbose):
     return obj, r.stderr
 
 
-def _ext_hash() -> str:
-    import torch
-
-    return _digest([EXT_SRC, HEADER], torch.__version__)
-
-
-def build_ext(force: bool = False) -> str:
-    """_paged_ext.so, rebuilt when its source, include/lq.h or the torch version changes."""
-    want = _ext_hash()
-    if not force and os.path.exists(EXT) and os.path.exists(EXT_HASH):
-        with open(EXT_HASH) as f:
-            if f.read().strip() == want:
-                return EXT
+def _ext_command(out: str) -> list:
+    """The host compiler's command line for _paged_ext.so."""
     import sysconfig
 
     import torch
@@ -127,13 +116,46 @@ def build_ext(force: bool = False) -> str:
     cuda = os.path.dirname(os.path.dirname(os.path.realpath(NVCC)))
     includes = [*cpp_extension.include_paths(), sysconfig.get_paths()["include"], os.path.join(cuda, "include")]
     libs = os.path.join(os.path.dirname(torch.__file__), "lib")
-    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
-           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *[f"-I{p}" for p in includes], EXT_SRC,
-           "-o", EXT + ".tmp", f"-L{libs}", "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_cuda",
-           f"-L{HERE}", "-l:liblq.so", "-Wl,-rpath,$ORIGIN"]
-    r = subprocess.run(cmd, capture_output=True, text=True)
-    if r.returncode != 0:
-        raise RuntimeError(f"{cmd[0]} failed on {os.path.basename(EXT_SRC)}:\n{r.stdout}\n{r.stderr}")
+    return [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *[f"-I{p}" for p in includes], EXT_SRC,
+            "-o", out, f"-L{libs}", "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_cuda",
+            f"-L{HERE}", "-l:liblq.so", "-Wl,-rpath,$ORIGIN"]
+
+
+def _ext_hash(cmd) -> str:
+    """Hash of what _paged_ext.so is made of and for: its source and header, the interpreter, torch, compiler and flags."""
+    import torch
+
+    made = [sys.implementation.cache_tag, torch.__version__, _version(cmd[0]), *cmd]
+    return _digest([EXT_SRC, HEADER], "\n".join(made))
+
+
+def _version(compiler: str) -> str:
+    try:
+        return subprocess.run([compiler, "--version"], capture_output=True, text=True).stdout
+    except OSError:
+        return ""
+
+
+def build_ext(force: bool = False) -> str:
+    """_paged_ext.so, rebuilt when its source, include/lq.h, the interpreter, torch, the compiler or its flags change. One that
+    does not compile leaves none behind, not an older one either."""
+    cmd = _ext_command(EXT + ".tmp")
+    want = _ext_hash(cmd)
+    if not force and os.path.exists(EXT) and os.path.exists(EXT_HASH):
+        with open(EXT_HASH) as f:
+            if f.read().strip() == want:
+                return EXT
+    for old in (EXT, EXT_HASH):
+        if os.path.exists(old):
+            os.remove(old)
+    try:
+        r = subprocess.run(cmd, capture_output=True, text=True)
+        why = f"{r.stdout}\n{r.stderr}" if r.returncode != 0 else ""
+    except OSError as e:
+        why = str(e)
+    if why:
+        raise RuntimeError(f"{cmd[0]} failed on {os.path.basename(EXT_SRC)}:\n{why}")
     os.replace(EXT + ".tmp", EXT)
     with open(EXT_HASH, "w") as f:
         f.write(want)
