@@ -163,8 +163,13 @@ def build_ext(force: bool = False) -> str:
 
 
 def build(force: bool = False, verbose: bool = False) -> str:
+    """liblq.so, and _paged_ext.so where it compiles: without it (no Python headers, say) all but paged.py and rotary.py
+    works, and those say what is missing."""
     lib = _build_lib(force, verbose)
-    build_ext(force)
+    try:
+        build_ext(force)
+    except RuntimeError as e:
+        print(f"_paged_ext.so is not built, paged.py and rotary.py will not run: {e}", file=sys.stderr)
     return lib
 
 
