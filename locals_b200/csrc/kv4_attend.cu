@@ -19,7 +19,7 @@
 //     values 2^-27 below the row's largest. A row by itself: the tile holds other heads and other tokens of the request;
 //   w to fp16 (2^-11 against the 2^-8 of a bf16 output; an fp16 output's error grows from 2.0e-4 to 2.2e-4 by it), after a
 //     power of two a row that puts the largest value scale that the row has seen at 2^5 .. 2^10 (vf for the warp, a row's
-//     difference from it, xl, in its probabilities). codes - z (exact on subnormals, one packed subtraction a pair) takes out of a group
+//     difference from it, xl, in its probabilities): values are held to 2^-30 of the largest that the row sees. codes - z (exact on subnormals, one packed subtraction a pair) takes out of a group
 //     what its codes and its bias have in common, so that this is a rounding of the value itself, however near to 0 it lies.
 // A score tile's accumulator layout is transposed into the value MMA's operand by movmatrix. The running maximum of a row is
 // only followed when it has grown by 2^4, so that most steps rescale nothing.
@@ -37,9 +37,11 @@
 //
 // What bounds it. The bytes are (D + D / 8) a key and kv head (144 at D = 128); the instructions are about 730 a warp and 32
 // keys (unpacking 200, z 64, MMAs 48, the rest loads, scales and softmax), and they are what the time goes to: 2.3 a clock
-// and SM, the ALU pipe 48% busy, tensor pipe 22%. Measured, GPU time of a call: 4 requests of 131,072 keys, 32 heads on 4,
-// D = 128, fp16: 81.7 us = 3.70 TB/s (56% of the copy rate); 64 requests of up to 8,191 keys, 32 heads on 4, bf16: 53.5 us =
-// 2.88 TB/s; one request of 1,001 keys: 8.4 us (launch, one pass of dependent loads, two cluster barriers).
+// and SM, the ALU pipe 47% busy, tensor pipe 21%: no pipe is full, a step's chain (scales, z, scores, maximum, exponentials,
+// values) waits on itself. Measured, GPU time of a call: 4 requests of 131,072 keys, 32 heads on 4, D = 128, fp16: 81.9 us =
+// 3.69 TB/s (56% of the copy rate); 64 requests of up to 8,191 keys, 32 heads on 4, bf16: 54.6 us = 2.83 TB/s; one request of
+// 1,001 keys: 6.9 us among others (launch, one pass of dependent loads, two cluster barriers). A power of two a row, for the
+// queries and for the values, is 0.6 us of that, 1.2 of 54.6 and 2.4 of 81.9.
 // Tried and slower: 4 CTAs a SM at 128 registers (89.6 against 83.3 us, it spills), 5 (126); a ring of 2 stages is as fast
 // as 3 at D = 128.
 #include <cuda_bf16.h>

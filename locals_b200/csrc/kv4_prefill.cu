@@ -11,7 +11,7 @@
 //     for two query tiles in turn, S0 PV0 S1 PV1 ..., so that one tile's softmax runs beside the other's products;
 //   * each of 256 threads owns a row: it reads its scores, keeps the running maximum and sum in fp32, and writes its
 //     probabilities back over them as fp16. The row's output is only rescaled when its maximum has grown by 2^8; until then a
-//     step is one pass over the scores (`once`), its probabilities in registers.
+//     step is one pass over the scores (`once`), its probabilities in registers. (Both are published methods.)
 // Two forms, by how often a key is met again (pf_dense):
 //   * unpacked in place: eight warps unpack, one step ahead through registers, told by a page warp where the keys lie; the
 //     registers of the block are shared out by role (setmaxnreg);
@@ -27,18 +27,22 @@
 // probabilities are multiplied by the difference while that is small, its outputs (as its maximum's growth does) where it
 // is not: so a step's values cost another step's no bits, and a row only those of the keys that it sees. A step with keys
 // whose values are 2^-16 of the largest or less has one a key (PF_WILD; key_exp), which each row's probabilities take in, in
-// the two-pass step: the large ones may be out of a row's sight. Within a key, values are held to 2^-35 of its largest.
+// the two-pass step: the large ones may be out of a row's sight. Within a key, values are held to 2^-35 of its largest, and
+// probabilities to 2^-25 of the row's largest.
 // A masked score is -inf, its probability 0; a value whose scale or bias is not finite is held as 0 and its key as NaN,
 // so that only rows that see it become NaN.
 // Work is dealt out as in kv4_attend.cu: the steps of all tiles (each as far as its last row sees) evenly over one CTA a
 // SM, parts joined by kv4_prefill_join_kernel.
 // What bounds it: 4 D operations a row and key on the tensor cores, and one exponential a row and key at 16 a clock and SM,
-// which take as long as the products do at D = 128. Measured, GPU time of a call, bf16: 4,096 new tokens on 28,672 cached,
-// 16 heads on 2, D = 128: 1,016 to 1,020 us = 1,012 TFLOP/s (62% of the measured peak; 1,081 before the one pass); a mixed
-// batch of 8 (1 to 1,024 new on up to 2,048 cached, 32 heads on 8): 177 us = 543 TFLOP/s, the items' ends and short tiles;
-// 16 requests of 5 drafted tokens on up to 4,003 keys, 16 heads on 2, D = 256: 42.2 us, latency: 4 us to find the share, 6
-// to fetch the queries, 2 to 8 steps, 2 to write, and the joins.
+// which take as long as the products do at D = 128 (tensor pipe 48% busy, exponentials 48%: they are not yet beside each
+// other all the time). Measured, GPU time of a call, bf16: 4,096 new tokens on 28,672 cached, 16 heads on 2, D = 128: 1,066 to
+// 1,143 us = 902 to 967 TFLOP/s by the clock that the power limit leaves (55 to 59% of the measured peak), fp16 1,210 to 1,271;
+// a mixed batch of 8 (1 to 1,024 new on up to 2,048 cached, 32 heads on 8): 193 us = 498 TFLOP/s, the items' ends and short
+// tiles; 16 requests of 5 drafted tokens on up to 4,003 keys, 16 heads on 2, D = 256: 50 to 52 us, latency: 4 us to find the
+// share, 6 to fetch the queries, 2 to 8 steps, 2 to write, and the joins. The powers of two a step, row and key take 2 to 5% of
+// these (bf16) and 9% of the fp16 piece.
 // Tried and slower: half the exponentials as polynomials (1,128 against 1,081 us); 4 unpacking warps of 128 registers (1,778);
+// the two-pass step out of line (a mixed batch 245 against 200); a row's powers of two in shared memory (no faster);
 // 48 registers for the issuing warp (1,904); query rows fetched by neighbouring lanes (no faster, and 1,061 against 1,029).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>

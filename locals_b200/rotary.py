@@ -15,7 +15,9 @@ from ._lib import ext
 
 
 def tables(positions: int, rot: int, base: float = 10000.0, device="cuda") -> Tuple[torch.Tensor, torch.Tensor]:
-    """cos and sin (positions, rot / 2) float32 of position * base^(-2 j / rot), computed in 64 bits."""
+    """cos and sin (positions, rot / 2) float32 of position * base^(-2 j / rot), computed in 64 bits: one run of frequencies
+    over all pairs, whatever their axes. Where an axis' pairs start the run anew, join the axes' own tables along the pairs
+    (``torch.cat([tables(n, 2 * pairs_of_axis)[0], ...], 1)``)."""
     inv = base ** (-torch.arange(0, rot, 2, dtype=torch.float64) / rot)
     angle = torch.arange(positions, dtype=torch.float64)[:, None] * inv
     return angle.cos().float().to(device), angle.sin().float().to(device)
