@@ -21,13 +21,13 @@
 // Roundings to fp16: queries after a power of two a row (exact for bf16 but for values 2^-26 below the row's largest); keys,
 // values and probabilities, 2^-11 each against the 2^-8 of a bf16 output (an fp16 output's error against 64 bits grows by
 // them from 2.1e-4 to 3.2e-4 .. 4.0e-4 of its size: the tensor cores take the operands in no finer type but at half the
-// rate). Keys after a power of two a step that puts the largest that its groups can hold at 2^13 .. 2^14, taken back with the
-// scores' factor: a group's scale and a sixteenth of it stay normal numbers down to 2^-19 of that, where the group's share of
+// rate). Keys after a power of two a step that puts the largest that its groups can hold at 2^14 .. 2^15, taken back with the
+// scores' factor: a group's scale and a sixteenth of it stay normal numbers down to 2^-20 of that, where the group's share of
 // a score is as small. Values after a power of two a step in the same way; a row's outputs have one of their own, and its
 // probabilities are multiplied by the difference while that is small, its outputs (as its maximum's growth does) where it
 // is not: so a step's values cost another step's no bits, and a row only those of the keys that it sees. A step with keys
-// whose values are 2^-16 of the largest or less has one a key (PF_WILD; key_exp), which each row's probabilities take in, in
-// the two-pass step: the large ones may be out of a row's sight. Within a key, values are held to 2^-35 of its largest, and
+// whose values are 2^-20 of the largest or less has one a key (PF_WILD; key_exp), which each row's probabilities take in, in
+// the two-pass step: the large ones may be out of a row's sight. Within a key, values are held to 2^-31 of its largest, and
 // probabilities to 2^-25 of the row's largest.
 // A masked score is -inf, its probability 0; a value whose scale or bias is not finite is held as 0 and its key as NaN,
 // so that only rows that see it become NaN.
@@ -334,9 +334,14 @@ __device__ __forceinline__ void pf_unpack(const uint4& codes, float s, float b, 
     }
 }
 
+// (Down to 2^-20 of a step's largest, a value's rounding and its scales' are below 2^-11. What holds less than PF_LEAST is not
+// asked for: groups and tokens of zeros, to which the quantizer gives scales of 1e-7.)
+constexpr float PF_LEAST = 0x1p-19f;
+__device__ __forceinline__ bool pf_wild(float least, float most) { return least < most * 0x1p-20f; }
+
 // A piece's scales and biases in fp32. A value scale or bias that is not finite makes the values 0 and the key NaN, which
 // only the rows that see it meet; so does an infinite key. Adds the largest |key| and |value| that the groups can hold, and
-// the least that is not 0 of the values'.
+// the least of the values' (from PF_LEAST on).
 template <typename T>
 __device__ __forceinline__ void pf_scales(uint16_t ks16, uint16_t kb16, uint16_t vs16, uint16_t vb16, float* ks, float* kb,
                                           float* vs, float* vb, float* k_top, float* v_top, float* v_low) {
@@ -349,21 +354,31 @@ __device__ __forceinline__ void pf_scales(uint16_t ks16, uint16_t kb16, uint16_t
         return;
     }
     *v_top = fmaxf(*v_top, v_most);
-    if (v_most > 0.0f) *v_low = fminf(*v_low, v_most);
+    if (v_most >= PF_LEAST) *v_low = fminf(*v_low, v_most);
     if (k_most < INFINITY) *k_top = fmaxf(*k_top, k_most);
 }
 // 2^e, e in -126 .. 127.
 __device__ __forceinline__ float pf_pow2(int e) { return __uint_as_float(uint32_t(127 + e) << 23); }
-// The power of two that puts M at 2^13 .. 2^14 (at least -114; 0 for 0).
-__device__ __forceinline__ int pf_fit(float M) { return M > 0.0f ? min(13 - (int(__float_as_uint(M) >> 23) - 127), 120) : 0; }
+// The power of two that puts M at 2^14 .. 2^15 (at least -113; 0 for 0).
+__device__ __forceinline__ int pf_fit(float M) { return M > 0.0f ? min(14 - (int(__float_as_uint(M) >> 23) - 127), 120) : 0; }
 // The powers of two of a step's keys and values in one word.
 __device__ __forceinline__ int pf_exps(int ke, int ve) { return int(uint32_t(ke) << 16 | (uint32_t(ve) & 0xffffu)); }
 // The values' of a step (or key) that holds none but zeros: any; and of a step whose keys have one each.
 constexpr int PF_ANY = 127, PF_WILD = 126;
-__device__ __forceinline__ bool pf_wild(float least, float most) { return least < most * 0x1p-16f; }
 __device__ __forceinline__ int8_t pf_key_exp(int top) { return int8_t(top ? pf_fit(__int_as_float(top)) : PF_ANY); }
-// A key's values' power of two from its largest (a finite |value| group): bits of an int are in a float's order.
+// A key's largest from its groups' (the bits of floats from 0 on are in their order).
 __device__ __forceinline__ void pf_key_max(int* top, float vs, float vb) { atomicMax(top, __float_as_int(fmaf(15.0f, fabsf(vs), fabsf(vb)))); }
+// Whether keys differ so widely, and not only a key's groups (a head of 64 dimensions in a place of 128): asked of whole warps.
+template <int KT>
+__device__ __forceinline__ bool pf_wild_keys(const int* top, float most) {
+    unsigned least = 0x7f800000u;
+#pragma unroll
+    for (int k = threadIdx.x & 31; k < KT; k += 32) {
+        const unsigned x = unsigned(*reinterpret_cast<const volatile int*>(top + k));
+        if (x >= unsigned(__float_as_uint(PF_LEAST))) least = min(least, x);
+    }
+    return pf_wild(__uint_as_float(__reduce_min_sync(0xffffffffu, least)), most);
+}
 // How far a row's outputs may lie from a step's values before they are multiplied: probabilities, at most 2^8, times 2^6 are
 // within fp16; times 2^-4, those below 2^-10 begin to lose bits, of values that are 2^-4 as large.
 constexpr int PF_UP = 6, PF_DOWN = -4;  // (ve is at most 120)
@@ -434,12 +449,13 @@ __global__ void __launch_bounds__(PD_WARPS * 32) kv4_dense_kernel(const Kv4AttAr
         low = fminf(low, low_part[i]);
     }
     const size_t at = ((size_t)b * a.pool.KVH + kvh) * a.dense_steps + s;
-    const bool wild = pf_wild(low, top);
+    bool wild = pf_wild(low, top);
     if (wild) {
 #pragma unroll
         for (int j = 0; j < P::J; ++j) pf_key_max(&key_top[P::key(j, warp, lane)], vs[j], vb[j]);
         __syncthreads();
-        if (threadIdx.x < S::KT) a.dense_keys[at * S::KT + threadIdx.x] = pf_key_exp(key_top[threadIdx.x]);
+        wild = pf_wild_keys<S::KT>(key_top, top);
+        if (wild && threadIdx.x < S::KT) a.dense_keys[at * S::KT + threadIdx.x] = pf_key_exp(key_top[threadIdx.x]);
     }
     const int ke = pf_fit(k_top);
     const float kf = pf_pow2(ke);
@@ -812,9 +828,12 @@ __global__ void __launch_bounds__(pf_threads(DENSE), 1) kv4_prefill_kernel(const
                 const int key0 = (walk.lo + walk.st0 + t) * KT;
                 const uint32_t miss = *reinterpret_cast<volatile uint32_t*>(&bar.miss[it & 3]);
                 // How far the row's outputs lie from the step's values: its probabilities are multiplied by 2^that. (Below PF_DOWN
-                // for PF_ANY and PF_WILD. Read where it is used: the one pass needs the registers.)
+                // for PF_WILD. Read where it is used: the one pass needs the registers.)
                 auto exps = [&]() { return *reinterpret_cast<volatile int*>(&bar.exps[it & 3]); };
-                auto apart = [&]() { return row_at.ve - int(int16_t(exps())); };
+                auto apart = [&]() {
+                    const int ve_t = int16_t(exps());
+                    return ve_t == PF_ANY ? 0 : row_at.ve - ve_t;
+                };
                 const bool all = key0 >= lo_all && key0 + KT <= hi_all && miss == 0;
                 const uint32_t s_col = tmem + lanes + buf * KT;
                 // One query tile: a step's scores are issued before the last step's product, so that without this a warp could
@@ -1061,7 +1080,7 @@ __global__ void __launch_bounds__(pf_threads(DENSE), 1) kv4_prefill_kernel(const
             const float kf = pf_pow2(ke);
             const int ve = pf_fit(M);
             const float vf = pf_pow2(ve);
-            const bool wild = pf_wild(low, M);  // (the same in all warps)
+            bool wild = pf_wild(low, M);  // (the same in all warps)
             if (wild) {
                 const int me = uw * 32 + lane;
                 if (me < KT) bar.key_top[me] = 0;
@@ -1069,7 +1088,8 @@ __global__ void __launch_bounds__(pf_threads(DENSE), 1) kv4_prefill_kernel(const
 #pragma unroll
                 for (int j = 0; j < J; ++j) pf_key_max(&bar.key_top[P::key(j, uw, lane)], vs[j], vb[j]);
                 named_barrier(1, PF_UNPACK * 32);
-                if (me < KT) bar.key_exp[it & 3][me] = pf_key_exp(bar.key_top[me]);
+                wild = pf_wild_keys<KT>(bar.key_top, M);
+                if (wild && me < KT) bar.key_exp[it & 3][me] = pf_key_exp(bar.key_top[me]);
             }
             if (uw == 0 && lane == 0) {
                 bar.exps[it & 3] = pf_exps(ke, wild ? PF_WILD : M > 0.0f ? ve : PF_ANY);

@@ -213,3 +213,29 @@ def test_large_values_out_of_sight(cuda, form, new, H, KVH, D, columns, e):
 @pytest.mark.parametrize("form,new,H,KVH,D,columns", [x for x in EACH if x[0] in (TILES, DENSE)])
 def test_large_values_out_of_sight_of_many_rows(cuda, form, new, H, KVH, D, columns, e):
     _out_of_sight(cuda, form, new, H, KVH, D, columns, e)
+
+
+@FORMS
+@pytest.mark.parametrize("what", ["a group of each head", "every 37th token", "all"])
+@pytest.mark.parametrize("least", [0.0, 1e-7])
+def test_values_of_zero(cuda, form, new, H, KVH, D, columns, what, least):
+    """Values that are 0, with scales of 0 or the quantizer's least: heads that fill half of their place, tokens of none."""
+    import torch
+    from locals_b200 import paged
+
+    n = 500
+    _, (q, keys, values, table, qs, scale, _) = _one(cuda, form, new, n, H, KVH, D, columns, seed=33)
+    w, s, b = (t.clone() for t in values)
+    if what == "a group of each head":
+        w[..., -8:], s[..., -1], b[..., -1] = 0, least, 0
+    else:
+        places = range(0, n, 37) if what == "every 37th token" else range(n)
+        for j in places:
+            at = int(table[0, j // 16]), slice(None), j % 16
+            w[at], s[at], b[at] = 0, least, 0
+    got = paged.attend(q, keys, (w, s, b), table, _i32([n], cuda), scale, q_start=qs, max_q=new)
+    ref, bound = R.attended(q, keys, (w, s, b), table, _i32([n], cuda), scale, qs, None, 0)
+    assert bool(((got.double() - ref).abs() <= bound).all())
+    if what == "all":
+        assert torch.count_nonzero(got).item() == 0
+    assert _status() == 0
