@@ -28,7 +28,7 @@
 // is not: so a step's values cost another step's no bits, and a row only those of the keys that it sees. A step with keys
 // whose values are 2^-20 of the largest or less has one a key (PF_WILD; key_exp), which each row's probabilities take in, in
 // the two-pass step: the large ones may be out of a row's sight. Within a key, values are held to 2^-31 of its largest, and
-// probabilities to 2^-25 of the row's largest.
+// probabilities to 2^-31 of the row's largest.
 // A masked score is -inf, its probability 0; a value whose scale or bias is not finite is held as 0 and its key as NaN,
 // so that only rows that see it become NaN.
 // Work is dealt out as in kv4_attend.cu: the steps of all tiles (each as far as its last row sees) evenly over one CTA a
@@ -360,7 +360,7 @@ __device__ __forceinline__ void pf_scales(uint16_t ks16, uint16_t kb16, uint16_t
 // 2^e, e in -126 .. 127.
 __device__ __forceinline__ float pf_pow2(int e) { return __uint_as_float(uint32_t(127 + e) << 23); }
 // The power of two that puts M at 2^14 .. 2^15 (at least -113; 0 for 0).
-__device__ __forceinline__ int pf_fit(float M) { return M > 0.0f ? min(14 - (int(__float_as_uint(M) >> 23) - 127), 120) : 0; }
+__device__ __forceinline__ int pf_fit(float M) { return M > 0.0f ? min(14 - (int(__float_as_uint(M) >> 23) - 127), 110) : 0; }
 // The powers of two of a step's keys and values in one word.
 __device__ __forceinline__ int pf_exps(int ke, int ve) { return int(uint32_t(ke) << 16 | (uint32_t(ve) & 0xffffu)); }
 // The values' of a step (or key) that holds none but zeros: any; and of a step whose keys have one each.
@@ -379,9 +379,12 @@ __device__ __forceinline__ bool pf_wild_keys(const int* top, float most) {
     }
     return pf_wild(__uint_as_float(__reduce_min_sync(0xffffffffu, least)), most);
 }
-// How far a row's outputs may lie from a step's values before they are multiplied: probabilities, at most 2^8, times 2^6 are
-// within fp16; times 2^-4, those below 2^-10 begin to lose bits, of values that are 2^-4 as large.
-constexpr int PF_UP = 6, PF_DOWN = -4;  // (ve is at most 120)
+// Probabilities are held 2^PF_BIAS times as large, so that fp16 has those down to 2^-20 of the row's largest in full, and
+// 2^-31 of it at least. Their upper end leaves room for a maximum that has grown by 2^PF_LAG since the row's reference and for
+// outputs that lie 2^PF_UP from a step's values, 2^15 in all; 2^PF_DOWN costs small ones bits, of values that are as much smaller.
+// Beyond these a row gets a new reference or power of two, which takes the step's scores twice (PF_LAG 5: a mixed batch 231 us
+// against 192).
+constexpr int PF_BIAS = 6, PF_LAG = 8, PF_UP = 1, PF_DOWN = -4;  // (a power of two of values is at most 110)
 
 // ---- the dense form's first pass: the keys and values of requests with many tiles, unpacked once ----
 // One CTA a (step of KT keys, kv head, request): the step's two tiles as they are to lie in shared memory, copied out whole,
@@ -504,7 +507,7 @@ struct PfRow {
 };
 
 // A new maximum mn, and, of a step that gives one (sized), a new power of two of the outputs: the step's, but no more than 2^64
-// above the least of the steps' before, whose sums (below 2^43) then stay within 32 bits' range. Returns what the outputs are
+// above the least of the steps' before, whose sums (below 2^50) then stay within 32 bits' range. Returns what the outputs are
 // multiplied by.
 __device__ __forceinline__ float pf_refit(PfRow& row, float mn, int ve_t, bool sized) {
     int to = row.ve;
@@ -551,7 +554,7 @@ __device__ __noinline__ PfRow pf_wild_step(PfRow row, PfBars* bars, int it, int 
     const float mn = fmaxf(row.m, mx * ct);
     const bool some = mx != -INFINITY;
     const int d = row.ve - ve_t;
-    const bool grow = mn > row.m + 8.0f || (row.m == -INFINITY && mn > row.m) || (some && (d < PF_DOWN || d > PF_UP));
+    const bool grow = mn > row.m + PF_LAG || (row.m == -INFINITY && mn > row.m) || (some && (d < PF_DOWN || d > PF_UP));
     if (__any_sync(0xffffffffu, grow)) {
         const float corr = pf_refit(row, mn, ve_t, some && sized);
         if (before) {
@@ -580,10 +583,10 @@ __device__ __noinline__ PfRow pf_wild_step(PfRow row, PfBars* bars, int it, int 
         for (int i = 0; i < 16; i += 2) {
             const float e0 = kv4_ex2(fmaf(pf_seen(x[i], v, i), ct, -mz));
             const float e1 = kv4_ex2(fmaf(pf_seen(x[i + 1], v, i + 1), ct, -mz));
-            // (the large ones' probabilities are at most 2^8 times 2^PF_UP, the small ones' may become 0 beside them)
+            // (the small ones' may become 0 beside the large ones')
             const uint32_t k = lds32(key_exp + ch * 16 + (i & ~3)) >> (8 * (i & 2));
-            p[i / 2] = cvt_f16x2(e1 * pf_pow2(min(max(row.ve - int(int8_t(k >> 8)), -126), 100)),
-                                 e0 * pf_pow2(min(max(row.ve - int(int8_t(k)), -126), 100)));
+            p[i / 2] = cvt_f16x2(e1 * pf_pow2(min(max(row.ve - int(int8_t(k >> 8)) + PF_BIAS, -126), 100)),
+                                 e0 * pf_pow2(min(max(row.ve - int(int8_t(k)) + PF_BIAS, -126), 100)));
             sum[i & 2] += e0;
             sum[(i & 2) + 1] += e1;
         }
@@ -845,7 +848,7 @@ __global__ void __launch_bounds__(pf_threads(DENSE), 1) kv4_prefill_kernel(const
                 // The common case, one pass: the reference from the steps before serves the step (found out at its end: the
                 // probabilities stay in registers until then, the scores in place).
                 auto once = [&](auto masked) -> bool {
-                    const float ct = pf_factor(c, exps()), md = float(apart()) - row_at.m;
+                    const float ct = pf_factor(c, exps()), md = float(apart() + PF_BIAS) - row_at.m;
                     const uint64_t c2 = pf_pair(ct, ct), m2 = pf_pair(md, md);
                     constexpr int CH = 16;  // scores at a time (32: 1082 against 1040 us for a 4096-token prompt piece)
                     uint32_t r[2][CH], p[KT / 2];
@@ -874,13 +877,13 @@ __global__ void __launch_bounds__(pf_threads(DENSE), 1) kv4_prefill_kernel(const
                             p[(ch * CH + i) / 2] = h;
                         }
                     }
-                    if (__any_sync(0xffffffffu, fmaxf(mx[0], mx[1]) * ct > row_at.m + 8.0f)) return false;
+                    if (__any_sync(0xffffffffu, fmaxf(mx[0], mx[1]) * ct > row_at.m + PF_LAG)) return false;
 #pragma unroll
                     for (int ch = 0; ch < KT / 64; ++ch) pf_tmem_st32(s_col + ch * 32, &p[ch * 32]);
                     float a0, a1, b0, b1;
                     pf_unpair(sums[0], &a0, &a1);
                     pf_unpair(sums[1], &b0, &b1);
-                    row_at.l = fmaf((a0 + a1) + (b0 + b1), pf_pow2(-apart()), row_at.l);
+                    row_at.l = fmaf((a0 + a1) + (b0 + b1), pf_pow2(-apart() - PF_BIAS), row_at.l);
                     tmem_wait_st();
                     tc_fence_before();
                     __syncwarp();
@@ -915,7 +918,7 @@ __global__ void __launch_bounds__(pf_threads(DENSE), 1) kv4_prefill_kernel(const
                     const float mn = fmaxf(row_at.m, mx * ct);
                     const bool some = mx != -INFINITY;
                     const int d = row_at.ve - ve_t;
-                    const bool grow = mn > row_at.m + 8.0f || (row_at.m == -INFINITY && mn > row_at.m) || (some && (d < PF_DOWN || d > PF_UP));
+                    const bool grow = mn > row_at.m + PF_LAG || (row_at.m == -INFINITY && mn > row_at.m) || (some && (d < PF_DOWN || d > PF_UP));
                     if (__any_sync(0xffffffffu, grow)) {
                         const float corr = pf_refit(row_at, mn, ve_t, some && sized);
                         if (t > 0) {
@@ -934,7 +937,7 @@ __global__ void __launch_bounds__(pf_threads(DENSE), 1) kv4_prefill_kernel(const
                     }
                     // (below PF_DOWN only after so large values that this step's are nothing beside them: their probabilities are 0
                     // in fp16, and still in the row's sum; and beyond PF_UP only in rows that see nothing of the step)
-                    const int dd = min(max(row_at.ve - ve_t, -60), 60);
+                    const int dd = min(max(row_at.ve - ve_t, -60), 60) + PF_BIAS;
                     const float mz = (row_at.m == -INFINITY ? 0.0f : row_at.m) - float(dd);
                     float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll 1
@@ -967,7 +970,7 @@ __global__ void __launch_bounds__(pf_threads(DENSE), 1) kv4_prefill_kernel(const
             tc_fence_after();
             const bool whole = walk.st0 == 0 && walk.st1 == walk.hi - walk.lo;
             const size_t part = ((size_t)blockIdx.x * 2 + (walk.st0 == 0 ? 1 : 0)) * R + row;
-            const float m = row_at.m, l = row_at.l, back = pf_pow2(-row_at.ve);
+            const float m = row_at.m, l = row_at.l, back = pf_pow2(-row_at.ve - PF_BIAS);
             float f = back;
             if (whole) {
                 const float sink = kv4_sink(a.sinks, head), M = fmaxf(m, sink);

@@ -239,3 +239,23 @@ def test_values_of_zero(cuda, form, new, H, KVH, D, columns, what, least):
     if what == "all":
         assert torch.count_nonzero(got).item() == 0
     assert _status() == 0
+
+
+@FORMS
+@pytest.mark.parametrize("least", [0.0, 1e-7])
+def test_values_of_one_token(cuda, form, new, H, KVH, D, columns, least):
+    """All values are 0 but the first token's: outputs are its weight times its values, however small the weight (to 2^-20 of the
+    row's largest; from there 2^-31 of it a value)."""
+    import torch
+    from locals_b200 import paged
+
+    n = 500
+    _, (q, keys, values, table, qs, scale, _) = _one(cuda, form, new, n, H, KVH, D, columns, seed=33)
+    w, s, b = (t.clone() for t in values)
+    for j in range(1, n):
+        at = int(table[0, j // 16]), slice(None), j % 16
+        w[at], s[at], b[at] = 0, least, 0
+    got = paged.attend(q, keys, (w, s, b), table, _i32([n], cuda), scale, q_start=qs, max_q=new)
+    ref, bound = R.attended(q, keys, (w, s, b), table, _i32([n], cuda), scale, qs, None, 0)
+    assert bool(((got.double() - ref).abs() <= bound + 2.0 ** -31 * R.unpacked(values).nan_to_num().abs().amax()).all())
+    assert _status() == 0
