@@ -30,7 +30,7 @@ struct Kv4AttArgs {
     float* part_o;     // (CTA, 2, rows) x D
     int32_t* records;  // (CTA) x 8: the item that the start of a CTA's share divides
     uint8_t* dense;    // (request, kv head, dense_steps) x {keys, values} of a step as fp16 tiles (kv4_prefill's dense form)
-    int8_t* dense_keys;  // powers of two of the keys' values, where those of a step differ widely
+    int8_t* dense_keys;  // powers of two of the keys' values and of the keys, where those of a step differ widely
     int2* dense_meta;  // their keys' and values' powers of two, and the runs of 8 keys without a page
     int dense_steps;
     float scale_log2;

@@ -20,14 +20,14 @@
 //     128 keys at D = 128 take 1.45 us of products alone, 1.29 of unpacking alone, 2.5 together.
 // Roundings to fp16: queries after a power of two a row (exact for bf16 but for values 2^-26 below the row's largest); keys,
 // values and probabilities, 2^-11 each against the 2^-8 of a bf16 output (an fp16 output's error against 64 bits grows by
-// them from 2.1e-4 to 3.2e-4 .. 4.0e-4 of its size: the tensor cores take the operands in no finer type but at half the
+// them from 2.1e-4 to 2.4e-4 .. 4.0e-4 of its size: the tensor cores take the operands in no finer type but at half the
 // rate). Keys after a power of two a step that puts the largest that its groups can hold at 2^14 .. 2^15, taken back with the
 // scores' factor: a group's scale and a sixteenth of it stay normal numbers down to 2^-20 of that, where the group's share of
 // a score is as small. Values after a power of two a step in the same way; a row's outputs have one of their own, and its
 // probabilities are multiplied by the difference while that is small, its outputs (as its maximum's growth does) where it
-// is not: so a step's values cost another step's no bits, and a row only those of the keys that it sees. A step with keys
-// whose values are 2^-20 of the largest or less has one a key (PF_WILD; key_exp), which each row's probabilities take in, in
-// the two-pass step: the large ones may be out of a row's sight. Within a key, values are held to 2^-31 of its largest, and
+// is not: so a step's values cost another step's no bits, and a row only those of the keys that it sees. A step with keys, or
+// keys' values, that are 2^-20 of the largest or less has one a key (PF_WILD; key_exp), which each row's scores or probabilities
+// take in, in a step of two passes: the large ones may be out of a row's sight. Within a key, values are held to 2^-31 of its largest, and
 // probabilities to 2^-31 of the row's largest.
 // A masked score is -inf, its probability 0; a value whose scale or bias is not finite is held as 0 and its key as NaN,
 // so that only rows that see it become NaN.
@@ -280,15 +280,15 @@ struct PfBars {
     int abort;          // a wait gave up: no one waits any more
     int exps[4];        // powers of two of the keys and values of step i & 3 (pf_exps)
     uint32_t miss[4];   // its runs of 8 keys without a page
-    alignas(16) int8_t key_exp[4][128];  // powers of two of its keys' values, where they differ widely (PF_WILD)
-    int key_top[128];   // bits of the largest |value| that a key's groups can hold, while those are found
+    alignas(16) int8_t key_exp[4][256];  // powers of two of its keys' values, and (from KT on) of the keys, where they differ
+                                         // widely (PF_WILD)
     // what the page warp tells the unpacking warps of step i & 3: the pool row of each run of 8 keys (none: KV4_NONE), the
     // keys from its first to the tile's end (0: no more steps), and the runs without a page
     uint32_t run[4][16];
     int left[4];
     uint32_t gone[4];
     float k_max[2][PF_UNPACK], v_max[2][PF_UNPACK];  // of step i & 1: what each unpacking warp's groups can hold at most
-    float v_min[2][PF_UNPACK];                       // (values: negative from a warp that has no step), and the least of that
+    float k_min[2][PF_UNPACK], v_min[2][PF_UNPACK];  // (values: negative from a warp that has no step), and the least of that
     int rows, steps;    // the item's (0: no more), from the first softmax warp to the issuing thread
 };
 
@@ -341,10 +341,10 @@ __device__ __forceinline__ bool pf_wild(float least, float most) { return least 
 
 // A piece's scales and biases in fp32. A value scale or bias that is not finite makes the values 0 and the key NaN, which
 // only the rows that see it meet; so does an infinite key. Adds the largest |key| and |value| that the groups can hold, and
-// the least of the values' (from PF_LEAST on).
+// the least of them (from PF_LEAST on).
 template <typename T>
 __device__ __forceinline__ void pf_scales(uint16_t ks16, uint16_t kb16, uint16_t vs16, uint16_t vb16, float* ks, float* kb,
-                                          float* vs, float* vb, float* k_top, float* v_top, float* v_low) {
+                                          float* vs, float* vb, float* k_top, float* v_top, float* k_low, float* v_low) {
     *ks = F16Traits<T>::to_f32(ks16), *kb = F16Traits<T>::to_f32(kb16);
     *vs = F16Traits<T>::to_f32(vs16), *vb = F16Traits<T>::to_f32(vb16);
     const float k_most = fmaf(15.0f, fabsf(*ks), fabsf(*kb)), v_most = fmaf(15.0f, fabsf(*vs), fabsf(*vb));
@@ -355,7 +355,10 @@ __device__ __forceinline__ void pf_scales(uint16_t ks16, uint16_t kb16, uint16_t
     }
     *v_top = fmaxf(*v_top, v_most);
     if (v_most >= PF_LEAST) *v_low = fminf(*v_low, v_most);
-    if (k_most < INFINITY) *k_top = fmaxf(*k_top, k_most);
+    if (k_most < INFINITY) {
+        *k_top = fmaxf(*k_top, k_most);
+        if (k_most >= PF_LEAST) *k_low = fminf(*k_low, k_most);
+    }
 }
 // 2^e, e in -126 .. 127.
 __device__ __forceinline__ float pf_pow2(int e) { return __uint_as_float(uint32_t(127 + e) << 23); }
@@ -363,11 +366,14 @@ __device__ __forceinline__ float pf_pow2(int e) { return __uint_as_float(uint32_
 __device__ __forceinline__ int pf_fit(float M) { return M > 0.0f ? min(14 - (int(__float_as_uint(M) >> 23) - 127), 110) : 0; }
 // The powers of two of a step's keys and values in one word.
 __device__ __forceinline__ int pf_exps(int ke, int ve) { return int(uint32_t(ke) << 16 | (uint32_t(ve) & 0xffffu)); }
-// The values' of a step (or key) that holds none but zeros: any; and of a step whose keys have one each.
+// The values' of a step (or key) that holds none but zeros: any; and of a step whose keys, and their values, have one each.
 constexpr int PF_ANY = 127, PF_WILD = 126;
 __device__ __forceinline__ int8_t pf_key_exp(int top) { return int8_t(top ? pf_fit(__int_as_float(top)) : PF_ANY); }
-// A key's largest from its groups' (the bits of floats from 0 on are in their order).
-__device__ __forceinline__ void pf_key_max(int* top, float vs, float vb) { atomicMax(top, __float_as_int(fmaf(15.0f, fabsf(vs), fabsf(vb)))); }
+// A key's largest (or its values') from its groups' that are finite (the bits of floats from 0 on are in their order).
+__device__ __forceinline__ void pf_key_max(int* top, float s, float b) {
+    const float most = fmaf(15.0f, fabsf(s), fabsf(b));
+    if (most < INFINITY) atomicMax(top, __float_as_int(most));
+}
 // Whether keys differ so widely, and not only a key's groups (a head of 64 dimensions in a place of 128): asked of whole warps.
 template <int KT>
 __device__ __forceinline__ bool pf_wild_keys(const int* top, float most) {
@@ -395,8 +401,8 @@ __global__ void __launch_bounds__(PD_WARPS * 32) kv4_dense_kernel(const Kv4AttAr
     using S = PfShape<D>;
     using P = PfPieces<D, PD_WARPS>;
     extern __shared__ __align__(1024) uint8_t pf_raw[];
-    __shared__ float part[PD_WARPS], k_part[PD_WARPS], low_part[PD_WARPS];
-    __shared__ int key_top[S::KT];
+    __shared__ float part[PD_WARPS], k_part[PD_WARPS], low_part[PD_WARPS], k_low_part[PD_WARPS];
+    __shared__ int key_top[2][S::KT];  // of the values, of the keys
     grid_dep_wait();
     const int s = blockIdx.x, kvh = blockIdx.y, b = blockIdx.z;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -422,7 +428,7 @@ __global__ void __launch_bounds__(PD_WARPS * 32) kv4_dense_kernel(const Kv4AttAr
     }
     const uint32_t miss = __ballot_sync(0xffffffffu, lane < RUNS && gone);
     uint4 kc[P::J], vc[P::J];
-    float ks[P::J], kb[P::J], vs[P::J], vb[P::J], k_top = 0.0f, top = 0.0f, low = INFINITY;
+    float ks[P::J], kb[P::J], vs[P::J], vb[P::J], k_top = 0.0f, top = 0.0f, k_low = INFINITY, low = INFINITY;
     uint16_t sc[P::J][4];
 #pragma unroll
     for (int j = 0; j < P::J; ++j) {
@@ -439,26 +445,31 @@ __global__ void __launch_bounds__(PD_WARPS * 32) kv4_dense_kernel(const Kv4AttAr
     }
 #pragma unroll
     for (int j = 0; j < P::J; ++j)
-        pf_scales<T>(sc[j][0], sc[j][1], sc[j][2], sc[j][3], &ks[j], &kb[j], &vs[j], &vb[j], &k_top, &top, &low);
+        pf_scales<T>(sc[j][0], sc[j][1], sc[j][2], sc[j][3], &ks[j], &kb[j], &vs[j], &vb[j], &k_top, &top, &k_low, &low);
     top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top)));
     k_top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(k_top)));
     low = __uint_as_float(__reduce_min_sync(0xffffffffu, __float_as_uint(low)));
-    if (lane == 0) part[warp] = top, k_part[warp] = k_top, low_part[warp] = low;
-    if (threadIdx.x < S::KT) key_top[threadIdx.x] = 0;
+    k_low = __uint_as_float(__reduce_min_sync(0xffffffffu, __float_as_uint(k_low)));
+    if (lane == 0) part[warp] = top, k_part[warp] = k_top, low_part[warp] = low, k_low_part[warp] = k_low;
+    if (threadIdx.x < S::KT) key_top[0][threadIdx.x] = key_top[1][threadIdx.x] = 0;
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < PD_WARPS; ++i) {
         top = fmaxf(top, part[i]), k_top = fmaxf(k_top, k_part[i]);
-        low = fminf(low, low_part[i]);
+        low = fminf(low, low_part[i]), k_low = fminf(k_low, k_low_part[i]);
     }
     const size_t at = ((size_t)b * a.pool.KVH + kvh) * a.dense_steps + s;
-    bool wild = pf_wild(low, top);
+    bool wild = pf_wild(low, top) || pf_wild(k_low, k_top);
     if (wild) {
 #pragma unroll
-        for (int j = 0; j < P::J; ++j) pf_key_max(&key_top[P::key(j, warp, lane)], vs[j], vb[j]);
+        for (int j = 0; j < P::J; ++j) {
+            pf_key_max(&key_top[0][P::key(j, warp, lane)], vs[j], vb[j]);
+            pf_key_max(&key_top[1][P::key(j, warp, lane)], ks[j], kb[j]);
+        }
         __syncthreads();
-        wild = pf_wild_keys<S::KT>(key_top, top);
-        if (wild && threadIdx.x < S::KT) a.dense_keys[at * S::KT + threadIdx.x] = pf_key_exp(key_top[threadIdx.x]);
+        wild = pf_wild_keys<S::KT>(key_top[0], top) || pf_wild_keys<S::KT>(key_top[1], k_top);
+        if (wild && threadIdx.x < 2 * S::KT)
+            a.dense_keys[at * (2 * S::KT) + threadIdx.x] = pf_key_exp(key_top[threadIdx.x / S::KT][threadIdx.x % S::KT]);
     }
     const int ke = pf_fit(k_top);
     const float kf = pf_pow2(ke);
@@ -467,8 +478,9 @@ __global__ void __launch_bounds__(PD_WARPS * 32) kv4_dense_kernel(const Kv4AttAr
 #pragma unroll
     for (int j = 0; j < P::J; ++j) {
         const int k = P::key(j, warp, lane), p = P::piece(j, warp, lane);
-        const float f = wild ? pf_pow2(pf_fit(__int_as_float(key_top[k]))) : vf;
-        pf_unpack<D>(kc[j], ks[j] * kf, kb[j] * kf, tile, k, p);
+        const float f = wild ? pf_pow2(pf_fit(__int_as_float(key_top[0][k]))) : vf;
+        const float fk = wild ? pf_pow2(pf_fit(__int_as_float(key_top[1][k]))) : kf;
+        pf_unpack<D>(kc[j], ks[j] * fk, kb[j] * fk, tile, k, p);
         pf_unpack<D>(vc[j], vs[j] * f, vb[j] * f, tile + S::TB, k, p);
     }
     fence_proxy_async();
@@ -520,15 +532,17 @@ __device__ __forceinline__ float pf_refit(PfRow& row, float mn, int ve_t, bool s
     return corr;
 }
 
-// A row's step whose keys' values have a power of two each (PF_WILD), in two passes over its scores (s_col), which its
+// A row's step whose keys and values have powers of two each (PF_WILD), in two passes over its scores (s_col), which its
 // probabilities replace; before: products into its outputs (o_col) so far, 0 for none. Out of line, since it is rare.
 template <typename T, int D>
 __device__ __noinline__ PfRow pf_wild_step(PfRow row, PfBars* bars, int it, int w, int before, uint32_t s_col, uint32_t o_col,
                                             int lo, int hi, float c) {
     constexpr int KT = PfShape<D>::KT;
-    const int exps = *reinterpret_cast<volatile int*>(&bars->exps[it & 3]);
     const uint32_t miss = *reinterpret_cast<volatile uint32_t*>(&bars->miss[it & 3]), key_exp = smem_u32(bars->key_exp[it & 3]);
-    const float ct = pf_factor(c, exps);
+    auto factor = [&](uint32_t k) {  // of a key's score, from the word that holds its power of two in the low byte
+        const int ke = int8_t(k);
+        return pf_factor(c, ke == PF_ANY ? 0 : ke * 65536);
+    };
     int ve_t = PF_ANY;  // the largest values' that the row sees
 #pragma unroll 1
     for (int k = 0; k < KT; k += 4) {
@@ -546,12 +560,13 @@ __device__ __noinline__ PfRow pf_wild_step(PfRow row, PfBars* bars, int it, int 
         tmem_ld_32x32b_x32(s_col + ch * 32, r);
         const uint32_t v = pf_sees(lo, hi, miss, ch);
         tmem_wait_ld();
-        float part[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-        for (int i = 0; i < 32; i += 2) part[(i >> 1) & 1] = fmaxf(fmaxf(part[(i >> 1) & 1], pf_seen(r[i], v, i)), pf_seen(r[i + 1], v, i + 1));
-        mx = fmaxf(mx, fmaxf(part[0], part[1]));
+        for (int i = 0; i < 32; i += 2) {
+            const uint32_t k = lds32(key_exp + KT + ch * 32 + (i & ~3)) >> (8 * (i & 2));
+            mx = fmaxf(fmaxf(mx, pf_seen(r[i], v, i) * factor(k)), pf_seen(r[i + 1], v, i + 1) * factor(k >> 8));
+        }
     }
-    const float mn = fmaxf(row.m, mx * ct);
+    const float mn = fmaxf(row.m, mx);
     const bool some = mx != -INFINITY;
     const int d = row.ve - ve_t;
     const bool grow = mn > row.m + PF_LAG || (row.m == -INFINITY && mn > row.m) || (some && (d < PF_DOWN || d > PF_UP));
@@ -581,8 +596,9 @@ __device__ __noinline__ PfRow pf_wild_step(PfRow row, PfBars* bars, int it, int 
         tmem_wait_ld();
 #pragma unroll
         for (int i = 0; i < 16; i += 2) {
-            const float e0 = kv4_ex2(fmaf(pf_seen(x[i], v, i), ct, -mz));
-            const float e1 = kv4_ex2(fmaf(pf_seen(x[i + 1], v, i + 1), ct, -mz));
+            const uint32_t kk = lds32(key_exp + KT + ch * 16 + (i & ~3)) >> (8 * (i & 2));
+            const float e0 = kv4_ex2(fmaf(pf_seen(x[i], v, i), factor(kk), -mz));
+            const float e1 = kv4_ex2(fmaf(pf_seen(x[i + 1], v, i + 1), factor(kk >> 8), -mz));
             // (the small ones' may become 0 beside the large ones')
             const uint32_t k = lds32(key_exp + ch * 16 + (i & ~3)) >> (8 * (i & 2));
             p[i / 2] = cvt_f16x2(e1 * pf_pow2(min(max(row.ve - int(int8_t(k >> 8)) + PF_BIAS, -126), 100)),
@@ -604,6 +620,7 @@ __global__ void __launch_bounds__(pf_threads(DENSE), 1) kv4_prefill_kernel(const
     extern __shared__ __align__(1024) uint8_t pf_raw[];
     __shared__ long long red[PF_THREADS / 32];
     __shared__ uint8_t* volatile pf_base;
+    __shared__ int key_top[DENSE ? 1 : KT];  // bits of the largest that a key's groups can hold, while those are found
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
     if (smem_u32(pf_raw) & 1023) {  // (the declaration's alignment; there is no room to make up for it)
@@ -1057,16 +1074,20 @@ __global__ void __launch_bounds__(pf_threads(DENSE), 1) kv4_prefill_kernel(const
         auto step_out = [&](const Held& h, int it, bool have) -> bool {
             const int st = it & 1;
             const uint32_t par = ((it >> 1) & 1) ^ 1;
-            float k_top = 0.0f, top = 0.0f, low = INFINITY, ks[J], kb[J], vs[J], vb[J];
+            float k_top = 0.0f, top = 0.0f, k_low = INFINITY, low = INFINITY, ks[J], kb[J], vs[J], vb[J];
             if (have) {
 #pragma unroll
                 for (int j = 0; j < J; ++j)
-                    pf_scales<T>(h.ks[j], h.kb[j], h.vs[j], h.vb[j], &ks[j], &kb[j], &vs[j], &vb[j], &k_top, &top, &low);
+                    pf_scales<T>(h.ks[j], h.kb[j], h.vs[j], h.vb[j], &ks[j], &kb[j], &vs[j], &vb[j], &k_top, &top, &k_low, &low);
             }
             top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top)));
             k_top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(k_top)));
             low = __uint_as_float(__reduce_min_sync(0xffffffffu, __float_as_uint(low)));
-            if (lane == 0) bar.v_max[st][uw] = have ? top : -1.0f, bar.k_max[st][uw] = k_top, bar.v_min[st][uw] = low;
+            k_low = __uint_as_float(__reduce_min_sync(0xffffffffu, __float_as_uint(k_low)));
+            if (lane == 0) {
+                bar.v_max[st][uw] = have ? top : -1.0f, bar.k_max[st][uw] = k_top;
+                bar.v_min[st][uw] = low, bar.k_min[st][uw] = k_low;
+            }
             named_barrier(1, PF_UNPACK * 32);  // (a slot is written again after the next step's barrier, which its readers pass later)
             float M = 0.0f;
             bool over = false;
@@ -1076,6 +1097,7 @@ __global__ void __launch_bounds__(pf_threads(DENSE), 1) kv4_prefill_kernel(const
                 M = fmaxf(M, x);
                 k_top = fmaxf(k_top, reinterpret_cast<volatile float*>(bar.k_max[st])[i]);
                 low = fminf(low, reinterpret_cast<volatile float*>(bar.v_min[st])[i]);
+                k_low = fminf(k_low, reinterpret_cast<volatile float*>(bar.k_min[st])[i]);
                 over = over || x < 0.0f;
             }
             if (over) return false;
@@ -1083,17 +1105,28 @@ __global__ void __launch_bounds__(pf_threads(DENSE), 1) kv4_prefill_kernel(const
             const float kf = pf_pow2(ke);
             const int ve = pf_fit(M);
             const float vf = pf_pow2(ve);
-            bool wild = pf_wild(low, M);  // (the same in all warps)
+            bool wild = pf_wild(low, M) || pf_wild(k_low, k_top);  // (the same in all warps)
+            int8_t* const key_exp = bar.key_exp[it & 3];
             if (wild) {
                 const int me = uw * 32 + lane;
-                if (me < KT) bar.key_top[me] = 0;
-                named_barrier(1, PF_UNPACK * 32);
+                wild = false;
 #pragma unroll
-                for (int j = 0; j < J; ++j) pf_key_max(&bar.key_top[P::key(j, uw, lane)], vs[j], vb[j]);
-                named_barrier(1, PF_UNPACK * 32);
-                wild = pf_wild_keys<KT>(bar.key_top, M);
-                if (wild && me < KT) bar.key_exp[it & 3][me] = pf_key_exp(bar.key_top[me]);
+                for (int keys = 0; keys < 2; ++keys) {  // values, keys
+                    if (me < KT) key_top[me] = 0;
+                    named_barrier(1, PF_UNPACK * 32);
+#pragma unroll
+                    for (int j = 0; j < J; ++j) pf_key_max(&key_top[P::key(j, uw, lane)], keys ? ks[j] : vs[j], keys ? kb[j] : vb[j]);
+                    named_barrier(1, PF_UNPACK * 32);
+                    wild = pf_wild_keys<KT>(key_top, keys ? k_top : M) || wild;
+                    if (me < KT) key_exp[keys * KT + me] = pf_key_exp(key_top[me]);
+                    named_barrier(1, PF_UNPACK * 32);
+                }
             }
+            // A key's own: of its values, or (from KT on) of itself.
+            auto own = [&](int key) -> float {
+                const int e = *reinterpret_cast<volatile int8_t*>(key_exp + key);
+                return pf_pow2(e == PF_ANY ? 0 : e);
+            };
             if (uw == 0 && lane == 0) {
                 bar.exps[it & 3] = pf_exps(ke, wild ? PF_WILD : M > 0.0f ? ve : PF_ANY);
                 bar.miss[it & 3] = bar.gone[it & 3];
@@ -1102,14 +1135,17 @@ __global__ void __launch_bounds__(pf_threads(DENSE), 1) kv4_prefill_kernel(const
             if (lane == 0) mbar_arrive(&bar.r_empty[it & 3]);
             pf_wait(&bar.k_empty[st], par, abort);
 #pragma unroll
-            for (int j = 0; j < J; ++j) pf_unpack<D>(h.k[j], ks[j] * kf, kb[j] * kf, sk + st * S::TB, P::key(j, uw, lane), P::piece(j, uw, lane));
+            for (int j = 0; j < J; ++j) {
+                const float f = wild ? own(KT + P::key(j, uw, lane)) : kf;
+                pf_unpack<D>(h.k[j], ks[j] * f, kb[j] * f, sk + st * S::TB, P::key(j, uw, lane), P::piece(j, uw, lane));
+            }
             fence_proxy_async();
             __syncwarp();
             if (lane == 0) mbar_arrive(&bar.k_full[st]);
             pf_wait(&bar.v_empty[st], par, abort);
 #pragma unroll
             for (int j = 0; j < J; ++j) {
-                const float f = wild ? pf_pow2(pf_fit(__int_as_float(bar.key_top[P::key(j, uw, lane)]))) : vf;
+                const float f = wild ? own(P::key(j, uw, lane)) : vf;
                 pf_unpack<D>(h.v[j], vs[j] * f, vb[j] * f, sv + st * S::TB, P::key(j, uw, lane), P::piece(j, uw, lane));
             }
             fence_proxy_async();
@@ -1155,9 +1191,9 @@ __global__ void __launch_bounds__(pf_threads(DENSE), 1) kv4_prefill_kernel(const
                     bar.exps[it & 3] = meta.x;
                     bar.miss[it & 3] = uint32_t(meta.y);
                     const bool wild = int16_t(meta.x) == PF_WILD;
-                    mbar_arrive_expect_tx(&bar.k_full[st], wild ? S::TB + KT : S::TB);
+                    mbar_arrive_expect_tx(&bar.k_full[st], wild ? S::TB + 2 * KT : S::TB);
                     copy(&bar.k_full[st], sk + st * S::TB, src, S::TB);
-                    if (wild) copy(&bar.k_full[st], smem_u32(bar.key_exp[it & 3]), a.dense_keys + (tile0 + t) * KT, KT);
+                    if (wild) copy(&bar.k_full[st], smem_u32(bar.key_exp[it & 3]), a.dense_keys + (tile0 + t) * (2 * KT), 2 * KT);
                     ++keys;
                     pf_wait(&bar.v_empty[st], par, abort);
                     if (*abort) break;
@@ -1322,7 +1358,7 @@ static bool pf_dense(int D, int B, int KVH, int G, int max_q, long long room, si
     const int R = D == 256 ? 128 : 256, KT = D == 256 ? 64 : 128;
     const long long n = (room + KT - 1) / KT, tiles = n * B * KVH;
     *steps = int(n);
-    *bytes = size_t(tiles) * (size_t(4) * KT * D + KT + sizeof(int2));
+    *bytes = size_t(tiles) * (size_t(4) * KT * D + 2 * KT + sizeof(int2));
     return (long long)max_q * G > 2 * R && tiles <= (1LL << 30) / (4LL * KT * D) && B <= 65535 && KVH <= 65535;
 }
 
@@ -1361,7 +1397,7 @@ static int kv4_prefill_d(Kv4AttArgs a, void* workspace, cudaStream_t st) {
         a.dense = static_cast<uint8_t*>(workspace) + pf_parts_bytes(D, n);
         const size_t tiles = size_t(a.dense_steps) * a.B * a.pool.KVH;
         a.dense_keys = reinterpret_cast<int8_t*>(a.dense + tiles * 2 * S::TB);
-        a.dense_meta = reinterpret_cast<int2*>(a.dense_keys + tiles * S::KT);
+        a.dense_meta = reinterpret_cast<int2*>(a.dense_keys + tiles * 2 * S::KT);
         rc = kv4_launch(kv4_dense_kernel<T, D>, set_first, dim3(a.dense_steps, a.pool.KVH, a.B), dim3(PD_WARPS * 32),
                         2 * S::TB + 128, st, a);
         if (!rc) rc = kv4_launch(kv4_prefill_kernel<T, D, true>, set_dense, dim3(n), dim3(pf_threads(true)), smem, st, a);

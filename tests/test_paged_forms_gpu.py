@@ -215,6 +215,34 @@ def test_large_values_out_of_sight_of_many_rows(cuda, form, new, H, KVH, D, colu
     _out_of_sight(cuda, form, new, H, KVH, D, columns, e)
 
 
+@pytest.mark.parametrize("e", [10, 20, 60, 100])
+@FORMS
+def test_large_keys_out_of_sight(cuda, form, new, H, KVH, D, columns, e):
+    """Keys 2^e of the usual size, as the values of test_large_values_out_of_sight: rows that do not see them answer as beside
+    ordinary keys there, but for the roundings of keys (the bound's), probabilities, values and outputs, of each."""
+    import torch
+    from locals_b200 import paged
+
+    n = 6000 if form in (CLUSTERS, SPLIT) else 640
+    for window, places, rows in ((n - 64 - new + 2, range(64), slice(2, None)), (0, range(n - 2, n - 1), slice(0, -2))):
+        plain, (q, keys, values, table, qs, scale, _) = _one(cuda, form, new, n, H, KVH, D, columns, seed=34, window=window)
+        s, b = keys[1].clone(), keys[2].clone()
+        for j in places:
+            at = int(table[0, j // 16]), slice(None), j % 16
+            s[at] *= 2.0 ** e
+            b[at] *= 2.0 ** e
+        got = paged.attend(q, (keys[0], s, b), values, table, _i32([n], cuda), scale, q_start=qs, max_q=new, window=window)
+        ref, bound = R.attended(q, keys, values, table, _i32([n], cuda), scale, qs, None, window)
+        off = ((got.double() - ref).abs() - bound)[rows]
+        assert bool((off <= 0).all()), (window, off.max().item())
+        size = _sizes(q, keys, values, table, n, scale, window)
+        near = 2 * (R.U[q.dtype] * size.clamp(max=plain.double().abs()) + size * (2.0 ** -10 + 2.0 ** -14)) + 2.0 ** -24
+        # (the roundings of the keys are the same but where one has a power of two of its own: by far most outputs are as near)
+        off = ((got.double() - plain.double()).abs() - near)[rows]
+        assert (off > 0).double().mean().item() < 0.01
+    assert _status() == 0
+
+
 @FORMS
 @pytest.mark.parametrize("what", ["a group of each head", "every 37th token", "all"])
 @pytest.mark.parametrize("least", [0.0, 1e-7])
