@@ -34,13 +34,13 @@
 // Work is dealt out as in kv4_attend.cu: the steps of all tiles (each as far as its last row sees) evenly over one CTA a
 // SM, parts joined by kv4_prefill_join_kernel.
 // What bounds it: 4 D operations a row and key on the tensor cores, and one exponential a row and key at 16 a clock and SM,
-// which take as long as the products do at D = 128 (tensor pipe 48% busy, exponentials 48%: they are not yet beside each
-// other all the time). Measured, GPU time of a call, bf16: 4,096 new tokens on 28,672 cached, 16 heads on 2, D = 128: 1,066 to
-// 1,143 us = 902 to 967 TFLOP/s by the clock that the power limit leaves (55 to 59% of the measured peak), fp16 1,210 to 1,271;
-// a mixed batch of 8 (1 to 1,024 new on up to 2,048 cached, 32 heads on 8): 193 us = 498 TFLOP/s, the items' ends and short
-// tiles; 16 requests of 5 drafted tokens on up to 4,003 keys, 16 heads on 2, D = 256: 50 to 52 us, latency: 4 us to find the
-// share, 6 to fetch the queries, 2 to 8 steps, 2 to write, and the joins. The powers of two a step, row and key take 2 to 5% of
-// these (bf16) and 9% of the fp16 piece.
+// which take as long as the products do at D = 128 (tensor pipe 47% busy, exponentials 47%: they are not yet beside each
+// other all the time). Measured, GPU time of a call, bf16: 4,096 new tokens on 28,672 cached, 16 heads on 2, D = 128: 1,086 to
+// 1,153 us = 894 to 949 TFLOP/s by the clock that the power limit leaves (55 to 58% of the measured peak), fp16 1,218 to 1,276;
+// a mixed batch of 8 (1 to 1,024 new on up to 2,048 cached, 32 heads on 8): 194 us = 494 TFLOP/s, the items' ends and short
+// tiles; 16 requests of 5 drafted tokens on up to 4,003 keys, 16 heads on 2, D = 256: 52 to 54 us, latency: 4 us to find the
+// share, 6 to fetch the queries, 2 to 8 steps, 2 to write, and the joins. The powers of two a step, row and key take 3 to 5% of
+// these, and 9% of the drafts and of the fp16 piece.
 // Tried and slower: half the exponentials as polynomials (1,128 against 1,081 us); 4 unpacking warps of 128 registers (1,778);
 // the two-pass step out of line (a mixed batch 245 against 200); a row's powers of two in shared memory (no faster);
 // 48 registers for the issuing warp (1,904); query rows fetched by neighbouring lanes (no faster, and 1,061 against 1,029).
