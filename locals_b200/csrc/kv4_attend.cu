@@ -19,8 +19,9 @@
 //     values 2^-27 below the row's largest. A row by itself: the tile holds other heads and other tokens of the request;
 //   w to fp16 (2^-11 against the 2^-8 of a bf16 output; an fp16 output's error grows from 2.0e-4 to 2.2e-4 by it), after a
 //     power of two a row that puts the largest value scale that the row has seen at 2^5 .. 2^10 (vf for the warp, a row's
-//     difference from it, xl, in its probabilities): values are held to 2^-30 of the largest that the row sees. codes - z (exact on subnormals, one packed subtraction a pair) takes out of a group
-//     what its codes and its bias have in common, so that this is a rounding of the value itself, however near to 0 it lies.
+//     difference from it, xl, in its probabilities): values are held to 2^-30 of the largest that the row sees. codes - z
+//     (exact on subnormals, one packed subtraction a pair) takes out of a group what its codes and its bias have in common,
+//     so that this is a rounding of the value itself, however near to 0 it lies.
 // A score tile's accumulator layout is transposed into the value MMA's operand by movmatrix. The running maximum of a row is
 // only followed when it has grown by 2^4, so that most steps rescale nothing.
 // A key's scales and biases become floats once a step, one key a lane, and go to its reads through shared memory. A masked

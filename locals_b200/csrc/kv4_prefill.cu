@@ -4,8 +4,9 @@
 // A CTA takes a tile of 256 rows of a (request, kv head) (128 at D = 256) and walks its keys in steps of 128 (64 at
 // D = 256). Per step
 //   * the codes of its keys and values become fp16 tiles in shared memory, (code | 1024) - 1024 and one fused multiply-add
-//     with the group's scale and bias (times a power of two), pairs (i, i + 4) of a word as they come out of one mask. The order of dimensions that
-//     this makes is met by the queries (stored in the same order) and undone when the output is written;
+//     with the group's scale and bias (times a power of two), pairs (i, i + 4) of a word as they come out of one mask. The
+//     order of dimensions that this makes is met by the queries (stored in the same order) and undone when the output is
+//     written;
 //   * one thread issues S = Q K^T (both in shared memory, K-major) and O += P V (P in tensor memory, V in shared memory as
 //     it lies, dimensions contiguous: the transposed B operand) as tcgen05.mma with fp32 accumulators in tensor memory:
 //     for two query tiles in turn, S0 PV0 S1 PV1 ..., so that one tile's softmax runs beside the other's products;
@@ -20,15 +21,15 @@
 //     128 keys at D = 128 take 1.45 us of products alone, 1.29 of unpacking alone, 2.5 together.
 // Roundings to fp16: queries after a power of two a row (exact for bf16 but for values 2^-26 below the row's largest); keys,
 // values and probabilities, 2^-11 each against the 2^-8 of a bf16 output (an fp16 output's error against 64 bits grows by
-// them from 2.1e-4 to 2.4e-4 .. 4.0e-4 of its size: the tensor cores take the operands in no finer type but at half the
-// rate). Keys after a power of two a step that puts the largest that its groups can hold at 2^14 .. 2^15, taken back with the
+// them from 2.1e-4 to 2.4e-4 .. 4.6e-4 of its size, mostly by the keys': the tensor cores take the operands in no finer type
+// but at half the rate). Keys after a power of two a step that puts the largest that its groups can hold at 2^14 .. 2^15, taken back with the
 // scores' factor: a group's scale and a sixteenth of it stay normal numbers down to 2^-20 of that, where the group's share of
 // a score is as small. Values after a power of two a step in the same way; a row's outputs have one of their own, and its
 // probabilities are multiplied by the difference while that is small, its outputs (as its maximum's growth does) where it
 // is not: so a step's values cost another step's no bits, and a row only those of the keys that it sees. A step with keys, or
 // keys' values, that are 2^-20 of the largest or less has one a key (PF_WILD; key_exp), which each row's scores or probabilities
-// take in, in a step of two passes: the large ones may be out of a row's sight. Within a key, values are held to 2^-31 of its largest, and
-// probabilities to 2^-31 of the row's largest.
+// take in, in a step of two passes: the large ones may be out of a row's sight. Within a key, values are held to 2^-31 of its
+// largest, and probabilities to 2^-31 of the row's largest.
 // A masked score is -inf, its probability 0; a value whose scale or bias is not finite is held as 0 and its key as NaN,
 // so that only rows that see it become NaN.
 // Work is dealt out as in kv4_attend.cu: the steps of all tiles (each as far as its last row sees) evenly over one CTA a
@@ -1088,7 +1089,9 @@ __global__ void __launch_bounds__(pf_threads(DENSE), 1) kv4_prefill_kernel(const
                 bar.v_max[st][uw] = have ? top : -1.0f, bar.k_max[st][uw] = k_top;
                 bar.v_min[st][uw] = low, bar.k_min[st][uw] = k_low;
             }
-            named_barrier(1, PF_UNPACK * 32);  // (a slot is written again after the next step's barrier, which its readers pass later)
+            __syncwarp();
+            // (a slot is written again after the next step's barrier, which its readers pass later)
+            named_barrier(1, PF_UNPACK * 32);
             float M = 0.0f;
             bool over = false;
 #pragma unroll
@@ -1113,12 +1116,16 @@ __global__ void __launch_bounds__(pf_threads(DENSE), 1) kv4_prefill_kernel(const
 #pragma unroll
                 for (int keys = 0; keys < 2; ++keys) {  // values, keys
                     if (me < KT) key_top[me] = 0;
+                    __syncwarp();
                     named_barrier(1, PF_UNPACK * 32);
 #pragma unroll
-                    for (int j = 0; j < J; ++j) pf_key_max(&key_top[P::key(j, uw, lane)], keys ? ks[j] : vs[j], keys ? kb[j] : vb[j]);
+                    for (int j = 0; j < J; ++j)
+                        pf_key_max(&key_top[P::key(j, uw, lane)], keys ? ks[j] : vs[j], keys ? kb[j] : vb[j]);
+                    __syncwarp();
                     named_barrier(1, PF_UNPACK * 32);
                     wild = pf_wild_keys<KT>(key_top, keys ? k_top : M) || wild;
                     if (me < KT) key_exp[keys * KT + me] = pf_key_exp(key_top[me]);
+                    __syncwarp();
                     named_barrier(1, PF_UNPACK * 32);
                 }
             }
