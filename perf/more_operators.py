@@ -99,7 +99,7 @@ def _codes(q):
     """Codes of 4 bits for magnitudes and signs of q: the nearest value, ties to the even code, 6 beyond."""
     a = q.abs()
     m = ((a > 0.25).to(torch.int32) + (a >= 0.75) + (a > 1.25) + (a >= 1.75) + (a > 2.5) + (a >= 3.5) + (a > 5.0))
-    return m + 8 * (q < 0)
+    return m + 8 * (q < 0).to(torch.int32)
 
 
 def _e4m3(t):
