@@ -306,6 +306,53 @@ int lq_kv4_attend(const void* q, int N, const int32_t* q_start, int max_q, const
                   int window, int H, int KVH, int head_dim, int dtype, void* workspace, size_t workspace_bytes,
                   void* out, void* stream);
 
+/* ---- microscaled 4-bit floating point (the reference's mxfp4 experts, locals/moe_kernel.py:68-155; nvfp4 has no
+ * counterpart there) ----
+ * A value is 4 bits (e2m1: 0, 0.5, 1, 1.5, 2, 3, 4, 6 and their negatives), a group along the row shares a scale byte:
+ * LQ_MXFP4 groups of 32, scale 2^(b - 127); LQ_NVFP4 groups of 16, scale an e4m3 number, and one float32 factor for the
+ * matrix (a device pointer, NULL = 1). codes (rows, Kp / 8) uint32, eight codes a word, lowest bits first, Kp = K rounded
+ * up to a multiple of 128, zero codes beyond K (to a word's end: mx's codes are MLX's own); 32-byte aligned. tiles: the scale
+ * bytes in tiles of 128 rows x 4 groups, (ceil(rows / 128), Kp / (4 * group), 512) bytes, the byte of row r and group g
+ * at 16 (r % 32) + 4 (r / 32 % 4) + g % 4 of tile (r / 128, g / 4); 16-byte aligned. A stack of matrices has each one's tiles in
+ * turn. Tile bytes of rows that do not exist are not used. */
+#define LQ_MXFP4 0
+#define LQ_NVFP4 1
+
+/* codes and tiles of x (rows, K), f16 / bf16 / f32, x_row elements from one row to the next. LQ_MXFP4: scale
+ * 2^max(floor(log2 amax) - 2, -127). LQ_NVFP4: the e4m3 number nearest to amax / (6 factor), at most 448. Codes: nearest to
+ * x / (scale * factor), ties to the even code, 6 beyond it. A group that holds an infinity or no number gets the scale that is
+ * not a number. factor: 1 float32 > 0 (LQ_NVFP4), or NULL. */
+int lq_fp4_quantize(const void* x, int dtype, int64_t x_row, int rows, int K, int mode, const float* factor,
+                    uint32_t* codes, uint8_t* tiles, void* stream);
+
+/* out (stack * rows, K) in dtype (f16 / bf16 / f32) = code * scale * factor, rounded once. */
+int lq_fp4_dequantize(const uint32_t* codes, const uint8_t* tiles, int stack, int rows, int K, int mode,
+                      const float* factor, int dtype, void* out, void* stream);
+
+/* y (M, N) = x . w^T of two operands in the same 4-bit format, 32-bit sums, y in dtype (f16 / bf16 / f32). glu != 0: rows of
+ * w are gate 0, up 0, gate 1, up 1, ... and y (M, N / 2) = silu(gate) * up, rounded once. */
+int lq_fp4_qmm(const uint32_t* x_codes, const uint8_t* x_tiles, const float* x_factor, const uint32_t* w_codes,
+               const uint8_t* w_tiles, const float* w_factor, int M, int N, int K, int mode, int glu, int dtype, void* y,
+               void* stream);
+
+/* y (M, N) = x . w^T of x (M, K) in f16 / bf16 (x_row elements from one row to the next) and w in LQ_MXFP4; y in x's
+ * dtype; glu as lq_fp4_qmm. x enters in pieces of e4m3 with a power of two a group of 32: exact down to 2^-13 of a group's
+ * largest magnitude, below that off by at most 2^-21 of it; a row that holds an infinity or no number gives no numbers.
+ * workspace: lq_fp4_linear_workspace(M, K, dtype) bytes, 256-byte aligned. */
+size_t lq_fp4_linear_workspace(int M, int K, int dtype);
+int lq_fp4_linear(const void* x, int64_t x_row, const uint32_t* codes, const uint8_t* tiles, int M, int N, int K, int glu,
+                  int dtype, void* y, void* workspace, size_t workspace_bytes, void* stream);
+
+/* lq_moe_experts for stacks in LQ_MXFP4: codes (E, N, Kp / 8), tiles (E, ceil(N / 128), Kp / 128, 512). out (P, N), or
+ * (P, N / 2) with glu as lq_fp4_qmm. x (x_rows, K): with gather_order, pair j reads row gather_order[j] / gather_k;
+ * without, row j. Segments as lq_moe_experts (an expert id E is padding, left unwritten); min(E + 1, P) <= 2047.
+ * workspace: lq_fp4_experts_workspace(P, max_rows, E, K, dtype) bytes, 256-byte aligned. */
+size_t lq_fp4_experts_workspace(int P, int max_rows, int E, int K, int dtype);
+int lq_fp4_experts(const void* x, int x_rows, const int32_t* gather_order, int gather_k, const int32_t* starts,
+                   const int32_t* experts, const int32_t* nseg, int P, int max_rows, int glu, const uint32_t* codes,
+                   const uint8_t* tiles, void* out, int E, int N, int K, int dtype, void* workspace,
+                   size_t workspace_bytes, void* stream);
+
 /* The column-sharded prefill with its own all-gather: this rank's N output columns of y = x . dequant(w)^T (the
  * dense path of lq_qmm_dense) are written by the GEMM in place at columns [col_off, col_off + N) of dst[0], this GPU's
  * row-major (M, ldo) buffer, then copied by one kernel of plain 16-byte peer stores into the same columns of

@@ -12,6 +12,7 @@ LIB_PATH = os.path.join(HERE, "liblq.so")
 
 LQ_OK, LQ_E_ARG, LQ_E_SHAPE, LQ_E_ALIGN, LQ_E_UNSUPPORTED, LQ_E_CUDA, LQ_E_DEVICE, LQ_E_SCRATCH = range(8)
 F16, BF16, F32 = 0, 1, 2
+MXFP4, NVFP4 = 0, 1
 FAM_AUTO, FAM_QMV, FAM_TC, FAM_TCV, FAM_QMVG, FAM_QMVQ = 0, 1, 2, 3, 4, 5
 
 # every function the header declares, with its argument types (checked by tests on CPU)
@@ -72,6 +73,14 @@ SIGNATURES = {
     "lq_kv4_attend_forms": ([_i, _i, _i, _i, _i, _i, _i, _i], _i),
     "lq_kv4_attend": ([_vp, _i, _vp, _i, _u32p, _vp, _vp, _u32p, _vp, _vp, _i, _i, _vp, _i, _vp, _i, _vp,
                        ctypes.c_float, _i, _i, _i, _i, _i, _vp, ctypes.c_size_t, _vp, _vp], _i),
+    "lq_fp4_quantize": ([_vp, _i, _i64, _i, _i, _i, _vp, _u32p, _vp, _vp], _i),
+    "lq_fp4_dequantize": ([_u32p, _vp, _i, _i, _i, _i, _vp, _i, _vp, _vp], _i),
+    "lq_fp4_qmm": ([_u32p, _vp, _vp, _u32p, _vp, _vp, _i, _i, _i, _i, _i, _i, _vp, _vp], _i),
+    "lq_fp4_linear_workspace": ([_i, _i, _i], ctypes.c_size_t),
+    "lq_fp4_linear": ([_vp, _i64, _u32p, _vp, _i, _i, _i, _i, _i, _vp, _vp, ctypes.c_size_t, _vp], _i),
+    "lq_fp4_experts_workspace": ([_i, _i, _i, _i, _i], ctypes.c_size_t),
+    "lq_fp4_experts": ([_vp, _i, _vp, _i, _vp, _vp, _vp, _i, _i, _i, _u32p, _vp, _vp, _i, _i, _i, _i, _vp,
+                        ctypes.c_size_t, _vp], _i),
     "lq_supported": ([_i, _i, _i, _i, _i, _i, _i], _i),
     "lq_list_configs": ([_i, _i, _i, _i, _i, _i, ctypes.POINTER(Cfg), _i], _i),
     "lq_device_status": ([_i], ctypes.c_uint),

@@ -1,0 +1,126 @@
+// Microscaled 4-bit floating point: the format, and the PTX of its block-scaled tensor-core products.
+//
+// A value is 4 bits (e2m1: sign, 2 exponent bits, 1 mantissa bit; 0, 0.5, 1, 1.5, 2, 3, 4, 6 and their negatives), eight
+// to a 32-bit word, lowest bits first; rows are filled with zero codes to a multiple of 128 values. Groups along a row share a
+// scale byte: "mxfp4" 32 values and 2^(b - 127) (255: not a number), "nvfp4" 16 values and an e4m3 number (127: not a
+// number). Scale bytes lie in tiles of 128 rows x 4 groups, 512 bytes, the order in which tcgen05.cp.32x128b takes them to
+// tensor memory: byte 16 (r % 32) + 4 (r / 32) + g % 4 of tile (r / 128, g / 4); the tiles of 128 rows follow one another
+// along the groups.
+#pragma once
+
+#include <cuda.h>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <stdint.h>
+
+#include "../../include/lq.h"
+#include "lq_ptx.cuh"
+
+namespace lq {
+
+constexpr int FP4_PAD = 128;  // values a row is filled to a multiple of
+
+__host__ __device__ constexpr int fp4_padded(int K) { return (K + FP4_PAD - 1) / FP4_PAD * FP4_PAD; }
+__host__ __device__ constexpr int fp4_group(int mode) { return mode == LQ_MXFP4 ? 32 : 16; }
+// 512-byte scale tiles along a row of K values
+__host__ __device__ constexpr int fp4_ktiles(int K, int mode) { return fp4_padded(K) / (4 * fp4_group(mode)); }
+
+__host__ __device__ constexpr int fp4_tile_byte(int row, int group) {
+    return 16 * (row % 32) + 4 * (row / 32) + group % 4;
+}
+
+// Two floats to two e2m1 codes (nearest, ties to even, saturating): `lo` in bits 0-3, `hi` in bits 4-7.
+__device__ __forceinline__ uint32_t cvt_e2m1x2(float hi, float lo) {
+    uint32_t r;
+    asm("{\n\t.reg .b8 b;\n\t"
+        "cvt.rn.satfinite.e2m1x2.f32 b, %1, %2;\n\t"
+        "cvt.u32.u8 %0, b;\n\t}"
+        : "=r"(r)
+        : "f"(hi), "f"(lo));
+    return r;
+}
+
+// Two floats to two e4m3 bytes, `lo` in the low one.
+__device__ __forceinline__ uint32_t cvt_e4m3x2(float hi, float lo) {
+    uint16_t r;
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+
+// Two e4m3 bytes to fp16 (exact).
+__device__ __forceinline__ float2 e4m3x2_to_f32(uint32_t v) {
+    uint32_t h;
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"(uint16_t(v)));
+    return __half22float2(*reinterpret_cast<__half2*>(&h));
+}
+
+// What a scale byte stands for.
+__device__ __forceinline__ float fp4_scale_value(uint32_t b, int mode) {
+    if (mode == LQ_MXFP4)  // 2^(b - 127): the exponent field, but for 0 (2^-127 is no normal number) and 255 (not a number)
+        return b == 0 ? __uint_as_float(0x00400000u) : b == 255 ? __uint_as_float(0x7FC00000u) : __uint_as_float(b << 23);
+    return e4m3x2_to_f32(b).x;
+}
+
+// ---- TMA: untiled bulk copy (16-byte aligned on both sides, a multiple of 16 bytes) ----
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                     smem_u32(dst)),
+                 "l"(src), "r"(bytes), "r"(smem_u32(bar))
+                 : "memory");
+}
+
+// ---- block-scaled tcgen05 ----
+
+// One scale tile (512 bytes of shared memory, rows of 16 bytes) to 4 columns of tensor memory, in all four lane quarters.
+__device__ __forceinline__ void tc_copy_scales(uint32_t taddr, uint64_t desc) {
+    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+}
+
+// Shared-memory descriptor of unswizzled 8-row x 16-byte core matrices that follow one another (128 bytes apart).
+__device__ __forceinline__ uint64_t umma_desc_scales(uint32_t smem_addr) {
+    return uint64_t((smem_addr >> 4) & 0x3FFFu) | (uint64_t(128 >> 4) << 16) | (uint64_t(128 >> 4) << 32) |
+           (uint64_t(1) << 46);
+}
+
+// The forms of a block-scaled MMA: both operands mxfp4 or both nvfp4 (K = 64 a MMA), or e2m1 (in bytes) by e4m3 (K = 32).
+enum { FP4_MX = 0, FP4_NV = 1, FP4_SPLIT = 2 };
+
+// Instruction descriptor: A e2m1, B e2m1 or e4m3, both K-major, M x N tile, the byte of each 32-bit scale word that
+// the MMA starts at in bits 4-5 (B) and 29-30 (A), the scales' type in bit 23 (1: powers of two).
+template <int KIND>
+__host__ __device__ constexpr uint32_t fp4_idesc(int M, int N) {
+    return (uint32_t(KIND == FP4_SPLIT ? 5 : 1) << 7) | (uint32_t(KIND == FP4_SPLIT ? 0 : 1) << 10) |
+           (uint32_t(N >> 3) << 17) | (uint32_t(KIND == FP4_NV ? 0 : 1) << 23) | (uint32_t(M >> 4) << 24);
+}
+__host__ __device__ constexpr uint32_t fp4_idesc_byte(int id) { return (uint32_t(id) << 4) | (uint32_t(id) << 29); }
+
+template <int KIND>
+__device__ __forceinline__ void tc_mma_fp4(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t sa,
+                                           uint32_t sb, uint32_t accumulate) {
+    if constexpr (KIND == FP4_MX)
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "setp.ne.b32 p, %6, 0;\n\t"
+            "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(
+                d_tmem),
+            "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(sa), "r"(sb), "r"(accumulate)
+            : "memory");
+    else if constexpr (KIND == FP4_NV)
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "setp.ne.b32 p, %6, 0;\n\t"
+            "tcgen05.mma.cta_group::1.kind::mxf4nvf4.block_scale.scale_vec::4X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(
+                d_tmem),
+            "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(sa), "r"(sb), "r"(accumulate)
+            : "memory");
+    else
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "setp.ne.b32 p, %6, 0;\n\t"
+            "tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(
+                d_tmem),
+            "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(sa), "r"(sb), "r"(accumulate)
+            : "memory");
+}
+
+}  // namespace lq

@@ -1,0 +1,663 @@
+// Products with microscaled 4-bit weights on the block-scaled tensor cores of sm_100a: y (M, N) = x . w^T, x in the same
+// 4-bit format, or in 16 bits against mxfp4 weights; dense, or grouped over the experts that rows are routed to.
+//
+// Mathematics. Each value of a group is code * scale, so a group's part of a sum is scale_x scale_w sum code_x code_w, and
+// the tensor core does all of it: the products of codes are exact, the scales enter as operands, sums are 32 bits. No
+// weight is ever unpacked. Activations of 16 bits are first split in pieces of e4m3 (4 significant bits), each with a power
+// of two a group of 32: bf16 (8 bits) is the sum of 2, fp16 (11 bits) of 3. With E the exponent of the largest magnitude of
+// the group, piece p has the scale 2^(E - 7 - 4 p) and is the rounded remainder of those before it, so the pieces' sum is x
+// exactly down to 2^-13 of that magnitude; below, it is off by at most 2^-21 (bf16) or 2^-25 (fp16) of it, less than
+// the 32-bit sum itself loses beside that value. A group that holds an infinity or no number is not a number.
+//
+// Layout. Weights are the MMA's A operand (128 rows of w a tile, one a tensor-memory lane), T tokens its N side, so that one
+// token costs a narrow MMA and not a row of an empty tile. Warp 4 streams a ring of stages by TMA: 128 bytes of every
+// row (256 codes; against e4m3, 128 codes that TMA spreads to bytes) and their scale tiles. Warp 5 copies the scales to
+// tensor memory and issues the MMAs; warps 0 to 3 write finished tiles out under the next tile's MMAs. The scales have two
+// places in tensor memory: a stage's are copied only when the MMAs of the stage before last are done.
+// Few tiles: a cluster of CTAs splits a tile's K and joins its sums through distributed shared memory, in rank order.
+#include <cuda_runtime.h>
+
+#include <type_traits>
+
+#include "fp4.cuh"
+#include "fp4_host.h"
+#include "lq_host.h"
+
+namespace lq {
+
+constexpr int FP4_THREADS = 192;
+constexpr int FP4_MAX_STAGES = 10;
+constexpr int FP4_MAX_SEGMENTS = 2048;
+
+template <int KIND_, int P_, int T_>
+struct Fp4Shape {
+    static constexpr int KIND = KIND_, P = P_, T = T_;
+    static constexpr bool STACK = KIND == FP4_SPLIT && T <= 32;  // a token's pieces as columns of one MMA
+    static constexpr int BK = KIND == FP4_SPLIT ? 128 : 256;     // values a stage
+    static constexpr int KB = KIND == FP4_MX ? 2 : KIND == FP4_NV ? 4 : 1;  // scale tiles a stage and 128 rows
+    static constexpr int NB = STACK ? 1 : P * ((T + 127) / 128);            // scale tiles of x beside each of w's
+    static constexpr int A_BYTES = 128 * 128, B_TILE = T * 128, B_BYTES = P * B_TILE;
+    // what TMA counts of a weight tile: the bytes that it reads, also where it spreads codes to bytes
+    static constexpr int A_TX = KIND == FP4_SPLIT ? A_BYTES / 2 : A_BYTES;
+    static constexpr int SFA = KB * 512, SFB = KB * NB * 512;
+    static constexpr int STAGE = (A_BYTES + B_BYTES + SFA + SFB + 1023) / 1024 * 1024;
+    static constexpr int SMEM = (T <= 64 ? 110 : 224) * 1024;  // narrow tiles leave room for a second CTA
+    static constexpr int FIT = SMEM / STAGE, NS = FIT < FP4_MAX_STAGES ? FIT : FP4_MAX_STAGES;
+    static constexpr int N = STACK ? P * T : T;
+    static constexpr int ACC = N <= 32 ? 32 : N <= 64 ? 64 : N <= 128 ? 128 : 256;
+    // 256 columns: the two accumulators share 128, which are read out first
+    static constexpr int ACC_STEP = ACC == 256 ? 128 : ACC;
+    static constexpr int SF_COL = ACC == 256 ? 384 : 2 * ACC, SF_COLS = 4 * KB * (1 + NB);
+    static constexpr int COLS = SF_COL + 2 * SF_COLS, TMEM = COLS <= 64 ? 64 : COLS <= 128 ? 128 : COLS <= 256 ? 256 : 512;
+    static_assert(COLS <= 512 && NS >= 2 && N % 16 == 0 && N <= 256 && B_TILE % 1024 == 0, "tile");
+    static_assert(!STACK || N <= 128, "stacked pieces share one scale tile");
+};
+
+struct Fp4Args {
+    int M, N, Kp;        // rows of x, rows of w (of an expert), padded K
+    int ns, ktiles;      // stages along K, scale tiles along K
+    int ntn, ntiles;     // tiles along N, all tiles (dense)
+    int ks;              // CTAs that split a tile's K
+    int glu, dtype;
+    int piece_rows;      // rows of one piece of x
+    const uint8_t* wt;   // scale tiles of w, and of x
+    const uint8_t* xt;
+    const float* xf;     // factors, or NULL
+    const float* wf;
+    void* y;
+    // grouped
+    int grouped, E;
+    const int32_t* starts;
+    const int32_t* experts;
+    const int32_t* nseg;
+    int max_seg;
+};
+
+// Tile `id` of the token tiles of all segments: segment s has tiles starts[s] / T + s, ... (one number a segment may be
+// unused). The rows [r0, r1) of it.
+struct Fp4Tile {
+    int n0, r0, r1;   // first row of w (of the expert), rows of x
+    int expert, id;   // id: the tile of x's scales
+};
+
+template <int T>
+__device__ __forceinline__ bool fp4_tile(const Fp4Args& a, const int32_t* starts, int nseg, int lin, Fp4Tile& t) {
+    if (!a.grouped) {
+        const int mt = a.ntiles / a.ntn;
+        t.id = lin % mt;  // token tiles next to one another in time share the weights
+        t.n0 = lin / mt * 128;
+        t.r0 = t.id * T;
+        t.r1 = min(a.M, t.r0 + T);
+        t.expert = 0;
+        return true;
+    }
+    t.id = lin / a.ntn;
+    t.n0 = (lin - t.id * a.ntn) * 128;
+    int lo = 0, hi = nseg;  // the last segment whose first tile is not beyond id
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) / 2;
+        if (starts[mid] / T + mid <= t.id) lo = mid; else hi = mid;
+    }
+    t.r0 = starts[lo] + (t.id - (starts[lo] / T + lo)) * T;
+    t.r1 = min(starts[lo + 1], t.r0 + T);
+    t.expert = a.experts[lo];
+    if (t.r0 >= t.r1 || t.expert == a.E) return false;
+    if (t.expert < 0 || t.expert > a.E) {
+        record_status(LQ_DEV_BOUNDS);
+        return false;
+    }
+    return true;
+}
+
+__device__ __forceinline__ void fp4_store(const Fp4Args& a, int64_t at, float v) {
+    if (a.dtype == LQ_F32)
+        reinterpret_cast<float*>(a.y)[at] = v;
+    else if (a.dtype == LQ_BF16)
+        reinterpret_cast<__nv_bfloat16*>(a.y)[at] = __float2bfloat16_rn(v);
+    else
+        reinterpret_cast<__half*>(a.y)[at] = __float2half_rn(v);
+}
+
+// Output column c of a tile: row n of w, v its sum. glu: rows of w are gate 0, up 0, gate 1, ...: neighbouring lanes.
+template <typename S>
+__device__ __forceinline__ void fp4_out(const Fp4Args& a, const Fp4Tile& t, int c, int n, float v) {
+    if (a.glu) {
+        const float up = __shfl_xor_sync(0xFFFFFFFFu, v, 1);
+        if (!(n & 1) && n < a.N && t.r0 + c < t.r1) fp4_store(a, int64_t(t.r0 + c) * (a.N / 2) + n / 2, v / (1.f + __expf(-v)) * up);
+    } else if (n < a.N && t.r0 + c < t.r1) {
+        fp4_store(a, int64_t(t.r0 + c) * a.N + n, v);
+    }
+}
+
+template <typename S>
+__global__ void __launch_bounds__(FP4_THREADS, 1)
+    fp4_gemm_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_x, const Fp4Args a) {
+    constexpr int T = S::T, P = S::P, NS = S::NS;
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint64_t* full = reinterpret_cast<uint64_t*>(smem + NS * S::STAGE);
+    uint64_t* empty = full + NS;
+    uint64_t* acc_full = empty + NS;     // [2] the MMAs of a tile are done
+    uint64_t* acc_empty = acc_full + 2;  // [2] the epilogue has read what the next tile writes
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
+    int32_t* seg = reinterpret_cast<int32_t*>(tmem_slot + 2);  // [0] segments, then their starts (grouped)
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int rank = a.ks > 1 ? int(cluster_ctarank()) : 0;
+    const int first = int(blockIdx.x) / a.ks, step = int(gridDim.x) / a.ks;
+    const int s_lo = a.ns * rank / a.ks, s_hi = a.ns * (rank + 1) / a.ks;  // this CTA's stages of a tile
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < NS; ++s) {
+            mbar_init(&full[s], 1);
+            mbar_init(&empty[s], 1);
+        }
+        for (int j = 0; j < 2; ++j) {
+            mbar_init(&acc_full[j], 1);
+            mbar_init(&acc_empty[j], 4);
+        }
+        fence_barrier_init();
+    }
+    if (warp == 5) {
+        tmem_alloc(tmem_slot, S::TMEM);
+        tmem_relinquish();
+    }
+    grid_dep_launch();
+    if (a.grouped) {
+        grid_dep_wait();
+        const int n = min(*a.nseg, a.max_seg);
+        for (int i = threadIdx.x; i <= n; i += FP4_THREADS) seg[1 + i] = min(max(a.starts[i], 0), a.M);
+        if (threadIdx.x == 0) seg[0] = n;
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+    const int nseg = a.grouped ? seg[0] : 0;
+    const int32_t* starts = seg + 1;
+    const int ntiles = a.grouped ? (nseg > 0 ? (starts[nseg] / T + nseg) * a.ntn : 0) : a.ntiles;
+    bool ok = true;
+
+    if (warp == 4) {
+        // ------------------------------ producer ------------------------------
+        if (lane == 0) {
+            prefetch_tmap(&tm_w);
+            prefetch_tmap(&tm_x);
+            const uint64_t pol_w = policy_evict_first(), pol_x = policy_evict_last();
+            int it = 0;
+            bool waited = a.grouped;
+            Fp4Tile t;
+            for (int lin = first; lin < ntiles && ok; lin += step) {
+                if (!fp4_tile<T>(a, starts, nseg, lin, t)) continue;
+                const int wrow = t.expert * a.N + t.n0;
+                const uint8_t* wt = a.wt + (int64_t(t.expert) * a.ntn + t.n0 / 128) * a.ktiles * 512;
+                auto weights = [&](int kb, int s, int kt) {
+                    uint8_t* st = smem + s * S::STAGE;
+                    tma_load_2d(st, &tm_w, &full[s], kb * 128, wrow, pol_w);
+                    bulk_load(st + S::A_BYTES + S::B_BYTES, wt + int64_t(kb) * S::KB * 512, kt * 512, &full[s]);
+                };
+                // scale tiles of this stage (fewer in a row's last), and blocks of 128 tokens that exist
+                const int xb = S::KIND == FP4_SPLIT ? S::NB : T <= 128 ? 1 : min(2, (a.M - t.r0 + 127) / 128);
+                auto tiles_of = [&](int kb) { return min(S::KB, a.ktiles - kb * S::KB); };
+                auto bytes_of = [&](int kt) { return uint32_t(S::A_TX + S::B_BYTES + kt * 512 * (1 + xb)); };
+                // Before this kernel came the split, which was launched on when the kernels before it were done: what they
+                // wrote, weights too, may be read before the split ends. A product of two 4-bit operands may follow the
+                // kernel that quantized its weights.
+                int ahead = 0;
+                if (!waited) {
+                    for (; S::KIND == FP4_SPLIT && ahead < NS && s_lo + ahead < s_hi; ++ahead) {
+                        const int kt = tiles_of(s_lo + ahead);
+                        mbar_arrive_expect_tx(&full[ahead], bytes_of(kt));
+                        weights(s_lo + ahead, ahead, kt);
+                    }
+                    grid_dep_wait();
+                    waited = true;
+                }
+                for (int kb = s_lo; kb < s_hi; ++kb, ++it) {
+                    const int s = it % NS, kt = tiles_of(kb);
+                    if (it >= NS && !(ok = mbar_wait(&empty[s], ((it / NS) - 1) & 1))) break;
+                    uint8_t* st = smem + s * S::STAGE;
+                    if (it >= ahead) {
+                        mbar_arrive_expect_tx(&full[s], bytes_of(kt));
+                        weights(kb, s, kt);
+                    }
+#pragma unroll
+                    for (int p = 0; p < P; ++p)
+                        tma_load_2d(st + S::A_BYTES + p * S::B_TILE, &tm_x, &full[s], kb * 128, p * a.piece_rows + t.r0, pol_x);
+                    uint8_t* sfb = st + S::A_BYTES + S::B_BYTES + S::SFA;
+                    if constexpr (S::KIND == FP4_SPLIT) {
+                        bulk_load(sfb, a.xt + (int64_t(t.id) * a.ktiles + kb) * S::SFB, S::SFB, &full[s]);
+                    } else {
+                        for (int b = 0; b < xb; ++b)
+                            bulk_load(sfb + b * S::SFA, a.xt + (int64_t(t.r0 / 128 + b) * a.ktiles + kb * S::KB) * 512, kt * 512,
+                                      &full[s]);
+                    }
+                }
+            }
+        }
+        __syncwarp();
+    } else if (warp == 5) {
+        // ------------------------------ MMA issuer ------------------------------
+        constexpr uint32_t idesc = fp4_idesc<S::KIND>(128, S::N);
+        int it = 0, j = 0;
+        Fp4Tile t;
+        for (int lin = first; lin < ntiles && ok; lin += step) {
+            if (!fp4_tile<T>(a, starts, nseg, lin, t)) continue;
+            if constexpr (S::ACC == 256) {
+                if (j >= 1) ok = mbar_wait(&acc_empty[0], (j - 1) & 1);
+            } else {
+                if (j >= 2) ok = mbar_wait(&acc_empty[j & 1], ((j >> 1) - 1) & 1);
+            }
+            if (!ok) break;
+            tc_fence_after();
+            const uint32_t acc = tmem + uint32_t((j & 1) * S::ACC_STEP);
+            for (int kb = s_lo; kb < s_hi && ok; ++kb, ++it) {
+                const int s = it % NS;
+                // the scales' place: the MMAs of the stage before last are done
+                if (it >= 2) ok = mbar_wait(&empty[(it - 2) % NS], ((it - 2) / NS) & 1);
+                if (ok) ok = mbar_wait(&full[s], (it / NS) & 1);
+                if (!ok) break;
+                tc_fence_after();
+                if (lane == 0) {
+                    const int kt = min(S::KB, a.ktiles - kb * S::KB);
+                    const uint32_t a_base = smem_u32(smem + s * S::STAGE), b_base = a_base + S::A_BYTES;
+                    const uint32_t fa = b_base + S::B_BYTES, fb = fa + S::SFA;
+                    const uint32_t sfa = tmem + S::SF_COL + uint32_t(it & 1) * S::SF_COLS, sfb = sfa + 4 * S::KB;
+#pragma unroll
+                    for (int q = 0; q < S::KB; ++q)
+                        if (q < kt) {
+                            tc_copy_scales(sfa + 4 * q, umma_desc_scales(fa + q * 512));
+#pragma unroll
+                            for (int b = 0; b < S::NB; ++b)
+                                tc_copy_scales(sfb + 4 * (q * S::NB + b), umma_desc_scales(fb + (b * S::KB + q) * 512));
+                        }
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        constexpr int PER = 4 / S::KB;  // MMAs a scale tile
+                        const int q = k / PER;
+                        if (q < kt) {
+                            const uint32_t id = fp4_idesc_byte(S::KIND == FP4_MX ? 2 * (k % 2) : S::KIND == FP4_NV ? 0 : k);
+#pragma unroll
+                            for (int p = 0; p < (S::STACK ? 1 : P); ++p)
+                                tc_mma_fp4<S::KIND>(acc, umma_desc_sw128(a_base + k * 32),
+                                                    umma_desc_sw128(b_base + p * S::B_TILE + k * 32), idesc | id, sfa + 4 * q,
+                                                    sfb + 4 * (q * S::NB + p * (S::NB / (S::STACK ? 1 : P))),
+                                                    (kb > s_lo || k > 0 || p > 0) ? 1u : 0u);
+                        }
+                    }
+                    tc_commit(&empty[s]);
+                }
+                __syncwarp();
+            }
+            if (lane == 0) tc_commit(&acc_full[j & 1]);
+            __syncwarp();
+            ++j;
+        }
+    } else {
+        // ------------------------------ epilogue warps 0-3 ------------------------------
+        grid_dep_wait();
+        const float f = (a.xf ? *a.xf : 1.f) * (a.wf ? *a.wf : 1.f);
+        int j = 0;
+        Fp4Tile t;
+        for (int lin = first; lin < ntiles; lin += step) {
+            if (!fp4_tile<T>(a, starts, nseg, lin, t)) continue;
+            if (ok) ok = mbar_wait(&acc_full[j & 1], (j >> 1) & 1);
+            if (!ok) break;
+            tc_fence_after();
+            const int n = t.n0 + 32 * warp + lane;
+            const uint32_t acc = tmem + (uint32_t(32 * warp) << 16) + uint32_t((j & 1) * S::ACC_STEP);
+            float* part = reinterpret_cast<float*>(smem);  // [T][128] sums of this CTA's share of K (split K: one tile a CTA)
+#pragma unroll 1
+            for (int i = 0; i < T; i += 16) {
+                // the columns that the next tile's accumulator covers come first
+                const int c0 = S::ACC == 256 ? (i + ((j & 1) ? 0 : 128)) % 256 : i;
+                uint32_t r[16];
+                float v[16];
+                tmem_ld_32x32b_x16(acc + c0, r);
+                tmem_wait_ld();
+#pragma unroll
+                for (int c = 0; c < 16; ++c) v[c] = __uint_as_float(r[c]);
+                if constexpr (S::STACK) {
+#pragma unroll
+                    for (int p = 1; p < P; ++p) {
+                        tmem_ld_32x32b_x16(acc + p * T + c0, r);
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int c = 0; c < 16; ++c) v[c] += __uint_as_float(r[c]);
+                    }
+                }
+                if (S::ACC == 256 && i + 16 == 128) {
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&acc_empty[0]);
+                }
+                if (a.ks > 1) {
+#pragma unroll
+                    for (int c = 0; c < 16; ++c) part[(c0 + c) * 128 + 32 * warp + lane] = v[c];
+                } else {
+#pragma unroll
+                    for (int c = 0; c < 16; ++c) fp4_out<S>(a, t, c0 + c, n, v[c] * f);
+                }
+            }
+            if constexpr (S::ACC != 256) {
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&acc_empty[j & 1]);
+            }
+            ++j;
+        }
+    }
+    if (a.ks > 1) {
+        // the CTAs of a cluster have one tile: each writes out the columns c with c % ks == its rank
+        __syncwarp();
+        cluster_sync();
+        Fp4Tile t;
+        if (warp < 4 && first < ntiles && fp4_tile<T>(a, starts, nseg, first, t)) {
+            const float f = (a.xf ? *a.xf : 1.f) * (a.wf ? *a.wf : 1.f);
+            const uint32_t part = smem_u32(smem) + (32 * warp + lane) * 4;
+            for (int c = rank; c < T && t.r0 + c < t.r1; c += a.ks) {
+                float v = 0.f;
+                for (int q = 0; q < a.ks; ++q) v += ld_dsmem_f(map_peer(part + c * 512, q));
+                fp4_out<S>(a, t, c, t.n0 + 32 * warp + lane, v * f);
+            }
+        }
+        __syncwarp();
+        cluster_sync();
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 5) {
+        tc_fence_after();
+        tmem_dealloc(tmem, S::TMEM);
+    }
+}
+
+// ---- activations of 16 bits in e4m3 pieces ---------------------------------------------------------
+
+struct SplitArgs {
+    const void* x;
+    int64_t x_row;
+    int rows, K, ktiles, nb, stack, T;
+    bool vec;
+    uint8_t* pieces;  // (P, rows, Kp)
+    uint8_t* tiles;   // (token tile, K tile, nb, 512)
+    const int32_t* order;  // row j is row order[j] / gather of x; NULL: row j
+    int gather, src_rows;
+    int grouped, max_seg;
+    const int32_t* starts;
+    const int32_t* nseg;
+};
+
+template <typename T16>
+__device__ __forceinline__ void split_load8(const T16* row, int k0, int K, bool vec, float (&v)[8]) {
+    if (vec && k0 + 8 <= K) {
+        const uint4 q = *reinterpret_cast<const uint4*>(row + k0);
+        const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = F16Traits<T16>::to_f32(w[i >> 1] >> (16 * (i & 1)) & 0xFFFFu);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            v[i] = k0 + i < K ? F16Traits<T16>::to_f32(reinterpret_cast<const uint16_t*>(row)[k0 + i]) : 0.f;
+    }
+}
+
+// A thread takes 8 values, four threads a group of 32.
+template <typename T16, int P>
+__global__ void __launch_bounds__(256) fp4_split_kernel(const SplitArgs a) {
+    grid_dep_wait();
+    grid_dep_launch();  // after the wait: the product reads weights ahead of this kernel's end
+    const int words = fp4_padded(a.K) / 8;
+    const int64_t n = int64_t(a.rows) * words;
+    for (int64_t u = int64_t(blockIdx.x) * blockDim.x + threadIdx.x; u < n; u += int64_t(gridDim.x) * blockDim.x) {
+        const int row = int(u / words), word = int(u - int64_t(row) * words);
+        const uint32_t mask = 0xFFFFu << (threadIdx.x & 16);
+        int64_t src = row;
+        if (a.order) {
+            src = a.order[row] / a.gather;
+            if (src < 0 || src >= a.src_rows) {
+                record_status(LQ_DEV_BOUNDS);
+                src = 0;
+            }
+        }
+        float v[8];
+        split_load8(static_cast<const T16*>(a.x) + src * a.x_row, 8 * word, a.K, a.vec, v);
+        float top = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) asm("max.NaN.f32 %0, %1, %2;" : "=f"(top) : "f"(top), "f"(fabsf(v[i])));
+#pragma unroll
+        for (int d = 1; d < 4; d *= 2) {
+            const float o = __shfl_xor_sync(mask, top, d);
+            asm("max.NaN.f32 %0, %1, %2;" : "=f"(top) : "f"(top), "f"(o));
+        }
+        int tile = row / a.T, at = row % a.T;
+        if (a.grouped) {
+            int lo = 0, hi = min(*a.nseg, a.max_seg);
+            while (hi - lo > 1) {
+                const int mid = (lo + hi) / 2;
+                if (a.starts[mid] <= row) lo = mid; else hi = mid;
+            }
+            const int s0 = min(max(a.starts[lo], 0), row);
+            tile = s0 / a.T + lo + (row - s0) / a.T;
+            at = (row - s0) % a.T;
+        }
+        const uint32_t e = __float_as_uint(top) >> 23 & 0xFF;
+        int byte = e == 255 ? 255 : e < 7 ? 0 : int(e) - 7;
+        const float up = __uint_as_float((254u - (e == 255 ? 127u : uint32_t(byte))) << 23);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] *= up;
+        const int g = word / 4;
+        uint8_t* tl = a.tiles + (int64_t(tile) * a.ktiles + (g >> 2)) * a.nb * 512;
+#pragma unroll
+        for (int p = 0; p < P; ++p) {
+            uint32_t w[2];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const uint32_t lo = cvt_e4m3x2(v[4 * h + 1], v[4 * h]), hi = cvt_e4m3x2(v[4 * h + 3], v[4 * h + 2]);
+                w[h] = lo | hi << 16;
+                const float2 x01 = e4m3x2_to_f32(lo), x23 = e4m3x2_to_f32(hi);
+                v[4 * h] -= x01.x;
+                v[4 * h + 1] -= x01.y;
+                v[4 * h + 2] -= x23.x;
+                v[4 * h + 3] -= x23.y;
+            }
+            *reinterpret_cast<uint2*>(a.pieces + (int64_t(p) * a.rows + row) * (words * 8) + 8 * word) = make_uint2(w[0], w[1]);
+            if (word % 4 == 0) {
+                const int q = a.stack ? p * a.T + at : at;
+                tl[(a.stack ? 0 : p * ((a.T + 127) / 128) + q / 128) * 512 + fp4_tile_byte(q % 128, g)] = uint8_t(byte);
+            }
+            const int next = byte == 255 ? 255 : byte < 4 ? 0 : byte - 4;
+            const float more = __uint_as_float(uint32_t(127 + (byte == 255 ? 0 : byte - next)) << 23);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] *= more;
+            byte = next;
+        }
+    }
+}
+
+// ---- host ------------------------------------------------------------------------------------------
+
+static int launch(const void* func, int grid, int threads, size_t smem, int cluster, cudaStream_t st, void** args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(unsigned(grid));
+    cfg.blockDim = dim3(unsigned(threads));
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = unsigned(cluster);
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = cluster > 1 ? 2 : 1;
+    return cudaLaunchKernelExC(&cfg, func, args) == cudaSuccess ? LQ_OK : LQ_E_CUDA;
+}
+
+struct Fp4Call {
+    const uint8_t* x;  // codes or pieces
+    const uint32_t* w;
+    int stack;         // experts, 1 for a dense product
+    int64_t tiles;     // most tiles that the call can have
+    Fp4Args a;
+};
+
+template <typename S>
+static int gemm_t(const Fp4Call& c, cudaStream_t st) {
+    Fp4Args a = c.a;
+    a.ns = (a.Kp + S::BK - 1) / S::BK;
+    CUtensorMap tw, tx;
+    if (S::KIND == FP4_SPLIT) {
+        const uint64_t dims[2] = {uint64_t(a.Kp), uint64_t(c.stack) * a.N}, str[1] = {uint64_t(a.Kp) / 2};
+        const uint32_t box[2] = {128, 128};
+        int rc = make_tmap(&tw, CU_TENSOR_MAP_DATA_TYPE_16U4_ALIGN16B, 2, c.w, dims, str, box, CU_TENSOR_MAP_SWIZZLE_128B);
+        if (rc) return rc;
+    } else {
+        const uint64_t dims[2] = {uint64_t(a.Kp) / 2, uint64_t(c.stack) * a.N}, str[1] = {uint64_t(a.Kp) / 2};
+        const uint32_t box[2] = {128, 128};
+        int rc = make_tmap(&tw, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, c.w, dims, str, box, CU_TENSOR_MAP_SWIZZLE_128B);
+        if (rc) return rc;
+    }
+    {
+        const uint64_t row = uint64_t(a.Kp) / (S::KIND == FP4_SPLIT ? 1 : 2);
+        const uint64_t dims[2] = {row, uint64_t(S::P) * a.M}, str[1] = {row};
+        const uint32_t box[2] = {128, uint32_t(S::T)};
+        int rc = make_tmap(&tx, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, c.x, dims, str, box, CU_TENSOR_MAP_SWIZZLE_128B);
+        if (rc) return rc;
+    }
+    const int sms = device_info().sm_count;
+    const int64_t slots = int64_t(sms) * (S::T <= 64 ? 2 : 1);
+    a.ks = 1;
+    if (S::ACC != 256 && c.tiles < sms) {  // a tile's K split over the CTAs of a cluster
+        const int most = a.ns < 8 ? a.ns : 8, ks = int(sms / c.tiles);  // every CTA has a stage
+        a.ks = ks < most ? ks : most;
+    }
+    const int64_t grid = a.ks > 1 ? c.tiles * a.ks : c.tiles < slots ? c.tiles : slots;
+    const size_t smem = 1024 + size_t(S::NS) * S::STAGE + (2 * S::NS + 4) * 8 + 8 + (a.grouped ? (FP4_MAX_SEGMENTS + 2) * 4 : 0);
+    static_assert(S::ACC == 256 || S::T * 512 <= S::NS * S::STAGE, "the partial sums of a split fit the ring");
+    auto kern = fp4_gemm_kernel<S>;
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem)) != cudaSuccess) return LQ_E_CUDA;
+    void* args[] = {&tw, &tx, &a};
+    return launch(reinterpret_cast<const void*>(kern), int(grid), FP4_THREADS, smem, a.ks, st, args);
+}
+
+template <int KIND, int P>
+static int gemm_tokens(const Fp4Call& c, int T, cudaStream_t st) {
+    switch (T) {
+        case 16: return gemm_t<Fp4Shape<KIND, P, 16>>(c, st);
+        case 32: return gemm_t<Fp4Shape<KIND, P, 32>>(c, st);
+        case 64: return gemm_t<Fp4Shape<KIND, P, 64>>(c, st);
+        case 128: return gemm_t<Fp4Shape<KIND, P, 128>>(c, st);
+        default:
+            if constexpr (P == 1) return gemm_t<Fp4Shape<KIND, P, 256>>(c, st);
+            return LQ_E_SHAPE;
+    }
+}
+
+// Tokens a tile. A product of both in 4 bits has scale tiles of 128 tokens, so narrower tiles only where one holds them all.
+static int tile_tokens(int rows, int P) {
+    return rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : rows <= 128 || P > 1 ? 128 : 256;
+}
+
+int fp4_qmm_run(const uint32_t* xc, const uint8_t* xt, const float* xf, const uint32_t* wc, const uint8_t* wt, const float* wf,
+                int M, int N, int K, int mode, int glu, int dtype, void* y, cudaStream_t st) {
+    Fp4Call c = {};
+    const int T = tile_tokens(M, 1);
+    c.x = reinterpret_cast<const uint8_t*>(xc);
+    c.w = wc;
+    c.stack = 1;
+    Fp4Args& a = c.a;
+    a.M = M;
+    a.N = N;
+    a.Kp = fp4_padded(K);
+    a.ktiles = fp4_ktiles(K, mode);
+    a.ntn = (N + 127) / 128;
+    c.tiles = int64_t(a.ntn) * ((M + T - 1) / T);
+    if (c.tiles > INT32_MAX) return LQ_E_SHAPE;
+    a.ntiles = int(c.tiles);
+    a.glu = glu;
+    a.dtype = dtype;
+    a.wt = wt;
+    a.xt = xt;
+    a.xf = xf;
+    a.wf = wf;
+    a.y = y;
+    return mode == LQ_MXFP4 ? gemm_tokens<FP4_MX, 1>(c, T, st) : gemm_tokens<FP4_NV, 1>(c, T, st);
+}
+
+// Token tiles of the rows of a call (grouped: one number a segment may go unused), and the bytes of the split's results.
+static int64_t split_tiles(int rows, int T, int segments) { return segments ? rows / T + segments : (rows + T - 1) / T; }
+static int split_blocks(int P, int T) { return T <= 32 ? 1 : P * ((T + 127) / 128); }
+static size_t split_pieces_bytes(int rows, int K, int P) { return (size_t(P) * rows * fp4_padded(K) + 511) / 512 * 512; }
+
+// Tokens a tile of rows that are dealt out to segments: twice the average, so that most segments are one tile.
+static int grouped_tokens(int rows, int segments, int max_rows, int P) {
+    const int64_t want = 2 * int64_t(rows) / (segments > 0 ? segments : 1);
+    return tile_tokens(int(want < max_rows ? want : max_rows), P);
+}
+
+size_t fp4_linear_workspace_bytes(int rows, int K, int dtype, int segments, int max_rows) {
+    const int P = dtype == LQ_BF16 ? 2 : 3, T = segments ? grouped_tokens(rows, segments, max_rows, P) : tile_tokens(rows, P);
+    return split_pieces_bytes(rows, K, P) +
+           size_t(split_tiles(rows, T, segments)) * fp4_ktiles(K, LQ_MXFP4) * split_blocks(P, T) * 512;
+}
+
+int fp4_linear_run(const Fp4Linear& l, cudaStream_t st) {
+    const int P = l.dtype == LQ_BF16 ? 2 : 3;
+    const int T = l.segments ? grouped_tokens(l.rows, l.segments, l.max_rows, P) : tile_tokens(l.rows, P);
+    uint8_t* ws = static_cast<uint8_t*>(l.ws);
+    SplitArgs s = {};
+    s.x = l.x;
+    s.x_row = l.x_row;
+    s.rows = l.rows;
+    s.K = l.K;
+    s.ktiles = fp4_ktiles(l.K, LQ_MXFP4);
+    s.nb = split_blocks(P, T);
+    s.stack = T <= 32;
+    s.T = T;
+    s.vec = aligned(l.x, 16) && l.x_row % 8 == 0;
+    s.pieces = ws;
+    s.tiles = ws + split_pieces_bytes(l.rows, l.K, P);
+    s.order = l.order;
+    s.gather = l.gather;
+    s.src_rows = l.src_rows;
+    s.grouped = l.segments > 0;
+    s.max_seg = l.segments;
+    s.starts = l.starts;
+    s.nseg = l.nseg;
+    const int64_t units = int64_t(l.rows) * (fp4_padded(l.K) / 8);
+    const int64_t most = int64_t(device_info().sm_count) * 16, blocks = (units + 255) / 256;
+    const void* split = l.dtype == LQ_BF16 ? reinterpret_cast<const void*>(fp4_split_kernel<__nv_bfloat16, 2>)
+                                           : reinterpret_cast<const void*>(fp4_split_kernel<__half, 3>);
+    void* sargs[] = {&s};
+    int rc = launch(split, int(blocks < most ? blocks : most), 256, 0, 1, st, sargs);
+    if (rc) return rc;
+    Fp4Call c = {};
+    c.x = s.pieces;
+    c.w = l.wc;
+    c.stack = l.segments ? l.E : 1;
+    Fp4Args& a = c.a;
+    a.M = l.rows;
+    a.N = l.N;
+    a.Kp = fp4_padded(l.K);
+    a.ktiles = s.ktiles;
+    a.ntn = (l.N + 127) / 128;
+    c.tiles = split_tiles(l.rows, T, l.segments) * a.ntn;
+    if (c.tiles > INT32_MAX) return LQ_E_SHAPE;
+    a.ntiles = int(c.tiles);
+    a.glu = l.glu;
+    a.dtype = l.dtype;
+    a.piece_rows = l.rows;
+    a.wt = l.wt;
+    a.xt = s.tiles;
+    a.y = l.y;
+    a.grouped = l.segments > 0;
+    a.E = l.E;
+    a.starts = l.starts;
+    a.experts = l.experts;
+    a.nseg = l.nseg;
+    a.max_seg = l.segments;
+    return l.dtype == LQ_BF16 ? gemm_tokens<FP4_SPLIT, 2>(c, T, st) : gemm_tokens<FP4_SPLIT, 3>(c, T, st);
+}
+
+}  // namespace lq

@@ -1,0 +1,32 @@
+// Host entry points of the microscaled 4-bit kernels (fp4_quant.cu, fp4_gemm.cu), for fp4_api.cu.
+#pragma once
+
+#include <cuda_runtime.h>
+#include <stddef.h>
+#include <stdint.h>
+
+namespace lq {
+
+int fp4_quantize_run(const void* x, int dt, int64_t x_row, int rows, int K, int mode, const float* factor, uint32_t* codes,
+                     uint8_t* tiles, cudaStream_t st);
+int fp4_dequantize_run(const uint32_t* codes, const uint8_t* tiles, int stack, int rows, int K, int mode, const float* factor,
+                       int dt, void* out, cudaStream_t st);
+int fp4_qmm_run(const uint32_t* xc, const uint8_t* xt, const float* xf, const uint32_t* wc, const uint8_t* wt, const float* wf,
+                int M, int N, int K, int mode, int glu, int dtype, void* y, cudaStream_t st);
+
+// A product of 16-bit rows with mxfp4 weights; segments > 0: grouped over at most that many segments.
+struct Fp4Linear {
+    const void* x;
+    int64_t x_row;
+    const int32_t *order, *starts, *experts, *nseg;
+    int gather, src_rows, segments, max_rows, E;
+    const uint32_t* wc;
+    const uint8_t* wt;
+    int rows, N, K, glu, dtype;
+    void* y;
+    void* ws;
+};
+size_t fp4_linear_workspace_bytes(int rows, int K, int dtype, int segments, int max_rows);
+int fp4_linear_run(const Fp4Linear& l, cudaStream_t st);
+
+}  // namespace lq

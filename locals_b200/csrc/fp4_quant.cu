@@ -1,0 +1,230 @@
+// Microscaled 4-bit floating point in and out: quantize, dequantize, and the e4m3 pieces that 16-bit activations enter the
+// block-scaled product as.
+//
+// quantize: a thread takes 8 values (one word of codes), a group is 4 (mxfp4) or 2 (nvfp4) threads, its largest magnitude
+// found with shuffles. mxfp4: scale 2^(floor(log2 amax) - 2), at least 2^-127: the exponent field of amax less 2, so that no
+// logarithm is taken, and x 2^-e is exact. nvfp4: scale = the e4m3 number nearest to amax / (6 f), f the matrix' factor, and
+// codes nearest to x / (scale f), both decided as in exact arithmetic: with 32-bit arithmetic where it is clear, in
+// 64 bits where a value lies within its error of the middle between two codes.
+#include <cuda_runtime.h>
+
+#include "fp4.cuh"
+#include "fp4_host.h"
+#include "lq_host.h"
+
+namespace lq {
+
+__device__ __forceinline__ float to_f32(uint16_t h, __nv_bfloat16) { return __uint_as_float(uint32_t(h) << 16); }
+__device__ __forceinline__ float to_f32(uint16_t h, __half) { return __half2float(*reinterpret_cast<__half*>(&h)); }
+
+// Values [k0, k0 + 8) of a row of K, zeros beyond it; `vec`: the row starts on a 16-byte boundary.
+template <typename T>
+__device__ __forceinline__ void load8(const T* row, int k0, int K, bool vec, float (&v)[8]) {
+    if (vec && k0 + 8 <= K) {
+        if constexpr (sizeof(T) == 4) {
+            const float4 a = *reinterpret_cast<const float4*>(row + k0), b = *reinterpret_cast<const float4*>(row + k0 + 4);
+            v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+            v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+        } else {
+            const uint4 a = *reinterpret_cast<const uint4*>(row + k0);
+            const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = to_f32(uint16_t(w[i >> 1] >> (16 * (i & 1))), T());
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            if (k0 + i >= K)
+                v[i] = 0.f;
+            else if constexpr (sizeof(T) == 4)
+                v[i] = row[k0 + i];
+            else
+                v[i] = to_f32(reinterpret_cast<const uint16_t*>(row)[k0 + i], T());
+        }
+    }
+}
+
+// The largest magnitude of 8 values; not a number if one of them is.
+__device__ __forceinline__ float amax_nan(float a, float b) {
+    float d;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+    return d;
+}
+
+__device__ __forceinline__ float amax8(const float (&v)[8]) {
+    float m = fabsf(v[0]);
+#pragma unroll
+    for (int i = 1; i < 8; ++i) m = amax_nan(m, fabsf(v[i]));
+    return m;
+}
+
+__device__ __forceinline__ uint32_t codes8(const float (&v)[8]) {
+    uint32_t w = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w |= cvt_e2m1x2(v[2 * i + 1], v[2 * i]) << (8 * i);
+    return w;
+}
+
+// The e4m3 byte nearest to t >= 0 (ties to even), at most 448.
+__device__ __forceinline__ uint32_t e4m3_of(double t) {
+    if (!(t < 448.0)) return t != t ? 0x7Fu : 0x7Eu;
+    int e = int((__double_as_longlong(t) >> 52) & 0x7FF) - 1023;
+    e = e < -6 ? -6 : e;
+    const double n = rint(t * __longlong_as_double((long long)(1023 + 3 - e) << 52));
+    return uint32_t((e + 6) * 8 + int(n));
+}
+
+// The code nearest to |x| / s, decided in 64 bits (s has at most 28 bits, so that s times a middle is exact).
+__device__ __noinline__ uint32_t code_exact(float x, double s) {
+    const double a = fabs(double(x));
+    uint32_t c = (a > 0.25 * s) + (a >= 0.75 * s) + (a > 1.25 * s) + (a >= 1.75 * s) + (a > 2.5 * s) + (a >= 3.5 * s) + (a > 5.0 * s);
+    return c | (__float_as_uint(x) >> 31 << 3);
+}
+
+template <typename T, int MODE>
+__global__ void __launch_bounds__(256) fp4_quantize_kernel(const T* __restrict__ x, int64_t x_row, int rows, int K, bool vec,
+                                                           const float* __restrict__ factor, uint32_t* __restrict__ codes,
+                                                           uint8_t* __restrict__ tiles) {
+    constexpr int LANES = MODE == LQ_MXFP4 ? 4 : 2;  // threads a group
+    const int words = fp4_padded(K) / 8, ktiles = fp4_ktiles(K, MODE);
+    grid_dep_wait();
+    const float f = MODE == LQ_NVFP4 && factor ? *factor : 1.f;
+    const int64_t n = int64_t(rows) * words;  // a multiple of 16
+    for (int64_t u = int64_t(blockIdx.x) * blockDim.x + threadIdx.x; u < n; u += int64_t(gridDim.x) * blockDim.x) {
+        const int row = int(u / words), word = int(u - int64_t(row) * words);
+        const uint32_t mask = 0xFFFFu << (threadIdx.x & 16);  // half a warp is inside or outside together
+        float v[8];
+        load8(x + int64_t(row) * x_row, 8 * word, K, vec, v);
+        float top = amax8(v);
+#pragma unroll
+        for (int d = 1; d < LANES; d *= 2) top = amax_nan(top, __shfl_xor_sync(mask, top, d));
+        uint32_t byte, w;
+        if constexpr (MODE == LQ_MXFP4) {
+            const uint32_t e = __float_as_uint(top) >> 23 & 0xFF;
+            byte = e == 255 ? 255u : e < 2 ? 0u : e - 2;
+            const float up = __uint_as_float((254u - (byte == 255 ? 127u : byte)) << 23);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] *= up;
+            w = codes8(v);
+        } else {
+            byte = top == INFINITY ? 0x7Fu : e4m3_of(double(top) / (6.0 * double(f)));
+            const float s = fp4_scale_value(byte, LQ_NVFP4);
+            w = 0;
+            if (byte != 0 && byte != 0x7F) {
+                const double sf = double(s) * double(f);
+                const float r = __frcp_rn(float(sf));
+                float lo[8], hi[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const float t = v[i] * r;
+                    lo[i] = t * (1.f - 0x1p-20f);
+                    hi[i] = t * (1.f + 0x1p-20f);
+                }
+                w = codes8(lo);
+                // (the reciprocal of a factor near the ends of the range is no normal number: 64 bits then)
+                if (w != codes8(hi) || !(r > 0x1p-126f && r < 0x1p127f)) {
+                    w = 0;
+#pragma unroll 1
+                    for (int i = 0; i < 8; ++i) w |= code_exact(v[i], sf) << (4 * i);
+                }
+            }
+        }
+        codes[u] = w;
+        const int g = word / LANES;
+        if (word % LANES == 0)
+            tiles[(int64_t(row >> 7) * ktiles + (g >> 2)) * 512 + fp4_tile_byte(row & 127, g)] = uint8_t(byte);
+    }
+}
+
+template <typename T>
+__device__ __forceinline__ T from_f32(float v);
+template <>
+__device__ __forceinline__ float from_f32<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+
+template <typename T, int MODE>
+__global__ void __launch_bounds__(256) fp4_dequantize_kernel(const uint32_t* __restrict__ codes,
+                                                             const uint8_t* __restrict__ tiles, int stack, int rows, int K,
+                                                             const float* __restrict__ factor, T* __restrict__ out, bool vec) {
+    constexpr int GROUP = MODE == LQ_MXFP4 ? 32 : 16;
+    const int stored = fp4_padded(K) / 8, words = (K + 7) / 8, ktiles = fp4_ktiles(K, MODE), rtiles = (rows + 127) / 128;
+    grid_dep_wait();
+    const float f = factor ? *factor : 1.f;
+    const int64_t n = int64_t(stack) * rows * words;
+    for (int64_t u = int64_t(blockIdx.x) * blockDim.x + threadIdx.x; u < n; u += int64_t(gridDim.x) * blockDim.x) {
+        const int64_t at = u / words;  // row of the stack
+        const int word = int(u - at * words), e = int(at / rows), row = int(at - int64_t(e) * rows);
+        const int g = word * 8 / GROUP;
+        const float s = fp4_scale_value(
+            tiles[((int64_t(e) * rtiles + (row >> 7)) * ktiles + (g >> 2)) * 512 + fp4_tile_byte(row & 127, g)], MODE);
+        const uint32_t w = codes[at * stored + word];
+        T* dst = out + at * K + 8 * word;
+        alignas(16) T v[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const uint32_t c = w >> (4 * i) & 7;  // 0, 0.5, then (2 + m) 2^(e - 2)
+            const float a = c < 2 ? 0.5f * c : __uint_as_float((127 - 1 + (c >> 1)) << 23 | (c & 1) << 22);
+            v[i] = from_f32<T>((w >> (4 * i) & 8 ? -a : a) * s * f);
+        }
+        if (vec) {
+#pragma unroll
+            for (int i = 0; i < int(8 * sizeof(T) / 16); ++i) reinterpret_cast<uint4*>(dst)[i] = reinterpret_cast<uint4*>(v)[i];
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (8 * word + i < K) dst[i] = v[i];
+        }
+    }
+}
+
+// ---- host ----
+
+static int spread(int64_t units, int threads) {
+    const int64_t blocks = (units + threads - 1) / threads, most = int64_t(device_info().sm_count) * 16;
+    return int(blocks < most ? blocks : most);
+}
+
+template <typename T>
+static int quantize_t(const void* x, int64_t x_row, int rows, int K, int mode, const float* factor, uint32_t* codes,
+                      uint8_t* tiles, cudaStream_t st) {
+    const int grid = spread(int64_t(rows) * (fp4_padded(K) / 8), 256);
+    const T* xs = static_cast<const T*>(x);
+    const bool vec = aligned(x, 16) && x_row * int64_t(sizeof(T)) % 16 == 0;
+    if (mode == LQ_MXFP4)
+        fp4_quantize_kernel<T, LQ_MXFP4><<<grid, 256, 0, st>>>(xs, x_row, rows, K, vec, factor, codes, tiles);
+    else
+        fp4_quantize_kernel<T, LQ_NVFP4><<<grid, 256, 0, st>>>(xs, x_row, rows, K, vec, factor, codes, tiles);
+    return cuda_status(cudaGetLastError());
+}
+
+int fp4_quantize_run(const void* x, int dt, int64_t x_row, int rows, int K, int mode, const float* factor, uint32_t* codes,
+                     uint8_t* tiles, cudaStream_t st) {
+    if (dt == LQ_F32) return quantize_t<float>(x, x_row, rows, K, mode, factor, codes, tiles, st);
+    if (dt == LQ_F16) return quantize_t<__half>(x, x_row, rows, K, mode, factor, codes, tiles, st);
+    return quantize_t<__nv_bfloat16>(x, x_row, rows, K, mode, factor, codes, tiles, st);
+}
+
+template <typename T>
+static int dequantize_t(const uint32_t* codes, const uint8_t* tiles, int stack, int rows, int K, int mode, const float* factor,
+                        void* out, cudaStream_t st) {
+    const int grid = spread(int64_t(stack) * rows * ((K + 7) / 8), 256);
+    T* o = static_cast<T*>(out);
+    const bool vec = K % 8 == 0 && aligned(out, 16);
+    if (mode == LQ_MXFP4)
+        fp4_dequantize_kernel<T, LQ_MXFP4><<<grid, 256, 0, st>>>(codes, tiles, stack, rows, K, factor, o, vec);
+    else
+        fp4_dequantize_kernel<T, LQ_NVFP4><<<grid, 256, 0, st>>>(codes, tiles, stack, rows, K, factor, o, vec);
+    return cuda_status(cudaGetLastError());
+}
+
+int fp4_dequantize_run(const uint32_t* codes, const uint8_t* tiles, int stack, int rows, int K, int mode, const float* factor,
+                       int dt, void* out, cudaStream_t st) {
+    if (dt == LQ_F32) return dequantize_t<float>(codes, tiles, stack, rows, K, mode, factor, out, st);
+    if (dt == LQ_F16) return dequantize_t<__half>(codes, tiles, stack, rows, K, mode, factor, out, st);
+    return dequantize_t<__nv_bfloat16>(codes, tiles, stack, rows, K, mode, factor, out, st);
+}
+
+}  // namespace lq
