@@ -69,11 +69,77 @@ __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t b
                  : "memory");
 }
 
-// ---- block-scaled tcgen05 ----
+// ---- pairs of CTAs ----
 
-// One scale tile (512 bytes of shared memory, rows of 16 bytes) to 4 columns of tensor memory, in all four lane quarters.
+// Arrive on the barrier at this offset of another CTA of the cluster.
+__device__ __forceinline__ void mbar_arrive_peer(uint64_t* bar, uint32_t rank) {
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(map_peer(smem_u32(bar), rank)) : "memory");
+}
+
+// mbar_wait for a barrier that another CTA of the cluster arrives on.
+__device__ __forceinline__ bool mbar_wait_cluster(uint64_t* bar, uint32_t parity) {
+    for (uint32_t i = 0; i < LQ_SPIN_LIMIT; ++i) {
+        uint32_t ok;
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+            "selp.u32 %0, 1, 0, p;\n\t}"
+            : "=r"(ok)
+            : "r"(smem_u32(bar)), "r"(parity)
+            : "memory");
+        if (ok) return true;
+    }
+    record_status(LQ_DEV_TIMEOUT);
+    return false;
+}
+
+template <int CG>
+__device__ __forceinline__ bool mbar_wait_cg(uint64_t* bar, uint32_t parity) {
+    return CG == 1 ? mbar_wait(bar, parity) : mbar_wait_cluster(bar, parity);
+}
+
+// ---- block-scaled tcgen05; CG: CTAs that work on a tile (1, or a pair whose lower rank issues for both) ----
+
+template <int CG>
+__device__ __forceinline__ void tc_alloc(uint32_t* dst_smem, uint32_t ncols) {
+    if constexpr (CG == 1) {
+        tmem_alloc(dst_smem, ncols);
+        tmem_relinquish();
+    } else {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(dst_smem)), "r"(ncols)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    }
+}
+
+template <int CG>
+__device__ __forceinline__ void tc_dealloc(uint32_t taddr, uint32_t ncols) {
+    if constexpr (CG == 1)
+        tmem_dealloc(taddr, ncols);
+    else
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(ncols) : "memory");
+}
+
+// Arrive on `bar` (of both CTAs of a pair) once every tcgen05 operation issued so far has completed.
+template <int CG>
+__device__ __forceinline__ void tc_commit_all(uint64_t* bar) {
+    if constexpr (CG == 1)
+        tc_commit(bar);
+    else
+        asm volatile(
+            "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(smem_u32(bar)),
+            "h"(uint16_t(3))
+            : "memory");
+}
+
+// One scale tile (512 bytes of shared memory, rows of 16 bytes) to 4 columns of tensor memory, in all four lane quarters (of
+// a pair: in each CTA from its own shared memory).
+template <int CG>
 __device__ __forceinline__ void tc_copy_scales(uint32_t taddr, uint64_t desc) {
-    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+    if constexpr (CG == 1)
+        asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+    else
+        asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
 }
 
 // Shared-memory descriptor of unswizzled 8-row x 16-byte core matrices that follow one another (128 bytes apart).
@@ -94,33 +160,24 @@ __host__ __device__ constexpr uint32_t fp4_idesc(int M, int N) {
 }
 __host__ __device__ constexpr uint32_t fp4_idesc_byte(int id) { return (uint32_t(id) << 4) | (uint32_t(id) << 29); }
 
-template <int KIND>
+#define LQ_FP4_MMA(CG_, FORM_)                                                                                         \
+    asm volatile(                                                                                                       \
+        "{\n\t.reg .pred p;\n\t"                                                                                        \
+        "setp.ne.b32 p, %6, 0;\n\t"                                                                                     \
+        "tcgen05.mma.cta_group::" CG_ ".kind::" FORM_ " [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d_tmem),            \
+        "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(sa), "r"(sb), "r"(accumulate)                                         \
+        : "memory")
+
+template <int KIND, int CG>
 __device__ __forceinline__ void tc_mma_fp4(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t sa,
                                            uint32_t sb, uint32_t accumulate) {
-    if constexpr (KIND == FP4_MX)
-        asm volatile(
-            "{\n\t.reg .pred p;\n\t"
-            "setp.ne.b32 p, %6, 0;\n\t"
-            "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(
-                d_tmem),
-            "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(sa), "r"(sb), "r"(accumulate)
-            : "memory");
-    else if constexpr (KIND == FP4_NV)
-        asm volatile(
-            "{\n\t.reg .pred p;\n\t"
-            "setp.ne.b32 p, %6, 0;\n\t"
-            "tcgen05.mma.cta_group::1.kind::mxf4nvf4.block_scale.scale_vec::4X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(
-                d_tmem),
-            "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(sa), "r"(sb), "r"(accumulate)
-            : "memory");
-    else
-        asm volatile(
-            "{\n\t.reg .pred p;\n\t"
-            "setp.ne.b32 p, %6, 0;\n\t"
-            "tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(
-                d_tmem),
-            "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(sa), "r"(sb), "r"(accumulate)
-            : "memory");
+    if constexpr (KIND == FP4_MX && CG == 1) LQ_FP4_MMA("1", "mxf4.block_scale.scale_vec::2X");
+    if constexpr (KIND == FP4_MX && CG == 2) LQ_FP4_MMA("2", "mxf4.block_scale.scale_vec::2X");
+    if constexpr (KIND == FP4_NV && CG == 1) LQ_FP4_MMA("1", "mxf4nvf4.block_scale.scale_vec::4X");
+    if constexpr (KIND == FP4_NV && CG == 2) LQ_FP4_MMA("2", "mxf4nvf4.block_scale.scale_vec::4X");
+    if constexpr (KIND == FP4_SPLIT && CG == 1) LQ_FP4_MMA("1", "mxf8f6f4.block_scale.scale_vec::1X");
+    if constexpr (KIND == FP4_SPLIT && CG == 2) LQ_FP4_MMA("2", "mxf8f6f4.block_scale.scale_vec::1X");
 }
+#undef LQ_FP4_MMA
 
 }  // namespace lq

@@ -29,14 +29,15 @@ constexpr int FP4_THREADS = 192;
 constexpr int FP4_MAX_STAGES = 10;
 constexpr int FP4_MAX_SEGMENTS = 2048;
 
-template <int KIND_, int P_, int T_>
+template <int KIND_, int P_, int T_, int CG_ = 1>
 struct Fp4Shape {
     static constexpr int KIND = KIND_, P = P_, T = T_;
+    static constexpr int CG = CG_;  // CTAs a tile: a pair has 128 rows of w and half of the tokens each
     static constexpr bool STACK = KIND == FP4_SPLIT && T <= 32;  // a token's pieces as columns of one MMA
     static constexpr int BK = KIND == FP4_SPLIT ? 128 : 256;     // values a stage
     static constexpr int KB = KIND == FP4_MX ? 2 : KIND == FP4_NV ? 4 : 1;  // scale tiles a stage and 128 rows
     static constexpr int NB = STACK ? 1 : P * ((T + 127) / 128);            // scale tiles of x beside each of w's
-    static constexpr int A_BYTES = 128 * 128, B_TILE = T * 128, B_BYTES = P * B_TILE;
+    static constexpr int A_BYTES = 128 * 128, B_TILE = T / CG * 128, B_BYTES = P * B_TILE;
     // what TMA counts of a weight tile: the bytes that it reads, also where it spreads codes to bytes
     static constexpr int A_TX = KIND == FP4_SPLIT ? A_BYTES / 2 : A_BYTES;
     static constexpr int SFA = KB * 512, SFB = KB * NB * 512;
@@ -57,6 +58,7 @@ struct Fp4Args {
     int M, N, Kp;        // rows of x, rows of w (of an expert), padded K
     int ns, ktiles;      // stages along K, scale tiles along K
     int ntn, ntiles;     // tiles along N, all tiles (dense)
+    int rtiles;          // scale tiles along N
     int ks;              // CTAs that split a tile's K
     int glu, dtype;
     int piece_rows;      // rows of one piece of x
@@ -80,19 +82,20 @@ struct Fp4Tile {
     int expert, id;   // id: the tile of x's scales
 };
 
-template <int T>
+template <typename S>
 __device__ __forceinline__ bool fp4_tile(const Fp4Args& a, const int32_t* starts, int nseg, int lin, Fp4Tile& t) {
+    constexpr int T = S::T, ROWS = 128 * S::CG;
     if (!a.grouped) {
         const int mt = a.ntiles / a.ntn;
         t.id = lin % mt;  // token tiles next to one another in time share the weights
-        t.n0 = lin / mt * 128;
+        t.n0 = lin / mt * ROWS;
         t.r0 = t.id * T;
         t.r1 = min(a.M, t.r0 + T);
         t.expert = 0;
         return true;
     }
     t.id = lin / a.ntn;
-    t.n0 = (lin - t.id * a.ntn) * 128;
+    t.n0 = (lin - t.id * a.ntn) * ROWS;
     int lo = 0, hi = nseg;  // the last segment whose first tile is not beyond id
     while (hi - lo > 1) {
         const int mid = (lo + hi) / 2;
@@ -132,35 +135,37 @@ __device__ __forceinline__ void fp4_out(const Fp4Args& a, const Fp4Tile& t, int 
 template <typename S>
 __global__ void __launch_bounds__(FP4_THREADS, 1)
     fp4_gemm_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_x, const Fp4Args a) {
-    constexpr int T = S::T, P = S::P, NS = S::NS;
+    constexpr int T = S::T, P = S::P, NS = S::NS, CG = S::CG;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint64_t* full = reinterpret_cast<uint64_t*>(smem + NS * S::STAGE);
     uint64_t* empty = full + NS;
-    uint64_t* acc_full = empty + NS;     // [2] the MMAs of a tile are done
+    uint64_t* peer = empty + NS;         // the other CTA's stage is full (a pair's lower rank)
+    uint64_t* acc_full = peer + NS;      // [2] the MMAs of a tile are done
     uint64_t* acc_empty = acc_full + 2;  // [2] the epilogue has read what the next tile writes
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
     int32_t* seg = reinterpret_cast<int32_t*>(tmem_slot + 2);  // [0] segments, then their starts (grouped)
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int rank = a.ks > 1 ? int(cluster_ctarank()) : 0;
-    const int first = int(blockIdx.x) / a.ks, step = int(gridDim.x) / a.ks;
-    const int s_lo = a.ns * rank / a.ks, s_hi = a.ns * (rank + 1) / a.ks;  // this CTA's stages of a tile
+    const int rank = CG == 2 || a.ks > 1 ? int(cluster_ctarank()) : 0;
+    const int share = CG == 2 ? 2 : a.ks, half = CG == 2 ? rank : 0;
+    const int first = int(blockIdx.x) / share, step = int(gridDim.x) / share;
+    const int s_lo = CG == 2 ? 0 : a.ns * rank / a.ks, s_hi = CG == 2 ? a.ns : a.ns * (rank + 1) / a.ks;  // stages of a tile
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < NS; ++s) {
             mbar_init(&full[s], 1);
             mbar_init(&empty[s], 1);
+            mbar_init(&peer[s], 1);
         }
         for (int j = 0; j < 2; ++j) {
             mbar_init(&acc_full[j], 1);
-            mbar_init(&acc_empty[j], 4);
+            mbar_init(&acc_empty[j], 4 * CG);
         }
         fence_barrier_init();
     }
     if (warp == 5) {
-        tmem_alloc(tmem_slot, S::TMEM);
-        tmem_relinquish();
+        tc_alloc<CG>(tmem_slot, S::TMEM);
     }
     grid_dep_launch();
     if (a.grouped) {
@@ -170,7 +175,10 @@ __global__ void __launch_bounds__(FP4_THREADS, 1)
         if (threadIdx.x == 0) seg[0] = n;
     }
     tc_fence_before();
-    __syncthreads();
+    if constexpr (CG == 2)
+        cluster_sync();
+    else
+        __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
     const int nseg = a.grouped ? seg[0] : 0;
@@ -188,18 +196,20 @@ __global__ void __launch_bounds__(FP4_THREADS, 1)
             bool waited = a.grouped;
             Fp4Tile t;
             for (int lin = first; lin < ntiles && ok; lin += step) {
-                if (!fp4_tile<T>(a, starts, nseg, lin, t)) continue;
-                const int wrow = t.expert * a.N + t.n0;
-                const uint8_t* wt = a.wt + (int64_t(t.expert) * a.ntn + t.n0 / 128) * a.ktiles * 512;
+                if (!fp4_tile<S>(a, starts, nseg, lin, t)) continue;
+                const int wrow = t.expert * a.N + t.n0 + 128 * half;
+                const int wtile = t.n0 / 128 + half;
+                const bool some = wtile < a.rtiles;  // the upper half of a pair's tile may be beyond the last row
+                const uint8_t* wt = a.wt + (int64_t(t.expert) * a.rtiles + wtile) * a.ktiles * 512;
                 auto weights = [&](int kb, int s, int kt) {
                     uint8_t* st = smem + s * S::STAGE;
                     tma_load_2d(st, &tm_w, &full[s], kb * 128, wrow, pol_w);
-                    bulk_load(st + S::A_BYTES + S::B_BYTES, wt + int64_t(kb) * S::KB * 512, kt * 512, &full[s]);
+                    if (some) bulk_load(st + S::A_BYTES + S::B_BYTES, wt + int64_t(kb) * S::KB * 512, kt * 512, &full[s]);
                 };
                 // scale tiles of this stage (fewer in a row's last), and blocks of 128 tokens that exist
                 const int xb = S::KIND == FP4_SPLIT ? S::NB : T <= 128 ? 1 : min(2, (a.M - t.r0 + 127) / 128);
                 auto tiles_of = [&](int kb) { return min(S::KB, a.ktiles - kb * S::KB); };
-                auto bytes_of = [&](int kt) { return uint32_t(S::A_TX + S::B_BYTES + kt * 512 * (1 + xb)); };
+                auto bytes_of = [&](int kt) { return uint32_t(S::A_TX + S::B_BYTES + kt * 512 * (int(some) + xb)); };
                 // Before this kernel came the split, which was launched on when the kernels before it were done: what they
                 // wrote, weights too, may be read before the split ends. A product of two 4-bit operands may follow the
                 // kernel that quantized its weights.
@@ -215,7 +225,7 @@ __global__ void __launch_bounds__(FP4_THREADS, 1)
                 }
                 for (int kb = s_lo; kb < s_hi; ++kb, ++it) {
                     const int s = it % NS, kt = tiles_of(kb);
-                    if (it >= NS && !(ok = mbar_wait(&empty[s], ((it / NS) - 1) & 1))) break;
+                    if (it >= NS && !(ok = mbar_wait_cg<CG>(&empty[s], ((it / NS) - 1) & 1))) break;
                     uint8_t* st = smem + s * S::STAGE;
                     if (it >= ahead) {
                         mbar_arrive_expect_tx(&full[s], bytes_of(kt));
@@ -223,7 +233,7 @@ __global__ void __launch_bounds__(FP4_THREADS, 1)
                     }
 #pragma unroll
                     for (int p = 0; p < P; ++p)
-                        tma_load_2d(st + S::A_BYTES + p * S::B_TILE, &tm_x, &full[s], kb * 128, p * a.piece_rows + t.r0, pol_x);
+                        tma_load_2d(st + S::A_BYTES + p * S::B_TILE, &tm_x, &full[s], kb * 128, p * a.piece_rows + t.r0 + half * (T / CG), pol_x);
                     uint8_t* sfb = st + S::A_BYTES + S::B_BYTES + S::SFA;
                     if constexpr (S::KIND == FP4_SPLIT) {
                         bulk_load(sfb, a.xt + (int64_t(t.id) * a.ktiles + kb) * S::SFB, S::SFB, &full[s]);
@@ -238,15 +248,24 @@ __global__ void __launch_bounds__(FP4_THREADS, 1)
         __syncwarp();
     } else if (warp == 5) {
         // ------------------------------ MMA issuer ------------------------------
-        constexpr uint32_t idesc = fp4_idesc<S::KIND>(128, S::N);
+        constexpr uint32_t idesc = fp4_idesc<S::KIND>(128 * CG, S::N);
         int it = 0, j = 0;
         Fp4Tile t;
-        for (int lin = first; lin < ntiles && ok; lin += step) {
-            if (!fp4_tile<T>(a, starts, nseg, lin, t)) continue;
+        // a pair's upper rank only says when its stages are full
+        for (int lin = first; CG == 2 && rank == 1 && lin < ntiles && ok; lin += step) {
+            if (!fp4_tile<S>(a, starts, nseg, lin, t)) continue;
+            for (int kb = 0; kb < a.ns && ok; ++kb, ++it) {
+                ok = mbar_wait(&full[it % NS], (it / NS) & 1);
+                if (ok && lane == 0) mbar_arrive_peer(&peer[it % NS], 0);
+                __syncwarp();
+            }
+        }
+        for (int lin = first; (CG == 1 || rank == 0) && lin < ntiles && ok; lin += step) {
+            if (!fp4_tile<S>(a, starts, nseg, lin, t)) continue;
             if constexpr (S::ACC == 256) {
-                if (j >= 1) ok = mbar_wait(&acc_empty[0], (j - 1) & 1);
+                if (j >= 1) ok = mbar_wait_cg<CG>(&acc_empty[0], (j - 1) & 1);
             } else {
-                if (j >= 2) ok = mbar_wait(&acc_empty[j & 1], ((j >> 1) - 1) & 1);
+                if (j >= 2) ok = mbar_wait_cg<CG>(&acc_empty[j & 1], ((j >> 1) - 1) & 1);
             }
             if (!ok) break;
             tc_fence_after();
@@ -254,8 +273,9 @@ __global__ void __launch_bounds__(FP4_THREADS, 1)
             for (int kb = s_lo; kb < s_hi && ok; ++kb, ++it) {
                 const int s = it % NS;
                 // the scales' place: the MMAs of the stage before last are done
-                if (it >= 2) ok = mbar_wait(&empty[(it - 2) % NS], ((it - 2) / NS) & 1);
+                if (it >= 2) ok = mbar_wait_cg<CG>(&empty[(it - 2) % NS], ((it - 2) / NS) & 1);
                 if (ok) ok = mbar_wait(&full[s], (it / NS) & 1);
+                if (CG == 2 && ok) ok = mbar_wait_cluster(&peer[s], (it / NS) & 1);
                 if (!ok) break;
                 tc_fence_after();
                 if (lane == 0) {
@@ -266,10 +286,10 @@ __global__ void __launch_bounds__(FP4_THREADS, 1)
 #pragma unroll
                     for (int q = 0; q < S::KB; ++q)
                         if (q < kt) {
-                            tc_copy_scales(sfa + 4 * q, umma_desc_scales(fa + q * 512));
+                            tc_copy_scales<CG>(sfa + 4 * q, umma_desc_scales(fa + q * 512));
 #pragma unroll
                             for (int b = 0; b < S::NB; ++b)
-                                tc_copy_scales(sfb + 4 * (q * S::NB + b), umma_desc_scales(fb + (b * S::KB + q) * 512));
+                                tc_copy_scales<CG>(sfb + 4 * (q * S::NB + b), umma_desc_scales(fb + (b * S::KB + q) * 512));
                         }
 #pragma unroll
                     for (int k = 0; k < 4; ++k) {
@@ -279,17 +299,17 @@ __global__ void __launch_bounds__(FP4_THREADS, 1)
                             const uint32_t id = fp4_idesc_byte(S::KIND == FP4_MX ? 2 * (k % 2) : S::KIND == FP4_NV ? 0 : k);
 #pragma unroll
                             for (int p = 0; p < (S::STACK ? 1 : P); ++p)
-                                tc_mma_fp4<S::KIND>(acc, umma_desc_sw128(a_base + k * 32),
+                                tc_mma_fp4<S::KIND, CG>(acc, umma_desc_sw128(a_base + k * 32),
                                                     umma_desc_sw128(b_base + p * S::B_TILE + k * 32), idesc | id, sfa + 4 * q,
                                                     sfb + 4 * (q * S::NB + p * (S::NB / (S::STACK ? 1 : P))),
                                                     (kb > s_lo || k > 0 || p > 0) ? 1u : 0u);
                         }
                     }
-                    tc_commit(&empty[s]);
+                    tc_commit_all<CG>(&empty[s]);
                 }
                 __syncwarp();
             }
-            if (lane == 0) tc_commit(&acc_full[j & 1]);
+            if (lane == 0) tc_commit_all<CG>(&acc_full[j & 1]);
             __syncwarp();
             ++j;
         }
@@ -297,14 +317,20 @@ __global__ void __launch_bounds__(FP4_THREADS, 1)
         // ------------------------------ epilogue warps 0-3 ------------------------------
         grid_dep_wait();
         const float f = (a.xf ? *a.xf : 1.f) * (a.wf ? *a.wf : 1.f);
+        auto acc_free = [&](int b) {
+            if constexpr (CG == 2)
+                mbar_arrive_peer(&acc_empty[b], 0);
+            else
+                mbar_arrive(&acc_empty[b]);
+        };
         int j = 0;
         Fp4Tile t;
         for (int lin = first; lin < ntiles; lin += step) {
-            if (!fp4_tile<T>(a, starts, nseg, lin, t)) continue;
-            if (ok) ok = mbar_wait(&acc_full[j & 1], (j >> 1) & 1);
+            if (!fp4_tile<S>(a, starts, nseg, lin, t)) continue;
+            if (ok) ok = mbar_wait_cg<CG>(&acc_full[j & 1], (j >> 1) & 1);
             if (!ok) break;
             tc_fence_after();
-            const int n = t.n0 + 32 * warp + lane;
+            const int n = t.n0 + 128 * half + 32 * warp + lane;
             const uint32_t acc = tmem + (uint32_t(32 * warp) << 16) + uint32_t((j & 1) * S::ACC_STEP);
             float* part = reinterpret_cast<float*>(smem);  // [T][128] sums of this CTA's share of K (split K: one tile a CTA)
 #pragma unroll 1
@@ -329,7 +355,7 @@ __global__ void __launch_bounds__(FP4_THREADS, 1)
                 if (S::ACC == 256 && i + 16 == 128) {
                     tc_fence_before();
                     __syncwarp();
-                    if (lane == 0) mbar_arrive(&acc_empty[0]);
+                    if (lane == 0) acc_free(0);
                 }
                 if (a.ks > 1) {
 #pragma unroll
@@ -342,17 +368,17 @@ __global__ void __launch_bounds__(FP4_THREADS, 1)
             if constexpr (S::ACC != 256) {
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&acc_empty[j & 1]);
+                if (lane == 0) acc_free(j & 1);
             }
             ++j;
         }
     }
-    if (a.ks > 1) {
+    if (CG == 1 && a.ks > 1) {
         // the CTAs of a cluster have one tile: each writes out the columns c with c % ks == its rank
         __syncwarp();
         cluster_sync();
         Fp4Tile t;
-        if (warp < 4 && first < ntiles && fp4_tile<T>(a, starts, nseg, first, t)) {
+        if (warp < 4 && first < ntiles && fp4_tile<S>(a, starts, nseg, first, t)) {
             const float f = (a.xf ? *a.xf : 1.f) * (a.wf ? *a.wf : 1.f);
             const uint32_t part = smem_u32(smem) + (32 * warp + lane) * 4;
             for (int c = rank; c < T && t.r0 + c < t.r1; c += a.ks) {
@@ -365,10 +391,14 @@ __global__ void __launch_bounds__(FP4_THREADS, 1)
         cluster_sync();
     }
     tc_fence_before();
-    __syncthreads();
+    __syncwarp();
+    if constexpr (CG == 2)
+        cluster_sync();  // neither CTA leaves while the other's MMAs or arrivals may reach it
+    else
+        __syncthreads();
     if (warp == 5) {
         tc_fence_after();
-        tmem_dealloc(tmem, S::TMEM);
+        tc_dealloc<CG>(tmem, S::TMEM);
     }
 }
 
@@ -498,7 +528,7 @@ struct Fp4Call {
     const uint8_t* x;  // codes or pieces
     const uint32_t* w;
     int stack;         // experts, 1 for a dense product
-    int64_t tiles;     // most tiles that the call can have
+    int64_t ttiles;    // most tiles of tokens that the call can have
     Fp4Args a;
 };
 
@@ -521,24 +551,29 @@ static int gemm_t(const Fp4Call& c, cudaStream_t st) {
     {
         const uint64_t row = uint64_t(a.Kp) / (S::KIND == FP4_SPLIT ? 1 : 2);
         const uint64_t dims[2] = {row, uint64_t(S::P) * a.M}, str[1] = {row};
-        const uint32_t box[2] = {128, uint32_t(S::T)};
+        const uint32_t box[2] = {128, uint32_t(S::T / S::CG)};
         int rc = make_tmap(&tx, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, c.x, dims, str, box, CU_TENSOR_MAP_SWIZZLE_128B);
         if (rc) return rc;
     }
     const int sms = device_info().sm_count;
     const int64_t slots = int64_t(sms) * (S::T <= 64 ? 2 : 1);
+    a.rtiles = (a.N + 127) / 128;
+    a.ntn = (a.rtiles + S::CG - 1) / S::CG;
+    const int64_t tiles = c.ttiles * a.ntn;
+    if (tiles > INT32_MAX) return LQ_E_SHAPE;
+    a.ntiles = int(tiles);
     a.ks = 1;
-    if (S::ACC != 256 && c.tiles < sms) {  // a tile's K split over the CTAs of a cluster
-        const int most = a.ns < 8 ? a.ns : 8, ks = int(sms / c.tiles);  // every CTA has a stage
+    if (S::CG == 1 && S::ACC != 256 && tiles < sms) {  // a tile's K split over the CTAs of a cluster
+        const int most = a.ns < 8 ? a.ns : 8, ks = int(sms / tiles);  // every CTA has a stage
         a.ks = ks < most ? ks : most;
     }
-    const int64_t grid = a.ks > 1 ? c.tiles * a.ks : c.tiles < slots ? c.tiles : slots;
-    const size_t smem = 1024 + size_t(S::NS) * S::STAGE + (2 * S::NS + 4) * 8 + 8 + (a.grouped ? (FP4_MAX_SEGMENTS + 2) * 4 : 0);
+    const int64_t grid = S::CG == 2 ? (tiles < sms / 2 ? tiles : sms / 2) * 2 : a.ks > 1 ? tiles * a.ks : tiles < slots ? tiles : slots;
+    const size_t smem = 1024 + size_t(S::NS) * S::STAGE + (3 * S::NS + 4) * 8 + 8 + (a.grouped ? (FP4_MAX_SEGMENTS + 2) * 4 : 0);
     static_assert(S::ACC == 256 || S::T * 512 <= S::NS * S::STAGE, "the partial sums of a split fit the ring");
     auto kern = fp4_gemm_kernel<S>;
     if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem)) != cudaSuccess) return LQ_E_CUDA;
     void* args[] = {&tw, &tx, &a};
-    return launch(reinterpret_cast<const void*>(kern), int(grid), FP4_THREADS, smem, a.ks, st, args);
+    return launch(reinterpret_cast<const void*>(kern), int(grid), FP4_THREADS, smem, S::CG == 2 ? 2 : a.ks, st, args);
 }
 
 template <int KIND, int P>
@@ -548,21 +583,19 @@ static int gemm_tokens(const Fp4Call& c, int T, cudaStream_t st) {
         case 32: return gemm_t<Fp4Shape<KIND, P, 32>>(c, st);
         case 64: return gemm_t<Fp4Shape<KIND, P, 64>>(c, st);
         case 128: return gemm_t<Fp4Shape<KIND, P, 128>>(c, st);
-        default:
-            if constexpr (P == 1) return gemm_t<Fp4Shape<KIND, P, 256>>(c, st);
-            return LQ_E_SHAPE;
+        default: return gemm_t<Fp4Shape<KIND, P, 256, 2>>(c, st);
     }
 }
 
 // Tokens a tile. A product of both in 4 bits has scale tiles of 128 tokens, so narrower tiles only where one holds them all.
-static int tile_tokens(int rows, int P) {
-    return rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : rows <= 128 || P > 1 ? 128 : 256;
+static int tile_tokens(int rows) {
+    return rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : rows <= 128 ? 128 : 256;
 }
 
 int fp4_qmm_run(const uint32_t* xc, const uint8_t* xt, const float* xf, const uint32_t* wc, const uint8_t* wt, const float* wf,
                 int M, int N, int K, int mode, int glu, int dtype, void* y, cudaStream_t st) {
     Fp4Call c = {};
-    const int T = tile_tokens(M, 1);
+    const int T = tile_tokens(M);
     c.x = reinterpret_cast<const uint8_t*>(xc);
     c.w = wc;
     c.stack = 1;
@@ -571,10 +604,7 @@ int fp4_qmm_run(const uint32_t* xc, const uint8_t* xt, const float* xf, const ui
     a.N = N;
     a.Kp = fp4_padded(K);
     a.ktiles = fp4_ktiles(K, mode);
-    a.ntn = (N + 127) / 128;
-    c.tiles = int64_t(a.ntn) * ((M + T - 1) / T);
-    if (c.tiles > INT32_MAX) return LQ_E_SHAPE;
-    a.ntiles = int(c.tiles);
+    c.ttiles = (M + T - 1) / T;
     a.glu = glu;
     a.dtype = dtype;
     a.wt = wt;
@@ -591,20 +621,20 @@ static int split_blocks(int P, int T) { return T <= 32 ? 1 : P * ((T + 127) / 12
 static size_t split_pieces_bytes(int rows, int K, int P) { return (size_t(P) * rows * fp4_padded(K) + 511) / 512 * 512; }
 
 // Tokens a tile of rows that are dealt out to segments: twice the average, so that most segments are one tile.
-static int grouped_tokens(int rows, int segments, int max_rows, int P) {
+static int grouped_tokens(int rows, int segments, int max_rows) {
     const int64_t want = 2 * int64_t(rows) / (segments > 0 ? segments : 1);
-    return tile_tokens(int(want < max_rows ? want : max_rows), P);
+    return tile_tokens(int(want < max_rows ? want : max_rows));
 }
 
 size_t fp4_linear_workspace_bytes(int rows, int K, int dtype, int segments, int max_rows) {
-    const int P = dtype == LQ_BF16 ? 2 : 3, T = segments ? grouped_tokens(rows, segments, max_rows, P) : tile_tokens(rows, P);
+    const int P = dtype == LQ_BF16 ? 2 : 3, T = segments ? grouped_tokens(rows, segments, max_rows) : tile_tokens(rows);
     return split_pieces_bytes(rows, K, P) +
            size_t(split_tiles(rows, T, segments)) * fp4_ktiles(K, LQ_MXFP4) * split_blocks(P, T) * 512;
 }
 
 int fp4_linear_run(const Fp4Linear& l, cudaStream_t st) {
     const int P = l.dtype == LQ_BF16 ? 2 : 3;
-    const int T = l.segments ? grouped_tokens(l.rows, l.segments, l.max_rows, P) : tile_tokens(l.rows, P);
+    const int T = l.segments ? grouped_tokens(l.rows, l.segments, l.max_rows) : tile_tokens(l.rows);
     uint8_t* ws = static_cast<uint8_t*>(l.ws);
     SplitArgs s = {};
     s.x = l.x;
@@ -641,10 +671,7 @@ int fp4_linear_run(const Fp4Linear& l, cudaStream_t st) {
     a.N = l.N;
     a.Kp = fp4_padded(l.K);
     a.ktiles = s.ktiles;
-    a.ntn = (l.N + 127) / 128;
-    c.tiles = split_tiles(l.rows, T, l.segments) * a.ntn;
-    if (c.tiles > INT32_MAX) return LQ_E_SHAPE;
-    a.ntiles = int(c.tiles);
+    c.ttiles = split_tiles(l.rows, T, l.segments);
     a.glu = l.glu;
     a.dtype = l.dtype;
     a.piece_rows = l.rows;
