@@ -345,7 +345,7 @@ int lq_fp4_linear(const void* x, int64_t x_row, const uint32_t* codes, const uin
 
 /* lq_moe_experts for stacks in LQ_MXFP4: codes (E, N, Kp / 8), tiles (E, ceil(N / 128), Kp / 128, 512). out (P, N), or
  * (P, N / 2) with glu as lq_fp4_qmm. x (x_rows, K): with gather_order, pair j reads row gather_order[j] / gather_k;
- * without, row j. Segments as lq_moe_experts (an expert id E is padding, left unwritten); min(E + 1, P) <= 2047.
+ * without, row j. Segments as lq_moe_experts (an expert id E is padding, left unwritten); min(E + 1, P) <= 1024.
  * workspace: lq_fp4_experts_workspace(P, max_rows, E, K, dtype) bytes, 256-byte aligned. */
 size_t lq_fp4_experts_workspace(int P, int max_rows, int E, int K, int dtype);
 int lq_fp4_experts(const void* x, int x_rows, const int32_t* gather_order, int gather_k, const int32_t* starts,

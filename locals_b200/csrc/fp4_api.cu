@@ -108,7 +108,7 @@ int lq_fp4_experts(const void* x, int x_rows, const int32_t* gather_order, int g
     if (!rc && (E < 1 || max_rows < 1 || x_rows < 1 || (!gather_order && x_rows < P))) rc = LQ_E_SHAPE;
     if (!rc) rc = fp4_rows_ok(int64_t(E) * N, K, LQ_MXFP4);
     if (rc) return rc;
-    if ((glu && N % 2) || fp4_segments(P, E) > 2047) return LQ_E_SHAPE;
+    if ((glu && N % 2) || fp4_segments(P, E) > 1024) return LQ_E_SHAPE;
     if (workspace_bytes < lq_fp4_experts_workspace(P, max_rows, E, K, dtype)) return LQ_E_SHAPE;
     if (!aligned(codes, 32) || !aligned(tiles, 16) || !aligned(workspace, 256) || !aligned(x, 2) || !aligned(out, 2)) return LQ_E_ALIGN;
     rc = check_device();

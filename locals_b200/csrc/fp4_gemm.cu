@@ -27,7 +27,7 @@ namespace lq {
 
 constexpr int FP4_THREADS = 192;
 constexpr int FP4_MAX_STAGES = 10;
-constexpr int FP4_MAX_SEGMENTS = 2048;
+constexpr int FP4_MAX_SEGMENTS = 1024;
 
 template <int KIND_, int P_, int T_, int CG_ = 1>
 struct Fp4Shape {
@@ -42,7 +42,7 @@ struct Fp4Shape {
     static constexpr int A_TX = KIND == FP4_SPLIT ? A_BYTES / 2 : A_BYTES;
     static constexpr int SFA = KB * 512, SFB = KB * NB * 512;
     static constexpr int STAGE = (A_BYTES + B_BYTES + SFA + SFB + 1023) / 1024 * 1024;
-    static constexpr int SMEM = (T <= 64 ? 110 : 224) * 1024;  // narrow tiles leave room for a second CTA
+    static constexpr int SMEM = (T <= 64 ? 96 : 216) * 1024;  // narrow tiles leave room for a second CTA
     static constexpr int FIT = SMEM / STAGE, NS = FIT < FP4_MAX_STAGES ? FIT : FP4_MAX_STAGES;
     static constexpr int N = STACK ? P * T : T;
     static constexpr int ACC = N <= 32 ? 32 : N <= 64 ? 64 : N <= 128 ? 128 : 256;
@@ -132,6 +132,50 @@ __device__ __forceinline__ void fp4_out(const Fp4Args& a, const Fp4Tile& t, int 
     }
 }
 
+__device__ __forceinline__ uint32_t fp4_pair(const Fp4Args& a, float lo, float hi) {
+    return a.dtype == LQ_BF16 ? cvt_bf16x2(hi, lo) : cvt_f16x2(hi, lo);
+}
+
+// 16 output columns (tokens) of a warp's 32 rows of w, v[c] the sum of this lane's row and token c0 + c: turned to rows of y
+// through 2 KB of shared memory, so that a token's 32 values leave in pieces of 16 bytes. Neighbouring lanes first swap
+// columns: the even lane then has two rows of an even column, the odd lane two of an odd one.
+__device__ __forceinline__ void fp4_out16(const Fp4Args& a, const Fp4Tile& t, int c0, int nb, const float (&v)[16], float f,
+                                          uint8_t* stage, int lane) {
+    const int odd = lane & 1;
+    int bytes, width = a.N;  // of a token's values here; of a row of y
+    if (a.dtype == LQ_F32 && !a.glu) {
+        bytes = 128;
+#pragma unroll
+        for (int c = 0; c < 16; ++c) reinterpret_cast<float*>(stage + c * 128)[lane] = v[c] * f;
+    } else {
+        width = a.glu ? a.N / 2 : a.N;
+        bytes = (a.glu ? 16 : 32) * (a.dtype == LQ_F32 ? 4 : 2);
+#pragma unroll
+        for (int c = 0; c < 16; c += 2) {
+            const float mine = (odd ? v[c + 1] : v[c]) * f, got = __shfl_xor_sync(0xFFFFFFFFu, odd ? v[c] : v[c + 1], 1) * f;
+            uint8_t* row = stage + (c + odd) * bytes;
+            if (a.glu) {
+                const float g = odd ? got : mine, u = odd ? mine : got, h = g / (1.f + __expf(-g)) * u;
+                if (a.dtype == LQ_F32)
+                    reinterpret_cast<float*>(row)[lane >> 1] = h;
+                else
+                    reinterpret_cast<uint16_t*>(row)[lane >> 1] = uint16_t(fp4_pair(a, h, 0.f));
+            } else {
+                reinterpret_cast<uint32_t*>(row)[lane >> 1] = odd ? fp4_pair(a, got, mine) : fp4_pair(a, mine, got);
+            }
+        }
+    }
+    __syncwarp();
+    const int per = bytes / 16, size = a.dtype == LQ_F32 ? 4 : 2;
+    uint8_t* y = static_cast<uint8_t*>(a.y) + (int64_t(t.r0 + c0) * width + (a.glu ? nb / 2 : nb)) * size;
+    for (int q = lane; q < 16 * per; q += 32) {
+        const int c = q / per;
+        if (t.r0 + c0 + c < t.r1)
+            *reinterpret_cast<uint4*>(y + int64_t(c) * width * size + (q - c * per) * 16) = *reinterpret_cast<uint4*>(stage + q * 16);
+    }
+    __syncwarp();
+}
+
 template <typename S>
 __global__ void __launch_bounds__(FP4_THREADS, 1)
     fp4_gemm_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_x, const Fp4Args a) {
@@ -144,7 +188,8 @@ __global__ void __launch_bounds__(FP4_THREADS, 1)
     uint64_t* acc_full = peer + NS;      // [2] the MMAs of a tile are done
     uint64_t* acc_empty = acc_full + 2;  // [2] the epilogue has read what the next tile writes
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
-    int32_t* seg = reinterpret_cast<int32_t*>(tmem_slot + 2);  // [0] segments, then their starts (grouped)
+    uint8_t* stage = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(tmem_slot + 1) + 15) & ~uintptr_t(15));  // 2 KB a warp
+    int32_t* seg = reinterpret_cast<int32_t*>(stage + 4 * 2048);  // [0] segments, then their starts (grouped)
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int rank = CG == 2 || a.ks > 1 ? int(cluster_ctarank()) : 0;
@@ -175,6 +220,9 @@ __global__ void __launch_bounds__(FP4_THREADS, 1)
         if (threadIdx.x == 0) seg[0] = n;
     }
     tc_fence_before();
+    // The cluster barrier counts warps: the one whose first lane sets up the mbarriers arrives when that lane has, not before
+    // (a load ahead of the wait below met a barrier that was then set up again).
+    __syncwarp();
     if constexpr (CG == 2)
         cluster_sync();
     else
@@ -244,6 +292,9 @@ __global__ void __launch_bounds__(FP4_THREADS, 1)
                     }
                 }
             }
+            // after a wait that gave up: the copies in flight land before the CTA's shared memory is another's
+            if (!ok)
+                for (int q = it > NS ? it - NS : 0; q < it; ++q) mbar_wait(&full[q % NS], (q / NS) & 1);
         }
         __syncwarp();
     } else if (warp == 5) {
@@ -317,6 +368,9 @@ __global__ void __launch_bounds__(FP4_THREADS, 1)
         // ------------------------------ epilogue warps 0-3 ------------------------------
         grid_dep_wait();
         const float f = (a.xf ? *a.xf : 1.f) * (a.wf ? *a.wf : 1.f);
+        // 16-byte pieces of y: its rows start on 16-byte boundaries
+        const int ysize = (a.glu ? a.N / 2 : a.N) * (a.dtype == LQ_F32 ? 4 : 2);
+        const bool wide = ysize % 16 == 0 && reinterpret_cast<uintptr_t>(a.y) % 16 == 0;
         auto acc_free = [&](int b) {
             if constexpr (CG == 2)
                 mbar_arrive_peer(&acc_empty[b], 0);
@@ -357,9 +411,11 @@ __global__ void __launch_bounds__(FP4_THREADS, 1)
                     __syncwarp();
                     if (lane == 0) acc_free(0);
                 }
-                if (a.ks > 1) {
+                if (CG == 1 && a.ks > 1) {
 #pragma unroll
                     for (int c = 0; c < 16; ++c) part[(c0 + c) * 128 + 32 * warp + lane] = v[c];
+                } else if (wide && n - lane + 32 <= a.N) {
+                    if (t.r0 + c0 < t.r1) fp4_out16(a, t, c0, n - lane, v, f, stage + 2048 * warp, lane);
                 } else {
 #pragma unroll
                     for (int c = 0; c < 16; ++c) fp4_out<S>(a, t, c0 + c, n, v[c] * f);
@@ -568,7 +624,7 @@ static int gemm_t(const Fp4Call& c, cudaStream_t st) {
         a.ks = ks < most ? ks : most;
     }
     const int64_t grid = S::CG == 2 ? (tiles < sms / 2 ? tiles : sms / 2) * 2 : a.ks > 1 ? tiles * a.ks : tiles < slots ? tiles : slots;
-    const size_t smem = 1024 + size_t(S::NS) * S::STAGE + (3 * S::NS + 4) * 8 + 8 + (a.grouped ? (FP4_MAX_SEGMENTS + 2) * 4 : 0);
+    const size_t smem = 1024 + size_t(S::NS) * S::STAGE + (3 * S::NS + 4) * 8 + 16 + 4 * 2048 + (a.grouped ? (FP4_MAX_SEGMENTS + 2) * 4 : 0);
     static_assert(S::ACC == 256 || S::T * 512 <= S::NS * S::STAGE, "the partial sums of a split fit the ring");
     auto kern = fp4_gemm_kernel<S>;
     if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem)) != cudaSuccess) return LQ_E_CUDA;
