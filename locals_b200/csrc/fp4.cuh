@@ -69,6 +69,19 @@ __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t b
                  : "memory");
 }
 
+// One lane of a whole warp, chosen in a way that the compiler knows to be uniform: tcgen05 and TMA instructions take their
+// operands from uniform registers, and behind `lane == 0` each operand is moved there one by one (70 cycles a tcgen05.cp and
+// 55 to 70 a small MMA; 20 and 45 behind this).
+__device__ __forceinline__ bool elect_one() {
+    uint32_t p;
+    asm volatile(
+        "{\n\t.reg .pred q;\n\t"
+        "elect.sync _|q, 0xFFFFFFFF;\n\t"
+        "selp.u32 %0, 1, 0, q;\n\t}"
+        : "=r"(p));
+    return p != 0;
+}
+
 // ---- pairs of CTAs ----
 
 // Arrive on the barrier at this offset of another CTA of the cluster.

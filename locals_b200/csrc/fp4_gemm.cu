@@ -191,7 +191,7 @@ __global__ void __launch_bounds__(FP4_THREADS, 1)
     uint8_t* stage = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(tmem_slot + 1) + 15) & ~uintptr_t(15));  // 2 KB a warp
     int32_t* seg = reinterpret_cast<int32_t*>(stage + 4 * 2048);  // [0] segments, then their starts (grouped)
 
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = __shfl_sync(0xFFFFFFFFu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     const int rank = CG == 2 || a.ks > 1 ? int(cluster_ctarank()) : 0;
     const int share = CG == 2 ? 2 : a.ks, half = CG == 2 ? rank : 0;
     const int first = int(blockIdx.x) / share, step = int(gridDim.x) / share;
@@ -236,11 +236,11 @@ __global__ void __launch_bounds__(FP4_THREADS, 1)
 
     if (warp == 4) {
         // ------------------------------ producer ------------------------------
-        if (lane == 0) {
+        if (elect_one()) {
             prefetch_tmap(&tm_w);
             prefetch_tmap(&tm_x);
             const uint64_t pol_w = policy_evict_first(), pol_x = policy_evict_last();
-            int it = 0;
+            int it = 0, s = 0, turn = 0;  // stages so far, the ring's next slot, rounds of the ring
             bool waited = a.grouped;
             Fp4Tile t;
             for (int lin = first; lin < ntiles && ok; lin += step) {
@@ -271,9 +271,13 @@ __global__ void __launch_bounds__(FP4_THREADS, 1)
                     grid_dep_wait();
                     waited = true;
                 }
-                for (int kb = s_lo; kb < s_hi; ++kb, ++it) {
-                    const int s = it % NS, kt = tiles_of(kb);
-                    if (it >= NS && !(ok = mbar_wait_cg<CG>(&empty[s], ((it / NS) - 1) & 1))) break;
+                for (int kb = s_lo; kb < s_hi; ++kb, ++it, ++s) {
+                    if (s == NS) {
+                        s = 0;
+                        ++turn;
+                    }
+                    const int kt = tiles_of(kb);
+                    if (turn > 0 && !(ok = mbar_wait_cg<CG>(&empty[s], (turn - 1) & 1))) break;
                     uint8_t* st = smem + s * S::STAGE;
                     if (it >= ahead) {
                         mbar_arrive_expect_tx(&full[s], bytes_of(kt));
@@ -300,14 +304,15 @@ __global__ void __launch_bounds__(FP4_THREADS, 1)
     } else if (warp == 5) {
         // ------------------------------ MMA issuer ------------------------------
         constexpr uint32_t idesc = fp4_idesc<S::KIND>(128 * CG, S::N);
-        int it = 0, j = 0;
+        const bool lead = elect_one();
+        int it = 0, j = 0, s = 0, turn = 0;
         Fp4Tile t;
         // a pair's upper rank only says when its stages are full
         for (int lin = first; CG == 2 && rank == 1 && lin < ntiles && ok; lin += step) {
             if (!fp4_tile<S>(a, starts, nseg, lin, t)) continue;
             for (int kb = 0; kb < a.ns && ok; ++kb, ++it) {
                 ok = mbar_wait(&full[it % NS], (it / NS) & 1);
-                if (ok && lane == 0) mbar_arrive_peer(&peer[it % NS], 0);
+                if (ok && lead) mbar_arrive_peer(&peer[it % NS], 0);
                 __syncwarp();
             }
         }
@@ -321,15 +326,18 @@ __global__ void __launch_bounds__(FP4_THREADS, 1)
             if (!ok) break;
             tc_fence_after();
             const uint32_t acc = tmem + uint32_t((j & 1) * S::ACC_STEP);
-            for (int kb = s_lo; kb < s_hi && ok; ++kb, ++it) {
-                const int s = it % NS;
+            for (int kb = s_lo; kb < s_hi && ok; ++kb, ++it, ++s) {
+                if (s == NS) {
+                    s = 0;
+                    ++turn;
+                }
                 // the scales' place: the MMAs of the stage before last are done
-                if (it >= 2) ok = mbar_wait_cg<CG>(&empty[(it - 2) % NS], ((it - 2) / NS) & 1);
-                if (ok) ok = mbar_wait(&full[s], (it / NS) & 1);
-                if (CG == 2 && ok) ok = mbar_wait_cluster(&peer[s], (it / NS) & 1);
+                if (it >= 2) ok = mbar_wait_cg<CG>(&empty[s >= 2 ? s - 2 : s - 2 + NS], (s >= 2 ? turn : turn - 1) & 1);
+                if (ok) ok = mbar_wait(&full[s], turn & 1);
+                if (CG == 2 && ok) ok = mbar_wait_cluster(&peer[s], turn & 1);
                 if (!ok) break;
                 tc_fence_after();
-                if (lane == 0) {
+                if (lead) {
                     const int kt = min(S::KB, a.ktiles - kb * S::KB);
                     const uint32_t a_base = smem_u32(smem + s * S::STAGE), b_base = a_base + S::A_BYTES;
                     const uint32_t fa = b_base + S::B_BYTES, fb = fa + S::SFA;
@@ -360,7 +368,7 @@ __global__ void __launch_bounds__(FP4_THREADS, 1)
                 }
                 __syncwarp();
             }
-            if (lane == 0) tc_commit_all<CG>(&acc_full[j & 1]);
+            if (lead) tc_commit_all<CG>(&acc_full[j & 1]);
             __syncwarp();
             ++j;
         }
