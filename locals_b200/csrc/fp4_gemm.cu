@@ -132,48 +132,67 @@ __device__ __forceinline__ void fp4_out(const Fp4Args& a, const Fp4Tile& t, int 
     }
 }
 
-__device__ __forceinline__ uint32_t fp4_pair(const Fp4Args& a, float lo, float hi) {
-    return a.dtype == LQ_BF16 ? cvt_bf16x2(hi, lo) : cvt_f16x2(hi, lo);
-}
-
 // 16 output columns (tokens) of a warp's 32 rows of w, v[c] the sum of this lane's row and token c0 + c: turned to rows of y
 // through 2 KB of shared memory, so that a token's 32 values leave in pieces of 16 bytes. Neighbouring lanes first swap
-// columns: the even lane then has two rows of an even column, the odd lane two of an odd one.
-__device__ __forceinline__ void fp4_out16(const Fp4Args& a, const Fp4Tile& t, int c0, int nb, const float (&v)[16], float f,
-                                          uint8_t* stage, int lane) {
-    const int odd = lane & 1;
-    int bytes, width = a.N;  // of a token's values here; of a row of y
-    if (a.dtype == LQ_F32 && !a.glu) {
-        bytes = 128;
+// columns: the even lane then has two rows of an even column, the odd lane two of an odd one. The type and form are fixed
+// here, not asked for at each value: with branches between the shuffles they ran one after another (1,670 cycles, not 150).
+template <typename O, bool GLU>
+__device__ __forceinline__ void fp4_out16_t(const Fp4Args& a, const Fp4Tile& t, int c0, int nb, const float (&v)[16], float f,
+                                            uint8_t* stage, int lane) {
+    constexpr int BYTES = (GLU ? 16 : 32) * int(sizeof(O)), PER = BYTES / 16;  // of a token's values here
+    const bool odd = lane & 1;
+    if constexpr (sizeof(O) == 4 && !GLU) {
 #pragma unroll
-        for (int c = 0; c < 16; ++c) reinterpret_cast<float*>(stage + c * 128)[lane] = v[c] * f;
+        for (int c = 0; c < 16; ++c) reinterpret_cast<float*>(stage + c * BYTES)[lane] = v[c] * f;
     } else {
-        width = a.glu ? a.N / 2 : a.N;
-        bytes = (a.glu ? 16 : 32) * (a.dtype == LQ_F32 ? 4 : 2);
+        float got[8];
 #pragma unroll
-        for (int c = 0; c < 16; c += 2) {
-            const float mine = (odd ? v[c + 1] : v[c]) * f, got = __shfl_xor_sync(0xFFFFFFFFu, odd ? v[c] : v[c + 1], 1) * f;
-            uint8_t* row = stage + (c + odd) * bytes;
-            if (a.glu) {
-                const float g = odd ? got : mine, u = odd ? mine : got, h = g / (1.f + __expf(-g)) * u;
-                if (a.dtype == LQ_F32)
+        for (int c = 0; c < 8; ++c) got[c] = __shfl_xor_sync(0xFFFFFFFFu, odd ? v[2 * c] : v[2 * c + 1], 1) * f;
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {
+            const float mine = (odd ? v[2 * c + 1] : v[2 * c]) * f, lo = odd ? got[c] : mine, hi = odd ? mine : got[c];
+            uint8_t* row = stage + (2 * c + odd) * BYTES;
+            if constexpr (GLU) {
+                const float h = lo / (1.f + __expf(-lo)) * hi;
+                if constexpr (sizeof(O) == 4)
                     reinterpret_cast<float*>(row)[lane >> 1] = h;
                 else
-                    reinterpret_cast<uint16_t*>(row)[lane >> 1] = uint16_t(fp4_pair(a, h, 0.f));
+                    reinterpret_cast<uint16_t*>(row)[lane >> 1] = F16Traits<O>::from_f32(h);
             } else {
-                reinterpret_cast<uint32_t*>(row)[lane >> 1] = odd ? fp4_pair(a, got, mine) : fp4_pair(a, mine, got);
+                reinterpret_cast<uint32_t*>(row)[lane >> 1] = F16Traits<O>::pack2(hi, lo);
             }
         }
     }
     __syncwarp();
-    const int per = bytes / 16, size = a.dtype == LQ_F32 ? 4 : 2;
-    uint8_t* y = static_cast<uint8_t*>(a.y) + (int64_t(t.r0 + c0) * width + (a.glu ? nb / 2 : nb)) * size;
-    for (int q = lane; q < 16 * per; q += 32) {
-        const int c = q / per;
-        if (t.r0 + c0 + c < t.r1)
-            *reinterpret_cast<uint4*>(y + int64_t(c) * width * size + (q - c * per) * 16) = *reinterpret_cast<uint4*>(stage + q * 16);
+    const int64_t width = GLU ? a.N / 2 : a.N;
+    O* y = static_cast<O*>(a.y) + int64_t(t.r0 + c0) * width + (GLU ? nb / 2 : nb);
+    const int rows = t.r1 - t.r0 - c0;
+#pragma unroll
+    for (int i = 0; i < (16 * PER + 31) / 32; ++i) {
+        const int q = lane + 32 * i, c = q / PER;
+        if (c < rows && q < 16 * PER)
+            *reinterpret_cast<uint4*>(y + c * width + (q % PER) * (16 / int(sizeof(O)))) = *reinterpret_cast<uint4*>(stage + q * 16);
     }
     __syncwarp();
+}
+
+__device__ __forceinline__ void fp4_out16(const Fp4Args& a, const Fp4Tile& t, int c0, int nb, const float (&v)[16], float f,
+                                          uint8_t* stage, int lane) {
+    if (a.glu) {
+        if (a.dtype == LQ_BF16)
+            fp4_out16_t<__nv_bfloat16, true>(a, t, c0, nb, v, f, stage, lane);
+        else if (a.dtype == LQ_F16)
+            fp4_out16_t<__half, true>(a, t, c0, nb, v, f, stage, lane);
+        else
+            fp4_out16_t<float, true>(a, t, c0, nb, v, f, stage, lane);
+    } else {
+        if (a.dtype == LQ_BF16)
+            fp4_out16_t<__nv_bfloat16, false>(a, t, c0, nb, v, f, stage, lane);
+        else if (a.dtype == LQ_F16)
+            fp4_out16_t<__half, false>(a, t, c0, nb, v, f, stage, lane);
+        else
+            fp4_out16_t<float, false>(a, t, c0, nb, v, f, stage, lane);
+    }
 }
 
 template <typename S>
