@@ -61,14 +61,6 @@ __device__ __forceinline__ float fp4_scale_value(uint32_t b, int mode) {
     return e4m3x2_to_f32(b).x;
 }
 
-// ---- TMA: untiled bulk copy (16-byte aligned on both sides, a multiple of 16 bytes) ----
-__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
-    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
-                     smem_u32(dst)),
-                 "l"(src), "r"(bytes), "r"(smem_u32(bar))
-                 : "memory");
-}
-
 // One lane of a whole warp, chosen in a way that the compiler knows to be uniform: tcgen05 and TMA instructions take their
 // operands from uniform registers, and behind `lane == 0` each operand is moved there one by one (70 cycles a tcgen05.cp and
 // 55 to 70 a small MMA; 20 and 45 behind this).
@@ -83,6 +75,39 @@ __device__ __forceinline__ bool elect_one() {
 }
 
 // ---- pairs of CTAs ----
+
+// Tiled loads to this CTA's shared memory; `bar` is an address of the cluster's window, in a pair the lower rank's barrier.
+template <int CG>
+__device__ __forceinline__ void load_2d(uint32_t dst, const CUtensorMap* m, uint32_t bar, int c0, int c1, uint64_t policy) {
+    if constexpr (CG == 1)
+        asm volatile(
+            "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint"
+            " [%0], [%1, {%3, %4}], [%2], %5;" ::"r"(dst),
+            "l"(m), "r"(bar), "r"(c0), "r"(c1), "l"(policy)
+            : "memory");
+    else
+        asm volatile(
+            "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint"
+            " [%0], [%1, {%3, %4}], [%2], %5;" ::"r"(dst),
+            "l"(m), "r"(bar), "r"(c0), "r"(c1), "l"(policy)
+            : "memory");
+}
+
+template <int CG>
+__device__ __forceinline__ void load_3d(uint32_t dst, const CUtensorMap* m, uint32_t bar, int c0, int c1, int c2, uint64_t policy) {
+    if constexpr (CG == 1)
+        asm volatile(
+            "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint"
+            " [%0], [%1, {%3, %4, %5}], [%2], %6;" ::"r"(dst),
+            "l"(m), "r"(bar), "r"(c0), "r"(c1), "r"(c2), "l"(policy)
+            : "memory");
+    else
+        asm volatile(
+            "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint"
+            " [%0], [%1, {%3, %4, %5}], [%2], %6;" ::"r"(dst),
+            "l"(m), "r"(bar), "r"(c0), "r"(c1), "r"(c2), "l"(policy)
+            : "memory");
+}
 
 // Arrive on the barrier at this offset of another CTA of the cluster.
 __device__ __forceinline__ void mbar_arrive_peer(uint64_t* bar, uint32_t rank) {

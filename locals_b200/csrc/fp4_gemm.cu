@@ -25,7 +25,8 @@
 
 namespace lq {
 
-constexpr int FP4_THREADS = 192;
+constexpr int FP4_OUT = 8;                           // warps that write tiles out
+constexpr int FP4_THREADS = 32 * (FP4_OUT + 3);
 constexpr int FP4_MAX_STAGES = 10;
 constexpr int FP4_MAX_SEGMENTS = 1024;
 
@@ -41,8 +42,9 @@ struct Fp4Shape {
     // what TMA counts of a weight tile: the bytes that it reads, also where it spreads codes to bytes
     static constexpr int A_TX = KIND == FP4_SPLIT ? A_BYTES / 2 : A_BYTES;
     static constexpr int SFA = KB * 512, SFB = KB * NB * 512;
+    static constexpr int TX = A_TX + B_BYTES + SFA + SFB;  // bytes that arrive for a stage (in each CTA)
     static constexpr int STAGE = (A_BYTES + B_BYTES + SFA + SFB + 1023) / 1024 * 1024;
-    static constexpr int SMEM = (T <= 64 ? 96 : 216) * 1024;  // narrow tiles leave room for a second CTA
+    static constexpr int SMEM = (T <= 32 ? 88 : 204) * 1024;  // narrow tiles leave room for a second CTA
     static constexpr int FIT = SMEM / STAGE, NS = FIT < FP4_MAX_STAGES ? FIT : FP4_MAX_STAGES;
     static constexpr int N = STACK ? P * T : T;
     static constexpr int ACC = N <= 32 ? 32 : N <= 64 ? 64 : N <= 128 ? 128 : 256;
@@ -62,8 +64,6 @@ struct Fp4Args {
     int ks;              // CTAs that split a tile's K
     int glu, dtype;
     int piece_rows;      // rows of one piece of x
-    const uint8_t* wt;   // scale tiles of w, and of x
-    const uint8_t* xt;
     const float* xf;     // factors, or NULL
     const float* wf;
     void* y;
@@ -195,20 +195,23 @@ __device__ __forceinline__ void fp4_out16(const Fp4Args& a, const Fp4Tile& t, in
     }
 }
 
+// The tensor maps of a product: codes of w and x (or pieces of x), scale tiles of w and x.
+struct Fp4Maps {
+    CUtensorMap w, x, ws, xs;
+};
+
 template <typename S>
-__global__ void __launch_bounds__(FP4_THREADS, 1)
-    fp4_gemm_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_x, const Fp4Args a) {
+__global__ void __launch_bounds__(FP4_THREADS, S::T <= 32 ? 2 : 1) fp4_gemm_kernel(const __grid_constant__ Fp4Maps m, const Fp4Args a) {
     constexpr int T = S::T, P = S::P, NS = S::NS, CG = S::CG;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    uint64_t* full = reinterpret_cast<uint64_t*>(smem + NS * S::STAGE);
+    uint64_t* full = reinterpret_cast<uint64_t*>(smem + NS * S::STAGE);  // (in a pair, the lower rank's, for both)
     uint64_t* empty = full + NS;
-    uint64_t* peer = empty + NS;         // the other CTA's stage is full (a pair's lower rank)
-    uint64_t* acc_full = peer + NS;      // [2] the MMAs of a tile are done
+    uint64_t* acc_full = empty + NS;     // [2] the MMAs of a tile are done
     uint64_t* acc_empty = acc_full + 2;  // [2] the epilogue has read what the next tile writes
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
     uint8_t* stage = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(tmem_slot + 1) + 15) & ~uintptr_t(15));  // 2 KB a warp
-    int32_t* seg = reinterpret_cast<int32_t*>(stage + 4 * 2048);  // [0] segments, then their starts (grouped)
+    int32_t* seg = reinterpret_cast<int32_t*>(stage + FP4_OUT * 2048);  // [0] segments, then their starts (grouped)
 
     const int warp = __shfl_sync(0xFFFFFFFFu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     const int rank = CG == 2 || a.ks > 1 ? int(cluster_ctarank()) : 0;
@@ -220,17 +223,14 @@ __global__ void __launch_bounds__(FP4_THREADS, 1)
         for (int s = 0; s < NS; ++s) {
             mbar_init(&full[s], 1);
             mbar_init(&empty[s], 1);
-            mbar_init(&peer[s], 1);
         }
         for (int j = 0; j < 2; ++j) {
             mbar_init(&acc_full[j], 1);
-            mbar_init(&acc_empty[j], 4 * CG);
+            mbar_init(&acc_empty[j], FP4_OUT * CG);
         }
         fence_barrier_init();
     }
-    if (warp == 5) {
-        tc_alloc<CG>(tmem_slot, S::TMEM);
-    }
+    if (warp == FP4_OUT + 1) tc_alloc<CG>(tmem_slot, S::TMEM);
     grid_dep_launch();
     if (a.grouped) {
         grid_dep_wait();
@@ -253,39 +253,39 @@ __global__ void __launch_bounds__(FP4_THREADS, 1)
     const int ntiles = a.grouped ? (nseg > 0 ? (starts[nseg] / T + nseg) * a.ntn : 0) : a.ntiles;
     bool ok = true;
 
-    if (warp == 4) {
-        // ------------------------------ producer ------------------------------
+    if (warp == FP4_OUT || warp == FP4_OUT + 2) {
+        // ------------------------------ producers: codes (and pieces), and scales ------------------------------
+        const bool scales = warp == FP4_OUT + 2;
         if (elect_one()) {
-            prefetch_tmap(&tm_w);
-            prefetch_tmap(&tm_x);
+            prefetch_tmap(scales ? &m.ws : &m.w);
+            prefetch_tmap(scales ? &m.xs : &m.x);
             const uint64_t pol_w = policy_evict_first(), pol_x = policy_evict_last();
+            const uint32_t ring = smem_u32(smem), bars = CG == 2 ? map_peer(smem_u32(full), 0) : smem_u32(full);
             int it = 0, s = 0, turn = 0;  // stages so far, the ring's next slot, rounds of the ring
             bool waited = a.grouped;
             Fp4Tile t;
+            // one thread says what arrives for a stage in both CTAs; a copy may arrive before that
+            auto expect = [&](int slot) {
+                if (!scales && (CG == 1 || rank == 0)) mbar_arrive_expect_tx(&full[slot], CG * S::TX);
+            };
             for (int lin = first; lin < ntiles && ok; lin += step) {
                 if (!fp4_tile<S>(a, starts, nseg, lin, t)) continue;
-                const int wrow = t.expert * a.N + t.n0 + 128 * half;
-                const int wtile = t.n0 / 128 + half;
-                const bool some = wtile < a.rtiles;  // the upper half of a pair's tile may be beyond the last row
-                const uint8_t* wt = a.wt + (int64_t(t.expert) * a.rtiles + wtile) * a.ktiles * 512;
-                auto weights = [&](int kb, int s, int kt) {
-                    uint8_t* st = smem + s * S::STAGE;
-                    tma_load_2d(st, &tm_w, &full[s], kb * 128, wrow, pol_w);
-                    if (some) bulk_load(st + S::A_BYTES + S::B_BYTES, wt + int64_t(kb) * S::KB * 512, kt * 512, &full[s]);
+                const int wrow = t.expert * a.N + t.n0 + 128 * half, wtile = t.expert * a.rtiles + t.n0 / 128 + half;
+                auto weights = [&](int kb, int slot) {
+                    const uint32_t st = ring + slot * S::STAGE, bar = bars + slot * 8;
+                    if (!scales)
+                        load_2d<CG>(st, &m.w, bar, kb * 128, wrow, pol_w);
+                    else
+                        load_3d<CG>(st + S::A_BYTES + S::B_BYTES, &m.ws, bar, 0, kb * S::KB, wtile, pol_w);
                 };
-                // scale tiles of this stage (fewer in a row's last), and blocks of 128 tokens that exist
-                const int xb = S::KIND == FP4_SPLIT ? S::NB : T <= 128 ? 1 : min(2, (a.M - t.r0 + 127) / 128);
-                auto tiles_of = [&](int kb) { return min(S::KB, a.ktiles - kb * S::KB); };
-                auto bytes_of = [&](int kt) { return uint32_t(S::A_TX + S::B_BYTES + kt * 512 * (int(some) + xb)); };
                 // Before this kernel came the split, which was launched on when the kernels before it were done: what they
                 // wrote, weights too, may be read before the split ends. A product of two 4-bit operands may follow the
                 // kernel that quantized its weights.
                 int ahead = 0;
                 if (!waited) {
                     for (; S::KIND == FP4_SPLIT && ahead < NS && s_lo + ahead < s_hi; ++ahead) {
-                        const int kt = tiles_of(s_lo + ahead);
-                        mbar_arrive_expect_tx(&full[ahead], bytes_of(kt));
-                        weights(s_lo + ahead, ahead, kt);
+                        expect(ahead);
+                        weights(s_lo + ahead, ahead);
                     }
                     grid_dep_wait();
                     waited = true;
@@ -295,46 +295,39 @@ __global__ void __launch_bounds__(FP4_THREADS, 1)
                         s = 0;
                         ++turn;
                     }
-                    const int kt = tiles_of(kb);
                     if (turn > 0 && !(ok = mbar_wait_cg<CG>(&empty[s], (turn - 1) & 1))) break;
-                    uint8_t* st = smem + s * S::STAGE;
                     if (it >= ahead) {
-                        mbar_arrive_expect_tx(&full[s], bytes_of(kt));
-                        weights(kb, s, kt);
+                        expect(s);
+                        weights(kb, s);
                     }
+                    const uint32_t st = ring + s * S::STAGE + S::A_BYTES, bar = bars + s * 8;
+                    if (!scales) {
 #pragma unroll
-                    for (int p = 0; p < P; ++p)
-                        tma_load_2d(st + S::A_BYTES + p * S::B_TILE, &tm_x, &full[s], kb * 128, p * a.piece_rows + t.r0 + half * (T / CG), pol_x);
-                    uint8_t* sfb = st + S::A_BYTES + S::B_BYTES + S::SFA;
-                    if constexpr (S::KIND == FP4_SPLIT) {
-                        bulk_load(sfb, a.xt + (int64_t(t.id) * a.ktiles + kb) * S::SFB, S::SFB, &full[s]);
+                        for (int p = 0; p < P; ++p)
+                            load_2d<CG>(st + p * S::B_TILE, &m.x, bar, kb * 128, p * a.piece_rows + t.r0 + half * (T / CG), pol_x);
+                    } else if constexpr (S::KIND == FP4_SPLIT) {
+                        load_3d<CG>(st + S::B_BYTES + S::SFA, &m.xs, bar, 0, 0, t.id * a.ktiles + kb, pol_x);
                     } else {
-                        for (int b = 0; b < xb; ++b)
-                            bulk_load(sfb + b * S::SFA, a.xt + (int64_t(t.r0 / 128 + b) * a.ktiles + kb * S::KB) * 512, kt * 512,
-                                      &full[s]);
+                        load_3d<CG>(st + S::B_BYTES + S::SFA, &m.xs, bar, 0, kb * S::KB, t.r0 / 128, pol_x);
                     }
                 }
             }
             // after a wait that gave up: the copies in flight land before the CTA's shared memory is another's
-            if (!ok)
+            if (!ok && !scales && (CG == 1 || rank == 0))
                 for (int q = it > NS ? it - NS : 0; q < it; ++q) mbar_wait(&full[q % NS], (q / NS) & 1);
         }
         __syncwarp();
-    } else if (warp == 5) {
-        // ------------------------------ MMA issuer ------------------------------
+    } else if (warp == FP4_OUT + 1) {
+        // ------------------------------ MMA issuer (in a pair, the lower rank's) ------------------------------
         constexpr uint32_t idesc = fp4_idesc<S::KIND>(128 * CG, S::N);
+        constexpr int PP = S::STACK ? 1 : P;  // MMAs a step along K
         const bool lead = elect_one();
+        const uint32_t ring = smem_u32(smem);
+        const uint64_t a_desc = umma_desc_sw128(ring), b_desc = umma_desc_sw128(ring + S::A_BYTES);
+        const uint64_t fa_desc = umma_desc_scales(ring + S::A_BYTES + S::B_BYTES);
+        const uint64_t fb_desc = umma_desc_scales(ring + S::A_BYTES + S::B_BYTES + S::SFA);
         int it = 0, j = 0, s = 0, turn = 0;
         Fp4Tile t;
-        // a pair's upper rank only says when its stages are full
-        for (int lin = first; CG == 2 && rank == 1 && lin < ntiles && ok; lin += step) {
-            if (!fp4_tile<S>(a, starts, nseg, lin, t)) continue;
-            for (int kb = 0; kb < a.ns && ok; ++kb, ++it) {
-                ok = mbar_wait(&full[it % NS], (it / NS) & 1);
-                if (ok && lead) mbar_arrive_peer(&peer[it % NS], 0);
-                __syncwarp();
-            }
-        }
         for (int lin = first; (CG == 1 || rank == 0) && lin < ntiles && ok; lin += step) {
             if (!fp4_tile<S>(a, starts, nseg, lin, t)) continue;
             if constexpr (S::ACC == 256) {
@@ -352,36 +345,36 @@ __global__ void __launch_bounds__(FP4_THREADS, 1)
                 }
                 // the scales' place: the MMAs of the stage before last are done
                 if (it >= 2) ok = mbar_wait_cg<CG>(&empty[s >= 2 ? s - 2 : s - 2 + NS], (s >= 2 ? turn : turn - 1) & 1);
-                if (ok) ok = mbar_wait(&full[s], turn & 1);
-                if (CG == 2 && ok) ok = mbar_wait_cluster(&peer[s], turn & 1);
+                if (ok) ok = mbar_wait_cg<CG>(&full[s], turn & 1);
                 if (!ok) break;
                 tc_fence_after();
-                if (lead) {
-                    const int kt = min(S::KB, a.ktiles - kb * S::KB);
-                    const uint32_t a_base = smem_u32(smem + s * S::STAGE), b_base = a_base + S::A_BYTES;
-                    const uint32_t fa = b_base + S::B_BYTES, fb = fa + S::SFA;
-                    const uint32_t sfa = tmem + S::SF_COL + uint32_t(it & 1) * S::SF_COLS, sfb = sfa + 4 * S::KB;
+                const uint64_t at = uint64_t(s * (S::STAGE / 16));
+                const uint32_t sfa = tmem + S::SF_COL + uint32_t(it & 1) * S::SF_COLS, sfb = sfa + 4 * S::KB;
+                const int kt = min(S::KB, a.ktiles - kb * S::KB);  // scale tiles of this stage: fewer in a row's last
+                auto issue = [&](int q) {                          // a scale tile's MMAs
+                    constexpr int PER = 4 / S::KB;
+                    tc_copy_scales<CG>(sfa + 4 * q, fa_desc + at + q * 32);
 #pragma unroll
-                    for (int q = 0; q < S::KB; ++q)
-                        if (q < kt) {
-                            tc_copy_scales<CG>(sfa + 4 * q, umma_desc_scales(fa + q * 512));
+                    for (int b = 0; b < S::NB; ++b)
+                        tc_copy_scales<CG>(sfb + 4 * (q * S::NB + b), fb_desc + at + (b * S::KB + q) * 32);
 #pragma unroll
-                            for (int b = 0; b < S::NB; ++b)
-                                tc_copy_scales<CG>(sfb + 4 * (q * S::NB + b), umma_desc_scales(fb + (b * S::KB + q) * 512));
-                        }
+                    for (int k = q * PER; k < (q + 1) * PER; ++k) {
+                        const uint32_t id = fp4_idesc_byte(S::KIND == FP4_MX ? 2 * (k % 2) : S::KIND == FP4_NV ? 0 : k);
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        constexpr int PER = 4 / S::KB;  // MMAs a scale tile
-                        const int q = k / PER;
-                        if (q < kt) {
-                            const uint32_t id = fp4_idesc_byte(S::KIND == FP4_MX ? 2 * (k % 2) : S::KIND == FP4_NV ? 0 : k);
-#pragma unroll
-                            for (int p = 0; p < (S::STACK ? 1 : P); ++p)
-                                tc_mma_fp4<S::KIND, CG>(acc, umma_desc_sw128(a_base + k * 32),
-                                                    umma_desc_sw128(b_base + p * S::B_TILE + k * 32), idesc | id, sfa + 4 * q,
-                                                    sfb + 4 * (q * S::NB + p * (S::NB / (S::STACK ? 1 : P))),
+                        for (int p = 0; p < PP; ++p)
+                            tc_mma_fp4<S::KIND, CG>(acc, a_desc + at + k * 2, b_desc + at + p * (S::B_TILE / 16) + k * 2, idesc | id,
+                                                    sfa + 4 * q, sfb + 4 * (q * S::NB + p * (S::NB / PP)),
                                                     (kb > s_lo || k > 0 || p > 0) ? 1u : 0u);
-                        }
+                    }
+                };
+                if (lead) {
+                    if (kt == S::KB) {
+#pragma unroll
+                        for (int q = 0; q < S::KB; ++q) issue(q);
+                    } else {
+#pragma unroll
+                        for (int q = 0; q < S::KB - 1; ++q)
+                            if (q < kt) issue(q);
                     }
                     tc_commit_all<CG>(&empty[s]);
                 }
@@ -392,18 +385,25 @@ __global__ void __launch_bounds__(FP4_THREADS, 1)
             ++j;
         }
     } else {
-        // ------------------------------ epilogue warps 0-3 ------------------------------
+        // ------------------------------ epilogue: two warps a quarter of the lanes ------------------------------
         grid_dep_wait();
         const float f = (a.xf ? *a.xf : 1.f) * (a.wf ? *a.wf : 1.f);
         // 16-byte pieces of y: its rows start on 16-byte boundaries
         const int ysize = (a.glu ? a.N / 2 : a.N) * (a.dtype == LQ_F32 ? 4 : 2);
         const bool wide = ysize % 16 == 0 && reinterpret_cast<uintptr_t>(a.y) % 16 == 0;
         auto acc_free = [&](int b) {
-            if constexpr (CG == 2)
-                mbar_arrive_peer(&acc_empty[b], 0);
-            else
-                mbar_arrive(&acc_empty[b]);
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) {
+                if constexpr (CG == 2)
+                    mbar_arrive_peer(&acc_empty[b], 0);
+                else
+                    mbar_arrive(&acc_empty[b]);
+            }
         };
+        constexpr int COLS = T <= 32 ? 16 : T <= 64 ? 32 : 64;  // of a warp at a time
+        constexpr int ROUNDS = (T + 2 * COLS - 1) / (2 * COLS);
+        const int quarter = warp & 3, side = warp >> 2;
         int j = 0;
         Fp4Tile t;
         for (int lin = first; lin < ntiles; lin += step) {
@@ -411,19 +411,23 @@ __global__ void __launch_bounds__(FP4_THREADS, 1)
             if (ok) ok = mbar_wait_cg<CG>(&acc_full[j & 1], (j >> 1) & 1);
             if (!ok) break;
             tc_fence_after();
-            const int n = t.n0 + 128 * half + 32 * warp + lane;
-            const uint32_t acc = tmem + (uint32_t(32 * warp) << 16) + uint32_t((j & 1) * S::ACC_STEP);
+            const int nb = t.n0 + 128 * half + 32 * quarter, n = nb + lane;
+            const uint32_t acc = tmem + (uint32_t(32 * quarter) << 16) + uint32_t((j & 1) * S::ACC_STEP);
             float* part = reinterpret_cast<float*>(smem);  // [T][128] sums of this CTA's share of K (split K: one tile a CTA)
 #pragma unroll 1
-            for (int i = 0; i < T; i += 16) {
-                // the columns that the next tile's accumulator covers come first
-                const int c0 = S::ACC == 256 ? (i + ((j & 1) ? 0 : 128)) % 256 : i;
+            for (int i = 0; i < ROUNDS; ++i) {
+                // The columns that the next tile's accumulator covers come first, and all of them to registers: the next tile's
+                // MMAs wait for that, not for the stores.
+                const int c0 = (S::ACC == 256 ? 128 * ((i + (j & 1) + 1) & 1) : 2 * COLS * i) + COLS * side;
+                if (c0 >= T) break;
+                float v[COLS];
                 uint32_t r[16];
-                float v[16];
-                tmem_ld_32x32b_x16(acc + c0, r);
-                tmem_wait_ld();
 #pragma unroll
-                for (int c = 0; c < 16; ++c) v[c] = __uint_as_float(r[c]);
+                for (int c = 0; c < COLS; c += 16) {
+                    uint32_t(&rr)[16] = *reinterpret_cast<uint32_t(*)[16]>(&v[c]);
+                    tmem_ld_32x32b_x16(acc + c0 + c, rr);
+                }
+                tmem_wait_ld();
                 if constexpr (S::STACK) {
 #pragma unroll
                     for (int p = 1; p < P; ++p) {
@@ -433,26 +437,23 @@ __global__ void __launch_bounds__(FP4_THREADS, 1)
                         for (int c = 0; c < 16; ++c) v[c] += __uint_as_float(r[c]);
                     }
                 }
-                if (S::ACC == 256 && i + 16 == 128) {
-                    tc_fence_before();
-                    __syncwarp();
-                    if (lane == 0) acc_free(0);
-                }
-                if (CG == 1 && a.ks > 1) {
+                if (S::ACC == 256 && i == 0) acc_free(0);
+                if (S::ACC != 256 && i == ROUNDS - 1) acc_free(j & 1);
 #pragma unroll
-                    for (int c = 0; c < 16; ++c) part[(c0 + c) * 128 + 32 * warp + lane] = v[c];
-                } else if (wide && n - lane + 32 <= a.N) {
-                    if (t.r0 + c0 < t.r1) fp4_out16(a, t, c0, n - lane, v, f, stage + 2048 * warp, lane);
-                } else {
+                for (int c = 0; c < COLS; c += 16) {
+                    float(&u)[16] = *reinterpret_cast<float(*)[16]>(&v[c]);
+                    if (CG == 1 && a.ks > 1) {
 #pragma unroll
-                    for (int c = 0; c < 16; ++c) fp4_out<S>(a, t, c0 + c, n, v[c] * f);
+                        for (int q = 0; q < 16; ++q) part[(c0 + c + q) * 128 + 32 * quarter + lane] = u[q];
+                    } else if (wide && nb + 32 <= a.N) {
+                        if (t.r0 + c0 + c < t.r1) fp4_out16(a, t, c0 + c, nb, u, f, stage + 2048 * warp, lane);
+                    } else {
+#pragma unroll
+                        for (int q = 0; q < 16; ++q) fp4_out<S>(a, t, c0 + c + q, n, u[q] * f);
+                    }
                 }
             }
-            if constexpr (S::ACC != 256) {
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) acc_free(j & 1);
-            }
+            if (S::ACC != 256 && ROUNDS == 1 && COLS * side >= T) acc_free(j & 1);  // (16 tokens: one warp a quarter reads)
             ++j;
         }
     }
@@ -461,13 +462,14 @@ __global__ void __launch_bounds__(FP4_THREADS, 1)
         __syncwarp();
         cluster_sync();
         Fp4Tile t;
-        if (warp < 4 && first < ntiles && fp4_tile<S>(a, starts, nseg, first, t)) {
+        if (warp < FP4_OUT && first < ntiles && fp4_tile<S>(a, starts, nseg, first, t)) {
             const float f = (a.xf ? *a.xf : 1.f) * (a.wf ? *a.wf : 1.f);
-            const uint32_t part = smem_u32(smem) + (32 * warp + lane) * 4;
-            for (int c = rank; c < T && t.r0 + c < t.r1; c += a.ks) {
+            const int row = 32 * (warp & 3) + lane;
+            const uint32_t part = smem_u32(smem) + row * 4;
+            for (int c = rank + a.ks * (warp >> 2); c < T && t.r0 + c < t.r1; c += 2 * a.ks) {
                 float v = 0.f;
                 for (int q = 0; q < a.ks; ++q) v += ld_dsmem_f(map_peer(part + c * 512, q));
-                fp4_out<S>(a, t, c, t.n0 + 32 * warp + lane, v * f);
+                fp4_out<S>(a, t, c, t.n0 + row, v * f);
             }
         }
         __syncwarp();
@@ -479,7 +481,7 @@ __global__ void __launch_bounds__(FP4_THREADS, 1)
         cluster_sync();  // neither CTA leaves while the other's MMAs or arrivals may reach it
     else
         __syncthreads();
-    if (warp == 5) {
+    if (warp == FP4_OUT + 1) {
         tc_fence_after();
         tc_dealloc<CG>(tmem, S::TMEM);
     }
@@ -609,38 +611,43 @@ static int launch(const void* func, int grid, int threads, size_t smem, int clus
 
 struct Fp4Call {
     const uint8_t* x;  // codes or pieces
+    const uint8_t* xt;
     const uint32_t* w;
+    const uint8_t* wt;
     int stack;         // experts, 1 for a dense product
     int64_t ttiles;    // most tiles of tokens that the call can have
     Fp4Args a;
 };
 
+// A matrix of bytes (or of packed 4-bit codes that TMA spreads to bytes), 128 of a row and `rows` rows a box.
+static int map_rows(CUtensorMap* m, const void* base, bool spread, uint64_t row_bytes, uint64_t rows, uint32_t box_rows) {
+    const uint64_t dims[2] = {spread ? 2 * row_bytes : row_bytes, rows}, str[1] = {row_bytes};
+    const uint32_t box[2] = {128, box_rows};
+    return make_tmap(m, spread ? CU_TENSOR_MAP_DATA_TYPE_16U4_ALIGN16B : CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, base, dims, str, box,
+                     CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
+// Scale tiles of 512 bytes, (outer, inner) of them; what a box has beyond the last is zeros.
+static int map_scales(CUtensorMap* m, const void* base, uint64_t inner, uint64_t outer, uint32_t box_inner, uint32_t box_outer) {
+    const uint64_t dims[3] = {128, inner, outer}, str[2] = {512, 512 * inner};
+    const uint32_t box[3] = {128, box_inner, box_outer};
+    return make_tmap(m, CU_TENSOR_MAP_DATA_TYPE_UINT32, 3, base, dims, str, box, CU_TENSOR_MAP_SWIZZLE_NONE);
+}
+
 template <typename S>
 static int gemm_t(const Fp4Call& c, cudaStream_t st) {
     Fp4Args a = c.a;
     a.ns = (a.Kp + S::BK - 1) / S::BK;
-    CUtensorMap tw, tx;
-    if (S::KIND == FP4_SPLIT) {
-        const uint64_t dims[2] = {uint64_t(a.Kp), uint64_t(c.stack) * a.N}, str[1] = {uint64_t(a.Kp) / 2};
-        const uint32_t box[2] = {128, 128};
-        int rc = make_tmap(&tw, CU_TENSOR_MAP_DATA_TYPE_16U4_ALIGN16B, 2, c.w, dims, str, box, CU_TENSOR_MAP_SWIZZLE_128B);
-        if (rc) return rc;
-    } else {
-        const uint64_t dims[2] = {uint64_t(a.Kp) / 2, uint64_t(c.stack) * a.N}, str[1] = {uint64_t(a.Kp) / 2};
-        const uint32_t box[2] = {128, 128};
-        int rc = make_tmap(&tw, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, c.w, dims, str, box, CU_TENSOR_MAP_SWIZZLE_128B);
-        if (rc) return rc;
-    }
-    {
-        const uint64_t row = uint64_t(a.Kp) / (S::KIND == FP4_SPLIT ? 1 : 2);
-        const uint64_t dims[2] = {row, uint64_t(S::P) * a.M}, str[1] = {row};
-        const uint32_t box[2] = {128, uint32_t(S::T / S::CG)};
-        int rc = make_tmap(&tx, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, c.x, dims, str, box, CU_TENSOR_MAP_SWIZZLE_128B);
-        if (rc) return rc;
-    }
-    const int sms = device_info().sm_count;
-    const int64_t slots = int64_t(sms) * (S::T <= 64 ? 2 : 1);
     a.rtiles = (a.N + 127) / 128;
+    Fp4Maps m;
+    int rc = map_rows(&m.w, c.w, S::KIND == FP4_SPLIT, uint64_t(a.Kp) / 2, uint64_t(c.stack) * a.N, 128);
+    if (!rc) rc = map_rows(&m.x, c.x, false, uint64_t(a.Kp) / (S::KIND == FP4_SPLIT ? 1 : 2), uint64_t(S::P) * a.M, S::T / S::CG);
+    if (!rc) rc = map_scales(&m.ws, c.wt, a.ktiles, uint64_t(c.stack) * a.rtiles, S::KB, 1);
+    if (!rc) rc = S::KIND == FP4_SPLIT ? map_scales(&m.xs, c.xt, S::NB, uint64_t(c.ttiles) * a.ktiles, S::NB, 1)
+                                       : map_scales(&m.xs, c.xt, a.ktiles, (uint64_t(a.M) + 127) / 128, S::KB, S::NB);
+    if (rc) return rc;
+    const int sms = device_info().sm_count;
+    const int64_t slots = int64_t(sms) * (S::T <= 32 ? 2 : 1);
     a.ntn = (a.rtiles + S::CG - 1) / S::CG;
     const int64_t tiles = c.ttiles * a.ntn;
     if (tiles > INT32_MAX) return LQ_E_SHAPE;
@@ -651,11 +658,11 @@ static int gemm_t(const Fp4Call& c, cudaStream_t st) {
         a.ks = ks < most ? ks : most;
     }
     const int64_t grid = S::CG == 2 ? (tiles < sms / 2 ? tiles : sms / 2) * 2 : a.ks > 1 ? tiles * a.ks : tiles < slots ? tiles : slots;
-    const size_t smem = 1024 + size_t(S::NS) * S::STAGE + (3 * S::NS + 4) * 8 + 16 + 4 * 2048 + (a.grouped ? (FP4_MAX_SEGMENTS + 2) * 4 : 0);
+    const size_t smem = 1024 + size_t(S::NS) * S::STAGE + (2 * S::NS + 4) * 8 + 32 + FP4_OUT * 2048 + (a.grouped ? (FP4_MAX_SEGMENTS + 2) * 4 : 0);
     static_assert(S::ACC == 256 || S::T * 512 <= S::NS * S::STAGE, "the partial sums of a split fit the ring");
     auto kern = fp4_gemm_kernel<S>;
     if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem)) != cudaSuccess) return LQ_E_CUDA;
-    void* args[] = {&tw, &tx, &a};
+    void* args[] = {&m, &a};
     return launch(reinterpret_cast<const void*>(kern), int(grid), FP4_THREADS, smem, S::CG == 2 ? 2 : a.ks, st, args);
 }
 
@@ -690,8 +697,8 @@ int fp4_qmm_run(const uint32_t* xc, const uint8_t* xt, const float* xf, const ui
     c.ttiles = (M + T - 1) / T;
     a.glu = glu;
     a.dtype = dtype;
-    a.wt = wt;
-    a.xt = xt;
+    c.wt = wt;
+    c.xt = xt;
     a.xf = xf;
     a.wf = wf;
     a.y = y;
@@ -758,8 +765,8 @@ int fp4_linear_run(const Fp4Linear& l, cudaStream_t st) {
     a.glu = l.glu;
     a.dtype = l.dtype;
     a.piece_rows = l.rows;
-    a.wt = l.wt;
-    a.xt = s.tiles;
+    c.wt = l.wt;
+    c.xt = s.tiles;
     a.y = l.y;
     a.grouped = l.segments > 0;
     a.E = l.E;
