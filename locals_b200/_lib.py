@@ -125,7 +125,7 @@ _ext = None
 
 
 def ext():
-    """The loaded _paged_ext.so (built beside liblq.so, which it is linked to): the host side of paged.py and rotary.py."""
+    """The loaded _paged_ext.so (built beside liblq.so, which it is linked to): the host side of paged.py, rotary.py and fp4.py."""
     global _ext
     if _ext is None:
         lib()

@@ -5,7 +5,7 @@
     python -m locals_b200.build -v         # with ptxas register / spill / shared-memory reports
 
 and _paged_ext.so beside it (csrc/paged_ext.cpp with the host compiler against the installed torch: the Python side of
-paged.py and rotary.py, linked to liblq.so).
+paged.py, rotary.py and fp4.py, linked to liblq.so).
 
 Each csrc/*.cu file is its own translation unit (compiled in parallel into csrc/../_build/*.o, then linked with the
 static CUDA runtime). The library is rebuilt whenever the hash of its sources, headers and flags differs from the
@@ -29,6 +29,7 @@ LIB = os.path.join(HERE, "liblq.so")
 HASH = LIB + ".srchash"
 EXT = os.path.join(HERE, "_paged_ext.so")
 EXT_SRC = os.path.join(CSRC, "paged_ext.cpp")
+EXT_FP4 = os.path.join(CSRC, "fp4_ext.h")  # included there
 EXT_HASH = EXT + ".srchash"
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 HEADER = os.path.join(HERE, "..", "include", "lq.h")
@@ -127,7 +128,7 @@ def _ext_hash(cmd) -> str:
     import torch
 
     made = [sys.implementation.cache_tag, torch.__version__, _version(cmd[0]), *cmd]
-    return _digest([EXT_SRC, HEADER], "\n".join(made))
+    return _digest([EXT_SRC, EXT_FP4, HEADER], "\n".join(made))
 
 
 def _version(compiler: str) -> str:
@@ -164,12 +165,12 @@ def build_ext(force: bool = False) -> str:
 
 def build(force: bool = False, verbose: bool = False) -> str:
     """liblq.so, and _paged_ext.so where it compiles: without it (no Python headers, say) all but paged.py and rotary.py
-    works, and those say what is missing."""
+    works (fp4.py needs it too), and those say what is missing."""
     lib = _build_lib(force, verbose)
     try:
         build_ext(force)
     except RuntimeError as e:
-        print(f"_paged_ext.so is not built, paged.py and rotary.py will not run: {e}", file=sys.stderr)
+        print(f"_paged_ext.so is not built, paged.py and rotary.py will not run, nor will fp4.py: {e}", file=sys.stderr)
     return lib
 
 

@@ -95,20 +95,23 @@ static int fp4_segments(int P, int E) { return P < E + 1 ? P : E + 1; }
 
 size_t lq_fp4_experts_workspace(int P, int max_rows, int E, int K, int dtype) {
     if (fp4_rows_ok(P, K, LQ_MXFP4) || !is16(dtype) || E < 1 || max_rows < 1) return 0;
-    return fp4_linear_workspace_bytes(P, K, dtype, fp4_segments(P, E), max_rows);
+    const size_t some = fp4_linear_workspace_bytes(P, K, dtype, fp4_segments(P, E), max_rows);
+    const size_t each = P <= 1024 ? fp4_linear_workspace_bytes(P, K, dtype, P, max_rows) : 0;  // without segments
+    return some > each ? some : each;
 }
 
 int lq_fp4_experts(const void* x, int x_rows, const int32_t* gather_order, int gather_k, const int32_t* starts,
                    const int32_t* experts, const int32_t* nseg, int P, int max_rows, int glu, const uint32_t* codes,
                    const uint8_t* tiles, void* out, int E, int N, int K, int dtype, void* workspace,
                    size_t workspace_bytes, void* stream) {
-    if (!x || !starts || !experts || !nseg || !codes || !tiles || !out || !workspace || !is16(dtype)) return LQ_E_ARG;
-    if (gather_order && gather_k < 1) return LQ_E_ARG;
+    if (!x || !experts || !codes || !tiles || !out || !workspace || !is16(dtype) || !starts != !nseg) return LQ_E_ARG;
+    if (gather_k < 0 || (gather_order && gather_k < 1)) return LQ_E_ARG;
     int rc = fp4_rows_ok(P, K, LQ_MXFP4);
-    if (!rc && (E < 1 || max_rows < 1 || x_rows < 1 || (!gather_order && x_rows < P))) rc = LQ_E_SHAPE;
+    if (!rc && (E < 1 || max_rows < 1 || x_rows < 1 || (!gather_order && x_rows <= (P - 1) / (gather_k ? gather_k : 1)))) rc = LQ_E_SHAPE;
     if (!rc) rc = fp4_rows_ok(int64_t(E) * N, K, LQ_MXFP4);
     if (rc) return rc;
-    if ((glu && N % 2) || fp4_segments(P, E) > 1024) return LQ_E_SHAPE;
+    const int segments = starts ? fp4_segments(P, E) : P;
+    if ((glu && N % 2) || segments > 1024) return LQ_E_SHAPE;
     if (workspace_bytes < lq_fp4_experts_workspace(P, max_rows, E, K, dtype)) return LQ_E_SHAPE;
     if (!aligned(codes, 32) || !aligned(tiles, 16) || !aligned(workspace, 256) || !aligned(x, 2) || !aligned(out, 2)) return LQ_E_ALIGN;
     rc = check_device();
@@ -122,7 +125,7 @@ int lq_fp4_experts(const void* x, int x_rows, const int32_t* gather_order, int g
     l.starts = starts;
     l.experts = experts;
     l.nseg = nseg;
-    l.segments = fp4_segments(P, E);
+    l.segments = segments;
     l.max_rows = max_rows;
     l.E = E;
     l.wc = codes;

@@ -5,8 +5,9 @@
 // the tensor core does all of it: the products of codes are exact, the scales enter as operands, sums are 32 bits. No
 // weight is ever unpacked. Activations of 16 bits are first split in pieces of e4m3 (4 significant bits), each with a power
 // of two a group of 32: bf16 (8 bits) is the sum of 2, fp16 (11 bits) of 3. With E the exponent of the largest magnitude of
-// the group, piece p has the scale 2^(E - 7 - 4 p) and is the rounded remainder of those before it, so the pieces' sum is x
-// exactly down to 2^-13 of that magnitude; below, it is off by at most 2^-21 (bf16) or 2^-25 (fp16) of it, less than
+// the group, piece p has the scale 2^(E - 7 - 5 p) (its values are below 2^8, so what is left after rounding them to 4 bits
+// is at most 2^3) and is the rounded remainder of those before it. The pieces' sum is x exactly down to 2^-14 of that
+// magnitude; below, it is off by at most half a last step, 2^-22 (bf16) or 2^-27 (fp16) of it, less than
 // the 32-bit sum itself loses beside that value. A group that holds an infinity or no number is not a number.
 //
 // Layout. Weights are the MMA's A operand (128 rows of w a tile, one a tensor-memory lane), T tokens its N side, so that one
@@ -234,8 +235,8 @@ __global__ void __launch_bounds__(FP4_THREADS, S::T <= 32 ? 2 : 1) fp4_gemm_kern
     grid_dep_launch();
     if (a.grouped) {
         grid_dep_wait();
-        const int n = min(*a.nseg, a.max_seg);
-        for (int i = threadIdx.x; i <= n; i += FP4_THREADS) seg[1 + i] = min(max(a.starts[i], 0), a.M);
+        const int n = a.nseg ? min(*a.nseg, a.max_seg) : a.M;  // without segments, each row is one
+        for (int i = threadIdx.x; i <= n; i += FP4_THREADS) seg[1 + i] = a.starts ? min(max(a.starts[i], 0), a.M) : i;
         if (threadIdx.x == 0) seg[0] = n;
     }
     tc_fence_before();
@@ -496,7 +497,7 @@ struct SplitArgs {
     bool vec;
     uint8_t* pieces;  // (P, rows, Kp)
     uint8_t* tiles;   // (token tile, K tile, nb, 512)
-    const int32_t* order;  // row j is row order[j] / gather of x; NULL: row j
+    const int32_t* order;  // gather > 0: row j is row order[j] / gather of x (order NULL: j / gather); 0: row j
     int gather, src_rows;
     int grouped, max_seg;
     const int32_t* starts;
@@ -528,8 +529,8 @@ __global__ void __launch_bounds__(256) fp4_split_kernel(const SplitArgs a) {
         const int row = int(u / words), word = int(u - int64_t(row) * words);
         const uint32_t mask = 0xFFFFu << (threadIdx.x & 16);
         int64_t src = row;
-        if (a.order) {
-            src = a.order[row] / a.gather;
+        if (a.gather) {
+            src = (a.order ? a.order[row] : row) / a.gather;
             if (src < 0 || src >= a.src_rows) {
                 record_status(LQ_DEV_BOUNDS);
                 src = 0;
@@ -547,12 +548,12 @@ __global__ void __launch_bounds__(256) fp4_split_kernel(const SplitArgs a) {
         }
         int tile = row / a.T, at = row % a.T;
         if (a.grouped) {
-            int lo = 0, hi = min(*a.nseg, a.max_seg);
+            int lo = a.starts ? 0 : row, hi = a.starts ? min(*a.nseg, a.max_seg) : 0;
             while (hi - lo > 1) {
                 const int mid = (lo + hi) / 2;
                 if (a.starts[mid] <= row) lo = mid; else hi = mid;
             }
-            const int s0 = min(max(a.starts[lo], 0), row);
+            const int s0 = a.starts ? min(max(a.starts[lo], 0), row) : row;
             tile = s0 / a.T + lo + (row - s0) / a.T;
             at = (row - s0) % a.T;
         }
@@ -581,7 +582,7 @@ __global__ void __launch_bounds__(256) fp4_split_kernel(const SplitArgs a) {
                 const int q = a.stack ? p * a.T + at : at;
                 tl[(a.stack ? 0 : p * ((a.T + 127) / 128) + q / 128) * 512 + fp4_tile_byte(q % 128, g)] = uint8_t(byte);
             }
-            const int next = byte == 255 ? 255 : byte < 4 ? 0 : byte - 4;
+            const int next = byte == 255 ? 255 : byte < 5 ? 0 : byte - 5;
             const float more = __uint_as_float(uint32_t(127 + (byte == 255 ? 0 : byte - next)) << 23);
 #pragma unroll
             for (int i = 0; i < 8; ++i) v[i] *= more;

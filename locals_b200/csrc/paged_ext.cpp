@@ -1,4 +1,4 @@
-// The host side of locals_b200.paged and locals_b200.rotary between Python and the C ABI (include/lq.h): argument checks,
+// The host side of locals_b200.paged, locals_b200.rotary and (fp4_ext.h) locals_b200.fp4 between Python and the C ABI (include/lq.h): argument checks,
 // outputs and workspaces from the tensor library's allocator on the current stream, one call of liblq.so each. What these
 // operators do at their smallest sizes takes the GPU a few microseconds, less than the checks and allocations take in
 // Python (attend at one token: 19.5 us a call there).
@@ -8,8 +8,10 @@
 
 #include <ATen/ATen.h>
 #include <c10/cuda/CUDAFunctions.h>
+#include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 
+#include <algorithm>
 #include <optional>
 #include <string>
 #include <tuple>
@@ -275,6 +277,8 @@ Tensor attend(Tensor q, const Triple& keys, const Triple& values, const Tensor& 
     return out;
 }
 
+#include "fp4_ext.h"
+
 }  // namespace
 
 PYBIND11_MODULE(_paged_ext, m) {
@@ -283,4 +287,10 @@ PYBIND11_MODULE(_paged_ext, m) {
     m.def("append", &append);
     m.def("read", &read_slots);
     m.def("attend", &attend);
+    m.def("fp4_quantize", &fp4::quantize);
+    m.def("fp4_dequantize", &fp4::dequantize);
+    m.def("fp4_product", &fp4::product);
+    m.def("fp4_linear", &fp4::linear);
+    m.def("fp4_grouped", &fp4::grouped);
+    m.def("fp4_experts", &fp4::experts);
 }

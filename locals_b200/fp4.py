@@ -16,16 +16,14 @@ only: the tensor cores take an e4m3 scale with 4 bits on both sides only.
 
 from __future__ import annotations
 
-from typing import NamedTuple, Optional, Sequence, Tuple
+from typing import NamedTuple, Optional, Tuple
 
 import torch
 
-from . import _lib, moe
-from ._lib import call
-from .kernels import _ptr, _stream, dtype_code
+from . import moe
+from ._lib import ext
 
 GROUP = {"mxfp4": 32, "nvfp4": 16}
-_MODE = {"mxfp4": _lib.MXFP4, "nvfp4": _lib.NVFP4}
 PAD = 128  # codes a row is filled to a multiple of
 
 
@@ -45,11 +43,11 @@ class Fp4(NamedTuple):
         return self.codes.shape[-2]
 
 
-def _mode(mode: str) -> int:
+def _group(mode: str) -> int:
     try:
-        return _MODE[mode]
+        return GROUP[mode]
     except KeyError:
-        raise ValueError(f"a 4-bit format is one of {', '.join(_MODE)}, not {mode!r}") from None
+        raise ValueError(f"a 4-bit format is one of {', '.join(GROUP)}, not {mode!r}") from None
 
 
 def _padded(K: int) -> int:
@@ -65,66 +63,13 @@ def _check_scale(scale: Optional[torch.Tensor], mode: str, device) -> None:
         raise ValueError("scale is one float32 element on the matrix' device")
 
 
-def _check(a: Fp4, what: str, dims: Sequence[int] = (2,)) -> None:
-    """An operand's tensors fit one another: the kernels read them through raw pointers."""
-    code = _mode(a.mode)
-    if not a.codes.is_cuda or a.tiles.device != a.codes.device:
-        raise ValueError(f"{what}: codes and tiles are CUDA tensors of one device")
-    if a.codes.dtype not in (torch.int32, torch.uint32) or a.tiles.dtype != torch.uint8:
-        raise TypeError(f"{what}: codes are 32-bit words and tiles uint8")
-    if a.codes.dim() not in dims:
-        raise ValueError(f"{what}: codes have {' or '.join(map(str, dims))} dimensions, not {a.codes.dim()}")
-    if a.K < 1:
-        raise ValueError(f"{what}: K={a.K}")
-    N, Kp = a.codes.shape[-2], _padded(a.K)
-    want = (*a.codes.shape[:-2], -(-N // 128), Kp // (4 * GROUP[a.mode]), 512)
-    if a.codes.shape[-1] != Kp // 8 or tuple(a.tiles.shape) != want:
-        raise ValueError(f"{what}: codes {tuple(a.codes.shape)} / tiles {tuple(a.tiles.shape)} do not hold {N} rows of "
-                         f"K={a.K} in {a.mode} (tiles {want})")
-    if not a.codes.is_contiguous() or not a.tiles.is_contiguous():
-        raise ValueError(f"{what}: codes and tiles are contiguous")
-    _check_scale(a.scale, a.mode, a.codes.device)
-    return code
-
-
-class _on:
-    """The device of a call's tensors made current where it is not."""
-
-    def __init__(self, device: torch.device):
-        i = device.index
-        self.guard = None if i is None or i == torch._C._cuda_getDevice() else torch.cuda.device(i)
-
-    def __enter__(self):
-        if self.guard is not None:
-            self.guard.__enter__()
-
-    def __exit__(self, *a):
-        if self.guard is not None:
-            self.guard.__exit__(*a)
-
-
-def _rows(x: torch.Tensor) -> torch.Tensor:
-    """x (..., K) as rows: a view where the rows lie at one distance and a row's values next to one another."""
-    if x.dim() == 0:
-        raise ValueError("a matrix of rows is wanted")
-    x2 = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
-    if x2.shape[1] > 1 and x2.stride(1) != 1 or x2.shape[0] > 1 and x2.stride(0) < x2.shape[1]:
-        x2 = x2.contiguous()
-    return x2
-
-
-def _row_stride(x2: torch.Tensor) -> int:
-    return x2.stride(0) if x2.shape[0] > 1 else x2.shape[1]
-
-
 # ---- the format ----------------------------------------------------------------------------------
 
 def pack(codes: torch.Tensor, scales: torch.Tensor, mode: str = "mxfp4", scale: Optional[torch.Tensor] = None) -> Fp4:
     """An operand of a matrix or stack in MLX's layout: ``codes`` (..., N, K/8) 32-bit words of eight codes, lowest bits
     first, ``scales`` uint8 (..., N, K/group). Done once: the scales are laid out in tiles (and codes copied where K is no
     multiple of 128)."""
-    _mode(mode)
-    group = GROUP[mode]
+    group = _group(mode)
     if codes.dtype not in (torch.int32, torch.uint32) or scales.dtype != torch.uint8:
         raise TypeError("codes are 32-bit words and scales uint8")
     K = codes.shape[-1] * 8
@@ -166,35 +111,12 @@ def quantize(x: torch.Tensor, mode: str = "mxfp4", scale: Optional[torch.Tensor]
     (one float32 element > 0; None: 1) is the matrix' factor, such as its largest magnitude / 2688. Codes are the nearest to
     x / (their scales), ties to the even code, and 6 beyond it. A group with an infinity or no number in it has the scale that is
     not a number."""
-    code = _mode(mode)
-    dt = dtype_code(x.dtype)
-    if not x.is_cuda:
-        raise ValueError("locals_b200 kernels take CUDA tensors")
-    _check_scale(scale, mode, x.device)
-    x2 = _rows(x)
-    R, K = x2.shape
-    if K < 1:
-        raise ValueError("rows of no values")
-    Kp = _padded(K)
-    codes = torch.empty((R, Kp // 8), dtype=torch.int32, device=x.device)
-    tiles = torch.empty((-(-R // 128), Kp // (4 * GROUP[mode]), 512), dtype=torch.uint8, device=x.device)
-    if R:
-        with _on(x.device):
-            call("lq_fp4_quantize", x2.data_ptr(), dt, _row_stride(x2), R, K, code, _ptr(scale), codes.data_ptr(),
-                 tiles.data_ptr(), _stream())
-    return Fp4(codes, tiles, mode, K, scale)
+    return Fp4(*ext().fp4_quantize(x, mode, scale), mode, x.shape[-1], scale)
 
 
 def dequantize(a: Fp4, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """The values of an operand, (N, K) or (E, N, K), rounded once to ``dtype``."""
-    code = _check(a, "dequantize", (2, 3))
-    dt = dtype_code(dtype)
-    out = torch.empty((*a.codes.shape[:-1], a.K), dtype=dtype, device=a.codes.device)
-    if out.numel():
-        with _on(out.device):
-            call("lq_fp4_dequantize", a.codes.data_ptr(), a.tiles.data_ptr(), a.codes.shape[0] if a.codes.dim() == 3 else 1,
-                 a.rows, a.K, code, _ptr(a.scale), dt, out.data_ptr(), _stream())
-    return out
+    return ext().fp4_dequantize(a, dtype)
 
 
 # ---- products ------------------------------------------------------------------------------------
@@ -202,51 +124,13 @@ def dequantize(a: Fp4, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
 def matmul(x, w: Fp4, dtype: Optional[torch.dtype] = None, glu: bool = False) -> torch.Tensor:
     """y = x . w^T with 32-bit sums, rounded once. ``x`` an ``Fp4`` matrix of w's format: y (M, N) in ``dtype`` (default
     bf16; fp16, fp32). ``x`` a tensor (..., K) in fp16 or bf16 and w in mxfp4: y (..., N) in x's dtype; x is exact down to
-    2^-13 of a group of 32's largest magnitude, below that off by at most 2^-21 of it, and a row with an infinity or no number in
+    2^-14 of a group of 32's largest magnitude, below that off by at most 2^-22 of it, and a row with an infinity or no number in
     it gives no numbers. ``glu``: w holds gate and up rows in turn (``interleave``) and y (..., N / 2) is silu(gate) * up."""
-    code = _check(w, "w")
-    N = w.rows
-    if glu and N % 2:
-        raise ValueError(f"{N} rows are no pairs of gate and up")
-    width = N // 2 if glu else N
     if isinstance(x, Fp4):
-        _check(x, "x")
-        if x.mode != w.mode or x.K != w.K:
-            raise ValueError(f"x ({x.mode}, K={x.K}) and w ({w.mode}, K={w.K}) do not multiply")
-        if x.codes.device != w.codes.device:
-            raise ValueError("x and w are on different devices")
-        dtype = dtype or torch.bfloat16
-        y = torch.empty((x.rows, width), dtype=dtype, device=w.codes.device)
-        dt = dtype_code(dtype)
-        if y.numel():
-            with _on(y.device):
-                call("lq_fp4_qmm", x.codes.data_ptr(), x.tiles.data_ptr(), _ptr(x.scale), w.codes.data_ptr(),
-                     w.tiles.data_ptr(), _ptr(w.scale), x.rows, N, w.K, code, int(glu), dt, y.data_ptr(), _stream())
-        return y
-    _check_16(x, w)
+        return ext().fp4_product(x, w, dtype or torch.bfloat16, glu)
     if dtype is not None and dtype != x.dtype:
         raise TypeError("a product of 16-bit activations has their dtype")
-    x2 = _rows(x)
-    M, dt = x2.shape[0], dtype_code(x.dtype)
-    y = torch.empty((M, width), dtype=x.dtype, device=x.device)
-    if y.numel():
-        with _on(y.device):
-            n = int(_lib.lib().lq_fp4_linear_workspace(M, w.K, dt))
-            ws = torch.empty(n, dtype=torch.uint8, device=x.device)
-            call("lq_fp4_linear", x2.data_ptr(), _row_stride(x2), w.codes.data_ptr(), w.tiles.data_ptr(), M, N, w.K, int(glu),
-                 dt, y.data_ptr(), ws.data_ptr(), n, _stream())
-    return y.reshape(*x.shape[:-1], width)
-
-
-def _check_16(x: torch.Tensor, w: Fp4) -> None:
-    if x.dtype not in (torch.float16, torch.bfloat16):
-        raise TypeError(f"activations are fp16, bf16 or Fp4, not {x.dtype}")
-    if w.mode != "mxfp4":
-        raise ValueError(f"16-bit activations are multiplied with mxfp4 weights, not {w.mode}: quantize them for it")
-    if x.device != w.codes.device:
-        raise ValueError("x and w are on different devices")
-    if x.dim() < 1 or x.shape[-1] != w.K:
-        raise ValueError(f"x {tuple(x.shape)} does not match K={w.K}")
+    return ext().fp4_linear(x, w, glu)
 
 
 # ---- routed experts --------------------------------------------------------------------------------
@@ -255,60 +139,24 @@ def grouped(xs: torch.Tensor, grouping, w: Fp4, max_rows: int, glu: bool = False
     """``moe.experts`` for a stack ``w`` (E, N, K) in mxfp4: the rows of each segment of ``grouping`` (moe.group) times its
     expert's matrix, (P, N), or (P, N / 2) with ``glu``. With gather_k, xs is the token matrix and row j of the pairs reads
     token order[j] // gather_k; otherwise xs holds one row a pair, in expert order."""
-    _check(w, "experts", (3,))
-    _check_16(xs, w)
     order, starts, experts_, nseg, _ = grouping
-    E, N, P = w.codes.shape[0], w.rows, order.numel()
-    if xs.dim() != 2 or not xs.is_contiguous():
-        raise ValueError("xs is a contiguous matrix of rows")
-    if glu and N % 2:
-        raise ValueError(f"{N} rows are no pairs of gate and up")
-    if not gather_k and xs.shape[0] < P:
-        raise ValueError(f"{xs.shape[0]} rows for {P} pairs")
-    out = torch.empty((P, N // 2 if glu else N), dtype=xs.dtype, device=xs.device)
-    if out.numel():
-        dt = dtype_code(xs.dtype)
-        with _on(out.device):
-            n = int(_lib.lib().lq_fp4_experts_workspace(P, max_rows, E, w.K, dt))
-            ws = torch.empty(n, dtype=torch.uint8, device=xs.device)
-            call("lq_fp4_experts", xs.data_ptr(), xs.shape[0], order.data_ptr() if gather_k else None, gather_k,
-                 starts.data_ptr(), experts_.data_ptr(), nseg.data_ptr(), P, max_rows, int(glu), w.codes.data_ptr(),
-                 w.tiles.data_ptr(), out.data_ptr(), E, N, w.K, dt, ws.data_ptr(), n, _stream())
-    return out
-
-
-def _check_experts(x: torch.Tensor, inds: torch.Tensor, gate_up: Fp4, down: Fp4) -> None:
-    _check(gate_up, "gate_up", (3,))
-    _check(down, "down", (3,))
-    if x.dim() != 2 or inds.dim() != 2 or inds.shape[0] != x.shape[0] or inds.dtype not in (torch.int32, torch.uint32):
-        raise ValueError(f"x (T, D) and inds int32 (T, k) are wanted, not {tuple(x.shape)} and {tuple(inds.shape)}")
-    if inds.device != x.device:
-        raise ValueError("x and inds are on different devices")
-    E, rows, D = gate_up.codes.shape[0], gate_up.rows, gate_up.K
-    if rows % 2 or down.codes.shape[0] != E or down.K != rows // 2 or down.rows != D:
-        raise ValueError(f"gate_up ({E}, {rows}, {D}) and down ({down.codes.shape[0]}, {down.rows}, {down.K}) are no experts")
-
-
-def _pairs(x: torch.Tensor, inds: torch.Tensor, gate_up: Fp4, down: Fp4, grouping) -> torch.Tensor:
-    M, k = inds.shape
-    h = grouped(x.contiguous(), grouping, gate_up, M, glu=True, gather_k=k)
-    return grouped(h, grouping, down, M)
-
-
-def _grouping(inds: torch.Tensor, E: int):
-    return moe.direct_grouping(inds) if inds.shape[0] <= moe.DIRECT_MAX_TOKENS else moe.group(inds, E)
+    return ext().fp4_grouped(xs, order, starts, experts_, nseg, w, max_rows, glu, gather_k)
 
 
 def switch_glu(x: torch.Tensor, inds: torch.Tensor, gate_up: Fp4, down: Fp4, grouping=None) -> torch.Tensor:
     """``moe.switch_glu`` for mxfp4 experts: x (M, D), expert ids inds (M, k), gate_up (E, 2 I, D) with gate and up rows in
     turn (``interleave``), down (E, D, I): (M, k, D), slot r of token t in row (t, r)."""
-    _check_experts(x, inds, gate_up, down)
     M, k = inds.shape
+    if x.dim() != 2 or x.shape[0] != M:
+        raise ValueError(f"x (M, D) and inds (M, k) are wanted, not {tuple(x.shape)} and {tuple(inds.shape)}")
+    if gate_up.rows != 2 * down.K or down.rows != gate_up.K or gate_up.codes.shape[0] != down.codes.shape[0]:
+        raise ValueError("gate_up (E, 2 I, D) and down (E, D, I) do not fit one another")
     if M == 0 or k == 0:
-        return x.new_empty((M, k, x.shape[1]))
-    with _on(x.device):
-        g = grouping if grouping is not None else _grouping(inds, gate_up.codes.shape[0])
-        ys = _pairs(x, inds, gate_up, down, g)
+        return x.new_empty((M, k, down.rows))
+    with torch.cuda.device(x.device):
+        g = grouping if grouping is not None else moe.group(inds, gate_up.codes.shape[0])
+        h = grouped(x.contiguous(), g, gate_up, M, glu=True, gather_k=k)
+        ys = grouped(h, g, down, M)
         if g[4] is not None:
             ys = moe.gather(ys, g[4], 1)
     return ys.reshape(M, k, -1)
@@ -316,15 +164,8 @@ def switch_glu(x: torch.Tensor, inds: torch.Tensor, gate_up: Fp4, down: Fp4, gro
 
 def experts(x: torch.Tensor, inds: torch.Tensor, weights: torch.Tensor, gate_up: Fp4, down: Fp4) -> torch.Tensor:
     """The routed experts of a step: sum over slots r of weights[t, r] * expert inds[t, r] of x[t], (T, D) in x's dtype
-    (``switch_glu``, then ``moe.combine``). weights float32 (T, k). A token names an expert at most once."""
-    _check_experts(x, inds, gate_up, down)
-    if weights.shape != inds.shape or weights.dtype != torch.float32 or weights.device != x.device:
-        raise ValueError("weights are float32, one an expert id")
-    if inds.numel() == 0:
-        return torch.zeros_like(x)
-    with _on(x.device):
-        g = _grouping(inds, gate_up.codes.shape[0])
-        return moe.combine(_pairs(x, inds, gate_up, down, g), weights.contiguous(), g[4])
+    (grouping, gate and up, down, ``moe.combine``). inds int32 and weights float32 (T, k), as moe.route gives them."""
+    return ext().fp4_experts(x, inds, weights, gate_up, down)
 
 
 class MoELayer:
