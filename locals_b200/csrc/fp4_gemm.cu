@@ -18,6 +18,7 @@
 // Few tiles: a cluster of CTAs splits a tile's K and joins its sums through distributed shared memory, in rank order.
 #include <cuda_runtime.h>
 
+#include <atomic>
 #include <type_traits>
 
 #include "fp4.cuh"
@@ -45,8 +46,9 @@ struct Fp4Shape {
     static constexpr int SFA = KB * 512, SFB = KB * NB * 512;
     static constexpr int TX = A_TX + B_BYTES + SFA + SFB;  // bytes that arrive for a stage (in each CTA)
     static constexpr int STAGE = (A_BYTES + B_BYTES + SFA + SFB + 1023) / 1024 * 1024;
-    static constexpr int SMEM = (T <= 32 ? 88 : 204) * 1024;  // narrow tiles leave room for a second CTA
-    static constexpr int FIT = SMEM / STAGE, NS = FIT < FP4_MAX_STAGES ? FIT : FP4_MAX_STAGES;
+    // stages of the ring: one CTA an SM, or (narrow tiles, more of them than SMs) two
+    static constexpr int ring(int kb) { return kb * 1024 / STAGE < FP4_MAX_STAGES ? kb * 1024 / STAGE : FP4_MAX_STAGES; }
+    static constexpr int NS = ring(204), NS_TWO = ring(88);
     static constexpr int N = STACK ? P * T : T;
     static constexpr int ACC = N <= 32 ? 32 : N <= 64 ? 64 : N <= 128 ? 128 : 256;
     // 256 columns: the two accumulators share 128, which are read out first
@@ -63,6 +65,7 @@ struct Fp4Args {
     int ntn, ntiles;     // tiles along N, all tiles (dense)
     int rtiles;          // scale tiles along N
     int ks;              // CTAs that split a tile's K
+    int nst;             // stages of the ring
     int glu, dtype;
     int piece_rows;      // rows of one piece of x
     const float* xf;     // factors, or NULL
@@ -196,6 +199,26 @@ __device__ __forceinline__ void fp4_out16(const Fp4Args& a, const Fp4Tile& t, in
     }
 }
 
+// Four neighbouring rows of w (two pairs of gate and up) and one token.
+__device__ __forceinline__ void fp4_out4(const Fp4Args& a, const Fp4Tile& t, int c, int n, float4 v, float f) {
+    float o[4] = {v.x * f, v.y * f, v.z * f, v.w * f};
+    const int width = a.glu ? a.N / 2 : a.N, at = a.glu ? n / 2 : n, some = a.glu ? 2 : 4;
+    if (a.glu) {
+        o[0] = o[0] / (1.f + __expf(-o[0])) * o[1];
+        o[1] = o[2] / (1.f + __expf(-o[2])) * o[3];
+    }
+    const int64_t first = int64_t(t.r0 + c) * width + at;
+    if (a.dtype != LQ_F32 && !a.glu && width % 4 == 0 && n + 4 <= a.N && reinterpret_cast<uintptr_t>(a.y) % 8 == 0) {
+        uint2 w = a.dtype == LQ_BF16 ? make_uint2(cvt_bf16x2(o[1], o[0]), cvt_bf16x2(o[3], o[2]))
+                                     : make_uint2(cvt_f16x2(o[1], o[0]), cvt_f16x2(o[3], o[2]));
+        *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.y) + first) = w;
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        if (i < some && at + i < width) fp4_store(a, first + i, o[i]);
+}
+
 // The tensor maps of a product: codes of w and x (or pieces of x), scale tiles of w and x.
 struct Fp4Maps {
     CUtensorMap w, x, ws, xs;
@@ -203,7 +226,8 @@ struct Fp4Maps {
 
 template <typename S>
 __global__ void __launch_bounds__(FP4_THREADS, S::T <= 32 ? 2 : 1) fp4_gemm_kernel(const __grid_constant__ Fp4Maps m, const Fp4Args a) {
-    constexpr int T = S::T, P = S::P, NS = S::NS, CG = S::CG;
+    constexpr int T = S::T, P = S::P, CG = S::CG;
+    const int NS = a.nst;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint64_t* full = reinterpret_cast<uint64_t*>(smem + NS * S::STAGE);  // (in a pair, the lower rank's, for both)
@@ -465,12 +489,22 @@ __global__ void __launch_bounds__(FP4_THREADS, S::T <= 32 ? 2 : 1) fp4_gemm_kern
         Fp4Tile t;
         if (warp < FP4_OUT && first < ntiles && fp4_tile<S>(a, starts, nseg, first, t)) {
             const float f = (a.xf ? *a.xf : 1.f) * (a.wf ? *a.wf : 1.f);
-            const int row = 32 * (warp & 3) + lane;
-            const uint32_t part = smem_u32(smem) + row * 4;
-            for (int c = rank + a.ks * (warp >> 2); c < T && t.r0 + c < t.r1; c += 2 * a.ks) {
-                float v = 0.f;
-                for (int q = 0; q < a.ks; ++q) v += ld_dsmem_f(map_peer(part + c * 512, q));
-                fp4_out<S>(a, t, c, t.n0 + row, v * f);
+            const uint32_t part = smem_u32(smem) + lane * 16;  // a lane takes four rows of w
+            for (int c = rank + a.ks * warp; c < T && t.r0 + c < t.r1; c += FP4_OUT * a.ks) {
+                float4 p[8];
+#pragma unroll
+                for (int q = 0; q < 8; ++q)
+                    if (q < a.ks) p[q] = ld_dsmem_f4(map_peer(part + c * 512, q));
+                float4 v = p[0];
+#pragma unroll
+                for (int q = 1; q < 8; ++q)
+                    if (q < a.ks) {
+                        v.x += p[q].x;
+                        v.y += p[q].y;
+                        v.z += p[q].z;
+                        v.w += p[q].w;
+                    }
+                fp4_out4(a, t, c, t.n0 + 4 * lane, v, f);
             }
         }
         __syncwarp();
@@ -635,6 +669,35 @@ static int map_scales(CUtensorMap* m, const void* base, uint64_t inner, uint64_t
     return make_tmap(m, CU_TENSOR_MAP_DATA_TYPE_UINT32, 3, base, dims, str, box, CU_TENSOR_MAP_SWIZZLE_NONE);
 }
 
+// Clusters of ks CTAs that the current device runs at once: its SMs come in groups that a cluster does not leave, so that 48
+// clusters of three need not fit 148 SMs. Asked once a device, kernel and size.
+template <typename S>
+static int max_clusters(int ks, size_t smem) {
+    static std::atomic<int> known[16][2][9];
+    const int dev = device_info().device;
+    if (dev < 0 || dev >= 16) return 0;
+    std::atomic<int>& k = known[dev][smem > size_t(S::T <= 32 ? S::NS_TWO : S::NS) * S::STAGE + 1024 + FP4_OUT * 2048 + 1024][ks];
+    int n = k.load(std::memory_order_relaxed);
+    if (n == 0) {
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3(unsigned(ks));
+        cfg.blockDim = dim3(FP4_THREADS);
+        cfg.dynamicSmemBytes = smem;
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = unsigned(ks);
+        attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = 1;
+        if (cudaOccupancyMaxActiveClusters(&n, fp4_gemm_kernel<S>, &cfg) != cudaSuccess) {
+            cudaGetLastError();
+            return 0;
+        }
+        k.store(n > 0 ? n : -1, std::memory_order_relaxed);
+    }
+    return n;
+}
+
 template <typename S>
 static int gemm_t(const Fp4Call& c, cudaStream_t st) {
     Fp4Args a = c.a;
@@ -648,21 +711,25 @@ static int gemm_t(const Fp4Call& c, cudaStream_t st) {
                                        : map_scales(&m.xs, c.xt, a.ktiles, (uint64_t(a.M) + 127) / 128, S::KB, S::NB);
     if (rc) return rc;
     const int sms = device_info().sm_count;
-    const int64_t slots = int64_t(sms) * (S::T <= 32 ? 2 : 1);
     a.ntn = (a.rtiles + S::CG - 1) / S::CG;
     const int64_t tiles = c.ttiles * a.ntn;
     if (tiles > INT32_MAX) return LQ_E_SHAPE;
     a.ntiles = int(tiles);
-    a.ks = 1;
-    if (S::CG == 1 && S::ACC != 256 && tiles < sms) {  // a tile's K split over the CTAs of a cluster
-        const int most = a.ns < 8 ? a.ns : 8, ks = int(sms / tiles);  // every CTA has a stage
-        a.ks = ks < most ? ks : most;
-    }
-    const int64_t grid = S::CG == 2 ? (tiles < sms / 2 ? tiles : sms / 2) * 2 : a.ks > 1 ? tiles * a.ks : tiles < slots ? tiles : slots;
-    const size_t smem = 1024 + size_t(S::NS) * S::STAGE + (2 * S::NS + 4) * 8 + 32 + FP4_OUT * 2048 + (a.grouped ? (FP4_MAX_SEGMENTS + 2) * 4 : 0);
-    static_assert(S::ACC == 256 || S::T * 512 <= S::NS * S::STAGE, "the partial sums of a split fit the ring");
+    a.nst = S::T <= 32 ? S::NS_TWO : S::NS;
+    const size_t smem = 1024 + size_t(a.nst) * S::STAGE + (2 * a.nst + 4) * 8 + 32 + FP4_OUT * 2048 + (a.grouped ? (FP4_MAX_SEGMENTS + 2) * 4 : 0);
+    static_assert(S::NS_TWO >= 2 || S::T > 32, "two CTAs an SM");
+    static_assert(S::ACC == 256 || S::T * 512 <= (S::T <= 32 ? S::NS_TWO : S::NS) * S::STAGE, "the partial sums of a split fit the ring");
     auto kern = fp4_gemm_kernel<S>;
     if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem)) != cudaSuccess) return LQ_E_CUDA;
+    // Few tiles: a tile's K split over as many CTAs of a cluster as still run all at once, each with a stage at least.
+    a.ks = 1;
+    if (S::CG == 1) {
+        const int most = a.ns < 8 ? a.ns : 8;
+        for (int ks = most; ks > 1 && a.ks == 1; --ks)
+            if (tiles * ks <= int64_t(sms) * (S::T <= 32 ? 2 : 1) && tiles <= max_clusters<S>(ks, smem)) a.ks = ks;
+    }
+    const int64_t slots = int64_t(sms) * (S::T <= 32 ? 2 : 1);
+    const int64_t grid = S::CG == 2 ? (tiles < sms / 2 ? tiles : sms / 2) * 2 : a.ks > 1 ? tiles * a.ks : tiles < slots ? tiles : slots;
     void* args[] = {&m, &a};
     return launch(reinterpret_cast<const void*>(kern), int(grid), FP4_THREADS, smem, S::CG == 2 ? 2 : a.ks, st, args);
 }
