@@ -66,13 +66,15 @@ size_t lq_fp4_linear_workspace(int M, int K, int dtype) {
 
 int lq_fp4_linear(const void* x, int64_t x_row, const uint32_t* codes, const uint8_t* tiles, int M, int N, int K, int glu,
                   int dtype, void* y, void* workspace, size_t workspace_bytes, void* stream) {
-    if (!x || !codes || !tiles || !y || !workspace || !is16(dtype)) return LQ_E_ARG;
+    if (!x || !codes || !tiles || !y || !is16(dtype)) return LQ_E_ARG;
     int rc = fp4_rows_ok(M, K, LQ_MXFP4);
     if (!rc) rc = fp4_rows_ok(N, K, LQ_MXFP4);
     if (rc) return rc;
     if (glu && N % 2) return LQ_E_SHAPE;
     if (x_row < K && M > 1) return LQ_E_SHAPE;
-    if (workspace_bytes < lq_fp4_linear_workspace(M, K, dtype)) return LQ_E_SHAPE;
+    const size_t bytes = lq_fp4_linear_workspace(M, K, dtype);
+    if (bytes && !workspace) return LQ_E_ARG;
+    if (workspace_bytes < bytes) return LQ_E_SHAPE;
     if (!aligned(codes, 32) || !aligned(tiles, 16) || !aligned(workspace, 256) || !aligned(x, 2) || !aligned(y, 2)) return LQ_E_ALIGN;
     rc = check_device();
     if (rc) return rc;
@@ -81,6 +83,7 @@ int lq_fp4_linear(const void* x, int64_t x_row, const uint32_t* codes, const uin
     l.x_row = x_row;
     l.wc = codes;
     l.wt = tiles;
+    l.src_rows = M;
     l.rows = M;
     l.N = N;
     l.K = K;
@@ -104,7 +107,7 @@ int lq_fp4_experts(const void* x, int x_rows, const int32_t* gather_order, int g
                    const int32_t* experts, const int32_t* nseg, int P, int max_rows, int glu, const uint32_t* codes,
                    const uint8_t* tiles, void* out, int E, int N, int K, int dtype, void* workspace,
                    size_t workspace_bytes, void* stream) {
-    if (!x || !experts || !codes || !tiles || !out || !workspace || !is16(dtype) || !starts != !nseg) return LQ_E_ARG;
+    if (!x || !experts || !codes || !tiles || !out || !is16(dtype) || !starts != !nseg) return LQ_E_ARG;
     if (gather_k < 0 || (gather_order && gather_k < 1)) return LQ_E_ARG;
     int rc = fp4_rows_ok(P, K, LQ_MXFP4);
     if (!rc && (E < 1 || max_rows < 1 || x_rows < 1 || (!gather_order && x_rows <= (P - 1) / (gather_k ? gather_k : 1)))) rc = LQ_E_SHAPE;
@@ -112,7 +115,9 @@ int lq_fp4_experts(const void* x, int x_rows, const int32_t* gather_order, int g
     if (rc) return rc;
     const int segments = starts ? fp4_segments(P, E) : P;
     if ((glu && N % 2) || segments > 1024) return LQ_E_SHAPE;
-    if (workspace_bytes < lq_fp4_experts_workspace(P, max_rows, E, K, dtype)) return LQ_E_SHAPE;
+    const size_t bytes = lq_fp4_experts_workspace(P, max_rows, E, K, dtype);
+    if (bytes && !workspace) return LQ_E_ARG;
+    if (workspace_bytes < bytes) return LQ_E_SHAPE;
     if (!aligned(codes, 32) || !aligned(tiles, 16) || !aligned(workspace, 256) || !aligned(x, 2) || !aligned(out, 2)) return LQ_E_ALIGN;
     rc = check_device();
     if (rc) return rc;

@@ -116,7 +116,16 @@ void check_16(const Tensor& x, const Operand& w) {
     need(x.dim() >= 1 && x.size(-1) == w.K, "x does not have w's K values a row");
 }
 
-Tensor workspace(size_t bytes, const Tensor& x) { return at::empty({int64_t(bytes)}, x.options().dtype(at::kByte)); }
+// A workspace of so many bytes, which the call that uses it outlives.
+struct Workspace {
+    Tensor t;
+    void* p = nullptr;
+    Workspace(size_t bytes, const Tensor& x) {
+        if (!bytes) return;
+        t = at::empty({int64_t(bytes)}, x.options().dtype(at::kByte));
+        p = t.data_ptr();
+    }
+};
 
 Tensor linear(Tensor x, const py::tuple& w, bool glu) {
     const Operand b = operand(w, 2);
@@ -129,8 +138,8 @@ Tensor linear(Tensor x, const py::tuple& w, bool glu) {
         const int64_t row = as_rows(x);
         const int M = narrow(x.size(0)), dt = dtype_code(x);
         const size_t n = lq_fp4_linear_workspace(M, b.K, dt);
-        Tensor ws = workspace(n, x);
-        run("lq_fp4_linear", lq_fp4_linear(x.data_ptr(), row, b.codes, b.tiles, M, b.rows, b.K, glu, dt, y.data_ptr(), ws.data_ptr(), n, stream()));
+        const Workspace ws(n, x);
+        run("lq_fp4_linear", lq_fp4_linear(x.data_ptr(), row, b.codes, b.tiles, M, b.rows, b.K, glu, dt, y.data_ptr(), ws.p, n, stream()));
     }
     return y;
 }
@@ -155,10 +164,10 @@ Tensor grouped(const Tensor& xs, const Tensor& order, const Tensor& starts, cons
     if (out.numel() && xs.size(0)) {
         const int dt = dtype_code(xs);
         const size_t bytes = lq_fp4_experts_workspace(narrow(P), narrow(max_rows), b.stack, b.K, dt);
-        Tensor ws = workspace(bytes, xs);
+        const Workspace ws(bytes, xs);
         run("lq_fp4_experts", lq_fp4_experts(xs.data_ptr(), narrow(xs.size(0)), gather_k ? o : nullptr, narrow(gather_k), s, e, n,
                                              narrow(P), narrow(max_rows), glu, b.codes, b.tiles, out.data_ptr(), b.stack, b.rows, b.K,
-                                             dt, ws.data_ptr(), bytes, stream()));
+                                             dt, ws.p, bytes, stream()));
     }
     return out;
 }
@@ -197,11 +206,12 @@ Tensor experts(Tensor x, Tensor inds, Tensor weights, const py::tuple& gate_up, 
         need(P <= 1024, "at most 1024 experts a token");
     }
     const size_t n1 = lq_fp4_experts_workspace(P, T, E, D, dt), n2 = lq_fp4_experts_workspace(P, T, E, I, dt), n = std::max(n1, n2);
-    Tensor ws = workspace(n, x), h = at::empty({P, I}, x.options()), ys = at::empty({P, D}, x.options());
+    const Workspace ws(n, x);
+    Tensor h = at::empty({P, I}, x.options()), ys = at::empty({P, D}, x.options());
     run("lq_fp4_experts", lq_fp4_experts(x.data_ptr(), narrow(x.size(0)), order, k, starts, ex, nseg, P, T, 1, g.codes, g.tiles,
-                                         h.data_ptr(), E, g.rows, D, dt, ws.data_ptr(), n, st));
+                                         h.data_ptr(), E, g.rows, D, dt, ws.p, n, st));
     run("lq_fp4_experts", lq_fp4_experts(h.data_ptr(), P, nullptr, 0, starts, ex, nseg, P, T, 0, d.codes, d.tiles, ys.data_ptr(), E, D, I, dt,
-                                         ws.data_ptr(), n, st));
+                                         ws.p, n, st));
     run("lq_moe_combine", lq_moe_combine(ys.data_ptr(), weights.data_ptr<float>(), pos, y.data_ptr(), T, k, D, dt, st));
     return y;
 }

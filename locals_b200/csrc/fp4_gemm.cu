@@ -36,7 +36,10 @@ template <int KIND_, int P_, int T_, int CG_ = 1>
 struct Fp4Shape {
     static constexpr int KIND = KIND_, P = P_, T = T_;
     static constexpr int CG = CG_;  // CTAs a tile: a pair has 128 rows of w and half of the tokens each
-    static constexpr bool STACK = KIND == FP4_SPLIT && T <= 32;  // a token's pieces as columns of one MMA
+    // Few tokens of 16 bits: four warps make the pieces in shared memory, with no kernel before this one, and a token's pieces
+    // are columns of one MMA.
+    static constexpr bool STACK = KIND == FP4_SPLIT && T <= 32;
+    static constexpr int OUT = STACK ? 4 : FP4_OUT;  // warps that write out
     static constexpr int BK = KIND == FP4_SPLIT ? 128 : 256;     // values a stage
     static constexpr int KB = KIND == FP4_MX ? 2 : KIND == FP4_NV ? 4 : 1;  // scale tiles a stage and 128 rows
     static constexpr int NB = STACK ? 1 : P * ((T + 127) / 128);            // scale tiles of x beside each of w's
@@ -44,7 +47,7 @@ struct Fp4Shape {
     // what TMA counts of a weight tile: the bytes that it reads, also where it spreads codes to bytes
     static constexpr int A_TX = KIND == FP4_SPLIT ? A_BYTES / 2 : A_BYTES;
     static constexpr int SFA = KB * 512, SFB = KB * NB * 512;
-    static constexpr int TX = A_TX + B_BYTES + SFA + SFB;  // bytes that arrive for a stage (in each CTA)
+    static constexpr int TX = A_TX + SFA + (STACK ? 0 : B_BYTES + SFB);  // bytes that arrive for a stage (in each CTA)
     static constexpr int STAGE = (A_BYTES + B_BYTES + SFA + SFB + 1023) / 1024 * 1024;
     // stages of the ring: one CTA an SM, or (narrow tiles, more of them than SMs) two
     static constexpr int ring(int kb) { return kb * 1024 / STAGE < FP4_MAX_STAGES ? kb * 1024 / STAGE : FP4_MAX_STAGES; }
@@ -71,6 +74,11 @@ struct Fp4Args {
     const float* xf;     // factors, or NULL
     const float* wf;
     void* y;
+    // x in 16 bits (few tokens)
+    const void* x16;
+    int64_t x_row;
+    int K, vec, gather, src_rows;  // vec: rows start on 16-byte boundaries
+    const int32_t* order;          // gather > 0: row j is row order[j] / gather of x (order NULL: j / gather); 0: row j
     // grouped
     int grouped, E;
     const int32_t* starts;
@@ -219,6 +227,62 @@ __device__ __forceinline__ void fp4_out4(const Fp4Args& a, const Fp4Tile& t, int
         if (i < some && at + i < width) fp4_store(a, first + i, o[i]);
 }
 
+// Values [k0, k0 + 8) of a row of K 16-bit values, zeros beyond it; `vec`: the row starts on a 16-byte boundary.
+template <typename T16>
+__device__ __forceinline__ uint4 load8_16(const T16* row, int k0, int K, bool vec) {
+    if (vec && k0 + 8 <= K) return *reinterpret_cast<const uint4*>(row + k0);
+    uint32_t w[4] = {};
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+        if (k0 + i < K) w[i >> 1] |= uint32_t(reinterpret_cast<const uint16_t*>(row)[k0 + i]) << (16 * (i & 1));
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// 8 values of a group of 32 (four lanes next to one another) to P pieces of e4m3 bytes and their scale bytes.
+template <typename T16, int P>
+__device__ __forceinline__ void split8(const uint4& x, uint32_t mask, uint2 (&piece)[P], int (&byte)[P]) {
+    const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+    float v[8], top = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        v[i] = F16Traits<T16>::to_f32(w[i >> 1] >> (16 * (i & 1)) & 0xFFFFu);
+        asm("max.NaN.f32 %0, %1, %2;" : "=f"(top) : "f"(top), "f"(fabsf(v[i])));
+    }
+#pragma unroll
+    for (int d = 1; d < 4; d *= 2) {
+        const float o = __shfl_xor_sync(mask, top, d);
+        asm("max.NaN.f32 %0, %1, %2;" : "=f"(top) : "f"(top), "f"(o));
+    }
+    const uint32_t e = __float_as_uint(top) >> 23 & 0xFF;
+    byte[0] = e == 255 ? 255 : e < 7 ? 0 : int(e) - 7;
+    const float up = __uint_as_float((254u - (e == 255 ? 127u : uint32_t(byte[0]))) << 23);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] *= up;
+#pragma unroll
+    for (int p = 0; p < P; ++p) {
+        uint32_t q[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const uint32_t lo = cvt_e4m3x2(v[4 * h + 1], v[4 * h]), hi = cvt_e4m3x2(v[4 * h + 3], v[4 * h + 2]);
+            q[h] = lo | hi << 16;
+            if (p + 1 < P) {
+                const float2 x01 = e4m3x2_to_f32(lo), x23 = e4m3x2_to_f32(hi);
+                v[4 * h] -= x01.x;
+                v[4 * h + 1] -= x01.y;
+                v[4 * h + 2] -= x23.x;
+                v[4 * h + 3] -= x23.y;
+            }
+        }
+        piece[p] = make_uint2(q[0], q[1]);
+        if (p + 1 < P) {
+            byte[p + 1] = byte[p] == 255 ? 255 : byte[p] < 5 ? 0 : byte[p] - 5;
+            const float more = __uint_as_float(uint32_t(127 + (byte[p] == 255 ? 0 : byte[p] - byte[p + 1])) << 23);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] *= more;
+        }
+    }
+}
+
 // The tensor maps of a product: codes of w and x (or pieces of x), scale tiles of w and x.
 struct Fp4Maps {
     CUtensorMap w, x, ws, xs;
@@ -246,12 +310,12 @@ __global__ void __launch_bounds__(FP4_THREADS, S::T <= 32 ? 2 : 1) fp4_gemm_kern
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < NS; ++s) {
-            mbar_init(&full[s], 1);
+            mbar_init(&full[s], S::STACK ? 2 : 1);
             mbar_init(&empty[s], 1);
         }
         for (int j = 0; j < 2; ++j) {
             mbar_init(&acc_full[j], 1);
-            mbar_init(&acc_empty[j], FP4_OUT * CG);
+            mbar_init(&acc_empty[j], S::OUT * CG);
         }
         fence_barrier_init();
     }
@@ -283,7 +347,7 @@ __global__ void __launch_bounds__(FP4_THREADS, S::T <= 32 ? 2 : 1) fp4_gemm_kern
         const bool scales = warp == FP4_OUT + 2;
         if (elect_one()) {
             prefetch_tmap(scales ? &m.ws : &m.w);
-            prefetch_tmap(scales ? &m.xs : &m.x);
+            if constexpr (!S::STACK) prefetch_tmap(scales ? &m.xs : &m.x);
             const uint64_t pol_w = policy_evict_first(), pol_x = policy_evict_last();
             const uint32_t ring = smem_u32(smem), bars = CG == 2 ? map_peer(smem_u32(full), 0) : smem_u32(full);
             int it = 0, s = 0, turn = 0;  // stages so far, the ring's next slot, rounds of the ring
@@ -304,11 +368,11 @@ __global__ void __launch_bounds__(FP4_THREADS, S::T <= 32 ? 2 : 1) fp4_gemm_kern
                         load_3d<CG>(st + S::A_BYTES + S::B_BYTES, &m.ws, bar, 0, kb * S::KB, wtile, pol_w);
                 };
                 // Before this kernel came the split, which was launched on when the kernels before it were done: what they
-                // wrote, weights too, may be read before the split ends. A product of two 4-bit operands may follow the
-                // kernel that quantized its weights.
+                // wrote, weights too, may be read before the split ends. Without one, this may follow the kernel that
+                // quantized the weights.
                 int ahead = 0;
                 if (!waited) {
-                    for (; S::KIND == FP4_SPLIT && ahead < NS && s_lo + ahead < s_hi; ++ahead) {
+                    for (; S::KIND == FP4_SPLIT && !S::STACK && ahead < NS && s_lo + ahead < s_hi; ++ahead) {
                         expect(ahead);
                         weights(s_lo + ahead, ahead);
                     }
@@ -326,7 +390,8 @@ __global__ void __launch_bounds__(FP4_THREADS, S::T <= 32 ? 2 : 1) fp4_gemm_kern
                         weights(kb, s);
                     }
                     const uint32_t st = ring + s * S::STAGE + S::A_BYTES, bar = bars + s * 8;
-                    if (!scales) {
+                    if constexpr (S::STACK) {
+                    } else if (!scales) {
 #pragma unroll
                         for (int p = 0; p < P; ++p)
                             load_2d<CG>(st + p * S::B_TILE, &m.x, bar, kb * 128, p * a.piece_rows + t.r0 + half * (T / CG), pol_x);
@@ -409,8 +474,70 @@ __global__ void __launch_bounds__(FP4_THREADS, S::T <= 32 ? 2 : 1) fp4_gemm_kern
             __syncwarp();
             ++j;
         }
+    } else if (warp >= S::OUT) {
+        // ------------------------------ converters: 16-bit x to pieces ------------------------------
+        // The warps take stages in turn, so that the loads of four stages are on their way; a lane takes 8 values of a token.
+        // No more warps than the ring has stages: one that is `turns` stages on has then seen, at its last stage, the place of
+        // the stage two rounds back handed over, and the parity that it waits for is not the one of two rounds before.
+        if constexpr (S::STACK) {
+            using T16 = typename std::conditional<P == 2, __nv_bfloat16, __half>::type;
+            constexpr int AHEAD = 4;  // loads of a lane before it converts
+            grid_dep_wait();
+            const int turns = NS < 4 ? NS : 4, mine = warp - S::OUT, chunk = lane & 15;
+            int who = 0, s = 0, turn = 0;  // the warp of the next stage, its place, rounds of the ring
+            Fp4Tile t;
+            for (int lin = first; lin < ntiles && ok; lin += step) {
+                if (!fp4_tile<S>(a, starts, nseg, lin, t)) continue;
+                int src = t.r0 + lane < t.r1 ? t.r0 + lane : -1;  // the row of x of the tile's token `lane`
+                if (a.gather && src >= 0) src = (a.order ? a.order[src] : src) / a.gather;
+                if (src >= a.src_rows || (src < 0 && t.r0 + lane < t.r1)) {
+                    record_status(LQ_DEV_BOUNDS);
+                    src = -1;  // zeros
+                }
+                const int tasks = (t.r1 - t.r0 + 1) / 2;  // of two tokens
+                for (int kb = s_lo; kb < s_hi; ++kb, ++who, ++s) {
+                    if (s == NS) {
+                        s = 0;
+                        ++turn;
+                    }
+                    if (who == turns) who = 0;
+                    if (who != mine) continue;
+                    bool free = turn == 0;
+                    uint8_t* b = smem + s * S::STAGE + S::A_BYTES;
+                    for (int i0 = 0; i0 < tasks; i0 += AHEAD) {
+                        uint4 v[AHEAD];
+#pragma unroll
+                        for (int i = 0; i < AHEAD; ++i) {
+                            const int row = __shfl_sync(0xFFFFFFFFu, src, (2 * (i0 + i) + (lane >> 4)) & 31);
+                            v[i] = make_uint4(0, 0, 0, 0);
+                            if (i0 + i < tasks && row >= 0)
+                                v[i] = load8_16(static_cast<const T16*>(a.x16) + int64_t(row) * a.x_row, kb * 128 + chunk * 8, a.K, a.vec);
+                        }
+                        if (!free && !(ok = mbar_wait(&empty[s], (turn - 1) & 1))) break;
+                        free = true;
+#pragma unroll
+                        for (int i = 0; i < AHEAD; ++i) {
+                            if (i0 + i >= tasks) break;
+                            uint2 piece[P];
+                            int byte[P];
+                            split8<T16, P>(v[i], 0xFFFFFFFFu, piece, byte);
+#pragma unroll
+                            for (int p = 0; p < P; ++p) {
+                                const int r = p * T + 2 * (i0 + i) + (lane >> 4);  // 128-byte rows, their 16-byte pieces swizzled
+                                *reinterpret_cast<uint2*>(b + r * 128 + (((chunk >> 1) ^ (r & 7)) << 4) + (chunk & 1) * 8) = piece[p];
+                                if (chunk % 4 == 0) b[S::B_BYTES + S::SFA + fp4_tile_byte(r, chunk / 4)] = uint8_t(byte[p]);
+                            }
+                        }
+                    }
+                    if (!ok) break;
+                    fence_proxy_async();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&full[s]);
+                }
+            }
+        }
     } else {
-        // ------------------------------ epilogue: two warps a quarter of the lanes ------------------------------
+        // ------------------------------ epilogue: two warps (few 16-bit tokens: one) a quarter of the lanes ------------------------------
         grid_dep_wait();
         const float f = (a.xf ? *a.xf : 1.f) * (a.wf ? *a.wf : 1.f);
         // 16-byte pieces of y: its rows start on 16-byte boundaries
@@ -427,7 +554,7 @@ __global__ void __launch_bounds__(FP4_THREADS, S::T <= 32 ? 2 : 1) fp4_gemm_kern
             }
         };
         constexpr int COLS = T <= 32 ? 16 : T <= 64 ? 32 : 64;  // of a warp at a time
-        constexpr int ROUNDS = (T + 2 * COLS - 1) / (2 * COLS);
+        constexpr int SIDES = S::OUT / 4, ROUNDS = (T + SIDES * COLS - 1) / (SIDES * COLS);
         const int quarter = warp & 3, side = warp >> 2;
         int j = 0;
         Fp4Tile t;
@@ -443,7 +570,7 @@ __global__ void __launch_bounds__(FP4_THREADS, S::T <= 32 ? 2 : 1) fp4_gemm_kern
             for (int i = 0; i < ROUNDS; ++i) {
                 // The columns that the next tile's accumulator covers come first, and all of them to registers: the next tile's
                 // MMAs wait for that, not for the stores.
-                const int c0 = (S::ACC == 256 ? 128 * ((i + (j & 1) + 1) & 1) : 2 * COLS * i) + COLS * side;
+                const int c0 = (S::ACC == 256 ? 128 * ((i + (j & 1) + 1) & 1) : SIDES * COLS * i) + COLS * side;
                 if (c0 >= T) break;
                 float v[COLS];
                 uint32_t r[16];
@@ -478,7 +605,7 @@ __global__ void __launch_bounds__(FP4_THREADS, S::T <= 32 ? 2 : 1) fp4_gemm_kern
                     }
                 }
             }
-            if (S::ACC != 256 && ROUNDS == 1 && COLS * side >= T) acc_free(j & 1);  // (16 tokens: one warp a quarter reads)
+            if (S::ACC != 256 && COLS * side >= T) acc_free(j & 1);  // (16 tokens: one warp a quarter reads)
             ++j;
         }
     }
@@ -527,7 +654,7 @@ __global__ void __launch_bounds__(FP4_THREADS, S::T <= 32 ? 2 : 1) fp4_gemm_kern
 struct SplitArgs {
     const void* x;
     int64_t x_row;
-    int rows, K, ktiles, nb, stack, T;
+    int rows, K, ktiles, nb, T;
     bool vec;
     uint8_t* pieces;  // (P, rows, Kp)
     uint8_t* tiles;   // (token tile, K tile, nb, 512)
@@ -537,20 +664,6 @@ struct SplitArgs {
     const int32_t* starts;
     const int32_t* nseg;
 };
-
-template <typename T16>
-__device__ __forceinline__ void split_load8(const T16* row, int k0, int K, bool vec, float (&v)[8]) {
-    if (vec && k0 + 8 <= K) {
-        const uint4 q = *reinterpret_cast<const uint4*>(row + k0);
-        const uint32_t w[4] = {q.x, q.y, q.z, q.w};
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = F16Traits<T16>::to_f32(w[i >> 1] >> (16 * (i & 1)) & 0xFFFFu);
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-            v[i] = k0 + i < K ? F16Traits<T16>::to_f32(reinterpret_cast<const uint16_t*>(row)[k0 + i]) : 0.f;
-    }
-}
 
 // A thread takes 8 values, four threads a group of 32.
 template <typename T16, int P>
@@ -567,18 +680,8 @@ __global__ void __launch_bounds__(256) fp4_split_kernel(const SplitArgs a) {
             src = (a.order ? a.order[row] : row) / a.gather;
             if (src < 0 || src >= a.src_rows) {
                 record_status(LQ_DEV_BOUNDS);
-                src = 0;
+                src = -1;  // zeros
             }
-        }
-        float v[8];
-        split_load8(static_cast<const T16*>(a.x) + src * a.x_row, 8 * word, a.K, a.vec, v);
-        float top = 0.f;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) asm("max.NaN.f32 %0, %1, %2;" : "=f"(top) : "f"(top), "f"(fabsf(v[i])));
-#pragma unroll
-        for (int d = 1; d < 4; d *= 2) {
-            const float o = __shfl_xor_sync(mask, top, d);
-            asm("max.NaN.f32 %0, %1, %2;" : "=f"(top) : "f"(top), "f"(o));
         }
         int tile = row / a.T, at = row % a.T;
         if (a.grouped) {
@@ -591,36 +694,16 @@ __global__ void __launch_bounds__(256) fp4_split_kernel(const SplitArgs a) {
             tile = s0 / a.T + lo + (row - s0) / a.T;
             at = (row - s0) % a.T;
         }
-        const uint32_t e = __float_as_uint(top) >> 23 & 0xFF;
-        int byte = e == 255 ? 255 : e < 7 ? 0 : int(e) - 7;
-        const float up = __uint_as_float((254u - (e == 255 ? 127u : uint32_t(byte))) << 23);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] *= up;
+        uint2 piece[P];
+        int byte[P];
+        split8<T16, P>(src < 0 ? make_uint4(0, 0, 0, 0) : load8_16(static_cast<const T16*>(a.x) + src * a.x_row, 8 * word, a.K, a.vec),
+                       mask, piece, byte);
         const int g = word / 4;
         uint8_t* tl = a.tiles + (int64_t(tile) * a.ktiles + (g >> 2)) * a.nb * 512;
 #pragma unroll
         for (int p = 0; p < P; ++p) {
-            uint32_t w[2];
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const uint32_t lo = cvt_e4m3x2(v[4 * h + 1], v[4 * h]), hi = cvt_e4m3x2(v[4 * h + 3], v[4 * h + 2]);
-                w[h] = lo | hi << 16;
-                const float2 x01 = e4m3x2_to_f32(lo), x23 = e4m3x2_to_f32(hi);
-                v[4 * h] -= x01.x;
-                v[4 * h + 1] -= x01.y;
-                v[4 * h + 2] -= x23.x;
-                v[4 * h + 3] -= x23.y;
-            }
-            *reinterpret_cast<uint2*>(a.pieces + (int64_t(p) * a.rows + row) * (words * 8) + 8 * word) = make_uint2(w[0], w[1]);
-            if (word % 4 == 0) {
-                const int q = a.stack ? p * a.T + at : at;
-                tl[(a.stack ? 0 : p * ((a.T + 127) / 128) + q / 128) * 512 + fp4_tile_byte(q % 128, g)] = uint8_t(byte);
-            }
-            const int next = byte == 255 ? 255 : byte < 5 ? 0 : byte - 5;
-            const float more = __uint_as_float(uint32_t(127 + (byte == 255 ? 0 : byte - next)) << 23);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] *= more;
-            byte = next;
+            *reinterpret_cast<uint2*>(a.pieces + (int64_t(p) * a.rows + row) * (words * 8) + 8 * word) = piece[p];
+            if (word % 4 == 0) tl[(p * ((a.T + 127) / 128) + at / 128) * 512 + fp4_tile_byte(at % 128, g)] = uint8_t(byte[p]);
         }
     }
 }
@@ -703,11 +786,11 @@ static int gemm_t(const Fp4Call& c, cudaStream_t st) {
     Fp4Args a = c.a;
     a.ns = (a.Kp + S::BK - 1) / S::BK;
     a.rtiles = (a.N + 127) / 128;
-    Fp4Maps m;
+    Fp4Maps m = {};
     int rc = map_rows(&m.w, c.w, S::KIND == FP4_SPLIT, uint64_t(a.Kp) / 2, uint64_t(c.stack) * a.N, 128);
-    if (!rc) rc = map_rows(&m.x, c.x, false, uint64_t(a.Kp) / (S::KIND == FP4_SPLIT ? 1 : 2), uint64_t(S::P) * a.M, S::T / S::CG);
+    if (!rc && !S::STACK) rc = map_rows(&m.x, c.x, false, uint64_t(a.Kp) / (S::KIND == FP4_SPLIT ? 1 : 2), uint64_t(S::P) * a.M, S::T / S::CG);
     if (!rc) rc = map_scales(&m.ws, c.wt, a.ktiles, uint64_t(c.stack) * a.rtiles, S::KB, 1);
-    if (!rc) rc = S::KIND == FP4_SPLIT ? map_scales(&m.xs, c.xt, S::NB, uint64_t(c.ttiles) * a.ktiles, S::NB, 1)
+    if (!rc && !S::STACK) rc = S::KIND == FP4_SPLIT ? map_scales(&m.xs, c.xt, S::NB, uint64_t(c.ttiles) * a.ktiles, S::NB, 1)
                                        : map_scales(&m.xs, c.xt, a.ktiles, (uint64_t(a.M) + 127) / 128, S::KB, S::NB);
     if (rc) return rc;
     const int sms = device_info().sm_count;
@@ -775,7 +858,7 @@ int fp4_qmm_run(const uint32_t* xc, const uint8_t* xt, const float* xf, const ui
 
 // Token tiles of the rows of a call (grouped: one number a segment may go unused), and the bytes of the split's results.
 static int64_t split_tiles(int rows, int T, int segments) { return segments ? rows / T + segments : (rows + T - 1) / T; }
-static int split_blocks(int P, int T) { return T <= 32 ? 1 : P * ((T + 127) / 128); }
+static int split_blocks(int P, int T) { return P * ((T + 127) / 128); }
 static size_t split_pieces_bytes(int rows, int K, int P) { return (size_t(P) * rows * fp4_padded(K) + 511) / 512 * 512; }
 
 // Tokens a tile of rows that are dealt out to segments: twice the average, so that most segments are one tile.
@@ -786,6 +869,7 @@ static int grouped_tokens(int rows, int segments, int max_rows) {
 
 size_t fp4_linear_workspace_bytes(int rows, int K, int dtype, int segments, int max_rows) {
     const int P = dtype == LQ_BF16 ? 2 : 3, T = segments ? grouped_tokens(rows, segments, max_rows) : tile_tokens(rows);
+    if (T <= 32) return 0;  // the product makes the pieces
     return split_pieces_bytes(rows, K, P) +
            size_t(split_tiles(rows, T, segments)) * fp4_ktiles(K, LQ_MXFP4) * split_blocks(P, T) * 512;
 }
@@ -795,31 +879,33 @@ int fp4_linear_run(const Fp4Linear& l, cudaStream_t st) {
     const int T = l.segments ? grouped_tokens(l.rows, l.segments, l.max_rows) : tile_tokens(l.rows);
     uint8_t* ws = static_cast<uint8_t*>(l.ws);
     SplitArgs s = {};
-    s.x = l.x;
-    s.x_row = l.x_row;
-    s.rows = l.rows;
-    s.K = l.K;
     s.ktiles = fp4_ktiles(l.K, LQ_MXFP4);
-    s.nb = split_blocks(P, T);
-    s.stack = T <= 32;
-    s.T = T;
-    s.vec = aligned(l.x, 16) && l.x_row % 8 == 0;
-    s.pieces = ws;
-    s.tiles = ws + split_pieces_bytes(l.rows, l.K, P);
-    s.order = l.order;
-    s.gather = l.gather;
-    s.src_rows = l.src_rows;
-    s.grouped = l.segments > 0;
-    s.max_seg = l.segments;
-    s.starts = l.starts;
-    s.nseg = l.nseg;
-    const int64_t units = int64_t(l.rows) * (fp4_padded(l.K) / 8);
-    const int64_t most = int64_t(device_info().sm_count) * 16, blocks = (units + 255) / 256;
-    const void* split = l.dtype == LQ_BF16 ? reinterpret_cast<const void*>(fp4_split_kernel<__nv_bfloat16, 2>)
-                                           : reinterpret_cast<const void*>(fp4_split_kernel<__half, 3>);
-    void* sargs[] = {&s};
-    int rc = launch(split, int(blocks < most ? blocks : most), 256, 0, 1, st, sargs);
-    if (rc) return rc;
+    const bool vec = aligned(l.x, 16) && l.x_row % 8 == 0;
+    if (T > 32) {
+        s.x = l.x;
+        s.x_row = l.x_row;
+        s.rows = l.rows;
+        s.K = l.K;
+        s.nb = split_blocks(P, T);
+        s.T = T;
+        s.vec = vec;
+        s.pieces = ws;
+        s.tiles = ws + split_pieces_bytes(l.rows, l.K, P);
+        s.order = l.order;
+        s.gather = l.gather;
+        s.src_rows = l.src_rows;
+        s.grouped = l.segments > 0;
+        s.max_seg = l.segments;
+        s.starts = l.starts;
+        s.nseg = l.nseg;
+        const int64_t units = int64_t(l.rows) * (fp4_padded(l.K) / 8);
+        const int64_t most = int64_t(device_info().sm_count) * 16, blocks = (units + 255) / 256;
+        const void* split = l.dtype == LQ_BF16 ? reinterpret_cast<const void*>(fp4_split_kernel<__nv_bfloat16, 2>)
+                                               : reinterpret_cast<const void*>(fp4_split_kernel<__half, 3>);
+        void* sargs[] = {&s};
+        const int rc = launch(split, int(blocks < most ? blocks : most), 256, 0, 1, st, sargs);
+        if (rc) return rc;
+    }
     Fp4Call c = {};
     c.x = s.pieces;
     c.w = l.wc;
@@ -833,6 +919,13 @@ int fp4_linear_run(const Fp4Linear& l, cudaStream_t st) {
     a.glu = l.glu;
     a.dtype = l.dtype;
     a.piece_rows = l.rows;
+    a.x16 = l.x;
+    a.x_row = l.x_row;
+    a.K = l.K;
+    a.vec = vec;
+    a.order = l.order;
+    a.gather = l.gather;
+    a.src_rows = l.src_rows;
     c.wt = l.wt;
     c.xt = s.tiles;
     a.y = l.y;
