@@ -515,17 +515,27 @@ __global__ void __launch_bounds__(FP4_THREADS, S::T <= 32 ? 2 : 1) fp4_gemm_kern
                         }
                         if (!free && !(ok = mbar_wait(&empty[s], (turn - 1) & 1))) break;
                         free = true;
-#pragma unroll
-                        for (int i = 0; i < AHEAD; ++i) {
-                            if (i0 + i >= tasks) break;
-                            uint2 piece[P];
-                            int byte[P];
-                            split8<T16, P>(v[i], 0xFFFFFFFFu, piece, byte);
+                        auto put = [&](int i, const uint2(&piece)[P], const int(&byte)[P]) {
 #pragma unroll
                             for (int p = 0; p < P; ++p) {
-                                const int r = p * T + 2 * (i0 + i) + (lane >> 4);  // 128-byte rows, their 16-byte pieces swizzled
+                                const int r = p * T + 2 * i + (lane >> 4);  // 128-byte rows, their 16-byte pieces swizzled
                                 *reinterpret_cast<uint2*>(b + r * 128 + (((chunk >> 1) ^ (r & 7)) << 4) + (chunk & 1) * 8) = piece[p];
                                 if (chunk % 4 == 0) b[S::B_BYTES + S::SFA + fp4_tile_byte(r, chunk / 4)] = uint8_t(byte[p]);
+                            }
+                        };
+                        // two at a time where there are two: one is a chain of conversions (some 550 cycles)
+#pragma unroll
+                        for (int i = 0; i < AHEAD; i += 2) {
+                            uint2 p0[P], p1[P];
+                            int b0[P], b1[P];
+                            if (i0 + i + 1 < tasks) {
+                                split8<T16, P>(v[i], 0xFFFFFFFFu, p0, b0);
+                                split8<T16, P>(v[i + 1], 0xFFFFFFFFu, p1, b1);
+                                put(i0 + i, p0, b0);
+                                put(i0 + i + 1, p1, b1);
+                            } else if (i0 + i < tasks) {
+                                split8<T16, P>(v[i], 0xFFFFFFFFu, p0, b0);
+                                put(i0 + i, p0, b0);
                             }
                         }
                     }
@@ -665,23 +675,30 @@ struct SplitArgs {
     const int32_t* nseg;
 };
 
-// A thread takes 8 values, four threads a group of 32.
+// A warp takes 1,024 values of a row: the row's place is found once, four loads a lane are on their way together. (With a
+// thread a group and its place searched at each, 16,004 gathered rows of 2,048 took 70 us.)
 template <typename T16, int P>
 __global__ void __launch_bounds__(256) fp4_split_kernel(const SplitArgs a) {
     grid_dep_wait();
     grid_dep_launch();  // after the wait: the product reads weights ahead of this kernel's end
-    const int words = fp4_padded(a.K) / 8;
-    const int64_t n = int64_t(a.rows) * words;
-    for (int64_t u = int64_t(blockIdx.x) * blockDim.x + threadIdx.x; u < n; u += int64_t(gridDim.x) * blockDim.x) {
-        const int row = int(u / words), word = int(u - int64_t(row) * words);
-        const uint32_t mask = 0xFFFFu << (threadIdx.x & 16);
+    const int lane = threadIdx.x & 31, words = fp4_padded(a.K) / 8, parts = (words + 127) / 128;
+    const int64_t tasks = int64_t(a.rows) * parts;
+    for (int64_t u = (int64_t(blockIdx.x) * blockDim.x + threadIdx.x) >> 5; u < tasks; u += (int64_t(gridDim.x) * blockDim.x) >> 5) {
+        const int row = int(u / parts), part = int(u - int64_t(row) * parts);
         int64_t src = row;
         if (a.gather) {
             src = (a.order ? a.order[row] : row) / a.gather;
             if (src < 0 || src >= a.src_rows) {
-                record_status(LQ_DEV_BOUNDS);
+                if (lane == 0) record_status(LQ_DEV_BOUNDS);
                 src = -1;  // zeros
             }
+        }
+        uint4 v[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int word = part * 128 + 32 * i + lane;
+            v[i] = make_uint4(0, 0, 0, 0);
+            if (src >= 0 && word < words) v[i] = load8_16(static_cast<const T16*>(a.x) + src * a.x_row, 8 * word, a.K, a.vec);
         }
         int tile = row / a.T, at = row % a.T;
         if (a.grouped) {
@@ -694,16 +711,23 @@ __global__ void __launch_bounds__(256) fp4_split_kernel(const SplitArgs a) {
             tile = s0 / a.T + lo + (row - s0) / a.T;
             at = (row - s0) % a.T;
         }
-        uint2 piece[P];
-        int byte[P];
-        split8<T16, P>(src < 0 ? make_uint4(0, 0, 0, 0) : load8_16(static_cast<const T16*>(a.x) + src * a.x_row, 8 * word, a.K, a.vec),
-                       mask, piece, byte);
-        const int g = word / 4;
-        uint8_t* tl = a.tiles + (int64_t(tile) * a.ktiles + (g >> 2)) * a.nb * 512;
+        uint8_t* tiles = a.tiles + int64_t(tile) * a.ktiles * a.nb * 512;
 #pragma unroll
-        for (int p = 0; p < P; ++p) {
-            *reinterpret_cast<uint2*>(a.pieces + (int64_t(p) * a.rows + row) * (words * 8) + 8 * word) = piece[p];
-            if (word % 4 == 0) tl[(p * ((a.T + 127) / 128) + at / 128) * 512 + fp4_tile_byte(at % 128, g)] = uint8_t(byte[p]);
+        for (int i = 0; i < 4; ++i) {
+            const int word = part * 128 + 32 * i + lane;
+            if (part * 128 + 32 * i >= words) break;  // (rows are a multiple of 16 words: half a warp may be beyond)
+            uint2 piece[P];
+            int byte[P];
+            split8<T16, P>(v[i], 0xFFFFFFFFu, piece, byte);
+            if (word < words) {
+                const int g = word / 4;
+                uint8_t* tl = tiles + int64_t(g >> 2) * a.nb * 512;
+#pragma unroll
+                for (int p = 0; p < P; ++p) {
+                    *reinterpret_cast<uint2*>(a.pieces + (int64_t(p) * a.rows + row) * (words * 8) + 8 * word) = piece[p];
+                    if (word % 4 == 0) tl[(p * ((a.T + 127) / 128) + at / 128) * 512 + fp4_tile_byte(at % 128, g)] = uint8_t(byte[p]);
+                }
+            }
         }
     }
 }
@@ -753,7 +777,8 @@ static int map_scales(CUtensorMap* m, const void* base, uint64_t inner, uint64_t
 }
 
 // Clusters of ks CTAs that the current device runs at once: its SMs come in groups that a cluster does not leave, so that 48
-// clusters of three need not fit 148 SMs. Asked once a device, kernel and size.
+// clusters of three need not fit 148 SMs. Asked once a device, kernel and size. (Of a kernel that allocates tensor memory the
+// runtime counts one CTA an SM, whatever it allocates; narrow tiles run two, as their start times show.)
 template <typename S>
 static int max_clusters(int ks, size_t smem) {
     static std::atomic<int> known[16][2][9];
@@ -803,13 +828,15 @@ static int gemm_t(const Fp4Call& c, cudaStream_t st) {
     static_assert(S::NS_TWO >= 2 || S::T > 32, "two CTAs an SM");
     static_assert(S::ACC == 256 || S::T * 512 <= (S::T <= 32 ? S::NS_TWO : S::NS) * S::STAGE, "the partial sums of a split fit the ring");
     auto kern = fp4_gemm_kernel<S>;
-    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem)) != cudaSuccess) return LQ_E_CUDA;
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem)) != cudaSuccess ||
+        cudaFuncSetAttribute(kern, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared) != cudaSuccess)
+        return LQ_E_CUDA;
     // Few tiles: a tile's K split over as many CTAs of a cluster as still run all at once, each with a stage at least.
     a.ks = 1;
     if (S::CG == 1) {
         const int most = a.ns < 8 ? a.ns : 8;
         for (int ks = most; ks > 1 && a.ks == 1; --ks)
-            if (tiles * ks <= int64_t(sms) * (S::T <= 32 ? 2 : 1) && tiles <= max_clusters<S>(ks, smem)) a.ks = ks;
+            if (tiles * ks <= int64_t(sms) * (S::T <= 32 ? 2 : 1) && tiles <= max_clusters<S>(ks, smem) * (S::T <= 32 ? 2 : 1)) a.ks = ks;
     }
     const int64_t slots = int64_t(sms) * (S::T <= 32 ? 2 : 1);
     const int64_t grid = S::CG == 2 ? (tiles < sms / 2 ? tiles : sms / 2) * 2 : a.ks > 1 ? tiles * a.ks : tiles < slots ? tiles : slots;
@@ -823,14 +850,19 @@ static int gemm_tokens(const Fp4Call& c, int T, cudaStream_t st) {
         case 16: return gemm_t<Fp4Shape<KIND, P, 16>>(c, st);
         case 32: return gemm_t<Fp4Shape<KIND, P, 32>>(c, st);
         case 64: return gemm_t<Fp4Shape<KIND, P, 64>>(c, st);
-        case 128: return gemm_t<Fp4Shape<KIND, P, 128>>(c, st);
+        case 128:  // enough tiles for all SMs: pairs; else one CTA a tile, or several that split its K
+            if (c.ttiles * ((c.a.N + 255) / 256) * 2 >= device_info().sm_count) return gemm_t<Fp4Shape<KIND, P, 128, 2>>(c, st);
+            return gemm_t<Fp4Shape<KIND, P, 128>>(c, st);
         default: return gemm_t<Fp4Shape<KIND, P, 256, 2>>(c, st);
     }
 }
 
-// Tokens a tile. A product of both in 4 bits has scale tiles of 128 tokens, so narrower tiles only where one holds them all.
+// Tokens a tile. (A product of both in 4 bits has scale tiles of 128 tokens, so narrower tiles only where one holds them all.)
+// Beyond 128 tokens tiles of 256 read the weights half as often as tiles of 128, which in turn end closer to the last token.
 static int tile_tokens(int rows) {
-    return rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : rows <= 128 ? 128 : 256;
+    if (rows <= 128) return rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : 128;
+    const int64_t narrow = (int64_t(rows) + 127) / 128 * 128, wide = (int64_t(rows) + 255) / 256 * 256;
+    return wide * 8 <= narrow * 9 ? 256 : 128;
 }
 
 int fp4_qmm_run(const uint32_t* xc, const uint8_t* xt, const float* xf, const uint32_t* wc, const uint8_t* wt, const float* wf,
@@ -861,10 +893,13 @@ static int64_t split_tiles(int rows, int T, int segments) { return segments ? ro
 static int split_blocks(int P, int T) { return P * ((T + 127) / 128); }
 static size_t split_pieces_bytes(int rows, int K, int P) { return (size_t(P) * rows * fp4_padded(K) + 511) / 512 * 512; }
 
-// Tokens a tile of rows that are dealt out to segments: twice the average, so that most segments are one tile.
+// Tokens a tile of rows that are dealt out to segments: twice the average, so that most segments are one tile; long segments
+// have tiles of 128, whose last is half as wide (250 rows each: 143 -> 110 us for 4,001 tokens' gate and up), until
+// that is a small part of them.
 static int grouped_tokens(int rows, int segments, int max_rows) {
-    const int64_t want = 2 * int64_t(rows) / (segments > 0 ? segments : 1);
-    return tile_tokens(int(want < max_rows ? want : max_rows));
+    const int64_t average = int64_t(rows) / (segments > 0 ? segments : 1), want = 2 * average;
+    const int T = tile_tokens(int(want < max_rows ? want : max_rows));
+    return T > 128 && average < 1024 ? 128 : T;
 }
 
 size_t fp4_linear_workspace_bytes(int rows, int K, int dtype, int segments, int max_rows) {
@@ -898,8 +933,8 @@ int fp4_linear_run(const Fp4Linear& l, cudaStream_t st) {
         s.max_seg = l.segments;
         s.starts = l.starts;
         s.nseg = l.nseg;
-        const int64_t units = int64_t(l.rows) * (fp4_padded(l.K) / 8);
-        const int64_t most = int64_t(device_info().sm_count) * 16, blocks = (units + 255) / 256;
+        const int64_t units = int64_t(l.rows) * ((fp4_padded(l.K) + 1023) / 1024);  // of a warp
+        const int64_t most = int64_t(device_info().sm_count) * 8, blocks = (units + 7) / 8;
         const void* split = l.dtype == LQ_BF16 ? reinterpret_cast<const void*>(fp4_split_kernel<__nv_bfloat16, 2>)
                                                : reinterpret_cast<const void*>(fp4_split_kernel<__half, 3>);
         void* sargs[] = {&s};
