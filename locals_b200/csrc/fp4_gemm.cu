@@ -32,6 +32,12 @@ constexpr int FP4_THREADS = 32 * (FP4_OUT + 3);
 constexpr int FP4_MAX_STAGES = 10;
 constexpr int FP4_MAX_SEGMENTS = 1024;
 
+// A grouped call's segments in shared memory: n of them, their first rows and experts, and the tiles of tokens before each.
+struct Fp4Segments {
+    int n;
+    int32_t starts[FP4_MAX_SEGMENTS + 1], tiles[FP4_MAX_SEGMENTS + 1], experts[FP4_MAX_SEGMENTS];
+};
+
 template <int KIND_, int P_, int T_, int CG_ = 1>
 struct Fp4Shape {
     static constexpr int KIND = KIND_, P = P_, T = T_;
@@ -49,16 +55,20 @@ struct Fp4Shape {
     static constexpr int SFA = KB * 512, SFB = KB * NB * 512;
     static constexpr int TX = A_TX + SFA + (STACK ? 0 : B_BYTES + SFB);  // bytes that arrive for a stage (in each CTA)
     static constexpr int STAGE = (A_BYTES + B_BYTES + SFA + SFB + 1023) / 1024 * 1024;
-    // stages of the ring: one CTA an SM, or (narrow tiles, more of them than SMs) two
-    static constexpr int ring(int kb) { return kb * 1024 / STAGE < FP4_MAX_STAGES ? kb * 1024 / STAGE : FP4_MAX_STAGES; }
-    static constexpr int NS = ring(204), NS_TWO = ring(88);
+    // shared memory beside the ring (segs: of a grouped call), and the ring's stages in what is left: of the SM's 227 KB, or
+    // of a half where tiles are narrow and two CTAs share it
+    static constexpr size_t beside(bool segs) { return 1024 + (2 * FP4_MAX_STAGES + 4) * 8 + 32 + OUT * 2048 + (segs ? sizeof(Fp4Segments) : 0); }
+    static constexpr int stages(bool segs) {
+        const int n = int(((T <= 32 ? 113 : 227) * 1024 - beside(segs)) / STAGE);
+        return n < FP4_MAX_STAGES ? n : FP4_MAX_STAGES;
+    }
     static constexpr int N = STACK ? P * T : T;
     static constexpr int ACC = N <= 32 ? 32 : N <= 64 ? 64 : N <= 128 ? 128 : 256;
     // 256 columns: the two accumulators share 128, which are read out first
     static constexpr int ACC_STEP = ACC == 256 ? 128 : ACC;
     static constexpr int SF_COL = ACC == 256 ? 384 : 2 * ACC, SF_COLS = 4 * KB * (1 + NB);
     static constexpr int COLS = SF_COL + 2 * SF_COLS, TMEM = COLS <= 64 ? 64 : COLS <= 128 ? 128 : COLS <= 256 ? 256 : 512;
-    static_assert(COLS <= 512 && NS >= 2 && N % 16 == 0 && N <= 256 && B_TILE % 1024 == 0, "tile");
+    static_assert(COLS <= 512 && stages(true) >= 2 && N % 16 == 0 && N <= 256 && B_TILE % 1024 == 0, "tile");
     static_assert(!STACK || N <= 128, "stacked pieces share one scale tile");
 };
 
@@ -87,15 +97,14 @@ struct Fp4Args {
     int max_seg;
 };
 
-// Tile `id` of the token tiles of all segments: segment s has tiles starts[s] / T + s, ... (one number a segment may be
-// unused). The rows [r0, r1) of it.
+// A tile's rows [r0, r1) of x.
 struct Fp4Tile {
     int n0, r0, r1;   // first row of w (of the expert), rows of x
-    int expert, id;   // id: the tile of x's scales
+    int expert, id;   // id: the tile of x's scales (segment s has starts[s] / T + s, ...; a number may go unused)
 };
 
 template <typename S>
-__device__ __forceinline__ bool fp4_tile(const Fp4Args& a, const int32_t* starts, int nseg, int lin, Fp4Tile& t) {
+__device__ __forceinline__ bool fp4_tile(const Fp4Args& a, const Fp4Segments& seg, int lin, Fp4Tile& t) {
     constexpr int T = S::T, ROWS = 128 * S::CG;
     if (!a.grouped) {
         const int mt = a.ntiles / a.ntn;
@@ -106,23 +115,29 @@ __device__ __forceinline__ bool fp4_tile(const Fp4Args& a, const int32_t* starts
         t.expert = 0;
         return true;
     }
-    t.id = lin / a.ntn;
-    t.n0 = (lin - t.id * a.ntn) * ROWS;
-    int lo = 0, hi = nseg;  // the last segment whose first tile is not beyond id
+    const int q = int(uint32_t(lin) / uint32_t(a.ntn));
+    t.n0 = (lin - q * a.ntn) * ROWS;
+    int lo = 0, hi = seg.n;  // the last segment whose first tile is not beyond q
     while (hi - lo > 1) {
         const int mid = (lo + hi) / 2;
-        if (starts[mid] / T + mid <= t.id) lo = mid; else hi = mid;
+        if (seg.tiles[mid] <= q) lo = mid; else hi = mid;
     }
-    t.r0 = starts[lo] + (t.id - (starts[lo] / T + lo)) * T;
-    t.r1 = min(starts[lo + 1], t.r0 + T);
-    t.expert = a.experts[lo];
-    if (t.r0 >= t.r1 || t.expert == a.E) return false;
+    const int first = seg.starts[lo], i = q - seg.tiles[lo];
+    t.id = int(uint32_t(first) / T) + lo + i;
+    t.r0 = first + i * T;
+    t.r1 = min(seg.starts[lo + 1], t.r0 + T);
+    t.expert = seg.experts[lo];
+    if (t.expert == a.E) return false;  // padding
     if (t.expert < 0 || t.expert > a.E) {
         record_status(LQ_DEV_BOUNDS);
         return false;
     }
     return true;
 }
+
+// x / (1 + e^-x) by the fast exponential and quotient (a few units of 2^-23; 0 below -88, where the quotient of so large a
+// divisor is).
+__device__ __forceinline__ float fp4_silu(float x) { return __fdividef(x, 1.f + __expf(-x)); }
 
 __device__ __forceinline__ void fp4_store(const Fp4Args& a, int64_t at, float v) {
     if (a.dtype == LQ_F32)
@@ -138,7 +153,7 @@ template <typename S>
 __device__ __forceinline__ void fp4_out(const Fp4Args& a, const Fp4Tile& t, int c, int n, float v) {
     if (a.glu) {
         const float up = __shfl_xor_sync(0xFFFFFFFFu, v, 1);
-        if (!(n & 1) && n < a.N && t.r0 + c < t.r1) fp4_store(a, int64_t(t.r0 + c) * (a.N / 2) + n / 2, v / (1.f + __expf(-v)) * up);
+        if (!(n & 1) && n < a.N && t.r0 + c < t.r1) fp4_store(a, int64_t(t.r0 + c) * (a.N / 2) + n / 2, fp4_silu(v) * up);
     } else if (n < a.N && t.r0 + c < t.r1) {
         fp4_store(a, int64_t(t.r0 + c) * a.N + n, v);
     }
@@ -165,7 +180,7 @@ __device__ __forceinline__ void fp4_out16_t(const Fp4Args& a, const Fp4Tile& t, 
             const float mine = (odd ? v[2 * c + 1] : v[2 * c]) * f, lo = odd ? got[c] : mine, hi = odd ? mine : got[c];
             uint8_t* row = stage + (2 * c + odd) * BYTES;
             if constexpr (GLU) {
-                const float h = lo / (1.f + __expf(-lo)) * hi;
+                const float h = fp4_silu(lo) * hi;
                 if constexpr (sizeof(O) == 4)
                     reinterpret_cast<float*>(row)[lane >> 1] = h;
                 else
@@ -212,8 +227,8 @@ __device__ __forceinline__ void fp4_out4(const Fp4Args& a, const Fp4Tile& t, int
     float o[4] = {v.x * f, v.y * f, v.z * f, v.w * f};
     const int width = a.glu ? a.N / 2 : a.N, at = a.glu ? n / 2 : n, some = a.glu ? 2 : 4;
     if (a.glu) {
-        o[0] = o[0] / (1.f + __expf(-o[0])) * o[1];
-        o[1] = o[2] / (1.f + __expf(-o[2])) * o[3];
+        o[0] = fp4_silu(o[0]) * o[1];
+        o[1] = fp4_silu(o[2]) * o[3];
     }
     const int64_t first = int64_t(t.r0 + c) * width + at;
     if (a.dtype != LQ_F32 && !a.glu && width % 4 == 0 && n + 4 <= a.N && reinterpret_cast<uintptr_t>(a.y) % 8 == 0) {
@@ -300,7 +315,7 @@ __global__ void __launch_bounds__(FP4_THREADS, S::T <= 32 ? 2 : 1) fp4_gemm_kern
     uint64_t* acc_empty = acc_full + 2;  // [2] the epilogue has read what the next tile writes
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
     uint8_t* stage = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(tmem_slot + 1) + 15) & ~uintptr_t(15));  // 2 KB a warp
-    int32_t* seg = reinterpret_cast<int32_t*>(stage + FP4_OUT * 2048);  // [0] segments, then their starts (grouped)
+    Fp4Segments& seg = *reinterpret_cast<Fp4Segments*>(stage + S::OUT * 2048);  // (grouped)
 
     const int warp = __shfl_sync(0xFFFFFFFFu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     const int rank = CG == 2 || a.ks > 1 ? int(cluster_ctarank()) : 0;
@@ -323,9 +338,26 @@ __global__ void __launch_bounds__(FP4_THREADS, S::T <= 32 ? 2 : 1) fp4_gemm_kern
     grid_dep_launch();
     if (a.grouped) {
         grid_dep_wait();
-        const int n = a.nseg ? min(*a.nseg, a.max_seg) : a.M;  // without segments, each row is one
-        for (int i = threadIdx.x; i <= n; i += FP4_THREADS) seg[1 + i] = a.starts ? min(max(a.starts[i], 0), a.M) : i;
-        if (threadIdx.x == 0) seg[0] = n;
+        const int n = a.nseg ? min(max(*a.nseg, 0), a.max_seg) : a.M;  // without segments, each row is one
+        for (int i = threadIdx.x; i <= n; i += FP4_THREADS) seg.starts[i] = a.starts ? min(max(a.starts[i], 0), a.M) : i;
+        for (int i = threadIdx.x; i < n; i += FP4_THREADS) seg.experts[i] = a.experts[i];
+        if (threadIdx.x == 0) seg.n = n;
+        __syncthreads();
+        if (warp == 0) {  // tiles before each segment
+            int before = 0;
+            for (int i0 = 0; i0 < n; i0 += 32) {
+                const int i = i0 + lane;
+                int v = i < n ? (max(seg.starts[i + 1] - seg.starts[i], 0) + T - 1) / T : 0, sum = v;
+#pragma unroll
+                for (int d = 1; d < 32; d *= 2) {
+                    const int o = __shfl_up_sync(0xFFFFFFFFu, sum, d);
+                    if (lane >= d) sum += o;
+                }
+                if (i < n) seg.tiles[i] = before + sum - v;
+                before += __shfl_sync(0xFFFFFFFFu, sum, 31);
+            }
+            if (lane == 0) seg.tiles[n] = before;
+        }
     }
     tc_fence_before();
     // The cluster barrier counts warps: the one whose first lane sets up the mbarriers arrives when that lane has, not before
@@ -337,9 +369,7 @@ __global__ void __launch_bounds__(FP4_THREADS, S::T <= 32 ? 2 : 1) fp4_gemm_kern
         __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
-    const int nseg = a.grouped ? seg[0] : 0;
-    const int32_t* starts = seg + 1;
-    const int ntiles = a.grouped ? (nseg > 0 ? (starts[nseg] / T + nseg) * a.ntn : 0) : a.ntiles;
+    const int ntiles = a.grouped ? seg.tiles[seg.n] * a.ntn : a.ntiles;
     bool ok = true;
 
     if (warp == FP4_OUT || warp == FP4_OUT + 2) {
@@ -358,7 +388,7 @@ __global__ void __launch_bounds__(FP4_THREADS, S::T <= 32 ? 2 : 1) fp4_gemm_kern
                 if (!scales && (CG == 1 || rank == 0)) mbar_arrive_expect_tx(&full[slot], CG * S::TX);
             };
             for (int lin = first; lin < ntiles && ok; lin += step) {
-                if (!fp4_tile<S>(a, starts, nseg, lin, t)) continue;
+                if (!fp4_tile<S>(a, seg, lin, t)) continue;
                 const int wrow = t.expert * a.N + t.n0 + 128 * half, wtile = t.expert * a.rtiles + t.n0 / 128 + half;
                 auto weights = [&](int kb, int slot) {
                     const uint32_t st = ring + slot * S::STAGE, bar = bars + slot * 8;
@@ -419,7 +449,7 @@ __global__ void __launch_bounds__(FP4_THREADS, S::T <= 32 ? 2 : 1) fp4_gemm_kern
         int it = 0, j = 0, s = 0, turn = 0;
         Fp4Tile t;
         for (int lin = first; (CG == 1 || rank == 0) && lin < ntiles && ok; lin += step) {
-            if (!fp4_tile<S>(a, starts, nseg, lin, t)) continue;
+            if (!fp4_tile<S>(a, seg, lin, t)) continue;
             if constexpr (S::ACC == 256) {
                 if (j >= 1) ok = mbar_wait_cg<CG>(&acc_empty[0], (j - 1) & 1);
             } else {
@@ -487,7 +517,7 @@ __global__ void __launch_bounds__(FP4_THREADS, S::T <= 32 ? 2 : 1) fp4_gemm_kern
             int who = 0, s = 0, turn = 0;  // the warp of the next stage, its place, rounds of the ring
             Fp4Tile t;
             for (int lin = first; lin < ntiles && ok; lin += step) {
-                if (!fp4_tile<S>(a, starts, nseg, lin, t)) continue;
+                if (!fp4_tile<S>(a, seg, lin, t)) continue;
                 int src = t.r0 + lane < t.r1 ? t.r0 + lane : -1;  // the row of x of the tile's token `lane`
                 if (a.gather && src >= 0) src = (a.order ? a.order[src] : src) / a.gather;
                 if (src >= a.src_rows || (src < 0 && t.r0 + lane < t.r1)) {
@@ -569,7 +599,7 @@ __global__ void __launch_bounds__(FP4_THREADS, S::T <= 32 ? 2 : 1) fp4_gemm_kern
         int j = 0;
         Fp4Tile t;
         for (int lin = first; lin < ntiles; lin += step) {
-            if (!fp4_tile<S>(a, starts, nseg, lin, t)) continue;
+            if (!fp4_tile<S>(a, seg, lin, t)) continue;
             if (ok) ok = mbar_wait_cg<CG>(&acc_full[j & 1], (j >> 1) & 1);
             if (!ok) break;
             tc_fence_after();
@@ -624,7 +654,7 @@ __global__ void __launch_bounds__(FP4_THREADS, S::T <= 32 ? 2 : 1) fp4_gemm_kern
         __syncwarp();
         cluster_sync();
         Fp4Tile t;
-        if (warp < FP4_OUT && first < ntiles && fp4_tile<S>(a, starts, nseg, first, t)) {
+        if (warp < FP4_OUT && first < ntiles && fp4_tile<S>(a, seg, first, t)) {
             const float f = (a.xf ? *a.xf : 1.f) * (a.wf ? *a.wf : 1.f);
             const uint32_t part = smem_u32(smem) + lane * 16;  // a lane takes four rows of w
             for (int c = rank + a.ks * warp; c < T && t.r0 + c < t.r1; c += FP4_OUT * a.ks) {
@@ -780,11 +810,11 @@ static int map_scales(CUtensorMap* m, const void* base, uint64_t inner, uint64_t
 // clusters of three need not fit 148 SMs. Asked once a device, kernel and size. (Of a kernel that allocates tensor memory the
 // runtime counts one CTA an SM, whatever it allocates; narrow tiles run two, as their start times show.)
 template <typename S>
-static int max_clusters(int ks, size_t smem) {
+static int max_clusters(int ks, size_t smem, int grouped) {
     static std::atomic<int> known[16][2][9];
     const int dev = device_info().device;
     if (dev < 0 || dev >= 16) return 0;
-    std::atomic<int>& k = known[dev][smem > size_t(S::T <= 32 ? S::NS_TWO : S::NS) * S::STAGE + 1024 + FP4_OUT * 2048 + 1024][ks];
+    std::atomic<int>& k = known[dev][grouped][ks];
     int n = k.load(std::memory_order_relaxed);
     if (n == 0) {
         cudaLaunchConfig_t cfg = {};
@@ -823,10 +853,9 @@ static int gemm_t(const Fp4Call& c, cudaStream_t st) {
     const int64_t tiles = c.ttiles * a.ntn;
     if (tiles > INT32_MAX) return LQ_E_SHAPE;
     a.ntiles = int(tiles);
-    a.nst = S::T <= 32 ? S::NS_TWO : S::NS;
-    const size_t smem = 1024 + size_t(a.nst) * S::STAGE + (2 * a.nst + 4) * 8 + 32 + FP4_OUT * 2048 + (a.grouped ? (FP4_MAX_SEGMENTS + 2) * 4 : 0);
-    static_assert(S::NS_TWO >= 2 || S::T > 32, "two CTAs an SM");
-    static_assert(S::ACC == 256 || S::T * 512 <= (S::T <= 32 ? S::NS_TWO : S::NS) * S::STAGE, "the partial sums of a split fit the ring");
+    a.nst = S::stages(a.grouped);
+    const size_t smem = S::beside(a.grouped) + size_t(a.nst) * S::STAGE;
+    static_assert(S::ACC == 256 || S::T * 512 <= S::stages(true) * S::STAGE, "the partial sums of a split fit the ring");
     auto kern = fp4_gemm_kernel<S>;
     if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem)) != cudaSuccess ||
         cudaFuncSetAttribute(kern, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared) != cudaSuccess)
@@ -836,7 +865,7 @@ static int gemm_t(const Fp4Call& c, cudaStream_t st) {
     if (S::CG == 1) {
         const int most = a.ns < 8 ? a.ns : 8;
         for (int ks = most; ks > 1 && a.ks == 1; --ks)
-            if (tiles * ks <= int64_t(sms) * (S::T <= 32 ? 2 : 1) && tiles <= max_clusters<S>(ks, smem) * (S::T <= 32 ? 2 : 1)) a.ks = ks;
+            if (tiles * ks <= int64_t(sms) * (S::T <= 32 ? 2 : 1) && tiles <= max_clusters<S>(ks, smem, a.grouped) * (S::T <= 32 ? 2 : 1)) a.ks = ks;
     }
     const int64_t slots = int64_t(sms) * (S::T <= 32 ? 2 : 1);
     const int64_t grid = S::CG == 2 ? (tiles < sms / 2 ? tiles : sms / 2) * 2 : a.ks > 1 ? tiles * a.ks : tiles < slots ? tiles : slots;
