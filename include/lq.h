@@ -337,7 +337,7 @@ int lq_fp4_qmm(const uint32_t* x_codes, const uint8_t* x_tiles, const float* x_f
 
 /* y (M, N) = x . w^T of x (M, K) in f16 / bf16 (x_row elements from one row to the next) and w in LQ_MXFP4; y in x's
  * dtype; glu as lq_fp4_qmm. x enters in pieces of e4m3 with a power of two a group of 32: exact down to 2^-14 of a group's
- * largest magnitude, below that off by at most 2^-22 of it; a row that holds an infinity or no number gives no numbers.
+ * largest magnitude, below that off by at most 2^-21 of it; a row that holds an infinity or no number gives no numbers.
  * workspace: lq_fp4_linear_workspace(M, K, dtype) bytes, 256-byte aligned (NULL when that is 0: few tokens). */
 size_t lq_fp4_linear_workspace(int M, int K, int dtype);
 int lq_fp4_linear(const void* x, int64_t x_row, const uint32_t* codes, const uint8_t* tiles, int M, int N, int K, int glu,

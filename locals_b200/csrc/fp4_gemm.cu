@@ -7,7 +7,7 @@
 // of two a group of 32: bf16 (8 bits) is the sum of 2, fp16 (11 bits) of 3. With E the exponent of the largest magnitude of
 // the group, piece p has the scale 2^(E - 7 - 5 p) (its values are below 2^8, so what is left after rounding them to 4 bits
 // is at most 2^3) and is the rounded remainder of those before it. The pieces' sum is x exactly down to 2^-14 of that
-// magnitude; below, it is off by at most half a last step, 2^-22 (bf16) or 2^-27 (fp16) of it, less than
+// magnitude; below, it is off by about half a last step, less than 2^-21 (bf16) or 2^-26 (fp16) of it, less than
 // the 32-bit sum itself loses beside that value. A group that holds an infinity or no number is not a number.
 //
 // Layout. Weights are the MMA's A operand (128 rows of w a tile, one a tensor-memory lane), T tokens its N side, so that one
@@ -253,16 +253,33 @@ __device__ __forceinline__ uint4 load8_16(const T16* row, int k0, int K, bool ve
     return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// 8 values of a group of 32 (four lanes next to one another) to P pieces of e4m3 bytes and their scale bytes.
+// The largest magnitude of 8 values (a number that is none, if one is).
+template <typename T2>
+__device__ __forceinline__ float amax8_16(const uint4& x) {
+    const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+    T2 m = __habs2(*reinterpret_cast<const T2*>(&w[0]));
+#pragma unroll
+    for (int i = 1; i < 4; ++i) m = __hmax2_nan(m, __habs2(*reinterpret_cast<const T2*>(&w[i])));
+    float lo, hi, top;
+    if constexpr (std::is_same<T2, __half2>::value) {
+        lo = __low2float(m);
+        hi = __high2float(m);
+    } else {
+        const uint32_t b = *reinterpret_cast<uint32_t*>(&m);
+        lo = __uint_as_float(b << 16);
+        hi = __uint_as_float(b & 0xFFFF0000u);
+    }
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(top) : "f"(lo), "f"(hi));
+    return top;
+}
+
+// 8 values of a group of 32 (four lanes next to one another) to P pieces of e4m3 bytes and their scale bytes. Scaled to below
+// 2^8 the values are fp16 numbers but for what lies below 2^-24 there, and the steps from piece to piece are exact in fp16.
 template <typename T16, int P>
 __device__ __forceinline__ void split8(const uint4& x, uint32_t mask, uint2 (&piece)[P], int (&byte)[P]) {
+    using T2 = typename std::conditional<std::is_same<T16, __half>::value, __half2, __nv_bfloat162>::type;
     const uint32_t w[4] = {x.x, x.y, x.z, x.w};
-    float v[8], top = 0.f;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        v[i] = F16Traits<T16>::to_f32(w[i >> 1] >> (16 * (i & 1)) & 0xFFFFu);
-        asm("max.NaN.f32 %0, %1, %2;" : "=f"(top) : "f"(top), "f"(fabsf(v[i])));
-    }
+    float top = amax8_16<T2>(x);
 #pragma unroll
     for (int d = 1; d < 4; d *= 2) {
         const float o = __shfl_xor_sync(mask, top, d);
@@ -271,29 +288,26 @@ __device__ __forceinline__ void split8(const uint4& x, uint32_t mask, uint2 (&pi
     const uint32_t e = __float_as_uint(top) >> 23 & 0xFF;
     byte[0] = e == 255 ? 255 : e < 7 ? 0 : int(e) - 7;
     const float up = __uint_as_float((254u - (e == 255 ? 127u : uint32_t(byte[0]))) << 23);
+    __half2 h[4];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] *= up;
+    for (int i = 0; i < 4; ++i)
+        h[i] = __floats2half2_rn(F16Traits<T16>::to_f32(w[i] & 0xFFFFu) * up, F16Traits<T16>::to_f32(w[i] >> 16) * up);
 #pragma unroll
     for (int p = 0; p < P; ++p) {
-        uint32_t q[2];
+        uint16_t q[4];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const uint32_t lo = cvt_e4m3x2(v[4 * h + 1], v[4 * h]), hi = cvt_e4m3x2(v[4 * h + 3], v[4 * h + 2]);
-            q[h] = lo | hi << 16;
-            if (p + 1 < P) {
-                const float2 x01 = e4m3x2_to_f32(lo), x23 = e4m3x2_to_f32(hi);
-                v[4 * h] -= x01.x;
-                v[4 * h + 1] -= x01.y;
-                v[4 * h + 2] -= x23.x;
-                v[4 * h + 3] -= x23.y;
-            }
-        }
-        piece[p] = make_uint2(q[0], q[1]);
+        for (int i = 0; i < 4; ++i)
+            asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(q[i]) : "r"(*reinterpret_cast<uint32_t*>(&h[i])));
+        piece[p] = make_uint2(q[0] | uint32_t(q[1]) << 16, q[2] | uint32_t(q[3]) << 16);
         if (p + 1 < P) {
             byte[p + 1] = byte[p] == 255 ? 255 : byte[p] < 5 ? 0 : byte[p] - 5;
-            const float more = __uint_as_float(uint32_t(127 + (byte[p] == 255 ? 0 : byte[p] - byte[p + 1])) << 23);
+            const __half2 more = __float2half2_rn(__uint_as_float(uint32_t(127 + (byte[p] == 255 ? 0 : byte[p] - byte[p + 1])) << 23));
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] *= more;
+            for (int i = 0; i < 4; ++i) {
+                uint32_t back;
+                asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(back) : "h"(q[i]));
+                h[i] = __hmul2(__hsub2(h[i], *reinterpret_cast<__half2*>(&back)), more);
+            }
         }
     }
 }

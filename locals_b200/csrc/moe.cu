@@ -159,10 +159,11 @@ __global__ void group_kernel(const uint32_t* inds, int P, int E, int32_t* order,
 // places its pairs in pair order (a match over each 32 pairs ranks equal experts by lane). Pair p of expert e lands
 // after every earlier pair of e, exactly as in group_kernel: the same order, starts, experts and pos.
 constexpr int GROUP_PAR_MAX_E = 1024;
+constexpr int GROUP_CLUSTER_MIN_P = 2049;  // from here a cluster of 8 CTAs (16,004 pairs 36 -> 9 us; 2,048 pairs 6.9 in one)
 
 __global__ void __launch_bounds__(1024) group_par_kernel(const uint32_t* inds, int P, int E, int32_t* order,
                                                          int32_t* starts, int32_t* experts, int32_t* nseg,
-                                                         int32_t* pos, int lo, int range, int staged) {
+                                                         int32_t* pos, int lo, int range, int ctas) {
     grid_dep_wait();
     grid_dep_launch();
     extern __shared__ int32_t sh[];
@@ -170,14 +171,12 @@ __global__ void __launch_bounds__(1024) group_par_kernel(const uint32_t* inds, i
     int32_t* cnt = sh + 32 * E;    // E totals
     int32_t* run = cnt + E;        // E segment starts
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int CH = (P + 31) / 32;
-    const int p0 = warp * CH, p1 = p0 + CH < P ? p0 + CH : P;
+    // many pairs: a cluster of CTAs, each with its share of them (the matches of equal experts bound one SM)
+    const int rank = ctas > 1 ? int(cluster_ctarank()) : 0;
+    const int share = (P + ctas - 1) / ctas, s0 = min(rank * share, P), s1 = min(s0 + share, P);
+    const int CH = (s1 - s0 + 31) / 32;
+    const int p0 = min(s0 + warp * CH, s1), p1 = p0 + CH < s1 ? p0 + CH : s1;
     for (int i = threadIdx.x; i < 32 * E; i += blockDim.x) hist[i] = 0;
-    if (staged) {  // the ids in shared memory: both passes walk them one 32 at a time (16,004 pairs 33 -> 12 us)
-        uint32_t* ids = reinterpret_cast<uint32_t*>(run + E);
-        for (int i = threadIdx.x; i < P; i += blockDim.x) ids[i] = inds[i];
-        inds = ids;
-    }
     __syncthreads();
     for (int c = p0; c < p1; c += 32) {
         const int p = c + lane;
@@ -199,11 +198,28 @@ __global__ void __launch_bounds__(1024) group_par_kernel(const uint32_t* inds, i
         cnt[e] = acc;
     }
     __syncthreads();
+    int32_t* all = cnt;    // totals of all CTAs, and of the ones before this
+    int32_t* before = run + E;
+    if (ctas > 1) {
+        all = before + E;
+        cluster_sync();
+        for (int e = threadIdx.x; e < E; e += blockDim.x) {
+            int sum = 0, lower = 0;
+            for (int r = 0; r < ctas; ++r) {
+                const int v = __float_as_int(ld_dsmem_f(map_peer(smem_u32(cnt + e), r)));
+                if (r < rank) lower += v;
+                sum += v;
+            }
+            all[e] = sum;
+            before[e] = lower;
+        }
+        __syncthreads();
+    }
     if (warp == 0) {
         int at = 0, sgi = 0;
         for (int c = 0; c < E; c += 32) {
             const int e = c + lane;
-            const int v = e < E ? cnt[e] : 0;
+            const int v = e < E ? all[e] : 0;
             int incl = v;
 #pragma unroll
             for (int d = 1; d < 32; d <<= 1) {
@@ -211,8 +227,8 @@ __global__ void __launch_bounds__(1024) group_par_kernel(const uint32_t* inds, i
                 if (lane >= d) incl += t;
             }
             const unsigned nz = __ballot_sync(0xFFFFFFFFu, v > 0);
-            if (e < E) run[e] = at + incl - v;
-            if (v > 0) {
+            if (e < E) run[e] = at + incl - v + (ctas > 1 ? before[e] : 0);
+            if (v > 0 && rank == 0) {
                 const int si = sgi + __popc(nz & ((1u << lane) - 1u));
                 starts[si] = at + incl - v;
                 experts[si] = e;
@@ -220,7 +236,7 @@ __global__ void __launch_bounds__(1024) group_par_kernel(const uint32_t* inds, i
             at += __shfl_sync(0xFFFFFFFFu, incl, 31);
             sgi += __popc(nz);
         }
-        if (lane == 0) {
+        if (lane == 0 && rank == 0) {
             starts[sgi] = at;
             nseg[0] = sgi;
         }
@@ -240,6 +256,10 @@ __global__ void __launch_bounds__(1024) group_par_kernel(const uint32_t* inds, i
             order[j] = p;
             if (pos) pos[p] = j;
         }
+    }
+    if (ctas > 1) {
+        __syncwarp();
+        cluster_sync();  // the counts stay until every CTA has read them
     }
 }
 
@@ -544,16 +564,33 @@ int route_topk_run(const float* logits, int T, int E, int k, int mode, uint32_t*
 static int group_impl(const uint32_t* inds, int P, int E, int32_t* order, int32_t* starts, int32_t* experts,
                       int32_t* nseg, int32_t* pos, cudaStream_t st, int lo, int range) {
     if (E <= GROUP_PAR_MAX_E && P > 256) {  // (up to 256 pairs the one-warp placement is as fast)
-        size_t smem = size_t(34) * E * sizeof(int32_t);
-        const int staged = P <= 16384;
-        if (staged) smem += size_t(P) * sizeof(uint32_t);
+        const int ctas = P >= GROUP_CLUSTER_MIN_P ? 8 : 1;
+        const size_t smem = size_t(ctas > 1 ? 36 : 34) * E * sizeof(int32_t);
         if (smem > 48 * 1024) {
             const cudaError_t e =
                 cudaFuncSetAttribute(group_par_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem));
             if (e != cudaSuccess) return LQ_E_CUDA;
         }
+        if (ctas > 1) {
+            cudaLaunchConfig_t cfg = {};
+            cfg.gridDim = dim3(unsigned(ctas));
+            cfg.blockDim = dim3(1024);
+            cfg.dynamicSmemBytes = smem;
+            cfg.stream = st;
+            cudaLaunchAttribute attr[2];
+            attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+            attr[0].val.programmaticStreamSerializationAllowed = 1;
+            attr[1].id = cudaLaunchAttributeClusterDimension;
+            attr[1].val.clusterDim.x = unsigned(ctas);
+            attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+            cfg.attrs = attr;
+            cfg.numAttrs = 2;
+            return cudaLaunchKernelEx(&cfg, group_par_kernel, inds, P, E, order, starts, experts, nseg, pos, lo, range, ctas) == cudaSuccess
+                       ? LQ_OK
+                       : LQ_E_CUDA;
+        }
         return launch_pdl(group_par_kernel, dim3(1), dim3(1024), smem, st, inds, P, E, order, starts, experts, nseg,
-                          pos, lo, range, staged);
+                          pos, lo, range, ctas);
     }
     const size_t smem = size_t(2) * E * sizeof(int32_t) + size_t(GROUP_STAGE) * sizeof(uint32_t);
     if (smem > 48 * 1024) {

@@ -124,7 +124,7 @@ def dequantize(a: Fp4, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
 def matmul(x, w: Fp4, dtype: Optional[torch.dtype] = None, glu: bool = False) -> torch.Tensor:
     """y = x . w^T with 32-bit sums, rounded once. ``x`` an ``Fp4`` matrix of w's format: y (M, N) in ``dtype`` (default
     bf16; fp16, fp32). ``x`` a tensor (..., K) in fp16 or bf16 and w in mxfp4: y (..., N) in x's dtype; x is exact down to
-    2^-14 of a group of 32's largest magnitude, below that off by at most 2^-22 of it, and a row with an infinity or no number in
+    2^-14 of a group of 32's largest magnitude, below that off by at most 2^-21 of it, and a row with an infinity or no number in
     it gives no numbers. ``glu``: w holds gate and up rows in turn (``interleave``) and y (..., N / 2) is silu(gate) * up."""
     if isinstance(x, Fp4):
         return ext().fp4_product(x, w, dtype or torch.bfloat16, glu)

@@ -621,3 +621,51 @@ def test_offsets_beyond_32_bits(cuda):
     back = fp4.dequantize(a)
     assert torch.equal(back[-2:], fp4.dequantize(small)) and not back[1000].any()
     _ok(cuda)
+
+
+# ---- what the experts share with the other formats -------------------------------------------------------------
+
+@pytest.mark.parametrize("P,E", [(2048, 64), (2049, 64), (2049, 1), (5000, 7), (16004, 64), (40000, 1000), (70001, 128)])
+def test_group_of_many_pairs(cuda, P, E):
+    """Ids grouped in their own order, whatever the number of CTAs."""
+    import torch
+    from locals_b200 import moe
+
+    g = _gen(cuda, P)
+    inds = (torch.rand(P, generator=g, device=cuda) ** 3 * E).long().clamp(max=E - 1)
+    inds[P // 2:P // 2 + 300] = E - 1
+    for lo, count in ((0, E), (E // 3, max(1, E // 2))):
+        if (lo, count) == (0, E):
+            order, starts, experts, nseg, pos = moe.group(inds.to(torch.int32), E)
+            key = inds
+        else:
+            order, starts, experts, nseg, pos = moe.group_range(inds.to(torch.int32), lo, count)
+            key = torch.where((inds >= lo) & (inds < lo + count), inds - lo, count)
+        want = torch.argsort(key, stable=True)
+        assert torch.equal(order.long(), want)
+        assert torch.equal(pos.long()[want], torch.arange(P, device=cuda))
+        ids, counts = torch.unique(key, return_counts=True)
+        n = int(nseg)
+        assert n == len(ids) and torch.equal(experts[:n].long(), ids)
+        assert torch.equal(starts[:n + 1].long(), torch.cat([torch.zeros(1, dtype=torch.long, device=cuda), counts.cumsum(0)]))
+    _ok(cuda)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("T,k,D", [(1, 4, 2048), (3, 1, 8), (77, 6, 136), (33, 2, 100), (500, 8, 264)])
+def test_combine_keeps_its_order_of_sums(cuda, dtype, T, k, D):
+    """Slots in order in 32 bits, fused multiply and add, rounded once: bit for bit, eight columns a thread or one."""
+    import torch
+    from locals_b200 import moe
+
+    g = _gen(cuda, T)
+    ys = torch.randn((T * k, D), generator=g, device=cuda).to(_dt(dtype))
+    w = torch.rand((T, k), generator=g, device=cuda)
+    for pos in (None, torch.randperm(T * k, generator=g, device=cuda).to(torch.int32)):
+        acc = torch.zeros((T, D), dtype=torch.float32, device=cuda)
+        for r in range(k):
+            rows = ys[pos.view(T, k)[:, r].long()] if pos is not None else ys.view(T, k, D)[:, r]
+            # a product of 8 or 11 bits by 24 and a sum of 24 bits: exact in 64 bits but for its last rounding, then to 32
+            acc = (rows.double() * w[:, r, None].double() + acc.double()).float()
+        assert torch.equal(moe.combine(ys, w, pos), acc.to(_dt(dtype)))
+    _ok(cuda)
