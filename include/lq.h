@@ -338,8 +338,8 @@ int lq_fp4_qmm(const uint32_t* x_codes, const uint8_t* x_tiles, const float* x_f
 /* y (M, N) = x . w^T of x (M, K) in f16 / bf16 (x_row elements from one row to the next) and w in LQ_MXFP4; y in x's
  * dtype; glu as lq_fp4_qmm. x enters in pieces of e4m3 with a power of two a group of 32: exact down to 2^-14 of a group's
  * largest magnitude, below that off by at most 2^-21 of it; a row that holds an infinity or no number gives no numbers.
- * workspace: lq_fp4_linear_workspace(M, K, dtype) bytes, 256-byte aligned (NULL when that is 0: few tokens). */
-size_t lq_fp4_linear_workspace(int M, int K, int dtype);
+ * workspace: lq_fp4_linear_workspace(M, N, K, dtype) bytes, 256-byte aligned (NULL when that is 0: few tokens). */
+size_t lq_fp4_linear_workspace(int M, int N, int K, int dtype);
 int lq_fp4_linear(const void* x, int64_t x_row, const uint32_t* codes, const uint8_t* tiles, int M, int N, int K, int glu,
                   int dtype, void* y, void* workspace, size_t workspace_bytes, void* stream);
 
@@ -347,8 +347,8 @@ int lq_fp4_linear(const void* x, int64_t x_row, const uint32_t* codes, const uin
  * (P, N / 2) with glu as lq_fp4_qmm. x (x_rows, K): with gather_k > 0, pair j reads row gather_order[j] / gather_k
  * (gather_order NULL: j / gather_k; a row that x does not have: zeros, and LQ_DEV_BOUNDS); with 0, row j. Segments as lq_moe_experts (an expert id E is padding, left unwritten), at most 1024 of them
  * (min(E + 1, P)); starts and nseg NULL: row j is a segment of its own, of expert experts[j].
- * workspace: lq_fp4_experts_workspace(P, max_rows, E, K, dtype) bytes, 256-byte aligned (NULL when that is 0). */
-size_t lq_fp4_experts_workspace(int P, int max_rows, int E, int K, int dtype);
+ * workspace: lq_fp4_experts_workspace(P, max_rows, E, N, K, dtype) bytes, 256-byte aligned (NULL when that is 0). */
+size_t lq_fp4_experts_workspace(int P, int max_rows, int E, int N, int K, int dtype);
 int lq_fp4_experts(const void* x, int x_rows, const int32_t* gather_order, int gather_k, const int32_t* starts,
                    const int32_t* experts, const int32_t* nseg, int P, int max_rows, int glu, const uint32_t* codes,
                    const uint8_t* tiles, void* out, int E, int N, int K, int dtype, void* workspace,

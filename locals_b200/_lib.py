@@ -76,9 +76,9 @@ SIGNATURES = {
     "lq_fp4_quantize": ([_vp, _i, _i64, _i, _i, _i, _vp, _u32p, _vp, _vp], _i),
     "lq_fp4_dequantize": ([_u32p, _vp, _i, _i, _i, _i, _vp, _i, _vp, _vp], _i),
     "lq_fp4_qmm": ([_u32p, _vp, _vp, _u32p, _vp, _vp, _i, _i, _i, _i, _i, _i, _vp, _vp], _i),
-    "lq_fp4_linear_workspace": ([_i, _i, _i], ctypes.c_size_t),
+    "lq_fp4_linear_workspace": ([_i, _i, _i, _i], ctypes.c_size_t),
     "lq_fp4_linear": ([_vp, _i64, _u32p, _vp, _i, _i, _i, _i, _i, _vp, _vp, ctypes.c_size_t, _vp], _i),
-    "lq_fp4_experts_workspace": ([_i, _i, _i, _i, _i], ctypes.c_size_t),
+    "lq_fp4_experts_workspace": ([_i, _i, _i, _i, _i, _i], ctypes.c_size_t),
     "lq_fp4_experts": ([_vp, _i, _vp, _i, _vp, _vp, _vp, _i, _i, _i, _u32p, _vp, _vp, _i, _i, _i, _i, _vp,
                         ctypes.c_size_t, _vp], _i),
     "lq_supported": ([_i, _i, _i, _i, _i, _i, _i], _i),

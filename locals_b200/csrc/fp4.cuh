@@ -13,6 +13,8 @@
 #include <cuda_fp16.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "../../include/lq.h"
 #include "lq_ptx.cuh"
 
@@ -29,21 +31,17 @@ __host__ __device__ constexpr int fp4_tile_byte(int row, int group) {
     return 16 * (row % 32) + 4 * (row / 32) + group % 4;
 }
 
-// Two floats to two e2m1 codes (nearest, ties to even, saturating): `lo` in bits 0-3, `hi` in bits 4-7.
-__device__ __forceinline__ uint32_t cvt_e2m1x2(float hi, float lo) {
+// Eight floats to a word of e2m1 codes (nearest, ties to even, saturating), the first in the lowest bits.
+__device__ __forceinline__ uint32_t codes8(const float (&v)[8]) {
     uint32_t r;
-    asm("{\n\t.reg .b8 b;\n\t"
-        "cvt.rn.satfinite.e2m1x2.f32 b, %1, %2;\n\t"
-        "cvt.u32.u8 %0, b;\n\t}"
+    asm("{\n\t.reg .b8 a, b, c, d;\n\t"
+        "cvt.rn.satfinite.e2m1x2.f32 a, %2, %1;\n\t"
+        "cvt.rn.satfinite.e2m1x2.f32 b, %4, %3;\n\t"
+        "cvt.rn.satfinite.e2m1x2.f32 c, %6, %5;\n\t"
+        "cvt.rn.satfinite.e2m1x2.f32 d, %8, %7;\n\t"
+        "mov.b32 %0, {a, b, c, d};\n\t}"
         : "=r"(r)
-        : "f"(hi), "f"(lo));
-    return r;
-}
-
-// Two floats to two e4m3 bytes, `lo` in the low one.
-__device__ __forceinline__ uint32_t cvt_e4m3x2(float hi, float lo) {
-    uint16_t r;
-    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
+        : "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]));
     return r;
 }
 
@@ -59,6 +57,37 @@ __device__ __forceinline__ float fp4_scale_value(uint32_t b, int mode) {
     if (mode == LQ_MXFP4)  // 2^(b - 127): the exponent field, but for 0 (2^-127 is no normal number) and 255 (not a number)
         return b == 0 ? __uint_as_float(0x00400000u) : b == 255 ? __uint_as_float(0x7FC00000u) : __uint_as_float(b << 23);
     return e4m3x2_to_f32(b).x;
+}
+
+// Values [k0, k0 + 8) of a row of K 16-bit values, zeros beyond it; `vec`: the row starts on a 16-byte boundary.
+template <typename T16>
+__device__ __forceinline__ uint4 load8_16(const T16* row, int k0, int K, bool vec) {
+    if (vec && k0 + 8 <= K) return *reinterpret_cast<const uint4*>(row + k0);
+    uint32_t w[4] = {};
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+        if (k0 + i < K) w[i >> 1] |= uint32_t(reinterpret_cast<const uint16_t*>(row)[k0 + i]) << (16 * (i & 1));
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// The largest magnitude of 8 values (a number that is none, if one is).
+template <typename T2>
+__device__ __forceinline__ float amax8_16(const uint4& x) {
+    const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+    T2 m = __habs2(*reinterpret_cast<const T2*>(&w[0]));
+#pragma unroll
+    for (int i = 1; i < 4; ++i) m = __hmax2_nan(m, __habs2(*reinterpret_cast<const T2*>(&w[i])));
+    float lo, hi, top;
+    if constexpr (std::is_same<T2, __half2>::value) {
+        lo = __low2float(m);
+        hi = __high2float(m);
+    } else {
+        const uint32_t b = *reinterpret_cast<uint32_t*>(&m);
+        lo = __uint_as_float(b << 16);
+        hi = __uint_as_float(b & 0xFFFF0000u);
+    }
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(top) : "f"(lo), "f"(hi));
+    return top;
 }
 
 // One lane of a whole warp, chosen in a way that the compiler knows to be uniform: tcgen05 and TMA instructions take their

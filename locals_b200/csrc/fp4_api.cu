@@ -60,8 +60,8 @@ int lq_fp4_qmm(const uint32_t* x_codes, const uint8_t* x_tiles, const float* x_f
                               reinterpret_cast<cudaStream_t>(stream)));
 }
 
-size_t lq_fp4_linear_workspace(int M, int K, int dtype) {
-    return fp4_rows_ok(M, K, LQ_MXFP4) || !is16(dtype) ? 0 : fp4_linear_workspace_bytes(M, K, dtype, 0, M);
+size_t lq_fp4_linear_workspace(int M, int N, int K, int dtype) {
+    return fp4_rows_ok(M, K, LQ_MXFP4) || fp4_rows_ok(N, K, LQ_MXFP4) || !is16(dtype) ? 0 : fp4_linear_workspace_bytes(M, N, K, dtype, 0, M);
 }
 
 int lq_fp4_linear(const void* x, int64_t x_row, const uint32_t* codes, const uint8_t* tiles, int M, int N, int K, int glu,
@@ -72,7 +72,7 @@ int lq_fp4_linear(const void* x, int64_t x_row, const uint32_t* codes, const uin
     if (rc) return rc;
     if (glu && N % 2) return LQ_E_SHAPE;
     if (x_row < K && M > 1) return LQ_E_SHAPE;
-    const size_t bytes = lq_fp4_linear_workspace(M, K, dtype);
+    const size_t bytes = lq_fp4_linear_workspace(M, N, K, dtype);
     if (bytes && !workspace) return LQ_E_ARG;
     if (workspace_bytes < bytes) return LQ_E_SHAPE;
     if (!aligned(codes, 32) || !aligned(tiles, 16) || !aligned(workspace, 256) || !aligned(x, 2) || !aligned(y, 2)) return LQ_E_ALIGN;
@@ -96,10 +96,10 @@ int lq_fp4_linear(const void* x, int64_t x_row, const uint32_t* codes, const uin
 
 static int fp4_segments(int P, int E) { return P < E + 1 ? P : E + 1; }
 
-size_t lq_fp4_experts_workspace(int P, int max_rows, int E, int K, int dtype) {
-    if (fp4_rows_ok(P, K, LQ_MXFP4) || !is16(dtype) || E < 1 || max_rows < 1) return 0;
-    const size_t some = fp4_linear_workspace_bytes(P, K, dtype, fp4_segments(P, E), max_rows);
-    const size_t each = P <= 1024 ? fp4_linear_workspace_bytes(P, K, dtype, P, max_rows) : 0;  // without segments
+size_t lq_fp4_experts_workspace(int P, int max_rows, int E, int N, int K, int dtype) {
+    if (fp4_rows_ok(P, K, LQ_MXFP4) || fp4_rows_ok(N, K, LQ_MXFP4) || !is16(dtype) || E < 1 || max_rows < 1) return 0;
+    const size_t some = fp4_linear_workspace_bytes(P, N, K, dtype, fp4_segments(P, E), max_rows);
+    const size_t each = P <= 1024 ? fp4_linear_workspace_bytes(P, N, K, dtype, P, max_rows) : 0;  // without segments
     return some > each ? some : each;
 }
 
@@ -115,7 +115,7 @@ int lq_fp4_experts(const void* x, int x_rows, const int32_t* gather_order, int g
     if (rc) return rc;
     const int segments = starts ? fp4_segments(P, E) : P;
     if ((glu && N % 2) || segments > 1024) return LQ_E_SHAPE;
-    const size_t bytes = lq_fp4_experts_workspace(P, max_rows, E, K, dtype);
+    const size_t bytes = lq_fp4_experts_workspace(P, max_rows, E, N, K, dtype);
     if (bytes && !workspace) return LQ_E_ARG;
     if (workspace_bytes < bytes) return LQ_E_SHAPE;
     if (!aligned(codes, 32) || !aligned(tiles, 16) || !aligned(workspace, 256) || !aligned(x, 2) || !aligned(out, 2)) return LQ_E_ALIGN;

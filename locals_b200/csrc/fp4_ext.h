@@ -137,7 +137,7 @@ Tensor linear(Tensor x, const py::tuple& w, bool glu) {
     if (y.numel()) {
         const int64_t row = as_rows(x);
         const int M = narrow(x.size(0)), dt = dtype_code(x);
-        const size_t n = lq_fp4_linear_workspace(M, b.K, dt);
+        const size_t n = lq_fp4_linear_workspace(M, b.rows, b.K, dt);
         const Workspace ws(n, x);
         run("lq_fp4_linear", lq_fp4_linear(x.data_ptr(), row, b.codes, b.tiles, M, b.rows, b.K, glu, dt, y.data_ptr(), ws.p, n, stream()));
     }
@@ -163,7 +163,7 @@ Tensor grouped(const Tensor& xs, const Tensor& order, const Tensor& starts, cons
     Tensor out = at::empty({P, width(b, glu)}, xs.options());
     if (out.numel() && xs.size(0)) {
         const int dt = dtype_code(xs);
-        const size_t bytes = lq_fp4_experts_workspace(narrow(P), narrow(max_rows), b.stack, b.K, dt);
+        const size_t bytes = lq_fp4_experts_workspace(narrow(P), narrow(max_rows), b.stack, b.rows, b.K, dt);
         const Workspace ws(bytes, xs);
         run("lq_fp4_experts", lq_fp4_experts(xs.data_ptr(), narrow(xs.size(0)), gather_k ? o : nullptr, narrow(gather_k), s, e, n,
                                              narrow(P), narrow(max_rows), glu, b.codes, b.tiles, out.data_ptr(), b.stack, b.rows, b.K,
@@ -205,7 +205,7 @@ Tensor experts(Tensor x, Tensor inds, Tensor weights, const py::tuple& gate_up, 
     } else {
         need(P <= 1024, "at most 1024 experts a token");
     }
-    const size_t n1 = lq_fp4_experts_workspace(P, T, E, D, dt), n2 = lq_fp4_experts_workspace(P, T, E, I, dt), n = std::max(n1, n2);
+    const size_t n1 = lq_fp4_experts_workspace(P, T, E, g.rows, D, dt), n2 = lq_fp4_experts_workspace(P, T, E, D, I, dt), n = std::max(n1, n2);
     const Workspace ws(n, x);
     Tensor h = at::empty({P, I}, x.options()), ys = at::empty({P, D}, x.options());
     run("lq_fp4_experts", lq_fp4_experts(x.data_ptr(), narrow(x.size(0)), order, k, starts, ex, nseg, P, T, 1, g.codes, g.tiles,

@@ -31,6 +31,7 @@ constexpr int FP4_OUT = 8;                           // warps that write tiles o
 constexpr int FP4_THREADS = 32 * (FP4_OUT + 3);
 constexpr int FP4_MAX_STAGES = 10;
 constexpr int FP4_MAX_SEGMENTS = 1024;
+constexpr int FP4_FUSE_SMS = 148;  // (fixed, so that a workspace's size does not need the device)
 
 // A grouped call's segments in shared memory: n of them, their first rows and experts, and the tiles of tokens before each.
 struct Fp4Segments {
@@ -38,14 +39,17 @@ struct Fp4Segments {
     int32_t starts[FP4_MAX_SEGMENTS + 1], tiles[FP4_MAX_SEGMENTS + 1], experts[FP4_MAX_SEGMENTS];
 };
 
-template <int KIND_, int P_, int T_, int CG_ = 1>
+template <int KIND_, int P_, int T_, int CG_ = 1, bool FUSE_ = false>
 struct Fp4Shape {
     static constexpr int KIND = KIND_, P = P_, T = T_;
     static constexpr int CG = CG_;  // CTAs a tile: a pair has 128 rows of w and half of the tokens each
-    // Few tokens of 16 bits: four warps make the pieces in shared memory, with no kernel before this one, and a token's pieces
-    // are columns of one MMA.
-    static constexpr bool STACK = KIND == FP4_SPLIT && T <= 32;
-    static constexpr int OUT = STACK ? 4 : FP4_OUT;  // warps that write out
+    static constexpr bool STACK = KIND == FP4_SPLIT && T <= 32;  // a token's pieces are columns of one MMA
+    // Few tokens of 16 bits and no more tiles than run at once: four warps make the pieces in shared memory, with no kernel before
+    // this one (one token and 6144 x 2560: 9.2 -> 6.6 us). With more tiles each CTA makes the same pieces again (64 tokens
+    // over 64 experts: 57 us with a kernel that makes them once, 65 without).
+    static constexpr bool FUSE = FUSE_;
+    static constexpr int OUT = FUSE ? 4 : FP4_OUT;  // warps that write out
+    static constexpr int TURN = KIND == FP4_SPLIT ? 1024 : 2048;  // bytes of a warp for 16 tokens on their way (of 16 bits; 32)
     static constexpr int BK = KIND == FP4_SPLIT ? 128 : 256;     // values a stage
     static constexpr int KB = KIND == FP4_MX ? 2 : KIND == FP4_NV ? 4 : 1;  // scale tiles a stage and 128 rows
     static constexpr int NB = STACK ? 1 : P * ((T + 127) / 128);            // scale tiles of x beside each of w's
@@ -53,11 +57,11 @@ struct Fp4Shape {
     // what TMA counts of a weight tile: the bytes that it reads, also where it spreads codes to bytes
     static constexpr int A_TX = KIND == FP4_SPLIT ? A_BYTES / 2 : A_BYTES;
     static constexpr int SFA = KB * 512, SFB = KB * NB * 512;
-    static constexpr int TX = A_TX + SFA + (STACK ? 0 : B_BYTES + SFB);  // bytes that arrive for a stage (in each CTA)
+    static constexpr int TX = A_TX + SFA + (FUSE ? 0 : B_BYTES + SFB);  // bytes that arrive for a stage (in each CTA)
     static constexpr int STAGE = (A_BYTES + B_BYTES + SFA + SFB + 1023) / 1024 * 1024;
     // shared memory beside the ring (segs: of a grouped call), and the ring's stages in what is left: of the SM's 227 KB, or
     // of a half where tiles are narrow and two CTAs share it
-    static constexpr size_t beside(bool segs) { return 1024 + (2 * FP4_MAX_STAGES + 4) * 8 + 32 + OUT * 2048 + (segs ? sizeof(Fp4Segments) : 0); }
+    static constexpr size_t beside(bool segs) { return 1024 + (2 * FP4_MAX_STAGES + 4) * 8 + 32 + OUT * TURN + (segs ? sizeof(Fp4Segments) : 0); }
     static constexpr int stages(bool segs) {
         const int n = int(((T <= 32 ? 113 : 227) * 1024 - beside(segs)) / STAGE);
         return n < FP4_MAX_STAGES ? n : FP4_MAX_STAGES;
@@ -69,6 +73,7 @@ struct Fp4Shape {
     static constexpr int SF_COL = ACC == 256 ? 384 : 2 * ACC, SF_COLS = 4 * KB * (1 + NB);
     static constexpr int COLS = SF_COL + 2 * SF_COLS, TMEM = COLS <= 64 ? 64 : COLS <= 128 ? 128 : COLS <= 256 ? 256 : 512;
     static_assert(COLS <= 512 && stages(true) >= 2 && N % 16 == 0 && N <= 256 && B_TILE % 1024 == 0, "tile");
+    static_assert(!FUSE || STACK, "few tokens");
     static_assert(!STACK || N <= 128, "stacked pieces share one scale tile");
 };
 
@@ -160,7 +165,7 @@ __device__ __forceinline__ void fp4_out(const Fp4Args& a, const Fp4Tile& t, int 
 }
 
 // 16 output columns (tokens) of a warp's 32 rows of w, v[c] the sum of this lane's row and token c0 + c: turned to rows of y
-// through 2 KB of shared memory, so that a token's 32 values leave in pieces of 16 bytes. Neighbouring lanes first swap
+// through shared memory, so that a token's 32 values leave in pieces of 16 bytes. Neighbouring lanes first swap
 // columns: the even lane then has two rows of an even column, the odd lane two of an odd one. The type and form are fixed
 // here, not asked for at each value: with branches between the shuffles they ran one after another (1,670 cycles, not 150).
 template <typename O, bool GLU>
@@ -242,37 +247,6 @@ __device__ __forceinline__ void fp4_out4(const Fp4Args& a, const Fp4Tile& t, int
         if (i < some && at + i < width) fp4_store(a, first + i, o[i]);
 }
 
-// Values [k0, k0 + 8) of a row of K 16-bit values, zeros beyond it; `vec`: the row starts on a 16-byte boundary.
-template <typename T16>
-__device__ __forceinline__ uint4 load8_16(const T16* row, int k0, int K, bool vec) {
-    if (vec && k0 + 8 <= K) return *reinterpret_cast<const uint4*>(row + k0);
-    uint32_t w[4] = {};
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-        if (k0 + i < K) w[i >> 1] |= uint32_t(reinterpret_cast<const uint16_t*>(row)[k0 + i]) << (16 * (i & 1));
-    return make_uint4(w[0], w[1], w[2], w[3]);
-}
-
-// The largest magnitude of 8 values (a number that is none, if one is).
-template <typename T2>
-__device__ __forceinline__ float amax8_16(const uint4& x) {
-    const uint32_t w[4] = {x.x, x.y, x.z, x.w};
-    T2 m = __habs2(*reinterpret_cast<const T2*>(&w[0]));
-#pragma unroll
-    for (int i = 1; i < 4; ++i) m = __hmax2_nan(m, __habs2(*reinterpret_cast<const T2*>(&w[i])));
-    float lo, hi, top;
-    if constexpr (std::is_same<T2, __half2>::value) {
-        lo = __low2float(m);
-        hi = __high2float(m);
-    } else {
-        const uint32_t b = *reinterpret_cast<uint32_t*>(&m);
-        lo = __uint_as_float(b << 16);
-        hi = __uint_as_float(b & 0xFFFF0000u);
-    }
-    asm("max.NaN.f32 %0, %1, %2;" : "=f"(top) : "f"(lo), "f"(hi));
-    return top;
-}
-
 // 8 values of a group of 32 (four lanes next to one another) to P pieces of e4m3 bytes and their scale bytes. Scaled to below
 // 2^8 the values are fp16 numbers but for what lies below 2^-24 there, and the steps from piece to piece are exact in fp16.
 template <typename T16, int P>
@@ -298,7 +272,8 @@ __device__ __forceinline__ void split8(const uint4& x, uint32_t mask, uint2 (&pi
 #pragma unroll
         for (int i = 0; i < 4; ++i)
             asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(q[i]) : "r"(*reinterpret_cast<uint32_t*>(&h[i])));
-        piece[p] = make_uint2(q[0] | uint32_t(q[1]) << 16, q[2] | uint32_t(q[3]) << 16);
+        asm("mov.b32 %0, {%1, %2};" : "=r"(piece[p].x) : "h"(q[0]), "h"(q[1]));
+        asm("mov.b32 %0, {%1, %2};" : "=r"(piece[p].y) : "h"(q[2]), "h"(q[3]));
         if (p + 1 < P) {
             byte[p + 1] = byte[p] == 255 ? 255 : byte[p] < 5 ? 0 : byte[p] - 5;
             const __half2 more = __float2half2_rn(__uint_as_float(uint32_t(127 + (byte[p] == 255 ? 0 : byte[p] - byte[p + 1])) << 23));
@@ -328,8 +303,8 @@ __global__ void __launch_bounds__(FP4_THREADS, S::T <= 32 ? 2 : 1) fp4_gemm_kern
     uint64_t* acc_full = empty + NS;     // [2] the MMAs of a tile are done
     uint64_t* acc_empty = acc_full + 2;  // [2] the epilogue has read what the next tile writes
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
-    uint8_t* stage = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(tmem_slot + 1) + 15) & ~uintptr_t(15));  // 2 KB a warp
-    Fp4Segments& seg = *reinterpret_cast<Fp4Segments*>(stage + S::OUT * 2048);  // (grouped)
+    uint8_t* stage = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(tmem_slot + 1) + 15) & ~uintptr_t(15));
+    Fp4Segments& seg = *reinterpret_cast<Fp4Segments*>(stage + S::OUT * S::TURN);  // (grouped)
 
     const int warp = __shfl_sync(0xFFFFFFFFu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     const int rank = CG == 2 || a.ks > 1 ? int(cluster_ctarank()) : 0;
@@ -339,7 +314,7 @@ __global__ void __launch_bounds__(FP4_THREADS, S::T <= 32 ? 2 : 1) fp4_gemm_kern
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < NS; ++s) {
-            mbar_init(&full[s], S::STACK ? 2 : 1);
+            mbar_init(&full[s], S::FUSE ? 2 : 1);
             mbar_init(&empty[s], 1);
         }
         for (int j = 0; j < 2; ++j) {
@@ -391,7 +366,7 @@ __global__ void __launch_bounds__(FP4_THREADS, S::T <= 32 ? 2 : 1) fp4_gemm_kern
         const bool scales = warp == FP4_OUT + 2;
         if (elect_one()) {
             prefetch_tmap(scales ? &m.ws : &m.w);
-            if constexpr (!S::STACK) prefetch_tmap(scales ? &m.xs : &m.x);
+            if constexpr (!S::FUSE) prefetch_tmap(scales ? &m.xs : &m.x);
             const uint64_t pol_w = policy_evict_first(), pol_x = policy_evict_last();
             const uint32_t ring = smem_u32(smem), bars = CG == 2 ? map_peer(smem_u32(full), 0) : smem_u32(full);
             int it = 0, s = 0, turn = 0;  // stages so far, the ring's next slot, rounds of the ring
@@ -416,7 +391,7 @@ __global__ void __launch_bounds__(FP4_THREADS, S::T <= 32 ? 2 : 1) fp4_gemm_kern
                 // quantized the weights.
                 int ahead = 0;
                 if (!waited) {
-                    for (; S::KIND == FP4_SPLIT && !S::STACK && ahead < NS && s_lo + ahead < s_hi; ++ahead) {
+                    for (; S::KIND == FP4_SPLIT && !S::FUSE && ahead < NS && s_lo + ahead < s_hi; ++ahead) {
                         expect(ahead);
                         weights(s_lo + ahead, ahead);
                     }
@@ -434,7 +409,7 @@ __global__ void __launch_bounds__(FP4_THREADS, S::T <= 32 ? 2 : 1) fp4_gemm_kern
                         weights(kb, s);
                     }
                     const uint32_t st = ring + s * S::STAGE + S::A_BYTES, bar = bars + s * 8;
-                    if constexpr (S::STACK) {
+                    if constexpr (S::FUSE) {
                     } else if (!scales) {
 #pragma unroll
                         for (int p = 0; p < P; ++p)
@@ -523,7 +498,7 @@ __global__ void __launch_bounds__(FP4_THREADS, S::T <= 32 ? 2 : 1) fp4_gemm_kern
         // The warps take stages in turn, so that the loads of four stages are on their way; a lane takes 8 values of a token.
         // No more warps than the ring has stages: one that is `turns` stages on has then seen, at its last stage, the place of
         // the stage two rounds back handed over, and the parity that it waits for is not the one of two rounds before.
-        if constexpr (S::STACK) {
+        if constexpr (S::FUSE) {
             using T16 = typename std::conditional<P == 2, __nv_bfloat16, __half>::type;
             constexpr int AHEAD = 4;  // loads of a lane before it converts
             grid_dep_wait();
@@ -652,7 +627,7 @@ __global__ void __launch_bounds__(FP4_THREADS, S::T <= 32 ? 2 : 1) fp4_gemm_kern
 #pragma unroll
                         for (int q = 0; q < 16; ++q) part[(c0 + c + q) * 128 + 32 * quarter + lane] = u[q];
                     } else if (wide && nb + 32 <= a.N) {
-                        if (t.r0 + c0 + c < t.r1) fp4_out16(a, t, c0 + c, nb, u, f, stage + 2048 * warp, lane);
+                        if (t.r0 + c0 + c < t.r1) fp4_out16(a, t, c0 + c, nb, u, f, stage + S::TURN * warp, lane);
                     } else {
 #pragma unroll
                         for (int q = 0; q < 16; ++q) fp4_out<S>(a, t, c0 + c + q, n, u[q] * f);
@@ -708,7 +683,7 @@ __global__ void __launch_bounds__(FP4_THREADS, S::T <= 32 ? 2 : 1) fp4_gemm_kern
 struct SplitArgs {
     const void* x;
     int64_t x_row;
-    int rows, K, ktiles, nb, T;
+    int rows, K, ktiles, nb, T, stack;  // stack: a token's pieces as rows of one scale tile
     bool vec;
     uint8_t* pieces;  // (P, rows, Kp)
     uint8_t* tiles;   // (token tile, K tile, nb, 512)
@@ -755,7 +730,14 @@ __global__ void __launch_bounds__(256) fp4_split_kernel(const SplitArgs a) {
             tile = s0 / a.T + lo + (row - s0) / a.T;
             at = (row - s0) % a.T;
         }
-        uint8_t* tiles = a.tiles + int64_t(tile) * a.ktiles * a.nb * 512;
+        const int tile_step = a.nb * 512;
+        uint8_t *rowp[P], *scale[P];
+#pragma unroll
+        for (int p = 0; p < P; ++p) {
+            const int r = a.stack ? p * a.T + at : at, block = a.stack ? 0 : p * ((a.T + 127) / 128) + r / 128;
+            rowp[p] = a.pieces + (int64_t(p) * a.rows + row) * (words * 8);
+            scale[p] = a.tiles + int64_t(tile) * a.ktiles * tile_step + block * 512 + fp4_tile_byte(r % 128, 0);
+        }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const int word = part * 128 + 32 * i + lane;
@@ -764,12 +746,10 @@ __global__ void __launch_bounds__(256) fp4_split_kernel(const SplitArgs a) {
             int byte[P];
             split8<T16, P>(v[i], 0xFFFFFFFFu, piece, byte);
             if (word < words) {
-                const int g = word / 4;
-                uint8_t* tl = tiles + int64_t(g >> 2) * a.nb * 512;
 #pragma unroll
                 for (int p = 0; p < P; ++p) {
-                    *reinterpret_cast<uint2*>(a.pieces + (int64_t(p) * a.rows + row) * (words * 8) + 8 * word) = piece[p];
-                    if (word % 4 == 0) tl[(p * ((a.T + 127) / 128) + at / 128) * 512 + fp4_tile_byte(at % 128, g)] = uint8_t(byte[p]);
+                    *reinterpret_cast<uint2*>(rowp[p] + 8 * word) = piece[p];
+                    if (word % 4 == 0) scale[p][(word >> 4) * tile_step + (word / 4 & 3)] = uint8_t(byte[p]);
                 }
             }
         }
@@ -857,9 +837,9 @@ static int gemm_t(const Fp4Call& c, cudaStream_t st) {
     a.rtiles = (a.N + 127) / 128;
     Fp4Maps m = {};
     int rc = map_rows(&m.w, c.w, S::KIND == FP4_SPLIT, uint64_t(a.Kp) / 2, uint64_t(c.stack) * a.N, 128);
-    if (!rc && !S::STACK) rc = map_rows(&m.x, c.x, false, uint64_t(a.Kp) / (S::KIND == FP4_SPLIT ? 1 : 2), uint64_t(S::P) * a.M, S::T / S::CG);
+    if (!rc && !S::FUSE) rc = map_rows(&m.x, c.x, false, uint64_t(a.Kp) / (S::KIND == FP4_SPLIT ? 1 : 2), uint64_t(S::P) * a.M, S::T / S::CG);
     if (!rc) rc = map_scales(&m.ws, c.wt, a.ktiles, uint64_t(c.stack) * a.rtiles, S::KB, 1);
-    if (!rc && !S::STACK) rc = S::KIND == FP4_SPLIT ? map_scales(&m.xs, c.xt, S::NB, uint64_t(c.ttiles) * a.ktiles, S::NB, 1)
+    if (!rc && !S::FUSE) rc = S::KIND == FP4_SPLIT ? map_scales(&m.xs, c.xt, S::NB, uint64_t(c.ttiles) * a.ktiles, S::NB, 1)
                                        : map_scales(&m.xs, c.xt, a.ktiles, (uint64_t(a.M) + 127) / 128, S::KB, S::NB);
     if (rc) return rc;
     const int sms = device_info().sm_count;
@@ -888,7 +868,9 @@ static int gemm_t(const Fp4Call& c, cudaStream_t st) {
 }
 
 template <int KIND, int P>
-static int gemm_tokens(const Fp4Call& c, int T, cudaStream_t st) {
+static int gemm_tokens(const Fp4Call& c, int T, bool fuse, cudaStream_t st) {
+    if constexpr (KIND == FP4_SPLIT)
+        if (fuse) return T == 16 ? gemm_t<Fp4Shape<KIND, P, 16, 1, true>>(c, st) : gemm_t<Fp4Shape<KIND, P, 32, 1, true>>(c, st);
     switch (T) {
         case 16: return gemm_t<Fp4Shape<KIND, P, 16>>(c, st);
         case 32: return gemm_t<Fp4Shape<KIND, P, 32>>(c, st);
@@ -928,12 +910,12 @@ int fp4_qmm_run(const uint32_t* xc, const uint8_t* xt, const float* xf, const ui
     a.xf = xf;
     a.wf = wf;
     a.y = y;
-    return mode == LQ_MXFP4 ? gemm_tokens<FP4_MX, 1>(c, T, st) : gemm_tokens<FP4_NV, 1>(c, T, st);
+    return mode == LQ_MXFP4 ? gemm_tokens<FP4_MX, 1>(c, T, false, st) : gemm_tokens<FP4_NV, 1>(c, T, false, st);
 }
 
 // Token tiles of the rows of a call (grouped: one number a segment may go unused), and the bytes of the split's results.
 static int64_t split_tiles(int rows, int T, int segments) { return segments ? rows / T + segments : (rows + T - 1) / T; }
-static int split_blocks(int P, int T) { return P * ((T + 127) / 128); }
+static int split_blocks(int P, int T) { return T <= 32 ? 1 : P * ((T + 127) / 128); }
 static size_t split_pieces_bytes(int rows, int K, int P) { return (size_t(P) * rows * fp4_padded(K) + 511) / 512 * 512; }
 
 // Tokens a tile of rows that are dealt out to segments: twice the average, so that most segments are one tile; long segments
@@ -945,9 +927,12 @@ static int grouped_tokens(int rows, int segments, int max_rows) {
     return T > 128 && average < 1024 ? 128 : T;
 }
 
-size_t fp4_linear_workspace_bytes(int rows, int K, int dtype, int segments, int max_rows) {
+// Whether the product makes the pieces of x itself: few tokens, and all tiles run at once.
+static bool fused(int T, int64_t ttiles, int N) { return T <= 32 && ttiles * ((N + 127) / 128) <= 2 * int64_t(FP4_FUSE_SMS); }
+
+size_t fp4_linear_workspace_bytes(int rows, int N, int K, int dtype, int segments, int max_rows) {
     const int P = dtype == LQ_BF16 ? 2 : 3, T = segments ? grouped_tokens(rows, segments, max_rows) : tile_tokens(rows);
-    if (T <= 32) return 0;  // the product makes the pieces
+    if (fused(T, split_tiles(rows, T, segments), N)) return 0;
     return split_pieces_bytes(rows, K, P) +
            size_t(split_tiles(rows, T, segments)) * fp4_ktiles(K, LQ_MXFP4) * split_blocks(P, T) * 512;
 }
@@ -959,13 +944,15 @@ int fp4_linear_run(const Fp4Linear& l, cudaStream_t st) {
     SplitArgs s = {};
     s.ktiles = fp4_ktiles(l.K, LQ_MXFP4);
     const bool vec = aligned(l.x, 16) && l.x_row % 8 == 0;
-    if (T > 32) {
+    const bool fuse = fused(T, split_tiles(l.rows, T, l.segments), l.N);
+    if (!fuse) {
         s.x = l.x;
         s.x_row = l.x_row;
         s.rows = l.rows;
         s.K = l.K;
         s.nb = split_blocks(P, T);
         s.T = T;
+        s.stack = T <= 32;
         s.vec = vec;
         s.pieces = ws;
         s.tiles = ws + split_pieces_bytes(l.rows, l.K, P);
@@ -1013,7 +1000,7 @@ int fp4_linear_run(const Fp4Linear& l, cudaStream_t st) {
     a.experts = l.experts;
     a.nseg = l.nseg;
     a.max_seg = l.segments;
-    return l.dtype == LQ_BF16 ? gemm_tokens<FP4_SPLIT, 2>(c, T, st) : gemm_tokens<FP4_SPLIT, 3>(c, T, st);
+    return l.dtype == LQ_BF16 ? gemm_tokens<FP4_SPLIT, 2>(c, T, fuse, st) : gemm_tokens<FP4_SPLIT, 3>(c, T, fuse, st);
 }
 
 }  // namespace lq

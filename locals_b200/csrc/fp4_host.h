@@ -26,7 +26,7 @@ struct Fp4Linear {
     void* y;
     void* ws;
 };
-size_t fp4_linear_workspace_bytes(int rows, int K, int dtype, int segments, int max_rows);
+size_t fp4_linear_workspace_bytes(int rows, int N, int K, int dtype, int segments, int max_rows);
 int fp4_linear_run(const Fp4Linear& l, cudaStream_t st);
 
 }  // namespace lq

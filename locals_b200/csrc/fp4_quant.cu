@@ -14,56 +14,53 @@
 
 namespace lq {
 
-__device__ __forceinline__ float to_f32(uint16_t h, __nv_bfloat16) { return __uint_as_float(uint32_t(h) << 16); }
-__device__ __forceinline__ float to_f32(uint16_t h, __half) { return __half2float(*reinterpret_cast<__half*>(&h)); }
-
-// Values [k0, k0 + 8) of a row of K, zeros beyond it; `vec`: the row starts on a 16-byte boundary.
-template <typename T>
-__device__ __forceinline__ void load8(const T* row, int k0, int K, bool vec, float (&v)[8]) {
-    if (vec && k0 + 8 <= K) {
-        if constexpr (sizeof(T) == 4) {
-            const float4 a = *reinterpret_cast<const float4*>(row + k0), b = *reinterpret_cast<const float4*>(row + k0 + 4);
-            v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-            v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-        } else {
-            const uint4 a = *reinterpret_cast<const uint4*>(row + k0);
-            const uint32_t w[4] = {a.x, a.y, a.z, a.w};
-#pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = to_f32(uint16_t(w[i >> 1] >> (16 * (i & 1))), T());
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            if (k0 + i >= K)
-                v[i] = 0.f;
-            else if constexpr (sizeof(T) == 4)
-                v[i] = row[k0 + i];
-            else
-                v[i] = to_f32(reinterpret_cast<const uint16_t*>(row)[k0 + i], T());
-        }
-    }
-}
-
-// The largest magnitude of 8 values; not a number if one of them is.
+// The largest magnitude of a and b; not a number if one of them is none.
 __device__ __forceinline__ float amax_nan(float a, float b) {
     float d;
     asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
     return d;
 }
 
-__device__ __forceinline__ float amax8(const float (&v)[8]) {
-    float m = fabsf(v[0]);
+// Values [k0, k0 + 8) of a row of K, zeros beyond it, as they lie in memory; `vec`: the row starts on a 16-byte boundary.
+template <typename T>
+struct Eight {
+    uint4 q;
+    __device__ __forceinline__ void load(const T* row, int k0, int K, bool vec) { q = load8_16(row, k0, K, vec); }
+    __device__ __forceinline__ float amax() const {
+        return amax8_16<typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type>(q);
+    }
+    __device__ __forceinline__ void times(float f, float (&v)[8]) const {
+        const uint32_t w[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
-    for (int i = 1; i < 8; ++i) m = amax_nan(m, fabsf(v[i]));
-    return m;
-}
-
-__device__ __forceinline__ uint32_t codes8(const float (&v)[8]) {
-    uint32_t w = 0;
+        for (int i = 0; i < 4; ++i) {
+            v[2 * i] = F16Traits<T>::to_f32(w[i] & 0xFFFFu) * f;
+            v[2 * i + 1] = F16Traits<T>::to_f32(w[i] >> 16) * f;
+        }
+    }
+};
+template <>
+struct Eight<float> {
+    float x[8];
+    __device__ __forceinline__ void load(const float* row, int k0, int K, bool vec) {
+        if (vec && k0 + 8 <= K) {
+            *reinterpret_cast<float4*>(x) = *reinterpret_cast<const float4*>(row + k0);
+            *reinterpret_cast<float4*>(x + 4) = *reinterpret_cast<const float4*>(row + k0 + 4);
+        } else {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) w |= cvt_e2m1x2(v[2 * i + 1], v[2 * i]) << (8 * i);
-    return w;
-}
+            for (int i = 0; i < 8; ++i) x[i] = k0 + i < K ? row[k0 + i] : 0.f;
+        }
+    }
+    __device__ __forceinline__ float amax() const {
+        float m = fabsf(x[0]);
+#pragma unroll
+        for (int i = 1; i < 8; ++i) m = amax_nan(m, fabsf(x[i]));
+        return m;
+    }
+    __device__ __forceinline__ void times(float f, float (&v)[8]) const {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = x[i] * f;
+    }
+};
 
 // The e4m3 byte nearest to t >= 0 (ties to even), at most 448.
 __device__ __forceinline__ uint32_t e4m3_of(double t) {
@@ -94,16 +91,17 @@ __global__ void __launch_bounds__(256) fp4_quantize_kernel(const T* __restrict__
     for (int64_t u = (int64_t(blockIdx.x) * blockDim.x + threadIdx.x) >> 5; u < tasks; u += (int64_t(gridDim.x) * blockDim.x) >> 5) {
         const int row = int(u / parts), w0 = int(u - int64_t(row) * parts) * 32 * UNR + lane;
         const T* src = x + int64_t(row) * x_row;
-        float vs[UNR][8];
+        uint32_t* codes_row = codes + int64_t(row) * words;
+        uint8_t* tiles_row = tiles + int64_t(row >> 7) * ktiles * 512 + fp4_tile_byte(row & 127, 0);
+        Eight<T> x8[UNR];
 #pragma unroll
         for (int i = 0; i < UNR; ++i)  // (beyond the row: zeros)
-            load8(src, 8 * (w0 + 32 * i), K, vec, vs[i]);
+            x8[i].load(src, 8 * (w0 + 32 * i), K, vec);
 #pragma unroll
         for (int i = 0; i < UNR; ++i) {
             const int word = w0 + 32 * i;
             if (word - lane >= words) break;  // (rows are a multiple of 16 words: half a warp may be beyond)
-            float(&v)[8] = vs[i];
-            float top = amax8(v);
+            float v[8], top = x8[i].amax();
 #pragma unroll
             for (int d = 1; d < LANES; d *= 2) top = amax_nan(top, __shfl_xor_sync(0xFFFFFFFFu, top, d));
             uint32_t byte, w;
@@ -111,8 +109,7 @@ __global__ void __launch_bounds__(256) fp4_quantize_kernel(const T* __restrict__
                 const uint32_t e = __float_as_uint(top) >> 23 & 0xFF;
                 byte = e == 255 ? 255u : e < 2 ? 0u : e - 2;
                 const float up = __uint_as_float((254u - (byte == 255 ? 127u : byte)) << 23);
-#pragma unroll
-                for (int q = 0; q < 8; ++q) v[q] *= up;
+                x8[i].times(up, v);
                 w = codes8(v);
             } else {
                 byte = top == INFINITY ? 0x7Fu : e4m3_of(double(top) / (6.0 * double(f)));
@@ -122,26 +119,26 @@ __global__ void __launch_bounds__(256) fp4_quantize_kernel(const T* __restrict__
                     const double sf = double(s) * double(f);
                     const float r = __frcp_rn(float(sf));
                     float lo[8], hi[8];
+                    x8[i].times(r, v);
 #pragma unroll
                     for (int q = 0; q < 8; ++q) {
-                        const float t = v[q] * r;
-                        lo[q] = t * (1.f - 0x1p-20f);
-                        hi[q] = t * (1.f + 0x1p-20f);
+                        lo[q] = v[q] * (1.f - 0x1p-20f);
+                        hi[q] = v[q] * (1.f + 0x1p-20f);
                     }
                     w = codes8(lo);
                     // (the reciprocal of a factor near the ends of the range is no normal number: 64 bits then)
                     if (w != codes8(hi) || !(r > 0x1p-126f && r < 0x1p127f)) {
                         w = 0;
+                        x8[i].times(1.f, v);
 #pragma unroll
                         for (int q = 0; q < 8; ++q) w |= code_exact(v[q], sf) << (4 * q);
                     }
                 }
             }
             if (word >= words) continue;
-            codes[int64_t(row) * words + word] = w;
+            codes_row[word] = w;
             const int g = word / LANES;
-            if (word % LANES == 0)
-                tiles[(int64_t(row >> 7) * ktiles + (g >> 2)) * 512 + fp4_tile_byte(row & 127, g)] = uint8_t(byte);
+            if (word % LANES == 0) tiles_row[(g >> 2) * 512 + (g & 3)] = uint8_t(byte);
         }
     }
 }
@@ -202,11 +199,31 @@ __global__ void __launch_bounds__(256) fp4_dequantize_kernel(const uint32_t* __r
 #pragma unroll
         for (int i = 0; i < UNR; ++i) {
             const int word = w0 + 32 * i;
-            if (word >= words) break;
+            if (word - lane >= words) break;
             const float s = fp4_scale_value(byte[i], MODE);
-            T* dst = out + at * K + 8 * word;
             float a[8];
             values8(w[i], a);
+            if constexpr (sizeof(T) == 4) {
+                // two lanes a word, 16 bytes each, so that a store fills whole sectors (72 -> 50 us for 14336 x 4096)
+                if (vec) {
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const int from = 16 * h + lane / 2;
+                        float4 q;
+                        float* qp = &q.x;
+#pragma unroll
+                        for (int c = 0; c < 4; ++c) {
+                            const float lo = __shfl_sync(0xFFFFFFFFu, a[c] * s * f, from), hi = __shfl_sync(0xFFFFFFFFu, a[4 + c] * s * f, from);
+                            qp[c] = lane & 1 ? hi : lo;
+                        }
+                        const int at8 = w0 - lane + 32 * i + from;
+                        if (at8 < words) *reinterpret_cast<float4*>(out + at * K + 8 * at8 + 4 * (lane & 1)) = q;
+                    }
+                    continue;
+                }
+            }
+            if (word >= words) break;
+            T* dst = out + at * K + 8 * word;
             alignas(16) T v[8];
 #pragma unroll
             for (int q = 0; q < 8; ++q) v[q] = from_f32<T>(a[q] * s * f);

@@ -159,7 +159,7 @@ __global__ void group_kernel(const uint32_t* inds, int P, int E, int32_t* order,
 // places its pairs in pair order (a match over each 32 pairs ranks equal experts by lane). Pair p of expert e lands
 // after every earlier pair of e, exactly as in group_kernel: the same order, starts, experts and pos.
 constexpr int GROUP_PAR_MAX_E = 1024;
-constexpr int GROUP_CLUSTER_MIN_P = 2049;  // from here a cluster of 8 CTAs (16,004 pairs 36 -> 9 us; 2,048 pairs 6.9 in one)
+constexpr int GROUP_CLUSTER_MIN_P = 2049;  // from here a cluster of 8 CTAs (16,004 pairs 36 -> 10 us; 2,048 pairs 6.9 in one)
 
 __global__ void __launch_bounds__(1024) group_par_kernel(const uint32_t* inds, int P, int E, int32_t* order,
                                                          int32_t* starts, int32_t* experts, int32_t* nseg,
@@ -306,7 +306,7 @@ __global__ void combine_kernel(const uint16_t* ys, const float* w, const int32_t
 }
 
 // The same sums in the same order, 8 neighbouring columns a thread (D a multiple of 8, rows on 16-byte boundaries):
-// 16,004 slots of 2,048 columns 48 -> 14 us (one column a thread reads 2 bytes at a time).
+// 16,004 slots of 2,048 columns 48 -> 16 us (one column a thread reads 2 bytes at a time).
 __global__ void __launch_bounds__(256) combine8_kernel(const uint4* ys, const float* w, const int32_t* pos, uint4* y, int T, int k,
                                                        int D8, int dt) {
     grid_dep_wait();

@@ -86,13 +86,13 @@ def test_abi_refusals():
     m = lambda x=OK, M=4, N=6, K=64, mode=E.NVFP4, glu=0, dt=E.BF16, y=OK: L.lq_fp4_qmm(x, OK, None, OK, OK, None, M, N, K, mode, glu, dt, y, None)  # noqa: E731
     assert m(x=None) == E.LQ_E_ARG and m(dt=9) == E.LQ_E_ARG and m(M=0) == E.LQ_E_SHAPE and m(N=0) == E.LQ_E_SHAPE
     assert m(N=7, glu=1) == E.LQ_E_SHAPE and m(mode=-1) == E.LQ_E_UNSUPPORTED and m(x=BAD) == E.LQ_E_ALIGN
-    n = L.lq_fp4_linear_workspace(100, 64, E.BF16)
-    assert n > 0 and L.lq_fp4_linear_workspace(4, 64, E.BF16) == 0 and L.lq_fp4_linear_workspace(4, 64, E.F32) == 0 and L.lq_fp4_linear_workspace(0, 64, E.BF16) == 0
+    n = L.lq_fp4_linear_workspace(100, 6, 64, E.BF16)
+    assert n > 0 and L.lq_fp4_linear_workspace(4, 6, 64, E.BF16) == 0 and L.lq_fp4_linear_workspace(100, 6, 64, E.F32) == 0 and L.lq_fp4_linear_workspace(0, 6, 64, E.BF16) == 0
     li = lambda x=OK, row=64, M=100, dt=E.BF16, ws=OK, b=n: L.lq_fp4_linear(x, row, OK, OK, M, 6, 64, 0, dt, OK, ws, b, None)  # noqa: E731
     assert li(x=None) == E.LQ_E_ARG and li(dt=E.F32) == E.LQ_E_ARG and li(ws=None) == E.LQ_E_ARG
     assert li(b=n - 1) == E.LQ_E_SHAPE and li(row=60) == E.LQ_E_SHAPE and li(ws=BAD) == E.LQ_E_ALIGN
-    n = L.lq_fp4_experts_workspace(800, 400, 8, 64, E.BF16)
-    assert n > 0 and L.lq_fp4_experts_workspace(8, 4, 16, 64, E.BF16) == 0
+    n = L.lq_fp4_experts_workspace(800, 400, 8, 6, 64, E.BF16)
+    assert n > 0 and L.lq_fp4_experts_workspace(8, 4, 16, 6, 64, E.BF16) == 0
     ex = lambda order=None, k=0, rows=800, st=OK, ns=OK, P=800, E_=8, b=n: L.lq_fp4_experts(OK, rows, order, k, st, OK, ns, P, 400, 0, OK, OK, OK, E_, 6, 64, E.BF16, OK, b, None)  # noqa: E731
     assert ex(order=OK) == E.LQ_E_ARG and ex(k=-1) == E.LQ_E_ARG and ex(st=None) == E.LQ_E_ARG
     assert ex(rows=799) == E.LQ_E_SHAPE and ex(k=2, rows=399) == E.LQ_E_SHAPE and ex(b=n - 1) == E.LQ_E_SHAPE and ex(E_=0) == E.LQ_E_SHAPE

@@ -461,7 +461,7 @@ def test_grouped_leaves_padding_segments_alone(cuda):
     order, starts, experts_, nseg, pos = moe.group_range(inds, 2, 3)
     P = T * k
     out = torch.full((P, N), 5.0, device=cuda, dtype=torch.bfloat16)
-    n = _lib.lib().lq_fp4_experts_workspace(P, T, 3, D, _lib.BF16)
+    n = _lib.lib().lq_fp4_experts_workspace(P, T, 3, N, D, _lib.BF16)
     ws = torch.empty(n, dtype=torch.uint8, device=cuda)
     _lib.call("lq_fp4_experts", x.data_ptr(), T, order.data_ptr(), k, starts.data_ptr(), experts_.data_ptr(), nseg.data_ptr(), P, T, 0,
               w.codes.data_ptr(), w.tiles.data_ptr(), out.data_ptr(), 3, N, D, _lib.BF16, ws.data_ptr(), n, _stream())
@@ -485,7 +485,7 @@ def test_experts_out_of_range_are_recorded_and_left_out(cuda):
     w, wv = _weights(cuda, g, 64, 128, "mxfp4", 3)
     x = torch.randn((2, 128), generator=g, device=cuda).to(torch.bfloat16)
     out = torch.full((4, 64), 5.0, device=cuda, dtype=torch.bfloat16)
-    n = _lib.lib().lq_fp4_experts_workspace(4, 2, 3, 128, _lib.BF16)
+    n = _lib.lib().lq_fp4_experts_workspace(4, 2, 3, 64, 128, _lib.BF16)
     ws = torch.empty(n, dtype=torch.uint8, device=cuda)
     ids = torch.tensor([1, -7, 1 << 20, 2], dtype=torch.int32, device=cuda)
     order = torch.tensor([0, 1, 2, 90], dtype=torch.int32, device=cuda)  # the last names a row that x does not have
