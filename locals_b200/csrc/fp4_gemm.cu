@@ -77,13 +77,16 @@ struct Fp4Shape {
         return n < FP4_MAX_STAGES ? n : FP4_MAX_STAGES;
     }
     static constexpr int N = STACK ? P * T : T;
-    static constexpr int ACC = N <= 32 ? 32 : N <= 64 ? 64 : N <= 128 ? 128 : 256;
+    static constexpr int ACC = N <= 32 ? 32 : N <= 64 ? 64 : N <= 96 ? 96 : N <= 128 ? 128 : 256;
     // 256 columns: the two accumulators share 128, which are read out first
     static constexpr int ACC_STEP = ACC == 256 ? 128 : ACC;
     static constexpr int SF_COL = ACC == 256 ? 384 : 2 * ACC, SF_COLS = 4 * KB * (1 + NB);
     static constexpr int COLS = SF_COL + 2 * SF_COLS, TMEM = COLS <= 64 ? 64 : COLS <= 128 ? 128 : COLS <= 256 ? 256 : 512;
     static_assert(COLS <= 512 && stages(true) >= 2 && N % 16 == 0 && N <= 256 && B_TILE % 1024 == 0, "tile");
     static_assert(!FUSE || STACK, "few tokens");
+    // Two CTAs of an SM both have their tensor memory: one that waited for the other's could hold up a cluster whose CTAs wait
+    // for one another at their join, and that cluster the other's.
+    static_assert(T > 32 || TMEM <= 256, "two CTAs an SM");
     static_assert(!STACK || N <= 128, "stacked pieces share one scale tile");
 };
 
@@ -334,7 +337,6 @@ __global__ void __launch_bounds__(FP4_THREADS, S::T <= 32 ? 2 : 1) fp4_gemm_kern
         fence_barrier_init();
     }
     if (warp == FP4_OUT + 1) tc_alloc<CG>(tmem_slot, S::TMEM);
-    grid_dep_launch();
     if (a.grouped) {
         grid_dep_wait();
         const int n = a.nseg ? min(max(*a.nseg, 0), a.max_seg) : a.M;  // without segments, each row is one
@@ -367,6 +369,7 @@ __global__ void __launch_bounds__(FP4_THREADS, S::T <= 32 ? 2 : 1) fp4_gemm_kern
     else
         __syncthreads();
     tc_fence_after();
+    grid_dep_launch();  // this CTA has its tensor memory: the next kernel's may wait for theirs
     const uint32_t tmem = *tmem_slot;
     const int ntiles = a.grouped ? seg.tiles[seg.n] * a.ntn : a.ntiles;
     bool ok = true;

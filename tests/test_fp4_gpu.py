@@ -669,3 +669,26 @@ def test_combine_keeps_its_order_of_sums(cuda, dtype, T, k, D):
             acc = (rows.double() * w[:, r, None].double() + acc.double()).float()
         assert torch.equal(moe.combine(ys, w, pos), acc.to(_dt(dtype)))
     _ok(cuda)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("M", [1, 16, 17, 24, 32])
+def test_split_sums_of_narrow_tiles_on_two_streams(cuda, dtype, M):
+    """Clusters that split K, two CTAs an SM: each has its tensor memory, whatever runs beside it."""
+    import torch
+    from locals_b200 import fp4
+
+    g = _gen(cuda, M)
+    shapes = [(6144, 2560), (4096, 4096), (2048, 768), (14336, 1024)]
+    ws = [_weights(cuda, g, n, k, "mxfp4")[0] for n, k in shapes]
+    xs = [torch.randn((M, k), generator=g, device=cuda).to(_dt(dtype)) for _, k in shapes]
+    want = [fp4.matmul(x, w) for x, w in zip(xs, ws)]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in range(2)], []
+    for _ in range(30):
+        for s in streams:
+            with torch.cuda.stream(s):
+                got.append([fp4.matmul(x, w) for x, w in zip(xs, ws)])
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for r in got for a, b in zip(r, want))
+    _ok(cuda)
