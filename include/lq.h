@@ -354,6 +354,17 @@ int lq_fp4_experts(const void* x, int x_rows, const int32_t* gather_order, int g
                    const uint8_t* tiles, void* out, int E, int N, int K, int dtype, void* workspace,
                    size_t workspace_bytes, void* stream);
 
+/* The routed mxfp4 experts of a step and their weighted sum, y (T, D) = sum over slots r of weights[t, r] * down_e .
+ * (silu(gate_e . x[t]) * (up_e . x[t])) with e = inds[t, r]: lq_moe_group, two grouped products and the combine in one call. The
+ * hidden rows and the experts' outputs are held in 32 bits (the former enter the down product in three pieces of e4m3, off by at most
+ * 2^-14 of a value, or 2^-27 of the largest of its group of 32); y is rounded once. x (T, D), y f16 / bf16; inds and weights (T, k);
+ * gate_up (E, 2 I, D) with gate and up rows in turn, down (E, D, I) as lq_fp4_experts; at most 1024 experts or T * k pairs, whichever is
+ * less (T 1: k pairs). workspace: lq_fp4_moe_workspace(T, k, E, D, I, dtype) bytes (0: sizes that are refused), 256-byte aligned. */
+size_t lq_fp4_moe_workspace(int T, int k, int E, int D, int I, int dtype);
+int lq_fp4_moe(const void* x, const int32_t* inds, const float* weights, const uint32_t* gate_up_codes,
+               const uint8_t* gate_up_tiles, const uint32_t* down_codes, const uint8_t* down_tiles, void* y, int T, int k, int E,
+               int D, int I, int dtype, void* workspace, size_t workspace_bytes, void* stream);
+
 /* The column-sharded prefill with its own all-gather: this rank's N output columns of y = x . dequant(w)^T (the
  * dense path of lq_qmm_dense) are written by the GEMM in place at columns [col_off, col_off + N) of dst[0], this GPU's
  * row-major (M, ldo) buffer, then copied by one kernel of plain 16-byte peer stores into the same columns of

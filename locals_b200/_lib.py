@@ -81,6 +81,8 @@ SIGNATURES = {
     "lq_fp4_experts_workspace": ([_i, _i, _i, _i, _i, _i], ctypes.c_size_t),
     "lq_fp4_experts": ([_vp, _i, _vp, _i, _vp, _vp, _vp, _i, _i, _i, _u32p, _vp, _vp, _i, _i, _i, _i, _vp,
                         ctypes.c_size_t, _vp], _i),
+    "lq_fp4_moe_workspace": ([_i, _i, _i, _i, _i, _i], ctypes.c_size_t),
+    "lq_fp4_moe": ([_vp, _vp, _vp, _u32p, _vp, _u32p, _vp, _vp, _i, _i, _i, _i, _i, _i, _vp, ctypes.c_size_t, _vp], _i),
     "lq_supported": ([_i, _i, _i, _i, _i, _i, _i], _i),
     "lq_list_configs": ([_i, _i, _i, _i, _i, _i, ctypes.POINTER(Cfg), _i], _i),
     "lq_device_status": ([_i], ctypes.c_uint),

@@ -90,6 +90,59 @@ __device__ __forceinline__ float amax8_16(const uint4& x) {
     return top;
 }
 
+// The largest magnitude of a and b; not a number if one of them is none.
+__device__ __forceinline__ float amax_nan(float a, float b) {
+    float d;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+    return d;
+}
+
+// Values [k0, k0 + 8) of a row of K, zeros beyond it, as they lie in memory; `vec`: the row starts on a 16-byte boundary.
+template <typename T>
+struct Eight {
+    uint4 q;
+    __device__ __forceinline__ void load(const T* row, int k0, int K, bool vec) { q = load8_16(row, k0, K, vec); }
+    __device__ __forceinline__ void zero() { q = make_uint4(0, 0, 0, 0); }
+    __device__ __forceinline__ float amax() const {
+        return amax8_16<typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type>(q);
+    }
+    __device__ __forceinline__ void times(float f, float (&v)[8]) const {
+        const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            v[2 * i] = F16Traits<T>::to_f32(w[i] & 0xFFFFu) * f;
+            v[2 * i + 1] = F16Traits<T>::to_f32(w[i] >> 16) * f;
+        }
+    }
+};
+template <>
+struct Eight<float> {
+    float x[8];
+    __device__ __forceinline__ void load(const float* row, int k0, int K, bool vec) {
+        if (vec && k0 + 8 <= K) {
+            *reinterpret_cast<float4*>(x) = *reinterpret_cast<const float4*>(row + k0);
+            *reinterpret_cast<float4*>(x + 4) = *reinterpret_cast<const float4*>(row + k0 + 4);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[i] = k0 + i < K ? row[k0 + i] : 0.f;
+        }
+    }
+    __device__ __forceinline__ void zero() {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = 0.f;
+    }
+    __device__ __forceinline__ float amax() const {
+        float m = fabsf(x[0]);
+#pragma unroll
+        for (int i = 1; i < 8; ++i) m = amax_nan(m, fabsf(x[i]));
+        return m;
+    }
+    __device__ __forceinline__ void times(float f, float (&v)[8]) const {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = x[i] * f;
+    }
+};
+
 // One lane of a whole warp, chosen in a way that the compiler knows to be uniform: tcgen05 and TMA instructions take their
 // operands from uniform registers, and behind `lane == 0` each operand is moved there one by one (70 cycles a tcgen05.cp and
 // 55 to 70 a small MMA; 20 and 45 behind this).

@@ -88,7 +88,7 @@ int lq_fp4_linear(const void* x, int64_t x_row, const uint32_t* codes, const uin
     l.N = N;
     l.K = K;
     l.glu = glu;
-    l.dtype = dtype;
+    l.x_dtype = l.dtype = dtype;
     l.y = y;
     l.ws = workspace;
     return finish(fp4_linear_run(l, reinterpret_cast<cudaStream_t>(stream)));
@@ -96,11 +96,15 @@ int lq_fp4_linear(const void* x, int64_t x_row, const uint32_t* codes, const uin
 
 static int fp4_segments(int P, int E) { return P < E + 1 ? P : E + 1; }
 
+static size_t fp4_grouped_bytes(int P, int max_rows, int E, int N, int K, int x_dtype) {
+    const size_t some = fp4_linear_workspace_bytes(P, N, K, x_dtype, fp4_segments(P, E), max_rows);
+    const size_t each = P <= 1024 ? fp4_linear_workspace_bytes(P, N, K, x_dtype, P, max_rows) : 0;  // without segments
+    return some > each ? some : each;
+}
+
 size_t lq_fp4_experts_workspace(int P, int max_rows, int E, int N, int K, int dtype) {
     if (fp4_rows_ok(P, K, LQ_MXFP4) || fp4_rows_ok(N, K, LQ_MXFP4) || !is16(dtype) || E < 1 || max_rows < 1) return 0;
-    const size_t some = fp4_linear_workspace_bytes(P, N, K, dtype, fp4_segments(P, E), max_rows);
-    const size_t each = P <= 1024 ? fp4_linear_workspace_bytes(P, N, K, dtype, P, max_rows) : 0;  // without segments
-    return some > each ? some : each;
+    return fp4_grouped_bytes(P, max_rows, E, N, K, dtype);
 }
 
 int lq_fp4_experts(const void* x, int x_rows, const int32_t* gather_order, int gather_k, const int32_t* starts,
@@ -139,10 +143,108 @@ int lq_fp4_experts(const void* x, int x_rows, const int32_t* gather_order, int g
     l.N = N;
     l.K = K;
     l.glu = glu;
-    l.dtype = dtype;
+    l.x_dtype = l.dtype = dtype;
     l.y = out;
     l.ws = workspace;
     return finish(fp4_linear_run(l, reinterpret_cast<cudaStream_t>(stream)));
+}
+
+// Where the parts of lq_fp4_moe's workspace lie, in bytes: hidden rows and experts' outputs in 32 bits, the grouping (from two
+// tokens on), the workspace of the two products in turn.
+struct MoeParts {
+    size_t hidden, outputs, group, product, all;
+    int segments;
+};
+
+static int fp4_moe_parts(int T, int k, int E, int D, int I, int dtype, MoeParts& m) {
+    if (!is16(dtype)) return LQ_E_ARG;
+    if (T < 1 || k < 1 || E < 1 || int64_t(T) * k > (1 << 29) || I > (1 << 28)) return LQ_E_SHAPE;
+    const int P = T * k;
+    int rc = fp4_rows_ok(int64_t(E) * 2 * I, D, LQ_MXFP4);
+    if (!rc) rc = fp4_rows_ok(int64_t(E) * D, I, LQ_MXFP4);
+    if (rc) return rc;
+    m.segments = T > 1 && E < P ? E : P;
+    if (m.segments > 1024) return LQ_E_SHAPE;
+    auto whole = [](size_t bytes) { return (bytes + 255) / 256 * 256; };
+    m.hidden = 0;
+    m.outputs = m.hidden + whole(size_t(P) * I * sizeof(float));
+    m.group = m.outputs + whole(size_t(P) * D * sizeof(float));
+    m.product = m.group + (T > 1 ? whole((2 * size_t(P) + 2 * m.segments + 2) * sizeof(int32_t)) : 0);
+    const size_t up = fp4_grouped_bytes(P, T, E, 2 * I, D, dtype), down = fp4_grouped_bytes(P, T, E, D, I, LQ_F32);
+    m.all = m.product + whole(up > down ? up : down);
+    return LQ_OK;
+}
+
+size_t lq_fp4_moe_workspace(int T, int k, int E, int D, int I, int dtype) {
+    MoeParts m;
+    return fp4_moe_parts(T, k, E, D, I, dtype, m) ? 0 : m.all;
+}
+
+int lq_fp4_moe(const void* x, const int32_t* inds, const float* weights, const uint32_t* gate_up_codes,
+               const uint8_t* gate_up_tiles, const uint32_t* down_codes, const uint8_t* down_tiles, void* y, int T, int k, int E,
+               int D, int I, int dtype, void* workspace, size_t workspace_bytes, void* stream) {
+    if (!x || !inds || !weights || !gate_up_codes || !gate_up_tiles || !down_codes || !down_tiles || !y || !workspace) return LQ_E_ARG;
+    MoeParts m;
+    int rc = fp4_moe_parts(T, k, E, D, I, dtype, m);
+    if (rc) return rc;
+    if (workspace_bytes < m.all) return LQ_E_SHAPE;
+    if (!aligned(gate_up_codes, 32) || !aligned(down_codes, 32) || !aligned(gate_up_tiles, 16) || !aligned(down_tiles, 16) ||
+        !aligned(workspace, 256) || !aligned(x, 2) || !aligned(y, 2) || !aligned(inds, 4) || !aligned(weights, 4))
+        return LQ_E_ALIGN;
+    rc = check_device();
+    if (rc) return rc;
+    const cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+    const int P = T * k;
+    uint8_t* ws = static_cast<uint8_t*>(workspace);
+    float *h = reinterpret_cast<float*>(ws + m.hidden), *ys = reinterpret_cast<float*>(ws + m.outputs);
+    int32_t *order = nullptr, *pos = nullptr;
+    Fp4Linear l = {};
+    l.experts = inds;  // one token: each slot is a segment of its own
+    if (T > 1) {
+        order = reinterpret_cast<int32_t*>(ws + m.group);
+        pos = order + P;
+        int32_t *starts = pos + P, *experts = starts + m.segments + 1, *nseg = experts + m.segments;
+        rc = group_run(reinterpret_cast<const uint32_t*>(inds), P, E, order, starts, experts, nseg, pos, st);
+        if (rc) return finish(rc);
+        l.starts = starts;
+        l.experts = experts;
+        l.nseg = nseg;
+    }
+    l.segments = m.segments;
+    l.max_rows = T;
+    l.E = E;
+    l.rows = P;
+    l.ws = ws + m.product;
+    l.x = x;  // gate and up: 16-bit tokens to 32-bit hidden rows
+    l.x_row = D;
+    l.x_dtype = dtype;
+    l.order = order;
+    l.gather = k;
+    l.src_rows = T;
+    l.wc = gate_up_codes;
+    l.wt = gate_up_tiles;
+    l.N = 2 * I;
+    l.K = D;
+    l.glu = 1;
+    l.dtype = LQ_F32;
+    l.y = h;
+    rc = fp4_linear_run(l, st);
+    if (rc) return finish(rc);
+    l.x = h;  // down: 32-bit hidden rows to 32-bit outputs
+    l.x_row = I;
+    l.x_dtype = LQ_F32;
+    l.order = nullptr;
+    l.gather = 0;
+    l.src_rows = P;
+    l.wc = down_codes;
+    l.wt = down_tiles;
+    l.N = D;
+    l.K = I;
+    l.glu = 0;
+    l.y = ys;
+    rc = fp4_linear_run(l, st);
+    if (rc) return finish(rc);
+    return finish(combine_f32_run(ys, weights, pos, y, T, k, D, dtype, st));
 }
 
 }  // extern "C"

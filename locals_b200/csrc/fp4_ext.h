@@ -172,8 +172,7 @@ Tensor grouped(const Tensor& xs, const Tensor& order, const Tensor& starts, cons
     return out;
 }
 
-// The routed experts of a step, and their weighted sum: group, gate and up, down, combine. One token's experts are each
-// a segment of their own, and need no grouping.
+// The routed experts of a step, and their weighted sum.
 Tensor experts(Tensor x, Tensor inds, Tensor weights, const py::tuple& gate_up, const py::tuple& down) {
     const Operand g = operand(gate_up, 3), d = operand(down, 3);
     need(x.dim() == 2 && inds.dim() == 2 && inds.size(0) == x.size(0), "x (T, D) and inds (T, k) are wanted");
@@ -187,32 +186,13 @@ Tensor experts(Tensor x, Tensor inds, Tensor weights, const py::tuple& gate_up, 
     x = x.contiguous();
     inds = inds.contiguous();
     weights = weights.contiguous();
-    const int T = narrow(x.size(0)), k = narrow(inds.size(1)), P = narrow(int64_t(T) * k), E = g.stack, D = g.K, I = d.K, dt = dtype_code(x);
-    if (P == 0) return at::zeros(x.sizes(), x.options());
+    const int T = narrow(x.size(0)), k = narrow(inds.size(1)), E = g.stack, D = g.K, I = d.K, dt = dtype_code(x);
+    if (T == 0 || k == 0) return at::zeros(x.sizes(), x.options());
     Tensor y = at::empty({T, D}, x.options());
-    const int S = std::min(E, P);
-    Tensor ints;
-    int32_t *order = nullptr, *pos = nullptr, *starts = nullptr, *nseg = nullptr, *ex = static_cast<int32_t*>(inds.data_ptr());
-    void* st = stream();
-    if (T > 1) {
-        ints = at::empty({int64_t(2) * P + 2 * S + 2}, x.options().dtype(at::kInt));
-        order = ints.data_ptr<int32_t>();
-        pos = order + P;
-        starts = pos + P;
-        ex = starts + S + 1;
-        nseg = ex + S;
-        run("lq_moe_group", lq_moe_group(static_cast<const uint32_t*>(inds.data_ptr()), P, E, order, starts, ex, nseg, pos, st));
-    } else {
-        need(P <= 1024, "at most 1024 experts a token");
-    }
-    const size_t n1 = lq_fp4_experts_workspace(P, T, E, g.rows, D, dt), n2 = lq_fp4_experts_workspace(P, T, E, D, I, dt), n = std::max(n1, n2);
+    const size_t n = lq_fp4_moe_workspace(T, k, E, D, I, dt);
     const Workspace ws(n, x);
-    Tensor h = at::empty({P, I}, x.options()), ys = at::empty({P, D}, x.options());
-    run("lq_fp4_experts", lq_fp4_experts(x.data_ptr(), narrow(x.size(0)), order, k, starts, ex, nseg, P, T, 1, g.codes, g.tiles,
-                                         h.data_ptr(), E, g.rows, D, dt, ws.p, n, st));
-    run("lq_fp4_experts", lq_fp4_experts(h.data_ptr(), P, nullptr, 0, starts, ex, nseg, P, T, 0, d.codes, d.tiles, ys.data_ptr(), E, D, I, dt,
-                                         ws.p, n, st));
-    run("lq_moe_combine", lq_moe_combine(ys.data_ptr(), weights.data_ptr<float>(), pos, y.data_ptr(), T, k, D, dt, st));
+    run("lq_fp4_moe", lq_fp4_moe(x.data_ptr(), static_cast<const int32_t*>(inds.data_ptr()), weights.data_ptr<float>(), g.codes, g.tiles,
+                                 d.codes, d.tiles, y.data_ptr(), T, k, E, D, I, dt, ws.p, n, stream()));
     return y;
 }
 

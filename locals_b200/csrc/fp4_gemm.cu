@@ -49,17 +49,19 @@ struct Fp4Segments {
     int32_t starts[FP4_MAX_SEGMENTS + 1], tiles[FP4_MAX_SEGMENTS + 1], experts[FP4_MAX_SEGMENTS];
 };
 
-template <int KIND_, int P_, int T_, int CG_ = 1, bool FUSE_ = false>
+// X_: the type of x where the product makes its pieces itself, else void.
+template <int KIND_, int P_, int T_, int CG_ = 1, typename X_ = void>
 struct Fp4Shape {
+    using X = X_;
     static constexpr int KIND = KIND_, P = P_, T = T_;
     static constexpr int CG = CG_;  // CTAs a tile: a pair has 128 rows of w and half of the tokens each
     static constexpr bool STACK = KIND == FP4_SPLIT && T <= 32;  // a token's pieces are columns of one MMA
     // Few tokens of 16 bits and no more tiles than run at once: four warps make the pieces in shared memory, with no kernel before
     // this one (one token and 6144 x 2560: 9.2 -> 6.6 us). With more tiles each CTA makes the same pieces again (64 tokens
     // over 64 experts: 57 us with a kernel that makes them once, 65 without).
-    static constexpr bool FUSE = FUSE_;
+    static constexpr bool FUSE = !std::is_same<X, void>::value;
     static constexpr int OUT = FUSE ? 4 : FP4_OUT;  // warps that write out
-    static constexpr int TURN = KIND == FP4_SPLIT ? 1024 : 2048;  // bytes of a warp for 16 tokens on their way (of 16 bits; 32)
+    static constexpr int TURN = KIND == FP4_SPLIT ? 1024 : 2048;  // bytes of a warp for tokens on their way: 16 (of 32 bits 8 or 16)
     static constexpr int BK = KIND == FP4_SPLIT ? 128 : 256;     // values a stage
     static constexpr int KB = KIND == FP4_MX ? 2 : KIND == FP4_NV ? 4 : 1;  // scale tiles a stage and 128 rows
     static constexpr int NB = STACK ? 1 : P * ((T + 127) / 128);            // scale tiles of x beside each of w's
@@ -102,8 +104,8 @@ struct Fp4Args {
     const float* xf;     // factors, or NULL
     const float* wf;
     void* y;
-    // x in 16 bits (few tokens)
-    const void* x16;
+    // x before it is split (few tokens)
+    const void* x_rows;
     int64_t x_row;
     int K, vec, gather, src_rows;  // vec: rows start on 16-byte boundaries
     const int32_t* order;          // gather > 0: row j is row order[j] / gather of x (order NULL: j / gather); 0: row j
@@ -181,15 +183,35 @@ __device__ __forceinline__ void fp4_out(const Fp4Args& a, const Fp4Tile& t, int 
 // through shared memory, so that a token's 32 values leave in pieces of 16 bytes. Neighbouring lanes first swap
 // columns: the even lane then has two rows of an even column, the odd lane two of an odd one. The type and form are fixed
 // here, not asked for at each value: with branches between the shuffles they ran one after another (1,670 cycles, not 150).
-template <typename O, bool GLU>
+template <typename O, bool GLU, int TURN>
 __device__ __forceinline__ void fp4_out16_t(const Fp4Args& a, const Fp4Tile& t, int c0, int nb, const float (&v)[16], float f,
                                             uint8_t* stage, int lane) {
     constexpr int BYTES = (GLU ? 16 : 32) * int(sizeof(O)), PER = BYTES / 16;  // of a token's values here
     const bool odd = lane & 1;
-    if constexpr (sizeof(O) == 4 && !GLU) {
+    const int64_t width = GLU ? a.N / 2 : a.N;
+    O* y = static_cast<O*>(a.y) + int64_t(t.r0 + c0) * width + (GLU ? nb / 2 : nb);
+    const int rows = t.r1 - t.r0 - c0;
+    auto leave = [&](int c_lo, auto count) {  // `count` tokens from c_lo on
+        constexpr int PIECES = decltype(count)::value * PER;
+        __syncwarp();
 #pragma unroll
-        for (int c = 0; c < 16; ++c) reinterpret_cast<float*>(stage + c * BYTES)[lane] = v[c] * f;
+        for (int i = 0; i < (PIECES + 31) / 32; ++i) {
+            const int q = lane + 32 * i, c = c_lo + q / PER;
+            if (c < rows && q < PIECES)
+                *reinterpret_cast<uint4*>(y + c * width + (q % PER) * (16 / int(sizeof(O)))) = *reinterpret_cast<uint4*>(stage + q * 16);
+        }
+        __syncwarp();
+    };
+    if constexpr (sizeof(O) == 4 && !GLU) {
+        constexpr int AT = TURN / BYTES < 16 ? TURN / BYTES : 16;  // tokens that fit
+#pragma unroll
+        for (int c1 = 0; c1 < 16; c1 += AT) {
+#pragma unroll
+            for (int c = 0; c < AT; ++c) reinterpret_cast<float*>(stage + c * BYTES)[lane] = v[c1 + c] * f;
+            leave(c1, std::integral_constant<int, AT>());
+        }
     } else {
+        static_assert(16 * BYTES <= TURN, "16 tokens fit");
         float got[8];
 #pragma unroll
         for (int c = 0; c < 8; ++c) got[c] = __shfl_xor_sync(0xFFFFFFFFu, odd ? v[2 * c] : v[2 * c + 1], 1) * f;
@@ -207,36 +229,27 @@ __device__ __forceinline__ void fp4_out16_t(const Fp4Args& a, const Fp4Tile& t, 
                 reinterpret_cast<uint32_t*>(row)[lane >> 1] = F16Traits<O>::pack2(hi, lo);
             }
         }
+        leave(0, std::integral_constant<int, 16>());
     }
-    __syncwarp();
-    const int64_t width = GLU ? a.N / 2 : a.N;
-    O* y = static_cast<O*>(a.y) + int64_t(t.r0 + c0) * width + (GLU ? nb / 2 : nb);
-    const int rows = t.r1 - t.r0 - c0;
-#pragma unroll
-    for (int i = 0; i < (16 * PER + 31) / 32; ++i) {
-        const int q = lane + 32 * i, c = q / PER;
-        if (c < rows && q < 16 * PER)
-            *reinterpret_cast<uint4*>(y + c * width + (q % PER) * (16 / int(sizeof(O)))) = *reinterpret_cast<uint4*>(stage + q * 16);
-    }
-    __syncwarp();
 }
 
+template <int TURN>
 __device__ __forceinline__ void fp4_out16(const Fp4Args& a, const Fp4Tile& t, int c0, int nb, const float (&v)[16], float f,
                                           uint8_t* stage, int lane) {
     if (a.glu) {
         if (a.dtype == LQ_BF16)
-            fp4_out16_t<__nv_bfloat16, true>(a, t, c0, nb, v, f, stage, lane);
+            fp4_out16_t<__nv_bfloat16, true, TURN>(a, t, c0, nb, v, f, stage, lane);
         else if (a.dtype == LQ_F16)
-            fp4_out16_t<__half, true>(a, t, c0, nb, v, f, stage, lane);
+            fp4_out16_t<__half, true, TURN>(a, t, c0, nb, v, f, stage, lane);
         else
-            fp4_out16_t<float, true>(a, t, c0, nb, v, f, stage, lane);
+            fp4_out16_t<float, true, TURN>(a, t, c0, nb, v, f, stage, lane);
     } else {
         if (a.dtype == LQ_BF16)
-            fp4_out16_t<__nv_bfloat16, false>(a, t, c0, nb, v, f, stage, lane);
+            fp4_out16_t<__nv_bfloat16, false, TURN>(a, t, c0, nb, v, f, stage, lane);
         else if (a.dtype == LQ_F16)
-            fp4_out16_t<__half, false>(a, t, c0, nb, v, f, stage, lane);
+            fp4_out16_t<__half, false, TURN>(a, t, c0, nb, v, f, stage, lane);
         else
-            fp4_out16_t<float, false>(a, t, c0, nb, v, f, stage, lane);
+            fp4_out16_t<float, false, TURN>(a, t, c0, nb, v, f, stage, lane);
     }
 }
 
@@ -261,40 +274,49 @@ __device__ __forceinline__ void fp4_out4(const Fp4Args& a, const Fp4Tile& t, int
 }
 
 // 8 values of a group of 32 (four lanes next to one another) to P pieces of e4m3 bytes and their scale bytes. Scaled to below
-// 2^8 the values are fp16 numbers but for what lies below 2^-24 there, and the steps from piece to piece are exact in fp16.
-template <typename T16, int P>
-__device__ __forceinline__ void split8(const uint4& x, uint32_t mask, uint2 (&piece)[P], int (&byte)[P]) {
-    using T2 = typename std::conditional<std::is_same<T16, __half>::value, __half2, __nv_bfloat162>::type;
-    const uint32_t w[4] = {x.x, x.y, x.z, x.w};
-    float top = amax8_16<T2>(x);
+// 2^8, 16-bit values are fp16 numbers but for what lies below 2^-24 there, and the steps from piece to piece are exact in fp16;
+// 32-bit values take theirs in 32 bits.
+template <typename X, int P>
+__device__ __forceinline__ void split8(const Eight<X>& x, uint32_t mask, uint2 (&piece)[P], int (&byte)[P]) {
+    float top = x.amax();
 #pragma unroll
-    for (int d = 1; d < 4; d *= 2) {
-        const float o = __shfl_xor_sync(mask, top, d);
-        asm("max.NaN.f32 %0, %1, %2;" : "=f"(top) : "f"(top), "f"(o));
-    }
+    for (int d = 1; d < 4; d *= 2) top = amax_nan(top, __shfl_xor_sync(mask, top, d));
     const uint32_t e = __float_as_uint(top) >> 23 & 0xFF;
     byte[0] = e == 255 ? 255 : e < 7 ? 0 : int(e) - 7;
     const float up = __uint_as_float((254u - (e == 255 ? 127u : uint32_t(byte[0]))) << 23);
+    float v[8];
+    x.times(up, v);
     __half2 h[4];
+    if constexpr (sizeof(X) == 2) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-        h[i] = __floats2half2_rn(F16Traits<T16>::to_f32(w[i] & 0xFFFFu) * up, F16Traits<T16>::to_f32(w[i] >> 16) * up);
+        for (int i = 0; i < 4; ++i) h[i] = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
+    }
 #pragma unroll
     for (int p = 0; p < P; ++p) {
         uint16_t q[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-            asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(q[i]) : "r"(*reinterpret_cast<uint32_t*>(&h[i])));
+        for (int i = 0; i < 4; ++i) {
+            if constexpr (sizeof(X) == 2)
+                asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(q[i]) : "r"(*reinterpret_cast<uint32_t*>(&h[i])));
+            else
+                asm("cvt.rn.satfinite.e4m3x2.f32 %0, %2, %1;" : "=h"(q[i]) : "f"(v[2 * i]), "f"(v[2 * i + 1]));
+        }
         asm("mov.b32 %0, {%1, %2};" : "=r"(piece[p].x) : "h"(q[0]), "h"(q[1]));
         asm("mov.b32 %0, {%1, %2};" : "=r"(piece[p].y) : "h"(q[2]), "h"(q[3]));
         if (p + 1 < P) {
             byte[p + 1] = byte[p] == 255 ? 255 : byte[p] < 5 ? 0 : byte[p] - 5;
-            const __half2 more = __float2half2_rn(__uint_as_float(uint32_t(127 + (byte[p] == 255 ? 0 : byte[p] - byte[p + 1])) << 23));
+            const float more = __uint_as_float(uint32_t(127 + (byte[p] == 255 ? 0 : byte[p] - byte[p + 1])) << 23);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                uint32_t back;
-                asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(back) : "h"(q[i]));
-                h[i] = __hmul2(__hsub2(h[i], *reinterpret_cast<__half2*>(&back)), more);
+                if constexpr (sizeof(X) == 2) {
+                    uint32_t back;
+                    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(back) : "h"(q[i]));
+                    h[i] = __hmul2(__hsub2(h[i], *reinterpret_cast<__half2*>(&back)), __float2half2_rn(more));
+                } else {
+                    const float2 back = e4m3x2_to_f32(q[i]);
+                    v[2 * i] = (v[2 * i] - back.x) * more;
+                    v[2 * i + 1] = (v[2 * i + 1] - back.y) * more;
+                }
             }
         }
     }
@@ -507,13 +529,13 @@ __global__ void __launch_bounds__(FP4_THREADS, S::T <= 32 ? 2 : 1) fp4_gemm_kern
             ++j;
         }
     } else if (warp >= S::OUT) {
-        // ------------------------------ converters: 16-bit x to pieces ------------------------------
+        // ------------------------------ converters: x to pieces ------------------------------
         // The warps take stages in turn, so that the loads of four stages are on their way; a lane takes 8 values of a token.
         // No more warps than the ring has stages: one that is `turns` stages on has then seen, at its last stage, the place of
         // the stage two rounds back handed over, and the parity that it waits for is not the one of two rounds before.
         if constexpr (S::FUSE) {
-            using T16 = typename std::conditional<P == 2, __nv_bfloat16, __half>::type;
-            constexpr int AHEAD = 4;  // loads of a lane before it converts
+            using X = typename S::X;
+            constexpr int AHEAD = 8 / int(sizeof(X));  // values of 8 that a lane loads before it converts (32-bit ones: 2)
             grid_dep_wait();
             const int turns = NS < 4 ? NS : 4, mine = warp - S::OUT, chunk = lane & 15;
             int who = 0, s = 0, turn = 0;  // the warp of the next stage, its place, rounds of the ring
@@ -537,13 +559,13 @@ __global__ void __launch_bounds__(FP4_THREADS, S::T <= 32 ? 2 : 1) fp4_gemm_kern
                     bool free = turn == 0;
                     uint8_t* b = smem + s * S::STAGE + S::A_BYTES;
                     for (int i0 = 0; i0 < tasks; i0 += AHEAD) {
-                        uint4 v[AHEAD];
+                        Eight<X> v[AHEAD];
 #pragma unroll
                         for (int i = 0; i < AHEAD; ++i) {
                             const int row = __shfl_sync(0xFFFFFFFFu, src, (2 * (i0 + i) + (lane >> 4)) & 31);
-                            v[i] = make_uint4(0, 0, 0, 0);
+                            v[i].zero();
                             if (i0 + i < tasks && row >= 0)
-                                v[i] = load8_16(static_cast<const T16*>(a.x16) + int64_t(row) * a.x_row, kb * 128 + chunk * 8, a.K, a.vec);
+                                v[i].load(static_cast<const X*>(a.x_rows) + int64_t(row) * a.x_row, kb * 128 + chunk * 8, a.K, a.vec);
                         }
                         if (!free && !(ok = mbar_wait(&empty[s], (turn - 1) & 1))) break;
                         free = true;
@@ -561,12 +583,12 @@ __global__ void __launch_bounds__(FP4_THREADS, S::T <= 32 ? 2 : 1) fp4_gemm_kern
                             uint2 p0[P], p1[P];
                             int b0[P], b1[P];
                             if (i0 + i + 1 < tasks) {
-                                split8<T16, P>(v[i], 0xFFFFFFFFu, p0, b0);
-                                split8<T16, P>(v[i + 1], 0xFFFFFFFFu, p1, b1);
+                                split8<X, P>(v[i], 0xFFFFFFFFu, p0, b0);
+                                split8<X, P>(v[i + 1], 0xFFFFFFFFu, p1, b1);
                                 put(i0 + i, p0, b0);
                                 put(i0 + i + 1, p1, b1);
                             } else if (i0 + i < tasks) {
-                                split8<T16, P>(v[i], 0xFFFFFFFFu, p0, b0);
+                                split8<X, P>(v[i], 0xFFFFFFFFu, p0, b0);
                                 put(i0 + i, p0, b0);
                             }
                         }
@@ -640,7 +662,7 @@ __global__ void __launch_bounds__(FP4_THREADS, S::T <= 32 ? 2 : 1) fp4_gemm_kern
 #pragma unroll
                         for (int q = 0; q < 16; ++q) part[(c0 + c + q) * 128 + 32 * quarter + lane] = u[q];
                     } else if (wide && nb + 32 <= a.N) {
-                        if (t.r0 + c0 + c < t.r1) fp4_out16(a, t, c0 + c, nb, u, f, stage + S::TURN * warp, lane);
+                        if (t.r0 + c0 + c < t.r1) fp4_out16<S::TURN>(a, t, c0 + c, nb, u, f, stage + S::TURN * warp, lane);
                     } else {
 #pragma unroll
                         for (int q = 0; q < 16; ++q) fp4_out<S>(a, t, c0 + c + q, n, u[q] * f);
@@ -709,7 +731,7 @@ struct SplitArgs {
 
 // A warp takes 1,024 values of a row: the row's place is found once, four loads a lane are on their way together. (With a
 // thread a group and its place searched at each, 16,004 gathered rows of 2,048 took 70 us.)
-template <typename T16, int P>
+template <typename X, int P>
 __global__ void __launch_bounds__(256) fp4_split_kernel(const SplitArgs a) {
     grid_dep_wait();
     grid_dep_launch();  // after the wait: the product reads weights ahead of this kernel's end
@@ -725,12 +747,12 @@ __global__ void __launch_bounds__(256) fp4_split_kernel(const SplitArgs a) {
                 src = -1;  // zeros
             }
         }
-        uint4 v[4];
+        Eight<X> v[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const int word = part * 128 + 32 * i + lane;
-            v[i] = make_uint4(0, 0, 0, 0);
-            if (src >= 0 && word < words) v[i] = load8_16(static_cast<const T16*>(a.x) + src * a.x_row, 8 * word, a.K, a.vec);
+            v[i].zero();
+            if (src >= 0 && word < words) v[i].load(static_cast<const X*>(a.x) + src * a.x_row, 8 * word, a.K, a.vec);
         }
         int tile = row / a.T, at = row % a.T;
         if (a.grouped) {
@@ -757,7 +779,7 @@ __global__ void __launch_bounds__(256) fp4_split_kernel(const SplitArgs a) {
             if (part * 128 + 32 * i >= words) break;  // (rows are a multiple of 16 words: half a warp may be beyond)
             uint2 piece[P];
             int byte[P];
-            split8<T16, P>(v[i], 0xFFFFFFFFu, piece, byte);
+            split8<X, P>(v[i], 0xFFFFFFFFu, piece, byte);
             if (word < words) {
 #pragma unroll
                 for (int p = 0; p < P; ++p) {
@@ -880,10 +902,10 @@ static int gemm_t(const Fp4Call& c, cudaStream_t st) {
     return launch(reinterpret_cast<const void*>(kern), int(grid), FP4_THREADS, smem, S::CG == 2 ? 2 : a.ks, st, args);
 }
 
-template <int KIND, int P>
+template <int KIND, int P, typename X = void>
 static int gemm_tokens(const Fp4Call& c, int T, bool fuse, cudaStream_t st) {
     if constexpr (KIND == FP4_SPLIT)
-        if (fuse) return T == 16 ? gemm_t<Fp4Shape<KIND, P, 16, 1, true>>(c, st) : gemm_t<Fp4Shape<KIND, P, 32, 1, true>>(c, st);
+        if (fuse) return T == 16 ? gemm_t<Fp4Shape<KIND, P, 16, 1, X>>(c, st) : gemm_t<Fp4Shape<KIND, P, 32, 1, X>>(c, st);
     switch (T) {
         case 16: return gemm_t<Fp4Shape<KIND, P, 16>>(c, st);
         case 32: return gemm_t<Fp4Shape<KIND, P, 32>>(c, st);
@@ -943,20 +965,23 @@ static int grouped_tokens(int rows, int segments, int max_rows) {
 // Whether the product makes the pieces of x itself: few tokens, and all tiles run at once.
 static bool fused(int T, int64_t ttiles, int N) { return T <= 32 && ttiles * ((N + 127) / 128) <= 2 * int64_t(FP4_FUSE_SMS); }
 
-size_t fp4_linear_workspace_bytes(int rows, int N, int K, int dtype, int segments, int max_rows) {
-    const int P = dtype == LQ_BF16 ? 2 : 3, T = segments ? grouped_tokens(rows, segments, max_rows) : tile_tokens(rows);
+// Pieces of a value: two hold the 8 bits of bf16, three the 11 of fp16 (and 14 or more of 32 bits).
+static int fp4_pieces(int x_dtype) { return x_dtype == LQ_BF16 ? 2 : 3; }
+
+size_t fp4_linear_workspace_bytes(int rows, int N, int K, int x_dtype, int segments, int max_rows) {
+    const int P = fp4_pieces(x_dtype), T = segments ? grouped_tokens(rows, segments, max_rows) : tile_tokens(rows);
     if (fused(T, split_tiles(rows, T, segments), N)) return 0;
     return split_pieces_bytes(rows, K, P) +
            size_t(split_tiles(rows, T, segments)) * fp4_ktiles(K, LQ_MXFP4) * split_blocks(P, T) * 512;
 }
 
 int fp4_linear_run(const Fp4Linear& l, cudaStream_t st) {
-    const int P = l.dtype == LQ_BF16 ? 2 : 3;
+    const int P = fp4_pieces(l.x_dtype);
     const int T = l.segments ? grouped_tokens(l.rows, l.segments, l.max_rows) : tile_tokens(l.rows);
     uint8_t* ws = static_cast<uint8_t*>(l.ws);
     SplitArgs s = {};
     s.ktiles = fp4_ktiles(l.K, LQ_MXFP4);
-    const bool vec = aligned(l.x, 16) && l.x_row % 8 == 0;
+    const bool vec = aligned(l.x, 16) && l.x_row % (l.x_dtype == LQ_F32 ? 4 : 8) == 0;
     const bool fuse = fused(T, split_tiles(l.rows, T, l.segments), l.N);
     if (!fuse) {
         s.x = l.x;
@@ -978,8 +1003,9 @@ int fp4_linear_run(const Fp4Linear& l, cudaStream_t st) {
         s.nseg = l.nseg;
         const int64_t units = int64_t(l.rows) * ((fp4_padded(l.K) + 1023) / 1024);  // of a warp
         const int64_t most = int64_t(device_info().sm_count) * 8, blocks = (units + 7) / 8;
-        const void* split = l.dtype == LQ_BF16 ? reinterpret_cast<const void*>(fp4_split_kernel<__nv_bfloat16, 2>)
-                                               : reinterpret_cast<const void*>(fp4_split_kernel<__half, 3>);
+        const void* split = l.x_dtype == LQ_BF16  ? reinterpret_cast<const void*>(fp4_split_kernel<__nv_bfloat16, 2>)
+                            : l.x_dtype == LQ_F16 ? reinterpret_cast<const void*>(fp4_split_kernel<__half, 3>)
+                                                  : reinterpret_cast<const void*>(fp4_split_kernel<float, 3>);
         void* sargs[] = {&s};
         const int rc = launch(split, int(blocks < most ? blocks : most), 256, 0, 1, st, sargs);
         if (rc) return rc;
@@ -997,7 +1023,7 @@ int fp4_linear_run(const Fp4Linear& l, cudaStream_t st) {
     a.glu = l.glu;
     a.dtype = l.dtype;
     a.piece_rows = l.rows;
-    a.x16 = l.x;
+    a.x_rows = l.x;
     a.x_row = l.x_row;
     a.K = l.K;
     a.vec = vec;
@@ -1013,7 +1039,9 @@ int fp4_linear_run(const Fp4Linear& l, cudaStream_t st) {
     a.experts = l.experts;
     a.nseg = l.nseg;
     a.max_seg = l.segments;
-    return l.dtype == LQ_BF16 ? gemm_tokens<FP4_SPLIT, 2>(c, T, fuse, st) : gemm_tokens<FP4_SPLIT, 3>(c, T, fuse, st);
+    if (l.x_dtype == LQ_BF16) return gemm_tokens<FP4_SPLIT, 2, __nv_bfloat16>(c, T, fuse, st);
+    if (l.x_dtype == LQ_F16) return gemm_tokens<FP4_SPLIT, 3, __half>(c, T, fuse, st);
+    return gemm_tokens<FP4_SPLIT, 3, float>(c, T, fuse, st);
 }
 
 }  // namespace lq

@@ -336,6 +336,36 @@ __global__ void __launch_bounds__(256) combine8_kernel(const uint4* ys, const fl
     y[i] = make_uint4(o[0], o[1], o[2], o[3]);
 }
 
+// The same sums of 32-bit rows (the experts' outputs as their product summed them): y rounded once. V columns a thread: 4, or 1
+// where D is no multiple of 4.
+template <int V>
+__global__ void __launch_bounds__(256) combine_f32_kernel(const float* ys, const float* w, const int32_t* pos, uint16_t* y, int T,
+                                                          int k, int D, int dt) {
+    grid_dep_wait();
+    grid_dep_launch();
+    const size_t i = size_t(blockIdx.x) * blockDim.x + threadIdx.x;
+    if (i >= size_t(T) * (D / V)) return;
+    const int t = int(i / (D / V)), d = int(i % (D / V)) * V;
+    float acc[V] = {};
+#pragma unroll 4
+    for (int r = 0; r < k; ++r) {
+        const int slot = t * k + r;
+        const int row = pos ? pos[slot] : slot;
+        const float* src = ys + size_t(row) * D + d;
+        float v[V];
+        if constexpr (V == 4)
+            *reinterpret_cast<float4*>(v) = *reinterpret_cast<const float4*>(src);
+        else
+            v[0] = *src;
+        const float ws = w[slot];
+#pragma unroll
+        for (int c = 0; c < V; ++c) acc[c] = fmaf(v[c], ws, acc[c]);
+    }
+#pragma unroll
+    for (int c = 0; c < V; ++c)
+        y[size_t(t) * D + d + c] = dt == LQ_BF16 ? F16Traits<__nv_bfloat16>::from_f32(acc[c]) : F16Traits<__half>::from_f32(acc[c]);
+}
+
 // Router logits and top-k, the experts split over a cluster of RC_CL CTAs and the tokens in tiles of TT (grid
 // (ceil(T / TT), RC_CL), cluster (1, RC_CL, 1), 256 threads; TT = ceil(T / 16) up to RC_TT, so up to 16 tokens run
 // one token a cluster). Each CTA stages its E / RC_CL experts' router rows in
@@ -631,6 +661,13 @@ int combine_run(const void* ys, const float* w, const int32_t* pos, void* y, int
     const size_t n = size_t(T) * D;
     return launch_pdl(combine_kernel, dim3(unsigned((n + threads - 1) / threads)), dim3(threads), 0, st,
                       reinterpret_cast<const uint16_t*>(ys), w, pos, reinterpret_cast<uint16_t*>(y), T, k, D, dt);
+}
+
+int combine_f32_run(const float* ys, const float* w, const int32_t* pos, void* y, int T, int k, int D, int dt, cudaStream_t st) {
+    const int V = D % 4 == 0 && aligned(ys, 16) ? 4 : 1, threads = 256;
+    const size_t n = size_t(T) * (D / V);
+    return launch_pdl(V == 4 ? combine_f32_kernel<4> : combine_f32_kernel<1>, dim3(unsigned((n + threads - 1) / threads)), dim3(threads),
+                      0, st, ys, w, pos, static_cast<uint16_t*>(y), T, k, D, dt);
 }
 
 }  // namespace lq

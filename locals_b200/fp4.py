@@ -164,8 +164,8 @@ def switch_glu(x: torch.Tensor, inds: torch.Tensor, gate_up: Fp4, down: Fp4, gro
 
 def experts(x: torch.Tensor, inds: torch.Tensor, weights: torch.Tensor, gate_up: Fp4, down: Fp4) -> torch.Tensor:
     """The routed experts of a step: sum over slots r of weights[t, r] * expert inds[t, r] of x[t], (T, D) in x's dtype
-    (grouping, gate and up, down, ``moe.combine``); silu(gate) * up and each expert's output are rounded to x's dtype on
-    their way, as ``moe.switch_glu`` rounds them. inds int32 and weights float32 (T, k), as moe.route gives them."""
+    (grouping, gate and up, down, weighted sum). silu(gate) * up and the experts' outputs stay in 32 bits, so that y is rounded
+    once; ``switch_glu`` gives both in x's dtype. inds int32 and weights float32 (T, k), as moe.route gives them."""
     return ext().fp4_experts(x, inds, weights, gate_up, down)
 
 

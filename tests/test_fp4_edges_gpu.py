@@ -1,0 +1,82 @@
+"""Microscaled 4-bit floating point on the GPU, where a call could go wrong: against statements in 64 bits."""
+
+import pytest
+
+from tests import fp4_reference as R
+
+pytestmark = pytest.mark.gpu
+
+
+def _gen(cuda, seed):
+    import torch
+
+    g = torch.Generator(device=cuda)
+    g.manual_seed(seed)
+    return g
+
+
+def _dt(name):
+    import torch
+
+    return {"bf16": torch.bfloat16, "f16": torch.float16, "f32": torch.float32}[name]
+
+
+def _status(cuda):
+    import torch
+    from locals_b200 import kernels
+
+    torch.cuda.synchronize()
+    return kernels.device_status()
+
+
+def _stack(cuda, g, E, rows, K, size=1.0):
+    """A stack of E random mxfp4 matrices, any K: (operand, values in 64 bits)."""
+    import torch
+    from locals_b200 import fp4
+
+    parts = [fp4.quantize(torch.randn((rows, K), generator=g, device=cuda) * size, "mxfp4") for _ in range(E)]
+    w = fp4.Fp4(torch.stack([p.codes for p in parts]), torch.stack([p.tiles for p in parts]), "mxfp4", K)
+    return w, torch.stack([fp4.dequantize(p, torch.float32).double() for p in parts])
+
+
+def _experts(x, inds, weights, gate_up, down):
+    """The routed experts in 64 bits; ids outside the stack contribute nothing."""
+    import torch
+
+    y = torch.zeros(x.shape, dtype=torch.float64, device=x.device)
+    for e in range(gate_up.shape[0]):
+        t, slot = torch.where(inds == e)
+        gu = x[t].double() @ gate_up[e].T
+        h = torch.nn.functional.silu(gu[:, 0::2]) * gu[:, 1::2]
+        y.index_add_(0, t, weights[t, slot, None].double() * (h @ down[e].T))
+    return y
+
+
+def _rms(t):
+    return float(t.double().square().mean().sqrt())
+
+
+# ---- routed experts ---------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("T,E,k,D,I", [(1, 8, 4, 256, 96), (1, 4, 2, 101, 37), (2, 8, 2, 160, 33), (20, 6, 2, 130, 64), (40, 2, 2, 254, 72),
+                                       (64, 16, 4, 256, 192), (300, 4, 2, 256, 130), (900, 2, 1, 64, 66)])
+def test_experts_are_rounded_once(cuda, dtype, T, E, k, D, I):
+    """y is off by little more than its own rounding. What else there is adds in squares: the hidden rows' pieces (2^-14 of a value
+    at most, where half a step is 2^-9 or 2^-12), sums in 32 bits (some 24 steps of 2^-22). A second rounding to 16 bits
+    anywhere would give 1.4 times as much."""
+    import torch
+    from locals_b200 import fp4
+
+    g = _gen(cuda, T + E + D)
+    gu, gv = _stack(cuda, g, E, 2 * I, D, D ** -0.5)
+    dn, dv = _stack(cuda, g, E, D, I, I ** -0.5)
+    x = torch.randn((T, D), generator=g, device=cuda).to(_dt(dtype))
+    inds = torch.rand((T, E), generator=g, device=cuda).topk(k, -1).indices.to(torch.int32)
+    weights = 0.5 + torch.rand((T, k), generator=g, device=cuda)
+    want = _experts(x, inds, weights, gv, dv)
+    y = fp4.experts(x, inds, weights, gu, dn)
+    assert _status(cuda) == 0
+    off, once = _rms(y.double() - want), _rms(want.to(_dt(dtype)).double() - want)
+    assert off <= 1.05 * once
+    assert torch.equal(y, fp4.experts(x, inds, weights, gu, dn))
