@@ -158,7 +158,7 @@ def switch_glu(x: torch.Tensor, inds: torch.Tensor, gate_up: Fp4, down: Fp4, gro
         h = grouped(x.contiguous(), g, gate_up, M, glu=True, gather_k=k)
         ys = grouped(h, g, down, M)
         if g[4] is not None:
-            ys = moe.gather(ys, g[4], 1)
+            ys = moe.gather(ys, g[4], 1) if ys.shape[1] % 8 == 0 else ys.index_select(0, g[4])  # (gather copies 16 bytes at a time)
     return ys.reshape(M, k, -1)
 
 

@@ -80,3 +80,24 @@ def test_experts_are_rounded_once(cuda, dtype, T, E, k, D, I):
     off, once = _rms(y.double() - want), _rms(want.to(_dt(dtype)).double() - want)
     assert off <= 1.05 * once
     assert torch.equal(y, fp4.experts(x, inds, weights, gu, dn))
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("T,k,D,I", [(1, 2, 130, 64), (20, 3, 130, 64), (300, 2, 101, 37), (20, 2, 128, 33)])
+def test_switch_glu_takes_any_width(cuda, dtype, T, k, D, I):
+    """Each slot's output is rounded once and its hidden row once before it: 1.41 roundings, added in squares."""
+    import torch
+    from locals_b200 import fp4
+
+    g = _gen(cuda, T + D)
+    E = 4
+    gu, gv = _stack(cuda, g, E, 2 * I, D, D ** -0.5)
+    dn, dv = _stack(cuda, g, E, D, I, I ** -0.5)
+    x = torch.randn((T, D), generator=g, device=cuda).to(_dt(dtype))
+    inds = torch.rand((T, E), generator=g, device=cuda).topk(k, -1).indices.to(torch.int32)
+    ys = fp4.switch_glu(x, inds, gu, dn)
+    assert _status(cuda) == 0 and ys.shape == (T, k, D)
+    one = torch.ones((T, 1), device=cuda)
+    want = torch.stack([_experts(x, inds[:, r:r + 1], one, gv, dv) for r in range(k)], 1)
+    off, once = _rms(ys.double() - want), _rms(want.to(_dt(dtype)).double() - want)
+    assert off <= 1.5 * once
