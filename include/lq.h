@@ -121,7 +121,9 @@ int lq_moe_route(const void* x, int x_dtype, const void* w, int w_dtype, int T, 
 
 /* Counting sort of P expert ids (locals/moe_kernel.py:28-66,191-197): order (P) = pair ids grouped
  * by ascending expert (ascending pair id within an expert), starts (min(E,P)+1), experts (min(E,P)),
- * nseg (1) and, if pos != NULL, pos (P) = the inverse of order. All int32 device arrays. E <= 8192. */
+ * nseg (1) and, if pos != NULL, pos (P) = the inverse of order. All int32 device arrays. E <= 8192. An id outside [0, E)
+ * is recorded (LQ_DEV_BOUNDS) and left out: the pair is in no segment, its pos is -1, and order has as many -1 behind the last
+ * segment. */
 int lq_moe_group(const uint32_t* inds, int P, int E, int32_t* order, int32_t* starts, int32_t* experts, int32_t* nseg,
                  int32_t* pos, void* stream);
 
@@ -133,7 +135,8 @@ int lq_moe_group(const uint32_t* inds, int P, int E, int32_t* order, int32_t* st
 int lq_moe_group_range(const uint32_t* inds, int P, int lo, int range, int32_t* order, int32_t* starts,
                        int32_t* experts, int32_t* nseg, int32_t* pos, void* stream);
 
-/* xs (P, D) = x[order[j] / k] for j < P: the tokens of the pairs in expert order (16-bit x, D % 8 == 0). */
+/* xs (P, D) = x[order[j] / k] for j < P: the tokens of the pairs in expert order (16-bit x, D % 8 == 0); zeros where order[j] is
+ * negative. */
 int lq_moe_gather(const void* x, const int32_t* order, int P, int k, int D, void* xs, void* stream);
 
 /* Grouped expert projections (locals/moe_kernel.py:68-155,206-239; mx.gather_qmm of mlx-lm's SwitchGLU,
@@ -182,7 +185,7 @@ int lq_moe_decode(const void* x, const void* router_w, int router_dtype, int E, 
                   void* stream);
 
 /* y (T, D) = sum over slots r of weights[t, r] * ys[pos[t*k + r], :] in float32, slots in order, rounded
- * to dtype (locals/moe.py:339-348). pos == NULL reads row t*k + r. */
+ * to dtype (locals/moe.py:339-348). pos == NULL reads row t*k + r; a slot whose pos is negative adds nothing. */
 int lq_moe_combine(const void* ys, const float* weights, const int32_t* pos, void* y, int T, int k, int D, int dtype,
                    void* stream);
 
@@ -196,7 +199,7 @@ int lq_add_rms_norm(const void* x, const void* r, const void* w, void* h, void* 
 /* The MoE combine with the shared expert, the layer's residual add and the next layer's input norm in one
  * pass (locals/moe.py:353-389): y[t] = T(res[t] + T(T(sum_r weights[t,r] * ys[pos[t*k + r]]) + shared[t])),
  * n[t] = T(nw * T(y[t] / sqrt(mean(y[t]^2) + eps))). shared == NULL: no shared expert; pos == NULL: row
- * t*k + r. Same shape rules as lq_add_rms_norm. */
+ * t*k + r, a negative pos adds nothing. Same shape rules as lq_add_rms_norm. */
 int lq_moe_combine_norm(const void* ys, const float* weights, const int32_t* pos, const void* shared, const void* res,
                         const void* nw, void* y, void* n, int T, int k, int D, float eps, int dtype, void* stream);
 
@@ -357,7 +360,8 @@ int lq_fp4_experts(const void* x, int x_rows, const int32_t* gather_order, int g
 /* The routed mxfp4 experts of a step and their weighted sum, y (T, D) = sum over slots r of weights[t, r] * down_e .
  * (silu(gate_e . x[t]) * (up_e . x[t])) with e = inds[t, r]: lq_moe_group, two grouped products and the combine in one call. The
  * hidden rows and the experts' outputs are held in 32 bits (the former enter the down product in three pieces of e4m3, off by at most
- * 2^-14 of a value, or 2^-27 of the largest of its group of 32); y is rounded once. x (T, D), y f16 / bf16; inds and weights (T, k);
+ * 2^-14 of a value, or 2^-27 of the largest of its group of 32); y is rounded once. A slot whose id is outside [0, E) adds nothing
+ * (and LQ_DEV_BOUNDS). x (T, D), y f16 / bf16; inds and weights (T, k);
  * gate_up (E, 2 I, D) with gate and up rows in turn, down (E, D, I) as lq_fp4_experts; at most 1024 experts or T * k pairs, whichever is
  * less (T 1: k pairs). workspace: lq_fp4_moe_workspace(T, k, E, D, I, dtype) bytes (0: sizes that are refused), 256-byte aligned. */
 size_t lq_fp4_moe_workspace(int T, int k, int E, int D, int I, int dtype);

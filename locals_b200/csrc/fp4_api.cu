@@ -244,7 +244,7 @@ int lq_fp4_moe(const void* x, const int32_t* inds, const float* weights, const u
     l.y = ys;
     rc = fp4_linear_run(l, st);
     if (rc) return finish(rc);
-    return finish(combine_f32_run(ys, weights, pos, y, T, k, D, dtype, st));
+    return finish(combine_f32_run(ys, weights, pos, inds, E, y, T, k, D, dtype, st));
 }
 
 }  // extern "C"

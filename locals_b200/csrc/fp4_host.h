@@ -33,6 +33,7 @@ int fp4_linear_run(const Fp4Linear& l, cudaStream_t st);
 // moe.cu
 int group_run(const uint32_t* inds, int P, int E, int32_t* order, int32_t* starts, int32_t* experts, int32_t* nseg,
               int32_t* pos, cudaStream_t st);
-int combine_f32_run(const float* ys, const float* w, const int32_t* pos, void* y, int T, int k, int D, int dt, cudaStream_t st);
+int combine_f32_run(const float* ys, const float* w, const int32_t* pos, const int32_t* ids, int E, void* y, int T, int k, int D, int dt,
+                    cudaStream_t st);
 
 }  // namespace lq

@@ -11,6 +11,8 @@
 //                  (locals/moe_kernel.py:28-66 with a deterministic order).
 //  gather_rows   : xs[j] = x[order[j] / k], the tokens laid out in pair order for the grouped kernel.
 //  combine       : y[t] = sum_r w[t, r] * ys[pos[t*k + r]] in float32, slots in order (locals/moe.py:339-348).
+// A pair whose id is no expert's is in no segment: its pos is -1, which gather and combine take for a row of zeros, and order
+// ends with as many -1.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -127,6 +129,7 @@ __global__ void group_kernel(const uint32_t* inds, int P, int E, int32_t* order,
             starts[s] = at;
             nseg[0] = s;
         }
+        for (int j = at + lane; j < P; j += 32) order[j] = -1;
     }
     for (int p0 = 0; p0 < P; p0 += GROUP_STAGE) {
         const int n = P - p0 < GROUP_STAGE ? P - p0 : GROUP_STAGE;
@@ -144,10 +147,8 @@ __global__ void group_kernel(const uint32_t* inds, int P, int E, int32_t* order,
                 __syncwarp();
                 if (valid && rank == 0) run[e] += __popc(peers);
                 __syncwarp();
-                if (valid) {
-                    order[j] = p0 + i;
-                    if (pos) pos[p0 + i] = j;
-                }
+                if (valid) order[j] = p0 + i;
+                if (i < n && pos) pos[p0 + i] = valid ? j : -1;
             }
         }
     }
@@ -240,6 +241,7 @@ __global__ void __launch_bounds__(1024) group_par_kernel(const uint32_t* inds, i
             starts[sgi] = at;
             nseg[0] = sgi;
         }
+        for (int j = at + lane; rank == 0 && j < P; j += 32) order[j] = -1;
     }
     __syncthreads();
     for (int c = p0; c < p1; c += 32) {
@@ -255,6 +257,8 @@ __global__ void __launch_bounds__(1024) group_par_kernel(const uint32_t* inds, i
         if (valid) {
             order[j] = p;
             if (pos) pos[p] = j;
+        } else if (pos && p < p1) {
+            pos[p] = -1;
         }
     }
     if (ctas > 1) {
@@ -269,9 +273,13 @@ __global__ void gather_rows_kernel(const uint16_t* x, const int32_t* order, int 
     grid_dep_launch();
     const int warp = (blockIdx.x * blockDim.x + threadIdx.x) >> 5, lane = threadIdx.x & 31;
     if (warp >= P) return;
-    const int tok = order[warp] / k;
-    const uint4* src = reinterpret_cast<const uint4*>(x + size_t(tok) * D);
+    const int pair = order[warp], tok = pair / k;
     uint4* dst = reinterpret_cast<uint4*>(xs + size_t(warp) * D);
+    if (pair < 0) {
+        for (int i = lane; i < D / 8; i += 32) dst[i] = make_uint4(0, 0, 0, 0);
+        return;
+    }
+    const uint4* src = reinterpret_cast<const uint4*>(x + size_t(tok) * D);
     for (int i = lane; i < D / 8; i += 32) dst[i] = src[i];
 }
 
@@ -287,14 +295,14 @@ __global__ void combine_kernel(const uint16_t* ys, const float* w, const int32_t
     for (int r = 0; r < k; ++r) {
         const int slot = t * k + r;
         const int row = pos ? pos[slot] : slot;
-        const uint16_t h = ys[size_t(row) * D + d];
+        const uint16_t h = ys[size_t(max(row, 0)) * D + d];
         float v;
         if (dt == LQ_BF16) {
             v = __uint_as_float(uint32_t(h) << 16);
         } else {
             v = __half2float(*reinterpret_cast<const __half*>(&h));
         }
-        acc = fmaf(v, w[slot], acc);
+        acc = row < 0 ? acc : fmaf(v, w[slot], acc);
     }
     if (dt == LQ_BF16) {
         __nv_bfloat16 b = __float2bfloat16_rn(acc);
@@ -319,9 +327,10 @@ __global__ void __launch_bounds__(256) combine8_kernel(const uint4* ys, const fl
     for (int r = 0; r < k; ++r) {
         const int slot = t * k + r;
         const int row = pos ? pos[slot] : slot;
-        const uint4 q = ys[size_t(row) * D8 + d];
-        const float ws = w[slot];
-        const uint32_t h[4] = {q.x, q.y, q.z, q.w};
+        const uint4 q = ys[size_t(max(row, 0)) * D8 + d];
+        const uint32_t there = row < 0 ? 0u : ~0u;  // (a mask: with a branch the slots' loads went one after another)
+        const float ws = __uint_as_float(__float_as_uint(w[slot]) & there);
+        const uint32_t h[4] = {q.x & there, q.y & there, q.z & there, q.w & there};
 #pragma unroll
         for (int c = 0; c < 8; ++c) {
             const uint32_t v = h[c >> 1] >> (16 * (c & 1)) & 0xFFFFu;
@@ -337,30 +346,34 @@ __global__ void __launch_bounds__(256) combine8_kernel(const uint4* ys, const fl
 }
 
 // The same sums of 32-bit rows (the experts' outputs as their product summed them): y rounded once. V columns a thread: 4, or 1
-// where D is no multiple of 4.
+// where D is no multiple of 4. Without a grouping (pos NULL) the ids tell which rows there are.
 template <int V>
-__global__ void __launch_bounds__(256) combine_f32_kernel(const float* ys, const float* w, const int32_t* pos, uint16_t* y, int T,
-                                                          int k, int D, int dt) {
+__global__ void __launch_bounds__(256) combine_f32_kernel(const float* ys, const float* w, const int32_t* pos, const int32_t* ids,
+                                                          int E, uint16_t* y, int T, int k, int D, int dt) {
     grid_dep_wait();
     grid_dep_launch();
     const size_t i = size_t(blockIdx.x) * blockDim.x + threadIdx.x;
     if (i >= size_t(T) * (D / V)) return;
     const int t = int(i / (D / V)), d = int(i % (D / V)) * V;
     float acc[V] = {};
+    bool odd = false;  // an id that is no expert's
 #pragma unroll 4
     for (int r = 0; r < k; ++r) {
         const int slot = t * k + r;
         const int row = pos ? pos[slot] : slot;
-        const float* src = ys + size_t(row) * D + d;
+        const bool there = pos ? unsigned(row) < unsigned(T * k) : unsigned(ids[slot]) < unsigned(E);
+        odd |= !there;
+        const float* src = ys + size_t(pos && !there ? 0 : row) * D + d;
         float v[V];
         if constexpr (V == 4)
             *reinterpret_cast<float4*>(v) = *reinterpret_cast<const float4*>(src);
         else
             v[0] = *src;
-        const float ws = w[slot];
+        const float ws = there ? w[slot] : 0.f;
 #pragma unroll
-        for (int c = 0; c < V; ++c) acc[c] = fmaf(v[c], ws, acc[c]);
+        for (int c = 0; c < V; ++c) acc[c] = fmaf(there ? v[c] : 0.f, ws, acc[c]);
     }
+    if (odd && !pos) record_status(LQ_DEV_BOUNDS);
 #pragma unroll
     for (int c = 0; c < V; ++c)
         y[size_t(t) * D + d + c] = dt == LQ_BF16 ? F16Traits<__nv_bfloat16>::from_f32(acc[c]) : F16Traits<__half>::from_f32(acc[c]);
@@ -663,11 +676,12 @@ int combine_run(const void* ys, const float* w, const int32_t* pos, void* y, int
                       reinterpret_cast<const uint16_t*>(ys), w, pos, reinterpret_cast<uint16_t*>(y), T, k, D, dt);
 }
 
-int combine_f32_run(const float* ys, const float* w, const int32_t* pos, void* y, int T, int k, int D, int dt, cudaStream_t st) {
+int combine_f32_run(const float* ys, const float* w, const int32_t* pos, const int32_t* ids, int E, void* y, int T, int k, int D, int dt,
+                    cudaStream_t st) {
     const int V = D % 4 == 0 && aligned(ys, 16) ? 4 : 1, threads = 256;
     const size_t n = size_t(T) * (D / V);
     return launch_pdl(V == 4 ? combine_f32_kernel<4> : combine_f32_kernel<1>, dim3(unsigned((n + threads - 1) / threads)), dim3(threads),
-                      0, st, ys, w, pos, static_cast<uint16_t*>(y), T, k, D, dt);
+                      0, st, ys, w, pos, ids, E, static_cast<uint16_t*>(y), T, k, D, dt);
 }
 
 }  // namespace lq

@@ -142,9 +142,11 @@ __global__ void __launch_bounds__(NORM_THREADS)
         for (int i = 0; i < 8; ++i) acc[i] = 0.0f;
         for (int k = 0; k < K; ++k) {
             const int slot = pos ? pos[t * K + k] : int(t * K + k);
-            const float wk = wts[t * K + k];
+            const uint32_t there = slot < 0 ? 0u : ~0u;  // (below 0: a pair of no expert, which adds 0 * 0)
+            const float wk = __uint_as_float(__float_as_uint(wts[t * K + k]) & there);
             Vec8 yv;
-            yv.u = *reinterpret_cast<const uint4*>(ys + size_t(slot) * D + c);
+            yv.u = *reinterpret_cast<const uint4*>(ys + size_t(max(slot, 0)) * D + c);
+            yv.u = make_uint4(yv.u.x & there, yv.u.y & there, yv.u.z & there, yv.u.w & there);
 #pragma unroll
             for (int i = 0; i < 8; ++i)  // product and sum rounded separately (no fused multiply-add), as the C restatement
                 acc[i] = __fadd_rn(acc[i], __fmul_rn(nt_f(vget<T>(yv, i)), wk));

@@ -219,7 +219,7 @@ __global__ void __launch_bounds__(QG_THREADS, 2)
                     seg = a.pos ? a.pos[r] : r;
                     fe = u;
                 }
-                int e = a.experts[seg];
+                int e = seg < 0 ? -1 : a.experts[seg];  // (a pair of no expert has no row either: its x below is zeros)
                 if (e < 0 || (e + 1) * a.rows_e > a.N) {
                     if (lane == 0) record_status(LQ_DEV_BOUNDS);
                     e = 0;
@@ -316,7 +316,7 @@ __global__ void __launch_bounds__(QG_THREADS, 2)
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt) {
             const int tok = 8 * mt + g;
-            if (tok < a.M && gi < a.kg) {
+            if (tok < a.M && gi < a.kg && xrow[mt] >= 0) {
                 const uint4* p = reinterpret_cast<const uint4*>(xg + (size_t(xrow[mt]) * a.K + gi * 64 + 16 * t) * 2);
                 u[mt][0] = p[0];
                 u[mt][1] = p[1];

@@ -158,14 +158,18 @@ def switch_glu(x: torch.Tensor, inds: torch.Tensor, gate_up: Fp4, down: Fp4, gro
         h = grouped(x.contiguous(), g, gate_up, M, glu=True, gather_k=k)
         ys = grouped(h, g, down, M)
         if g[4] is not None:
-            ys = moe.gather(ys, g[4], 1) if ys.shape[1] % 8 == 0 else ys.index_select(0, g[4])  # (gather copies 16 bytes at a time)
+            if ys.shape[1] % 8 == 0:
+                ys = moe.gather(ys, g[4], 1)
+            else:  # (gather copies 16 bytes at a time)
+                ys = ys.index_select(0, g[4].clamp(min=0)).masked_fill_((g[4] < 0)[:, None], 0)
     return ys.reshape(M, k, -1)
 
 
 def experts(x: torch.Tensor, inds: torch.Tensor, weights: torch.Tensor, gate_up: Fp4, down: Fp4) -> torch.Tensor:
     """The routed experts of a step: sum over slots r of weights[t, r] * expert inds[t, r] of x[t], (T, D) in x's dtype
     (grouping, gate and up, down, weighted sum). silu(gate) * up and the experts' outputs stay in 32 bits, so that y is rounded
-    once; ``switch_glu`` gives both in x's dtype. inds int32 and weights float32 (T, k), as moe.route gives them."""
+    once; ``switch_glu`` gives both in x's dtype. inds int32 and weights float32 (T, k), as moe.route gives them; an id that is no
+    expert's adds nothing and is recorded (``kernels.device_status``)."""
     return ext().fp4_experts(x, inds, weights, gate_up, down)
 
 

@@ -48,7 +48,8 @@ def route_topk(logits: torch.Tensor, k: int, mode: int = SOFTMAX) -> Tuple[torch
 
 def group(inds: torch.Tensor, E: int):
     """(order, starts, experts, nseg, pos) of the flat expert ids (the reference's group(),
-    locals/moe_kernel.py:191-197, plus the inverse permutation)."""
+    locals/moe_kernel.py:191-197, plus the inverse permutation). A pair whose id is no expert's is in no segment: its pos is
+    -1, which ``gather`` and the combines take for a row of zeros."""
     flat = inds.reshape(-1).contiguous()
     _check_cuda(flat)
     P = flat.numel()

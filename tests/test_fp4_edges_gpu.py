@@ -103,3 +103,96 @@ def test_switch_glu_takes_any_width(cuda, dtype, T, k, D, I):
     want = torch.stack([_experts(x, inds[:, r:r + 1], one, gv, dv) for r in range(k)], 1)
     off, once = _rms(ys.double() - want), _rms(want.to(_dt(dtype)).double() - want)
     assert off <= 2.3 * once
+
+
+def _poison(cuda):
+    """Memory that the allocator hands out next holds no numbers."""
+    import torch
+
+    for n in (1 << 12, 1 << 16, 1 << 20, 1 << 24):
+        t = torch.full((n,), float("nan"), device=cuda)
+        del t
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("T,k,D", [(1, 4, 256), (1, 3, 101), (20, 2, 256), (20, 3, 130), (300, 2, 256), (1200, 2, 128)])
+def test_experts_leave_ids_out_that_are_no_experts(cuda, dtype, T, k, D):
+    """Ids of -1 and beyond the last expert add nothing, and are recorded; a token of none but those is zeros."""
+    import torch
+    from locals_b200 import fp4
+
+    g = _gen(cuda, T + k)
+    E, I = 5, 96
+    gu, gv = _stack(cuda, g, E, 2 * I, D, D ** -0.5)
+    dn, dv = _stack(cuda, g, E, D, I, I ** -0.5)
+    x = torch.randn((T, D), generator=g, device=cuda).to(_dt(dtype))
+    weights = 0.5 + torch.rand((T, k), generator=g, device=cuda)
+    for bad in (-1, E, 1 << 30, -2 ** 31):
+        inds = torch.randint(0, E, (T, k), generator=g, device=cuda).to(torch.int32)
+        inds[::2, 0] = bad
+        if T > 1:
+            inds[1] = bad
+        _poison(cuda)
+        y = fp4.experts(x, inds, weights, gu, dn)
+        assert _status(cuda) == 2  # LQ_DEV_BOUNDS
+        want = _experts(x, inds, weights, gv, dv)
+        assert bool(torch.isfinite(y).all()) and (T == 1 or not bool(y[1].any()))
+        off, once = _rms(y.double() - want), _rms(want.to(_dt(dtype)).double() - want)
+        assert off <= 1.05 * once
+        if T > 1:
+            ys = fp4.switch_glu(x, inds, gu, dn)
+            assert _status(cuda) == 2
+            assert not bool(ys[(inds < 0) | (inds >= E)].any()) and bool(torch.isfinite(ys).all())
+
+
+@pytest.mark.parametrize("T,k,E", [(1, 2, 4), (40, 3, 6), (200, 2, 40), (1500, 2, 6)])
+def test_a_grouping_marks_pairs_of_no_expert_and_its_readers_skip_them(cuda, T, k, E):
+    import torch
+    from locals_b200 import moe
+
+    g = _gen(cuda, T)
+    inds = torch.randint(-1, E + 1, (T, k), generator=g, device=cuda).to(torch.int32)
+    inds[0, 0] = -1
+    _poison(cuda)
+    order, starts, experts, nseg, pos = moe.group(inds, E)
+    assert _status(cuda) == 2
+    flat = inds.reshape(-1)
+    fine = (flat >= 0) & (flat < E)
+    n = int(fine.sum())
+    want = torch.argsort(torch.where(fine, flat, E), stable=True)[:n]
+    assert torch.equal(order[:n].long(), want) and bool((order[n:] == -1).all())
+    assert bool((pos[~fine] == -1).all()) and torch.equal(pos[want].long(), torch.arange(n, device=cuda))
+    assert int(starts[int(nseg)]) == n
+    x = torch.randn((T, 64), generator=g, device=cuda).to(torch.bfloat16)
+    xs = moe.gather(x, order, k)
+    assert torch.equal(xs[:n], x[want // k]) and not bool(xs[n:].any())
+    ys = torch.randn((T * k, 64), generator=g, device=cuda).to(torch.bfloat16)
+    w = torch.rand((T, k), generator=g, device=cuda)
+    kept = torch.where(fine[:, None], ys[pos.long().clamp(min=0)], torch.zeros_like(ys))  # the same sums, of zeros in their place
+    a, b = moe.combine(ys, w, pos), moe.combine(kept, w, None)
+    assert torch.equal(a, b)
+    odd = moe.combine(ys[:, :63].contiguous(), w, pos)  # one column a thread
+    assert torch.equal(odd, b[:, :63])
+    res, nw = torch.randn((T, 64), generator=g, device=cuda).to(torch.bfloat16), torch.ones(64, device=cuda, dtype=torch.bfloat16)
+    for p, q in zip(moe.combine_norm(ys, w, pos, res, nw, 1e-5), moe.combine_norm(kept, w, None, res, nw, 1e-5)):
+        assert torch.equal(p, q)
+    assert _status(cuda) == 0
+
+
+def test_one_tokens_affine_down_projection_skips_a_pair_of_no_expert(cuda):
+    import torch
+    from locals_b200 import moe
+
+    g = _gen(cuda, 4)
+    E, D, I = 4, 256, 512
+    w = torch.randint(-2 ** 31, 2 ** 31, (E, D, I // 8), generator=g, device=cuda).to(torch.int32)
+    s, b = (torch.rand((E, D, I // 64), generator=g, device=cuda).to(torch.bfloat16) * 0.01 for _ in range(2))
+    h = torch.randn((3, I), generator=g, device=cuda).to(torch.bfloat16)
+    weights = torch.rand((1, 3), generator=g, device=cuda)
+    grouping = moe.group(torch.tensor([[2, -1, 0]], device=cuda, dtype=torch.int32), E)
+    assert _status(cuda) == 2
+    y = moe.down_combine(h, grouping, weights, (w, s, b))
+    assert y is not None and _status(cuda) == 2
+    rest = moe.group(torch.tensor([[2, 0]], device=cuda, dtype=torch.int32), E)
+    want = moe.down_combine(h[:2].contiguous(), rest, weights[:, [0, 2]].contiguous(), (w, s, b))
+    assert torch.equal(y, want)
