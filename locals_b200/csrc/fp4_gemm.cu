@@ -543,7 +543,10 @@ __global__ void __launch_bounds__(FP4_THREADS, S::T <= 32 ? 2 : 1) fp4_gemm_kern
             for (int lin = first; lin < ntiles && ok; lin += step) {
                 if (!fp4_tile<S>(a, seg, lin, t)) continue;
                 int src = t.r0 + lane < t.r1 ? t.r0 + lane : -1;  // the row of x of the tile's token `lane`
-                if (a.gather && src >= 0) src = (a.order ? a.order[src] : src) / a.gather;
+                if (a.gather && src >= 0) {
+                    const int pair = a.order ? a.order[src] : src;
+                    src = pair < 0 ? -1 : pair / a.gather;
+                }
                 if (src >= a.src_rows || (src < 0 && t.r0 + lane < t.r1)) {
                     record_status(LQ_DEV_BOUNDS);
                     src = -1;  // zeros
@@ -741,8 +744,9 @@ __global__ void __launch_bounds__(256) fp4_split_kernel(const SplitArgs a) {
         const int row = int(u / parts), part = int(u - int64_t(row) * parts);
         int64_t src = row;
         if (a.gather) {
-            src = (a.order ? a.order[row] : row) / a.gather;
-            if (src < 0 || src >= a.src_rows) {
+            const int pair = a.order ? a.order[row] : row;
+            src = pair / a.gather;
+            if (pair < 0 || src >= a.src_rows) {
                 if (lane == 0) record_status(LQ_DEV_BOUNDS);
                 src = -1;  // zeros
             }

@@ -196,3 +196,32 @@ def test_one_tokens_affine_down_projection_skips_a_pair_of_no_expert(cuda):
     rest = moe.group(torch.tensor([[2, 0]], device=cuda, dtype=torch.int32), E)
     want = moe.down_combine(h[:2].contiguous(), rest, weights[:, [0, 2]].contiguous(), (w, s, b))
     assert torch.equal(y, want)
+
+
+@pytest.mark.parametrize("P,gather", [(4, 2), (4, 3), (200, 2), (700, 5)])
+def test_a_negative_row_to_gather_is_recorded_and_zeros(cuda, P, gather):
+    """-1 .. -(gather - 1) are no rows either (divided, they would be row 0): in the product that makes its pieces itself (few rows)
+    and in the split before it."""
+    import torch
+    from locals_b200 import _lib
+    from locals_b200.kernels import _stream
+
+    g = _gen(cuda, P)
+    N, K = 64, 128
+    w, wv = _stack(cuda, g, 1, N, K)
+    x = torch.randn((P, K), generator=g, device=cuda).to(torch.bfloat16)
+    order = torch.arange(P, device=cuda, dtype=torch.int32) * gather
+    bad = torch.tensor([1, P // 2, P - 1], device=cuda)
+    order[bad] = torch.tensor([-1, 1 - gather, -2 ** 31], device=cuda, dtype=torch.int32)
+    starts, ids, nseg = (torch.tensor(v, device=cuda, dtype=torch.int32) for v in ([0, P], [0], [1]))
+    out = torch.full((P, N), 5.0, device=cuda, dtype=torch.bfloat16)
+    n = _lib.lib().lq_fp4_experts_workspace(P, P, 1, N, K, _lib.BF16)
+    ws = torch.empty(n, dtype=torch.uint8, device=cuda)
+    _lib.call("lq_fp4_experts", x.data_ptr(), P, order.data_ptr(), gather, starts.data_ptr(), ids.data_ptr(), nseg.data_ptr(), P, P, 0,
+              w.codes.data_ptr(), w.tiles.data_ptr(), out.data_ptr(), 1, N, K, _lib.BF16, ws.data_ptr() if n else None, n, _stream())
+    assert _status(cuda) == 2
+    assert not bool(out[bad].any())
+    keep = torch.ones(P, dtype=torch.bool, device=cuda)
+    keep[bad] = False
+    want, bound = R.linear(x[keep], wv[0], torch.bfloat16)
+    assert bool(((out[keep].double() - want).abs() <= bound).all())
