@@ -324,7 +324,7 @@ int lq_kv4_attend(const void* q, int N, const int32_t* q_start, int max_q, const
 /* codes and tiles of x (rows, K), f16 / bf16 / f32, x_row elements from one row to the next. LQ_MXFP4: scale
  * 2^max(floor(log2 amax) - 2, -127). LQ_NVFP4: the e4m3 number nearest to amax / (6 factor), at most 448. Codes: nearest to
  * x / (scale * factor), ties to the even code, 6 beyond it. A group that holds an infinity or no number gets the scale that is
- * not a number. factor: 1 float32 > 0 (LQ_NVFP4), or NULL. */
+ * not a number, a group of zeros scale 0. factor: 1 float32 > 0 (LQ_NVFP4; 0 for a matrix of zeros), or NULL. */
 int lq_fp4_quantize(const void* x, int dtype, int64_t x_row, int rows, int K, int mode, const float* factor,
                     uint32_t* codes, uint8_t* tiles, void* stream);
 

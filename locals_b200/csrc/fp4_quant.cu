@@ -64,7 +64,8 @@ __global__ void __launch_bounds__(256) fp4_quantize_kernel(const T* __restrict__
                 x8[i].times(up, v);
                 w = codes8(v);
             } else {
-                byte = top == INFINITY ? 0x7Fu : e4m3_of(double(top) / (6.0 * double(f)));
+                // (zeros have scale 0 whatever the factor is: that of a matrix of zeros is 0 where it is made of its largest)
+                byte = top == INFINITY ? 0x7Fu : top == 0.f ? 0u : e4m3_of(double(top) / (6.0 * double(f)));
                 const float s = fp4_scale_value(byte, LQ_NVFP4);
                 w = 0;
                 if (byte != 0 && byte != 0x7F) {

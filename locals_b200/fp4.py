@@ -108,7 +108,7 @@ def interleave(gate: Tuple[torch.Tensor, torch.Tensor], up: Tuple[torch.Tensor, 
 def quantize(x: torch.Tensor, mode: str = "mxfp4", scale: Optional[torch.Tensor] = None) -> Fp4:
     """x (..., K) in fp16, bf16 or fp32 to 4 bits, its leading dimensions flattened to rows. mxfp4: a group's scale is
     2^(floor(log2 of its largest magnitude) - 2). nvfp4: the e4m3 number nearest to that magnitude / (6 scale), where ``scale``
-    (one float32 element > 0; None: 1) is the matrix' factor, such as its largest magnitude / 2688. Codes are the nearest to
+    (one float32 element > 0; None: 1) is the matrix' factor, such as its largest magnitude / 2688 (0 for a matrix of zeros). Codes are the nearest to
     x / (their scales), ties to the even code, and 6 beyond it. A group with an infinity or no number in it has the scale that is
     not a number."""
     return Fp4(*ext().fp4_quantize(x, mode, scale), mode, x.shape[-1], scale)

@@ -225,3 +225,28 @@ def test_a_negative_row_to_gather_is_recorded_and_zeros(cuda, P, gather):
     keep[bad] = False
     want, bound = R.linear(x[keep], wv[0], torch.bfloat16)
     assert bool(((out[keep].double() - want).abs() <= bound).all())
+
+
+# ---- quantize, and the matrices' factors -----------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("rows,K", [(1, 16), (3, 40), (200, 640)])
+def test_a_matrix_of_zeros_with_its_own_factor_is_zeros(cuda, dtype, rows, K):
+    """Its largest magnitude / 2688 is 0: scales and codes are 0, and so is every product with it."""
+    import torch
+    from locals_b200 import fp4
+
+    x = torch.zeros((rows, K), device=cuda, dtype=_dt(dtype))
+    x[:, ::3] = -0.0
+    f = (x.float().abs().amax() / 2688).reshape(1)
+    assert float(f) == 0
+    _poison(cuda)
+    a = fp4.quantize(x, "nvfp4", scale=f)
+    assert not bool(a.codes.any()) and not bool(fp4.unpack(a)[1].any())
+    assert bool((fp4.dequantize(a, torch.float32) == 0).all())
+    w = torch.randn((70, K), generator=_gen(cuda, K), device=cuda)
+    fw = (w.abs().amax() / 2688).reshape(1)
+    q = fp4.quantize(w, "nvfp4", scale=fw)
+    for y in (fp4.matmul(a, q, dtype=torch.float32), fp4.matmul(q, a, dtype=torch.float32), fp4.matmul(a, q, dtype=torch.float32, glu=True)):
+        assert bool((y == 0).all())
+    assert _status(cuda) == 0
