@@ -159,6 +159,18 @@ __device__ __forceinline__ bool fp4_tile(const Fp4Args& a, const Fp4Segments& se
 // divisor is).
 __device__ __forceinline__ float fp4_silu(float x) { return __fdividef(x, 1.f + __expf(-x)); }
 
+// The product of the matrices' factors, as two numbers to multiply a sum by in turn: the second is 1 but where the product is
+// beyond 2^120 or below 2^-121. Multiplied first, factors of 1e-22 each were 0 or a few bits, and two of 1e25 an infinity,
+// whatever the sum is.
+__device__ __forceinline__ float2 fp4_factors(const Fp4Args& a) {
+    int ex, ew;
+    const float mx = frexpf(a.xf ? *a.xf : 1.f, &ex), mw = frexpf(a.wf ? *a.wf : 1.f, &ew);
+    const float m = mx * mw;
+    if (!(fabsf(m) < 1.f)) return make_float2(m, 1.f);  // (an infinity or no number)
+    const int e = ex + ew, e1 = max(-120, min(120, e));
+    return make_float2(ldexpf(m, e1), ldexpf(1.f, max(-126, min(126, e - e1))));
+}
+
 __device__ __forceinline__ void fp4_store(const Fp4Args& a, int64_t at, float v) {
     if (a.dtype == LQ_F32)
         reinterpret_cast<float*>(a.y)[at] = v;
@@ -179,13 +191,13 @@ __device__ __forceinline__ void fp4_out(const Fp4Args& a, const Fp4Tile& t, int 
     }
 }
 
-// 16 output columns (tokens) of a warp's 32 rows of w, v[c] the sum of this lane's row and token c0 + c: turned to rows of y
+// 16 output columns (tokens) of a warp's 32 rows of w, v[c] the value of this lane's row and token c0 + c: turned to rows of y
 // through shared memory, so that a token's 32 values leave in pieces of 16 bytes. Neighbouring lanes first swap
 // columns: the even lane then has two rows of an even column, the odd lane two of an odd one. The type and form are fixed
 // here, not asked for at each value: with branches between the shuffles they ran one after another (1,670 cycles, not 150).
 template <typename O, bool GLU, int TURN>
-__device__ __forceinline__ void fp4_out16_t(const Fp4Args& a, const Fp4Tile& t, int c0, int nb, const float (&v)[16], float f,
-                                            uint8_t* stage, int lane) {
+__device__ __forceinline__ void fp4_out16_t(const Fp4Args& a, const Fp4Tile& t, int c0, int nb, const float (&v)[16], uint8_t* stage,
+                                            int lane) {
     constexpr int BYTES = (GLU ? 16 : 32) * int(sizeof(O)), PER = BYTES / 16;  // of a token's values here
     const bool odd = lane & 1;
     const int64_t width = GLU ? a.N / 2 : a.N;
@@ -207,17 +219,17 @@ __device__ __forceinline__ void fp4_out16_t(const Fp4Args& a, const Fp4Tile& t, 
 #pragma unroll
         for (int c1 = 0; c1 < 16; c1 += AT) {
 #pragma unroll
-            for (int c = 0; c < AT; ++c) reinterpret_cast<float*>(stage + c * BYTES)[lane] = v[c1 + c] * f;
+            for (int c = 0; c < AT; ++c) reinterpret_cast<float*>(stage + c * BYTES)[lane] = v[c1 + c];
             leave(c1, std::integral_constant<int, AT>());
         }
     } else {
         static_assert(16 * BYTES <= TURN, "16 tokens fit");
         float got[8];
 #pragma unroll
-        for (int c = 0; c < 8; ++c) got[c] = __shfl_xor_sync(0xFFFFFFFFu, odd ? v[2 * c] : v[2 * c + 1], 1) * f;
+        for (int c = 0; c < 8; ++c) got[c] = __shfl_xor_sync(0xFFFFFFFFu, odd ? v[2 * c] : v[2 * c + 1], 1);
 #pragma unroll
         for (int c = 0; c < 8; ++c) {
-            const float mine = (odd ? v[2 * c + 1] : v[2 * c]) * f, lo = odd ? got[c] : mine, hi = odd ? mine : got[c];
+            const float mine = odd ? v[2 * c + 1] : v[2 * c], lo = odd ? got[c] : mine, hi = odd ? mine : got[c];
             uint8_t* row = stage + (2 * c + odd) * BYTES;
             if constexpr (GLU) {
                 const float h = fp4_silu(lo) * hi;
@@ -234,28 +246,28 @@ __device__ __forceinline__ void fp4_out16_t(const Fp4Args& a, const Fp4Tile& t, 
 }
 
 template <int TURN>
-__device__ __forceinline__ void fp4_out16(const Fp4Args& a, const Fp4Tile& t, int c0, int nb, const float (&v)[16], float f,
-                                          uint8_t* stage, int lane) {
+__device__ __forceinline__ void fp4_out16(const Fp4Args& a, const Fp4Tile& t, int c0, int nb, const float (&v)[16], uint8_t* stage,
+                                          int lane) {
     if (a.glu) {
         if (a.dtype == LQ_BF16)
-            fp4_out16_t<__nv_bfloat16, true, TURN>(a, t, c0, nb, v, f, stage, lane);
+            fp4_out16_t<__nv_bfloat16, true, TURN>(a, t, c0, nb, v, stage, lane);
         else if (a.dtype == LQ_F16)
-            fp4_out16_t<__half, true, TURN>(a, t, c0, nb, v, f, stage, lane);
+            fp4_out16_t<__half, true, TURN>(a, t, c0, nb, v, stage, lane);
         else
-            fp4_out16_t<float, true, TURN>(a, t, c0, nb, v, f, stage, lane);
+            fp4_out16_t<float, true, TURN>(a, t, c0, nb, v, stage, lane);
     } else {
         if (a.dtype == LQ_BF16)
-            fp4_out16_t<__nv_bfloat16, false, TURN>(a, t, c0, nb, v, f, stage, lane);
+            fp4_out16_t<__nv_bfloat16, false, TURN>(a, t, c0, nb, v, stage, lane);
         else if (a.dtype == LQ_F16)
-            fp4_out16_t<__half, false, TURN>(a, t, c0, nb, v, f, stage, lane);
+            fp4_out16_t<__half, false, TURN>(a, t, c0, nb, v, stage, lane);
         else
-            fp4_out16_t<float, false, TURN>(a, t, c0, nb, v, f, stage, lane);
+            fp4_out16_t<float, false, TURN>(a, t, c0, nb, v, stage, lane);
     }
 }
 
 // Four neighbouring rows of w (two pairs of gate and up) and one token.
-__device__ __forceinline__ void fp4_out4(const Fp4Args& a, const Fp4Tile& t, int c, int n, float4 v, float f) {
-    float o[4] = {v.x * f, v.y * f, v.z * f, v.w * f};
+__device__ __forceinline__ void fp4_out4(const Fp4Args& a, const Fp4Tile& t, int c, int n, float4 v) {
+    float o[4] = {v.x, v.y, v.z, v.w};
     const int width = a.glu ? a.N / 2 : a.N, at = a.glu ? n / 2 : n, some = a.glu ? 2 : 4;
     if (a.glu) {
         o[0] = fp4_silu(o[0]) * o[1];
@@ -606,7 +618,7 @@ __global__ void __launch_bounds__(FP4_THREADS, S::T <= 32 ? 2 : 1) fp4_gemm_kern
     } else {
         // ------------------------------ epilogue: two warps (few 16-bit tokens: one) a quarter of the lanes ------------------------------
         grid_dep_wait();
-        const float f = (a.xf ? *a.xf : 1.f) * (a.wf ? *a.wf : 1.f);
+        const float2 f = S::KIND == FP4_SPLIT ? make_float2(1.f, 1.f) : fp4_factors(a);
         // 16-byte pieces of y: its rows start on 16-byte boundaries
         const int ysize = (a.glu ? a.N / 2 : a.N) * (a.dtype == LQ_F32 ? 4 : 2);
         const bool wide = ysize % 16 == 0 && reinterpret_cast<uintptr_t>(a.y) % 16 == 0;
@@ -664,11 +676,21 @@ __global__ void __launch_bounds__(FP4_THREADS, S::T <= 32 ? 2 : 1) fp4_gemm_kern
                     if (CG == 1 && a.ks > 1) {
 #pragma unroll
                         for (int q = 0; q < 16; ++q) part[(c0 + c + q) * 128 + 32 * quarter + lane] = u[q];
-                    } else if (wide && nb + 32 <= a.N) {
-                        if (t.r0 + c0 + c < t.r1) fp4_out16<S::TURN>(a, t, c0 + c, nb, u, f, stage + S::TURN * warp, lane);
                     } else {
+                        if constexpr (S::KIND != FP4_SPLIT) {
 #pragma unroll
-                        for (int q = 0; q < 16; ++q) fp4_out<S>(a, t, c0 + c + q, n, u[q] * f);
+                            for (int q = 0; q < 16; ++q) u[q] *= f.x;
+                            if (f.y != 1.f) {
+#pragma unroll
+                                for (int q = 0; q < 16; ++q) u[q] *= f.y;
+                            }
+                        }
+                        if (wide && nb + 32 <= a.N) {
+                            if (t.r0 + c0 + c < t.r1) fp4_out16<S::TURN>(a, t, c0 + c, nb, u, stage + S::TURN * warp, lane);
+                        } else {
+#pragma unroll
+                            for (int q = 0; q < 16; ++q) fp4_out<S>(a, t, c0 + c + q, n, u[q]);
+                        }
                     }
                 }
             }
@@ -682,7 +704,7 @@ __global__ void __launch_bounds__(FP4_THREADS, S::T <= 32 ? 2 : 1) fp4_gemm_kern
         cluster_sync();
         Fp4Tile t;
         if (warp < FP4_OUT && first < ntiles && fp4_tile<S>(a, seg, first, t)) {
-            const float f = (a.xf ? *a.xf : 1.f) * (a.wf ? *a.wf : 1.f);
+            const float2 f = S::KIND == FP4_SPLIT ? make_float2(1.f, 1.f) : fp4_factors(a);
             const uint32_t part = smem_u32(smem) + lane * 16;  // a lane takes four rows of w
             for (int c = rank + a.ks * warp; c < T && t.r0 + c < t.r1; c += FP4_OUT * a.ks) {
                 float4 p[8];
@@ -698,7 +720,8 @@ __global__ void __launch_bounds__(FP4_THREADS, S::T <= 32 ? 2 : 1) fp4_gemm_kern
                         v.z += p[q].z;
                         v.w += p[q].w;
                     }
-                fp4_out4(a, t, c, t.n0 + 4 * lane, v, f);
+                if constexpr (S::KIND != FP4_SPLIT) v = make_float4(v.x * f.x * f.y, v.y * f.x * f.y, v.z * f.x * f.y, v.w * f.x * f.y);
+                fp4_out4(a, t, c, t.n0 + 4 * lane, v);
             }
         }
         __syncwarp();

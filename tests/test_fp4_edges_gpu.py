@@ -250,3 +250,37 @@ def test_a_matrix_of_zeros_with_its_own_factor_is_zeros(cuda, dtype, rows, K):
     for y in (fp4.matmul(a, q, dtype=torch.float32), fp4.matmul(q, a, dtype=torch.float32), fp4.matmul(a, q, dtype=torch.float32, glu=True)):
         assert bool((y == 0).all())
     assert _status(cuda) == 0
+
+
+@pytest.mark.parametrize("M,N,K", [(1, 96, 256), (17, 130, 64), (70, 96, 256), (300, 257, 256)])
+@pytest.mark.parametrize("fx,fw", [(1e-22, 3e-22), (1e-30, 1e-10), (2e25, 1e25), (1e-40, 1e30), (3e38, 3e38), (1e-45, 1e-45), (0.7, 1.3)])
+def test_factors_near_the_ends_of_the_range(cuda, M, N, K, fx, fw):
+    """A product of factors that 32 bits do not hold does not spoil sums that its result does: 0 stays 0, and what is a normal
+    number has its bits."""
+    import torch
+    from locals_b200 import fp4
+
+    g = _gen(cuda, M)
+
+    def operand(rows, f, zero):
+        codes = torch.randint(0, 16, (rows, K), generator=g, device=cuda, dtype=torch.int32)
+        byte = torch.randint(1, 127, (rows, K // 16), generator=g, device=cuda).to(torch.uint8)
+        codes[zero] = 0
+        words = (codes.unflatten(-1, (-1, 8)) << (4 * torch.arange(8, device=cuda, dtype=torch.int32))).sum(-1, dtype=torch.int32)
+        t = torch.tensor([f], device=cuda)
+        return fp4.pack(words, byte, "nvfp4", t), R.values(codes, byte, "nvfp4", K), t.double()
+
+    x, xv, dx = operand(M, fx, 0)
+    w, wv, dw = operand(N, fw, 1)
+    f = dx * dw
+    want = (xv @ wv.T) * f
+    y = fp4.matmul(x, w, dtype=torch.float32)
+    assert _status(cuda) == 0
+    assert bool((y[0] == 0).all()) and bool((y[:, 1] == 0).all())
+    top = torch.finfo(torch.float32).max
+    # sums in 32 bits; the product of the factors, and its product with a sum, rounded once each; what is no normal number to the step there
+    bound = R.lost(K, xv, wv) * f + 2.0 ** -22 * want.abs() + 2 * 2.0 ** -149
+    fine = want.abs() + bound < top
+    assert bool(((y.double() - want).abs() <= bound)[fine].all())
+    over = want.abs() - bound > top * (1 + 2.0 ** -24)
+    assert torch.equal(y[over], (torch.sign(want) * float("inf")).float()[over])
