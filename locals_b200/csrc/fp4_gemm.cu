@@ -155,9 +155,13 @@ __device__ __forceinline__ bool fp4_tile(const Fp4Args& a, const Fp4Segments& se
     return true;
 }
 
-// x / (1 + e^-x) by the fast exponential and quotient (a few units of 2^-23; 0 below -88, where the quotient of so large a
-// divisor is).
-__device__ __forceinline__ float fp4_silu(float x) { return __fdividef(x, 1.f + __expf(-x)); }
+// x / (1 + e^-x), below 0 as x e^x / (1 + e^x), so that no exponential overflows and the divisor is 1 to 2: some four units in the
+// last place, down to where e^x is no normal number (-87.3; its own step there, 2^-149, times x). (The fast exponential's error
+// grows with |x|: 25 units at -20, some 95 at -80.)
+__device__ __forceinline__ float fp4_silu(float x) {
+    const float t = expf(-fabsf(x)), s = __fdividef(x, 1.f + t);
+    return x < 0.f ? s * t : s;
+}
 
 // The product of the matrices' factors, as two numbers to multiply a sum by in turn: the second is 1 but where the product is
 // beyond 2^120 or below 2^-121. Multiplied first, factors of 1e-22 each were 0 or a few bits, and two of 1e25 an infinity,

@@ -284,3 +284,39 @@ def test_factors_near_the_ends_of_the_range(cuda, M, N, K, fx, fw):
     assert bool(((y.double() - want).abs() <= bound)[fine].all())
     over = want.abs() - bound > top * (1 + 2.0 ** -24)
     assert torch.equal(y[over], (torch.sign(want) * float("inf")).float()[over])
+
+
+# ---- SwiGLU ------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("mode", ["mxfp4", "nvfp4"])
+@pytest.mark.parametrize("M", [1, 20, 70, 200, 300])
+def test_glu_of_gates_far_below_zero(cuda, mode, M):
+    """silu in 32 bits has its bits where the gate is -10 to -100. expf is off by one unit in the last place (2^-23 of the value at
+    most), the fast quotient by two for divisors in range, the sum with 1, the product and the product with up round once each
+    (2^-24): 3 * 2^-23 + 3 * 2^-24 in all; where e^gate is no normal number, that is off by a step of 2^-149 at most, which the gate
+    and up (64) multiply."""
+    import torch
+    from locals_b200 import fp4
+
+    K, gates = 32, [-0.5 * i for i in range(0, 201)] + [0.5 * i for i in range(1, 41)]
+    left = torch.tensor(gates).double()
+    codes = torch.zeros((len(gates), 2, K), dtype=torch.int32)
+    values = [6.0, 4.0, 3.0, 2.0, 1.5, 1.0, 0.5]
+    for k in range(K):  # each gate as a sum of K values, the largest first
+        for c, v in zip(range(7, 0, -1), values):
+            take = (left.abs() >= v) & (codes[:, 0, k] == 0)
+            codes[take, 0, k] = torch.where(left[take] < 0, c + 8, c).to(torch.int32)
+            left = torch.where(take, left - torch.sign(left) * v, left)
+    assert not left.any()
+    codes[:, 1, :16] = 6  # up: 16 times 4
+    words = (codes.flatten(0, 1).unflatten(-1, (-1, 8)) << (4 * torch.arange(8, dtype=torch.int32))).sum(-1, dtype=torch.int32)
+    one = 127 if mode == "mxfp4" else 0x38
+    w = fp4.pack(words.to(cuda), torch.full((2 * len(gates), K // R.GROUP[mode]), one, dtype=torch.uint8, device=cuda), mode)
+    x = fp4.pack(torch.full((M, K // 8), 0x22222222, dtype=torch.int32, device=cuda),
+                 torch.full((M, K // R.GROUP[mode]), one, dtype=torch.uint8, device=cuda), mode)
+    y = fp4.matmul(x, w, dtype=torch.float32, glu=True)
+    assert _status(cuda) == 0
+    g = torch.tensor(gates, dtype=torch.float64, device=cuda)
+    want = 64 * g / (1 + torch.exp(-g))
+    bound = (3 * 2.0 ** -23 + 3 * 2.0 ** -24) * want.abs() + 2.0 ** -149 * 64 * g.abs() + 2.0 ** -149
+    assert bool(((y.double() - want).abs() <= bound).all())
