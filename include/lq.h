@@ -328,7 +328,8 @@ int lq_kv4_attend(const void* q, int N, const int32_t* q_start, int max_q, const
 int lq_fp4_quantize(const void* x, int dtype, int64_t x_row, int rows, int K, int mode, const float* factor,
                     uint32_t* codes, uint8_t* tiles, void* stream);
 
-/* out (stack * rows, K) in dtype (f16 / bf16 / f32) = code * scale * factor, rounded once. */
+/* out (stack * rows, K) in dtype (f16 / bf16 / f32) = code * scale * factor, rounded once; with a factor and a 16-bit dtype, to 32 bits
+ * first. */
 int lq_fp4_dequantize(const uint32_t* codes, const uint8_t* tiles, int stack, int rows, int K, int mode,
                       const float* factor, int dtype, void* out, void* stream);
 

@@ -1,5 +1,4 @@
-// Microscaled 4-bit floating point in and out: quantize, dequantize, and the e4m3 pieces that 16-bit activations enter the
-// block-scaled product as.
+// Microscaled 4-bit floating point in and out: quantize and dequantize.
 //
 // quantize: a lane takes 8 values (one word of codes) at a time, a group is 4 (mxfp4) or 2 (nvfp4) threads, its largest magnitude
 // found with shuffles. mxfp4: scale 2^(floor(log2 amax) - 2), at least 2^-127: the exponent field of amax less 2, so that no

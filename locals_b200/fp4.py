@@ -115,7 +115,7 @@ def quantize(x: torch.Tensor, mode: str = "mxfp4", scale: Optional[torch.Tensor]
 
 
 def dequantize(a: Fp4, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
-    """The values of an operand, (N, K) or (E, N, K), rounded once to ``dtype``."""
+    """The values of an operand, (N, K) or (E, N, K), rounded once to ``dtype`` (with a factor and 16 bits, to 32 bits first)."""
     return ext().fp4_dequantize(a, dtype)
 
 

@@ -320,3 +320,44 @@ def test_glu_of_gates_far_below_zero(cuda, mode, M):
     want = 64 * g / (1 + torch.exp(-g))
     bound = (3 * 2.0 ** -23 + 3 * 2.0 ** -24) * want.abs() + 2.0 ** -149 * 64 * g.abs() + 2.0 ** -149
     assert bool(((y.double() - want).abs() <= bound).all())
+
+
+# ---- dequantize ----------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("f", [1e-38, 3e-40, 1.0, 1e35, 3e38])
+def test_dequantize_with_factors_near_the_ends_of_the_range(cuda, dtype, f):
+    import torch
+    from locals_b200 import fp4
+
+    g = _gen(cuda, 7)
+    codes = torch.randint(0, 16, (40, 96), generator=g, device=cuda, dtype=torch.int32)
+    byte = torch.randint(0, 127, (40, 6), generator=g, device=cuda).to(torch.uint8)
+    words = (codes.unflatten(-1, (-1, 8)) << (4 * torch.arange(8, device=cuda, dtype=torch.int32))).sum(-1, dtype=torch.int32)
+    scale = torch.tensor([f], device=cuda)
+    want = R.values(codes, byte, "nvfp4", 96, scale)
+    got = fp4.dequantize(fp4.pack(words, byte, "nvfp4", scale), _dt(dtype)).double()
+    i = torch.finfo(_dt(dtype))
+    over = want.abs() >= i.max * (1 + R.half_step(_dt(dtype))) * (1 + 2.0 ** -23)
+    assert torch.equal(got[over], torch.sign(want[over]) * float("inf"))
+    # half a step of the type, and half a step of 32 bits for the product with the factor before it
+    once = torch.maximum(R.half_step(_dt(dtype)) * want.abs(), torch.tensor(i.smallest_normal * i.eps / 2, dtype=torch.float64, device=cuda))
+    bound = once + torch.maximum(2.0 ** -24 * want.abs(), torch.tensor(2.0 ** -150, dtype=torch.float64, device=cuda))
+    under = want.abs() <= i.max
+    assert bool(((got - want).abs() <= bound)[under].all())
+
+
+# ---- refusals ------------------------------------------------------------------------------------------------
+
+def test_glu_of_an_odd_number_of_rows_is_refused(cuda):
+    import torch
+    from locals_b200 import fp4
+
+    g = _gen(cuda, 1)
+    w = fp4.quantize(torch.randn((95, 128), generator=g, device=cuda))
+    x = torch.randn((4, 128), generator=g, device=cuda).to(torch.bfloat16)
+    for a in (x, fp4.quantize(x)):
+        assert fp4.matmul(a, w).shape == (4, 95)
+        with pytest.raises(ValueError, match="gate and up"):
+            fp4.matmul(a, w, glu=True)
+    assert _status(cuda) == 0
