@@ -917,7 +917,11 @@ static int gemm_t(const Fp4Call& c, cudaStream_t st) {
     const size_t smem = S::beside(a.grouped) + size_t(a.nst) * S::STAGE;
     static_assert(S::ACC == 256 || S::T * 512 <= S::stages(true) * S::STAGE, "the partial sums of a split fit the ring");
     auto kern = fp4_gemm_kernel<S>;
-    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem)) != cudaSuccess ||
+    // The same limit at every call: set to the call's own size, a dense call on one host thread lowered it between a grouped call's
+    // setting and its launch on another, which was then refused.
+    constexpr size_t dense = S::beside(false) + size_t(S::stages(false)) * S::STAGE, grouped = S::beside(true) + size_t(S::stages(true)) * S::STAGE;
+    constexpr int limit = int(dense > grouped ? dense : grouped);
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, limit) != cudaSuccess ||
         cudaFuncSetAttribute(kern, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared) != cudaSuccess)
         return LQ_E_CUDA;
     // Few tiles: a tile's K split over as many CTAs of a cluster as still run all at once, each with a stage at least.

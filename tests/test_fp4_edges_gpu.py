@@ -361,3 +361,59 @@ def test_glu_of_an_odd_number_of_rows_is_refused(cuda):
         with pytest.raises(ValueError, match="gate and up"):
             fp4.matmul(a, w, glu=True)
     assert _status(cuda) == 0
+
+
+# ---- host threads ----------------------------------------------------------------------------------------------
+
+def _at_once(calls, rounds=3000):
+    """Each call over and over on a host thread and stream of its own (the C ABI's calls run without the interpreter's lock): their
+    return codes."""
+    import threading
+
+    import torch
+
+    codes, go = [set() for _ in calls], threading.Barrier(len(calls))
+
+    def work(i, call, stream):
+        torch.cuda.set_device(0)
+        go.wait()
+        for _ in range(rounds):
+            codes[i].add(call(stream))
+
+    streams = [torch.cuda.Stream() for _ in calls]
+    threads = [threading.Thread(target=work, args=(i, c, s.cuda_stream)) for i, (c, s) in enumerate(zip(calls, streams))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    return codes
+
+
+def test_dense_and_grouped_products_of_two_host_threads(cuda):
+    """They run the same kernel with shared memory of different sizes."""
+    import torch
+    from locals_b200 import _lib
+
+    L, g = _lib.lib(), _gen(cuda, 3)
+    N, K, M, P = 128, 256, 40, 96
+    w, wv = _stack(cuda, g, 2, N, K)
+    x = torch.randn((P, K), generator=g, device=cuda).to(torch.bfloat16)
+    starts, ids, nseg = (torch.tensor(v, device=cuda, dtype=torch.int32) for v in ([0, 50, P], [0, 1], [2]))
+    y, z = (torch.zeros((n, N), device=cuda, dtype=torch.bfloat16) for n in (M, P))
+    n1, n2 = L.lq_fp4_linear_workspace(M, N, K, _lib.BF16), L.lq_fp4_experts_workspace(P, P, 2, N, K, _lib.BF16)
+    w1, w2 = (torch.empty(max(n, 1), device=cuda, dtype=torch.uint8) for n in (n1, n2))
+    torch.cuda.synchronize()
+
+    def dense(st):
+        return L.lq_fp4_linear(x.data_ptr(), K, w.codes.data_ptr(), w.tiles.data_ptr(), M, N, K, 0, _lib.BF16, y.data_ptr(), w1.data_ptr(), n1, st)
+
+    def grouped(st):
+        return L.lq_fp4_experts(x.data_ptr(), P, None, 0, starts.data_ptr(), ids.data_ptr(), nseg.data_ptr(), P, P, 0, w.codes.data_ptr(),
+                                w.tiles.data_ptr(), z.data_ptr(), 2, N, K, _lib.BF16, w2.data_ptr(), n2, st)
+
+    assert _at_once([dense, grouped]) == [{0}, {0}]
+    assert _status(cuda) == 0
+    for got, rows, m in ((y, slice(0, M), wv[0]), (z[:50], slice(0, 50), wv[0]), (z[50:], slice(50, P), wv[1])):
+        want, bound = R.linear(x[rows], m, torch.bfloat16)
+        assert bool(((got.double() - want).abs() <= bound).all())
