@@ -160,6 +160,7 @@ __global__ void group_kernel(const uint32_t* inds, int P, int E, int32_t* order,
 // places its pairs in pair order (a match over each 32 pairs ranks equal experts by lane). Pair p of expert e lands
 // after every earlier pair of e, exactly as in group_kernel: the same order, starts, experts and pos.
 constexpr int GROUP_PAR_MAX_E = 1024;
+constexpr int GROUP_MAX_E = 8192;  // what lq_moe_group takes
 constexpr int GROUP_CLUSTER_MIN_P = 2049;  // from here a cluster of 8 CTAs (16,004 pairs 36 -> 10 us; 2,048 pairs 6.9 in one)
 
 __global__ void __launch_bounds__(1024) group_par_kernel(const uint32_t* inds, int P, int E, int32_t* order,
@@ -609,9 +610,9 @@ static int group_impl(const uint32_t* inds, int P, int E, int32_t* order, int32_
     if (E <= GROUP_PAR_MAX_E && P > 256) {  // (up to 256 pairs the one-warp placement is as fast)
         const int ctas = P >= GROUP_CLUSTER_MIN_P ? 8 : 1;
         const size_t smem = size_t(ctas > 1 ? 36 : 34) * E * sizeof(int32_t);
-        if (smem > 48 * 1024) {
-            const cudaError_t e =
-                cudaFuncSetAttribute(group_par_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem));
+        if (smem > 48 * 1024) {  // (the most that a call takes: a limit by the call's own size, another host thread's call may lower)
+            const cudaError_t e = cudaFuncSetAttribute(group_par_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                       36 * GROUP_PAR_MAX_E * int(sizeof(int32_t)));
             if (e != cudaSuccess) return LQ_E_CUDA;
         }
         if (ctas > 1) {
@@ -637,7 +638,8 @@ static int group_impl(const uint32_t* inds, int P, int E, int32_t* order, int32_
     }
     const size_t smem = size_t(2) * E * sizeof(int32_t) + size_t(GROUP_STAGE) * sizeof(uint32_t);
     if (smem > 48 * 1024) {
-        const cudaError_t e = cudaFuncSetAttribute(group_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem));
+        const cudaError_t e = cudaFuncSetAttribute(group_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                   (2 * GROUP_MAX_E + GROUP_STAGE) * int(sizeof(int32_t)));
         if (e != cudaSuccess) return LQ_E_CUDA;
     }
     return launch_pdl(group_kernel, dim3(1), dim3(1024), smem, st, inds, P, E, order, starts, experts, nseg, pos, lo,

@@ -417,3 +417,20 @@ def test_dense_and_grouped_products_of_two_host_threads(cuda):
     for got, rows, m in ((y, slice(0, M), wv[0]), (z[:50], slice(0, 50), wv[0]), (z[50:], slice(50, P), wv[1])):
         want, bound = R.linear(x[rows], m, torch.bfloat16)
         assert bool(((got.double() - want).abs() <= bound).all())
+
+
+def test_groupings_of_two_host_threads(cuda):
+    import torch
+    from locals_b200 import _lib
+
+    L, P, calls, keep = _lib.lib(), 2500, [], []
+    for E in (400, 1024):
+        ids = (torch.arange(P, device=cuda, dtype=torch.int32) * 7) % E
+        b = [torch.empty(n, device=cuda, dtype=torch.int32) for n in (P, E + 1, E, 1, P)]
+        keep.append((ids, b, E))
+        calls.append(lambda st, a=(ids.data_ptr(), P, E, *(t.data_ptr() for t in b)): L.lq_moe_group(*a, st))
+    torch.cuda.synchronize()
+    assert _at_once(calls) == [{0}, {0}]
+    assert _status(cuda) == 0
+    for ids, b, E in keep:
+        assert torch.equal(b[0].long(), torch.argsort(ids, stable=True))
