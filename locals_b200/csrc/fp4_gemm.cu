@@ -86,8 +86,7 @@ struct Fp4Shape {
     static constexpr int COLS = SF_COL + 2 * SF_COLS, TMEM = COLS <= 64 ? 64 : COLS <= 128 ? 128 : COLS <= 256 ? 256 : 512;
     static_assert(COLS <= 512 && stages(true) >= 2 && N % 16 == 0 && N <= 256 && B_TILE % 1024 == 0, "tile");
     static_assert(!FUSE || STACK, "few tokens");
-    // Two CTAs of an SM both have their tensor memory: one that waited for the other's could hold up a cluster whose CTAs wait
-    // for one another at their join, and that cluster the other's.
+    // Two CTAs of an SM both have their tensor memory, so that neither waits for the other's work.
     static_assert(T > 32 || TMEM <= 256, "two CTAs an SM");
     static_assert(!STACK || N <= 128, "stacked pieces share one scale tile");
 };
@@ -702,10 +701,23 @@ __global__ void __launch_bounds__(FP4_THREADS, S::T <= 32 ? 2 : 1) fp4_gemm_kern
             ++j;
         }
     }
+    tc_fence_before();
+    __syncwarp();
     if (CG == 1 && a.ks > 1) {
-        // the CTAs of a cluster have one tile: each writes out the columns c with c % ks == its rank
-        __syncwarp();
-        cluster_sync();
+        // The CTAs of a cluster have one tile: each writes out the columns c with c % ks == its rank. Tensor memory is given back
+        // before this one waits for the others' sums: held there, while another CTA of the cluster waits for its own, it could hold
+        // up, and be held up by, a cluster of any kernel that does the same. (Between arriving and waiting, since all warps
+        // together before it cost 0.2 us.)
+        constexpr int readers = 32 * (S::OUT + 1);
+        cluster_arrive();
+        if (warp < S::OUT) named_arrive(1, readers);
+        if (warp == FP4_OUT + 1) {
+            named_barrier(1, readers);
+            tc_fence_after();
+            tc_dealloc<CG>(tmem, S::TMEM);
+            __syncwarp();
+        }
+        cluster_wait();
         Fp4Tile t;
         if (warp < FP4_OUT && first < ntiles && fp4_tile<S>(a, seg, first, t)) {
             const float2 f = S::KIND == FP4_SPLIT ? make_float2(1.f, 1.f) : fp4_factors(a);
@@ -730,9 +742,8 @@ __global__ void __launch_bounds__(FP4_THREADS, S::T <= 32 ? 2 : 1) fp4_gemm_kern
         }
         __syncwarp();
         cluster_sync();
+        return;
     }
-    tc_fence_before();
-    __syncwarp();
     if constexpr (CG == 2)
         cluster_sync();  // neither CTA leaves while the other's MMAs or arrivals may reach it
     else

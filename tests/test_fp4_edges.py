@@ -65,3 +65,40 @@ def test_every_place_that_a_combine_may_read_is_written(P, E, ctas):
     assert sorted(order) == list(range(P)) and sorted(pos) == list(range(P))
     assert all(order[j] == p for p, j in pos.items() if j >= 0)
     assert all((j == -1) == (not 0 <= ids[p] < E) for p, j in pos.items())
+
+
+def _clusters(needs, frees_before_join, seed):
+    """Two clusters of two CTAs, one a SM of 512 columns of tensor memory: each takes `needs` columns of its SM (and waits until it
+    has them), works, and waits for the other of its cluster. "ok", or "deadlock", of a random schedule."""
+    rng = random.Random(seed)
+    free = [512, 512]
+    state = {(c, sm): "start" for c in range(2) for sm in range(2)}
+    while any(v != "done" for v in state.values()):
+        moves = []
+        for (c, sm), v in state.items():
+            if v == "start" and free[sm] >= needs[c]:
+                moves.append((c, sm, "has"))
+            elif v == "has":
+                moves.append((c, sm, "join"))
+            elif v == "join" and state[(c, 1 - sm)] in ("join", "done"):
+                moves.append((c, sm, "done"))
+        if not moves:
+            return "deadlock"
+        c, sm, to = rng.choice(moves)
+        state[(c, sm)] = to
+        if to == "has":
+            free[sm] -= needs[c]
+        if to == ("join" if frees_before_join[c] else "done"):
+            free[sm] += needs[c]
+    return "ok"
+
+
+@pytest.mark.parametrize("needs", [(256, 512), (512, 512), (256, 256), (64, 512)])
+@pytest.mark.parametrize("other", [True, False])
+def test_tensor_memory_given_back_before_the_join_holds_no_cluster_up(needs, other):
+    """The product's clusters (the first), beside a kernel that does the same or holds its own across its join."""
+    assert {_clusters(needs, (True, other), s) for s in range(300)} == {"ok"}
+
+
+def test_tensor_memory_held_across_both_joins_would():
+    assert "deadlock" in {_clusters((256, 512), (False, False), s) for s in range(300)}
