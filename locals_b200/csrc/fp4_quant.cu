@@ -36,7 +36,6 @@ __global__ void __launch_bounds__(256) fp4_quantize_kernel(const T* __restrict__
                                                            uint8_t* __restrict__ tiles) {
     constexpr int LANES = MODE == LQ_MXFP4 ? 4 : 2;  // threads a group
     const int lane = threadIdx.x & 31, words = fp4_padded(K) / 8, ktiles = fp4_ktiles(K, MODE), parts = (words + 32 * UNR - 1) / (32 * UNR);
-    grid_dep_wait();
     const float f = MODE == LQ_NVFP4 && factor ? *factor : 1.f;
     const int64_t tasks = int64_t(rows) * parts;
     for (int64_t u = (int64_t(blockIdx.x) * blockDim.x + threadIdx.x) >> 5; u < tasks; u += (int64_t(gridDim.x) * blockDim.x) >> 5) {
@@ -131,7 +130,6 @@ __global__ void __launch_bounds__(256) fp4_dequantize_kernel(const uint32_t* __r
     constexpr int GROUP = MODE == LQ_MXFP4 ? 32 : 16, UNR = 4;
     const int stored = fp4_padded(K) / 8, words = (K + 7) / 8, ktiles = fp4_ktiles(K, MODE), rtiles = (rows + 127) / 128;
     const int lane = threadIdx.x & 31, parts = (words + 32 * UNR - 1) / (32 * UNR);
-    grid_dep_wait();
     const float f = factor ? *factor : 1.f;
     const int64_t tasks = int64_t(stack) * rows * parts;
     for (int64_t u = (int64_t(blockIdx.x) * blockDim.x + threadIdx.x) >> 5; u < tasks; u += (int64_t(gridDim.x) * blockDim.x) >> 5) {
