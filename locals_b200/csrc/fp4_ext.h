@@ -161,7 +161,8 @@ Tensor grouped(const Tensor& xs, const Tensor& order, const Tensor& starts, cons
     need(gather_k >= 0 && (gather_k || xs.size(0) >= P), "xs has a row a pair, or gather_k says how many pairs a token has");
     const c10::cuda::CUDAGuard guard(b.dev);
     Tensor out = at::empty({P, width(b, glu)}, xs.options());
-    if (out.numel() && xs.size(0)) {
+    if (out.numel()) {
+        need(xs.size(0) >= 1 && max_rows >= 1, "pairs have tokens");
         const int dt = dtype_code(xs);
         const size_t bytes = lq_fp4_experts_workspace(narrow(P), narrow(max_rows), b.stack, b.rows, b.K, dt);
         const Workspace ws(bytes, xs);

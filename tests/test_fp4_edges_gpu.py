@@ -363,6 +363,25 @@ def test_glu_of_an_odd_number_of_rows_is_refused(cuda):
     assert _status(cuda) == 0
 
 
+def test_pairs_without_tokens_are_refused(cuda):
+    """They were answered with whatever the memory held."""
+    import torch
+    from locals_b200 import fp4, moe
+
+    g = _gen(cuda, 1)
+    w, _ = _stack(cuda, g, 3, 64, 128)
+    grouping = moe.group(torch.tensor([0, 2, 1, 1], device=cuda, dtype=torch.int32), 3)
+    x = torch.randn((2, 128), generator=g, device=cuda).to(torch.bfloat16)
+    assert fp4.grouped(x, grouping, w, 2, gather_k=2).shape == (4, 64)
+    with pytest.raises(ValueError):
+        fp4.grouped(x[:0], grouping, w, 2, gather_k=2)
+    with pytest.raises(ValueError):
+        fp4.grouped(x, grouping, w, 0, gather_k=2)
+    none = tuple(torch.empty(n, device=cuda, dtype=torch.int32) for n in (0, 1, 0, 1, 0))
+    assert fp4.grouped(x[:0], none, w, 1, gather_k=2).shape == (0, 64)
+    assert _status(cuda) == 0
+
+
 # ---- host threads ----------------------------------------------------------------------------------------------
 
 def _at_once(calls, rounds=3000):
