@@ -181,7 +181,8 @@ class MoELayer:
 
     def __call__(self, x: torch.Tensor) -> torch.Tensor:
         x2 = x.reshape(-1, x.shape[-1]).contiguous()
-        inds, weights = moe.route(x2, self.router_w, self.top_k, self.mode)
+        with torch.cuda.device(x.device):
+            inds, weights = moe.route(x2, self.router_w, self.top_k, self.mode)
         return experts(x2, inds, weights, self.gate_up, self.down).reshape(x.shape)
 
 
