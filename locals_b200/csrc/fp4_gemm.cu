@@ -379,7 +379,10 @@ __global__ void __launch_bounds__(FP4_THREADS, S::T <= 32 ? 2 : 1) fp4_gemm_kern
         const int n = a.nseg ? min(max(*a.nseg, 0), a.max_seg) : a.M;  // without segments, each row is one
         for (int i = threadIdx.x; i <= n; i += FP4_THREADS) seg.starts[i] = a.starts ? min(max(a.starts[i], 0), a.M) : i;
         for (int i = threadIdx.x; i < n; i += FP4_THREADS) seg.experts[i] = a.experts[i];
-        if (threadIdx.x == 0) seg.n = n;
+        if (threadIdx.x == 0) {
+            seg.n = n;
+            if (a.nseg && *a.nseg != n) record_status(LQ_DEV_BOUNDS);  // a grouping of more experts than there are
+        }
         __syncthreads();
         if (warp == 0) {  // tiles before each segment
             int before = 0;

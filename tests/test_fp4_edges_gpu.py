@@ -382,6 +382,25 @@ def test_pairs_without_tokens_are_refused(cuda):
     assert _status(cuda) == 0
 
 
+@pytest.mark.parametrize("P", [8, 96, 800])
+def test_a_grouping_of_more_experts_than_the_stack_has_is_recorded(cuda, P):
+    """Segments of experts that the stack does not have are left out; those that it has are answered."""
+    import torch
+    from locals_b200 import fp4, moe
+
+    g = _gen(cuda, P)
+    w, wv = _stack(cuda, g, 3, 64, 128)
+    inds = torch.arange(P, device=cuda, dtype=torch.int32) % 8
+    grouping = moe.group(inds, 8)
+    x = torch.randn((P, 128), generator=g, device=cuda).to(torch.bfloat16)
+    got = fp4.grouped(x, grouping, w, P)
+    assert _status(cuda) == 2  # LQ_DEV_BOUNDS
+    ids = inds[grouping[0].long()]
+    for e in range(3):
+        want, bound = R.linear(x[ids == e], wv[e], torch.bfloat16)
+        assert bool(((got[ids == e].double() - want).abs() <= bound).all())
+
+
 # ---- host threads ----------------------------------------------------------------------------------------------
 
 def _at_once(calls, rounds=3000):
