@@ -102,3 +102,138 @@ def test_tensor_memory_given_back_before_the_join_holds_no_cluster_up(needs, oth
 
 def test_tensor_memory_held_across_both_joins_would():
     assert "deadlock" in {_clusters((256, 512), (False, False), s) for s in range(300)}
+
+
+class _Barrier:
+    """An mbarrier: arrivals and bytes outstanding; a phase is over when both are none."""
+
+    def __init__(self, count):
+        self.count, self.pending, self.tx, self.phase = count, count, 0, 0
+
+    def arrive(self, expect=0):
+        self.tx += expect
+        self.pending -= 1
+        self._over()
+
+    def bytes(self, n):
+        self.tx -= n
+        self._over()
+
+    def _over(self):
+        assert self.pending >= 0
+        if self.pending == 0 and self.tx == 0:
+            self.phase += 1
+            self.pending = self.count
+
+    def passes(self, parity):  # a parity wait: the phase of that parity is the last one that is over
+        return self.phase % 2 != parity
+
+
+def _ring(ctas, places, stages, seed):
+    """The wide products' ring of stages: in each CTA a warp for codes and one for scales load a stage's bytes once its place is
+    free there, all of a pair's on the lower rank's barrier, for which one thread says what arrives; the issuer takes a stage when it
+    is full, and its commit frees the place in each CTA. Loads land and commits arrive at any time. "ok", or what went wrong."""
+    rng = random.Random(seed)
+    full = [_Barrier(1) for _ in range(places)]
+    empty = [[_Barrier(1) for _ in range(places)] for _ in range(ctas)]
+    following = {(c, what): 0 for c in range(ctas) for what in ("codes", "scales")}
+    flying, held, commits, used = [], {}, [], 0
+    while used < stages or commits:
+        moves = [("land", i) for i in range(len(flying))]
+        if commits:
+            moves.append(("commit", 0))
+        for key, x in following.items():
+            place, turn = x % places, x // places
+            if x < stages and (turn == 0 or empty[key[0]][place].passes((turn - 1) % 2)):
+                moves.append(("load", key))
+        # (the scales' two places of tensor memory: the stage before last is done)
+        done = used < 2 or empty[0][(used - 2) % places].passes((used - 2) // places % 2)
+        if used < stages and done and full[used % places].passes(used // places % 2):
+            moves.append(("issue", 0))
+        if not moves:
+            return "deadlock"
+        kind, at = rng.choice(moves)
+        if kind == "load":
+            x = following[at]
+            following[at] += 1
+            if at == (0, "codes"):  # what arrives in all CTAs, of both warps
+                full[x % places].arrive(expect=2 * ctas)
+            flying.append((at, x))
+        elif kind == "land":
+            key, x = flying.pop(at)
+            if held.get((key, x % places), -1) >= 0:
+                return "overrun"
+            held[(key, x % places)] = x
+            full[x % places].bytes(1)
+        elif kind == "issue":
+            for key in following:
+                if held.get((key, used % places), -1) != used:
+                    return "not there"
+            commits.append(used)
+            used += 1
+        else:  # commits arrive in order
+            x = commits.pop(0)
+            for key in following:
+                held[(key, x % places)] = -1
+            for c in range(ctas):
+                empty[c][x % places].arrive()
+    return "ok"
+
+
+@pytest.mark.parametrize("ctas", [1, 2])
+@pytest.mark.parametrize("places", [2, 3, 4, 5])
+def test_the_ring_of_a_pair_never_overruns(ctas, places):
+    assert {_ring(ctas, places, 30, s) for s in range(150)} == {"ok"}
+
+
+def _accumulators(columns, warps, tiles, seed, first_half=True):
+    """Two accumulators of `columns`: of 256 they share 128, which the writing-out warps read first, and free for the next tile; of 128
+    or less they lie side by side, each freed when it is read. The issuer writes a tile's columns, warps read them."""
+    rng = random.Random(seed)
+    shared = columns == 256
+    step = 128 if shared else columns
+    full, empty = [_Barrier(1) for _ in range(2)], [_Barrier(warps) for _ in range(2)]
+    owner, read = {}, {}  # a column's tile; how often a tile's column was read
+    issued, at = 0, [(0, 0)] * warps  # a warp's tile and half
+    while any(j < tiles for j, _ in at):
+        moves = []
+        j = issued
+        if shared:
+            ready = j < 1 or empty[0].passes((j - 1) % 2)
+        else:
+            ready = j < 2 or empty[j % 2].passes((j // 2 - 1) % 2)
+        if j < tiles and ready:
+            moves.append(None)
+        moves += [w for w, (k, half) in enumerate(at) if k < tiles and (half or full[k % 2].passes(k // 2 % 2))]
+        if not moves:
+            return "deadlock"
+        w = rng.choice(moves)
+        if w is None:
+            for c in range(j % 2 * step, j % 2 * step + columns):
+                if c in owner and read.get((owner[c], c), 0) < warps:
+                    return "overwritten"
+                owner[c] = j
+            full[j % 2].arrive()
+            issued += 1
+        else:
+            k, half = at[w]
+            n = columns // 2
+            lo = k % 2 * step + n * ((half + k % 2 + first_half) % 2 if shared else half)
+            for c in range(lo, lo + n):
+                if owner[c] != k:
+                    return "stale"
+                read[(k, c)] = read.get((k, c), 0) + 1
+            if half == (0 if shared else 1):
+                empty[0 if shared else k % 2].arrive()
+            at[w] = (k + half, 1 - half)
+    return "ok"
+
+
+@pytest.mark.parametrize("columns", [256, 128])
+@pytest.mark.parametrize("warps", [2, 8, 16])
+def test_an_accumulator_is_read_before_the_next_tile_writes_it(columns, warps):
+    assert {_accumulators(columns, warps, 12, s) for s in range(60)} == {"ok"}
+
+
+def test_the_other_half_first_would_be_overwritten():
+    assert {"overwritten", "stale"} & {_accumulators(256, 8, 12, s, first_half=False) for s in range(60)}

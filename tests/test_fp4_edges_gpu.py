@@ -347,6 +347,47 @@ def test_dequantize_with_factors_near_the_ends_of_the_range(cuda, dtype, f):
     assert bool(((got - want).abs() <= bound)[under].all())
 
 
+# ---- 16 bits by 4, long rows -------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("M", [1, 20, 70, 300])
+@pytest.mark.parametrize("K", [4096, 9728, 14336])
+def test_linear_picks_single_values_out_of_long_rows(cuda, dtype, M, K):
+    """Each row of w picks one value of x by a code of 1 and a scale of 1: all of its bits, from every piece, wherever it stands."""
+    import torch
+    from locals_b200 import fp4
+
+    g = _gen(cuda, M + K)
+    N = 512
+    at = torch.randperm(K, generator=g, device=cuda)[:N]
+    at[:4] = torch.tensor([0, 31, K - 32, K - 1], device=cuda)
+    words = torch.zeros((N, K // 8), dtype=torch.int32, device=cuda)
+    words[torch.arange(N, device=cuda), at // 8] = (2 << (4 * (at % 8))).to(torch.int32)
+    w = fp4.pack(words, torch.full((N, K // 32), 127, dtype=torch.uint8, device=cuda))
+    x = (1 + torch.rand((M, K), generator=g, device=cuda)) * torch.exp2(torch.randint(-12, 1, (M, K), generator=g, device=cuda).float())
+    x = torch.where(torch.rand((M, K), generator=g, device=cuda) < 0.5, -x, x).to(_dt(dtype))
+    assert torch.equal(fp4.matmul(x, w), x[:, at])
+    assert _status(cuda) == 0
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("M,N,K", [(1, 2048, 9728), (20, 512, 9728), (70, 512, 9728), (300, 512, 14336), (2, 4096, 4096)])
+def test_linear_over_long_rows_is_rounded_once(cuda, dtype, M, N, K):
+    """Sums in 32 bits add little to one rounding of the result: 1,344 steps (K / 32 of three pieces) of 2^-22 of a sum are 2^-17 of it in
+    their mean square, a twentieth of a rounding to fp16 (2^-12.8), so 1.002 in squares. Without its last piece a value is off by up to
+    2^-4 (bf16) or 2^-9 (fp16), several roundings."""
+    import torch
+    from locals_b200 import fp4
+
+    g = _gen(cuda, N + K)
+    w = fp4.quantize(torch.randn((N, K), generator=g, device=cuda) * 0.02)
+    x = torch.randn((M, K), generator=g, device=cuda).to(_dt(dtype))
+    want = x.double() @ fp4.dequantize(w, torch.float32).double().T
+    off, once = _rms(fp4.matmul(x, w).double() - want), _rms(want.to(_dt(dtype)).double() - want)
+    assert _status(cuda) == 0
+    assert off <= 1.05 * once
+
+
 # ---- refusals ------------------------------------------------------------------------------------------------
 
 def test_glu_of_an_odd_number_of_rows_is_refused(cuda):
