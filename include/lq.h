@@ -364,7 +364,8 @@ int lq_fp4_experts(const void* x, int x_rows, const int32_t* gather_order, int g
  * 2^-14 of a value, or 2^-27 of the largest of its group of 32); y is rounded once. A slot whose id is outside [0, E) adds nothing
  * (and LQ_DEV_BOUNDS). x (T, D), y f16 / bf16; inds and weights (T, k);
  * gate_up (E, 2 I, D) with gate and up rows in turn, down (E, D, I) as lq_fp4_experts; at most 1024 experts or T * k pairs, whichever is
- * less (T 1: k pairs). workspace: lq_fp4_moe_workspace(T, k, E, D, I, dtype) bytes (0: sizes that are refused), 256-byte aligned. */
+ * less (T 1: k pairs). workspace: lq_fp4_moe_workspace(T, k, E, D, I, dtype) bytes (0: sizes that are refused; 4 T k (D + I) and what the products
+ * take), 256-byte aligned. */
 size_t lq_fp4_moe_workspace(int T, int k, int E, int D, int I, int dtype);
 int lq_fp4_moe(const void* x, const int32_t* inds, const float* weights, const uint32_t* gate_up_codes,
                const uint8_t* gate_up_tiles, const uint32_t* down_codes, const uint8_t* down_tiles, void* y, int T, int k, int E,

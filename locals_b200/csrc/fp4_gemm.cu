@@ -1,5 +1,6 @@
 // Products with microscaled 4-bit weights on the block-scaled tensor cores of sm_100a: y (M, N) = x . w^T, x in the same
-// 4-bit format, or in 16 bits against mxfp4 weights; dense, or grouped over the experts that rows are routed to.
+// 4-bit format, or in 16 bits (experts' hidden rows: 32) against mxfp4 weights; dense, or grouped over the experts that rows are
+// routed to.
 //
 // Mathematics. Each value of a group is code * scale, so a group's part of a sum is scale_x scale_w sum code_x code_w, and
 // the tensor core does all of it: the products of codes are exact, the scales enter as operands, sums are 32 bits. No
@@ -8,7 +9,9 @@
 // the group, piece p has the scale 2^(E - 7 - 5 p) (its values are below 2^8, so what is left after rounding them to 4 bits
 // is at most 2^3) and is the rounded remainder of those before it. The pieces' sum is x exactly down to 2^-14 of that
 // magnitude; below, it is off by about half a last step, less than 2^-21 (bf16) or 2^-26 (fp16) of it, less than
-// the 32-bit sum itself loses beside that value. A group that holds an infinity or no number is not a number.
+// the 32-bit sum itself loses beside that value. A group that holds an infinity or no number is not a number. Values of 32 bits
+// (the hidden rows between experts' two products, which lq_fp4_moe does not round) enter as three pieces: off by at most 2^-14 of
+// themselves, 1/32 of a rounding to bf16 and 1/4 of one to fp16. Two pieces would do for bf16 but for 7% more error in all.
 //
 // Layout. Weights are the MMA's A operand (128 rows of w a tile, one a tensor-memory lane), T tokens its N side, so that one
 // token costs a narrow MMA and not a row of an empty tile. Warp 8 streams a ring of stages by TMA, 128 bytes of every row (256
@@ -21,11 +24,13 @@
 // read from L2 half as often. Two accumulators of 256 columns share 128, since scales take the rest of tensor memory.
 //
 // Measured on a B200 (captured graphs; floors at 6,458 GB/s and 1,653 TFLOP/s of bf16, four times that for 4 by 4 bits):
-// both in nvfp4, 4,096 tokens by 14336 x 4096 110 us (4.4 PFLOP/s; 132 in a long run under the power limit), bound by the one
-// thread that issues (12 scale copies and 4 MMAs a stage take it about as long as the MMAs run) and by the waits of
-// a stage; the tensor pipe is busy 37 to 45% of the time. bf16 by mxfp4, 2,048 tokens by the same 171 us (1.4 PFLOP/s,
-// 85% of the bf16 rate): the tensor pipe, 69% busy, and 7 rounds of tiles of which the last is 5% full. One token by
-// 14336 x 4096 9.4 us (3.5 TB/s) and by 6144 x 2560 6.6 us: start, first loads and join, some 4 us whatever the size.
+// both in nvfp4, 4,096 tokens by 14336 x 4096 111 to 113 us (4.3 PFLOP/s; 130 over 1.6 s, the SMs at 1,597 MHz under the power
+// limit), bound by the one thread that issues (12 scale copies and 4 MMAs a stage take it about as long as the MMAs run) and by
+// the waits of a stage; the tensor pipe is busy 37 to 45% of the time. bf16 by mxfp4, 2,048 tokens by the same 170 us (1.4 PFLOP/s,
+// 85% of the bf16 rate; 202 over 2.4 s at 1,537 MHz): the tensor pipe, 69% busy, and 7 rounds of tiles of which the last is 5% full;
+// fp16, with three pieces, 249 us. One token by 14336 x 4096 9.3 us and by 6144 x 2560 5.9 us, weights rotated through more than
+// L2 or not (9.3 and 5.8 over three sets): start, first loads and join, some 4 us whatever the size; one launch alone and cold
+// takes the former 15.6 us (the profile).
 #include <cuda_runtime.h>
 
 #include <atomic>
@@ -967,7 +972,10 @@ static int gemm_tokens(const Fp4Call& c, int T, bool fuse, cudaStream_t st) {
 }
 
 // Tokens a tile. (A product of both in 4 bits has scale tiles of 128 tokens, so narrower tiles only where one holds them all.)
-// Beyond 128 tokens tiles of 256 read the weights half as often as tiles of 128, which in turn end closer to the last token.
+// Beyond 128 tokens tiles of 256 read the weights half as often as tiles of 128, which in turn end closer to the last token: 256 but
+// where that adds an eighth of tokens or more. Both ways, 16 bits by 14336 x 4096: 256 tokens 31 us in tiles of 256 and 33 of 128, 300
+// tokens 51 and 44, 600 71 and 58, 1,200 101 and 116, 2,048 183 and 189. The rule does not count tiles, and where weights have
+// few rows pairs of CTAs leave SMs idle: 256 tokens by 2560 x 9728 take 53 us, 25 in tiles of 128; 512 by 4096 x 4096 39 and 29.
 static int tile_tokens(int rows) {
     if (rows <= 128) return rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : 128;
     const int64_t narrow = (int64_t(rows) + 127) / 128 * 128, wide = (int64_t(rows) + 255) / 256 * 256;
@@ -1003,8 +1011,8 @@ static int split_blocks(int P, int T) { return T <= 32 ? 1 : P * ((T + 127) / 12
 static size_t split_pieces_bytes(int rows, int K, int P) { return (size_t(P) * rows * fp4_padded(K) + 511) / 512 * 512; }
 
 // Tokens a tile of rows that are dealt out to segments: twice the average, so that most segments are one tile; long segments
-// have tiles of 128, whose last is half as wide (250 rows each: 143 -> 110 us for 4,001 tokens' gate and up), until
-// that is a small part of them.
+// have tiles of 128, whose last is half as wide (64 experts, 250 rows each: 143 us in tiles of 256, 110 of 128, for 4,001 tokens'
+// gate and up), until that is a small part of them (8 experts: 250 rows each 26 and 27 us, 1,000 59 and 65, 2,000 112 and 119).
 static int grouped_tokens(int rows, int segments, int max_rows) {
     const int64_t average = int64_t(rows) / (segments > 0 ? segments : 1), want = 2 * average;
     const int T = tile_tokens(int(want < max_rows ? want : max_rows));

@@ -161,7 +161,9 @@ __global__ void group_kernel(const uint32_t* inds, int P, int E, int32_t* order,
 // after every earlier pair of e, exactly as in group_kernel: the same order, starts, experts and pos.
 constexpr int GROUP_PAR_MAX_E = 1024;
 constexpr int GROUP_MAX_E = 8192;  // what lq_moe_group takes
-constexpr int GROUP_CLUSTER_MIN_P = 2049;  // from here a cluster of 8 CTAs (16,004 pairs 36 -> 10 us; 2,048 pairs 6.9 in one)
+// From here a cluster of 8 CTAs. One and eight: 1,024 pairs of 64 experts 4.9 and 5.0 us, of 8 3.1 and 5.0; 2,049 of 64 7.6 and 5.0, of 8
+// 5.0 and 5.1; 16,004 of 64 36 and 8.9.
+constexpr int GROUP_CLUSTER_MIN_P = 2049;
 
 __global__ void __launch_bounds__(1024) group_par_kernel(const uint32_t* inds, int P, int E, int32_t* order,
                                                          int32_t* starts, int32_t* experts, int32_t* nseg,
