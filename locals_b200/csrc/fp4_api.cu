@@ -91,6 +91,7 @@ int lq_fp4_linear(const void* x, int64_t x_row, const uint32_t* codes, const uin
     l.x_dtype = l.dtype = dtype;
     l.y = y;
     l.ws = workspace;
+    l.ws_bytes = workspace_bytes;
     return finish(fp4_linear_run(l, reinterpret_cast<cudaStream_t>(stream)));
 }
 
@@ -146,6 +147,7 @@ int lq_fp4_experts(const void* x, int x_rows, const int32_t* gather_order, int g
     l.x_dtype = l.dtype = dtype;
     l.y = out;
     l.ws = workspace;
+    l.ws_bytes = workspace_bytes;
     return finish(fp4_linear_run(l, reinterpret_cast<cudaStream_t>(stream)));
 }
 
@@ -170,7 +172,9 @@ static int fp4_moe_parts(int T, int k, int E, int D, int I, int dtype, MoeParts&
     m.outputs = m.hidden + whole(size_t(P) * I * sizeof(float));
     m.group = m.outputs + whole(size_t(P) * D * sizeof(float));
     m.product = m.group + (T > 1 ? whole((2 * size_t(P) + 2 * m.segments + 2) * sizeof(int32_t)) : 0);
-    const size_t up = fp4_grouped_bytes(P, T, E, 2 * I, D, dtype), down = fp4_grouped_bytes(P, T, E, D, I, LQ_F32);
+    // (of the very segments that the products run with: tiles, and so these bytes, go by their number)
+    const size_t up = fp4_linear_workspace_bytes(P, 2 * I, D, dtype, m.segments, T);
+    const size_t down = fp4_linear_workspace_bytes(P, D, I, LQ_F32, m.segments, T);
     m.all = m.product + whole(up > down ? up : down);
     return LQ_OK;
 }
@@ -183,10 +187,11 @@ size_t lq_fp4_moe_workspace(int T, int k, int E, int D, int I, int dtype) {
 int lq_fp4_moe(const void* x, const int32_t* inds, const float* weights, const uint32_t* gate_up_codes,
                const uint8_t* gate_up_tiles, const uint32_t* down_codes, const uint8_t* down_tiles, void* y, int T, int k, int E,
                int D, int I, int dtype, void* workspace, size_t workspace_bytes, void* stream) {
-    if (!x || !inds || !weights || !gate_up_codes || !gate_up_tiles || !down_codes || !down_tiles || !y || !workspace) return LQ_E_ARG;
+    if (!x || !inds || !weights || !gate_up_codes || !gate_up_tiles || !down_codes || !down_tiles || !y) return LQ_E_ARG;
     MoeParts m;
     int rc = fp4_moe_parts(T, k, E, D, I, dtype, m);
     if (rc) return rc;
+    if (!workspace) return LQ_E_ARG;
     if (workspace_bytes < m.all) return LQ_E_SHAPE;
     if (!aligned(gate_up_codes, 32) || !aligned(down_codes, 32) || !aligned(gate_up_tiles, 16) || !aligned(down_tiles, 16) ||
         !aligned(workspace, 256) || !aligned(x, 2) || !aligned(y, 2) || !aligned(inds, 4) || !aligned(weights, 4))
@@ -215,6 +220,7 @@ int lq_fp4_moe(const void* x, const int32_t* inds, const float* weights, const u
     l.E = E;
     l.rows = P;
     l.ws = ws + m.product;
+    l.ws_bytes = m.all - m.product;
     l.x = x;  // gate and up: 16-bit tokens to 32-bit hidden rows
     l.x_row = D;
     l.x_dtype = dtype;

@@ -1035,6 +1035,7 @@ size_t fp4_linear_workspace_bytes(int rows, int N, int K, int x_dtype, int segme
 int fp4_linear_run(const Fp4Linear& l, cudaStream_t st) {
     const int P = fp4_pieces(l.x_dtype);
     const int T = l.segments ? grouped_tokens(l.rows, l.segments, l.max_rows) : tile_tokens(l.rows);
+    if (l.ws_bytes < fp4_linear_workspace_bytes(l.rows, l.N, l.K, l.x_dtype, l.segments, l.max_rows)) return LQ_E_SHAPE;
     uint8_t* ws = static_cast<uint8_t*>(l.ws);
     SplitArgs s = {};
     s.ktiles = fp4_ktiles(l.K, LQ_MXFP4);

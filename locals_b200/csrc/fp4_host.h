@@ -26,6 +26,7 @@ struct Fp4Linear {
     int rows, N, K, glu, x_dtype, dtype;
     void* y;
     void* ws;
+    size_t ws_bytes;
 };
 size_t fp4_linear_workspace_bytes(int rows, int N, int K, int x_dtype, int segments, int max_rows);
 int fp4_linear_run(const Fp4Linear& l, cudaStream_t st);

@@ -237,3 +237,39 @@ def test_an_accumulator_is_read_before_the_next_tile_writes_it(columns, warps):
 
 def test_the_other_half_first_would_be_overwritten():
     assert {"overwritten", "stale"} & {_accumulators(256, 8, 12, s, first_half=False) for s in range(60)}
+
+
+def _product_bytes(rows, N, K, pieces, segments, max_rows):
+    """What a grouped product with pieces takes, by its rules for tiles."""
+    average = rows // segments
+    want = min(2 * average, max_rows)
+    if want <= 128:
+        tokens = next(t for t in (16, 32, 64, 128) if want <= t)
+    else:
+        narrow, wide = -(-want // 128) * 128, -(-want // 256) * 256
+        tokens = 256 if wide * 8 <= narrow * 9 and average >= 1024 else 128
+    tiles, Kp = rows // tokens + segments, -(-K // 128) * 128
+    if tokens <= 32 and tiles * -(-N // 128) <= 2 * 148:
+        return 0
+    blocks = 1 if tokens <= 32 else pieces * -(-tokens // 128)
+    return -(-pieces * rows * Kp // 512) * 512 + tiles * (Kp // 128) * blocks * 512
+
+
+def test_the_workspace_of_routed_experts_holds_what_its_products_take():
+    """Their tiles go by the number of segments: sized for one more than they run with (17 rows a segment or 13), they wrote past its
+    end."""
+    L, rng = _lib.lib(), random.Random(0)
+    cases = [(34, 2, 4, 256, 96), (17, 1, 1, 128, 64), (2, 17, 2, 128, 64)]
+    cases += [(rng.choice([1, 2, 3, rng.randint(2, 60), rng.randint(2, 3000)]), rng.randint(1, 9), rng.choice([1, 2, 3, 4, 8, 60, 64, 128, 1000]),
+               rng.randint(1, 3000), rng.randint(1, 1500)) for _ in range(4000)]
+    for T, k, E, D, I in cases:
+        P = T * k
+        segments = min(E, P) if T > 1 else P
+        for dtype, pieces in ((_lib.BF16, 2), (_lib.F16, 3)):
+            n = L.lq_fp4_moe_workspace(T, k, E, D, I, dtype)
+            if segments > 1024:
+                assert n == 0
+                continue
+            ints = (2 * P + 2 * segments + 2) * 4 if T > 1 else 0
+            product = max(_product_bytes(P, 2 * I, D, pieces, segments, T), _product_bytes(P, D, I, 3, segments, T))
+            assert n >= 4 * P * (D + I) + ints + product, (T, k, E, D, I)

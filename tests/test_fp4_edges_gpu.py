@@ -388,6 +388,47 @@ def test_linear_over_long_rows_is_rounded_once(cuda, dtype, M, N, K):
     assert off <= 1.05 * once
 
 
+@pytest.mark.parametrize("T,k,E,D,I", [(34, 2, 4, 256, 96), (17, 1, 1, 128, 64), (2, 17, 2, 128, 64), (1, 5, 8, 128, 64), (300, 4, 8, 130, 66)])
+def test_routed_experts_stay_within_their_workspace(cuda, T, k, E, D, I):
+    import torch
+    from locals_b200 import _lib
+    from locals_b200.kernels import _stream
+
+    g = _gen(cuda, T)
+    gu, gv = _stack(cuda, g, E, 2 * I, D, D ** -0.5)
+    dn, dv = _stack(cuda, g, E, D, I, I ** -0.5)
+    x = torch.randn((T, D), generator=g, device=cuda).to(torch.bfloat16)
+    inds = torch.randint(0, E, (T, k), generator=g, device=cuda).to(torch.int32)
+    weights = 0.5 + torch.rand((T, k), generator=g, device=cuda)
+    n = _lib.lib().lq_fp4_moe_workspace(T, k, E, D, I, _lib.BF16)
+    ws = torch.full((n + (1 << 22),), 0xA5, dtype=torch.uint8, device=cuda)
+    y = torch.full((T + 4, D), 7.0, dtype=torch.bfloat16, device=cuda)
+    _lib.call("lq_fp4_moe", x.data_ptr(), inds.data_ptr(), weights.data_ptr(), gu.codes.data_ptr(), gu.tiles.data_ptr(), dn.codes.data_ptr(),
+              dn.tiles.data_ptr(), y.data_ptr(), T, k, E, D, I, _lib.BF16, ws.data_ptr(), n, _stream())
+    assert _status(cuda) == 0
+    assert bool((ws[n:] == 0xA5).all()) and bool((y[T:] == 7.0).all())
+    want = _experts(x, inds, weights, gv, dv)
+    off, once = _rms(y[:T].double() - want), _rms(want.to(torch.bfloat16).double() - want)
+    assert off <= 1.05 * once
+
+
+def test_more_experts_than_segments_are_refused(cuda):
+    import torch
+    from locals_b200 import fp4
+
+    E, D, I = 1025, 32, 32
+    gu = fp4.Fp4(torch.zeros((E, 2 * I, 16), dtype=torch.int32, device=cuda), torch.full((E, 1, 1, 512), 127, dtype=torch.uint8, device=cuda), "mxfp4", D)
+    dn = fp4.Fp4(torch.zeros((E, D, 16), dtype=torch.int32, device=cuda), torch.full((E, 1, 1, 512), 127, dtype=torch.uint8, device=cuda), "mxfp4", I)
+    x = torch.ones((600, D), dtype=torch.bfloat16, device=cuda)
+    for T, k in ((600, 2), (1, 1025)):
+        inds, weights = torch.zeros((T, k), dtype=torch.int32, device=cuda), torch.ones((T, k), device=cuda)
+        with pytest.raises(Exception, match="shape"):
+            fp4.experts(x[:T], inds, weights, gu, dn)
+    few = torch.full((300, 2), 1024, dtype=torch.int32, device=cuda)  # 600 pairs of the same stack are answered
+    assert not bool(fp4.experts(x[:300], few, torch.ones((300, 2), device=cuda), gu, dn).any())
+    assert _status(cuda) == 0
+
+
 # ---- refusals ------------------------------------------------------------------------------------------------
 
 def test_glu_of_an_odd_number_of_rows_is_refused(cuda):
