@@ -363,8 +363,8 @@ int lq_fp4_experts(const void* x, int x_rows, const int32_t* gather_order, int g
  * hidden rows and the experts' outputs are held in 32 bits (the former enter the down product in three pieces of e4m3, off by at most
  * 2^-14 of a value, or 2^-27 of the largest of its group of 32); y is rounded once. A slot whose id is outside [0, E) adds nothing
  * (and LQ_DEV_BOUNDS). x (T, D), y f16 / bf16; inds and weights (T, k);
- * gate_up (E, 2 I, D) with gate and up rows in turn, down (E, D, I) as lq_fp4_experts; at most 1024 experts or T * k pairs, whichever is
- * less (T 1: k pairs). workspace: lq_fp4_moe_workspace(T, k, E, D, I, dtype) bytes (0: sizes that are refused; 4 T k (D + I) and what the products
+ * gate_up (E, 2 I, D) with gate and up rows in turn, down (E, D, I) as lq_fp4_experts. min(E, T k) <= 1024 and E <= 8192 (T 1: k <= 1024).
+ * workspace: lq_fp4_moe_workspace(T, k, E, D, I, dtype) bytes (0: sizes that are refused; 4 T k (D + I) and what the products
  * take), 256-byte aligned. */
 size_t lq_fp4_moe_workspace(int T, int k, int E, int D, int I, int dtype);
 int lq_fp4_moe(const void* x, const int32_t* inds, const float* weights, const uint32_t* gate_up_codes,

@@ -97,15 +97,11 @@ int lq_fp4_linear(const void* x, int64_t x_row, const uint32_t* codes, const uin
 
 static int fp4_segments(int P, int E) { return P < E + 1 ? P : E + 1; }
 
-static size_t fp4_grouped_bytes(int P, int max_rows, int E, int N, int K, int x_dtype) {
-    const size_t some = fp4_linear_workspace_bytes(P, N, K, x_dtype, fp4_segments(P, E), max_rows);
-    const size_t each = P <= 1024 ? fp4_linear_workspace_bytes(P, N, K, x_dtype, P, max_rows) : 0;  // without segments
-    return some > each ? some : each;
-}
-
 size_t lq_fp4_experts_workspace(int P, int max_rows, int E, int N, int K, int dtype) {
     if (fp4_rows_ok(P, K, LQ_MXFP4) || fp4_rows_ok(N, K, LQ_MXFP4) || !is16(dtype) || E < 1 || max_rows < 1) return 0;
-    return fp4_grouped_bytes(P, max_rows, E, N, K, dtype);
+    const size_t some = fp4_linear_workspace_bytes(P, N, K, dtype, fp4_segments(P, E), max_rows);
+    const size_t each = P <= 1024 ? fp4_linear_workspace_bytes(P, N, K, dtype, P, max_rows) : 0;  // without segments
+    return some > each ? some : each;
 }
 
 int lq_fp4_experts(const void* x, int x_rows, const int32_t* gather_order, int gather_k, const int32_t* starts,
@@ -166,7 +162,7 @@ static int fp4_moe_parts(int T, int k, int E, int D, int I, int dtype, MoeParts&
     if (!rc) rc = fp4_rows_ok(int64_t(E) * D, I, LQ_MXFP4);
     if (rc) return rc;
     m.segments = T > 1 && E < P ? E : P;
-    if (m.segments > 1024) return LQ_E_SHAPE;
+    if (m.segments > 1024 || (T > 1 && E > 8192)) return LQ_E_SHAPE;  // (lq_moe_group's experts)
     auto whole = [](size_t bytes) { return (bytes + 255) / 256 * 256; };
     m.hidden = 0;
     m.outputs = m.hidden + whole(size_t(P) * I * sizeof(float));
